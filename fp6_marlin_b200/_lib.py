@@ -17,6 +17,18 @@ OK, ERR_PROB_SHAPE, ERR_KERN_SHAPE, ERR_VALUE_RANGE, ERR_BAD_ARG = 0, 1, 2, 3, 4
 ERR_WORKSPACE, ERR_SCRATCH, ERR_CUDA, ERR_TIMEOUT, ERR_NO_MEMORY = 5, 6, 7, 8, 9
 LAYOUT_REFERENCE, LAYOUT_B200 = 0, 1
 EPILOGUE_NONE, EPILOGUE_SILU_MUL, EPILOGUE_RESIDUAL = 0, 1, 2
+TYPE_F16, TYPE_BF16 = 0, 1
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """fp6m_tree_attention_args of include/fp6m.h."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("q", "k", "v", "out", "k_cache", "v_cache", "page_table", "lengths", "tree")]
+                + [(name, ctypes.c_longlong * 3) for name in ("q_stride", "k_stride", "v_stride", "out_stride", "k_cache_stride", "v_cache_stride")]
+                + [(name, ctypes.c_longlong) for name in ("page_table_stride", "tree_stride")]
+                + [(name, ctypes.c_int) for name in ("batch", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "max_pages", "type")]
+                + [("scale", ctypes.c_float)])
+
 
 # every symbol include/fp6m.h declares, with its ctypes signature
 _vp, _sz, _i, _i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64
@@ -57,6 +69,12 @@ SIGNATURES = {
     "fp6m_pack_b200_device": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int] * 4 + [ctypes.c_void_p] * 2 + [ctypes.c_int, ctypes.c_void_p]),
     "fp6m_quantize_pack_b200_device": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp]),
     "fp6m_gather_columns": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "fp6m_rms_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, ctypes.c_float, _i, _i, _vp]),
+    "fp6m_quantize_fp8": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "fp6m_mul_fp8_scratch_bytes": (_sz, [_i, _i, _i, _i]),
+    "fp6m_mul_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _i, _vp, _vp]),
+    "fp6m_tree_attention_scratch_bytes": (_sz, [_i]),
+    "fp6m_tree_attention": (_i, [ctypes.POINTER(TreeAttentionArgs), _vp, _sz, _i, _vp, _vp]),
     "fp6m_set_launch_overlap": (ctypes.c_int, [ctypes.c_int]),
     "fp6m_set_ordered_sums": (ctypes.c_int, [ctypes.c_int]),
     "fp6m_last_cuda_error": (ctypes.c_char_p, []),

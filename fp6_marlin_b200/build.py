@@ -21,7 +21,8 @@ CALL_PATH = os.path.join(PKG_DIR, "_call.so")          # extension module: the P
 CALL_SOURCES = [os.path.join(CSRC, "py_call.cpp"), os.path.join(os.path.dirname(PKG_DIR), "include", "fp6m.h")]
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 
-CUDA_SOURCES = ["c_api.cu", "gemm_few.cu", "gemm_team.cu", "gemm_tc5.cu", "gemm_wide.cu", "dump_operands.cu", "prep_gpu.cu", "gather_columns.cu", "peer.cu"]
+CUDA_SOURCES = ["c_api.cu", "gemm_few.cu", "gemm_team.cu", "gemm_tc5.cu", "gemm_wide.cu", "dump_operands.cu", "prep_gpu.cu", "gather_columns.cu", "peer.cu",
+                "rows.cu", "mul_fp8.cu", "tree_attention.cu"]
 HOST_SOURCES = ["host_pack.cpp"]
 
 NVCC_FLAGS = [

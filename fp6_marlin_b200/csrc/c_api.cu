@@ -11,12 +11,11 @@
 #include "../../include/fp6m.h"
 #include "fp6m_layout.h"
 #include "gemm_params.h"
+#include "host_common.h"
 
-namespace {
+namespace fp6m {
 
-using namespace fp6m;
-
-thread_local char g_cuda_error[256] = "";
+static thread_local char g_cuda_error[256] = "";
 
 int cuda_fail(cudaError_t e, const char* where) {
   std::snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", where, cudaGetErrorString(e));
@@ -34,16 +33,11 @@ int sm_count(int dev) {
   return n;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+}  // namespace fp6m
 
-struct DeviceGuard {
-  int prev = -1;
-  bool switched = false;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) == cudaSuccess && prev != dev) switched = cudaSetDevice(dev) == cudaSuccess;
-  }
-  ~DeviceGuard() { if (switched) cudaSetDevice(prev); }
-};
+namespace {
+
+using namespace fp6m;
 
 // How a GEMM of M rows is cut into launches: kernel, tile of rows, rows per launch, grid.
 struct LaunchPlan {
@@ -329,7 +323,7 @@ int fp6m_set_ordered_sums(int enable) {
   return before;
 }
 
-const char* fp6m_last_cuda_error(void) { return g_cuda_error; }
+const char* fp6m_last_cuda_error(void) { return fp6m::g_cuda_error; }
 
 const char* fp6m_version(void) { return "fp6m-b200 0.1 (sm_100a)"; }
 

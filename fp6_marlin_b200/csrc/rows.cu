@@ -1,0 +1,169 @@
+// Row operators between the products of a decoder block: the root-mean-square norm with the residual's addition, and the
+// rounding of rows to E4M3 with a scale for each 128 neighbours (with or without the norm in front).
+//
+//   h = x + r          in fp32; rounded once to the 16-bit type where it is stored, the norm goes on with the fp32 sum
+//   y = h * rsqrt(mean(h^2) + eps) * w
+//   s[g] = max(max |y| of group g, 1e-30) / 448,  q = round(y * (448 / max(...)))      (NaN stays NaN in both)
+//
+// The reference has no counterpart; its layer lists (bench.py:53-86) name the products on either side.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+
+#include "../../include/fp6m.h"
+#include "host_common.h"
+
+namespace {
+
+using namespace fp6m;
+
+constexpr int kGroup = 128;              // neighbours that share a scale
+constexpr float kE4m3Max = 448.f, kSmallest = 1e-30f;
+
+template <class T> struct Pair;
+template <> struct Pair<half> {
+  static __device__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<half2*>(&v)); }
+  static __device__ uint32_t pack(float a, float b) { half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<uint32_t*>(&h); }
+};
+template <> struct Pair<__nv_bfloat16> {
+  static __device__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+  static __device__ uint32_t pack(float a, float b) { __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<uint32_t*>(&h); }
+};
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 two = Pair<T>::unpack(w[i]);
+    f[2 * i] = two.x;
+    f[2 * i + 1] = two.y;
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
+}
+// the larger of two, NaN if one is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+struct RowParams {
+  const void *x, *weight, *residual;
+  void *residual_out, *y;
+  float* scales;
+  int M, N;
+  float eps;
+};
+
+// One CTA a row, eight neighbouring values a thread at a time; every pass reads the row again.
+template <class T, bool kNorm, bool kFp8>
+__global__ void rows_kernel(const RowParams p) {
+  __shared__ float part[32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const size_t row = blockIdx.x;
+  const int vecs = p.N / 8, groups = (p.N + kGroup - 1) / kGroup;
+  const uint4* x = static_cast<const uint4*>(p.x) + row * vecs;
+  const uint4* r = p.residual ? static_cast<const uint4*>(p.residual) + row * vecs : nullptr;
+  auto load = [&](int v, float (&f)[8]) {
+    unpack8<T>(x[v], f);
+    if (kNorm && r) {
+      float add[8];
+      unpack8<T>(r[v], add);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] += add[i];
+    }
+  };
+  float factor = 1.f;
+  if (kNorm) {
+    float sum = 0.f;
+    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+      float f[8];
+      load(v, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += f[i] * f[i];
+    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) sum += part[w];
+    factor = rsqrtf(sum / p.N + p.eps);
+  }
+  for (int v0 = 0; v0 < vecs; v0 += blockDim.x) {
+    const int v = v0 + threadIdx.x;
+    const bool live = v < vecs;
+    float f[8] = {};
+    if (live) {
+      load(v, f);
+      if (kNorm) {
+        if (p.residual_out) static_cast<uint4*>(p.residual_out)[row * vecs + v] = pack8<T>(f);
+        float w[8];
+        unpack8<T>(static_cast<const uint4*>(p.weight)[v], w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = f[i] * factor * w[i];
+      }
+    }
+    if (kFp8) {
+      float top = kSmallest;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
+#pragma unroll
+      for (int o = 8; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));     // the 16 lanes of a group
+      if (live) {
+        const float up = kE4m3Max / top;
+        uint2 q;
+        auto two = [&](int i) { return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[i] * up, f[i + 1] * up), __NV_SATFINITE, __NV_E4M3); };
+        q.x = two(0) | two(2) << 16;
+        q.y = two(4) | two(6) << 16;
+        static_cast<uint2*>(p.y)[row * vecs + v] = q;
+        if (v % 16 == 0) p.scales[row * groups + v / 16] = top / kE4m3Max;
+      }
+    } else if (live) {
+      static_cast<uint4*>(p.y)[row * vecs + v] = pack8<T>(f);
+    }
+  }
+}
+
+template <class T>
+cudaError_t launch_rows(const RowParams& p, bool norm, cudaStream_t stream) {
+  void (*kernel)(RowParams) = !norm ? rows_kernel<T, false, true> : p.scales ? rows_kernel<T, true, true> : rows_kernel<T, true, false>;
+  const int vecs = p.N / 8;
+  const int threads = vecs >= 512 ? 512 : (vecs + 31) / 32 * 32;
+  return launch_overlapped(kernel, dim3(p.M), dim3(threads), 0, stream, p);
+}
+
+int rows_impl(const RowParams& p, bool norm, int type, int dev, void* stream, const char* what) {
+  if (p.M < 0 || p.N < 0 || p.N % 8 || (type != FP6M_TYPE_F16 && type != FP6M_TYPE_BF16)) return FP6M_ERR_BAD_ARG;
+  if (p.M == 0 || p.N == 0) return FP6M_OK;
+  if (!p.x || !p.y || (norm && !p.weight) || (p.residual != nullptr) != (p.residual_out != nullptr)) return FP6M_ERR_BAD_ARG;
+  if (!aligned16(p.x) || !aligned16(p.weight) || !aligned16(p.residual) || !aligned16(p.residual_out) || !aligned16(p.y) ||
+      (reinterpret_cast<uintptr_t>(p.scales) & 3))
+    return FP6M_ERR_BAD_ARG;
+  DeviceGuard guard(dev);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = type == FP6M_TYPE_F16 ? launch_rows<half>(p, norm, st) : launch_rows<__nv_bfloat16>(p, norm, st);
+  return e == cudaSuccess ? FP6M_OK : cuda_fail(e, what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp6m_rms_norm(const void* x, const void* weight, const void* residual, void* residual_out, void* y, void* scales, int M, int N, float eps, int type,
+                  int dev, void* stream) {
+  RowParams p = {x, weight, residual, residual_out, y, static_cast<float*>(scales), M, N, eps};
+  return rows_impl(p, true, type, dev, stream, "rms_norm launch");
+}
+
+int fp6m_quantize_fp8(const void* x, void* q, void* scales, int M, int N, int type, int dev, void* stream) {
+  if (M > 0 && N > 0 && !scales) return FP6M_ERR_BAD_ARG;
+  RowParams p = {x, nullptr, nullptr, nullptr, q, static_cast<float*>(scales), M, N, 0.f};
+  return rows_impl(p, false, type, dev, stream, "quantize_fp8 launch");
+}
+
+}  // extern "C"

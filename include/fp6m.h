@@ -224,6 +224,61 @@ int fp6m_quantize_pack_b200_device(const void* w, int K, int N, int quant_cols, 
  * 0..N-1 gives NaN.  The reference leaves the column order to its caller (fp6_marlin_cuda.cpp:93-122). */
 int fp6m_gather_columns(const void* c, void* y, const void* src, const void* bias, int M, int N, int dev, void* stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* GPU side: what stands between the products of a decoder block                              */
+/* ------------------------------------------------------------------------------------------ */
+
+/* 16-bit types of the operators below. */
+enum { FP6M_TYPE_F16 = 0, FP6M_TYPE_BF16 = 1 };
+
+/* Root-mean-square norm of the M rows of x (M x N, row-major, 16 bits), with the residual's addition and, if `scales` is
+ * given, E4M3 output:  h = x + residual (fp32; written to residual_out, rounded once, which may be x or residual itself),
+ * y = h * rsqrt(mean(h^2) + eps) * weight.  The norm goes on with the sum before that rounding.
+ *   scales == null: y is M x N in x's type
+ *   else            y is M x N in E4M3 and scales M x ceil(N / 128) fp32: max(largest |y| of the 128 neighbours, 1e-30) / 448,
+ *                   y[m, n] * scales[m, n / 128] stands for the value; this is what fp6m_mul_fp8 takes
+ * residual and residual_out are given together or not at all.  N a multiple of 8, pointers 16-byte aligned (scales: 4).
+ * No counterpart in the reference; nor have the next ones. */
+int fp6m_rms_norm(const void* x, const void* weight, const void* residual, void* residual_out, void* y, void* scales, int M, int N, float eps,
+                  int type, int dev, void* stream);
+/* The same rounding to E4M3 without the norm. */
+int fp6m_quantize_fp8(const void* x, void* q, void* scales, int M, int N, int type, int dev, void* stream);
+
+/* C[M, N] = A[M, K] B[N, K]^T, A and B in E4M3 (row-major), C in `type` (overwritten), with fp32 scales for blocks of 128:
+ * sa (M x ceil(K / 128)) for 128 neighbours of a row of A, sb (ceil(N / 128) x ceil(K / 128)) for 128 x 128 values of B.  Sums in
+ * fp32, one rounding.  K a multiple of 16, N of 8 (FP6M_ERR_PROB_SHAPE otherwise); A, B, C and scratch 16-byte aligned.
+ *   scratch     >= fp6m_mul_fp8_scratch_bytes(...) bytes of device memory, zeroed before the first use and then left to this
+ *               function; calls that can overlap on the GPU need one each
+ *   status_dev  optional device int: set to FP6M_ERR_TIMEOUT if a bounded wait ran out */
+size_t fp6m_mul_fp8_scratch_bytes(int M, int N, int K, int sms);
+int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const void* sb, int M, int N, int K, int type, void* scratch, size_t scratch_bytes,
+                 int dev, void* stream, int* status_dev);
+
+/* Attention of `tokens` (0..64) drafted tokens of each of `batch` sequences over a paged cache of committed tokens and over one
+ * another.  Token i of sequence b sees the first lengths[b] tokens of the sequence's pages and the drafted tokens j whose bit j
+ * is set in tree[b * tree_stride + i]; a mask of zero marks padding, which sees nothing and gives zeros.  With one token and
+ * the mask 1 this is ordinary decoding.  Heads of queries share the heads of keys in groups of heads / kv_heads neighbours.
+ * Strides are in elements, multiples of 8; the head_dim (64 or 128) values of a head lie next to one another; pointers 16-byte
+ * aligned.  Lengths are read on the device, cut to 0 .. max_pages * page_size; a page number outside 0 .. pages - 1 hides its
+ * tokens and sets the status word to FP6M_ERR_BAD_ARG.  Entries of page_table behind a sequence's last page, and slots
+ * of a page behind its last token, are not read. */
+typedef struct fp6m_tree_attention_args {
+  const void *q, *k, *v;              /* batch x tokens x (heads | kv_heads) x head_dim */
+  void* out;                          /* like q */
+  const void *k_cache, *v_cache;      /* pages x page_size x kv_heads x head_dim */
+  const int *page_table;              /* batch x max_pages */
+  const int *lengths;                 /* batch */
+  const unsigned long long *tree;     /* batch x tokens */
+  long long q_stride[3], k_stride[3], v_stride[3], out_stride[3];      /* batch, token, head */
+  long long k_cache_stride[3], v_cache_stride[3];                      /* page, slot, head */
+  long long page_table_stride, tree_stride;                            /* from one sequence to the next (0: all alike) */
+  int batch, tokens, heads, kv_heads, head_dim, pages, page_size, max_pages, type;
+  float scale;                        /* of the scores, usually head_dim ** -0.5 */
+} fp6m_tree_attention_args;
+/* Scratch as in fp6m_mul_fp8; enough for any shape on a device with `sms` multiprocessors. */
+size_t fp6m_tree_attention_scratch_bytes(int sms);
+int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
+
 /* Process-wide option, off by default; returns the previous setting (a negative argument only queries).
  * GEMMs of up to 128 rows are always launched with programmatic stream serialisation: such a GEMM sets itself up (and brings the first
  * lines of B into L2) while the kernel before it in the stream finishes, and reads and writes memory only after that
