@@ -86,6 +86,7 @@ cudaError_t launch_gemm_team(const MulParams& p, cudaStream_t stream);
 cudaError_t encode_activation_map(const half* A, int M, int K, int box_rows, CUtensorMap* map);
 cudaError_t encode_activation_segment_map(const half* A, int M, int K, int box_rows, CUtensorMap* map);
 cudaError_t encode_output_map(const half* base, int rows, int ld, CUtensorMap* map);
+cudaError_t encode_bytes_map(const void* base, int rows, int K, int box_rows, CUtensorMap* map);
 constexpr int kMaxWideCtas = 192;   // one CTA per SM
 constexpr int kMaxRowTiles = 32;    // 8192 rows of A per launch
 constexpr int kWideTileRows = 256;  // most rows of a tile

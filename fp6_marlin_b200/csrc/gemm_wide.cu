@@ -625,16 +625,16 @@ static EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// A map of fp16 data whose elements outside read as zero.  The encoder is a driver call and needs a current context, which a
+// A map of data whose elements outside read as zero.  The encoder is a driver call and needs a current context, which a
 // thread that has made no other CUDA call does not have: cudaGetDevice binds none, so the first attempt fails there.
-static cudaError_t encode_f16(CUtensorMap* map, int rank, const half* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
-                              CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
-  EncodeTiledFn encode = encode_tiled();
-  if (!encode) return cudaErrorNotSupported;
+static cudaError_t encode(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                          const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  EncodeTiledFn encode_fn = encode_tiled();
+  if (!encode_fn) return cudaErrorNotSupported;
   const cuuint32_t elem[3] = {1, 1, 1};
   for (int attempt = 0; attempt < 2; ++attempt) {
-    if (encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<half*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+    if (encode_fn(map, type, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
       return cudaSuccess;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -642,6 +642,11 @@ static cudaError_t encode_f16(CUtensorMap* map, int rank, const half* base, cons
     if (e != cudaSuccess) return e;
   }
   return cudaErrorInvalidValue;
+}
+
+static cudaError_t encode_f16(CUtensorMap* map, int rank, const half* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                              CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, base, dims, strides, box, swizzle, promotion);
 }
 
 // The last few tensor maps of the calling thread: a decode loop calls with the same activation buffer again
@@ -709,6 +714,19 @@ cudaError_t encode_activation_segment_map(const half* A, int M, int K, int box_r
   const cuuint64_t strides[2] = {(cuuint64_t)K * 2, 128};
   const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 2};
   const cudaError_t e = encode_f16(map, 3, A, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+  if (e == cudaSuccess) g_map_cache.put(mk, *map);
+  return e;
+}
+
+// A matrix of bytes (E4M3), `rows` x K, K contiguous; one box = 128 bytes x `box_rows` rows with the 128-byte swizzle; what lies
+// outside reads as zero.
+cudaError_t encode_bytes_map(const void* base, int rows, int K, int box_rows, CUtensorMap* map) {
+  const MapKey mk = {base, rows, K, box_rows, 5};
+  if (g_map_cache.find(mk, map)) return cudaSuccess;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)K};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cudaError_t e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
   if (e == cudaSuccess) g_map_cache.put(mk, *map);
   return e;
 }

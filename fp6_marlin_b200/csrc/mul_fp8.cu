@@ -2,100 +2,445 @@
 //
 // A (M x K) and B (N x K) in E4M3, fp32 scales, fp32 sums, C in fp16 or bf16 with one rounding.
 // The reference has no counterpart: its weights have four or six bits.
+//
+// The product is computed transposed, as in the GEMMs of this library: 128 rows of B - one strip, and one scale per block of K -
+// are the M dimension of tcgen05.mma.kind::f8f6f4 (a TMEM lane per column of C), up to 256 rows of A its N dimension.  The scales
+// change with every block of 128 values of K, so a block is one accumulator tile of its own (four MMAs, the first one overwrites):
+// warps read it back, multiply it by sa * sb and add it to their sums in registers while the tensor cores work on the next blocks.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include "../../include/fp6m.h"
+#include "device_utils.cuh"
+#include "gemm_params.h"
 #include "host_common.h"
+#include "tc5_common.cuh"
+
+namespace fp6m {
 
 namespace {
 
-using namespace fp6m;
-
-constexpr int kBlock = 128;      // values of K, and columns of B, that share a scale
+constexpr int kBlock = 128;              // values of K, and columns of C, that share a scale
+constexpr int kStripBytes = kBlock * kBlock;
+constexpr int kMaxFp8Ctas = 192;         // one CTA per multiprocessor
 
 struct Fp8Params {
-  const uint8_t *A, *B;
   void* C;
   const float *sa, *sb;
-  int M, N, K, kb;
+  int M, N, kb;                          // kb: blocks of K
+  int strips, row_tiles, tile_rows;      // tile_rows: rows of A per tile, a multiple of 16
+  int weights_early;                     // the kernel in front does not write B: its first blocks are read before that has finished
+  unsigned int* epochs;
+  unsigned long long* partials;          // [CTA][tile_rows][128] words {value, tag}
+  int* status;
 };
 
-__device__ __forceinline__ void store(half* c, float v) { *c = __float2half_rn(v); }
-__device__ __forceinline__ void store(__nv_bfloat16* c, float v) { *c = __float2bfloat16_rn(v); }
+template <int ROWS_, int WARPS_>
+struct Fp8Cfg {
+  static constexpr int kRows = ROWS_;                        // most rows of A per tile
+  static constexpr int kWarps = WARPS_;                      // warps that read accumulators back, four share all 128 lanes
+  static constexpr int kMine = kRows / (kWarps / 4);         // rows of a thread
+  static constexpr int kStageBytes = kStripBytes + kRows * kBlock;
+  static constexpr int kStages = 200 * 1024 / kStageBytes < 11 ? 200 * 1024 / kStageBytes : 11;
+  static constexpr int kTiles = kRows <= 128 ? 4 : 2;        // accumulator tiles in tensor memory
+  static constexpr int kTmemCols = kTiles * kRows < 32 ? 32 : kTiles * kRows;
+  static constexpr int kScales = 8;                          // blocks whose scales wait in shared memory
+  static constexpr int kNumBars = 2 * kStages + 2 * kTiles + 2 * kScales + 1;
+  static constexpr int kThreads = 32 * (4 + kWarps);
+  static constexpr int kSmemBytes = kStages * kStageBytes + kScales * kRows * 4 + kNumBars * 8 + 16 + 1024;
+  static constexpr int kChunk = kMine < 32 ? kMine : 32;     // values per read-back
+};
 
-// 32 x 64 results a CTA, 2 x 4 a thread, on plain fp32 arithmetic
-template <class T>
-__global__ void __launch_bounds__(256) mul_fp8_plain_kernel(const Fp8Params p) {
-  constexpr int TM = 32, TN = 64, TK = 32;
-  __shared__ float as[TK][TM + 1], bs[TK][TN + 1];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float sum[2][4] = {};
-  for (int b = 0; b < p.kb; ++b) {
-    float part[2][4] = {};
-    for (int k0 = b * kBlock; k0 < p.K && k0 < (b + 1) * kBlock; k0 += TK) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < (TM + TN) * TK; i += 256) {
-        const int k = i % TK, r = i / TK;
-        const bool is_a = r < TM;
-        const int row = is_a ? m0 + r : n0 + r - TM;
-        float v = 0.f;
-        if (row < (is_a ? p.M : p.N) && k0 + k < p.K) {
-          __nv_fp8_e4m3 e;
-          e.__x = (is_a ? p.A : p.B)[(size_t)row * p.K + k0 + k];
-          v = (float)e;
-        }
-        if (is_a) as[k][r] = v; else bs[k][r - TM] = v;
-      }
-      __syncthreads();
-      for (int k = 0; k < TK; ++k)
+// x (bytes of K) is a multiple of 128: the copy starts on a 16-byte boundary
+__device__ __forceinline__ void tma_load_bytes(uint32_t dst, const CUtensorMap* map, int x, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_bytes(const CUtensorMap* map, int x, int row) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(row) : "memory");
+}
+// D[128 x N] = A[128 x 128] B[N x 128]^T of E4M3 values, both in 128-byte rows with the 128-byte swizzle: four MMAs of 32 values of K
+__device__ __forceinline__ void mma_block(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i)
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        ::"r"(d_tmem), "l"(a_desc + 2 * i), "l"(b_desc + 2 * i), "r"(idesc), "r"(i) : "memory");
+}
+template <int kCount>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[kCount]) {
+  static_assert(kCount == 16 || kCount == 32, "columns per load");
+  if constexpr (kCount == 16) {
+    tc_ld16(taddr, v);
+  } else {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+    tc_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] += as[k][ty * 2 + i] * bs[k][tx + 16 * j];
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + ty * 2 + i, n = n0 + tx + 16 * j;
-        if (m < p.M && n < p.N) sum[i][j] += part[i][j] * (p.sa[(size_t)m * p.kb + b] * p.sb[(size_t)(n / kBlock) * p.kb + b]);
-      }
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty * 2 + i, n = n0 + tx + 16 * j;
-      if (m < p.M && n < p.N) store(static_cast<T*>(p.C) + (size_t)m * p.N + n, sum[i][j]);
+}
+__device__ __forceinline__ float4 lds_float4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_value(half* c, float v) { *c = __float2half_rn(v); }
+__device__ __forceinline__ void store_value(__nv_bfloat16* c, float v) { *c = __float2bfloat16_rn(v); }
+
+// The blocks of all (strip, row tile) pairs, K fastest, then row tiles, are cut into as many equal ranges as there are CTAs.
+__device__ __forceinline__ int range_start(const Fp8Params& p, int cta) {
+  return (int)((long long)p.strips * p.row_tiles * p.kb * cta / (int)gridDim.x);
+}
+
+template <class T, class C>
+__global__ void __launch_bounds__(C::kThreads, 1)
+mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap) {
+  constexpr int S = C::kStages, D = C::kTiles, R = C::kScales;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* scales = reinterpret_cast<float*>(smem + S * C::kStageBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(scales + R * C::kRows);
+  volatile uint32_t* misc = reinterpret_cast<uint32_t*>(bars + C::kNumBars);        // [0] TMEM base, [1] launch epoch
+  const uint32_t full = smem_u32(bars), empty = full + 8 * S, done = empty + 8 * S, taken = done + 8 * D;
+  const uint32_t scaled = taken + 8 * D, used = scaled + 8 * R, epoch_bar = used + 8 * R;
+
+  const int tid = threadIdx.x, warp = uniform_warp_index(), lane = tid & 31;
+  // Ranges are handed out from the last to the first: a CTA that waits for the partials of higher ranges waits for CTAs that
+  // were dispatched before it.
+  const int cta = gridDim.x - 1 - blockIdx.x;
+  const int B0 = range_start(p, cta), B1 = range_start(p, cta + 1);
+  const int nt = p.tile_rows;
+  launch_dependents();
+
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full + 8 * s, 1);            // the expect_tx arrival of the producer
+      mbar_init(empty + 8 * s, 1);           // tcgen05.commit: the block's MMAs have read the stage
     }
+    for (int d = 0; d < D; ++d) {
+      mbar_init(done + 8 * d, 1);            // tcgen05.commit: the tile holds the block's products
+      mbar_init(taken + 8 * d, C::kWarps);   // the warps have read it back
+    }
+    for (int r = 0; r < R; ++r) {
+      mbar_init(scaled + 8 * r, 1);
+      mbar_init(used + 8 * r, C::kWarps);
+    }
+    mbar_init(epoch_bar, 1);
+    mbar_fence_init();
+  }
+  if (warp == 3) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(misc))), "r"(C::kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, misc[0], 0);
+  bool dead = false;
+
+  if (warp == 0) {
+    // ================================================================== producer of weights and activations
+    const uint32_t bytes = kStripBytes + nt * kBlock;
+    const int first = B1 - B0 < S ? B1 - B0 : S;                     // blocks whose stages are free from the start
+    auto load_weights = [&](int n, int u) {
+      mbar_arrive_expect_tx(full + 8 * n, bytes);
+      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes, &bmap, u % p.kb * kBlock, u / p.kb / p.row_tiles * kBlock, full + 8 * n);
+    };
+    auto load_rows = [&](int n, int u) {
+      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes + kStripBytes, &amap, u % p.kb * kBlock, u / p.kb % p.row_tiles * nt, full + 8 * n);
+    };
+    if (elect_one()) {
+      for (int n = 0; n < first; ++n)
+        if (p.weights_early) load_weights(n, B0 + n);
+        else tma_prefetch_bytes(&bmap, (B0 + n) % p.kb * kBlock, (B0 + n) / p.kb / p.row_tiles * kBlock);
+    }
+    __syncwarp();
+    grid_dependency_wait();
+    if (elect_one()) {
+      for (int n = 0; n < first; ++n) {
+        if (!p.weights_early) load_weights(n, B0 + n);
+        load_rows(n, B0 + n);
+      }
+    }
+    __syncwarp();
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int u = B0 + first; u < B1; ++u) {
+      mbar_wait_bounded<100>(empty + 8 * stage, phase, p.status, dead);
+      if (elect_one()) {
+        load_weights(stage, u);
+        load_rows(stage, u);
+      }
+      __syncwarp();
+      if (++stage == S) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1) {
+    // ================================================================== MMA issuer
+    grid_dependency_wait();                  // the bounded waits start when the kernel in front has finished
+    const uint64_t desc0 = wide_act_desc(smem_u32(smem));
+    // D fp32, A and B E4M3, K-major; N = rows of the tile, M = 128
+    const uint32_t idesc = (1u << 4) | ((uint32_t)(nt >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    int stage = 0, tile = 0;
+    uint32_t phase = 0, tphase = 0;
+    for (int u = B0; u < B1; ++u) {
+      mbar_wait_bounded<20>(taken + 8 * tile, tphase ^ 1, p.status, dead);
+      mbar_wait_bounded<20>(full + 8 * stage, phase, p.status, dead);
+      tc_fence_after();
+      // the descriptor's low 14 bits hold the address / 16: adding an offset never carries out of them
+      const uint64_t a_desc = desc0 + (uint64_t)(stage * (C::kStageBytes >> 4));
+      if (elect_one()) {
+        mma_block(tmem + tile * C::kRows, a_desc, a_desc + (kStripBytes >> 4), idesc);
+        tc_commit(empty + 8 * stage);
+        tc_commit(done + 8 * tile);
+      }
+      __syncwarp();
+      if (++stage == S) { stage = 0; phase ^= 1; }
+      if (++tile == D) { tile = 0; tphase ^= 1; }
+    }
+  } else if (warp == 2) {
+    // ================================================================== scales: sa * sb of the block for every row of the tile
+    grid_dependency_wait();
+    constexpr int E = (C::kRows + 31) / 32;
+    float now[E];
+    auto load = [&](int u) {
+      const int b = u % p.kb, v = u / p.kb, row0 = v % p.row_tiles * nt;
+      const float column = p.sb[(size_t)(v / p.row_tiles) * p.kb + b];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int m = lane + 32 * i;
+        now[i] = m < nt && row0 + m < p.M ? p.sa[(size_t)(row0 + m) * p.kb + b] * column : 0.f;
+      }
+    };
+    if (B0 < B1) load(B0);
+    int r = 0;
+    uint32_t phase = 0;
+    for (int u = B0; u < B1; ++u) {
+      mbar_wait_bounded<100>(used + 8 * r, phase ^ 1, p.status, dead);
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (C::kRows % 32 == 0 || lane + 32 * i < C::kRows) sts_f32(smem_u32(scales + r * C::kRows + lane + 32 * i), now[i]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(scaled + 8 * r);
+      if (u + 1 < B1) load(u + 1);
+      if (++r == R) { r = 0; phase ^= 1; }
+    }
+  } else if (warp == 3) {
+    // ================================================================== launch epoch: the tag of this launch's partials is epoch + 1
+    if (lane == 0) {
+      grid_dependency_wait();
+      misc[1] = read_epoch_and_count(p.epochs, gridDim.x);
+      mbar_arrive(epoch_bar);
+    }
+    __syncwarp();
+  } else {
+    // ================================================================== sums: thread = column of the strip, kMine rows
+    constexpr int CH = C::kChunk, E = C::kMine;
+    const int quarter = warp & 3, row_base = (warp - 4) / 4 * E;
+    const int c = quarter * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + row_base;
+    grid_dependency_wait();
+    float sum[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum[i] = 0.f;
+    int tile = 0, r = 0, slice_start = B0;
+    uint32_t tphase = 0, rphase = 0;
+    for (int u = B0; u < B1; ++u) {
+      mbar_wait_bounded<20>(scaled + 8 * r, rphase, p.status, dead);
+      mbar_wait_bounded<20>(done + 8 * tile, tphase, p.status, dead);
+      tc_fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < E; c0 += CH) {
+        if (row_base + c0 < nt) {            // the same for all threads of the warp
+          float v[CH];
+          tmem_load<CH>(lane_base + tile * C::kRows + c0, v);
+          const uint32_t from = smem_u32(scales + r * C::kRows + row_base + c0);
+#pragma unroll
+          for (int i = 0; i < CH; i += 4) {
+            const float4 s = lds_float4(from + 4 * i);
+            sum[c0 + i] = fmaf(v[i], s.x, sum[c0 + i]);
+            sum[c0 + i + 1] = fmaf(v[i + 1], s.y, sum[c0 + i + 1]);
+            sum[c0 + i + 2] = fmaf(v[i + 2], s.z, sum[c0 + i + 2]);
+            sum[c0 + i + 3] = fmaf(v[i + 3], s.w, sum[c0 + i + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(taken + 8 * tile);
+        mbar_arrive(used + 8 * r);
+      }
+      if (++tile == D) { tile = 0; tphase ^= 1; }
+      if (++r == R) { r = 0; rphase ^= 1; }
+
+      const bool strip_ends = (u + 1) % p.kb == 0;
+      if (!strip_ends && u + 1 < B1) continue;
+      // ---- the end of a slice: this CTA's blocks of one strip and row tile
+      const int v = u / p.kb, row0 = v % p.row_tiles * nt + row_base;
+      const int column = v / p.row_tiles * kBlock + c;
+      const bool starts = slice_start % p.kb == 0;
+      const int rows = min(min(nt - row_base, E), p.M - row0);           // rows of this thread that exist
+      uint32_t tag = 0;
+      if (!starts || !strip_ends) {
+        mbar_wait_bounded<20>(epoch_bar, 0, p.status, dead);
+        tag = misc[1] + 1;
+      }
+      auto slot_of = [&](int other) { return p.partials + ((size_t)other * nt + row_base) * kBlock + c; };
+      if (!starts) {
+        // Only the first slice of a CTA can start inside a strip, so a CTA has one partial.
+        unsigned long long* slot = slot_of(cta);
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (i < rows) st_relaxed_u64(slot + (size_t)i * kBlock, ((unsigned long long)tag << 32) | __float_as_uint(sum[i]));
+      } else {
+        // The CTA in which a strip starts adds the partials of the CTAs behind it, in their order.
+        if (!strip_ends) {
+          const int end = (v + 1) * p.kb;
+#pragma unroll 1
+          for (int other = cta + 1; other < (int)gridDim.x && range_start(p, other) < end; ++other) {
+            const unsigned long long* slot = slot_of(other);
+#pragma unroll
+            for (int i0 = 0; i0 < E; i0 += 16) {
+              unsigned long long w[16];
+              bool here = i0 >= rows;
+#pragma unroll 1
+              for (int spin = 0; spin < (1 << 20) && !here; ++spin) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = i0 + i < rows ? ld_relaxed_u64(slot + (size_t)(i0 + i) * kBlock) : 0;
+                here = true;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) here = here && (i0 + i >= rows || (uint32_t)(w[i] >> 32) == tag);
+                if (dead) break;             // a wait of this thread ran out before: do not wait again
+              }
+              if (!here && !dead) {
+                dead = true;
+                if (p.status) atomicExch(p.status, kStatusTimeout);
+              }
+              if (i0 < rows) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum[i0 + i] += i0 + i < rows ? __uint_as_float((uint32_t)w[i]) : 0.f;
+              }
+            }
+          }
+        }
+        if (column < p.N) {
+          T* out = static_cast<T*>(p.C) + (size_t)row0 * p.N + column;
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if (i < rows) store_value(out + (size_t)i * p.N, sum[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) sum[i] = 0.f;
+      slice_start = u + 1;
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+}
+
+struct Fp8Plan {
+  int row_tiles, tile_rows, ctas;
+};
+Fp8Plan plan_fp8(int M, int N, int K, int sms) {
+  Fp8Plan plan;
+  plan.row_tiles = (M + 255) / 256;
+  plan.tile_rows = ((M + plan.row_tiles - 1) / plan.row_tiles + 15) / 16 * 16;
+  const long long blocks = (long long)((N + kBlock - 1) / kBlock) * plan.row_tiles * ((K + kBlock - 1) / kBlock);
+  long long ctas = sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas;
+  if (ctas > (blocks + 3) / 4) ctas = (blocks + 3) / 4;
+  plan.ctas = (int)ctas;
+  return plan;
+}
+size_t plan_bytes(const Fp8Plan& plan) {
+  return kEpochWords * sizeof(unsigned int) + (size_t)plan.ctas * plan.tile_rows * kBlock * sizeof(unsigned long long);
+}
+
+template <class T, class C>
+cudaError_t launch_fp8(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(mul_fp8_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(mul_fp8_kernel<T, C>, dim3(ctas), dim3(C::kThreads), C::kSmemBytes, stream, p, amap, bmap);
+}
+template <class T>
+cudaError_t launch_fp8_rows(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+  if (p.tile_rows <= 16) return launch_fp8<T, Fp8Cfg<16, 4>>(p, ctas, amap, bmap, stream);
+  if (p.tile_rows <= 32) return launch_fp8<T, Fp8Cfg<32, 4>>(p, ctas, amap, bmap, stream);
+  if (p.tile_rows <= 64) return launch_fp8<T, Fp8Cfg<64, 8>>(p, ctas, amap, bmap, stream);
+  if (p.tile_rows <= 128) return launch_fp8<T, Fp8Cfg<128, 8>>(p, ctas, amap, bmap, stream);
+  return launch_fp8<T, Fp8Cfg<256, 8>>(p, ctas, amap, bmap, stream);
 }
 
 }  // namespace
 
-extern "C" int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const void* sb, int M, int N, int K, int type, void* scratch,
-                            size_t scratch_bytes, int dev, void* stream, int* status_dev) {
+}  // namespace fp6m
+
+extern "C" {
+
+size_t fp6m_mul_fp8_scratch_bytes(int M, int N, int K, int sms) {
+  if (M <= 0 || N <= 0 || K <= 0) return 256;
+  return (fp6m::plan_bytes(fp6m::plan_fp8(M, N, K, sms)) + 255) & ~(size_t)255;
+}
+
+int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const void* sb, int M, int N, int K, int type, void* scratch, size_t scratch_bytes,
+                 int dev, void* stream, int* status_dev) {
+  using namespace fp6m;
   if (M < 0 || N < 0 || K < 0 || (type != FP6M_TYPE_F16 && type != FP6M_TYPE_BF16)) return FP6M_ERR_BAD_ARG;
   if (K % 16 || N % 8) return FP6M_ERR_PROB_SHAPE;
   if (M == 0 || N == 0) return FP6M_OK;
   if (!C || !aligned16(C)) return FP6M_ERR_BAD_ARG;
-  DeviceGuard guard(dev);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (K == 0) {                          // an empty sum
+    DeviceGuard guard(dev);
     const cudaError_t e = cudaMemsetAsync(C, 0, (size_t)M * N * 2, st);
     return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "mul_fp8 of no terms");
   }
-  if (!A || !B || !sa || !sb || !aligned16(A) || !aligned16(B) || ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sb)) & 3)) return FP6M_ERR_BAD_ARG;
-  const Fp8Params p = {static_cast<const uint8_t*>(A), static_cast<const uint8_t*>(B), C, static_cast<const float*>(sa), static_cast<const float*>(sb),
-                       M, N, K, (K + kBlock - 1) / kBlock};
-  const dim3 grid((N + 63) / 64, (M + 31) / 32);
-  if (grid.y > 65535) return FP6M_ERR_PROB_SHAPE;
-  const cudaError_t e = type == FP6M_TYPE_F16 ? launch_overlapped(mul_fp8_plain_kernel<half>, grid, dim3(256), 0, st, p)
-                                              : launch_overlapped(mul_fp8_plain_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p);
+  if (!A || !B || !sa || !sb || !scratch || !aligned16(A) || !aligned16(B) || !aligned16(scratch) ||
+      ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sb)) & 3))
+    return FP6M_ERR_BAD_ARG;
+  if ((long long)((N + kBlock - 1) / kBlock) * ((M + 255) / 256) * ((K + kBlock - 1) / kBlock) > 0x3fffffff) return FP6M_ERR_PROB_SHAPE;
+  DeviceGuard guard(dev);
+  const int sms = sm_count(dev);
+  if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
+  const Fp8Plan plan = plan_fp8(M, N, K, sms);
+  if (scratch_bytes < plan_bytes(plan)) return FP6M_ERR_SCRATCH;
+  Fp8Params p;
+  p.C = C;
+  p.sa = static_cast<const float*>(sa);
+  p.sb = static_cast<const float*>(sb);
+  p.M = M;
+  p.N = N;
+  p.kb = (K + kBlock - 1) / kBlock;
+  p.strips = (N + kBlock - 1) / kBlock;
+  p.row_tiles = plan.row_tiles;
+  p.tile_rows = plan.tile_rows;
+  p.weights_early = tc5_get_overlap() ? 1 : 0;
+  p.epochs = static_cast<unsigned int*>(scratch);
+  p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(scratch) + kEpochWords * sizeof(unsigned int));
+  p.status = status_dev;
+  CUtensorMap amap, bmap;
+  cudaError_t e = encode_bytes_map(A, M, K, plan.tile_rows, &amap);
+  if (e == cudaSuccess) e = encode_bytes_map(B, N, K, kBlock, &bmap);
+  if (e != cudaSuccess) return cuda_fail(e, "mul_fp8 tensor maps");
+  e = type == FP6M_TYPE_F16 ? launch_fp8_rows<half>(p, plan.ctas, amap, bmap, st) : launch_fp8_rows<__nv_bfloat16>(p, plan.ctas, amap, bmap, st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "mul_fp8 launch");
 }
 
-extern "C" size_t fp6m_mul_fp8_scratch_bytes(int M, int N, int K, int sms) { return 256; }
+}  // extern "C"
