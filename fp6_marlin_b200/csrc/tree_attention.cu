@@ -4,75 +4,570 @@
 //
 // over the lengths[b] cached tokens and the drafted tokens j whose bit is set in the mask of i.  A mask of zero marks padding:
 // it sees nothing and gives zeros.  The reference has no counterpart; its layer lists (bench.py:53-86) name the products on either side.
+//
+// The queries that share a head of keys - T tokens times heads / kv_heads heads - are the rows of one product; a sequence's keys
+// are its cached tokens followed by its drafted ones, in tiles of 64.  The (sequence, head of keys, row tile, key tile) units
+// are cut into equal ranges, one per CTA, so that long and short sequences and few heads load all multiprocessors alike; the
+// cut is made on the device, from the lengths, and the launch does not depend on them.  One pass over the keys keeps a
+// running maximum and sum per row in fp32.  Rows whose keys are shared by several CTAs are joined by the one that finishes
+// last (an arrival counter; nobody waits), in the order of the ranges, so results do not depend on who that is.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "../../include/fp6m.h"
+#include "device_utils.cuh"
 #include "host_common.h"
 
 namespace {
 
 using namespace fp6m;
 
-__device__ __forceinline__ float to_float(half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void store(half* c, float v) { *c = __float2half_rn(v); }
-__device__ __forceinline__ void store(__nv_bfloat16* c, float v) { *c = __float2bfloat16_rn(v); }
+constexpr int kKeys = 64;                // keys per tile
+constexpr int kThreads = 128;
+constexpr int kMaxCtas = 512;
+constexpr int kCounterBytes = kMaxCtas * 4;
 
-// One warp a query, a key at a time.
-template <class T, int D>
-__global__ void __launch_bounds__(128) tree_attention_plain_kernel(const fp6m_tree_attention_args a, int* status) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const long long query = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (query >= (long long)a.batch * a.tokens * a.heads) return;
-  const int h = (int)(query % a.heads), t = (int)(query / a.heads % a.tokens), b = (int)(query / a.heads / a.tokens);
-  const int g = h / (a.heads / a.kv_heads);
-  constexpr int E = D / 32;
-  const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + t * a.q_stride[1] + h * a.q_stride[2];
-  float qf[E], o[E] = {}, top = -INFINITY, total = 0.f;
-  for (int i = 0; i < E; ++i) qf[i] = to_float(q[lane + 32 * i]) * a.scale;
-  const unsigned long long mask = static_cast<const unsigned long long*>(a.tree)[b * a.tree_stride + t];
-  const int capacity = a.max_pages * a.page_size;
-  int length = static_cast<const int*>(a.lengths)[b];
-  length = length < 0 ? 0 : length > capacity ? capacity : length;
-  auto visit = [&](const T* k, const T* v) {
-    float s = 0.f;
-    for (int i = 0; i < E; ++i) s += qf[i] * to_float(k[lane + 32 * i]);
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float now = fmaxf(top, s);
-    if (now == -INFINITY) return;
-    const float keep = __expf(top - now), p = __expf(s - now);
-    total = total * keep + p;
-    for (int i = 0; i < E; ++i) o[i] = o[i] * keep + p * to_float(v[lane + 32 * i]);
-    top = now;
-  };
-  if (mask) {
-    for (int j = 0; j < length; ++j) {
-      const int page = static_cast<const int*>(a.page_table)[b * a.page_table_stride + j / a.page_size];
-      if (page < 0 || page >= a.pages) {
-        if (lane == 0 && status) atomicExch(status, FP6M_ERR_BAD_ARG);
-        continue;
-      }
-      const long long slot = j % a.page_size;
-      visit(static_cast<const T*>(a.k_cache) + page * a.k_cache_stride[0] + slot * a.k_cache_stride[1] + g * a.k_cache_stride[2],
-            static_cast<const T*>(a.v_cache) + page * a.v_cache_stride[0] + slot * a.v_cache_stride[1] + g * a.v_cache_stride[2]);
-    }
-    for (int j = 0; j < a.tokens; ++j)
-      if (mask >> j & 1)
-        visit(static_cast<const T*>(a.k) + b * a.k_stride[0] + j * a.k_stride[1] + g * a.k_stride[2],
-              static_cast<const T*>(a.v) + b * a.v_stride[0] + j * a.v_stride[1] + g * a.v_stride[2]);
+struct TreeParams {
+  fp6m_tree_attention_args a;
+  int group, rows, row_tiles;            // heads of queries per head of keys; rows and row tiles of a head of keys
+  unsigned long long page_magic;         // division by the page size: n * magic >> shift, exact for n < 2^31
+  int page_shift;
+  float scale_log2;                      // scale * log2(e): the softmax is computed in powers of two
+  unsigned int* arrived;                 // [CTA] contributors that have left their partial for the rows that start in that CTA
+  float* partials;                       // [CTA][2]: sums of row tile x head_dim, then maxima, then totals
+  int* status;
+};
+
+template <class T> struct Mma;
+template <> struct Mma<half> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + t * a.out_stride[1] + h * a.out_stride[2];
-  for (int i = 0; i < E; ++i) store(out + lane + 32 * i, total > 0.f ? o[i] / total : total == total ? 0.f : total);
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ float value(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
+  static constexpr uint32_t kExponent = 0x7c00u;
+};
+template <> struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ float value(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
+  static constexpr uint32_t kExponent = 0x7f80u;
+};
+
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// sixteen bytes, or zeros where `bytes` is 0 (the source is not read then)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
+__device__ __forceinline__ int length_of(const TreeParams& p, int b) {
+  const int n = p.a.lengths[b], most = p.a.max_pages * p.a.page_size;
+  return n < 0 ? 0 : n > most ? most : n;
+}
+__device__ __forceinline__ int tiles_of(const TreeParams& p, int length) { return (int)(((long long)length + p.a.tokens + kKeys - 1) / kKeys); }
+
+// The start of a CTA's range, and the CTA whose range a unit lies in.
+__device__ __forceinline__ long long range_start(long long units, int ctas, int cta) { return units * cta / ctas; }
+__device__ __forceinline__ int cta_of(long long units, int ctas, long long unit) {
+  int c = (int)(unit * ctas / units);
+  while (c + 1 < ctas && range_start(units, ctas, c + 1) <= unit) ++c;
+  while (range_start(units, ctas, c) > unit) --c;
+  return c;
+}
+
+// A place in the sequence of units: the key tile of a (head of keys, row tile) pair of a sequence.
+struct Cursor {
+  int b, length, tiles, pair, tile;
+  __device__ __forceinline__ void next(const TreeParams& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++pair < p.a.kv_heads * p.row_tiles) return;
+    pair = 0;
+    if (++b < p.a.batch) {
+      length = length_of(p, b);
+      tiles = tiles_of(p, length);
+    }
+  }
+};
+
+// kRowTile rows, a warp for every 16 of them; the warps that this leaves share the keys of a tile and pool their sums.
+template <class T, int D, int kRowTile>
+__global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __grid_constant__ TreeParams p) {
+  constexpr int kRowWarps = kRowTile / 16, kKeyWarps = 4 / kRowWarps;
+  constexpr int kMine = kKeys / kKeyWarps;                           // keys of a tile that a warp works on
+  constexpr int kRowBytes = D * 2, kTileBytes = kKeys * kRowBytes;   // keys or values of a tile
+  constexpr int kStages = 3 * 128 / D;
+  constexpr int kChunks = D / 8, kRowsPerPass = kThreads / kChunks, kPasses = kKeys / kRowsPerPass;
+  constexpr int kPool = D / kRowWarps;                               // columns of the sums that are pooled at a time
+  constexpr int kSlot = kRowTile * (D + 2);                          // floats of a partial
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* pool = reinterpret_cast<float*>(smem + kStages * 2 * kTileBytes);        // [kRowTile][kPool]
+  float* stats = pool + kRowTile * kPool;                                          // [warp][2][16]: maxima, totals
+  long long* plan = reinterpret_cast<long long*>(stats + 4 * 32);                  // total units; unit of the first pair, b
+  int* flags = reinterpret_cast<int*>(plan + 4);                                   // [0] a page did not exist, [1] last to arrive
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row_warp = warp / kKeyWarps, key_warp = warp % kKeyWarps;
+  const fp6m_tree_attention_args& a = p.a;
+  const int pairs = a.kv_heads * p.row_tiles;
+  if (tid == 0) flags[0] = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- the plan: units of all sequences, and where this CTA's range starts
+  if (warp == 0) {
+    long long units = 0;
+    for (int b = lane; b < a.batch; b += 32) units += (long long)tiles_of(p, length_of(p, b)) * pairs;
+    for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+    const int ctas = (long long)gridDim.x < units ? (int)gridDim.x : (int)units;
+    const long long first = (int)blockIdx.x < ctas ? range_start(units, ctas, blockIdx.x) : units;
+    long long before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int b = b0 + lane;
+      const long long mine = b < a.batch ? (long long)tiles_of(p, length_of(p, b)) * pairs : 0;
+      long long upto = mine;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += other;
+      }
+      if (first >= before + upto - mine && first < before + upto) {
+        plan[1] = first - (before + upto - mine);
+        plan[2] = b;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+      if (before > first) break;
+    }
+    if (lane == 0) plan[0] = units;
+  }
+  __syncthreads();
+  const long long units = plan[0];
+  const int ctas = (long long)gridDim.x < units ? (int)gridDim.x : (int)units;
+  const int cta = blockIdx.x;
+  if (cta >= ctas) return;
+  const long long u0 = range_start(units, ctas, cta);
+  const int count = (int)(range_start(units, ctas, cta + 1) - u0);
+  Cursor at;
+  at.b = (int)plan[2];
+  at.length = length_of(p, at.b);
+  at.tiles = tiles_of(p, at.length);
+  at.pair = (int)(plan[1] / at.tiles);
+  at.tile = (int)(plan[1] % at.tiles);
+
+  // ---- copies of a tile: a row of keys and one of values per token, zeros behind the last
+  const int load_row = tid / kChunks, chunk = tid % kChunks;
+  const uint32_t smem_base = smem_u32(smem);
+  auto load = [&](const Cursor& c, int stage) {
+    const int g = c.pair / p.row_tiles, last = c.length + a.tokens;
+    const uint32_t dst = smem_base + stage * 2 * kTileBytes;
+    const int* table = a.page_table + c.b * a.page_table_stride;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int row = load_row + i * kRowsPerPass, j = c.tile * kKeys + row;
+      const T *k = static_cast<const T*>(a.q), *v = k;
+      uint32_t bytes = 0;
+      if (j < c.length) {
+        const int index = (int)((unsigned long long)j * p.page_magic >> p.page_shift);
+        const int page = table[index], slot = j - index * a.page_size;
+        if ((unsigned)page < (unsigned)a.pages) {
+          k = static_cast<const T*>(a.k_cache) + page * a.k_cache_stride[0] + slot * a.k_cache_stride[1] + g * a.k_cache_stride[2];
+          v = static_cast<const T*>(a.v_cache) + page * a.v_cache_stride[0] + slot * a.v_cache_stride[1] + g * a.v_cache_stride[2];
+          bytes = 16;
+        } else {
+          flags[0] = 1;
+        }
+      } else if (j < last) {
+        k = static_cast<const T*>(a.k) + c.b * a.k_stride[0] + (j - c.length) * a.k_stride[1] + g * a.k_stride[2];
+        v = static_cast<const T*>(a.v) + c.b * a.v_stride[0] + (j - c.length) * a.v_stride[1] + g * a.v_stride[2];
+        bytes = 16;
+      }
+      const uint32_t to = dst + row * kRowBytes + ((chunk ^ (row & 7)) * 16);
+      copy16(to, k + chunk * 8, bytes);
+      copy16(to + kTileBytes, v + chunk * 8, bytes);
+    }
+  };
+
+  Cursor ahead = at;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (s < count) {
+      load(ahead, s);
+      ahead.next(p);
+    }
+    copies_commit();
+  }
+
+  const int quad = lane >> 2, col = (lane & 3) * 2;                  // this thread's rows quad and quad + 8, columns col and col + 1 of a fragment
+  uint32_t q[D / 16][4];
+  float o[D / 8][4], top[2], total[2];
+  unsigned long long mask[2];
+  bool fresh = true;
+  int segment_tile = 0;
+  long long item_unit = 0;                                           // the first unit of these rows
+  int stage = 0;
+#pragma unroll 1
+  for (int n = 0; n < count; ++n) {
+    const int g = at.pair / p.row_tiles, tile_row0 = at.pair % p.row_tiles * kRowTile;
+    if (fresh) {
+      // ---- new rows: queries and masks
+      fresh = false;
+      segment_tile = at.tile;
+      item_unit = u0 + n - at.tile;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = tile_row0 + row_warp * 16 + quad + 8 * h;
+        mask[h] = 0;
+        const T* src = nullptr;
+        if (r < p.rows) {
+          const int t = r / p.group, head = g * p.group + (r - t * p.group);
+          mask[h] = a.tree[at.b * a.tree_stride + t];
+          src = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          q[i][h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + col) : 0u;
+          q[i][2 + h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + 8 + col) : 0u;
+        }
+        top[h] = -INFINITY;
+        total[h] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    }
+    copies_wait<kStages - 2>();
+    __syncthreads();
+    if (n + kStages - 1 < count) {
+      load(ahead, (stage + kStages - 1) % kStages);
+      ahead.next(p);
+    }
+    copies_commit();
+
+    // ---- scores of this warp's keys
+    const uint32_t keys = smem_base + stage * 2 * kTileBytes + key_warp * kMine * kRowBytes, values = keys + kTileBytes;
+    float s[kMine / 8][4];
+#pragma unroll
+    for (int i = 0; i < kMine / 8; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+      const int row = i * 8 + (lane & 7);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        uint32_t k[4];
+        ldsm(k, keys + row * kRowBytes + (((d * 4 + (lane >> 3)) ^ (row & 7)) * 16));
+        Mma<T>::run(s[i], q[2 * d], k[0], k[1]);
+        Mma<T>::run(s[i], q[2 * d + 1], k[2], k[3]);
+      }
+    }
+    const int j0 = at.tile * kKeys + key_warp * kMine;               // this warp's first key
+    const bool drafted = at.tile * kKeys + kKeys > at.length;        // the tile holds drafted tokens, or the end
+    const bool hidden = flags[0] != 0;                               // a page of this CTA's tiles did not exist
+#pragma unroll
+    for (int i = 0; i < kMine / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
+    if (drafted) {
+#pragma unroll
+      for (int i = 0; i < kMine / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = j0 + i * 8 + col + (e & 1) - at.length;      // drafted token, negative: cached
+          if (t >= 0 && (t >= 64 || !(mask[e >> 1] >> t & 1))) s[i][e] = -INFINITY;
+        }
+    }
+    if (hidden) {
+      const int* table = a.page_table + at.b * a.page_table_stride;
+#pragma unroll 1
+      for (int i = 0; i < kMine; ++i) {
+        const int j = j0 + i;
+        if (j >= at.length || (unsigned)table[(int)((unsigned long long)j * p.page_magic >> p.page_shift)] < (unsigned)a.pages) continue;
+#pragma unroll
+        for (int k = 0; k < kMine / 8; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (k * 8 + col + (e & 1) == i) s[k][e] = -INFINITY;
+      }
+    }
+
+    // ---- running maximum and sum; weights in the values' type for the second product
+    float keep[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float m = top[h];
+#pragma unroll
+      for (int i = 0; i < kMine / 8; ++i) m = fmaxf(m, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const float base = m == -INFINITY ? 0.f : m;                   // nothing seen so far
+      keep[h] = exp2_approx(top[h] - base);
+      top[h] = m;
+      total[h] *= keep[h];
+#pragma unroll
+      for (int i = 0; i < kMine / 8; ++i)
+#pragma unroll
+        for (int e = 2 * h; e < 2 * h + 2; ++e) {
+          s[i][e] = exp2_approx(s[i][e] - base);
+          total[h] += s[i][e];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] *= keep[e >> 1];
+
+    // ---- infinities and NaN among the drafted values: a weight of zero must not meet them
+    if (drafted) {
+      const int from = max(at.length - at.tile * kKeys, 0), upto = min(at.length + a.tokens - at.tile * kKeys, kKeys);
+      const uint32_t tile_values = smem_base + stage * 2 * kTileBytes + kTileBytes;
+      bool odd = false;
+      for (int i = tid; i < (upto - from) * kChunks; i += kThreads) {
+        const int row = from + i / kChunks;
+        uint4 w;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(tile_values + row * kRowBytes + i % kChunks * 16) : "memory");
+        constexpr uint32_t E = Mma<T>::kExponent;
+        auto is_odd = [&](uint32_t x) { return (x & E) == E || (x >> 16 & E) == E; };
+        odd = odd || is_odd(w.x) || is_odd(w.y) || is_odd(w.z) || is_odd(w.w);
+      }
+      if (__syncthreads_or(odd)) {
+        // each is multiplied by the weights of the rows that see it only, and is zero in the product below
+#pragma unroll 1
+        for (int j = 0; j < kMine; ++j) {
+          float w[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mine = 0.f;
+#pragma unroll
+            for (int k = 0; k < kMine / 8; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (k * 8 + e == (j & ~7) + (j & 1)) mine = s[k][2 * h + e];
+            w[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + (j & 7) / 2);
+          }
+          const int t = j0 + j - at.length;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            uint32_t two;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(values + j * kRowBytes + ((i ^ (j & 7)) * 16) + col * 2) : "memory");
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t bits = e & 1 ? two >> 16 : two & 0xffffu;
+              const bool sees = t >= 0 && t < 64 && (mask[e >> 1] >> t & 1);
+              if (sees && (bits & Mma<T>::kExponent) == Mma<T>::kExponent) o[i][e] += w[e >> 1] * Mma<T>::value((uint16_t)bits);
+            }
+          }
+        }
+        __syncthreads();
+        for (int i = tid; i < (upto - from) * D / 2; i += kThreads) {
+          const uint32_t addr = tile_values + (from + i / (D / 2)) * kRowBytes + i % (D / 2) * 4;
+          uint32_t two;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(addr) : "memory");
+          constexpr uint32_t E = Mma<T>::kExponent;
+          if ((two & E) == E) two &= 0xffff0000u;
+          if ((two >> 16 & E) == E) two &= 0xffffu;
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(two) : "memory");
+        }
+        __syncthreads();
+      }
+    }
+
+    // ---- weights times values
+#pragma unroll
+    for (int k = 0; k < kMine / 16; ++k) {
+      const uint32_t w[4] = {Mma<T>::pack(s[2 * k][0], s[2 * k][1]), Mma<T>::pack(s[2 * k][2], s[2 * k][3]),
+                             Mma<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), Mma<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
+      const int row = k * 16 + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t v[4];
+        ldsm_t(v, values + row * kRowBytes + (((2 * i + (lane >> 4)) ^ (row & 7)) * 16));
+        Mma<T>::run(o[2 * i], w, v[0], v[1]);
+        Mma<T>::run(o[2 * i + 1], w, v[2], v[3]);
+      }
+    }
+    stage = (stage + 1) % kStages;
+
+    const bool ends = at.tile + 1 == at.tiles;
+    if (ends || n + 1 == count) {
+      // ---- the end of this CTA's keys for these rows
+      fresh = true;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        total[h] += __shfl_xor_sync(0xffffffffu, total[h], 1);
+        total[h] += __shfl_xor_sync(0xffffffffu, total[h], 2);
+      }
+      if constexpr (kKeyWarps > 1) {
+        // the warps that shared the keys pool their sums, the last one first
+        if ((lane & 3) == 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            stats[warp * 32 + quad + 8 * h] = top[h];
+            stats[warp * 32 + 16 + quad + 8 * h] = total[h];
+          }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float* of = stats + row_warp * kKeyWarps * 32 + quad + 8 * h;
+          float m = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < kKeyWarps; ++w) m = fmaxf(m, of[w * 32]);
+          const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int w = 0; w < kKeyWarps; ++w) sum += of[w * 32 + 16] * exp2_approx(of[w * 32] - base);
+          const float mine = exp2_approx(top[h] - base);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][2 * h] *= mine;
+            o[i][2 * h + 1] *= mine;
+          }
+          top[h] = m;
+          total[h] = sum;
+        }
+#pragma unroll
+        for (int part = 0; part < kRowWarps; ++part) {
+#pragma unroll
+          for (int w = kKeyWarps - 1; w >= 0; --w) {
+            if (key_warp == w) {
+#pragma unroll
+              for (int i = 0; i < kPool / 8; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float2* place = reinterpret_cast<float2*>(pool + (row_warp * 16 + quad + 8 * h) * kPool + i * 8 + col);
+                  float (&mine)[4] = o[part * (kPool / 8) + i];
+                  if (w < kKeyWarps - 1) {
+                    const float2 sum = *place;
+                    mine[2 * h] += sum.x;
+                    mine[2 * h + 1] += sum.y;
+                  }
+                  if (w > 0) *place = make_float2(mine[2 * h], mine[2 * h + 1]);
+                }
+            }
+            __syncthreads();
+          }
+        }
+      }
+      const bool whole = segment_tile == 0 && ends;
+      auto out_row = [&](int r) {
+        const int t = r / p.group, head = g * p.group + (r - t * p.group);
+        return static_cast<T*>(a.out) + at.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+      };
+      if (whole) {
+        if (key_warp == 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = tile_row0 + row_warp * 16 + quad + 8 * h;
+            if (r < p.rows) {
+              // padding, and rows that see nothing, are zero
+              const bool none = mask[h] == 0 || total[h] == 0.f;
+              const float f = 1.f / total[h];
+              T* out = out_row(r) + col;
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<uint32_t*>(out + 8 * i) = none ? 0u : Mma<T>::pack(o[i][2 * h] * f, o[i][2 * h + 1] * f);
+            }
+          }
+        }
+      } else {
+        // a partial: the slot of a range's first rows, or that of its last ones
+        float* slot = p.partials + (size_t)(2 * cta + (segment_tile == 0 ? 1 : 0)) * kSlot;
+        if (key_warp == 0) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = row_warp * 16 + quad + 8 * h;
+            if (tile_row0 + r < p.rows) {
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(slot + r * D + i * 8 + col) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+              if ((lane & 3) == 0) {
+                slot[kRowTile * D + r] = top[h];
+                slot[kRowTile * (D + 1) + r] = total[h];
+              }
+            }
+          }
+        }
+        const int first_cta = segment_tile == 0 ? cta : cta_of(units, ctas, item_unit);
+        const int last_cta = cta_of(units, ctas, item_unit + at.tiles - 1);
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const unsigned int before = atomicAdd(p.arrived + first_cta, 1u);
+          const bool is_last = before == (unsigned)(last_cta - first_cta);
+          if (is_last) p.arrived[first_cta] = 0;                     // for the next launch
+          flags[1] = is_last;
+        }
+        __syncthreads();
+        if (flags[1]) {
+          __threadfence();
+          // a warp per row, sixteen or eight bytes a lane
+          constexpr int V = D / 32;
+          for (int r = warp; r < kRowTile && tile_row0 + r < p.rows; r += 4) {
+            float m = -INFINITY, sum = 0.f, acc[V] = {};
+            for (int c = first_cta; c <= last_cta; ++c) {
+              const float* from = p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot;
+              const float cm = __ldcg(from + kRowTile * D + r), ct = __ldcg(from + kRowTile * (D + 1) + r);
+              float v[V];
+#pragma unroll
+              for (int i = 0; i < V; i += 2) {
+                const float2 two = __ldcg(reinterpret_cast<const float2*>(from + r * D + lane * V + i));
+                v[i] = two.x;
+                v[i + 1] = two.y;
+              }
+              const float now = fmaxf(m, cm), base = now == -INFINITY ? 0.f : now;
+              const float old = exp2_approx(m - base), add = exp2_approx(cm - base);
+              sum = sum * old + ct * add;
+#pragma unroll
+              for (int i = 0; i < V; ++i) acc[i] = acc[i] * old + v[i] * add;
+              m = now;
+            }
+            const int t = (tile_row0 + r) / p.group;
+            const bool none = a.tree[at.b * a.tree_stride + t] == 0 || sum == 0.f;
+            const float f = 1.f / sum;
+            T* out = out_row(tile_row0 + r) + lane * V;
+#pragma unroll
+            for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Mma<T>::pack(acc[i] * f, acc[i + 1] * f);
+          }
+        }
+      }
+    }
+    at.next(p);
+  }
+  copies_wait<0>();
+  if (tid == 0 && flags[0] && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
+}
+
+template <class T, int D, int kRowTile>
+cudaError_t launch_tile(const TreeParams& p, int ctas, cudaStream_t stream) {
+  constexpr int bytes = 3 * 128 / D * 2 * kKeys * D * 2 + 16 * D * 4 + 4 * 32 * 4 + 4 * 8 + 16;
+  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, D, kRowTile>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(tree_attention_kernel<T, D, kRowTile>, dim3(ctas), dim3(kThreads), bytes, stream, p);
+}
 template <class T>
-cudaError_t launch_tree(const fp6m_tree_attention_args& a, cudaStream_t stream, int* status) {
-  const long long warps = (long long)a.batch * a.tokens * a.heads;
-  return launch_overlapped(a.head_dim == 64 ? tree_attention_plain_kernel<T, 64> : tree_attention_plain_kernel<T, 128>, dim3((unsigned)((warps + 3) / 4)), dim3(128),
-                           0, stream, a, status);
+cudaError_t launch_tree(const TreeParams& p, int row_tile, int ctas, cudaStream_t stream) {
+  if (p.a.head_dim == 64)
+    return row_tile == 16 ? launch_tile<T, 64, 16>(p, ctas, stream) : row_tile == 32 ? launch_tile<T, 64, 32>(p, ctas, stream) : launch_tile<T, 64, 64>(p, ctas, stream);
+  return row_tile == 16 ? launch_tile<T, 128, 16>(p, ctas, stream) : row_tile == 32 ? launch_tile<T, 128, 32>(p, ctas, stream) : launch_tile<T, 128, 64>(p, ctas, stream);
+}
+
+int tree_ctas(int sms) {
+  const int want = sms > 0 ? 2 * sms : kMaxCtas;
+  return want < kMaxCtas ? want : kMaxCtas;
 }
 
 // addresses and strides (in elements) of a tensor that is read or written sixteen bytes at a time
@@ -87,7 +582,7 @@ bool rows_aligned(const void* p, const long long (&strides)[kStrides]) {
 
 extern "C" {
 
-size_t fp6m_tree_attention_scratch_bytes(int sms) { return 256; }
+size_t fp6m_tree_attention_scratch_bytes(int sms) { return kCounterBytes + (size_t)tree_ctas(sms) * 2 * 64 * (128 + 2) * sizeof(float); }
 
 int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev) {
   if (!args) return FP6M_ERR_BAD_ARG;
@@ -97,13 +592,30 @@ int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, siz
   if (a.batch == 0 || a.tokens == 0 || a.heads == 0) return FP6M_OK;
   if (a.kv_heads <= 0 || a.heads % a.kv_heads) return FP6M_ERR_PROB_SHAPE;
   if (a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fffff00ll) return FP6M_ERR_PROB_SHAPE;
-  if ((long long)a.batch * a.tokens * a.heads > 0x7fffffffll) return FP6M_ERR_PROB_SHAPE;
+  if ((long long)a.tokens * a.heads > 0xffffffll) return FP6M_ERR_PROB_SHAPE;
   if (!rows_aligned(a.q, a.q_stride) || !rows_aligned(a.k, a.k_stride) || !rows_aligned(a.v, a.v_stride) || !rows_aligned(a.out, a.out_stride)) return FP6M_ERR_BAD_ARG;
-  if (!a.lengths || !a.tree || a.tree_stride < 0) return FP6M_ERR_BAD_ARG;
+  if (!a.lengths || !a.tree || a.tree_stride < 0 || !scratch || !aligned16(scratch)) return FP6M_ERR_BAD_ARG;
   if (a.max_pages > 0 && (!rows_aligned(a.k_cache, a.k_cache_stride) || !rows_aligned(a.v_cache, a.v_cache_stride) || !a.page_table || a.page_table_stride < 0)) return FP6M_ERR_BAD_ARG;
   DeviceGuard guard(dev);
+  const int sms = sm_count(dev);
+  if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
+  if (scratch_bytes < fp6m_tree_attention_scratch_bytes(sms)) return FP6M_ERR_SCRATCH;
+  TreeParams p;
+  p.a = a;
+  p.group = a.heads / a.kv_heads;
+  p.rows = a.tokens * p.group;
+  const int row_tile = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64;
+  p.row_tiles = (p.rows + row_tile - 1) / row_tile;
+  int log2 = 0;
+  while ((1ll << log2) < a.page_size) ++log2;
+  p.page_shift = 31 + log2;
+  p.page_magic = ((1ull << p.page_shift) + a.page_size - 1) / a.page_size;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.arrived = static_cast<unsigned int*>(scratch);
+  p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + kCounterBytes);
+  p.status = status_dev;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a.type == FP6M_TYPE_F16 ? launch_tree<half>(a, st, status_dev) : launch_tree<__nv_bfloat16>(a, st, status_dev);
+  const cudaError_t e = a.type == FP6M_TYPE_F16 ? launch_tree<half>(p, row_tile, tree_ctas(sms), st) : launch_tree<__nv_bfloat16>(p, row_tile, tree_ctas(sms), st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "tree_attention launch");
 }
 
