@@ -4,13 +4,16 @@
 // The reference has no counterpart: its weights have four or six bits.
 //
 // The product is computed transposed, as in the GEMMs of this library: 128 rows of B - one strip, and one scale per block of K -
-// are the M dimension of tcgen05.mma.kind::f8f6f4 (a TMEM lane per column of C), up to 256 rows of A its N dimension.  The scales
+// are the M dimension of tcgen05.mma.kind::f8f6f4 (a TMEM lane per column of C), up to 128 rows of A its N dimension.  The scales
 // change with every block of 128 values of K, so a block is one accumulator tile of its own (four MMAs, the first one overwrites):
 // warps read it back, multiply it by sa * sb and add it to their sums in registers while the tensor cores work on the next blocks.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
+#include <utility>
 
 #include "../../include/fp6m.h"
 #include "device_utils.cuh"
@@ -31,6 +34,7 @@ struct Fp8Params {
   const float *sa, *sb;
   int M, N, kb;                          // kb: blocks of K
   int strips, row_tiles, tile_rows;      // tile_rows: rows of A per tile, a multiple of 16
+  int group_rows;                        // of them, those of a group of four warps; the last group may have fewer
   int weights_early;                     // the kernel in front does not write B: its first blocks are read before that has finished
   unsigned int* epochs;
   unsigned long long* partials;          // [CTA][tile_rows][128] words {value, tag}
@@ -44,13 +48,14 @@ struct Fp8Cfg {
   static constexpr int kMine = kRows / (kWarps / 4);         // rows of a thread
   static constexpr int kStageBytes = kStripBytes + kRows * kBlock;
   static constexpr int kStages = 200 * 1024 / kStageBytes < 11 ? 200 * 1024 / kStageBytes : 11;
-  static constexpr int kTiles = kRows <= 128 ? 4 : 2;        // accumulator tiles in tensor memory
+  static constexpr int kTiles = 4;       // accumulator tiles in tensor memory
   static constexpr int kTmemCols = kTiles * kRows < 32 ? 32 : kTiles * kRows;
   static constexpr int kScales = 8;                          // blocks whose scales wait in shared memory
   static constexpr int kNumBars = 2 * kStages + 2 * kTiles + 2 * kScales + 1;
   static constexpr int kThreads = 32 * (4 + kWarps);
-  static constexpr int kSmemBytes = kStages * kStageBytes + kScales * kRows * 4 + kNumBars * 8 + 16 + 1024;
-  static constexpr int kChunk = kMine < 32 ? kMine : 32;     // values per read-back
+  static constexpr int kOutRow = 32 * 2 + 16;                // bytes of a row of 32 finished values in shared memory, with a gap
+  static constexpr int kSmemBytes = kStages * kStageBytes + kScales * kRows * 4 + kWarps * 16 * kOutRow + kNumBars * 8 + 16 + 1024;
+  static constexpr int kChunk = kMine < 32 ? 16 : 32;     // values per read-back
 };
 
 // x (bytes of K) is a multiple of 128: the copy starts on a 16-byte boundary
@@ -73,30 +78,54 @@ __device__ __forceinline__ void mma_block(uint32_t d_tmem, uint64_t a_desc, uint
         "}\n"
         ::"r"(d_tmem), "l"(a_desc + 2 * i), "l"(b_desc + 2 * i), "r"(idesc), "r"(i) : "memory");
 }
+// kCount (16 or 32) columns of this warp's lanes; the values are there after tc_wait_ld
 template <int kCount>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&v)[kCount]) {
-  static_assert(kCount == 16 || kCount == 32, "columns per load");
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
   if constexpr (kCount == 16) {
-    tc_ld16(taddr, v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
   } else {
-    uint32_t r[32];
+    static_assert(kCount == 32, "columns per load");
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
         "%28,%29,%30,%31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
           "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
           "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr) : "memory");
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        : "r"(taddr));
   }
+}
+// Waits for tcgen05.ld; the registers pass through, so that nothing that uses them can be moved in front of the wait.
+template <int kCount>
+__device__ __forceinline__ void tmem_loaded(uint32_t* r) {
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ float4 lds_float4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+// Partials of one column lie kBlock words apart: their places are constants in the instructions, not registers (with an address
+// register for each of 64 values the sums were spilled).
+template <int kRow>
+__device__ __forceinline__ unsigned long long ld_partial(const unsigned long long* slot) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1 + %2];" : "=l"(v) : "l"(slot), "n"(kRow * kBlock * 8) : "memory");
+  return v;
+}
+template <int kRow>
+__device__ __forceinline__ void st_partial(unsigned long long* slot, unsigned long long v) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0 + %1], %2;" ::"l"(slot), "n"(kRow * kBlock * 8), "l"(v) : "memory");
+}
+template <int kFirst, class F, int... kI>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, kI...>) { (f(std::integral_constant<int, kFirst + kI>()), ...); }
+// f(kFirst) ... f(kFirst + kCount - 1), the argument a constant
+template <int kFirst, int kCount, class F>
+__device__ __forceinline__ void each(F&& f) { each_of<kFirst>(f, std::make_integer_sequence<int, kCount>()); }
 __device__ __forceinline__ void store_value(half* c, float v) { *c = __float2half_rn(v); }
 __device__ __forceinline__ void store_value(__nv_bfloat16* c, float v) { *c = __float2bfloat16_rn(v); }
 
@@ -112,7 +141,8 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* scales = reinterpret_cast<float*>(smem + S * C::kStageBytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(scales + R * C::kRows);
+  uint8_t* out_stage = reinterpret_cast<uint8_t*>(scales + R * C::kRows);           // [warp][16 rows][kOutRow]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_stage + C::kWarps * 16 * C::kOutRow);
   volatile uint32_t* misc = reinterpret_cast<uint32_t*>(bars + C::kNumBars);        // [0] TMEM base, [1] launch epoch
   const uint32_t full = smem_u32(bars), empty = full + 8 * S, done = empty + 8 * S, taken = done + 8 * D;
   const uint32_t scaled = taken + 8 * D, used = scaled + 8 * R, epoch_bar = used + 8 * R;
@@ -150,30 +180,51 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, misc[0], 0);
   bool dead = false;
+  // The launch gives 168 registers a thread (384 threads); the eight warps that hold sums take 216, the first four keep 72:
+  // 256 * 216 + 128 * 72 = 384 * 168.
+  auto fewer_registers = [] { if constexpr (C::kMine >= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); };
+  auto more_registers = [] { if constexpr (C::kMine >= 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); };
 
   if (warp == 0) {
     // ================================================================== producer of weights and activations
+    fewer_registers();
     const uint32_t bytes = kStripBytes + nt * kBlock;
     const int first = B1 - B0 < S ? B1 - B0 : S;                     // blocks whose stages are free from the start
-    auto load_weights = [&](int n, int u) {
+    // (places are counted on: divisions by run-time values would take longer than a block)
+    struct Place {
+      int x, tile, strip;                                            // byte of K, row tile, strip
+    };
+    const Place start = {B0 % p.kb * kBlock, B0 / p.kb % p.row_tiles, B0 / p.kb / p.row_tiles};
+    auto next = [&](Place& at) {
+      at.x += kBlock;
+      if (at.x < p.kb * kBlock) return;
+      at.x = 0;
+      if (++at.tile == p.row_tiles) { at.tile = 0; ++at.strip; }
+    };
+    auto load_weights = [&](int n, const Place& at) {
       mbar_arrive_expect_tx(full + 8 * n, bytes);
-      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes, &bmap, u % p.kb * kBlock, u / p.kb / p.row_tiles * kBlock, full + 8 * n);
+      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes, &bmap, at.x, at.strip * kBlock, full + 8 * n);
     };
-    auto load_rows = [&](int n, int u) {
-      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes + kStripBytes, &amap, u % p.kb * kBlock, u / p.kb % p.row_tiles * nt, full + 8 * n);
+    auto load_rows = [&](int n, const Place& at) {
+      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes + kStripBytes, &amap, at.x, at.tile * nt, full + 8 * n);
     };
-    if (elect_one()) {
-      for (int n = 0; n < first; ++n)
-        if (p.weights_early) load_weights(n, B0 + n);
-        else tma_prefetch_bytes(&bmap, (B0 + n) % p.kb * kBlock, (B0 + n) / p.kb / p.row_tiles * kBlock);
+    Place at = start;
+    for (int n = 0; n < first; ++n) {
+      if (elect_one()) {
+        if (p.weights_early) load_weights(n, at);
+        else tma_prefetch_bytes(&bmap, at.x, at.strip * kBlock);
+      }
+      next(at);
     }
     __syncwarp();
     grid_dependency_wait();
-    if (elect_one()) {
-      for (int n = 0; n < first; ++n) {
-        if (!p.weights_early) load_weights(n, B0 + n);
-        load_rows(n, B0 + n);
+    at = start;
+    for (int n = 0; n < first; ++n) {
+      if (elect_one()) {
+        if (!p.weights_early) load_weights(n, at);
+        load_rows(n, at);
       }
+      next(at);
     }
     __syncwarp();
     int stage = 0;
@@ -181,14 +232,16 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     for (int u = B0 + first; u < B1; ++u) {
       mbar_wait_bounded<100>(empty + 8 * stage, phase, p.status, dead);
       if (elect_one()) {
-        load_weights(stage, u);
-        load_rows(stage, u);
+        load_weights(stage, at);
+        load_rows(stage, at);
       }
       __syncwarp();
+      next(at);
       if (++stage == S) { stage = 0; phase ^= 1; }
     }
   } else if (warp == 1) {
     // ================================================================== MMA issuer
+    fewer_registers();
     grid_dependency_wait();                  // the bounded waits start when the kernel in front has finished
     const uint64_t desc0 = wide_act_desc(smem_u32(smem));
     // D fp32, A and B E4M3, K-major; N = rows of the tile, M = 128
@@ -212,33 +265,48 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     }
   } else if (warp == 2) {
     // ================================================================== scales: sa * sb of the block for every row of the tile
+    fewer_registers();
     grid_dependency_wait();
-    constexpr int E = (C::kRows + 31) / 32;
-    float now[E];
-    auto load = [&](int u) {
-      const int b = u % p.kb, v = u / p.kb, row0 = v % p.row_tiles * nt;
-      const float column = p.sb[(size_t)(v / p.row_tiles) * p.kb + b];
+    // The scales of kAhead blocks are on their way together: with one block at a time the loads' latency was longer than a block takes.
+    constexpr int E = (C::kRows + 31) / 32, kAhead = 4;
+    float now[kAhead][E], column[kAhead];
+    int b = B0 % p.kb, tile = B0 / p.kb % p.row_tiles, strip = B0 / p.kb / p.row_tiles, left = B1 - B0;      // of the block to load
+    auto load = [&](int j) {
+      const bool live = left > 0;
+      const int row0 = tile * nt;
+      column[j] = live ? p.sb[(size_t)strip * p.kb + b] : 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int m = lane + 32 * i;
-        now[i] = m < nt && row0 + m < p.M ? p.sa[(size_t)(row0 + m) * p.kb + b] * column : 0.f;
+        now[j][i] = live && m < nt && row0 + m < p.M ? p.sa[(size_t)(row0 + m) * p.kb + b] : 0.f;
+      }
+      --left;
+      if (++b == p.kb) {
+        b = 0;
+        if (++tile == p.row_tiles) { tile = 0; ++strip; }
       }
     };
-    if (B0 < B1) load(B0);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) load(j);
     int r = 0;
     uint32_t phase = 0;
-    for (int u = B0; u < B1; ++u) {
-      mbar_wait_bounded<100>(used + 8 * r, phase ^ 1, p.status, dead);
+    for (int u0 = B0; u0 < B1; u0 += kAhead) {
 #pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (C::kRows % 32 == 0 || lane + 32 * i < C::kRows) sts_f32(smem_u32(scales + r * C::kRows + lane + 32 * i), now[i]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(scaled + 8 * r);
-      if (u + 1 < B1) load(u + 1);
-      if (++r == R) { r = 0; phase ^= 1; }
+      for (int j = 0; j < kAhead; ++j) {
+        if (u0 + j >= B1) break;
+        mbar_wait_bounded<100>(used + 8 * r, phase ^ 1, p.status, dead);
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (C::kRows % 32 == 0 || lane + 32 * i < C::kRows) sts_f32(smem_u32(scales + r * C::kRows + lane + 32 * i), now[j][i] * column[j]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scaled + 8 * r);
+        load(j);
+        if (++r == R) { r = 0; phase ^= 1; }
+      }
     }
   } else if (warp == 3) {
     // ================================================================== launch epoch: the tag of this launch's partials is epoch + 1
+    fewer_registers();
     if (lane == 0) {
       grid_dependency_wait();
       misc[1] = read_epoch_and_count(p.epochs, gridDim.x);
@@ -247,100 +315,116 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     __syncwarp();
   } else {
     // ================================================================== sums: thread = column of the strip, kMine rows
+    more_registers();
     constexpr int CH = C::kChunk, E = C::kMine;
-    const int quarter = warp & 3, row_base = (warp - 4) / 4 * E;
+    const int quarter = warp & 3, row_base = (warp - 4) / 4 * p.group_rows;
     const int c = quarter * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + row_base;
+    const int my_rows = min(p.group_rows, nt - row_base);
     grid_dependency_wait();
     float sum[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) sum[i] = 0.f;
-    int tile = 0, r = 0, slice_start = B0;
+    int tile = 0, r = 0, slice_start = B0, block = B0 % p.kb;
     uint32_t tphase = 0, rphase = 0;
     for (int u = B0; u < B1; ++u) {
       mbar_wait_bounded<20>(scaled + 8 * r, rphase, p.status, dead);
       mbar_wait_bounded<20>(done + 8 * tile, tphase, p.status, dead);
       tc_fence_after();
+      // all read-backs are on their way before the scales are loaded, and the tile is given back before the sums
+      uint32_t v[E];
 #pragma unroll
-      for (int c0 = 0; c0 < E; c0 += CH) {
-        if (row_base + c0 < nt) {            // the same for all threads of the warp
-          float v[CH];
-          tmem_load<CH>(lane_base + tile * C::kRows + c0, v);
-          const uint32_t from = smem_u32(scales + r * C::kRows + row_base + c0);
+      for (int c0 = 0; c0 < E; c0 += CH)
+        if (c0 < my_rows) tmem_load<CH>(lane_base + tile * C::kRows + c0, v + c0);       // the same for all threads of the warp
+      const uint32_t from = smem_u32(scales + r * C::kRows + row_base);
+      float4 scale[E / 4];
 #pragma unroll
-          for (int i = 0; i < CH; i += 4) {
-            const float4 s = lds_float4(from + 4 * i);
-            sum[c0 + i] = fmaf(v[i], s.x, sum[c0 + i]);
-            sum[c0 + i + 1] = fmaf(v[i + 1], s.y, sum[c0 + i + 1]);
-            sum[c0 + i + 2] = fmaf(v[i + 2], s.z, sum[c0 + i + 2]);
-            sum[c0 + i + 3] = fmaf(v[i + 3], s.w, sum[c0 + i + 3]);
-          }
-        }
-      }
+      for (int i = 0; i < E / 4; ++i) scale[i] = lds_float4(from + 16 * i);
+      tmem_loaded<E>(v);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(taken + 8 * tile);
         mbar_arrive(used + 8 * r);
       }
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        sum[4 * i] = fmaf(__uint_as_float(v[4 * i]), scale[i].x, sum[4 * i]);
+        sum[4 * i + 1] = fmaf(__uint_as_float(v[4 * i + 1]), scale[i].y, sum[4 * i + 1]);
+        sum[4 * i + 2] = fmaf(__uint_as_float(v[4 * i + 2]), scale[i].z, sum[4 * i + 2]);
+        sum[4 * i + 3] = fmaf(__uint_as_float(v[4 * i + 3]), scale[i].w, sum[4 * i + 3]);
+      }
       if (++tile == D) { tile = 0; tphase ^= 1; }
       if (++r == R) { r = 0; rphase ^= 1; }
 
-      const bool strip_ends = (u + 1) % p.kb == 0;
+      const bool strip_ends = ++block == p.kb;
+      if (strip_ends) block = 0;
       if (!strip_ends && u + 1 < B1) continue;
       // ---- the end of a slice: this CTA's blocks of one strip and row tile
-      const int v = u / p.kb, row0 = v % p.row_tiles * nt + row_base;
-      const int column = v / p.row_tiles * kBlock + c;
+      const int slice = u / p.kb, row0 = slice % p.row_tiles * nt + row_base;
+      const int column = slice / p.row_tiles * kBlock + c;
       const bool starts = slice_start % p.kb == 0;
-      const int rows = min(min(nt - row_base, E), p.M - row0);           // rows of this thread that exist
+      const int rows = min(my_rows, p.M - row0);           // rows of this thread that exist
       uint32_t tag = 0;
       if (!starts || !strip_ends) {
         mbar_wait_bounded<20>(epoch_bar, 0, p.status, dead);
         tag = misc[1] + 1;
       }
+      // Threads of many rows exchange whole sixteens (a slot has room for them): a condition for every row costs registers that they
+      // do not have.
+      auto first_of_check = [](int i) constexpr { return E <= 32 ? i : i / 16 * 16; };
       auto slot_of = [&](int other) { return p.partials + ((size_t)other * nt + row_base) * kBlock + c; };
       if (!starts) {
         // Only the first slice of a CTA can start inside a strip, so a CTA has one partial.
         unsigned long long* slot = slot_of(cta);
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (i < rows) st_relaxed_u64(slot + (size_t)i * kBlock, ((unsigned long long)tag << 32) | __float_as_uint(sum[i]));
+        each<0, E>([&](auto i) {
+          if (first_of_check(i) < rows) st_partial<i>(slot, ((unsigned long long)tag << 32) | __float_as_uint(sum[i]));
+        });
       } else {
         // The CTA in which a strip starts adds the partials of the CTAs behind it, in their order.
         if (!strip_ends) {
-          const int end = (v + 1) * p.kb;
+          const int end = (slice + 1) * p.kb;
 #pragma unroll 1
           for (int other = cta + 1; other < (int)gridDim.x && range_start(p, other) < end; ++other) {
             const unsigned long long* slot = slot_of(other);
-#pragma unroll
-            for (int i0 = 0; i0 < E; i0 += 16) {
+            each<0, E / 16>([&](auto part) {
+              constexpr int i0 = 16 * part;
+              if (i0 >= rows) return;
               unsigned long long w[16];
-              bool here = i0 >= rows;
+              bool here = false;
 #pragma unroll 1
               for (int spin = 0; spin < (1 << 20) && !here; ++spin) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = i0 + i < rows ? ld_relaxed_u64(slot + (size_t)(i0 + i) * kBlock) : 0;
+                each<0, 16>([&](auto i) { w[i] = first_of_check(i0 + i) < rows ? ld_partial<i0 + i>(slot) : (unsigned long long)tag << 32; });
                 here = true;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) here = here && (i0 + i >= rows || (uint32_t)(w[i] >> 32) == tag);
+                for (int i = 0; i < 16; ++i) here = here && (uint32_t)(w[i] >> 32) == tag;
                 if (dead) break;             // a wait of this thread ran out before: do not wait again
               }
               if (!here && !dead) {
                 dead = true;
                 if (p.status) atomicExch(p.status, kStatusTimeout);
               }
-              if (i0 < rows) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum[i0 + i] += i0 + i < rows ? __uint_as_float((uint32_t)w[i]) : 0.f;
-              }
-            }
+              for (int i = 0; i < 16; ++i) sum[i0 + i] += __uint_as_float((uint32_t)w[i]);
+            });
           }
         }
-        if (column < p.N) {
-          T* out = static_cast<T*>(p.C) + (size_t)row0 * p.N + column;
+        // A warp turns 16 rows x 32 columns at a time round in shared memory and stores sixteen bytes a lane.
+        uint8_t* mine = out_stage + (warp - 4) * 16 * C::kOutRow;
+        const int out_column = column - lane + (lane & 3) * 8;
 #pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (i < rows) store_value(out + (size_t)i * p.N, sum[i]);
+        for (int i0 = 0; i0 < E; i0 += 16) {
+          if (i0 >= rows) break;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) store_value(reinterpret_cast<T*>(mine + i * C::kOutRow) + lane, sum[i0 + i]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+            const int r = i + (lane >> 2);
+            if (i0 + r < rows && out_column < p.N)
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (size_t)(row0 + i0 + r) * p.N + out_column) = *reinterpret_cast<const uint4*>(mine + r * C::kOutRow + (lane & 3) * 16);
+          }
+          __syncwarp();
         }
       }
 #pragma unroll
@@ -361,7 +445,7 @@ struct Fp8Plan {
 };
 Fp8Plan plan_fp8(int M, int N, int K, int sms) {
   Fp8Plan plan;
-  plan.row_tiles = (M + 255) / 256;
+  plan.row_tiles = (M + 127) / 128;
   plan.tile_rows = ((M + plan.row_tiles - 1) / plan.row_tiles + 15) / 16 * 16;
   const long long blocks = (long long)((N + kBlock - 1) / kBlock) * plan.row_tiles * ((K + kBlock - 1) / kBlock);
   long long ctas = sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas;
@@ -384,8 +468,7 @@ cudaError_t launch_fp8_rows(const Fp8Params& p, int ctas, const CUtensorMap& ama
   if (p.tile_rows <= 16) return launch_fp8<T, Fp8Cfg<16, 4>>(p, ctas, amap, bmap, stream);
   if (p.tile_rows <= 32) return launch_fp8<T, Fp8Cfg<32, 4>>(p, ctas, amap, bmap, stream);
   if (p.tile_rows <= 64) return launch_fp8<T, Fp8Cfg<64, 8>>(p, ctas, amap, bmap, stream);
-  if (p.tile_rows <= 128) return launch_fp8<T, Fp8Cfg<128, 8>>(p, ctas, amap, bmap, stream);
-  return launch_fp8<T, Fp8Cfg<256, 8>>(p, ctas, amap, bmap, stream);
+  return launch_fp8<T, Fp8Cfg<128, 8>>(p, ctas, amap, bmap, stream);
 }
 
 }  // namespace
@@ -415,7 +498,7 @@ int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const vo
   if (!A || !B || !sa || !sb || !scratch || !aligned16(A) || !aligned16(B) || !aligned16(scratch) ||
       ((reinterpret_cast<uintptr_t>(sa) | reinterpret_cast<uintptr_t>(sb)) & 3))
     return FP6M_ERR_BAD_ARG;
-  if ((long long)((N + kBlock - 1) / kBlock) * ((M + 255) / 256) * ((K + kBlock - 1) / kBlock) > 0x3fffffff) return FP6M_ERR_PROB_SHAPE;
+  if ((long long)((N + kBlock - 1) / kBlock) * ((M + 127) / 128) * ((K + kBlock - 1) / kBlock) > 0x3fffffff) return FP6M_ERR_PROB_SHAPE;
   DeviceGuard guard(dev);
   const int sms = sm_count(dev);
   if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
@@ -431,6 +514,8 @@ int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const vo
   p.strips = (N + kBlock - 1) / kBlock;
   p.row_tiles = plan.row_tiles;
   p.tile_rows = plan.tile_rows;
+  const int groups = plan.tile_rows <= 32 ? 1 : 2;       // of four warps, see launch_fp8_rows
+  p.group_rows = (plan.tile_rows / groups + 15) / 16 * 16;
   p.weights_early = tc5_get_overlap() ? 1 : 0;
   p.epochs = static_cast<unsigned int*>(scratch);
   p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(scratch) + kEpochWords * sizeof(unsigned int));
