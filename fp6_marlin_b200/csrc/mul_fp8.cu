@@ -4,36 +4,24 @@
 // The reference has no counterpart: its weights have four or six bits.
 //
 // The product is computed transposed, as in the GEMMs of this library: 128 rows of B - one strip, and one scale per block of K -
-// are the M dimension of tcgen05.mma.kind::f8f6f4 (a TMEM lane per column of C), up to 128 rows of A its N dimension.  The scales
+// are the M dimension of tcgen05.mma.kind::f8f6f4 (a TMEM lane per column of C), up to 64 rows of A its N dimension (more: mul_fp8_rows.cu).  The scales
 // change with every block of 128 values of K, so a block is one accumulator tile of its own (four MMAs, the first one overwrites):
 // warps read it back, multiply it by sa * sb and add it to their sums in registers while the tensor cores work on the next blocks.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include <type_traits>
-#include <utility>
-
 #include "../../include/fp6m.h"
-#include "device_utils.cuh"
-#include "gemm_params.h"
 #include "host_common.h"
-#include "tc5_common.cuh"
+#include "mul_fp8.cuh"
 
 namespace fp6m {
 
 namespace {
 
-constexpr int kBlock = 128;              // values of K, and columns of C, that share a scale
-constexpr int kStripBytes = kBlock * kBlock;
 constexpr int kMaxFp8Ctas = 192;         // one CTA per multiprocessor
 
 struct Fp8Params {
   void* C;
   const float *sa, *sb;
   int M, N, kb;                          // kb: blocks of K
-  int strips, row_tiles, tile_rows;      // tile_rows: rows of A per tile, a multiple of 16
+  int strips, tile_rows;                 // tile_rows: rows of A, rounded up to a multiple of 16
   int group_rows;                        // of them, those of a group of four warps; the last group may have fewer
   int weights_early;                     // the kernel in front does not write B: its first blocks are read before that has finished
   unsigned int* epochs;
@@ -58,14 +46,6 @@ struct Fp8Cfg {
   static constexpr int kChunk = kMine < 32 ? 16 : 32;     // values per read-back
 };
 
-// x (bytes of K) is a multiple of 128: the copy starts on a 16-byte boundary
-__device__ __forceinline__ void tma_load_bytes(uint32_t dst, const CUtensorMap* map, int x, int row, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void tma_prefetch_bytes(const CUtensorMap* map, int x, int row) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(row) : "memory");
-}
 // D[128 x N] = A[128 x 128] B[N x 128]^T of E4M3 values, both in 128-byte rows with the 128-byte swizzle: four MMAs of 32 values of K
 __device__ __forceinline__ void mma_block(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
 #pragma unroll
@@ -78,60 +58,9 @@ __device__ __forceinline__ void mma_block(uint32_t d_tmem, uint64_t a_desc, uint
         "}\n"
         ::"r"(d_tmem), "l"(a_desc + 2 * i), "l"(b_desc + 2 * i), "r"(idesc), "r"(i) : "memory");
 }
-// kCount (16 or 32) columns of this warp's lanes; the values are there after tc_wait_ld
-template <int kCount>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
-  if constexpr (kCount == 16) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
-  } else {
-    static_assert(kCount == 32, "columns per load");
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-        "%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-  }
-}
-// Waits for tcgen05.ld; the registers pass through, so that nothing that uses them can be moved in front of the wait.
-template <int kCount>
-__device__ __forceinline__ void tmem_loaded(uint32_t* r) {
-  tc_wait_ld();
-#pragma unroll
-  for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(r[i]));
-}
-__device__ __forceinline__ float4 lds_float4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-// Partials of one column lie kBlock words apart: their places are constants in the instructions, not registers (with an address
-// register for each of 64 values the sums were spilled).
-template <int kRow>
-__device__ __forceinline__ unsigned long long ld_partial(const unsigned long long* slot) {
-  unsigned long long v;
-  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1 + %2];" : "=l"(v) : "l"(slot), "n"(kRow * kBlock * 8) : "memory");
-  return v;
-}
-template <int kRow>
-__device__ __forceinline__ void st_partial(unsigned long long* slot, unsigned long long v) {
-  asm volatile("st.relaxed.gpu.global.u64 [%0 + %1], %2;" ::"l"(slot), "n"(kRow * kBlock * 8), "l"(v) : "memory");
-}
-template <int kFirst, class F, int... kI>
-__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, kI...>) { (f(std::integral_constant<int, kFirst + kI>()), ...); }
-// f(kFirst) ... f(kFirst + kCount - 1), the argument a constant
-template <int kFirst, int kCount, class F>
-__device__ __forceinline__ void each(F&& f) { each_of<kFirst>(f, std::make_integer_sequence<int, kCount>()); }
-__device__ __forceinline__ void store_value(half* c, float v) { *c = __float2half_rn(v); }
-__device__ __forceinline__ void store_value(__nv_bfloat16* c, float v) { *c = __float2bfloat16_rn(v); }
-
-// The blocks of all (strip, row tile) pairs, K fastest, then row tiles, are cut into as many equal ranges as there are CTAs.
+// The blocks of all strips, K fastest, are cut into as many equal ranges as there are CTAs.
 __device__ __forceinline__ int range_start(const Fp8Params& p, int cta) {
-  return (int)((long long)p.strips * p.row_tiles * p.kb * cta / (int)gridDim.x);
+  return (int)((long long)p.strips * p.kb * cta / (int)gridDim.x);
 }
 
 template <class T, class C>
@@ -180,39 +109,34 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, misc[0], 0);
   bool dead = false;
-  // The launch gives 168 registers a thread (384 threads); the eight warps that hold sums take 216, the first four keep 72:
-  // 256 * 216 + 128 * 72 = 384 * 168.
-  auto fewer_registers = [] { if constexpr (C::kMine >= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); };
-  auto more_registers = [] { if constexpr (C::kMine >= 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); };
 
   if (warp == 0) {
     // ================================================================== producer of weights and activations
-    fewer_registers();
     const uint32_t bytes = kStripBytes + nt * kBlock;
     const int first = B1 - B0 < S ? B1 - B0 : S;                     // blocks whose stages are free from the start
     // (places are counted on: divisions by run-time values would take longer than a block)
     struct Place {
-      int x, tile, strip;                                            // byte of K, row tile, strip
+      int x, row;                                                    // byte of K, row of B
     };
-    const Place start = {B0 % p.kb * kBlock, B0 / p.kb % p.row_tiles, B0 / p.kb / p.row_tiles};
+    const Place start = {B0 % p.kb * kBlock, B0 / p.kb * kBlock};
     auto next = [&](Place& at) {
       at.x += kBlock;
       if (at.x < p.kb * kBlock) return;
       at.x = 0;
-      if (++at.tile == p.row_tiles) { at.tile = 0; ++at.strip; }
+      at.row += kBlock;
     };
     auto load_weights = [&](int n, const Place& at) {
       mbar_arrive_expect_tx(full + 8 * n, bytes);
-      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes, &bmap, at.x, at.strip * kBlock, full + 8 * n);
+      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes, &bmap, at.x, at.row, full + 8 * n);
     };
     auto load_rows = [&](int n, const Place& at) {
-      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes + kStripBytes, &amap, at.x, at.tile * nt, full + 8 * n);
+      tma_load_bytes(smem_u32(smem) + n * C::kStageBytes + kStripBytes, &amap, at.x, 0, full + 8 * n);
     };
     Place at = start;
     for (int n = 0; n < first; ++n) {
       if (elect_one()) {
         if (p.weights_early) load_weights(n, at);
-        else tma_prefetch_bytes(&bmap, at.x, at.strip * kBlock);
+        else tma_prefetch_bytes(&bmap, at.x, at.row);
       }
       next(at);
     }
@@ -241,7 +165,6 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     }
   } else if (warp == 1) {
     // ================================================================== MMA issuer
-    fewer_registers();
     grid_dependency_wait();                  // the bounded waits start when the kernel in front has finished
     const uint64_t desc0 = wide_act_desc(smem_u32(smem));
     // D fp32, A and B E4M3, K-major; N = rows of the tile, M = 128
@@ -265,25 +188,23 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     }
   } else if (warp == 2) {
     // ================================================================== scales: sa * sb of the block for every row of the tile
-    fewer_registers();
     grid_dependency_wait();
     // The scales of kAhead blocks are on their way together: with one block at a time the loads' latency was longer than a block takes.
     constexpr int E = (C::kRows + 31) / 32, kAhead = 4;
     float now[kAhead][E], column[kAhead];
-    int b = B0 % p.kb, tile = B0 / p.kb % p.row_tiles, strip = B0 / p.kb / p.row_tiles, left = B1 - B0;      // of the block to load
+    int b = B0 % p.kb, strip = B0 / p.kb, left = B1 - B0;      // of the block to load
     auto load = [&](int j) {
       const bool live = left > 0;
-      const int row0 = tile * nt;
       column[j] = live ? p.sb[(size_t)strip * p.kb + b] : 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int m = lane + 32 * i;
-        now[j][i] = live && m < nt && row0 + m < p.M ? p.sa[(size_t)(row0 + m) * p.kb + b] : 0.f;
+        now[j][i] = live && m < p.M ? p.sa[(size_t)m * p.kb + b] : 0.f;
       }
       --left;
       if (++b == p.kb) {
         b = 0;
-        if (++tile == p.row_tiles) { tile = 0; ++strip; }
+        ++strip;
       }
     };
 #pragma unroll
@@ -306,7 +227,6 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     }
   } else if (warp == 3) {
     // ================================================================== launch epoch: the tag of this launch's partials is epoch + 1
-    fewer_registers();
     if (lane == 0) {
       grid_dependency_wait();
       misc[1] = read_epoch_and_count(p.epochs, gridDim.x);
@@ -315,7 +235,6 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
     __syncwarp();
   } else {
     // ================================================================== sums: thread = column of the strip, kMine rows
-    more_registers();
     constexpr int CH = C::kChunk, E = C::kMine;
     const int quarter = warp & 3, row_base = (warp - 4) / 4 * p.group_rows;
     const int c = quarter * 32 + lane;
@@ -360,30 +279,26 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
       const bool strip_ends = ++block == p.kb;
       if (strip_ends) block = 0;
       if (!strip_ends && u + 1 < B1) continue;
-      // ---- the end of a slice: this CTA's blocks of one strip and row tile
-      const int slice = u / p.kb, row0 = slice % p.row_tiles * nt + row_base;
-      const int column = slice / p.row_tiles * kBlock + c;
+      // ---- the end of a slice: this CTA's blocks of one strip
+      const int strip = u / p.kb, column = strip * kBlock + c;
       const bool starts = slice_start % p.kb == 0;
-      const int rows = min(my_rows, p.M - row0);           // rows of this thread that exist
+      const int rows = min(my_rows, p.M - row_base);           // rows of this thread that exist
       uint32_t tag = 0;
       if (!starts || !strip_ends) {
         mbar_wait_bounded<20>(epoch_bar, 0, p.status, dead);
         tag = misc[1] + 1;
       }
-      // Threads of many rows exchange whole sixteens (a slot has room for them): a condition for every row costs registers that they
-      // do not have.
-      auto first_of_check = [](int i) constexpr { return E <= 32 ? i : i / 16 * 16; };
       auto slot_of = [&](int other) { return p.partials + ((size_t)other * nt + row_base) * kBlock + c; };
       if (!starts) {
         // Only the first slice of a CTA can start inside a strip, so a CTA has one partial.
         unsigned long long* slot = slot_of(cta);
         each<0, E>([&](auto i) {
-          if (first_of_check(i) < rows) st_partial<i>(slot, ((unsigned long long)tag << 32) | __float_as_uint(sum[i]));
+          if (i < rows) st_partial<i * kBlock>(slot, ((unsigned long long)tag << 32) | __float_as_uint(sum[i]));
         });
       } else {
         // The CTA in which a strip starts adds the partials of the CTAs behind it, in their order.
         if (!strip_ends) {
-          const int end = (slice + 1) * p.kb;
+          const int end = (strip + 1) * p.kb;
 #pragma unroll 1
           for (int other = cta + 1; other < (int)gridDim.x && range_start(p, other) < end; ++other) {
             const unsigned long long* slot = slot_of(other);
@@ -394,7 +309,7 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
               bool here = false;
 #pragma unroll 1
               for (int spin = 0; spin < (1 << 20) && !here; ++spin) {
-                each<0, 16>([&](auto i) { w[i] = first_of_check(i0 + i) < rows ? ld_partial<i0 + i>(slot) : (unsigned long long)tag << 32; });
+                each<0, 16>([&](auto i) { w[i] = i0 + i < rows ? ld_partial<(i0 + i) * kBlock>(slot) : (unsigned long long)tag << 32; });
                 here = true;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) here = here && (uint32_t)(w[i] >> 32) == tag;
@@ -422,7 +337,7 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
           for (int i = 0; i < 16; i += 8) {
             const int r = i + (lane >> 2);
             if (i0 + r < rows && out_column < p.N)
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (size_t)(row0 + i0 + r) * p.N + out_column) = *reinterpret_cast<const uint4*>(mine + r * C::kOutRow + (lane & 3) * 16);
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (size_t)(row_base + i0 + r) * p.N + out_column) = *reinterpret_cast<const uint4*>(mine + r * C::kOutRow + (lane & 3) * 16);
           }
           __syncwarp();
         }
@@ -440,35 +355,53 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
   if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
 }
 
-struct Fp8Plan {
-  int row_tiles, tile_rows, ctas;
-};
-Fp8Plan plan_fp8(int M, int N, int K, int sms) {
-  Fp8Plan plan;
-  plan.row_tiles = (M + 127) / 128;
-  plan.tile_rows = ((M + plan.row_tiles - 1) / plan.row_tiles + 15) / 16 * 16;
-  const long long blocks = (long long)((N + kBlock - 1) / kBlock) * plan.row_tiles * ((K + kBlock - 1) / kBlock);
-  long long ctas = sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas;
-  if (ctas > (blocks + 3) / 4) ctas = (blocks + 3) / 4;
-  plan.ctas = (int)ctas;
-  return plan;
+constexpr int kMostRows = 64;            // rows of A of this kernel
+
+int columns_ctas(int N, int K, int sms) {
+  const long long blocks = (long long)((N + kBlock - 1) / kBlock) * ((K + kBlock - 1) / kBlock);
+  const int ctas = sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas;
+  return ctas < (blocks + 3) / 4 ? ctas : (int)((blocks + 3) / 4);
 }
-size_t plan_bytes(const Fp8Plan& plan) {
-  return kEpochWords * sizeof(unsigned int) + (size_t)plan.ctas * plan.tile_rows * kBlock * sizeof(unsigned long long);
+size_t columns_scratch_bytes(int M, int N, int K, int sms) {
+  return kEpochWords * sizeof(unsigned int) + (size_t)columns_ctas(N, K, sms) * ((M + 15) / 16 * 16) * kBlock * sizeof(unsigned long long);
+}
+size_t fp8_scratch_bytes(int M, int N, int K, int sms) {
+  return M <= kMostRows ? columns_scratch_bytes(M, N, K, sms) : fp8_rows_scratch_bytes(M, N, K, sms);
 }
 
 template <class T, class C>
-cudaError_t launch_fp8(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+cudaError_t launch_with(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
   cudaError_t e = cudaFuncSetAttribute(mul_fp8_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(mul_fp8_kernel<T, C>, dim3(ctas), dim3(C::kThreads), C::kSmemBytes, stream, p, amap, bmap);
 }
 template <class T>
-cudaError_t launch_fp8_rows(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
-  if (p.tile_rows <= 16) return launch_fp8<T, Fp8Cfg<16, 4>>(p, ctas, amap, bmap, stream);
-  if (p.tile_rows <= 32) return launch_fp8<T, Fp8Cfg<32, 4>>(p, ctas, amap, bmap, stream);
-  if (p.tile_rows <= 64) return launch_fp8<T, Fp8Cfg<64, 8>>(p, ctas, amap, bmap, stream);
-  return launch_fp8<T, Fp8Cfg<128, 8>>(p, ctas, amap, bmap, stream);
+cudaError_t launch_typed(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
+  if (p.tile_rows <= 16) return launch_with<T, Fp8Cfg<16, 4>>(p, ctas, amap, bmap, stream);
+  if (p.tile_rows <= 32) return launch_with<T, Fp8Cfg<32, 4>>(p, ctas, amap, bmap, stream);
+  return launch_with<T, Fp8Cfg<64, 8>>(p, ctas, amap, bmap, stream);
+}
+cudaError_t launch_fp8_columns(const Fp8Args& a, int sms, cudaStream_t stream) {
+  Fp8Params p;
+  p.C = a.C;
+  p.sa = a.sa;
+  p.sb = a.sb;
+  p.M = a.M;
+  p.N = a.N;
+  p.kb = a.kb;
+  p.strips = (a.N + kBlock - 1) / kBlock;
+  p.tile_rows = (a.M + 15) / 16 * 16;
+  p.group_rows = p.tile_rows <= 32 ? p.tile_rows : 32;
+  p.weights_early = tc5_get_overlap() ? 1 : 0;
+  p.epochs = static_cast<unsigned int*>(a.scratch);
+  p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(a.scratch) + kEpochWords * sizeof(unsigned int));
+  p.status = a.status;
+  CUtensorMap amap, bmap;
+  cudaError_t e = encode_bytes_map(a.A, a.M, a.K, p.tile_rows, &amap);
+  if (e == cudaSuccess) e = encode_bytes_map(a.B, a.N, a.K, kBlock, &bmap);
+  if (e != cudaSuccess) return e;
+  const int ctas = columns_ctas(a.N, a.K, sms);
+  return a.bf16 ? launch_typed<__nv_bfloat16>(p, ctas, amap, bmap, stream) : launch_typed<half>(p, ctas, amap, bmap, stream);
 }
 
 }  // namespace
@@ -479,7 +412,7 @@ extern "C" {
 
 size_t fp6m_mul_fp8_scratch_bytes(int M, int N, int K, int sms) {
   if (M <= 0 || N <= 0 || K <= 0) return 256;
-  return (fp6m::plan_bytes(fp6m::plan_fp8(M, N, K, sms)) + 255) & ~(size_t)255;
+  return (fp6m::fp8_scratch_bytes(M, N, K, sms) + 255) & ~(size_t)255;
 }
 
 int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const void* sb, int M, int N, int K, int type, void* scratch, size_t scratch_bytes,
@@ -502,29 +435,9 @@ int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const vo
   DeviceGuard guard(dev);
   const int sms = sm_count(dev);
   if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
-  const Fp8Plan plan = plan_fp8(M, N, K, sms);
-  if (scratch_bytes < plan_bytes(plan)) return FP6M_ERR_SCRATCH;
-  Fp8Params p;
-  p.C = C;
-  p.sa = static_cast<const float*>(sa);
-  p.sb = static_cast<const float*>(sb);
-  p.M = M;
-  p.N = N;
-  p.kb = (K + kBlock - 1) / kBlock;
-  p.strips = (N + kBlock - 1) / kBlock;
-  p.row_tiles = plan.row_tiles;
-  p.tile_rows = plan.tile_rows;
-  const int groups = plan.tile_rows <= 32 ? 1 : 2;       // of four warps, see launch_fp8_rows
-  p.group_rows = (plan.tile_rows / groups + 15) / 16 * 16;
-  p.weights_early = tc5_get_overlap() ? 1 : 0;
-  p.epochs = static_cast<unsigned int*>(scratch);
-  p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(scratch) + kEpochWords * sizeof(unsigned int));
-  p.status = status_dev;
-  CUtensorMap amap, bmap;
-  cudaError_t e = encode_bytes_map(A, M, K, plan.tile_rows, &amap);
-  if (e == cudaSuccess) e = encode_bytes_map(B, N, K, kBlock, &bmap);
-  if (e != cudaSuccess) return cuda_fail(e, "mul_fp8 tensor maps");
-  e = type == FP6M_TYPE_F16 ? launch_fp8_rows<half>(p, plan.ctas, amap, bmap, st) : launch_fp8_rows<__nv_bfloat16>(p, plan.ctas, amap, bmap, st);
+  if (scratch_bytes < fp8_scratch_bytes(M, N, K, sms)) return FP6M_ERR_SCRATCH;
+  const Fp8Args a = {A, B, C, static_cast<const float*>(sa), static_cast<const float*>(sb), M, N, K, (K + kBlock - 1) / kBlock, type == FP6M_TYPE_BF16, scratch, status_dev};
+  const cudaError_t e = M <= kMostRows ? launch_fp8_columns(a, sms, st) : launch_fp8_rows(a, sms, st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "mul_fp8 launch");
 }
 

@@ -1,0 +1,96 @@
+// Shared by the kernels of the product of E4M3 matrices with scales for blocks of 128 (mul_fp8.cu, mul_fp8_rows.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+#include <utility>
+
+#include "device_utils.cuh"
+#include "gemm_params.h"
+#include "tc5_common.cuh"
+
+namespace fp6m {
+
+constexpr int kBlock = 128;              // values of K, and columns of C, that share a scale
+constexpr int kStripBytes = kBlock * kBlock;
+
+struct Fp8Args {
+  const void *A, *B;
+  void* C;
+  const float *sa, *sb;
+  int M, N, K, kb;                       // kb: blocks of K
+  bool bf16;
+  void* scratch;
+  int* status;
+};
+// mul_fp8_rows.cu
+size_t fp8_rows_scratch_bytes(int M, int N, int K, int sms);
+cudaError_t launch_fp8_rows(const Fp8Args& a, int sms, cudaStream_t stream);
+
+#ifdef __CUDACC__
+// x (bytes of K) is a multiple of 128: the copy starts on a 16-byte boundary
+__device__ __forceinline__ void tma_load_bytes(uint32_t dst, const CUtensorMap* map, int x, int row, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_bytes(const CUtensorMap* map, int x, int row) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(row) : "memory");
+}
+// kCount (16 or 32) columns of this warp's lanes; the values are there after tc_wait_ld
+template <int kCount>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
+  if constexpr (kCount == 16) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+  } else {
+    static_assert(kCount == 32, "columns per load");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+  }
+}
+// Waits for tcgen05.ld; the registers pass through, so that nothing that uses them can be moved in front of the wait.
+template <int kCount>
+__device__ __forceinline__ void tmem_loaded(uint32_t* r) {
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ float4 lds_float4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// Words of a partial at constant distances: their places are constants in the instructions, not registers (with an address register
+// for each of 64 values the sums were spilled).
+template <int kOffset>
+__device__ __forceinline__ unsigned long long ld_partial(const unsigned long long* slot) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1 + %2];" : "=l"(v) : "l"(slot), "n"(kOffset * 8) : "memory");
+  return v;
+}
+template <int kOffset>
+__device__ __forceinline__ void st_partial(unsigned long long* slot, unsigned long long v) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0 + %1], %2;" ::"l"(slot), "n"(kOffset * 8), "l"(v) : "memory");
+}
+template <int kFirst, class F, int... kI>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, kI...>) { (f(std::integral_constant<int, kFirst + kI>()), ...); }
+// f(kFirst) ... f(kFirst + kCount - 1), the argument a constant
+template <int kFirst, int kCount, class F>
+__device__ __forceinline__ void each(F&& f) { each_of<kFirst>(f, std::make_integer_sequence<int, kCount>()); }
+__device__ __forceinline__ void store_value(half* c, float v) { *c = __float2half_rn(v); }
+__device__ __forceinline__ void store_value(__nv_bfloat16* c, float v) { *c = __float2bfloat16_rn(v); }
+#endif  // __CUDACC__
+
+}  // namespace fp6m
