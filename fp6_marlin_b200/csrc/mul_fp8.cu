@@ -15,8 +15,6 @@ namespace fp6m {
 
 namespace {
 
-constexpr int kMaxFp8Ctas = 192;         // one CTA per multiprocessor
-
 struct Fp8Params {
   void* C;
   const float *sa, *sb;
@@ -355,18 +353,16 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
   if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
 }
 
-constexpr int kMostRows = 64;            // rows of A of this kernel
-
 int columns_ctas(int N, int K, int sms) {
   const long long blocks = (long long)((N + kBlock - 1) / kBlock) * ((K + kBlock - 1) / kBlock);
   const int ctas = sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas;
   return ctas < (blocks + 3) / 4 ? ctas : (int)((blocks + 3) / 4);
 }
 size_t columns_scratch_bytes(int M, int N, int K, int sms) {
-  return kEpochWords * sizeof(unsigned int) + (size_t)columns_ctas(N, K, sms) * ((M + 15) / 16 * 16) * kBlock * sizeof(unsigned long long);
+  return kFp8Header + (size_t)columns_ctas(N, K, sms) * ((M + 15) / 16 * 16) * kBlock * sizeof(unsigned long long);
 }
 size_t fp8_scratch_bytes(int M, int N, int K, int sms) {
-  return M <= kMostRows ? columns_scratch_bytes(M, N, K, sms) : fp8_rows_scratch_bytes(M, N, K, sms);
+  return M <= kMostColumnsRows ? columns_scratch_bytes(M, N, K, sms) : fp8_rows_scratch_bytes(M, N, K, sms);
 }
 
 template <class T, class C>
@@ -394,7 +390,7 @@ cudaError_t launch_fp8_columns(const Fp8Args& a, int sms, cudaStream_t stream) {
   p.group_rows = p.tile_rows <= 32 ? p.tile_rows : 32;
   p.weights_early = tc5_get_overlap() ? 1 : 0;
   p.epochs = static_cast<unsigned int*>(a.scratch);
-  p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(a.scratch) + kEpochWords * sizeof(unsigned int));
+  p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(a.scratch) + kFp8Header);
   p.status = a.status;
   CUtensorMap amap, bmap;
   cudaError_t e = encode_bytes_map(a.A, a.M, a.K, p.tile_rows, &amap);
@@ -437,7 +433,7 @@ int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const vo
   if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
   if (scratch_bytes < fp8_scratch_bytes(M, N, K, sms)) return FP6M_ERR_SCRATCH;
   const Fp8Args a = {A, B, C, static_cast<const float*>(sa), static_cast<const float*>(sb), M, N, K, (K + kBlock - 1) / kBlock, type == FP6M_TYPE_BF16, scratch, status_dev};
-  const cudaError_t e = M <= kMostRows ? launch_fp8_columns(a, sms, st) : launch_fp8_rows(a, sms, st);
+  const cudaError_t e = M <= kMostColumnsRows ? launch_fp8_columns(a, sms, st) : launch_fp8_rows(a, sms, st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "mul_fp8 launch");
 }
 

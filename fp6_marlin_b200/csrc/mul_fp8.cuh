@@ -19,6 +19,13 @@ namespace fp6m {
 constexpr int kBlock = 128;              // values of K, and columns of C, that share a scale
 constexpr int kStripBytes = kBlock * kBlock;
 
+constexpr int kMaxFp8Ctas = 192;         // one CTA per multiprocessor
+// The scratch: launch epoch and counters, then the tagged words of the kernel for few rows, then the sums of the other.  Each keeps to
+// its own part: sums must not be taken for tags.
+constexpr int kMostColumnsRows = 64;     // rows of A of the kernel for few rows
+constexpr size_t kFp8Header = (kEpochWords + kMaxFp8Ctas) * sizeof(unsigned int);
+constexpr size_t kRowsScratch = kFp8Header + (size_t)kMaxFp8Ctas * kMostColumnsRows * kBlock * sizeof(unsigned long long);
+
 struct Fp8Args {
   const void *A, *B;
   void* C;

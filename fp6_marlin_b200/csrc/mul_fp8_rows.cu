@@ -6,8 +6,9 @@
 // the tensor cores; one CTA alone would have to bring 48 KB, more than the 64 bytes a cycle that reach a multiprocessor.
 // Up to 128 rows: one CTA, 128 columns.
 //
-// Every pair of CTAs (or CTA) computes whole tiles, in the order of the tiles, as long as all have one; what is left is cut along K
-// into equal ranges, whose sums are exchanged as in mul_fp8.cu.
+// Every pair of CTAs (or CTA) computes whole tiles, in the order of the tiles, as long as all have one.  What is left is cut along K
+// into equal ranges if that shortens the end by more than the exchange of their sums takes: all leave theirs in the scratch, and the
+// CTA that does so last adds them in the order of the ranges (an arrival counter; nobody waits).
 #include "../../include/fp6m.h"
 #include "host_common.h"
 #include "mul_fp8.cuh"
@@ -16,7 +17,7 @@ namespace fp6m {
 
 namespace {
 
-constexpr int kMaxTeams = 192;
+constexpr int kMaxTeams = kMaxFp8Ctas;
 
 struct RowsParams {
   void* C;
@@ -24,10 +25,11 @@ struct RowsParams {
   int M, N, kb;
   int row_tiles, tiles;                  // tiles in the order of their columns, row tiles next to one another
   int whole;                             // whole tiles of every team
-  int sharers;                           // teams that share the tiles that are left, cut along K
+  int extra;                             // the first teams that take one more, if the tiles that are left are not cut
+  int sharers;                           // teams that share the tiles that are left, cut along K (0: see extra)
   int weights_early;
-  unsigned int* epochs;
-  unsigned long long* partials;          // [CTA][value][thread] words {value, tag}
+  unsigned int* arrived;                 // [CTA] sums that were left for the tile that starts in that CTA's range
+  float4* partials;                      // [CTA][2][warp][4 columns][lane]: sums of a tile that starts before, in, the CTA's range
   int* status;
 };
 
@@ -42,10 +44,13 @@ struct RowsCfg {
   static constexpr int kMine = kColumns / 2;                 // columns of a thread
   static constexpr int kWarps = 8;
   static constexpr int kThreads = 32 * (4 + kWarps);
-  static constexpr int kNumBars = 2 * kStages + 2 * kTiles + 1;
+  static constexpr int kAhead = 8;                           // blocks of K whose scales are brought together
+  static constexpr int kScalePitch = 132;                    // floats from one block's row scales to the next: no bank conflicts
+  static constexpr int kScaleFloats = kAhead * (kScalePitch + 2);
+  static constexpr int kNumBars = 2 * kStages + 2 * kTiles + 4;
   static constexpr int kOutRow = 32 * 2 + 16;                // bytes of a row of 32 finished values in shared memory, with a gap
-  static constexpr int kSmemBytes = kStages * kStageBytes + kWarps * 32 * kOutRow + kNumBars * 8 + 16 + 1024;
-  static constexpr int kSlotWords = kMine * kWarps * 32;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kWarps * 32 * kOutRow + 2 * kScaleFloats * 4 + kNumBars * 8 + 16 + 1024;
+  static constexpr int kSlotFloat4 = kWarps * kMine / 4 * 32;
 };
 
 // A team's work: segments of one tile and a range of blocks of K each.
@@ -58,11 +63,11 @@ struct Segments {
   }
   // The start of a team's range among the blocks of the shared tiles.
   static __device__ __forceinline__ long long start_of(const RowsParams& p, int team, int teams) {
-    return (long long)(p.tiles - p.whole * teams) * p.kb * min(team, p.sharers) / max(p.sharers, 1);
+    return p.sharers ? (long long)(p.tiles - p.whole * teams) * p.kb * min(team, p.sharers) / p.sharers : 0;
   }
   __device__ __forceinline__ long long start_of(const RowsParams& p, int t) const { return start_of(p, t, teams); }
   __device__ __forceinline__ bool next(const RowsParams& p, int& tile, int& k0, int& k1) {
-    if (index < p.whole) {
+    if (index < p.whole + (team < p.extra)) {
       tile = team + teams * index++;
       k0 = 0;
       k1 = p.kb;
@@ -85,7 +90,7 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {       // the same
   return r;
 }
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
@@ -116,13 +121,6 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
   }
 }
-// two sums at a time
-__device__ __forceinline__ void fma2(unsigned long long& sum, uint32_t lo, uint32_t hi, unsigned long long scale) {
-  asm("{\n.reg .b64 v;\nmov.b64 v, {%1, %2};\nfma.rn.f32x2 %0, v, %3, %0;\n}\n" : "+l"(sum) : "r"(lo), "r"(hi), "l"(scale));
-}
-__device__ __forceinline__ float low(unsigned long long v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float high(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
-
 template <class T> struct Two;
 template <> struct Two<half> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) { half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<uint32_t*>(&h); }
@@ -138,15 +136,14 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* out_stage = smem + S * C::kStageBytes;                                   // [warp][32 rows][kOutRow]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(out_stage + C::kWarps * 32 * C::kOutRow);
-  volatile uint32_t* misc = reinterpret_cast<uint32_t*>(bars + C::kNumBars);        // [0] TMEM base, [1] launch epoch
-  const uint32_t full = smem_u32(bars), empty = full + 8 * S, done = empty + 8 * S, taken = done + 8 * D, epoch_bar = taken + 8 * D;
+  float* scales = reinterpret_cast<float*>(out_stage + C::kWarps * 32 * C::kOutRow);    // [2]: [block][row], then [block][128 columns]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(scales + 2 * C::kScaleFloats);
+  volatile uint32_t* misc = reinterpret_cast<uint32_t*>(bars + C::kNumBars);        // [0] TMEM base, [1] this CTA arrived last
+  const uint32_t full = smem_u32(bars), empty = full + 8 * S, done = empty + 8 * S, taken = done + 8 * D, scaled = taken + 8 * D, used = scaled + 16;
 
   const int tid = threadIdx.x, warp = uniform_warp_index(), lane = tid & 31;
   const int rank = G == 1 ? 0 : blockIdx.x & 1;              // in the team (clusters are neighbouring CTAs)
-  // Ranges are handed out from the last to the first: a team that waits for the partials of higher ones waits for CTAs that were
-  // dispatched before it.
-  const int teams = gridDim.x / G, team = teams - 1 - (int)blockIdx.x / G;
+  const int teams = gridDim.x / G, team = (int)blockIdx.x / G;
   launch_dependents();
 
   if (tid == 0) {
@@ -158,7 +155,10 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
       mbar_init(done + 8 * d, 1);                            // tcgen05.commit: the tile holds the block's products
       mbar_init(taken + 8 * d, G * C::kWarps);               // the warps of the team have read it back (in the first CTA)
     }
-    mbar_init(epoch_bar, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(scaled + 8 * i, 1);
+      mbar_init(used + 8 * i, C::kWarps);
+    }
     mbar_fence_init();
   }
   if (warp == 3) {
@@ -258,17 +258,40 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
         }
     }
   } else if (warp == 2) {
+    // ================================================================== scales, of eight blocks of K at a time
+    // (Loaded by the warps that sum, a row and block a lane, they cost those warps 280 cycles a block.)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     grid_dependency_wait();
-  } else if (warp == 3) {
-    // ================================================================== launch epoch: the tag of this launch's partials is epoch + 1
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (lane == 0) {
-      grid_dependency_wait();
-      misc[1] = read_epoch_and_count(p.epochs, gridDim.x);
-      mbar_arrive(epoch_bar);
+    constexpr int A = C::kAhead;
+    const int block = lane % A, row_of_lane = lane / A, step = 32 / A;
+    int turn = 0;
+    uint32_t phase = 0;
+    while (segments.next(p, tile, k0, k1)) {
+      const int row0 = tile % p.row_tiles * (128 * G) + rank * 128;
+      const int strip = min((tile / p.row_tiles) * G + (lane / A) % G, (p.N - 1) / kBlock);
+      for (int k = k0; k < k1; k += A) {
+        const bool live = k + block < k1;
+        float row_scale[128 / step];
+#pragma unroll
+        for (int i = 0; i < 128 / step; ++i) {
+          const int row = row0 + row_of_lane + step * i;
+          row_scale[i] = live && row < p.M ? p.sa[(size_t)row * p.kb + k + block] : 0.f;
+        }
+        const float strip_scale = live ? p.sb[(size_t)strip * p.kb + k + block] : 0.f;
+        float* to = scales + turn * C::kScaleFloats;
+        mbar_wait_bounded<100>(used + 8 * turn, phase ^ 1, p.status, dead);
+#pragma unroll
+        for (int i = 0; i < 128 / step; ++i) sts_f32(smem_u32(to + block * C::kScalePitch + row_of_lane + step * i), row_scale[i]);
+        if (lane < A * G) sts_f32(smem_u32(to + A * C::kScalePitch + block * G + lane / A), strip_scale);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scaled + 8 * turn);
+        turn ^= 1;
+        if (turn == 0) phase ^= 1;
+      }
     }
-    __syncwarp();
+  } else if (warp == 3) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    grid_dependency_wait();
   } else {
     // ================================================================== sums: thread = row of the tile, kMine columns
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -278,43 +301,41 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + column_in;
     const uint32_t taken0 = G == 1 ? taken : in_leader(taken);
     grid_dependency_wait();
-    unsigned long long sum[E / 2];                           // pairs of fp32 sums
-    int buffer = 0;
-    uint32_t tphase = 0;
-    float now[4], coming[4], coming_sb[4];                   // scales of four blocks, and of the next four, which are multiplied when they are used
-    const float *sa = nullptr, *sb = nullptr;
-    bool row_lives = false;
-    auto open = [&](int tile) {
-      const int row = tile % p.row_tiles * (128 * G) + rank * 128 + row_in;
-      const int block = ((tile / p.row_tiles) * C::kColumns + column_in) / kBlock;
-      row_lives = row < p.M;
-      sa = p.sa + (size_t)(row_lives ? row : 0) * p.kb;
-      sb = p.sb + (size_t)min(block, (p.N - 1) / kBlock) * p.kb;
-    };
-    auto fetch = [&](int k, int k1) {
+    float sum[E];
+    int buffer = 0, turn = 0;
+    uint32_t tphase = 0, sphase = 0;
+    // A warp turns 32 rows x 32 columns at a time round in shared memory: four lanes store 64 bytes of a row.
+    uint8_t* mine = out_stage + (warp - 4) * 32 * C::kOutRow;
+    auto put = [&](const float* v, int row0, int column0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        coming[j] = row_lives && k + j < k1 ? sa[k + j] : 0.f;
-        coming_sb[j] = k + j < k1 ? sb[k + j] : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = Two<T>::pack(v[i * 8 + 2 * e], v[i * 8 + 2 * e + 1]);
+        *reinterpret_cast<uint4*>(mine + lane * C::kOutRow + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      __syncwarp();
+      const int column = column0 + (lane & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        if (row0 + r < p.M && column < p.N)
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (size_t)(row0 + r) * p.N + column) = *reinterpret_cast<const uint4*>(mine + r * C::kOutRow + (lane & 3) * 16);
+      }
+      __syncwarp();
     };
-    bool more = segments.next(p, tile, k0, k1);
-    if (more) {
-      open(tile);
-      fetch(k0, k1);
-    }
-    while (more) {
+    while (segments.next(p, tile, k0, k1)) {
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) sum[i] = 0;
-      for (int k = k0; k < k1; k += 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) now[j] = coming[j] * coming_sb[j];
-        fetch(k + 4, k1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (k + j >= k1) break;
-          unsigned long long scale;
-          asm("mov.b64 %0, {%1, %1};" : "=l"(scale) : "f"(now[j]));
+      for (int i = 0; i < E; ++i) sum[i] = 0.f;
+#pragma unroll 1
+      for (int k = k0; k < k1; k += C::kAhead) {
+        mbar_wait_bounded<20>(scaled + 8 * turn, sphase, p.status, dead);
+        const uint32_t row_scale = smem_u32(scales + turn * C::kScaleFloats + row_in);
+        const uint32_t strip_scale = smem_u32(scales + turn * C::kScaleFloats + C::kAhead * C::kScalePitch + (G == 1 ? 0 : half_index));
+        const int blocks = min(C::kAhead, k1 - k);
+#pragma unroll 1
+        for (int j = 0; j < blocks; ++j) {
+          const float scale = lds_f32(row_scale + j * C::kScalePitch * 4) * lds_f32(strip_scale + j * G * 4);
           mbar_wait_bounded<20>(done + 8 * buffer, tphase, p.status, dead);
           tc_fence_after();
           const uint32_t from = lane_base + buffer * C::kColumns;
@@ -335,88 +356,65 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
               }
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) fma2(sum[c * 16 + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], scale);
+            for (int i = 0; i < 32; ++i) sum[c * 32 + i] = fmaf(__uint_as_float(v[c & 1][i]), scale, sum[c * 32 + i]);
           }
           if (++buffer == D) { buffer = 0; tphase ^= 1; }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(used + 8 * turn);
+        turn ^= 1;
+        if (turn == 0) sphase ^= 1;
       }
       // ---- the end of a segment
       const int row0 = tile % p.row_tiles * (128 * G) + rank * 128 + quarter * 32, column0 = (tile / p.row_tiles) * C::kColumns + column_in;
-      const bool starts = k0 == 0, ends = k1 == p.kb;
-      const int shared_tile = tile - p.whole * teams;
-      more = segments.next(p, tile, k0, k1);
-      if (more) {                                            // the next segment's first scales
-        open(tile);
-        fetch(k0, k1);
-      }
-      uint32_t tag = 0;
-      if (!starts || !ends) {
-        mbar_wait_bounded<20>(epoch_bar, 0, p.status, dead);
-        tag = misc[1] + 1;
-      }
-      auto slot_of = [&](int other) { return p.partials + (size_t)(other * G + rank) * C::kSlotWords + (warp - 4) * 32 + lane; };
-      constexpr int kStep = C::kWarps * 32;
-      if (!starts) {
-        // only a team's first segment of the shared tiles can start inside a tile, so a CTA has one partial
-        unsigned long long* slot = slot_of(team);
-        each<0, E / 2>([&](auto i) {
-          st_partial<2 * i * kStep>(slot, ((unsigned long long)tag << 32) | (uint32_t)sum[i]);
-          st_partial<(2 * i + 1) * kStep>(slot, ((unsigned long long)tag << 32) | (sum[i] >> 32));
-        });
+      if (k0 == 0 && k1 == p.kb) {
+#pragma unroll
+        for (int c = 0; c < E / 32; ++c) put(sum + c * 32, row0, column0 + c * 32);
         continue;
       }
-      if (!ends) {
-        // The team in which a tile starts adds the partials of the teams behind it, in their order.
-        const long long end = (long long)(shared_tile + 1) * p.kb;
-#pragma unroll 1
-        for (int other = team + 1; other < teams && segments.start_of(p, other) < end; ++other) {
-          if (segments.start_of(p, other) >= segments.start_of(p, other + 1)) break;
-          const unsigned long long* slot = slot_of(other);
-          each<0, E / 16>([&](auto part) {
-            constexpr int i0 = 16 * part;
-            unsigned long long w[16];
-            bool here = false;
-#pragma unroll 1
-            for (int spin = 0; spin < (1 << 20) && !here; ++spin) {
-              each<0, 16>([&](auto i) { w[i] = ld_partial<(i0 + i) * kStep>(slot); });
-              here = true;
+      // Part of a tile.  Only a team's first segment of the shared tiles can start inside a tile, only its last one can end inside.
+      constexpr int kPart = E / 4 * 32;
+      auto slot_of = [&](int t, int which) { return p.partials + ((size_t)(t * G + rank) * 2 + which) * C::kSlotFloat4 + (warp - 4) * kPart + lane; };
+      float4* slot = slot_of(team, k0 == 0 ? 1 : 0);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) here = here && (uint32_t)(w[i] >> 32) == tag;
-              if (dead) break;                               // a wait of this thread ran out before: do not wait again
-            }
-            if (!here && !dead) {
-              dead = true;
-              if (p.status) atomicExch(p.status, kStatusTimeout);
-            }
+      for (int i = 0; i < E / 4; ++i) __stcg(slot + i * 32, make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]));
+      const long long begin = (long long)(tile - p.whole * teams) * p.kb, end = begin + p.kb;
+      int first = team, last = team;
+      while (segments.start_of(p, first) > begin) --first;
+      while (last + 1 < p.sharers && segments.start_of(p, last + 1) < end) ++last;
+      __threadfence();
+      named_bar_sync(1, C::kWarps * 32);
+      if (tid == 128) {
+        const bool is_last = atomicAdd(p.arrived + first * G + rank, 1u) == (unsigned)(last - first);
+        if (is_last) p.arrived[first * G + rank] = 0;        // for the next launch
+        misc[1] = is_last;
+      }
+      named_bar_sync(1, C::kWarps * 32);
+      if (misc[1]) {
+        __threadfence();
+#pragma unroll 1
+        for (int c = 0; c < E / 32; ++c) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+#pragma unroll 1
+          for (int t = first; t <= last; ++t) {
+            const float4* from = slot_of(t, t == first ? 1 : 0) + c * 8 * 32;
+            float4 w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __ldcg(from + i * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const unsigned long long two = (w[2 * i] & 0xffffffffull) | w[2 * i + 1] << 32;
-              asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[i0 / 2 + i]) : "l"(two));
+              v[4 * i] += w[i].x;
+              v[4 * i + 1] += w[i].y;
+              v[4 * i + 2] += w[i].z;
+              v[4 * i + 3] += w[i].w;
             }
-          });
+          }
+          put(v, row0, column0 + c * 32);
         }
       }
-      // A warp turns 32 rows x 32 columns at a time round in shared memory: four lanes store 64 bytes of a row.
-      uint8_t* mine = out_stage + (warp - 4) * 32 * C::kOutRow;
-#pragma unroll
-      for (int c = 0; c < E / 32; ++c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = Two<T>::pack(low(sum[c * 16 + i * 4 + e]), high(sum[c * 16 + i * 4 + e]));
-          *reinterpret_cast<uint4*>(mine + lane * C::kOutRow + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        __syncwarp();
-        const int column = column0 + c * 32 + (lane & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 8 + (lane >> 2);
-          if (row0 + r < p.M && column < p.N)
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (size_t)(row0 + r) * p.N + column) = *reinterpret_cast<const uint4*>(mine + r * C::kOutRow + (lane & 3) * 16);
-        }
-        __syncwarp();
-      }
+      named_bar_sync(1, C::kWarps * 32);                     // all have read the answer
     }
   }
 
@@ -431,7 +429,7 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
 }
 
 struct RowsPlan {
-  int group, row_tiles, tiles, teams, whole, sharers;
+  int group, row_tiles, tiles, teams, whole, extra, sharers;
 };
 RowsPlan plan_rows(int M, int N, int K, int sms) {
   RowsPlan plan;
@@ -439,23 +437,30 @@ RowsPlan plan_rows(int M, int N, int K, int sms) {
   const int edge = 128 * plan.group, kb = (K + kBlock - 1) / kBlock;
   plan.row_tiles = (M + edge - 1) / edge;
   plan.tiles = plan.row_tiles * ((N + edge - 1) / edge);
-  int teams = (sms > 0 && sms < kMaxTeams ? sms : kMaxTeams) / plan.group;
-  const long long blocks = (long long)plan.tiles * kb;
-  if (teams > (blocks + 3) / 4) teams = (int)((blocks + 3) / 4);
-  plan.teams = teams < 1 ? 1 : teams;
+  plan.teams = (sms > 0 && sms < kMaxTeams ? sms : kMaxTeams) / plan.group;
+  if (plan.teams < 1) plan.teams = 1;
   plan.whole = plan.tiles / plan.teams;
-  const long long left = (long long)(plan.tiles - plan.whole * plan.teams) * kb;
-  plan.sharers = (int)(left / 4 < plan.teams ? (left + 3) / 4 : plan.teams);
+  const int left = plan.tiles - plan.whole * plan.teams;
+  plan.extra = left;
+  plan.sharers = 0;
+  // cut along K: at least four blocks each, and only where that saves more blocks than the exchange takes time
+  const long long blocks = (long long)left * kb;
+  const int sharers = (int)(blocks / 4 < plan.teams ? (blocks + 3) / 4 : plan.teams);
+  if (left > 0 && kb - (int)((blocks + sharers - 1) / sharers) >= 10) {
+    plan.extra = 0;
+    plan.sharers = sharers;
+  }
+  if (plan.whole == 0) plan.teams = plan.sharers ? plan.sharers : left;
   return plan;
 }
 size_t rows_bytes(const RowsPlan& plan) {
-  return kEpochWords * sizeof(unsigned int) + (size_t)plan.teams * plan.group * (plan.group * 64) * 256 * sizeof(unsigned long long);
+  return plan.sharers ? kRowsScratch + (size_t)plan.teams * plan.group * 2 * (plan.group * 64) * 256 * sizeof(float) : kRowsScratch;
 }
 
 template <class T, int kGroup>
 cudaError_t launch_rows(const RowsParams& p, int teams, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
   using C = RowsCfg<kGroup>;
-  static_assert(C::kSlotWords == kGroup * 64 * 256, "slot");
+  static_assert(C::kSlotFloat4 * 4 == kGroup * 64 * 256, "slot");
   cudaError_t e = cudaFuncSetAttribute(mul_fp8_rows_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -490,10 +495,11 @@ cudaError_t launch_fp8_rows(const Fp8Args& a, int sms, cudaStream_t stream) {
   p.row_tiles = plan.row_tiles;
   p.tiles = plan.tiles;
   p.whole = plan.whole;
+  p.extra = plan.extra;
   p.sharers = plan.sharers;
   p.weights_early = tc5_get_overlap() ? 1 : 0;
-  p.epochs = static_cast<unsigned int*>(a.scratch);
-  p.partials = reinterpret_cast<unsigned long long*>(static_cast<unsigned char*>(a.scratch) + kEpochWords * sizeof(unsigned int));
+  p.arrived = static_cast<unsigned int*>(a.scratch) + kEpochWords;
+  p.partials = reinterpret_cast<float4*>(static_cast<unsigned char*>(a.scratch) + kRowsScratch);
   p.status = a.status;
   CUtensorMap amap, bmap;
   cudaError_t e = encode_bytes_map(a.A, a.M, a.K, kBlock, &amap);
