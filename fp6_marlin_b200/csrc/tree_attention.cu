@@ -11,33 +11,18 @@
 // cut is made on the device, from the lengths, and the launch does not depend on them.  One pass over the keys keeps a
 // running maximum and sum per row in fp32.  Rows whose keys are shared by several CTAs are joined by the one that finishes
 // last (an arrival counter; nobody waits), in the order of the ranges, so results do not depend on who that is.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include "../../include/fp6m.h"
 #include "device_utils.cuh"
 #include "host_common.h"
+#include "tree_attention.cuh"
 
 namespace {
 
 using namespace fp6m;
 
-constexpr int kKeys = 64;                // keys per tile
 constexpr int kThreads = 128;
 constexpr int kMaxCtas = 512;
+constexpr int kLeastUnits = 3;           // of a CTA: fewer key tiles cost less than joining what more CTAs leave
 constexpr int kCounterBytes = kMaxCtas * 4;
-
-struct TreeParams {
-  fp6m_tree_attention_args a;
-  int group, rows, row_tiles;            // heads of queries per head of keys; rows and row tiles of a head of keys
-  unsigned long long page_magic;         // division by the page size: n * magic >> shift, exact for n < 2^31
-  int page_shift;
-  float scale_log2;                      // scale * log2(e): the softmax is computed in powers of two
-  unsigned int* arrived;                 // [CTA] contributors that have left their partial for the rows that start in that CTA
-  float* partials;                       // [CTA][2]: sums of row tile x head_dim, then maxima, then totals
-  int* status;
-};
 
 template <class T> struct Mma;
 template <> struct Mma<half> {
@@ -45,18 +30,12 @@ template <> struct Mma<half> {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) { half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<uint32_t*>(&h); }
-  static __device__ __forceinline__ float value(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
-  static constexpr uint32_t kExponent = 0x7c00u;
 };
 template <> struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) { __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<uint32_t*>(&h); }
-  static __device__ __forceinline__ float value(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
-  static constexpr uint32_t kExponent = 0x7f80u;
 };
 
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
@@ -65,49 +44,6 @@ __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// sixteen bytes, or zeros where `bytes` is 0 (the source is not read then)
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ int length_of(const TreeParams& p, int b) {
-  const int n = p.a.lengths[b], most = p.a.max_pages * p.a.page_size;
-  return n < 0 ? 0 : n > most ? most : n;
-}
-__device__ __forceinline__ int tiles_of(const TreeParams& p, int length) { return (int)(((long long)length + p.a.tokens + kKeys - 1) / kKeys); }
-
-// The start of a CTA's range, and the CTA whose range a unit lies in.
-__device__ __forceinline__ long long range_start(long long units, int ctas, int cta) { return units * cta / ctas; }
-__device__ __forceinline__ int cta_of(long long units, int ctas, long long unit) {
-  int c = (int)(unit * ctas / units);
-  while (c + 1 < ctas && range_start(units, ctas, c + 1) <= unit) ++c;
-  while (range_start(units, ctas, c) > unit) --c;
-  return c;
-}
-
-// A place in the sequence of units: the key tile of a (head of keys, row tile) pair of a sequence.
-struct Cursor {
-  int b, length, tiles, pair, tile;
-  __device__ __forceinline__ void next(const TreeParams& p) {
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++pair < p.a.kv_heads * p.row_tiles) return;
-    pair = 0;
-    if (++b < p.a.batch) {
-      length = length_of(p, b);
-      tiles = tiles_of(p, length);
-    }
-  }
-};
-
 // kRowTile rows, a warp for every 16 of them; the warps that this leaves share the keys of a tile and pool their sums.
 template <class T, int D, int kRowTile>
 __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __grid_constant__ TreeParams p) {
@@ -121,144 +57,116 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
   extern __shared__ __align__(128) uint8_t smem[];
   float* pool = reinterpret_cast<float*>(smem + kStages * 2 * kTileBytes);        // [kRowTile][kPool]
   float* stats = pool + kRowTile * kPool;                                          // [warp][2][16]: maxima, totals
-  long long* plan = reinterpret_cast<long long*>(stats + 4 * 32);                  // total units; unit of the first pair, b
+  long long* plan = reinterpret_cast<long long*>(stats + 4 * 32);                  // total units; unit of the first item, its sequence
   int* flags = reinterpret_cast<int*>(plan + 4);                                   // [0] a page did not exist, [1] last to arrive
+  const T** places = reinterpret_cast<const T**>(flags + 4);                       // [2][128]: where the keys, then the values, of a tile are
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row_warp = warp / kKeyWarps, key_warp = warp % kKeyWarps;
   const fp6m_tree_attention_args& a = p.a;
-  const int pairs = a.kv_heads * p.row_tiles;
   if (tid == 0) flags[0] = 0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- the plan: units of all sequences, and where this CTA's range starts
-  if (warp == 0) {
-    long long units = 0;
-    for (int b = lane; b < a.batch; b += 32) units += (long long)tiles_of(p, length_of(p, b)) * pairs;
-    for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-    const int ctas = (long long)gridDim.x < units ? (int)gridDim.x : (int)units;
-    const long long first = (int)blockIdx.x < ctas ? range_start(units, ctas, blockIdx.x) : units;
-    long long before = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      const int b = b0 + lane;
-      const long long mine = b < a.batch ? (long long)tiles_of(p, length_of(p, b)) * pairs : 0;
-      long long upto = mine;
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += other;
-      }
-      if (first >= before + upto - mine && first < before + upto) {
-        plan[1] = first - (before + upto - mine);
-        plan[2] = b;
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-      if (before > first) break;
-    }
-    if (lane == 0) plan[0] = units;
-  }
+  const int cta = blockIdx.x;
+  auto ctas_of = [&](long long units) { return (long long)gridDim.x < units / kLeastUnits ? (int)gridDim.x : max((int)(units / kLeastUnits), 1); };
+  if (warp == 0)
+    make_plan(p, plan, [&](long long units) {
+      const int n = ctas_of(units);
+      return cta < n ? range_start(units, n, cta) : units;
+    });
   __syncthreads();
   const long long units = plan[0];
-  const int ctas = (long long)gridDim.x < units ? (int)gridDim.x : (int)units;
-  const int cta = blockIdx.x;
+  const int ctas = ctas_of(units);
   if (cta >= ctas) return;
   const long long u0 = range_start(units, ctas, cta);
-  const int count = (int)(range_start(units, ctas, cta + 1) - u0);
-  Cursor at;
-  at.b = (int)plan[2];
-  at.length = length_of(p, at.b);
-  at.tiles = tiles_of(p, at.length);
-  at.pair = (int)(plan[1] / at.tiles);
-  at.tile = (int)(plan[1] % at.tiles);
+  Segments seg(p, plan, u0, range_start(units, ctas, cta + 1) - u0);
 
-  // ---- copies of a tile: a row of keys and one of values per token, zeros behind the last
-  const int load_row = tid / kChunks, chunk = tid % kChunks;
+  // ---- copies of a tile: a row of keys and one of values per token, zeros behind the last.  A thread works out where one row is (the
+  // same by all threads that copy a piece of it cost half of the kernel's instructions); the others take it from shared memory.
   const uint32_t smem_base = smem_u32(smem);
-  auto load = [&](const Cursor& c, int stage) {
-    const int g = c.pair / p.row_tiles, last = c.length + a.tokens;
+  const int load_row = tid / kChunks, chunk = tid % kChunks;
+  Segments ahead = seg;                                              // of the places, which are worked out a tile ahead of the copies
+  int ahead_tile = 0;
+  bool ahead_lives = ahead.next(p);
+  if (ahead_lives) ahead_tile = ahead.t0;
+  auto advance = [&] {
+    if (!ahead_lives || ++ahead_tile < ahead.t1) return;
+    ahead_lives = ahead.next(p);
+    ahead_tile = ahead.t0;
+  };
+  const int my_key = tid % kKeys;
+  auto look_up = [&] { return ahead_lives ? page_of(p, ahead, ahead_tile * kKeys + my_key) : 0; };
+  auto put_place = [&](int page, int parity) {
+    const int j = ahead_tile * kKeys + my_key;
+    const T* place = ahead_lives ? place_of<T>(p, ahead, ahead.item / p.row_tiles, j, page, tid >= kKeys) : nullptr;
+    if (ahead_lives && !place && j < ahead.length) flags[0] = 1;
+    places[parity * kThreads + tid] = place;
+  };
+  auto copy = [&](int stage, int parity) {
     const uint32_t dst = smem_base + stage * 2 * kTileBytes;
-    const int* table = a.page_table + c.b * a.page_table_stride;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int row = load_row + i * kRowsPerPass, j = c.tile * kKeys + row;
-      const T *k = static_cast<const T*>(a.q), *v = k;
-      uint32_t bytes = 0;
-      if (j < c.length) {
-        const int index = (int)((unsigned long long)j * p.page_magic >> p.page_shift);
-        const int page = table[index], slot = j - index * a.page_size;
-        if ((unsigned)page < (unsigned)a.pages) {
-          k = static_cast<const T*>(a.k_cache) + page * a.k_cache_stride[0] + slot * a.k_cache_stride[1] + g * a.k_cache_stride[2];
-          v = static_cast<const T*>(a.v_cache) + page * a.v_cache_stride[0] + slot * a.v_cache_stride[1] + g * a.v_cache_stride[2];
-          bytes = 16;
-        } else {
-          flags[0] = 1;
-        }
-      } else if (j < last) {
-        k = static_cast<const T*>(a.k) + c.b * a.k_stride[0] + (j - c.length) * a.k_stride[1] + g * a.k_stride[2];
-        v = static_cast<const T*>(a.v) + c.b * a.v_stride[0] + (j - c.length) * a.v_stride[1] + g * a.v_stride[2];
-        bytes = 16;
-      }
+      const int row = load_row + i * kRowsPerPass;
+      const T *k = places[parity * kThreads + row], *v = places[parity * kThreads + kKeys + row];
       const uint32_t to = dst + row * kRowBytes + ((chunk ^ (row & 7)) * 16);
-      copy16(to, k + chunk * 8, bytes);
-      copy16(to + kTileBytes, v + chunk * 8, bytes);
+      copy16(to, k ? k + chunk * 8 : static_cast<const T*>(a.q), k ? 16 : 0);
+      copy16(to + kTileBytes, v ? v + chunk * 8 : static_cast<const T*>(a.q), v ? 16 : 0);
     }
   };
-
-  Cursor ahead = at;
+  put_place(look_up(), 0);
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    if (s < count) {
-      load(ahead, s);
-      ahead.next(p);
-    }
+    __syncthreads();
+    const bool live = ahead_lives;
+    advance();
+    const int page = look_up();
+    if (live) copy(s, s & 1);
     copies_commit();
+    put_place(page, (s + 1) & 1);
   }
 
   const int quad = lane >> 2, col = (lane & 3) * 2;                  // this thread's rows quad and quad + 8, columns col and col + 1 of a fragment
+  int stage = 0, turn = (kStages - 1) & 1;                           // turn: of the places
+#pragma unroll 1
+  while (seg.next(p)) {
+  const int g = seg.item / p.row_tiles, tile_row0 = seg.item % p.row_tiles * kRowTile;
+  // ---- new rows: queries and masks
   uint32_t q[D / 16][4];
   float o[D / 8][4], top[2], total[2];
   unsigned long long mask[2];
-  bool fresh = true;
-  int segment_tile = 0;
-  long long item_unit = 0;                                           // the first unit of these rows
-  int stage = 0;
-#pragma unroll 1
-  for (int n = 0; n < count; ++n) {
-    const int g = at.pair / p.row_tiles, tile_row0 = at.pair % p.row_tiles * kRowTile;
-    if (fresh) {
-      // ---- new rows: queries and masks
-      fresh = false;
-      segment_tile = at.tile;
-      item_unit = u0 + n - at.tile;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = tile_row0 + row_warp * 16 + quad + 8 * h;
-        mask[h] = 0;
-        const T* src = nullptr;
-        if (r < p.rows) {
-          const int t = r / p.group, head = g * p.group + (r - t * p.group);
-          mask[h] = a.tree[at.b * a.tree_stride + t];
-          src = static_cast<const T*>(a.q) + at.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
-        }
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          q[i][h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + col) : 0u;
-          q[i][2 + h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + 8 + col) : 0u;
-        }
-        top[h] = -INFINITY;
-        total[h] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  for (int h = 0; h < 2; ++h) {
+    const int r = tile_row0 + row_warp * 16 + quad + 8 * h;
+    mask[h] = 0;
+    const T* src = nullptr;
+    if (r < p.rows) {
+      const int t = r / p.group, head = g * p.group + (r - t * p.group);
+      mask[h] = a.tree[seg.b * a.tree_stride + t];
+      src = static_cast<const T*>(a.q) + seg.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
     }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      q[i][h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + col) : 0u;
+      q[i][2 + h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + 8 + col) : 0u;
+    }
+    top[h] = -INFINITY;
+    total[h] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+#pragma unroll 1
+  for (int tile = seg.t0; tile < seg.t1; ++tile) {
     copies_wait<kStages - 2>();
     __syncthreads();
-    if (n + kStages - 1 < count) {
-      load(ahead, (stage + kStages - 1) % kStages);
-      ahead.next(p);
-    }
+    const bool live = ahead_lives;
+    advance();
+    const int page = look_up();
+    if (live) copy((stage + kStages - 1) % kStages, turn);
     copies_commit();
+    turn ^= 1;
 
     // ---- scores of this warp's keys
     const uint32_t keys = smem_base + stage * 2 * kTileBytes + key_warp * kMine * kRowBytes, values = keys + kTileBytes;
@@ -276,8 +184,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
         Mma<T>::run(s[i], q[2 * d + 1], k[2], k[3]);
       }
     }
-    const int j0 = at.tile * kKeys + key_warp * kMine;               // this warp's first key
-    const bool drafted = at.tile * kKeys + kKeys > at.length;        // the tile holds drafted tokens, or the end
+    const int j0 = tile * kKeys + key_warp * kMine;               // this warp's first key
+    const bool drafted = tile * kKeys + kKeys > seg.length;        // the tile holds drafted tokens, or the end
     const bool hidden = flags[0] != 0;                               // a page of this CTA's tiles did not exist
 #pragma unroll
     for (int i = 0; i < kMine / 8; ++i)
@@ -288,16 +196,15 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
       for (int i = 0; i < kMine / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int t = j0 + i * 8 + col + (e & 1) - at.length;      // drafted token, negative: cached
+          const int t = j0 + i * 8 + col + (e & 1) - seg.length;      // drafted token, negative: cached
           if (t >= 0 && (t >= 64 || !(mask[e >> 1] >> t & 1))) s[i][e] = -INFINITY;
         }
     }
     if (hidden) {
-      const int* table = a.page_table + at.b * a.page_table_stride;
 #pragma unroll 1
       for (int i = 0; i < kMine; ++i) {
         const int j = j0 + i;
-        if (j >= at.length || (unsigned)table[(int)((unsigned long long)j * p.page_magic >> p.page_shift)] < (unsigned)a.pages) continue;
+        if (j >= seg.length || (unsigned)page_of(p, seg, j) < (unsigned)a.pages) continue;
 #pragma unroll
         for (int k = 0; k < kMine / 8; ++k)
 #pragma unroll
@@ -334,16 +241,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 
     // ---- infinities and NaN among the drafted values: a weight of zero must not meet them
     if (drafted) {
-      const int from = max(at.length - at.tile * kKeys, 0), upto = min(at.length + a.tokens - at.tile * kKeys, kKeys);
+      const int from = max(seg.length - tile * kKeys, 0), upto = min(seg.length + a.tokens - tile * kKeys, kKeys);
       const uint32_t tile_values = smem_base + stage * 2 * kTileBytes + kTileBytes;
       bool odd = false;
       for (int i = tid; i < (upto - from) * kChunks; i += kThreads) {
         const int row = from + i / kChunks;
         uint4 w;
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(tile_values + row * kRowBytes + i % kChunks * 16) : "memory");
-        constexpr uint32_t E = Mma<T>::kExponent;
-        auto is_odd = [&](uint32_t x) { return (x & E) == E || (x >> 16 & E) == E; };
-        odd = odd || is_odd(w.x) || is_odd(w.y) || is_odd(w.z) || is_odd(w.w);
+        odd = odd || is_odd<T>(w.x) || is_odd<T>(w.y) || is_odd<T>(w.z) || is_odd<T>(w.w);
       }
       if (__syncthreads_or(odd)) {
         // each is multiplied by the weights of the rows that see it only, and is zero in the product below
@@ -360,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
                 if (k * 8 + e == (j & ~7) + (j & 1)) mine = s[k][2 * h + e];
             w[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + (j & 7) / 2);
           }
-          const int t = j0 + j - at.length;
+          const int t = j0 + j - seg.length;
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) {
             uint32_t two;
@@ -369,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             for (int e = 0; e < 4; ++e) {
               const uint32_t bits = e & 1 ? two >> 16 : two & 0xffffu;
               const bool sees = t >= 0 && t < 64 && (mask[e >> 1] >> t & 1);
-              if (sees && (bits & Mma<T>::kExponent) == Mma<T>::kExponent) o[i][e] += w[e >> 1] * Mma<T>::value((uint16_t)bits);
+              if (sees && (bits & Half16<T>::kExponent) == Half16<T>::kExponent) o[i][e] += w[e >> 1] * Half16<T>::value((uint16_t)bits);
             }
           }
         }
@@ -378,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
           const uint32_t addr = tile_values + (from + i / (D / 2)) * kRowBytes + i % (D / 2) * 4;
           uint32_t two;
           asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(addr) : "memory");
-          constexpr uint32_t E = Mma<T>::kExponent;
+          constexpr uint32_t E = Half16<T>::kExponent;
           if ((two & E) == E) two &= 0xffff0000u;
           if ((two >> 16 & E) == E) two &= 0xffffu;
           asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(two) : "memory");
@@ -390,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     // ---- weights times values
 #pragma unroll
     for (int k = 0; k < kMine / 16; ++k) {
-      const uint32_t w[4] = {Mma<T>::pack(s[2 * k][0], s[2 * k][1]), Mma<T>::pack(s[2 * k][2], s[2 * k][3]),
-                             Mma<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), Mma<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
+      const uint32_t w[4] = {Half16<T>::pack(s[2 * k][0], s[2 * k][1]), Half16<T>::pack(s[2 * k][2], s[2 * k][3]),
+                             Half16<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), Half16<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
       const int row = k * 16 + (lane & 15);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
@@ -403,10 +308,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
     }
     stage = (stage + 1) % kStages;
 
-    const bool ends = at.tile + 1 == at.tiles;
-    if (ends || n + 1 == count) {
+    put_place(page, turn);
+  }
+
       // ---- the end of this CTA's keys for these rows
-      fresh = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         total[h] += __shfl_xor_sync(0xffffffffu, total[h], 1);
@@ -463,10 +368,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
           }
         }
       }
-      const bool whole = segment_tile == 0 && ends;
+      const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
       auto out_row = [&](int r) {
         const int t = r / p.group, head = g * p.group + (r - t * p.group);
-        return static_cast<T*>(a.out) + at.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+        return static_cast<T*>(a.out) + seg.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
       };
       if (whole) {
         if (key_warp == 0) {
@@ -480,13 +385,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
               T* out = out_row(r) + col;
 #pragma unroll
               for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<uint32_t*>(out + 8 * i) = none ? 0u : Mma<T>::pack(o[i][2 * h] * f, o[i][2 * h + 1] * f);
+                *reinterpret_cast<uint32_t*>(out + 8 * i) = none ? 0u : Half16<T>::pack(o[i][2 * h] * f, o[i][2 * h + 1] * f);
             }
           }
         }
       } else {
         // a partial: the slot of a range's first rows, or that of its last ones
-        float* slot = p.partials + (size_t)(2 * cta + (segment_tile == 0 ? 1 : 0)) * kSlot;
+        float* slot = p.partials + (size_t)(2 * cta + (seg.t0 == 0 ? 1 : 0)) * kSlot;
         if (key_warp == 0) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -501,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             }
           }
         }
-        const int first_cta = segment_tile == 0 ? cta : cta_of(units, ctas, item_unit);
-        const int last_cta = cta_of(units, ctas, item_unit + at.tiles - 1);
+        const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
+        const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -536,16 +441,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
               m = now;
             }
             const int t = (tile_row0 + r) / p.group;
-            const bool none = a.tree[at.b * a.tree_stride + t] == 0 || sum == 0.f;
+            const bool none = a.tree[seg.b * a.tree_stride + t] == 0 || sum == 0.f;
             const float f = 1.f / sum;
             T* out = out_row(tile_row0 + r) + lane * V;
 #pragma unroll
-            for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Mma<T>::pack(acc[i] * f, acc[i + 1] * f);
+            for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[i] * f, acc[i + 1] * f);
           }
         }
       }
-    }
-    at.next(p);
   }
   copies_wait<0>();
   if (tid == 0 && flags[0] && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
@@ -553,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 
 template <class T, int D, int kRowTile>
 cudaError_t launch_tile(const TreeParams& p, int ctas, cudaStream_t stream) {
-  constexpr int bytes = 3 * 128 / D * 2 * kKeys * D * 2 + 16 * D * 4 + 4 * 32 * 4 + 4 * 8 + 16;
+  constexpr int bytes = 3 * 128 / D * 2 * kKeys * D * 2 + 16 * D * 4 + 4 * 32 * 4 + 4 * 8 + 16 + 2 * kThreads * 8;
   cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, D, kRowTile>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(tree_attention_kernel<T, D, kRowTile>, dim3(ctas), dim3(kThreads), bytes, stream, p);
@@ -610,6 +513,7 @@ int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, siz
   while ((1ll << log2) < a.page_size) ++log2;
   p.page_shift = 31 + log2;
   p.page_magic = ((1ull << p.page_shift) + a.page_size - 1) / a.page_size;
+  p.overhead = 2;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.arrived = static_cast<unsigned int*>(scratch);
   p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + kCounterBytes);

@@ -1,0 +1,173 @@
+// Shared by the kernels of attention over a paged cache (tree_attention.cu, tree_attention_tc5.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/fp6m.h"
+
+namespace fp6m {
+
+constexpr int kKeys = 64;                // keys per tile
+
+struct TreeParams {
+  fp6m_tree_attention_args a;
+  int group, rows, row_tiles;            // heads of queries per head of keys; rows of a head of keys and the tiles they are cut into
+  int overhead;                          // what the rows of an item cost besides their key tiles, in key tiles
+  unsigned long long page_magic;         // division by the page size: n * magic >> shift, exact for n < 2^31
+  int page_shift;
+  float scale_log2;                      // scale * log2(e): the softmax is computed in powers of two
+  unsigned int* arrived;                 // contributors that have left their partial for the rows that start in a CTA
+  float* partials;
+  int* status;
+};
+
+// tree_attention_tc5.cu: more rows than kFewRows
+constexpr int kFewRows = 32;
+size_t tree_tc5_scratch_bytes(int sms);
+cudaError_t launch_tree_tc5(const TreeParams& p, int sms, cudaStream_t stream);
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ int length_of(const TreeParams& p, int b) {
+  const int n = p.a.lengths[b], most = p.a.max_pages * p.a.page_size;
+  return n < 0 ? 0 : n > most ? most : n;
+}
+__device__ __forceinline__ int tiles_of(const TreeParams& p, int length) { return (int)(((long long)length + p.a.tokens + kKeys - 1) / kKeys); }
+
+// The work is a line of units: for every sequence, head of keys and row tile (an item) `overhead` units, then one for each key tile.
+// CTAs take equal ranges of it.
+__device__ __forceinline__ long long range_start(long long units, int ctas, int cta) { return units * cta / ctas; }
+__device__ __forceinline__ int cta_of(long long units, int ctas, long long unit) {
+  int c = (int)(unit * ctas / units);
+  while (c + 1 < ctas && range_start(units, ctas, c + 1) <= unit) ++c;
+  while (range_start(units, ctas, c) > unit) --c;
+  return c;
+}
+
+// Of one warp: the total of the units, and the sequence in which `first_of(total)` lies with the unit that it starts at; lane 0's answer
+// goes to plan[0 .. 2].
+template <class F>
+__device__ __forceinline__ void make_plan(const TreeParams& p, long long* plan, F&& first_of) {
+  const int lane = threadIdx.x & 31;
+  const long long items = (long long)p.a.kv_heads * p.row_tiles;
+  long long units = 0;
+  for (int b = lane; b < p.a.batch; b += 32) units += (tiles_of(p, length_of(p, b)) + p.overhead) * items;
+  for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+  const long long first = first_of(units);
+  long long before = 0;
+  for (int b0 = 0; b0 < p.a.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const long long mine = b < p.a.batch ? (tiles_of(p, length_of(p, b)) + p.overhead) * items : 0;
+    long long upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    if (first >= before + upto - mine && first < before + upto) {
+      plan[1] = first - (before + upto - mine);
+      plan[2] = b;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    if (before > first) break;
+  }
+  if (lane == 0) plan[0] = units;
+}
+
+// A CTA's range as a sequence of segments: the key tiles t0 .. t1 - 1 of an item.
+struct Segments {
+  int b, length, tiles, item, t0, t1;    // the segment
+  long long unit;                        // where its item starts
+  int at;                                // unit inside the item of what follows
+  long long left;                        // units that follow
+  __device__ __forceinline__ Segments(const TreeParams& p, const long long* plan, long long start, long long count) {
+    b = (int)plan[2];
+    length = length_of(p, b);
+    tiles = tiles_of(p, length);
+    const int size = tiles + p.overhead;
+    item = (int)(plan[1] / size);
+    at = (int)(plan[1] - (long long)item * size);
+    unit = start - at;
+    left = count;
+  }
+  __device__ __forceinline__ bool next(const TreeParams& p) {
+    while (left > 0) {
+      const int size = tiles + p.overhead;
+      if (at == size) {
+        at = 0;
+        unit += size;
+        if (++item == p.a.kv_heads * p.row_tiles) {
+          item = 0;
+          ++b;
+          length = length_of(p, b);
+          tiles = tiles_of(p, length);
+        }
+        continue;
+      }
+      const int take = left < size - at ? (int)left : size - at;
+      t0 = max(at - p.overhead, 0);
+      t1 = at + take - p.overhead;
+      at += take;
+      left -= take;
+      if (t1 > t0) return true;
+    }
+    return false;
+  }
+};
+
+// The first value of key (or value) j of a sequence, null where there is none: behind the last one, or in a page that does not exist.
+template <class T>
+__device__ __forceinline__ const T* place_of(const TreeParams& p, const Segments& s, int g, int j, int page, bool values) {
+  const fp6m_tree_attention_args& a = p.a;
+  const long long* strides = values ? a.v_cache_stride : a.k_cache_stride;
+  if (j < s.length) {
+    if ((unsigned)page >= (unsigned)a.pages) return nullptr;
+    const int slot = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
+    return static_cast<const T*>(values ? a.v_cache : a.k_cache) + page * strides[0] + slot * strides[1] + g * strides[2];
+  }
+  if (j - s.length >= a.tokens) return nullptr;
+  const long long* drafted = values ? a.v_stride : a.k_stride;
+  return static_cast<const T*>(values ? a.v : a.k) + s.b * drafted[0] + (j - s.length) * drafted[1] + g * drafted[2];
+}
+__device__ __forceinline__ int page_of(const TreeParams& p, const Segments& s, int j) {
+  return j < s.length ? p.a.page_table[s.b * p.a.page_table_stride + (int)((unsigned long long)j * p.page_magic >> p.page_shift)] : 0;
+}
+
+// sixteen bytes, or zeros where `bytes` is 0 (the source is not read then)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <class T> struct Half16;
+template <> struct Half16<half> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ float value(uint16_t bits) { return __half2float(__ushort_as_half(bits)); }
+  static constexpr uint32_t kExponent = 0x7c00u;       // all ones: infinite or NaN
+  static constexpr uint32_t kMmaFormat = 0;
+};
+template <> struct Half16<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) { __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ float value(uint16_t bits) { return __uint_as_float((uint32_t)bits << 16); }
+  static constexpr uint32_t kExponent = 0x7f80u;
+  static constexpr uint32_t kMmaFormat = 1;
+};
+// whether one of the two values is infinite or NaN
+template <class T>
+__device__ __forceinline__ bool is_odd(uint32_t two) {
+  constexpr uint32_t E = Half16<T>::kExponent;
+  return (two & E) == E || (two >> 16 & E) == E;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace fp6m
