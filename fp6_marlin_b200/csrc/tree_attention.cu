@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
   auto look_up = [&] { return ahead_lives ? page_of(p, ahead, ahead_tile * kKeys + my_key) : 0; };
   auto put_place = [&](int page, int parity) {
     const int j = ahead_tile * kKeys + my_key;
-    const T* place = ahead_lives ? place_of<T>(p, ahead, ahead.item / p.row_tiles, j, page, tid >= kKeys) : nullptr;
+    const T* place = ahead_lives ? place_of<T>(p, ahead, ahead.item, j, page, tid >= kKeys) : nullptr;
     if (ahead_lives && !place && j < ahead.length) flags[0] = 1;
     places[parity * kThreads + tid] = place;
   };
@@ -130,19 +130,19 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
   int stage = 0, turn = (kStages - 1) & 1;                           // turn: of the places
 #pragma unroll 1
   while (seg.next(p)) {
-  const int g = seg.item / p.row_tiles, tile_row0 = seg.item % p.row_tiles * kRowTile;
+  const int g = seg.item;
   // ---- new rows: queries and masks
   uint32_t q[D / 16][4];
   float o[D / 8][4], top[2], total[2];
   unsigned long long mask[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = tile_row0 + row_warp * 16 + quad + 8 * h;
+    const int r = row_warp * 16 + quad + 8 * h;
     mask[h] = 0;
     const T* src = nullptr;
     if (r < p.rows) {
       const int t = r / p.group, head = g * p.group + (r - t * p.group);
-      mask[h] = a.tree[seg.b * a.tree_stride + t];
+      mask[h] = mask_of(p, seg.b, t);
       src = static_cast<const T*>(a.q) + seg.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
     }
 #pragma unroll
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
         if (key_warp == 0) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int r = tile_row0 + row_warp * 16 + quad + 8 * h;
+            const int r = row_warp * 16 + quad + 8 * h;
             if (r < p.rows) {
               // padding, and rows that see nothing, are zero
               const bool none = mask[h] == 0 || total[h] == 0.f;
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = row_warp * 16 + quad + 8 * h;
-            if (tile_row0 + r < p.rows) {
+            if (r < p.rows) {
 #pragma unroll
               for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(slot + r * D + i * 8 + col) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
               if ((lane & 3) == 0) {
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
           __threadfence();
           // a warp per row, sixteen or eight bytes a lane
           constexpr int V = D / 32;
-          for (int r = warp; r < kRowTile && tile_row0 + r < p.rows; r += 4) {
+          for (int r = warp; r < p.rows; r += 4) {
             float m = -INFINITY, sum = 0.f, acc[V] = {};
             for (int c = first_cta; c <= last_cta; ++c) {
               const float* from = p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot;
@@ -440,10 +440,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
               for (int i = 0; i < V; ++i) acc[i] = acc[i] * old + v[i] * add;
               m = now;
             }
-            const int t = (tile_row0 + r) / p.group;
-            const bool none = a.tree[seg.b * a.tree_stride + t] == 0 || sum == 0.f;
+            const int t = r / p.group;
+            const bool none = mask_of(p, seg.b, t) == 0 || sum == 0.f;
             const float f = 1.f / sum;
-            T* out = out_row(tile_row0 + r) + lane * V;
+            T* out = out_row(r) + lane * V;
 #pragma unroll
             for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[i] * f, acc[i + 1] * f);
           }
@@ -462,10 +462,9 @@ cudaError_t launch_tile(const TreeParams& p, int ctas, cudaStream_t stream) {
   return launch_overlapped(tree_attention_kernel<T, D, kRowTile>, dim3(ctas), dim3(kThreads), bytes, stream, p);
 }
 template <class T>
-cudaError_t launch_tree(const TreeParams& p, int row_tile, int ctas, cudaStream_t stream) {
-  if (p.a.head_dim == 64)
-    return row_tile == 16 ? launch_tile<T, 64, 16>(p, ctas, stream) : row_tile == 32 ? launch_tile<T, 64, 32>(p, ctas, stream) : launch_tile<T, 64, 64>(p, ctas, stream);
-  return row_tile == 16 ? launch_tile<T, 128, 16>(p, ctas, stream) : row_tile == 32 ? launch_tile<T, 128, 32>(p, ctas, stream) : launch_tile<T, 128, 64>(p, ctas, stream);
+cudaError_t launch_tree(const TreeParams& p, int ctas, cudaStream_t stream) {
+  if (p.a.head_dim == 64) return p.rows <= 16 ? launch_tile<T, 64, 16>(p, ctas, stream) : launch_tile<T, 64, 32>(p, ctas, stream);
+  return p.rows <= 16 ? launch_tile<T, 128, 16>(p, ctas, stream) : launch_tile<T, 128, 32>(p, ctas, stream);
 }
 
 int tree_ctas(int sms) {
@@ -485,7 +484,10 @@ bool rows_aligned(const void* p, const long long (&strides)[kStrides]) {
 
 extern "C" {
 
-size_t fp6m_tree_attention_scratch_bytes(int sms) { return kCounterBytes + (size_t)tree_ctas(sms) * 2 * 64 * (128 + 2) * sizeof(float); }
+size_t fp6m_tree_attention_scratch_bytes(int sms) { 
+  const size_t few = (size_t)tree_ctas(sms) * 2 * kFewRows * (128 + 2) * sizeof(float), many = tree_tc5_partial_bytes(sms);
+  return kCounterBytes + (few > many ? few : many);
+}
 
 int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev) {
   if (!args) return FP6M_ERR_BAD_ARG;
@@ -507,19 +509,19 @@ int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, siz
   p.a = a;
   p.group = a.heads / a.kv_heads;
   p.rows = a.tokens * p.group;
-  const int row_tile = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64;
-  p.row_tiles = (p.rows + row_tile - 1) / row_tile;
+  p.row_tiles = p.parts = 1;
+  p.overhead = 4;
   int log2 = 0;
   while ((1ll << log2) < a.page_size) ++log2;
   p.page_shift = 31 + log2;
   p.page_magic = ((1ull << p.page_shift) + a.page_size - 1) / a.page_size;
-  p.overhead = 2;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.arrived = static_cast<unsigned int*>(scratch);
   p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + kCounterBytes);
   p.status = status_dev;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a.type == FP6M_TYPE_F16 ? launch_tree<half>(p, row_tile, tree_ctas(sms), st) : launch_tree<__nv_bfloat16>(p, row_tile, tree_ctas(sms), st);
+  const cudaError_t e = p.rows > kFewRows ? launch_tree_tc5(p, sms, st)
+                        : a.type == FP6M_TYPE_F16 ? launch_tree<half>(p, tree_ctas(sms), st) : launch_tree<__nv_bfloat16>(p, tree_ctas(sms), st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "tree_attention launch");
 }
 

@@ -14,7 +14,8 @@ constexpr int kKeys = 64;                // keys per tile
 
 struct TreeParams {
   fp6m_tree_attention_args a;
-  int group, rows, row_tiles;            // heads of queries per head of keys; rows of a head of keys and the tiles they are cut into
+  int group, rows;                       // heads of queries per head of keys; rows of a head of keys
+  int row_tiles, parts;                  // the tiles that the rows are cut into, and the items they make (one or two tiles each)
   int overhead;                          // what the rows of an item cost besides their key tiles, in key tiles
   unsigned long long page_magic;         // division by the page size: n * magic >> shift, exact for n < 2^31
   int page_shift;
@@ -26,18 +27,22 @@ struct TreeParams {
 
 // tree_attention_tc5.cu: more rows than kFewRows
 constexpr int kFewRows = 32;
-size_t tree_tc5_scratch_bytes(int sms);
-cudaError_t launch_tree_tc5(const TreeParams& p, int sms, cudaStream_t stream);
+size_t tree_tc5_partial_bytes(int sms);
+cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream);
 
 #ifdef __CUDACC__
 
+// The drafted tokens that token t of sequence b sees.
+__device__ __forceinline__ unsigned long long mask_of(const TreeParams& p, int b, int t) {
+  return p.a.tree[b * p.a.tree_stride + t] & (~0ull >> (64 - p.a.tokens));
+}
 __device__ __forceinline__ int length_of(const TreeParams& p, int b) {
   const int n = p.a.lengths[b], most = p.a.max_pages * p.a.page_size;
   return n < 0 ? 0 : n > most ? most : n;
 }
 __device__ __forceinline__ int tiles_of(const TreeParams& p, int length) { return (int)(((long long)length + p.a.tokens + kKeys - 1) / kKeys); }
 
-// The work is a line of units: for every sequence, head of keys and row tile (an item) `overhead` units, then one for each key tile.
+// The work is a line of units: for every sequence, head of keys and row tile (an item: one row tile, or two) `overhead` units, then one for each key tile.
 // CTAs take equal ranges of it.
 __device__ __forceinline__ long long range_start(long long units, int ctas, int cta) { return units * cta / ctas; }
 __device__ __forceinline__ int cta_of(long long units, int ctas, long long unit) {
@@ -52,7 +57,7 @@ __device__ __forceinline__ int cta_of(long long units, int ctas, long long unit)
 template <class F>
 __device__ __forceinline__ void make_plan(const TreeParams& p, long long* plan, F&& first_of) {
   const int lane = threadIdx.x & 31;
-  const long long items = (long long)p.a.kv_heads * p.row_tiles;
+  const long long items = (long long)p.a.kv_heads * p.parts;
   long long units = 0;
   for (int b = lane; b < p.a.batch; b += 32) units += (tiles_of(p, length_of(p, b)) + p.overhead) * items;
   for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
@@ -98,7 +103,7 @@ struct Segments {
       if (at == size) {
         at = 0;
         unit += size;
-        if (++item == p.a.kv_heads * p.row_tiles) {
+        if (++item == p.a.kv_heads * p.parts) {
           item = 0;
           ++b;
           length = length_of(p, b);

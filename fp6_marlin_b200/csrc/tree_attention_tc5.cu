@@ -1,0 +1,633 @@
+// Attention over a paged cache for more than 32 rows per head of keys, on tcgen05 (fewer rows, and what is computed: tree_attention.cu).
+//
+// A row tile of 128 rows is the M dimension: scores S (128 x 64 keys) = Q K^T with both operands in shared memory, then
+// O (128 x head_dim) += P V with the weights P as the operand in tensor memory, written over S in 16 bits, and V as it lies (keys
+// in rows, so its operand is "transposed").  A thread owns a row: no exchange between threads for maxima and sums.  Two groups of four warps
+// compute weights in turn; each has two score tiles, so that the tensor cores work on the next scores of one and the product of
+// the other meanwhile.  More than 128 rows: a group for each of two row tiles, which share the keys in shared memory.  Up to 128 rows: the
+// groups take the key tiles in turn and their sums are joined at the end.
+//
+// O is rescaled only where a row's maximum grows by more than a factor of 2^8: until then the weights are taken relative to the older
+// maximum, which changes neither the result nor, in fp32 sums and 16-bit floating-point weights, its precision.
+#include "../../include/fp6m.h"
+#include "device_utils.cuh"
+#include "gemm_params.h"
+#include "host_common.h"
+#include "tc5_common.cuh"
+#include "tree_attention.cuh"
+
+namespace fp6m {
+
+namespace {
+
+constexpr int kRowTile = 128;
+constexpr int kMostTreeCtas = 192;       // one per multiprocessor
+constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs (three idle), twice four that compute weights
+constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass
+
+template <int D_>
+struct TreeCfg {
+  static constexpr int D = D_;
+  static constexpr int kTileBytes = kKeys * D * 2;           // keys or values of a tile
+  static constexpr int kQBytes = kRowTile * D * 2;
+  static constexpr int kStages = 4 * 128 / D;                // of keys, and of values
+  static constexpr int kExchange = kRowTile * 32 * 4;        // 32 columns of a group's sums
+  static constexpr int kNumBars = 4 * kStages + 2 + 4 + 4 + 2;
+  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kTileBytes, kX = kV + kStages * kTileBytes;
+  static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
+  static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
+  static constexpr int kBars = kPlaces + 4 * kKeys * 8;
+  static constexpr int kSmemBytes = kBars + kNumBars * 8 + (4 + 32) * 4 + 1024;
+  static constexpr int kSlotFloats = kRowTile * (D + 2) + 4; // a partial: sums [4 columns][row], maxima, totals, whether odd values were met
+  static_assert(kSmemBytes <= 232448, "shared memory");
+};
+constexpr int kOddRing = 32;             // segments: more than the copies can be ahead of the sums
+
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// operand with 128-byte swizzle whose 128-byte rows hold 64 values of K (keys and queries), or of N (`pitch`: from one 64 columns to the next)
+__device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return wide_act_desc(addr); }
+__device__ __forceinline__ uint64_t columns_desc(uint32_t addr, uint32_t pitch) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(pitch >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
+// waits for the loads; the registers pass through, so that nothing that uses them can be moved in front of the wait
+__device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
+  tc_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
+
+// kPair: two row tiles of an item share its keys, a group each; else the groups share one row tile.
+template <class T, class C, bool kPair>
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p) {
+  constexpr int D = C::D, S = C::kStages;
+  constexpr int kAhead = kPair ? 1 : 2;                              // key tiles whose scores are issued before the weights of the first are there
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t base = smem_u32(smem);
+  const uint32_t full_k = base + C::kBars, empty_k = full_k + 8 * S, full_v = empty_k + 8 * S, empty_v = full_v + 8 * S;
+  const uint32_t q_free = empty_v + 8 * S, scores = q_free + 16, weights = scores + 32, product = weights + 32;
+  volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, [2, 3] last to arrive
+  volatile uint32_t* odd_ring = misc + 4;                            // [segment]: infinities or NaN among its drafted values
+  __shared__ long long plan[4];
+  const int tid = threadIdx.x, warp = uniform_warp_index(), lane = tid & 31;
+  const fp6m_tree_attention_args& a = p.a;
+
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full_k + 8 * s, 64);         // the threads that copy: their copies have landed
+      mbar_init(empty_k + 8 * s, 1);         // tcgen05.commit: the scores are computed
+      mbar_init(full_v + 8 * s, 64);
+      mbar_init(empty_v + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_free + 8 * i, 1);          // tcgen05.commit: an item's last scores are computed
+      mbar_init(product + 8 * i, 1);         // tcgen05.commit: a group's weights are multiplied
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(scores + 8 * i, 1);          // [group][buffer] tcgen05.commit
+      mbar_init(weights + 8 * i, 4);         // [group][buffer] the warps of the group have written weights (one per buffer: a warp may be a job ahead)
+    }
+    mbar_fence_init();
+    misc[1] = 0;
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(const_cast<uint32_t*>(misc))) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  grid_dependency_wait();
+  const int cta = blockIdx.x;
+  auto ctas_of = [&](long long units) { return (long long)gridDim.x < units / 3 ? (int)gridDim.x : max((int)(units / 3), 1); };
+  if (warp == 0)
+    make_plan(p, plan, [&](long long units) {
+      const int n = ctas_of(units);
+      return cta < n ? range_start(units, n, cta) : units;
+    });
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, misc[0], 0);
+  const long long units = plan[0];
+  const int ctas = ctas_of(units);
+  const bool works = cta < ctas;
+  const long long u0 = works ? range_start(units, ctas, cta) : 0;
+  bool dead = false;
+
+  if (works) {
+    Segments seg(p, plan, u0, range_start(units, ctas, cta + 1) - u0);
+    // score tiles [group][2] of 64 columns, then a tile of sums per group
+    const uint32_t tmem_o = tmem + 256;
+    if (warp < 4) {
+      // ================================================================== copies: two warps the keys and queries, two the values
+      const bool values = warp >= 2;
+      const int me = tid & 63, chunk = me % (D / 8), row0 = me / (D / 8);
+      constexpr int kRowsPerPass = 64 / (D / 8), kPasses = kKeys / kRowsPerPass;
+      const uint32_t ring = base + (values ? C::kV : C::kK), full = values ? full_v : full_k, empty = values ? empty_v : empty_k;
+      const T** places = reinterpret_cast<const T**>(smem + C::kPlaces) + (values ? 2 * kKeys : 0);
+      const int bar_id = values ? 3 : 2;
+      auto put_place = [&](const Segments& s, int tile, int page, int parity) {
+        const int j = tile * kKeys + me;
+        const T* place = place_of<T>(p, s, s.item / p.parts, j, page, values);
+        if (!place && j < s.length) misc[1] = 1;
+        places[parity * kKeys + me] = place;
+      };
+      Segments ahead = seg;
+      bool lives = ahead.next(p);
+      int tile = ahead.t0;
+      if (lives) put_place(ahead, tile, page_of(p, ahead, tile * kKeys + me), 0);
+      int n = 0, landed = 0, segment = 0;                            // tiles issued, of them signalled
+      bool fresh = true;
+      auto signal_upto = [&](int upto) {
+        if (landed >= upto) return;
+        fence_async_proxy();
+        for (; landed < upto; ++landed) mbar_arrive(full + 8 * (landed % S));
+      };
+      while (lives) {
+        named_bar_sync(bar_id, 64);                                  // the places are there
+        const int stage = n % S;
+        if (n >= S && !mbar_try_wait(empty + 8 * stage, (n / S + 1) & 1)) {
+          // no room: hand over what has landed meanwhile
+          copies_wait<0>();
+          signal_upto(n);
+          mbar_wait_bounded<50>(empty + 8 * stage, (n / S + 1) & 1, p.status, dead);
+        }
+        const Segments now = ahead;
+        const int this_tile = tile, this_segment = segment;
+        if (values && fresh && me == 0) odd_ring[segment % kOddRing] = 0;
+        if (!values && fresh) {
+          // the queries of an item come with its first keys
+          const int set = kPair ? 0 : segment & 1, turn = kPair ? segment : segment >> 1;
+          if (turn > 0) {
+            copies_wait<0>();
+            signal_upto(n);
+            mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
+          }
+          constexpr int kTiles = kPair ? 2 : 1;
+          const int g = now.item / p.parts, first_row = now.item % p.parts * kTiles * kRowTile;
+          for (int i = row0; i < kTiles * kRowTile; i += kRowsPerPass) {
+            const int r = first_row + i;
+            const T* src = nullptr;
+            if (r < p.rows) {
+              const int t = r / p.group, head = g * p.group + (r - t * p.group);
+              src = static_cast<const T*>(a.q) + now.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
+            }
+            const uint32_t to = base + C::kQ + (kPair ? i / kRowTile : set) * C::kQBytes + (chunk >> 3) * (kRowTile * 128) + (i % kRowTile) * 128 + (((chunk & 7) ^ (i & 7)) * 16);
+            copy16(to, src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
+          }
+        }
+        // the next tile's page is looked up while this one is copied
+        fresh = false;
+        if (++tile >= ahead.t1) {
+          lives = ahead.next(p);
+          tile = ahead.t0;
+          fresh = true;
+          ++segment;
+        }
+        const int page = lives ? page_of(p, ahead, tile * kKeys + me) : 0;
+        const uint32_t dst = ring + stage * C::kTileBytes;
+#pragma unroll 4
+        for (int i = 0; i < kPasses; ++i) {
+          const int row = row0 + i * kRowsPerPass;
+          const T* src = places[(n & 1) * kKeys + row];
+          copy16(dst + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
+        }
+        copies_commit();
+        if (lives) put_place(ahead, tile, page, (n + 1) & 1);
+        if (values && this_tile * kKeys + kKeys > now.length) {
+          // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
+          // that see them at the end.
+          copies_wait<0>();
+          named_bar_sync(bar_id, 64);
+          const int j = this_tile * kKeys + me;
+          bool odd = false;
+          if (j >= now.length) {
+            for (int c = 0; c < D / 8; ++c) {
+              const uint32_t at = dst + (c >> 3) * (kKeys * 128) + me * 128 + (((c & 7) ^ (me & 7)) * 16);
+              uint4 w = lds128(at);
+              if (is_odd<T>(w.x) || is_odd<T>(w.y) || is_odd<T>(w.z) || is_odd<T>(w.w)) {
+                odd = true;
+                uint32_t v[4] = {w.x, w.y, w.z, w.w};
+                constexpr uint32_t E = Half16<T>::kExponent;
+                for (int e = 0; e < 4; ++e) {
+                  if ((v[e] & E) == E) v[e] &= 0xffff0000u;
+                  if ((v[e] >> 16 & E) == E) v[e] &= 0xffffu;
+                  sts_u32(at + 4 * e, v[e]);
+                }
+              }
+            }
+          }
+          if (odd) odd_ring[this_segment % kOddRing] = 1;
+        }
+        ++n;
+        copies_wait<2>();
+        signal_upto(n - 2);
+      }
+      copies_wait<0>();
+      signal_upto(n);
+    } else if (warp == 4) {
+      // ================================================================== MMA issuer
+      constexpr uint32_t kFormats = (1u << 4) | (Half16<T>::kMmaFormat << 7) | (Half16<T>::kMmaFormat << 10) | ((uint32_t)(kRowTile >> 4) << 24);
+      constexpr uint32_t idesc_s = kFormats | ((uint32_t)(kKeys >> 3) << 17);
+      constexpr uint32_t idesc_o = kFormats | (1u << 16) | ((uint32_t)(D >> 3) << 17);         // values are N-major
+      Segments front = seg, back = seg;                              // of the scores, of the products
+      bool front_lives = front.next(p), back_lives = back.next(p);
+      int front_tile = front.t0, back_tile = back.t0, issued = 0, multiplied = 0, segment = 0;
+      int score_jobs[2] = {0, 0}, product_jobs[2] = {0, 0};
+      uint32_t started = 0;                                          // groups whose sums of the segment hold something
+      auto groups_of = [&](const Segments& s) {                      // of a pair, the second may have no rows
+        return kPair && s.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1;
+      };
+      while (back_lives) {
+        while (front_lives && issued < multiplied + 1 + kAhead) {
+          const int stage = issued % S, set = kPair ? 0 : segment & 1;
+          mbar_wait_bounded<20>(full_k + 8 * stage, (issued / S) & 1, p.status, dead);
+          tc_fence_after();
+          const uint64_t k_desc = rows_desc(base + C::kK + stage * C::kTileBytes);
+          const bool last = front_tile + 1 >= front.t1;
+          const int groups = groups_of(front);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (kPair ? w >= groups : w != (issued & 1)) continue;
+            const uint64_t q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * C::kQBytes);
+            const int buffer = score_jobs[w] & 1;
+            if (elect_one()) {
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+                mma_smem(tmem + (w * 2 + buffer) * kKeys, q_desc + (i >> 2) * (kRowTile * 128 >> 4) + (i & 3) * 2, k_desc + (i >> 2) * (kKeys * 128 >> 4) + (i & 3) * 2, idesc_s, i);
+              tc_commit(scores + 8 * (w * 2 + buffer));
+            }
+            __syncwarp();
+            ++score_jobs[w];
+          }
+          if (elect_one()) {
+            tc_commit(empty_k + 8 * stage);
+            if (last) tc_commit(q_free + 8 * set);
+          }
+          __syncwarp();
+          ++issued;
+          if (++front_tile >= front.t1) {
+            front_lives = front.next(p);
+            front_tile = front.t0;
+            ++segment;
+          }
+        }
+        const int stage = multiplied % S;
+        mbar_wait_bounded<20>(full_v + 8 * stage, (multiplied / S) & 1, p.status, dead);
+        const int groups = groups_of(back);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (kPair ? w >= groups : w != (multiplied & 1)) continue;
+          const int buffer = product_jobs[w] & 1;
+          mbar_wait_bounded<20>(weights + 8 * (w * 2 + buffer), (product_jobs[w] >> 1) & 1, p.status, dead);
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < kKeys / 16; ++i)
+              mma_tmem(tmem_o + w * 128, tmem + (w * 2 + buffer) * kKeys + i * 8, columns_desc(base + C::kV + stage * C::kTileBytes + i * 16 * 128, kKeys * 128), idesc_o,
+                       i > 0 ? 1u : started >> w & 1);
+            tc_commit(product + 8 * w);
+          }
+          __syncwarp();
+          started |= 1u << w;
+          ++product_jobs[w];
+        }
+        if (elect_one()) tc_commit(empty_v + 8 * stage);
+        __syncwarp();
+        ++multiplied;
+        if (++back_tile >= back.t1) {
+          back_lives = back.next(p);
+          back_tile = back.t0;
+          started = 0;
+        }
+      }
+    } else if (warp >= 8) {
+      // ================================================================== weights: thread = row
+      const int group = (warp - 8) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane;
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const uint32_t my_scores = tmem + lanes + group * 2 * kKeys, my_sums = tmem_o + lanes + group * 128;
+      const float sl = p.scale_log2;
+      float* stats = reinterpret_cast<float*>(smem + C::kStats);
+      float4* exchange = reinterpret_cast<float4*>(smem + C::kX);
+      int job = 0, n = 0, segment = -1;                              // jobs of this group, tiles of the CTA
+      while (seg.next(p)) {
+        ++segment;
+        const int g = seg.item / p.parts, row_tile = kPair ? seg.item % p.parts * 2 + group : seg.item % p.parts;
+        const int row = row_tile * kRowTile + row_in;
+        const bool row_lives = row < p.rows;
+        const bool warp_lives = row_tile * kRowTile + quarter * 32 < p.rows;
+        const int t = row_lives ? row / p.group : 0, head = g * p.group + (row_lives ? row - t * p.group : 0);
+        const unsigned long long mask = row_lives ? mask_of(p, seg.b, t) : 0;
+        float top = -INFINITY, total = 0.f;                          // the maximum that the weights are relative to
+        bool any = false;                                            // the sums hold something
+        const bool group_lives = !kPair || row_tile < p.row_tiles;
+        for (int tile = seg.t0; tile < seg.t1; ++tile, ++n) {
+          if (!group_lives || (!kPair && (n & 1) != group)) continue;
+          const int buffer = job & 1;
+          mbar_wait_bounded<20>(scores + 8 * (group * 2 + buffer), (job >> 1) & 1, p.status, dead);
+          tc_fence_after();
+          if (warp_lives) {
+            uint32_t s[kKeys];
+            tmem_load32(my_scores + buffer * kKeys, s);
+            tmem_load32(my_scores + buffer * kKeys + 32, s + 32);
+            // which keys the row sees: all cached ones, then those of its mask
+            unsigned long long sees = ~0ull;
+            const int cached = seg.length - tile * kKeys;            // of this tile
+            if (cached < kKeys) sees = cached > 0 ? mask << cached | ((1ull << cached) - 1) : cached > -64 ? mask >> -cached : 0ull;
+            if (misc[1]) {
+              for (int i = 0; i < min(cached, kKeys); ++i)
+                if ((unsigned)page_of(p, seg, tile * kKeys + i) >= (unsigned)a.pages) sees &= ~(1ull << i);
+            }
+            tmem_loaded32(s);
+            tmem_loaded32(s + 32);
+            // the largest of the scores that are seen; a negative scale turns the order round
+            const bool all = sees == ~0ull;
+            const bool mixed = __any_sync(0xffffffffu, !all);
+            if (mixed) {
+#pragma unroll
+              for (int i = 0; i < kKeys; ++i)
+                if (!(sees >> i & 1)) s[i] = __float_as_uint(sl < 0.f ? INFINITY : -INFINITY);
+            }
+            float m0 = as_float(s[0]), m1 = as_float(s[1]), m2 = as_float(s[2]), m3 = as_float(s[3]);
+            if (sl >= 0.f) {
+#pragma unroll
+              for (int i = 4; i < kKeys; i += 4) {
+                m0 = fmaxf(m0, as_float(s[i]));
+                m1 = fmaxf(m1, as_float(s[i + 1]));
+                m2 = fmaxf(m2, as_float(s[i + 2]));
+                m3 = fmaxf(m3, as_float(s[i + 3]));
+              }
+              m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+            } else {
+#pragma unroll
+              for (int i = 4; i < kKeys; i += 4) {
+                m0 = fminf(m0, as_float(s[i]));
+                m1 = fminf(m1, as_float(s[i + 1]));
+                m2 = fminf(m2, as_float(s[i + 2]));
+                m3 = fminf(m3, as_float(s[i + 3]));
+              }
+              m0 = fminf(fminf(m0, m1), fminf(m2, m3));
+            }
+            const float m = sees ? m0 * sl : -INFINITY;
+            const bool grows = m > top + kGrowth || (top == -INFINITY && m > top);
+            if (__any_sync(0xffffffffu, grows)) {
+              const float now = fmaxf(top, m);
+              const float keep = exp2_approx(top - (now == -INFINITY ? 0.f : now));
+              top = now;
+              total *= keep;
+              if (any) {
+                mbar_wait_bounded<20>(product + 8 * group, (job - 1) & 1, p.status, dead);
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tmem_load32(my_sums + c, o);
+                  tmem_loaded32(o);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
+                  tmem_store32(my_sums + c, o);
+                }
+              }
+            }
+            const float base_log2 = top == -INFINITY ? 0.f : top;
+            float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 4) {
+              float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
+              float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
+              if (mixed) {
+                e0 = sees >> i & 1 ? e0 : 0.f;
+                e1 = sees >> (i + 1) & 1 ? e1 : 0.f;
+                e2 = sees >> (i + 2) & 1 ? e2 : 0.f;
+                e3 = sees >> (i + 3) & 1 ? e3 : 0.f;
+              }
+              t0 += e0;
+              t1 += e1;
+              t2 += e2;
+              t3 += e3;
+              w[i / 2] = Half16<T>::pack(e0, e1);
+              w[i / 2 + 1] = Half16<T>::pack(e2, e3);
+            }
+            total += (t0 + t1) + (t2 + t3);
+            tmem_store32(my_scores + buffer * kKeys, w);
+            tc_wait_st();
+          }
+          any = true;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(weights + 8 * (group * 2 + buffer));
+          ++job;
+        }
+        if (kPair && !group_lives) continue;
+
+        // ---- the end of a segment
+        if (any) {
+          mbar_wait_bounded<20>(product + 8 * group, (job - 1) & 1, p.status, dead);
+          tc_fence_after();
+        }
+        const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
+        float* slot = nullptr;
+        constexpr int kGroups = kPair ? 2 : 1;                       // that leave a partial
+        const int which = kPair ? group : 0;
+        auto slot_of = [&](int c, bool first) { return p.partials + ((size_t)(c * kGroups + which) * 2 + (first ? 1 : 0)) * C::kSlotFloats; };
+        if (!whole) slot = slot_of(cta, seg.t0 == 0);
+        float mine = 1.f, theirs = 0.f;
+        if (!kPair) {
+          // the second group hands its maxima, totals and sums to the first
+          if (group == 1) {
+            stats[row_in] = top;
+            stats[kRowTile + row_in] = total;
+          }
+          named_bar_sync(1, 256);
+          if (group == 0) {
+            const float other = stats[row_in], both = fmaxf(top, other), base_log2 = both == -INFINITY ? 0.f : both;
+            mine = exp2_approx(top - base_log2);
+            theirs = exp2_approx(other - base_log2);
+            total = total * mine + stats[kRowTile + row_in] * theirs;
+            top = both;
+          }
+        }
+        bool odd = odd_ring[segment % kOddRing] != 0;                // (both groups' products are done)
+        const bool none = mask == 0 || total == 0.f;                 // padding, and rows that see nothing, are zero
+        const float f = 1.f / total;
+        T* out = static_cast<T*>(a.out) + seg.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+        // infinite and NaN values of drafted tokens, for the rows that see them
+        auto add_odd = [&](float (&v)[32], int c) {
+          for (int j = 0; j < a.tokens; ++j) {
+            if (!(mask >> j & 1)) continue;
+            const uint16_t* from = static_cast<const uint16_t*>(a.v) + seg.b * a.v_stride[0] + j * a.v_stride[1] + g * a.v_stride[2] + c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((from[i] & Half16<T>::kExponent) == Half16<T>::kExponent) v[i] += Half16<T>::value(from[i]);
+          }
+        };
+        auto put = [&](float (&v)[32], int c, float by, bool zero, bool add) {
+          if (!row_lives) return;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= by;
+          if (add) add_odd(v, c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = zero ? 0u : Half16<T>::pack(v[8 * i + 2 * e], v[8 * i + 2 * e + 1]);
+            *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        };
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          if (any && warp_lives) {
+            tmem_load32(my_sums + c0, o);
+            tmem_loaded32(o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          if (!kPair) {
+            if (group == 1) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) exchange[i * kRowTile + row_in] = make_float4(as_float(o[4 * i]), as_float(o[4 * i + 1]), as_float(o[4 * i + 2]), as_float(o[4 * i + 3]));
+            }
+            named_bar_sync(1, 256);
+          }
+          if ((kPair || group == 0) && warp_lives) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = as_float(o[i]) * mine;
+            if (!kPair) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 x = exchange[i * kRowTile + row_in];
+                v[4 * i] = fmaf(x.x, theirs, v[4 * i]);
+                v[4 * i + 1] = fmaf(x.y, theirs, v[4 * i + 1]);
+                v[4 * i + 2] = fmaf(x.z, theirs, v[4 * i + 2]);
+                v[4 * i + 3] = fmaf(x.w, theirs, v[4 * i + 3]);
+              }
+            }
+            if (whole) {
+              put(v, c0, f, none, odd);
+            } else {
+              float4* to = reinterpret_cast<float4*>(slot) + c0 / 4 * kRowTile + row_in;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) __stcg(to + i * kRowTile, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+            }
+          }
+          if (!kPair) named_bar_sync(1, 256);
+        }
+        if (whole || (!kPair && group == 1)) continue;
+        slot[kRowTile * D + row_in] = top;
+        slot[kRowTile * (D + 1) + row_in] = total;
+        if (row_in == 0) reinterpret_cast<int*>(slot)[kRowTile * (D + 2)] = odd;
+        const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
+        const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
+        __threadfence();
+        named_bar_sync(4 + which, 128);
+        if (row_in == 0) {
+          unsigned int* counter = p.arrived + first_cta * 2 + which;
+          const bool is_last = atomicAdd(counter, 1u) == (unsigned)(last_cta - first_cta);
+          if (is_last) *counter = 0;                                 // for the next launch
+          misc[2 + which] = is_last;
+        }
+        named_bar_sync(4 + which, 128);
+        if (!misc[2 + which]) continue;
+        __threadfence();
+        float m = -INFINITY;
+        odd = false;
+        for (int c = first_cta; c <= last_cta; ++c) {
+          const float* from = slot_of(c, c == first_cta);
+          m = fmaxf(m, __ldcg(from + kRowTile * D + row_in));
+          odd = odd || __ldcg(reinterpret_cast<const int*>(from) + kRowTile * (D + 2)) != 0;
+        }
+        const float base_log2 = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+        for (int c = first_cta; c <= last_cta; ++c) {
+          const float* from = slot_of(c, c == first_cta);
+          sum += __ldcg(from + kRowTile * (D + 1) + row_in) * exp2_approx(__ldcg(from + kRowTile * D + row_in) - base_log2);
+        }
+        if (warp_lives) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+#pragma unroll 1
+            for (int c = first_cta; c <= last_cta; ++c) {
+              const float* from = slot_of(c, c == first_cta);
+              const float by = exp2_approx(__ldcg(from + kRowTile * D + row_in) - base_log2);
+              const float4* at = reinterpret_cast<const float4*>(from) + c0 / 4 * kRowTile + row_in;
+              float4 x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = __ldcg(at + i * kRowTile);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                v[4 * i] = fmaf(x[i].x, by, v[4 * i]);
+                v[4 * i + 1] = fmaf(x[i].y, by, v[4 * i + 1]);
+                v[4 * i + 2] = fmaf(x[i].z, by, v[4 * i + 2]);
+                v[4 * i + 3] = fmaf(x[i].w, by, v[4 * i + 3]);
+              }
+            }
+            put(v, c0, 1.f / sum, mask == 0 || sum == 0.f, odd);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && misc[1] && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
+  if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <class T, class C, bool kPair>
+cudaError_t launch_tc5(const TreeParams& p, int ctas, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(tree_attention_tc5_kernel<T, C, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(tree_attention_tc5_kernel<T, C, kPair>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p);
+}
+template <class T>
+cudaError_t launch_typed(const TreeParams& p, int ctas, cudaStream_t stream) {
+  const bool pair = p.row_tiles > 1;
+  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64>, true>(p, ctas, stream) : launch_tc5<T, TreeCfg<64>, false>(p, ctas, stream);
+  return pair ? launch_tc5<T, TreeCfg<128>, true>(p, ctas, stream) : launch_tc5<T, TreeCfg<128>, false>(p, ctas, stream);
+}
+
+}  // namespace
+
+// (a CTA leaves at most two partials for each of two row tiles)
+size_t tree_tc5_partial_bytes(int sms) { return (size_t)(sms > 0 && sms < kMostTreeCtas ? sms : kMostTreeCtas) * 4 * TreeCfg<128>::kSlotFloats * sizeof(float); }
+
+cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream) {
+  p.row_tiles = (p.rows + kRowTile - 1) / kRowTile;
+  p.parts = (p.row_tiles + 1) / 2;
+  p.overhead = 4;
+  const int ctas = sms < kMostTreeCtas ? sms : kMostTreeCtas;
+  return p.a.type == FP6M_TYPE_F16 ? launch_typed<half>(p, ctas, stream) : launch_typed<__nv_bfloat16>(p, ctas, stream);
+}
+
+}  // namespace fp6m
