@@ -43,7 +43,12 @@ struct TreeCfg {
 };
 constexpr int kOddRing = 32;             // segments: more than the copies can be ahead of the sums
 
+// What was written to shared memory by copies and stores is seen by the MMAs that follow.  It stands where the MMAs are issued, behind the
+// barrier that counts the copies: in a thread that copies it would wait for all of that thread's copies in flight (measured: a tile
+// per latency of memory, 7000 cycles, in place of four tiles on their way).
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// arrives once this thread's copies so far have landed
+__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 // operand with 128-byte swizzle whose 128-byte rows hold 64 values of K (keys and queries), or of N (`pitch`: from one 64 columns to the next)
 __device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return wide_act_desc(addr); }
 __device__ __forceinline__ uint64_t columns_desc(uint32_t addr, uint32_t pitch) {
@@ -159,33 +164,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       bool lives = ahead.next(p);
       int tile = ahead.t0;
       if (lives) put_place(ahead, tile, page_of(p, ahead, tile * kKeys + me), 0);
-      int n = 0, landed = 0, segment = 0;                            // tiles issued, of them signalled
+      int n = 0, segment = 0;
       bool fresh = true;
-      auto signal_upto = [&](int upto) {
-        if (landed >= upto) return;
-        fence_async_proxy();
-        for (; landed < upto; ++landed) mbar_arrive(full + 8 * (landed % S));
-      };
       while (lives) {
         named_bar_sync(bar_id, 64);                                  // the places are there
         const int stage = n % S;
-        if (n >= S && !mbar_try_wait(empty + 8 * stage, (n / S + 1) & 1)) {
-          // no room: hand over what has landed meanwhile
-          copies_wait<0>();
-          signal_upto(n);
-          mbar_wait_bounded<50>(empty + 8 * stage, (n / S + 1) & 1, p.status, dead);
-        }
+        if (n >= S) mbar_wait_bounded<50>(empty + 8 * stage, (n / S + 1) & 1, p.status, dead);
         const Segments now = ahead;
         const int this_tile = tile, this_segment = segment;
         if (values && fresh && me == 0) odd_ring[segment % kOddRing] = 0;
         if (!values && fresh) {
           // the queries of an item come with its first keys
           const int set = kPair ? 0 : segment & 1, turn = kPair ? segment : segment >> 1;
-          if (turn > 0) {
-            copies_wait<0>();
-            signal_upto(n);
-            mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
-          }
+          if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
           constexpr int kTiles = kPair ? 2 : 1;
           const int g = now.item / p.parts, first_row = now.item % p.parts * kTiles * kRowTile;
           for (int i = row0; i < kTiles * kRowTile; i += kRowsPerPass) {
@@ -215,12 +206,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           const T* src = places[(n & 1) * kKeys + row];
           copy16(dst + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
         }
-        copies_commit();
+        const bool drafted = values && this_tile * kKeys + kKeys > now.length;
+        if (!drafted) copies_arrive(full + 8 * stage);
         if (lives) put_place(ahead, tile, page, (n + 1) & 1);
-        if (values && this_tile * kKeys + kKeys > now.length) {
+        if (drafted) {
           // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
           // that see them at the end.
-          copies_wait<0>();
+          asm volatile("cp.async.wait_all;" ::: "memory");
           named_bar_sync(bar_id, 64);
           const int j = this_tile * kKeys + me;
           bool odd = false;
@@ -241,13 +233,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             }
           }
           if (odd) odd_ring[this_segment % kOddRing] = 1;
+          mbar_arrive(full + 8 * stage);
         }
         ++n;
-        copies_wait<2>();
-        signal_upto(n - 2);
       }
-      copies_wait<0>();
-      signal_upto(n);
     } else if (warp == 4) {
       // ================================================================== MMA issuer
       constexpr uint32_t kFormats = (1u << 4) | (Half16<T>::kMmaFormat << 7) | (Half16<T>::kMmaFormat << 10) | ((uint32_t)(kRowTile >> 4) << 24);
@@ -265,6 +254,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         while (front_lives && issued < multiplied + 1 + kAhead) {
           const int stage = issued % S, set = kPair ? 0 : segment & 1;
           mbar_wait_bounded<20>(full_k + 8 * stage, (issued / S) & 1, p.status, dead);
+          fence_async_proxy();
           tc_fence_after();
           const uint64_t k_desc = rows_desc(base + C::kK + stage * C::kTileBytes);
           const bool last = front_tile + 1 >= front.t1;
@@ -297,6 +287,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         }
         const int stage = multiplied % S;
         mbar_wait_bounded<20>(full_v + 8 * stage, (multiplied / S) & 1, p.status, dead);
+        fence_async_proxy();
         const int groups = groups_of(back);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
