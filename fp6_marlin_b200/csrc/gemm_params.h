@@ -87,6 +87,7 @@ cudaError_t encode_activation_map(const half* A, int M, int K, int box_rows, CUt
 cudaError_t encode_activation_segment_map(const half* A, int M, int K, int box_rows, CUtensorMap* map);
 cudaError_t encode_output_map(const half* base, int rows, int ld, CUtensorMap* map);
 cudaError_t encode_bytes_map(const void* base, int rows, int K, int box_rows, CUtensorMap* map);
+cudaError_t encode_cache_map(const void* base, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, CUtensorMap* map);
 constexpr int kMaxWideCtas = 192;   // one CTA per SM
 constexpr int kMaxRowTiles = 32;    // 8192 rows of A per launch
 constexpr int kWideTileRows = 256;  // most rows of a tile

@@ -41,6 +41,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cstring>
 
 #include "device_utils.cuh"
 #include "fp6m_layout.h"
@@ -631,7 +632,7 @@ static cudaError_t encode(CUtensorMap* map, CUtensorMapDataType type, int rank, 
                           const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   EncodeTiledFn encode_fn = encode_tiled();
   if (!encode_fn) return cudaErrorNotSupported;
-  const cuuint32_t elem[3] = {1, 1, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
   for (int attempt = 0; attempt < 2; ++attempt) {
     if (encode_fn(map, type, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
@@ -655,6 +656,7 @@ namespace {
 struct MapKey {
   const void* A;
   int M, K, box_rows, dims;
+  long long more[5] = {};                 // of a paged cache: heads, tokens and strides
 };
 struct MapCache {
   static constexpr int kEntries = 96;      // a GEMM of many launches onto eight outputs has 64 output maps
@@ -663,7 +665,8 @@ struct MapCache {
   int next = 0;
   bool find(const MapKey& k, CUtensorMap* out) const {
     for (int i = 0; i < kEntries; ++i)
-      if (key[i].A == k.A && key[i].M == k.M && key[i].K == k.K && key[i].box_rows == k.box_rows && key[i].dims == k.dims) {
+      if (key[i].A == k.A && key[i].M == k.M && key[i].K == k.K && key[i].box_rows == k.box_rows && key[i].dims == k.dims &&
+          (k.dims != 6 || std::memcmp(key[i].more, k.more, sizeof(k.more)) == 0)) {
         *out = map[i];
         return true;
       }
@@ -727,6 +730,19 @@ cudaError_t encode_bytes_map(const void* base, int rows, int K, int box_rows, CU
   const cuuint64_t strides[1] = {(cuuint64_t)K};
   const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
   const cudaError_t e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+  if (e == cudaSuccess) g_map_cache.put(mk, *map);
+  return e;
+}
+
+// A paged cache of 16-bit values as a tensor of head_dim x heads x page_size x pages with any strides (elements: page, slot, head); one box
+// = 64 values of `run` neighbouring tokens, in 128-byte rows with the 128-byte swizzle; what lies outside reads as zero.
+cudaError_t encode_cache_map(const void* base, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, CUtensorMap* map) {
+  const MapKey mk = {base, pages, head_dim, run, 6, {heads, page_size, strides[0], strides[1], strides[2]}};
+  if (g_map_cache.find(mk, map)) return cudaSuccess;
+  const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)page_size, (cuuint64_t)pages};
+  const cuuint64_t pitches[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)run, 1};
+  const cudaError_t e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, pitches, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
   if (e == cudaSuccess) g_map_cache.put(mk, *map);
   return e;
 }

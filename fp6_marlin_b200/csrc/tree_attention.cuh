@@ -19,6 +19,7 @@ struct TreeParams {
   int overhead;                          // what the rows of an item cost besides their key tiles, in key tiles
   unsigned long long page_magic;         // division by the page size: n * magic >> shift, exact for n < 2^31
   int page_shift;
+  int run;                               // tokens of a page that one TMA copy brings (0: none does)
   float scale_log2;                      // scale * log2(e): the softmax is computed in powers of two
   unsigned int* arrived;                 // contributors that have left their partial for the rows that start in a CTA
   float* partials;

@@ -49,6 +49,14 @@ constexpr int kOddRing = 32;             // segments: more than the copies can b
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // arrives once this thread's copies so far have landed
 __device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+// 64 values of p.run tokens: value x, head, slot, page.  x is 0 or 64 (bytes: a multiple of 128), so the copy starts on a 16-byte boundary.
+__device__ __forceinline__ void tma_load_run(uint32_t dst, const CUtensorMap* map, int x, int head, int slot, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 // operand with 128-byte swizzle whose 128-byte rows hold 64 values of K (keys and queries), or of N (`pitch`: from one 64 columns to the next)
 __device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return wide_act_desc(addr); }
 __device__ __forceinline__ uint64_t columns_desc(uint32_t addr, uint32_t pitch) {
@@ -88,7 +96,7 @@ __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v
 
 // kPair: two row tiles of an item share its keys, a group each; else the groups share one row tile.
 template <class T, class C, bool kPair>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   constexpr int D = C::D, S = C::kStages;
   constexpr int kAhead = kPair ? 1 : 2;                              // key tiles whose scores are issued before the weights of the first are there
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -154,69 +162,78 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       const uint32_t ring = base + (values ? C::kV : C::kK), full = values ? full_v : full_k, empty = values ? empty_v : empty_k;
       const T** places = reinterpret_cast<const T**>(smem + C::kPlaces) + (values ? 2 * kKeys : 0);
       const int bar_id = values ? 3 : 2;
-      auto put_place = [&](const Segments& s, int tile, int page, int parity) {
-        const int j = tile * kKeys + me;
-        const T* place = place_of<T>(p, s, s.item / p.parts, j, page, values);
-        if (!place && j < s.length) misc[1] = 1;
-        places[parity * kKeys + me] = place;
-      };
+      const CUtensorMap* map = values ? &vmap : &kmap;
+      // Tiles of cached tokens come by tiled TMA, p.run tokens of a page at a time (0: the pages' size or the cache's layout does not allow it);
+      // other tiles, sixteen bytes a thread.  (All tiles in the second way took 2500 cycles of the copying warps each.)
+      auto whole_runs = [&](const Segments& s, int tile) { return p.run > 0 && (tile + 1) * kKeys <= s.length; };
+      auto look_up = [&](const Segments& s, int tile) { return page_of(p, s, tile * kKeys + (whole_runs(s, tile) ? min(me * p.run, kKeys - 1) : me)); };
       Segments ahead = seg;
       bool lives = ahead.next(p);
       int tile = ahead.t0;
-      if (lives) put_place(ahead, tile, page_of(p, ahead, tile * kKeys + me), 0);
+      int page = lives ? look_up(ahead, tile) : 0;                   // of this thread's run, or key, of the tile
       int n = 0, segment = 0;
       bool fresh = true;
       while (lives) {
-        named_bar_sync(bar_id, 64);                                  // the places are there
-        const int stage = n % S;
+        const int stage = n % S, g = ahead.item / p.parts;
+        const uint32_t dst = ring + stage * C::kTileBytes;
+        const bool runs = whole_runs(ahead, tile);
+        if (!runs) {
+          const int j = tile * kKeys + me;
+          const T* place = place_of<T>(p, ahead, g, j, page, values);
+          if (!place && j < ahead.length) misc[1] = 1;
+          places[(n & 1) * kKeys + me] = place;
+          named_bar_sync(bar_id, 64);
+        }
         if (n >= S) mbar_wait_bounded<50>(empty + 8 * stage, (n / S + 1) & 1, p.status, dead);
-        const Segments now = ahead;
-        const int this_tile = tile, this_segment = segment;
         if (values && fresh && me == 0) odd_ring[segment % kOddRing] = 0;
         if (!values && fresh) {
           // the queries of an item come with its first keys
           const int set = kPair ? 0 : segment & 1, turn = kPair ? segment : segment >> 1;
           if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
           constexpr int kTiles = kPair ? 2 : 1;
-          const int g = now.item / p.parts, first_row = now.item % p.parts * kTiles * kRowTile;
+          const int first_row = ahead.item % p.parts * kTiles * kRowTile;
           for (int i = row0; i < kTiles * kRowTile; i += kRowsPerPass) {
             const int r = first_row + i;
             const T* src = nullptr;
             if (r < p.rows) {
               const int t = r / p.group, head = g * p.group + (r - t * p.group);
-              src = static_cast<const T*>(a.q) + now.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
+              src = static_cast<const T*>(a.q) + ahead.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
             }
             const uint32_t to = base + C::kQ + (kPair ? i / kRowTile : set) * C::kQBytes + (chunk >> 3) * (kRowTile * 128) + (i % kRowTile) * 128 + (((chunk & 7) ^ (i & 7)) * 16);
             copy16(to, src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
           }
         }
-        // the next tile's page is looked up while this one is copied
-        fresh = false;
-        if (++tile >= ahead.t1) {
-          lives = ahead.next(p);
-          tile = ahead.t0;
-          fresh = true;
-          ++segment;
-        }
-        const int page = lives ? page_of(p, ahead, tile * kKeys + me) : 0;
-        const uint32_t dst = ring + stage * C::kTileBytes;
+        if (runs) {
+          if (me == 0) mbar_expect_tx(full + 8 * stage, C::kTileBytes);
+          if (me < 32) {
+            __syncwarp();
+            const int index = tile * kKeys + me * p.run;
+            if (me * p.run < kKeys) {
+              const int slot = index - (int)((unsigned long long)index * p.page_magic >> p.page_shift) * a.page_size;
+              if ((unsigned)page >= (unsigned)a.pages) misc[1] = 1;  // reads zeros
+              const int real = (unsigned)page < (unsigned)a.pages ? page : a.pages;
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h) tma_load_run(dst + h * (kKeys * 128) + me * p.run * 128, map, h * 64, g, slot, real, full + 8 * stage);
+            }
+          }
+        } else {
 #pragma unroll 4
-        for (int i = 0; i < kPasses; ++i) {
-          const int row = row0 + i * kRowsPerPass;
-          const T* src = places[(n & 1) * kKeys + row];
-          copy16(dst + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
+          for (int i = 0; i < kPasses; ++i) {
+            const int row = row0 + i * kRowsPerPass;
+            const T* src = places[(n & 1) * kKeys + row];
+            copy16(dst + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
+          }
         }
-        const bool drafted = values && this_tile * kKeys + kKeys > now.length;
+        const bool drafted = values && tile * kKeys + kKeys > ahead.length;
         if (!drafted) copies_arrive(full + 8 * stage);
-        if (lives) put_place(ahead, tile, page, (n + 1) & 1);
         if (drafted) {
           // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
           // that see them at the end.
           asm volatile("cp.async.wait_all;" ::: "memory");
           named_bar_sync(bar_id, 64);
-          const int j = this_tile * kKeys + me;
+          const int j = tile * kKeys + me;
           bool odd = false;
-          if (j >= now.length) {
+          if (j >= ahead.length) {
             for (int c = 0; c < D / 8; ++c) {
               const uint32_t at = dst + (c >> 3) * (kKeys * 128) + me * 128 + (((c & 7) ^ (me & 7)) * 16);
               uint4 w = lds128(at);
@@ -232,10 +249,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               }
             }
           }
-          if (odd) odd_ring[this_segment % kOddRing] = 1;
+          if (odd) odd_ring[segment % kOddRing] = 1;
           mbar_arrive(full + 8 * stage);
         }
         ++n;
+        fresh = false;
+        if (++tile >= ahead.t1) {
+          lives = ahead.next(p);
+          tile = ahead.t0;
+          fresh = true;
+          ++segment;
+        }
+        if (lives) page = look_up(ahead, tile);
       }
     } else if (warp == 4) {
       // ================================================================== MMA issuer
@@ -596,16 +621,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
 }
 
 template <class T, class C, bool kPair>
-cudaError_t launch_tc5(const TreeParams& p, int ctas, cudaStream_t stream) {
+cudaError_t launch_tc5(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
   cudaError_t e = cudaFuncSetAttribute(tree_attention_tc5_kernel<T, C, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(tree_attention_tc5_kernel<T, C, kPair>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p);
+  return launch_overlapped(tree_attention_tc5_kernel<T, C, kPair>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p, kmap, vmap);
 }
 template <class T>
-cudaError_t launch_typed(const TreeParams& p, int ctas, cudaStream_t stream) {
+cudaError_t launch_typed(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
   const bool pair = p.row_tiles > 1;
-  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64>, true>(p, ctas, stream) : launch_tc5<T, TreeCfg<64>, false>(p, ctas, stream);
-  return pair ? launch_tc5<T, TreeCfg<128>, true>(p, ctas, stream) : launch_tc5<T, TreeCfg<128>, false>(p, ctas, stream);
+  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64>, true>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<64>, false>(p, ctas, kmap, vmap, stream);
+  return pair ? launch_tc5<T, TreeCfg<128>, true>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<128>, false>(p, ctas, kmap, vmap, stream);
 }
 
 }  // namespace
@@ -618,7 +643,15 @@ cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream) {
   p.parts = (p.row_tiles + 1) / 2;
   p.overhead = 4;
   const int ctas = sms < kMostTreeCtas ? sms : kMostTreeCtas;
-  return p.a.type == FP6M_TYPE_F16 ? launch_typed<half>(p, ctas, stream) : launch_typed<__nv_bfloat16>(p, ctas, stream);
+  // the tokens that lie next to one another in a page and start at a multiple of their number in a tile: swizzled rows need eight
+  const fp6m_tree_attention_args& a = p.a;
+  p.run = kKeys;
+  while (a.page_size % p.run) p.run /= 2;
+  CUtensorMap kmap = {}, vmap = {};
+  if (p.run < 8 || a.max_pages == 0 || encode_cache_map(a.k_cache, a.head_dim, a.kv_heads, a.page_size, a.pages, a.k_cache_stride, p.run, &kmap) != cudaSuccess ||
+      encode_cache_map(a.v_cache, a.head_dim, a.kv_heads, a.page_size, a.pages, a.v_cache_stride, p.run, &vmap) != cudaSuccess)
+    p.run = 0;
+  return a.type == FP6M_TYPE_F16 ? launch_typed<half>(p, ctas, kmap, vmap, stream) : launch_typed<__nv_bfloat16>(p, ctas, kmap, vmap, stream);
 }
 
 }  // namespace fp6m
