@@ -516,6 +516,7 @@ int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, siz
   p.page_shift = 31 + log2;
   p.page_magic = ((1ull << p.page_shift) + a.page_size - 1) / a.page_size;
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  if (p.scale_log2 == 0.f) p.scale_log2 = 1e-37f;      // a masked score of minus infinity stays that
   p.arrived = static_cast<unsigned int*>(scratch);
   p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + kCounterBytes);
   p.status = status_dev;

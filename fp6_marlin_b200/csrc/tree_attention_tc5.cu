@@ -32,7 +32,7 @@ struct TreeCfg {
   static constexpr int kQBytes = kRowTile * D * 2;
   static constexpr int kStages = 4 * 128 / D;                // of keys, and of values
   static constexpr int kExchange = kRowTile * 32 * 4;        // 32 columns of a group's sums
-  static constexpr int kNumBars = 4 * kStages + 2 + 4 + 4 + 2;
+  static constexpr int kNumBars = 4 * kStages + 2 + 4 + 4 + 4;
   static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kTileBytes, kX = kV + kStages * kTileBytes;
   static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
   static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
@@ -119,11 +119,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_free + 8 * i, 1);          // tcgen05.commit: an item's last scores are computed
-      mbar_init(product + 8 * i, 1);         // tcgen05.commit: a group's weights are multiplied
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(scores + 8 * i, 1);          // [group][buffer] tcgen05.commit
       mbar_init(weights + 8 * i, 4);         // [group][buffer] the warps of the group have written weights (one per buffer: a warp may be a job ahead)
+      mbar_init(product + 8 * i, 1);         // [group][buffer] tcgen05.commit: the weights are multiplied (one per buffer: the last two products may be pending)
     }
     mbar_fence_init();
     misc[1] = 0;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             for (int i = 0; i < kKeys / 16; ++i)
               mma_tmem(tmem_o + w * 128, tmem + (w * 2 + buffer) * kKeys + i * 8, columns_desc(base + C::kV + stage * C::kTileBytes + i * 16 * 128, kKeys * 128), idesc_o,
                        i > 0 ? 1u : started >> w & 1);
-            tc_commit(product + 8 * w);
+            tc_commit(product + 8 * (w * 2 + buffer));
           }
           __syncwarp();
           started |= 1u << w;
@@ -369,24 +369,25 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             uint32_t s[kKeys];
             tmem_load32(my_scores + buffer * kKeys, s);
             tmem_load32(my_scores + buffer * kKeys + 32, s + 32);
-            // which keys the row sees: all cached ones, then those of its mask
-            unsigned long long sees = ~0ull;
             const int cached = seg.length - tile * kKeys;            // of this tile
-            if (cached < kKeys) sees = cached > 0 ? mask << cached | ((1ull << cached) - 1) : cached > -64 ? mask >> -cached : 0ull;
-            if (misc[1]) {
-              for (int i = 0; i < min(cached, kKeys); ++i)
-                if ((unsigned)page_of(p, seg, tile * kKeys + i) >= (unsigned)a.pages) sees &= ~(1ull << i);
-            }
+            const bool hidden = misc[1] != 0;
             tmem_loaded32(s);
             tmem_loaded32(s + 32);
-            // the largest of the scores that are seen; a negative scale turns the order round
-            const bool all = sees == ~0ull;
-            const bool mixed = __any_sync(0xffffffffu, !all);
-            if (mixed) {
+            if (cached < kKeys || hidden) {
+              // The row sees all cached keys, then those of its mask.  The score of another is the lowest there is: the highest, if a negative
+              // scale turns the order round (scale_log2 is never zero), so that its weight is zero.
+              unsigned long long sees = ~0ull;
+              if (cached < kKeys) sees = cached > 0 ? mask << cached | ((1ull << cached) - 1) : cached > -64 ? mask >> -cached : 0ull;
+              if (hidden) {
+                for (int i = 0; i < min(cached, kKeys); ++i)
+                  if ((unsigned)page_of(p, seg, tile * kKeys + i) >= (unsigned)a.pages) sees &= ~(1ull << i);
+              }
+              const uint32_t lowest = __float_as_uint(sl < 0.f ? INFINITY : -INFINITY);
 #pragma unroll
               for (int i = 0; i < kKeys; ++i)
-                if (!(sees >> i & 1)) s[i] = __float_as_uint(sl < 0.f ? INFINITY : -INFINITY);
+                if (!(sees >> i & 1)) s[i] = lowest;
             }
+            // the largest of the scores
             float m0 = as_float(s[0]), m1 = as_float(s[1]), m2 = as_float(s[2]), m3 = as_float(s[3]);
             if (sl >= 0.f) {
 #pragma unroll
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               }
               m0 = fminf(fminf(m0, m1), fminf(m2, m3));
             }
-            const float m = sees ? m0 * sl : -INFINITY;
+            const float m = m0 * sl;
             const bool grows = m > top + kGrowth || (top == -INFINITY && m > top);
             if (__any_sync(0xffffffffu, grows)) {
               const float now = fmaxf(top, m);
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               top = now;
               total *= keep;
               if (any) {
-                mbar_wait_bounded<20>(product + 8 * group, (job - 1) & 1, p.status, dead);
+                mbar_wait_bounded<20>(product + 8 * (group * 2 + (buffer ^ 1)), ((job - 1) >> 1) & 1, p.status, dead);
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
@@ -435,12 +436,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             for (int i = 0; i < kKeys; i += 4) {
               float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
               float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
-              if (mixed) {
-                e0 = sees >> i & 1 ? e0 : 0.f;
-                e1 = sees >> (i + 1) & 1 ? e1 : 0.f;
-                e2 = sees >> (i + 2) & 1 ? e2 : 0.f;
-                e3 = sees >> (i + 3) & 1 ? e3 : 0.f;
-              }
               t0 += e0;
               t1 += e1;
               t2 += e2;
@@ -462,7 +457,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
 
         // ---- the end of a segment
         if (any) {
-          mbar_wait_bounded<20>(product + 8 * group, (job - 1) & 1, p.status, dead);
+          mbar_wait_bounded<20>(product + 8 * (group * 2 + ((job - 1) & 1)), ((job - 1) >> 1) & 1, p.status, dead);
           tc_fence_after();
         }
         const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
