@@ -25,15 +25,18 @@ constexpr int kMostTreeCtas = 192;       // one per multiprocessor
 constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs (three idle), twice four that compute weights
 constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass
 
-template <int D_>
+template <int D_, bool PAIR_>
 struct TreeCfg {
   static constexpr int D = D_;
+  static constexpr bool kPair = PAIR_;                       // two row tiles of an item share its keys, a group each; else the groups share one row tile
   static constexpr int kTileBytes = kKeys * D * 2;           // keys or values of a tile
   static constexpr int kQBytes = kRowTile * D * 2;
-  static constexpr int kStages = 4 * 128 / D;                // of keys, and of values
+  // Tiles of keys and of values.  Values are used two tiles (of a pair: one) after their keys and given back last: with four tiles of them a key tile
+  // took at least as long as a copy (2300 cycles).
+  static constexpr int kKeyStages = 4 * 128 / D, kValueStages = (kPair ? 4 : 6) * 128 / D;
   static constexpr int kExchange = kRowTile * 32 * 4;        // 32 columns of a group's sums
-  static constexpr int kNumBars = 4 * kStages + 2 + 4 + 4 + 4;
-  static constexpr int kQ = 0, kK = 2 * kQBytes, kV = kK + kStages * kTileBytes, kX = kV + kStages * kTileBytes;
+  static constexpr int kNumBars = 2 * kKeyStages + 2 * kValueStages + 2 + 4 + 4 + 4;
+  static constexpr int kQ = 0, kK = (kPair ? 2 : 1) * kQBytes, kV = kK + kKeyStages * kTileBytes, kX = kV + kValueStages * kTileBytes;
   static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
   static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
   static constexpr int kBars = kPlaces + 4 * kKeys * 8;
@@ -94,16 +97,16 @@ __device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
 }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
 
-// kPair: two row tiles of an item share its keys, a group each; else the groups share one row tile.
-template <class T, class C, bool kPair>
+template <class T, class C>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  constexpr int D = C::D, S = C::kStages;
+  constexpr int D = C::D, SK = C::kKeyStages, SV = C::kValueStages;
+  constexpr bool kPair = C::kPair;
   constexpr int kAhead = kPair ? 1 : 2;                              // key tiles whose scores are issued before the weights of the first are there
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t base = smem_u32(smem);
-  const uint32_t full_k = base + C::kBars, empty_k = full_k + 8 * S, full_v = empty_k + 8 * S, empty_v = full_v + 8 * S;
-  const uint32_t q_free = empty_v + 8 * S, scores = q_free + 16, weights = scores + 32, product = weights + 32;
+  const uint32_t full_k = base + C::kBars, empty_k = full_k + 8 * SK, full_v = empty_k + 8 * SK, empty_v = full_v + 8 * SV;
+  const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 32, product = weights + 32;
   volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, [2, 3] last to arrive
   volatile uint32_t* odd_ring = misc + 4;                            // [segment]: infinities or NaN among its drafted values
   __shared__ long long plan[4];
@@ -111,9 +114,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   const fp6m_tree_attention_args& a = p.a;
 
   if (tid == 0) {
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < SK; ++s) {
       mbar_init(full_k + 8 * s, 64);         // the threads that copy: their copies have landed
       mbar_init(empty_k + 8 * s, 1);         // tcgen05.commit: the scores are computed
+    }
+    for (int s = 0; s < SV; ++s) {
       mbar_init(full_v + 8 * s, 64);
       mbar_init(empty_v + 8 * s, 1);
     }
@@ -149,6 +154,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   const bool works = cta < ctas;
   const long long u0 = works ? range_start(units, ctas, cta) : 0;
   bool dead = false;
+  // Up to 64 rows there is room for the queries of two items; a row tile is 128 rows all the same, what the others hold is nobody's.
+  const int q_rows = !kPair && p.rows <= 64 ? 64 : kRowTile, q_sets = !kPair && p.rows <= 64 ? 2 : 1;
+  const uint32_t q_bytes = q_rows * D * 2;                           // of a row tile; halves of a row of 128 values lie q_rows * 128 bytes apart
 
   if (works) {
     Segments seg(p, plan, u0, range_start(units, ctas, cta + 1) - u0);
@@ -166,55 +174,75 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       // Tiles of cached tokens come by tiled TMA, p.run tokens of a page at a time (0: the pages' size or the cache's layout does not allow it);
       // other tiles, sixteen bytes a thread.  (All tiles in the second way took 2500 cycles of the copying warps each.)
       auto whole_runs = [&](const Segments& s, int tile) { return p.run > 0 && (tile + 1) * kKeys <= s.length; };
-      auto look_up = [&](const Segments& s, int tile) { return page_of(p, s, tile * kKeys + (whole_runs(s, tile) ? min(me * p.run, kKeys - 1) : me)); };
       Segments ahead = seg;
       bool lives = ahead.next(p);
       int tile = ahead.t0;
-      int page = lives ? look_up(ahead, tile) : 0;                   // of this thread's run, or key, of the tile
-      int n = 0, segment = 0;
+      // The lanes of a warp keep the pages of 32 runs, and those of the next 32 are on their way.
+      const int tile_runs = p.run > 0 ? kKeys / p.run : 1, block_tiles = 32 / tile_runs, block_shift = 31 - __clz(block_tiles);
+      auto pages_of = [&](int block) {
+        const int j = (block * 32 + lane) * p.run;
+        return p.run > 0 ? page_of(p, ahead, j < ahead.length ? j : max(ahead.length - 1, 0)) : 0;
+      };
+      int n = 0, segment = 0, stage = 0, pages = 0, pages_next = 0;
+      uint32_t phase = 1;                                            // of `empty`; the first round of stages is free
       bool fresh = true;
+      const int stages = values ? SV : SK;
       while (lives) {
-        const int stage = n % S, g = ahead.item / p.parts;
+        const int g = ahead.item / p.parts;
         const uint32_t dst = ring + stage * C::kTileBytes;
         const bool runs = whole_runs(ahead, tile);
+        if (fresh && p.run > 0) {
+          pages = pages_of(tile >> block_shift);
+          pages_next = pages_of((tile >> block_shift) + 1);
+        } else if (p.run > 0 && (tile & (block_tiles - 1)) == 0) {
+          pages = pages_next;
+          pages_next = pages_of((tile >> block_shift) + 1);
+        }
         if (!runs) {
           const int j = tile * kKeys + me;
-          const T* place = place_of<T>(p, ahead, g, j, page, values);
+          const T* place = place_of<T>(p, ahead, g, j, page_of(p, ahead, j), values);
           if (!place && j < ahead.length) misc[1] = 1;
           places[(n & 1) * kKeys + me] = place;
           named_bar_sync(bar_id, 64);
         }
-        if (n >= S) mbar_wait_bounded<50>(empty + 8 * stage, (n / S + 1) & 1, p.status, dead);
+        mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
         if (values && fresh && me == 0) odd_ring[segment % kOddRing] = 0;
         if (!values && fresh) {
           // the queries of an item come with its first keys
-          const int set = kPair ? 0 : segment & 1, turn = kPair ? segment : segment >> 1;
+          const int set = segment % q_sets, turn = segment / q_sets;
           if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
           constexpr int kTiles = kPair ? 2 : 1;
           const int first_row = ahead.item % p.parts * kTiles * kRowTile;
-          for (int i = row0; i < kTiles * kRowTile; i += kRowsPerPass) {
+          for (int i = row0; i < kTiles * q_rows; i += kRowsPerPass) {
             const int r = first_row + i;
             const T* src = nullptr;
             if (r < p.rows) {
               const int t = r / p.group, head = g * p.group + (r - t * p.group);
               src = static_cast<const T*>(a.q) + ahead.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
             }
-            const uint32_t to = base + C::kQ + (kPair ? i / kRowTile : set) * C::kQBytes + (chunk >> 3) * (kRowTile * 128) + (i % kRowTile) * 128 + (((chunk & 7) ^ (i & 7)) * 16);
+            const uint32_t to = base + C::kQ + (kPair ? i / kRowTile : set) * q_bytes + (chunk >> 3) * (q_rows * 128) + (i % q_rows) * 128 + (((chunk & 7) ^ (i & 7)) * 16);
             copy16(to, src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
           }
         }
         if (runs) {
-          if (me == 0) mbar_expect_tx(full + 8 * stage, C::kTileBytes);
-          if (me < 32) {
+          const int mine = lane & (tile_runs - 1), page = __shfl_sync(0xffffffffu, pages, (tile & (block_tiles - 1)) * tile_runs + mine);
+          const int index = tile * kKeys + mine * p.run;
+          const int slot = index - (int)((unsigned long long)index * p.page_magic >> p.page_shift) * a.page_size;
+          const bool exists = (unsigned)page < (unsigned)a.pages;
+          if (!exists) misc[1] = 1;
+          const int real = exists ? page : a.pages;                  // behind the last page the copy reads zeros
+          // One lane of each warp issues copies - one warp those of the first 64 values, the other those of the second, or every other run - with
+          // operands that are uniform to the compiler.  (150 cycles each from one warp; a lane each took longer.)
+          const uint32_t bar = __shfl_sync(0xffffffffu, full + 8 * stage, 0), to = __shfl_sync(0xffffffffu, dst, 0);
+          const int head = __shfl_sync(0xffffffffu, g, 0), second = warp & 1;
+          if (second == 0 && elect_one()) mbar_expect_tx(bar, C::kTileBytes);
+          named_bar_sync(bar_id, 64);
+          constexpr int kStep = D == 128 ? 1 : 2, kHalf = D == 128 ? 64 : 0;
+#pragma unroll 2
+          for (int i = D == 128 ? 0 : second; i < tile_runs; i += kStep) {
+            const int the_slot = __shfl_sync(0xffffffffu, slot, i), the_page = __shfl_sync(0xffffffffu, real, i);
+            if (elect_one()) tma_load_run(to + (kHalf ? second : 0) * (kKeys * 128) + i * p.run * 128, map, second * kHalf, head, the_slot, the_page, bar);
             __syncwarp();
-            const int index = tile * kKeys + me * p.run;
-            if (me * p.run < kKeys) {
-              const int slot = index - (int)((unsigned long long)index * p.page_magic >> p.page_shift) * a.page_size;
-              if ((unsigned)page >= (unsigned)a.pages) misc[1] = 1;  // reads zeros
-              const int real = (unsigned)page < (unsigned)a.pages ? page : a.pages;
-#pragma unroll
-              for (int h = 0; h < D / 64; ++h) tma_load_run(dst + h * (kKeys * 128) + me * p.run * 128, map, h * 64, g, slot, real, full + 8 * stage);
-            }
           }
         } else {
 #pragma unroll 4
@@ -260,39 +288,48 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           fresh = true;
           ++segment;
         }
-        if (lives) page = look_up(ahead, tile);
+        if (++stage == stages) { stage = 0; phase ^= 1; }
       }
     } else if (warp == 4) {
       // ================================================================== MMA issuer
       constexpr uint32_t kFormats = (1u << 4) | (Half16<T>::kMmaFormat << 7) | (Half16<T>::kMmaFormat << 10) | ((uint32_t)(kRowTile >> 4) << 24);
       constexpr uint32_t idesc_s = kFormats | ((uint32_t)(kKeys >> 3) << 17);
       constexpr uint32_t idesc_o = kFormats | (1u << 16) | ((uint32_t)(D >> 3) << 17);         // values are N-major
-      Segments front = seg, back = seg;                              // of the scores, of the products
+      // What follows from the lengths is made uniform to the compiler (read from lane 0): MMAs whose operands it takes to differ between lanes
+      // cost ten times as much to issue (eight of them: 620 cycles).
+      struct Tiles {                                                 // of a segment that are left
+        Segments seg;
+        int left, groups;
+        __device__ __forceinline__ bool next(const TreeParams& p) {
+          const bool lives = seg.next(p);
+          left = __shfl_sync(0xffffffffu, lives ? seg.t1 - seg.t0 : 0, 0);
+          // of a pair of row tiles, the second may have no rows
+          groups = __shfl_sync(0xffffffffu, kPair && seg.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1, 0);
+          return left > 0;
+        }
+      };
+      Tiles front = {seg, 0, 0}, back = {seg, 0, 0};                 // of the scores, of the products
       bool front_lives = front.next(p), back_lives = back.next(p);
-      int front_tile = front.t0, back_tile = back.t0, issued = 0, multiplied = 0, segment = 0;
+      int issued = 0, multiplied = 0, segment = 0;
       int score_jobs[2] = {0, 0}, product_jobs[2] = {0, 0};
       uint32_t started = 0;                                          // groups whose sums of the segment hold something
-      auto groups_of = [&](const Segments& s) {                      // of a pair, the second may have no rows
-        return kPair && s.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1;
-      };
       while (back_lives) {
         while (front_lives && issued < multiplied + 1 + kAhead) {
-          const int stage = issued % S, set = kPair ? 0 : segment & 1;
-          mbar_wait_bounded<20>(full_k + 8 * stage, (issued / S) & 1, p.status, dead);
+          const int stage = issued % SK, set = segment % q_sets;
+          mbar_wait_bounded<20>(full_k + 8 * stage, (issued / SK) & 1, p.status, dead);
           fence_async_proxy();
           tc_fence_after();
           const uint64_t k_desc = rows_desc(base + C::kK + stage * C::kTileBytes);
-          const bool last = front_tile + 1 >= front.t1;
-          const int groups = groups_of(front);
+          const bool last = front.left == 1;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            if (kPair ? w >= groups : w != (issued & 1)) continue;
-            const uint64_t q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * C::kQBytes);
+            if (kPair ? w >= front.groups : w != (issued & 1)) continue;
+            const uint64_t q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * q_bytes);
             const int buffer = score_jobs[w] & 1;
             if (elect_one()) {
 #pragma unroll
               for (int i = 0; i < D / 16; ++i)
-                mma_smem(tmem + (w * 2 + buffer) * kKeys, q_desc + (i >> 2) * (kRowTile * 128 >> 4) + (i & 3) * 2, k_desc + (i >> 2) * (kKeys * 128 >> 4) + (i & 3) * 2, idesc_s, i);
+                mma_smem(tmem + (w * 2 + buffer) * kKeys, q_desc + (i >> 2) * (q_rows * 128 >> 4) + (i & 3) * 2, k_desc + (i >> 2) * (kKeys * 128 >> 4) + (i & 3) * 2, idesc_s, i);
               tc_commit(scores + 8 * (w * 2 + buffer));
             }
             __syncwarp();
@@ -304,19 +341,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           }
           __syncwarp();
           ++issued;
-          if (++front_tile >= front.t1) {
+          if (--front.left == 0) {
             front_lives = front.next(p);
-            front_tile = front.t0;
             ++segment;
           }
         }
-        const int stage = multiplied % S;
-        mbar_wait_bounded<20>(full_v + 8 * stage, (multiplied / S) & 1, p.status, dead);
+        const int stage = multiplied % SV;
+        mbar_wait_bounded<20>(full_v + 8 * stage, (multiplied / SV) & 1, p.status, dead);
         fence_async_proxy();
-        const int groups = groups_of(back);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          if (kPair ? w >= groups : w != (multiplied & 1)) continue;
+          if (kPair ? w >= back.groups : w != (multiplied & 1)) continue;
           const int buffer = product_jobs[w] & 1;
           mbar_wait_bounded<20>(weights + 8 * (w * 2 + buffer), (product_jobs[w] >> 1) & 1, p.status, dead);
           tc_fence_after();
@@ -334,9 +369,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         if (elect_one()) tc_commit(empty_v + 8 * stage);
         __syncwarp();
         ++multiplied;
-        if (++back_tile >= back.t1) {
+        if (--back.left == 0) {
           back_lives = back.next(p);
-          back_tile = back.t0;
           started = 0;
         }
       }
@@ -615,23 +649,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <class T, class C, bool kPair>
+template <class T, class C>
 cudaError_t launch_tc5(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(tree_attention_tc5_kernel<T, C, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  cudaError_t e = cudaFuncSetAttribute(tree_attention_tc5_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(tree_attention_tc5_kernel<T, C, kPair>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p, kmap, vmap);
+  return launch_overlapped(tree_attention_tc5_kernel<T, C>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p, kmap, vmap);
 }
 template <class T>
 cudaError_t launch_typed(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
   const bool pair = p.row_tiles > 1;
-  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64>, true>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<64>, false>(p, ctas, kmap, vmap, stream);
-  return pair ? launch_tc5<T, TreeCfg<128>, true>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<128>, false>(p, ctas, kmap, vmap, stream);
+  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64, true>>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<64, false>>(p, ctas, kmap, vmap, stream);
+  return pair ? launch_tc5<T, TreeCfg<128, true>>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<128, false>>(p, ctas, kmap, vmap, stream);
 }
 
 }  // namespace
 
 // (a CTA leaves at most two partials for each of two row tiles)
-size_t tree_tc5_partial_bytes(int sms) { return (size_t)(sms > 0 && sms < kMostTreeCtas ? sms : kMostTreeCtas) * 4 * TreeCfg<128>::kSlotFloats * sizeof(float); }
+size_t tree_tc5_partial_bytes(int sms) { return (size_t)(sms > 0 && sms < kMostTreeCtas ? sms : kMostTreeCtas) * 4 * TreeCfg<128, true>::kSlotFloats * sizeof(float); }
 
 cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream) {
   p.row_tiles = (p.rows + kRowTile - 1) / kRowTile;
