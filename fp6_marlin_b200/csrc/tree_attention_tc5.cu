@@ -601,19 +601,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         named_bar_sync(4 + which, 128);
         if (!misc[2 + which]) continue;
         __threadfence();
-        float m = -INFINITY;
+        // (two contributors at a time: what this takes is the latency of its loads)
+        float m = -INFINITY, sum = 0.f;
         odd = false;
+#pragma unroll 2
         for (int c = first_cta; c <= last_cta; ++c) {
           const float* from = slot_of(c, c == first_cta);
-          m = fmaxf(m, __ldcg(from + kRowTile * D + row_in));
+          const float cm = __ldcg(from + kRowTile * D + row_in), ct = __ldcg(from + kRowTile * (D + 1) + row_in);
           odd = odd || __ldcg(reinterpret_cast<const int*>(from) + kRowTile * (D + 2)) != 0;
+          const float now = fmaxf(m, cm), base_log2 = now == -INFINITY ? 0.f : now;
+          sum = sum * exp2_approx(m - base_log2) + ct * exp2_approx(cm - base_log2);
+          m = now;
         }
         const float base_log2 = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-        for (int c = first_cta; c <= last_cta; ++c) {
-          const float* from = slot_of(c, c == first_cta);
-          sum += __ldcg(from + kRowTile * (D + 1) + row_in) * exp2_approx(__ldcg(from + kRowTile * D + row_in) - base_log2);
-        }
         if (warp_lives) {
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
@@ -621,19 +621,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
 #pragma unroll 1
-            for (int c = first_cta; c <= last_cta; ++c) {
-              const float* from = slot_of(c, c == first_cta);
-              const float by = exp2_approx(__ldcg(from + kRowTile * D + row_in) - base_log2);
-              const float4* at = reinterpret_cast<const float4*>(from) + c0 / 4 * kRowTile + row_in;
-              float4 x[8];
+            for (int c = first_cta; c <= last_cta; c += 2) {
+              float by[2];
+              float4 x[2][8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] = __ldcg(at + i * kRowTile);
+              for (int e = 0; e < 2; ++e) {
+                const float* from = slot_of(min(c + e, last_cta), c + e == first_cta);
+                const float4* at = reinterpret_cast<const float4*>(from) + c0 / 4 * kRowTile + row_in;
+                by[e] = __ldcg(from + kRowTile * D + row_in);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                v[4 * i] = fmaf(x[i].x, by, v[4 * i]);
-                v[4 * i + 1] = fmaf(x[i].y, by, v[4 * i + 1]);
-                v[4 * i + 2] = fmaf(x[i].z, by, v[4 * i + 2]);
-                v[4 * i + 3] = fmaf(x[i].w, by, v[4 * i + 3]);
+                for (int i = 0; i < 8; ++i) x[e][i] = __ldcg(at + i * kRowTile);
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float f = c + e <= last_cta ? exp2_approx(by[e] - base_log2) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  v[4 * i] = fmaf(x[e][i].x, f, v[4 * i]);
+                  v[4 * i + 1] = fmaf(x[e][i].y, f, v[4 * i + 1]);
+                  v[4 * i + 2] = fmaf(x[e][i].z, f, v[4 * i + 2]);
+                  v[4 * i + 3] = fmaf(x[e][i].w, f, v[4 * i + 3]);
+                }
               }
             }
             put(v, c0, 1.f / sum, mask == 0 || sum == 0.f, odd);
