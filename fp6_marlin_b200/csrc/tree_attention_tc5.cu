@@ -171,43 +171,29 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       const T** places = reinterpret_cast<const T**>(smem + C::kPlaces) + (values ? 2 * kKeys : 0);
       const int bar_id = values ? 3 : 2;
       const CUtensorMap* map = values ? &vmap : &kmap;
-      // Tiles of cached tokens come by tiled TMA, p.run tokens of a page at a time (0: the pages' size or the cache's layout does not allow it);
-      // other tiles, sixteen bytes a thread.  (All tiles in the second way took 2500 cycles of the copying warps each.)
-      auto whole_runs = [&](const Segments& s, int tile) { return p.run > 0 && (tile + 1) * kKeys <= s.length; };
-      Segments ahead = seg;
-      bool lives = ahead.next(p);
-      int tile = ahead.t0;
-      // The lanes of a warp keep the pages of 32 runs, and those of the next 32 are on their way.
+      const int second = warp & 1, stages = values ? SV : SK;
+      // Tiles of cached tokens come by tiled TMA, p.run tokens of a page at a time (0: the pages' size or the cache's layout does not allow it):
+      // a warp those of the first 64 values, the other those of the second (heads of 64 values: every other run).  Other tiles, sixteen bytes a thread;
+      // all tiles in that way took 2500 cycles of the copying warps each.
+      // The first warp keeps the pages of 32 runs, a lane each, and those of the next 32 are on their way.
       const int tile_runs = p.run > 0 ? kKeys / p.run : 1, block_tiles = 32 / tile_runs, block_shift = 31 - __clz(block_tiles);
+      constexpr int kWarpRuns = D == 128 ? 1 : 2;                    // a warp issues one of so many runs
+      const uint32_t warp_bytes = p.run > 0 ? (D == 128 ? tile_runs : (tile_runs + 1 - second) / 2) * p.run * 128 : 0;
+      Segments ahead = seg;
       auto pages_of = [&](int block) {
         const int j = (block * 32 + lane) * p.run;
-        return p.run > 0 ? page_of(p, ahead, j < ahead.length ? j : max(ahead.length - 1, 0)) : 0;
+        return page_of(p, ahead, j < ahead.length ? j : max(ahead.length - 1, 0));
       };
-      int n = 0, segment = 0, stage = 0, pages = 0, pages_next = 0;
+      int stage = 0, parity = 0, segment = 0;
       uint32_t phase = 1;                                            // of `empty`; the first round of stages is free
-      bool fresh = true;
-      const int stages = values ? SV : SK;
-      while (lives) {
-        const int g = ahead.item / p.parts;
-        const uint32_t dst = ring + stage * C::kTileBytes;
-        const bool runs = whole_runs(ahead, tile);
-        if (fresh && p.run > 0) {
-          pages = pages_of(tile >> block_shift);
-          pages_next = pages_of((tile >> block_shift) + 1);
-        } else if (p.run > 0 && (tile & (block_tiles - 1)) == 0) {
-          pages = pages_next;
-          pages_next = pages_of((tile >> block_shift) + 1);
-        }
-        if (!runs) {
-          const int j = tile * kKeys + me;
-          const T* place = place_of<T>(p, ahead, g, j, page_of(p, ahead, j), values);
-          if (!place && j < ahead.length) misc[1] = 1;
-          places[(n & 1) * kKeys + me] = place;
-          named_bar_sync(bar_id, 64);
-        }
-        mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
-        if (values && fresh && me == 0) odd_ring[segment % kOddRing] = 0;
-        if (!values && fresh) {
+      while (__shfl_sync(0xffffffffu, (int)ahead.next(p), 0)) {
+        // What follows from the lengths is made uniform to the compiler (read from lane 0): copies whose operands it takes to differ between
+        // lanes cost 150 cycles each to issue.
+        const int t0 = __shfl_sync(0xffffffffu, ahead.t0, 0), t1 = __shfl_sync(0xffffffffu, ahead.t1, 0), length = __shfl_sync(0xffffffffu, ahead.length, 0);
+        const int g = __shfl_sync(0xffffffffu, ahead.item / p.parts, 0);
+        if (values) {
+          if (me == 0) odd_ring[segment % kOddRing] = 0;
+        } else {
           // the queries of an item come with its first keys
           const int set = segment % q_sets, turn = segment / q_sets;
           if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
@@ -224,36 +210,56 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             copy16(to, src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
           }
         }
+        int pages = 0, pages_next = 0, slot = 0;
+        if (p.run > 0) {
+          pages = pages_of(t0 >> block_shift);
+          pages_next = pages_of((t0 >> block_shift) + 1);
+          slot = t0 * kKeys - (int)((unsigned long long)(t0 * kKeys) * p.page_magic >> p.page_shift) * a.page_size;
+        }
+#pragma unroll 1
+        for (int tile = t0; tile < t1; ++tile) {
+        const uint32_t dst = ring + stage * C::kTileBytes, bar = full + 8 * stage;
+        const bool runs = p.run > 0 && (tile + 1) * kKeys <= length;
+        const bool drafted = values && (tile + 1) * kKeys > length;
         if (runs) {
-          const int mine = lane & (tile_runs - 1), page = __shfl_sync(0xffffffffu, pages, (tile & (block_tiles - 1)) * tile_runs + mine);
-          const int index = tile * kKeys + mine * p.run;
-          const int slot = index - (int)((unsigned long long)index * p.page_magic >> p.page_shift) * a.page_size;
-          const bool exists = (unsigned)page < (unsigned)a.pages;
-          if (!exists) misc[1] = 1;
-          const int real = exists ? page : a.pages;                  // behind the last page the copy reads zeros
-          // One lane of each warp issues copies - one warp those of the first 64 values, the other those of the second, or every other run - with
-          // operands that are uniform to the compiler.  (150 cycles each from one warp; a lane each took longer.)
-          const uint32_t bar = __shfl_sync(0xffffffffu, full + 8 * stage, 0), to = __shfl_sync(0xffffffffu, dst, 0);
-          const int head = __shfl_sync(0xffffffffu, g, 0), second = warp & 1;
-          if (second == 0 && elect_one()) mbar_expect_tx(bar, C::kTileBytes);
-          named_bar_sync(bar_id, 64);
-          constexpr int kStep = D == 128 ? 1 : 2, kHalf = D == 128 ? 64 : 0;
-#pragma unroll 2
-          for (int i = D == 128 ? 0 : second; i < tile_runs; i += kStep) {
-            const int the_slot = __shfl_sync(0xffffffffu, slot, i), the_page = __shfl_sync(0xffffffffu, real, i);
-            if (elect_one()) tma_load_run(to + (kHalf ? second : 0) * (kKeys * 128) + i * p.run * 128, map, second * kHalf, head, the_slot, the_page, bar);
-            __syncwarp();
+          const int at = tile & (block_tiles - 1);
+          if (at == 0 && tile != t0) {
+            pages = pages_next;
+            pages_next = pages_of((tile >> block_shift) + 1);
+          }
+          mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
+          if (elect_one()) mbar_expect_tx(bar, warp_bytes);
+          __syncwarp();
+#pragma unroll 1
+          for (int i = 0; i < tile_runs; ++i) {
+            int page = __shfl_sync(0xffffffffu, pages, at * tile_runs + i);
+            if ((unsigned)page >= (unsigned)a.pages) {
+              misc[1] = 1;
+              page = a.pages;                                        // behind the last page the copy reads zeros
+            }
+            if (kWarpRuns == 1 || (i & 1) == second) {
+              if (elect_one()) tma_load_run(dst + (D == 128 ? second : 0) * (kKeys * 128) + i * p.run * 128, map, D == 128 ? second * 64 : 0, g, slot, page, bar);
+              __syncwarp();
+            }
+            slot += p.run;
+            if (slot == a.page_size) slot = 0;
           }
         } else {
+          const int j = tile * kKeys + me;
+          const T* place = place_of<T>(p, ahead, g, j, page_of(p, ahead, j), values);
+          if (!place && j < length) misc[1] = 1;
+          places[parity * kKeys + me] = place;
+          named_bar_sync(bar_id, 64);
+          mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
 #pragma unroll 4
           for (int i = 0; i < kPasses; ++i) {
             const int row = row0 + i * kRowsPerPass;
-            const T* src = places[(n & 1) * kKeys + row];
+            const T* src = places[parity * kKeys + row];
             copy16(dst + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
           }
+          parity ^= 1;
         }
-        const bool drafted = values && tile * kKeys + kKeys > ahead.length;
-        if (!drafted) copies_arrive(full + 8 * stage);
+        if (!drafted) copies_arrive(bar);
         if (drafted) {
           // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
           // that see them at the end.
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           named_bar_sync(bar_id, 64);
           const int j = tile * kKeys + me;
           bool odd = false;
-          if (j >= ahead.length) {
+          if (j >= length) {
             for (int c = 0; c < D / 8; ++c) {
               const uint32_t at = dst + (c >> 3) * (kKeys * 128) + me * 128 + (((c & 7) ^ (me & 7)) * 16);
               uint4 w = lds128(at);
@@ -278,17 +284,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             }
           }
           if (odd) odd_ring[segment % kOddRing] = 1;
-          mbar_arrive(full + 8 * stage);
-        }
-        ++n;
-        fresh = false;
-        if (++tile >= ahead.t1) {
-          lives = ahead.next(p);
-          tile = ahead.t0;
-          fresh = true;
-          ++segment;
+          mbar_arrive(bar);
         }
         if (++stage == stages) { stage = 0; phase ^= 1; }
+        }
+        ++segment;
       }
     } else if (warp == 4) {
       // ================================================================== MMA issuer
@@ -299,25 +299,31 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       // cost ten times as much to issue (eight of them: 620 cycles).
       struct Tiles {                                                 // of a segment that are left
         Segments seg;
-        int left, groups;
+        int left, plain, groups;                                     // of them, those that TMA brings
         __device__ __forceinline__ bool next(const TreeParams& p) {
           const bool lives = seg.next(p);
           left = __shfl_sync(0xffffffffu, lives ? seg.t1 - seg.t0 : 0, 0);
+          plain = p.run > 0 ? __shfl_sync(0xffffffffu, min(seg.t1, seg.length / kKeys) - seg.t0, 0) : 0;
           // of a pair of row tiles, the second may have no rows
           groups = __shfl_sync(0xffffffffu, kPair && seg.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1, 0);
           return left > 0;
         }
       };
-      Tiles front = {seg, 0, 0}, back = {seg, 0, 0};                 // of the scores, of the products
+      Tiles front = {seg, 0, 0, 0}, back = {seg, 0, 0, 0};                 // of the scores, of the products
       bool front_lives = front.next(p), back_lives = back.next(p);
-      int issued = 0, multiplied = 0, segment = 0;
+      int issued = 0, multiplied = 0, segment = 0, k_stage = 0, v_stage = 0;
+      uint32_t k_phase = 0, v_phase = 0;
+      bool first = true;                                             // of a segment: the queries come with it, by other copies
       int score_jobs[2] = {0, 0}, product_jobs[2] = {0, 0};
       uint32_t started = 0;                                          // groups whose sums of the segment hold something
       while (back_lives) {
         while (front_lives && issued < multiplied + 1 + kAhead) {
-          const int stage = issued % SK, set = segment % q_sets;
-          mbar_wait_bounded<20>(full_k + 8 * stage, (issued / SK) & 1, p.status, dead);
-          fence_async_proxy();
+          const int stage = k_stage, set = q_sets == 2 ? segment & 1 : 0;
+          mbar_wait_bounded<20>(full_k + 8 * stage, k_phase, p.status, dead);
+          if (first || front.plain <= 0) fence_async_proxy();
+          first = false;
+          --front.plain;
+          if (++k_stage == SK) { k_stage = 0; k_phase ^= 1; }
           tc_fence_after();
           const uint64_t k_desc = rows_desc(base + C::kK + stage * C::kTileBytes);
           const bool last = front.left == 1;
@@ -343,12 +349,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           ++issued;
           if (--front.left == 0) {
             front_lives = front.next(p);
+            first = true;
             ++segment;
           }
         }
-        const int stage = multiplied % SV;
-        mbar_wait_bounded<20>(full_v + 8 * stage, (multiplied / SV) & 1, p.status, dead);
-        fence_async_proxy();
+        const int stage = v_stage;
+        mbar_wait_bounded<20>(full_v + 8 * stage, v_phase, p.status, dead);
+        if (back.plain-- <= 0) fence_async_proxy();
+        if (++v_stage == SV) { v_stage = 0; v_phase ^= 1; }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           if (kPair ? w >= back.groups : w != (multiplied & 1)) continue;
