@@ -1,11 +1,12 @@
 // Attention over a paged cache for more than 32 rows per head of keys, on tcgen05 (fewer rows, and what is computed: tree_attention.cu).
 //
-// A row tile of 128 rows is the M dimension: scores S (128 x 64 keys) = Q K^T with both operands in shared memory, then
-// O (128 x head_dim) += P V with the weights P as the operand in tensor memory, written over S in 16 bits, and V as it lies (keys
+// A row tile of 128 rows is the M dimension: scores S (128 x 128 keys, two key tiles: a job) = Q K^T with both operands in shared memory,
+// then O (128 x head_dim) += P V with the weights P as the operand in tensor memory, written over S in 16 bits, and V as it lies (keys
 // in rows, so its operand is "transposed").  A thread owns a row: no exchange between threads for maxima and sums.  Two groups of four warps
-// compute weights in turn; each has two score tiles, so that the tensor cores work on the next scores of one and the product of
-// the other meanwhile.  More than 128 rows: a group for each of two row tiles, which share the keys in shared memory.  Up to 128 rows: the
-// groups take the key tiles in turn and their sums are joined at the end.
+// compute weights, so that the tensor cores work on the product and the next scores of one while the other computes.  More than 128 rows: a group
+// for each of two row tiles, which share the keys in shared memory.  Up to 128 rows: the groups take the jobs in turn and their sums
+// are joined at the end.  (Jobs of 64 keys with two score tiles per group: the MMAs of 64 columns take 77 cycles each in place of 64 for 128,
+// and what is passed between the warps, about 1300 cycles a job, bound the kernel.)
 //
 // O is rescaled only where a row's maximum grows by more than a factor of 2^8: until then the weights are taken relative to the older
 // maximum, which changes neither the result nor, in fp32 sums and 16-bit floating-point weights, its precision.
@@ -31,12 +32,12 @@ struct TreeCfg {
   static constexpr bool kPair = PAIR_;                       // two row tiles of an item share its keys, a group each; else the groups share one row tile
   static constexpr int kTileBytes = kKeys * D * 2;           // keys or values of a tile
   static constexpr int kQBytes = kRowTile * D * 2;
-  // Tiles of keys and of values.  Values are used two tiles (of a pair: one) after their keys and given back last: with four tiles of them a key tile
-  // took at least as long as a copy (2300 cycles).
-  static constexpr int kKeyStages = 4 * 128 / D, kValueStages = (kPair ? 4 : 6) * 128 / D;
+  // Stages of keys and of values, a job each.  Values are used later than their keys.
+  static constexpr int kKeyStages = 2 * 128 / D, kValueStages = (kPair ? 2 : 3) * 128 / D;
+  static constexpr int kStageBytes = 2 * kTileBytes, kHalfBytes = 2 * kKeys * 128;     // [half of a row][128 keys][64 values]
   static constexpr int kExchange = kRowTile * 32 * 4;        // 32 columns of a group's sums
-  static constexpr int kNumBars = 2 * kKeyStages + 2 * kValueStages + 2 + 4 + 4 + 4;
-  static constexpr int kQ = 0, kK = (kPair ? 2 : 1) * kQBytes, kV = kK + kKeyStages * kTileBytes, kX = kV + kValueStages * kTileBytes;
+  static constexpr int kNumBars = 2 * kKeyStages + 2 * kValueStages + 2 + 2 + 2 + 2;
+  static constexpr int kQ = 0, kK = (kPair ? 2 : 1) * kQBytes, kV = kK + kKeyStages * kStageBytes, kX = kV + kValueStages * kStageBytes;
   static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
   static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
   static constexpr int kBars = kPlaces + 4 * kKeys * 8;
@@ -82,31 +83,36 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
         "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-      "%28,%29,%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+               : "memory");
 }
 // waits for the loads; the registers pass through, so that nothing that uses them can be moved in front of the wait
-__device__ __forceinline__ void tmem_loaded32(uint32_t* r) {
+template <int kCount>
+__device__ __forceinline__ void tmem_loaded(uint32_t* r) {
   tc_wait_ld();
 #pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+  for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(r[i]));
 }
+__device__ __forceinline__ void tmem_loaded32(uint32_t* r) { tmem_loaded<32>(r); }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
 
 template <class T, class C>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   constexpr int D = C::D, SK = C::kKeyStages, SV = C::kValueStages;
   constexpr bool kPair = C::kPair;
-  constexpr int kAhead = kPair ? 1 : 2;                              // key tiles whose scores are issued before the weights of the first are there
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t base = smem_u32(smem);
   const uint32_t full_k = base + C::kBars, empty_k = full_k + 8 * SK, full_v = empty_k + 8 * SK, empty_v = full_v + 8 * SV;
-  const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 32, product = weights + 32;
+  const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 16, product = weights + 16;
   volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, [2, 3] last to arrive
   volatile uint32_t* odd_ring = misc + 4;                            // [segment]: infinities or NaN among its drafted values
   __shared__ long long plan[4];
@@ -115,20 +121,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
 
   if (tid == 0) {
     for (int s = 0; s < SK; ++s) {
-      mbar_init(full_k + 8 * s, 64);         // the threads that copy: their copies have landed
+      mbar_init(full_k + 8 * s, 128);        // the threads that copy, once for each of two key tiles: their copies have landed
       mbar_init(empty_k + 8 * s, 1);         // tcgen05.commit: the scores are computed
     }
     for (int s = 0; s < SV; ++s) {
-      mbar_init(full_v + 8 * s, 64);
+      mbar_init(full_v + 8 * s, 128);
       mbar_init(empty_v + 8 * s, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_free + 8 * i, 1);          // tcgen05.commit: an item's last scores are computed
-    }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(scores + 8 * i, 1);          // [group][buffer] tcgen05.commit
-      mbar_init(weights + 8 * i, 4);         // [group][buffer] the warps of the group have written weights (one per buffer: a warp may be a job ahead)
-      mbar_init(product + 8 * i, 1);         // [group][buffer] tcgen05.commit: the weights are multiplied (one per buffer: the last two products may be pending)
+      mbar_init(scores + 8 * i, 1);          // [group] tcgen05.commit
+      mbar_init(weights + 8 * i, 4);         // [group] its warps have written the weights of a job
+      mbar_init(product + 8 * i, 1);         // [group] tcgen05.commit: a segment's last weights are multiplied
     }
     mbar_fence_init();
     misc[1] = 0;
@@ -218,7 +222,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         }
 #pragma unroll 1
         for (int tile = t0; tile < t1; ++tile) {
-        const uint32_t dst = ring + stage * C::kTileBytes, bar = full + 8 * stage;
+        const int odd_tile = (tile - t0) & 1;
+        const uint32_t dst = ring + stage * C::kStageBytes + odd_tile * (kKeys * 128), bar = full + 8 * stage;
         const bool runs = p.run > 0 && (tile + 1) * kKeys <= length;
         const bool drafted = values && (tile + 1) * kKeys > length;
         if (runs) {
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             pages = pages_next;
             pages_next = pages_of((tile >> block_shift) + 1);
           }
-          mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
+          if (!odd_tile) mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
           if (elect_one()) mbar_expect_tx(bar, warp_bytes);
           __syncwarp();
 #pragma unroll 1
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               page = a.pages;                                        // behind the last page the copy reads zeros
             }
             if (kWarpRuns == 1 || (i & 1) == second) {
-              if (elect_one()) tma_load_run(dst + (D == 128 ? second : 0) * (kKeys * 128) + i * p.run * 128, map, D == 128 ? second * 64 : 0, g, slot, page, bar);
+              if (elect_one()) tma_load_run(dst + (D == 128 ? second : 0) * C::kHalfBytes + i * p.run * 128, map, D == 128 ? second * 64 : 0, g, slot, page, bar);
               __syncwarp();
             }
             slot += p.run;
@@ -250,12 +255,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           if (!place && j < length) misc[1] = 1;
           places[parity * kKeys + me] = place;
           named_bar_sync(bar_id, 64);
-          mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
+          if (!odd_tile) mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
 #pragma unroll 4
           for (int i = 0; i < kPasses; ++i) {
             const int row = row0 + i * kRowsPerPass;
             const T* src = places[parity * kKeys + row];
-            copy16(dst + (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
+            copy16(dst + (chunk >> 3) * C::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
           }
           parity ^= 1;
         }
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           bool odd = false;
           if (j >= length) {
             for (int c = 0; c < D / 8; ++c) {
-              const uint32_t at = dst + (c >> 3) * (kKeys * 128) + me * 128 + (((c & 7) ^ (me & 7)) * 16);
+              const uint32_t at = dst + (c >> 3) * C::kHalfBytes + me * 128 + (((c & 7) ^ (me & 7)) * 16);
               uint4 w = lds128(at);
               if (is_odd<T>(w.x) || is_odd<T>(w.y) || is_odd<T>(w.z) || is_odd<T>(w.w)) {
                 odd = true;
@@ -286,20 +291,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           if (odd) odd_ring[segment % kOddRing] = 1;
           mbar_arrive(bar);
         }
-        if (++stage == stages) { stage = 0; phase ^= 1; }
+        if (!odd_tile && tile + 1 == t1) mbar_arrive(bar);           // for the second tile that the job does not have
+        if ((odd_tile || tile + 1 == t1) && ++stage == stages) { stage = 0; phase ^= 1; }
         }
         ++segment;
       }
     } else if (warp == 4) {
       // ================================================================== MMA issuer
       constexpr uint32_t kFormats = (1u << 4) | (Half16<T>::kMmaFormat << 7) | (Half16<T>::kMmaFormat << 10) | ((uint32_t)(kRowTile >> 4) << 24);
-      constexpr uint32_t idesc_s = kFormats | ((uint32_t)(kKeys >> 3) << 17);
+      constexpr uint32_t idesc_s = kFormats | ((uint32_t)(kKeys >> 3) << 17), idesc_s2 = kFormats | ((uint32_t)(2 * kKeys >> 3) << 17);
       constexpr uint32_t idesc_o = kFormats | (1u << 16) | ((uint32_t)(D >> 3) << 17);         // values are N-major
-      // What follows from the lengths is made uniform to the compiler (read from lane 0): MMAs whose operands it takes to differ between lanes
-      // cost ten times as much to issue (eight of them: 620 cycles).
-      struct Tiles {                                                 // of a segment that are left
+      // What follows from the lengths is made uniform to the compiler (read from lane 0), so that MMAs are issued with uniform operands.
+      struct Jobs {
         Segments seg;
-        int left, plain, groups;                                     // of them, those that TMA brings
+        int left, plain, groups;                                     // key tiles of the segment that are left, of them those that TMA brings; groups
+        int stage;
+        uint32_t phase;
         __device__ __forceinline__ bool next(const TreeParams& p) {
           const bool lives = seg.next(p);
           left = __shfl_sync(0xffffffffu, lives ? seg.t1 - seg.t0 : 0, 0);
@@ -308,89 +315,106 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           groups = __shfl_sync(0xffffffffu, kPair && seg.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1, 0);
           return left > 0;
         }
-      };
-      Tiles front = {seg, 0, 0, 0}, back = {seg, 0, 0, 0};                 // of the scores, of the products
-      bool front_lives = front.next(p), back_lives = back.next(p);
-      int issued = 0, multiplied = 0, segment = 0, k_stage = 0, v_stage = 0;
-      uint32_t k_phase = 0, v_phase = 0;
-      bool first = true;                                             // of a segment: the queries come with it, by other copies
-      int score_jobs[2] = {0, 0}, product_jobs[2] = {0, 0};
-      uint32_t started = 0;                                          // groups whose sums of the segment hold something
-      while (back_lives) {
-        while (front_lives && issued < multiplied + 1 + kAhead) {
-          const int stage = k_stage, set = q_sets == 2 ? segment & 1 : 0;
-          mbar_wait_bounded<20>(full_k + 8 * stage, k_phase, p.status, dead);
-          if (first || front.plain <= 0) fence_async_proxy();
-          first = false;
-          --front.plain;
-          if (++k_stage == SK) { k_stage = 0; k_phase ^= 1; }
+        // waits for the next stage; other copies than TMA's (the queries come with a segment's first) need a proxy fence
+        __device__ __forceinline__ void wait(uint32_t full, bool other_copies, int* status, bool& dead) {
+          mbar_wait_bounded<20>(full + 8 * stage, phase, status, dead);
+          if (other_copies || plain < min(left, 2)) fence_async_proxy();
           tc_fence_after();
-          const uint64_t k_desc = rows_desc(base + C::kK + stage * C::kTileBytes);
-          const bool last = front.left == 1;
+        }
+        __device__ __forceinline__ bool advance(const TreeParams& p, int stages) {
+          if (++stage == stages) { stage = 0; phase ^= 1; }
+          left -= 2;
+          plain -= 2;
+          return left > 0 || next(p);
+        }
+      };
+      Jobs front = {seg, 0, 0, 0, 0, 0}, back = front;               // of the scores, of the products
+      bool front_lives = front.next(p), back_lives = back.next(p), fresh = true;       // fresh: a segment's first scores
+      int segment = 0, scored = 0, multiplied = 0, part = 0;         // jobs; the group whose scores of the front job are next
+      uint32_t weight_phase = 0, started = 0;                        // of both groups, a bit each; groups whose sums of the segment hold something
+      // scores of the front job for group w; the job is done with the last group's
+      auto issue_scores = [&](int w) {
+        const int set = q_sets == 2 ? segment & 1 : 0;
+        if (!kPair || w == 0) front.wait(full_k, fresh, p.status, dead);
+        fresh = false;
+        const uint64_t k_desc = rows_desc(base + C::kK + front.stage * C::kStageBytes), q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * q_bytes);
+        const uint32_t idesc = front.left > 1 ? idesc_s2 : idesc_s;
+        const bool whole_job = !kPair || w + 1 == front.groups;
+        if (elect_one()) {
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (kPair ? w >= front.groups : w != (issued & 1)) continue;
-            const uint64_t q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * q_bytes);
-            const int buffer = score_jobs[w] & 1;
-            if (elect_one()) {
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i)
-                mma_smem(tmem + (w * 2 + buffer) * kKeys, q_desc + (i >> 2) * (q_rows * 128 >> 4) + (i & 3) * 2, k_desc + (i >> 2) * (kKeys * 128 >> 4) + (i & 3) * 2, idesc_s, i);
-              tc_commit(scores + 8 * (w * 2 + buffer));
-            }
-            __syncwarp();
-            ++score_jobs[w];
-          }
-          if (elect_one()) {
-            tc_commit(empty_k + 8 * stage);
-            if (last) tc_commit(q_free + 8 * set);
-          }
-          __syncwarp();
-          ++issued;
-          if (--front.left == 0) {
-            front_lives = front.next(p);
-            first = true;
-            ++segment;
+          for (int i = 0; i < D / 16; ++i)
+            mma_smem(tmem + w * 128, q_desc + (i >> 2) * (q_rows * 128 >> 4) + (i & 3) * 2, k_desc + (i >> 2) * (C::kHalfBytes >> 4) + (i & 3) * 2, idesc, i);
+          tc_commit(scores + 8 * w);
+          if (whole_job) {
+            tc_commit(empty_k + 8 * front.stage);
+            if (front.left <= 2) tc_commit(q_free + 8 * set);
           }
         }
-        const int stage = v_stage;
-        mbar_wait_bounded<20>(full_v + 8 * stage, v_phase, p.status, dead);
-        if (back.plain-- <= 0) fence_async_proxy();
-        if (++v_stage == SV) { v_stage = 0; v_phase ^= 1; }
+        __syncwarp();
+        part = whole_job ? 0 : w + 1;
+        if (whole_job) {
+          ++scored;
+          if (front.left <= 2) {
+            ++segment;
+            fresh = true;
+          }
+          front_lives = front.advance(p, SK);
+        }
+      };
+      if constexpr (kPair) {
+        if (front_lives) {                                           // (a range may hold nothing but the overhead of an item)
+          do issue_scores(part); while (part);
+        }
+      } else {
+        for (int i = 0; i < 2 && front_lives; ++i) issue_scores(scored & 1);
+      }
+      while (back_lives) {
+        back.wait(full_v, false, p.status, dead);
+        const uint64_t v_desc = columns_desc(base + C::kV + back.stage * C::kStageBytes, C::kHalfBytes);
+        // the group's last job of the segment
+        const bool last = kPair ? back.left <= 2 : back.left <= 4;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           if (kPair ? w >= back.groups : w != (multiplied & 1)) continue;
-          const int buffer = product_jobs[w] & 1;
-          mbar_wait_bounded<20>(weights + 8 * (w * 2 + buffer), (product_jobs[w] >> 1) & 1, p.status, dead);
+          mbar_wait_bounded<20>(weights + 8 * w, weight_phase >> w & 1, p.status, dead);
+          weight_phase ^= 1u << w;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < kKeys / 16; ++i)
-              mma_tmem(tmem_o + w * 128, tmem + (w * 2 + buffer) * kKeys + i * 8, columns_desc(base + C::kV + stage * C::kTileBytes + i * 16 * 128, kKeys * 128), idesc_o,
-                       i > 0 ? 1u : started >> w & 1);
-            tc_commit(product + 8 * (w * 2 + buffer));
+            for (int i = 0; i < 2 * kKeys / 16; ++i)
+              if (i < kKeys / 16 || back.left > 1) mma_tmem(tmem_o + w * 128, tmem + w * 128 + i * 8, v_desc + i * (16 * 128 >> 4), idesc_o, i > 0 ? 1u : started >> w & 1);
+            if (last) tc_commit(product + 8 * w);
+            if (!kPair || w + 1 == back.groups) tc_commit(empty_v + 8 * back.stage);
           }
           __syncwarp();
           started |= 1u << w;
-          ++product_jobs[w];
+          // the group's next scores, over the weights that the product has read by then
+          if (front_lives && (!kPair || part == w)) {
+            if constexpr (kPair) {
+              // (the front job is the one behind this: not that of the next turn)
+              if (scored == multiplied + 1) issue_scores(w);
+            } else {
+              issue_scores(w);
+            }
+          }
         }
-        if (elect_one()) tc_commit(empty_v + 8 * stage);
-        __syncwarp();
+        if constexpr (kPair) {
+          while (part) issue_scores(part);
+        }
         ++multiplied;
-        if (--back.left == 0) {
-          back_lives = back.next(p);
-          started = 0;
-        }
+        const bool segment_ends = back.left <= 2;
+        back_lives = back.advance(p, SV);
+        if (segment_ends) started = 0;
       }
     } else if (warp >= 8) {
       // ================================================================== weights: thread = row
       const int group = (warp - 8) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane;
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-      const uint32_t my_scores = tmem + lanes + group * 2 * kKeys, my_sums = tmem_o + lanes + group * 128;
+      const uint32_t my_scores = tmem + lanes + group * 128, my_sums = tmem_o + lanes + group * 128;
       const float sl = p.scale_log2;
       float* stats = reinterpret_cast<float*>(smem + C::kStats);
       float4* exchange = reinterpret_cast<float4*>(smem + C::kX);
-      int job = 0, n = 0, segment = -1;                              // jobs of this group, tiles of the CTA
+      int job = 0, n = 0, segment = -1, ended = 0;                   // jobs of this group, jobs of the CTA; segments that this group has jobs of
       while (seg.next(p)) {
         ++segment;
         const int g = seg.item / p.parts, row_tile = kPair ? seg.item % p.parts * 2 + group : seg.item % p.parts;
@@ -402,54 +426,70 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         float top = -INFINITY, total = 0.f;                          // the maximum that the weights are relative to
         bool any = false;                                            // the sums hold something
         const bool group_lives = !kPair || row_tile < p.row_tiles;
-        for (int tile = seg.t0; tile < seg.t1; ++tile, ++n) {
+        for (int tile = seg.t0; tile < seg.t1; tile += 2, ++n) {
           if (!group_lives || (!kPair && (n & 1) != group)) continue;
-          const int buffer = job & 1;
-          mbar_wait_bounded<20>(scores + 8 * (group * 2 + buffer), (job >> 1) & 1, p.status, dead);
+          mbar_wait_bounded<20>(scores + 8 * group, job & 1, p.status, dead);
           tc_fence_after();
           if (warp_lives) {
-            uint32_t s[kKeys];
-            tmem_load32(my_scores + buffer * kKeys, s);
-            tmem_load32(my_scores + buffer * kKeys + 32, s + 32);
-            const int cached = seg.length - tile * kKeys;            // of this tile
-            const bool hidden = misc[1] != 0;
-            tmem_loaded32(s);
-            tmem_loaded32(s + 32);
-            if (cached < kKeys || hidden) {
-              // The row sees all cached keys, then those of its mask.  The score of another is the lowest there is: the highest, if a negative
-              // scale turns the order round (scale_log2 is never zero), so that its weight is zero.
-              unsigned long long sees = ~0ull;
-              if (cached < kKeys) sees = cached > 0 ? mask << cached | ((1ull << cached) - 1) : cached > -64 ? mask >> -cached : 0ull;
-              if (hidden) {
-                for (int i = 0; i < min(cached, kKeys); ++i)
-                  if ((unsigned)page_of(p, seg, tile * kKeys + i) >= (unsigned)a.pages) sees &= ~(1ull << i);
-              }
-              const uint32_t lowest = __float_as_uint(sl < 0.f ? INFINITY : -INFINITY);
+            const int chunks = tile + 1 < seg.t1 ? 4 : 2;            // of 32 keys
+            // The row sees all cached keys, then those of its mask.  The score of another is the lowest there is: the highest, if a negative
+            // scale turns the order round (scale_log2 is never zero), so that its weight is zero.
+            const int cached = seg.length - tile * kKeys;            // from the job's first key on
+            const bool hidden = misc[1] != 0, masked = cached < chunks * 32 || hidden;
+            const uint32_t lowest = __float_as_uint(sl < 0.f ? INFINITY : -INFINITY);
+            uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
+            if (masked) {
 #pragma unroll
-              for (int i = 0; i < kKeys; ++i)
-                if (!(sees >> i & 1)) s[i] = lowest;
+              for (int h = 0; h < 2; ++h) {
+                const int here = cached - h * kKeys;
+                unsigned long long word = ~0ull;
+                if (here < kKeys) word = here > 0 ? mask << here | ((1ull << here) - 1) : here > -64 ? mask >> -here : 0ull;
+                if (hidden) {
+                  for (int i = 0; i < min(here, kKeys); ++i)
+                    if ((unsigned)page_of(p, seg, (tile + h) * kKeys + i) >= (unsigned)a.pages) word &= ~(1ull << i);
+                }
+                sees[2 * h] = (uint32_t)word;
+                sees[2 * h + 1] = (uint32_t)(word >> 32);
+              }
             }
-            // the largest of the scores
-            float m0 = as_float(s[0]), m1 = as_float(s[1]), m2 = as_float(s[2]), m3 = as_float(s[3]);
-            if (sl >= 0.f) {
+            auto hide = [&](uint32_t* v, int c) {
+              if (masked) {
 #pragma unroll
-              for (int i = 4; i < kKeys; i += 4) {
-                m0 = fmaxf(m0, as_float(s[i]));
-                m1 = fmaxf(m1, as_float(s[i + 1]));
-                m2 = fmaxf(m2, as_float(s[i + 2]));
-                m3 = fmaxf(m3, as_float(s[i + 3]));
+                for (int i = 0; i < 32; ++i)
+                  if (!(sees[c] >> i & 1)) v[i] = lowest;
               }
-              m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-            } else {
+            };
+            // the largest of the scores; they are read once more below, because 128 of them would not stay in registers
+            uint32_t v[2][32];
+            float m0 = as_float(lowest), m1 = m0, m2 = m0, m3 = m0;
+            tmem_load32(my_scores, v[0]);
 #pragma unroll
-              for (int i = 4; i < kKeys; i += 4) {
-                m0 = fminf(m0, as_float(s[i]));
-                m1 = fminf(m1, as_float(s[i + 1]));
-                m2 = fminf(m2, as_float(s[i + 2]));
-                m3 = fminf(m3, as_float(s[i + 3]));
+            for (int c = 0; c < 4; ++c) {
+              if (c >= chunks) break;
+              tmem_loaded32(v[c & 1]);
+              if (c + 1 < chunks) tmem_load32(my_scores + 32 * (c + 1), v[(c + 1) & 1]);
+              uint32_t* s = v[c & 1];
+              hide(s, c);
+              if (sl >= 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  m0 = fmaxf(m0, as_float(s[i]));
+                  m1 = fmaxf(m1, as_float(s[i + 1]));
+                  m2 = fmaxf(m2, as_float(s[i + 2]));
+                  m3 = fmaxf(m3, as_float(s[i + 3]));
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  m0 = fminf(m0, as_float(s[i]));
+                  m1 = fminf(m1, as_float(s[i + 1]));
+                  m2 = fminf(m2, as_float(s[i + 2]));
+                  m3 = fminf(m3, as_float(s[i + 3]));
+                }
               }
-              m0 = fminf(fminf(m0, m1), fminf(m2, m3));
             }
+            tmem_load32(my_scores, v[0]);
+            m0 = sl >= 0.f ? fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) : fminf(fminf(m0, m1), fminf(m2, m3));
             const float m = m0 * sl;
             const bool grows = m > top + kGrowth || (top == -INFINITY && m > top);
             if (__any_sync(0xffffffffu, grows)) {
@@ -458,48 +498,55 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               top = now;
               total *= keep;
               if (any) {
-                mbar_wait_bounded<20>(product + 8 * (group * 2 + (buffer ^ 1)), ((job - 1) >> 1) & 1, p.status, dead);
-                tc_fence_after();
+                // (the product before these scores is done: the tensor cores work in the order of issue)
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tmem_load32(my_sums + c, o);
-                  tmem_loaded32(o);
+                for (int c = 0; c < D; c += 16) {
+                  uint32_t o[16];
+                  tmem_load16(my_sums + c, o);
+                  tmem_loaded<16>(o);
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
-                  tmem_store32(my_sums + c, o);
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
+                  tmem_store16(my_sums + c, o);
                 }
               }
             }
             const float base_log2 = top == -INFINITY ? 0.f : top;
             float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
-            uint32_t w[32];
 #pragma unroll
-            for (int i = 0; i < kKeys; i += 4) {
-              float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
-              float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
-              t0 += e0;
-              t1 += e1;
-              t2 += e2;
-              t3 += e3;
-              w[i / 2] = Half16<T>::pack(e0, e1);
-              w[i / 2 + 1] = Half16<T>::pack(e2, e3);
+            for (int c = 0; c < 4; ++c) {
+              if (c >= chunks) break;
+              tmem_loaded32(v[c & 1]);
+              if (c + 1 < chunks) tmem_load32(my_scores + 32 * (c + 1), v[(c + 1) & 1]);
+              uint32_t* s = v[c & 1];
+              hide(s, c);
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
+                const float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
+                t0 += e0;
+                t1 += e1;
+                t2 += e2;
+                t3 += e3;
+                w[i / 2] = Half16<T>::pack(e0, e1);
+                w[i / 2 + 1] = Half16<T>::pack(e2, e3);
+              }
+              tmem_store16(my_scores + 16 * c, w);                   // over scores that have been read
             }
             total += (t0 + t1) + (t2 + t3);
-            tmem_store32(my_scores + buffer * kKeys, w);
             tc_wait_st();
           }
           any = true;
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(weights + 8 * (group * 2 + buffer));
+          if (lane == 0) mbar_arrive(weights + 8 * group);
           ++job;
         }
         if (kPair && !group_lives) continue;
 
         // ---- the end of a segment
         if (any) {
-          mbar_wait_bounded<20>(product + 8 * (group * 2 + ((job - 1) & 1)), ((job - 1) >> 1) & 1, p.status, dead);
+          mbar_wait_bounded<20>(product + 8 * group, ended++ & 1, p.status, dead);
           tc_fence_after();
         }
         const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
