@@ -452,73 +452,69 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
                 sees[2 * h + 1] = (uint32_t)(word >> 32);
               }
             }
-            auto hide = [&](uint32_t* v, int c) {
+            float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
+            // 32 scores to weights, relative to the maximum that has been let stand so far
+            auto weigh = [&](uint32_t* s, int c) {
               if (masked) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (!(sees[c] >> i & 1)) v[i] = lowest;
+                  if (!(sees[c] >> i & 1)) s[i] = lowest;
               }
-            };
-            // the largest of the scores; they are read once more below, because 128 of them would not stay in registers
-            uint32_t v[2][32];
-            float m0 = as_float(lowest), m1 = m0, m2 = m0, m3 = m0;
-            tmem_load32(my_scores, v[0]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c >= chunks) break;
-              tmem_loaded32(v[c & 1]);
-              if (c + 1 < chunks) tmem_load32(my_scores + 32 * (c + 1), v[(c + 1) & 1]);
-              uint32_t* s = v[c & 1];
-              hide(s, c);
+              float m0 = as_float(s[0]), m1 = as_float(s[1]), m2 = as_float(s[2]), m3 = as_float(s[3]);
               if (sl >= 0.f) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
+                for (int i = 4; i < 32; i += 4) {
                   m0 = fmaxf(m0, as_float(s[i]));
                   m1 = fmaxf(m1, as_float(s[i + 1]));
                   m2 = fmaxf(m2, as_float(s[i + 2]));
                   m3 = fmaxf(m3, as_float(s[i + 3]));
                 }
+                m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
               } else {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
+                for (int i = 4; i < 32; i += 4) {
                   m0 = fminf(m0, as_float(s[i]));
                   m1 = fminf(m1, as_float(s[i + 1]));
                   m2 = fminf(m2, as_float(s[i + 2]));
                   m3 = fminf(m3, as_float(s[i + 3]));
                 }
+                m0 = fminf(fminf(m0, m1), fminf(m2, m3));
               }
-            }
-            tmem_load32(my_scores, v[0]);
-            m0 = sl >= 0.f ? fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) : fminf(fminf(m0, m1), fminf(m2, m3));
-            const float m = m0 * sl;
-            const bool grows = m > top + kGrowth || (top == -INFINITY && m > top);
-            if (__any_sync(0xffffffffu, grows)) {
-              const float now = fmaxf(top, m);
-              const float keep = exp2_approx(top - (now == -INFINITY ? 0.f : now));
-              top = now;
-              total *= keep;
-              if (any) {
-                // (the product before these scores is done: the tensor cores work in the order of issue)
+              const float m = m0 * sl;
+              if (__any_sync(0xffffffffu, m > top + kGrowth || (top == -INFINITY && m > top))) {
+                // rare but for a segment's first job: what was computed relative to the old maximum is scaled
+                const float now = fmaxf(top, m);
+                const float keep = exp2_approx(top - (now == -INFINITY ? 0.f : now));
+                top = now;
+                total *= keep;
+                t0 *= keep;
+                t1 *= keep;
+                t2 *= keep;
+                t3 *= keep;
+                tc_wait_st();
+                if (any) {
+                  // (the product before these scores is done: the tensor cores work in the order of issue)
 #pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                  uint32_t o[16];
-                  tmem_load16(my_sums + c, o);
-                  tmem_loaded<16>(o);
+                  for (int at = 0; at < D; at += 16) {
+                    uint32_t o[16];
+                    tmem_load16(my_sums + at, o);
+                    tmem_loaded<16>(o);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
-                  tmem_store16(my_sums + c, o);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
+                    tmem_store16(my_sums + at, o);
+                  }
+                }
+#pragma unroll 1
+                for (int at = 0; at < 16 * c; at += 16) {
+                  uint32_t w[16];
+                  tmem_load16(my_scores + at, w);
+                  tmem_loaded<16>(w);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) w[i] = Half16<T>::pack(Half16<T>::value((uint16_t)w[i]) * keep, Half16<T>::value((uint16_t)(w[i] >> 16)) * keep);
+                  tmem_store16(my_scores + at, w);
                 }
               }
-            }
-            const float base_log2 = top == -INFINITY ? 0.f : top;
-            float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (c >= chunks) break;
-              tmem_loaded32(v[c & 1]);
-              if (c + 1 < chunks) tmem_load32(my_scores + 32 * (c + 1), v[(c + 1) & 1]);
-              uint32_t* s = v[c & 1];
-              hide(s, c);
+              const float base_log2 = top == -INFINITY ? 0.f : top;
               uint32_t w[16];
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
@@ -532,6 +528,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
                 w[i / 2 + 1] = Half16<T>::pack(e2, e3);
               }
               tmem_store16(my_scores + 16 * c, w);                   // over scores that have been read
+            };
+            uint32_t v0[32], v1[32];
+            tmem_load32(my_scores, v0);
+#pragma unroll 1
+            for (int c = 0; c < chunks; c += 2) {
+              tmem_loaded32(v0);
+              tmem_load32(my_scores + 32 * (c + 1), v1);
+              weigh(v0, c);
+              tmem_loaded32(v1);
+              if (c + 2 < chunks) tmem_load32(my_scores + 32 * (c + 2), v0);
+              weigh(v1, c + 1);
             }
             total += (t0 + t1) + (t2 + t3);
             tc_wait_st();
