@@ -10,6 +10,8 @@
 //
 // O is rescaled only where a row's maximum grows by more than a factor of 2^8: until then the weights are taken relative to the older
 // maximum, which changes neither the result nor, in fp32 sums and 16-bit floating-point weights, its precision.
+#include <type_traits>
+
 #include "../../include/fp6m.h"
 #include "device_utils.cuh"
 #include "gemm_params.h"
@@ -299,7 +301,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
     } else if (warp == 4) {
       // ================================================================== MMA issuer
       constexpr uint32_t kFormats = (1u << 4) | (Half16<T>::kMmaFormat << 7) | (Half16<T>::kMmaFormat << 10) | ((uint32_t)(kRowTile >> 4) << 24);
-      constexpr uint32_t idesc_s = kFormats | ((uint32_t)(kKeys >> 3) << 17), idesc_s2 = kFormats | ((uint32_t)(2 * kKeys >> 3) << 17);
+      const uint32_t sign = p.scale_log2 < 0.f ? 1u << 13 : 0u;      // the queries are negated
+      const uint32_t idesc_s = kFormats | sign | ((uint32_t)(kKeys >> 3) << 17), idesc_s2 = kFormats | sign | ((uint32_t)(2 * kKeys >> 3) << 17);
       constexpr uint32_t idesc_o = kFormats | (1u << 16) | ((uint32_t)(D >> 3) << 17);         // values are N-major
       // What follows from the lengths is made uniform to the compiler (read from lane 0), so that MMAs are issued with uniform operands.
       struct Jobs {
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       const int group = (warp - 8) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane;
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const uint32_t my_scores = tmem + lanes + group * 128, my_sums = tmem_o + lanes + group * 128;
-      const float sl = p.scale_log2;
+      const float sl = fabsf(p.scale_log2);                          // its sign is in the scores
       float* stats = reinterpret_cast<float*>(smem + C::kStats);
       float4* exchange = reinterpret_cast<float4*>(smem + C::kX);
       int job = 0, n = 0, segment = -1, ended = 0;                   // jobs of this group, jobs of the CTA; segments that this group has jobs of
@@ -432,115 +435,108 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           tc_fence_after();
           if (warp_lives) {
             const int chunks = tile + 1 < seg.t1 ? 4 : 2;            // of 32 keys
-            // The row sees all cached keys, then those of its mask.  The score of another is the lowest there is: the highest, if a negative
-            // scale turns the order round (scale_log2 is never zero), so that its weight is zero.
             const int cached = seg.length - tile * kKeys;            // from the job's first key on
-            const bool hidden = misc[1] != 0, masked = cached < chunks * 32 || hidden;
-            const uint32_t lowest = __float_as_uint(sl < 0.f ? INFINITY : -INFINITY);
-            uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
-            if (masked) {
+            const bool hidden = misc[1] != 0;
+            // The largest score, then the weights: scores are read twice, because 128 of them would not stay in registers.  `hides`: some of the job's keys are
+            // not seen by every row.  (A branch for every 32 scores, for what is hidden or grows, cost 150 cycles each: the two cases are apart.)
+            auto weigh = [&](auto hides) {
+              constexpr bool kHides = decltype(hides)::value;
+              // The row sees all cached keys, then those of its mask; the score of another is the lowest there is.
+              uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
+              if constexpr (kHides) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int here = cached - h * kKeys;
-                unsigned long long word = ~0ull;
-                if (here < kKeys) word = here > 0 ? mask << here | ((1ull << here) - 1) : here > -64 ? mask >> -here : 0ull;
-                if (hidden) {
-                  for (int i = 0; i < min(here, kKeys); ++i)
-                    if ((unsigned)page_of(p, seg, (tile + h) * kKeys + i) >= (unsigned)a.pages) word &= ~(1ull << i);
+                for (int h = 0; h < 2; ++h) {
+                  const int here = cached - h * kKeys;
+                  unsigned long long word = ~0ull;
+                  if (here < kKeys) word = here > 0 ? mask << here | ((1ull << here) - 1) : here > -64 ? mask >> -here : 0ull;
+                  if (hidden) {
+                    for (int i = 0; i < min(here, kKeys); ++i)
+                      if ((unsigned)page_of(p, seg, (tile + h) * kKeys + i) >= (unsigned)a.pages) word &= ~(1ull << i);
+                  }
+                  sees[2 * h] = (uint32_t)word;
+                  sees[2 * h + 1] = (uint32_t)(word >> 32);
                 }
-                sees[2 * h] = (uint32_t)word;
-                sees[2 * h + 1] = (uint32_t)(word >> 32);
               }
-            }
-            float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
-            // 32 scores to weights, relative to the maximum that has been let stand so far
-            auto weigh = [&](uint32_t* s, int c) {
-              if (masked) {
+              auto hide = [&](uint32_t* s, int c) {
+                if constexpr (kHides) {
+                  const uint32_t word = c == 0 ? sees[0] : c == 1 ? sees[1] : c == 2 ? sees[2] : sees[3];
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!(sees[c] >> i & 1)) s[i] = lowest;
-              }
-              float m0 = as_float(s[0]), m1 = as_float(s[1]), m2 = as_float(s[2]), m3 = as_float(s[3]);
-              if (sl >= 0.f) {
-#pragma unroll
-                for (int i = 4; i < 32; i += 4) {
-                  m0 = fmaxf(m0, as_float(s[i]));
-                  m1 = fmaxf(m1, as_float(s[i + 1]));
-                  m2 = fmaxf(m2, as_float(s[i + 2]));
-                  m3 = fmaxf(m3, as_float(s[i + 3]));
+                  for (int i = 0; i < 32; ++i)
+                    if (!(word >> i & 1)) s[i] = __float_as_uint(-INFINITY);
                 }
-                m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-              } else {
+              };
+              uint32_t v0[32], v1[32];
+              float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+              auto largest = [&](uint32_t* s, int c) {
+                hide(s, c);
 #pragma unroll
-                for (int i = 4; i < 32; i += 4) {
-                  m0 = fminf(m0, as_float(s[i]));
-                  m1 = fminf(m1, as_float(s[i + 1]));
-                  m2 = fminf(m2, as_float(s[i + 2]));
-                  m3 = fminf(m3, as_float(s[i + 3]));
+                for (int i = 0; i < 32; i += 8) {
+                  m0 = fmaxf(m0, fmaxf(as_float(s[i]), as_float(s[i + 1])));
+                  m1 = fmaxf(m1, fmaxf(as_float(s[i + 2]), as_float(s[i + 3])));
+                  m2 = fmaxf(m2, fmaxf(as_float(s[i + 4]), as_float(s[i + 5])));
+                  m3 = fmaxf(m3, fmaxf(as_float(s[i + 6]), as_float(s[i + 7])));
                 }
-                m0 = fminf(fminf(m0, m1), fminf(m2, m3));
+              };
+              tmem_load32(my_scores, v0);
+#pragma unroll 1
+              for (int c = 0; c < chunks; c += 2) {
+                tmem_loaded32(v0);
+                tmem_load32(my_scores + 32 * (c + 1), v1);
+                largest(v0, c);
+                tmem_loaded32(v1);
+                tmem_load32(my_scores + 32 * (c + 2 < chunks ? c + 2 : 0), v0);        // (the last one: the first again)
+                largest(v1, c + 1);
               }
-              const float m = m0 * sl;
+              const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * sl;
               if (__any_sync(0xffffffffu, m > top + kGrowth || (top == -INFINITY && m > top))) {
-                // rare but for a segment's first job: what was computed relative to the old maximum is scaled
                 const float now = fmaxf(top, m);
                 const float keep = exp2_approx(top - (now == -INFINITY ? 0.f : now));
                 top = now;
                 total *= keep;
-                t0 *= keep;
-                t1 *= keep;
-                t2 *= keep;
-                t3 *= keep;
-                tc_wait_st();
                 if (any) {
                   // (the product before these scores is done: the tensor cores work in the order of issue)
 #pragma unroll 1
-                  for (int at = 0; at < D; at += 16) {
+                  for (int c = 0; c < D; c += 16) {
                     uint32_t o[16];
-                    tmem_load16(my_sums + at, o);
+                    tmem_load16(my_sums + c, o);
                     tmem_loaded<16>(o);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
-                    tmem_store16(my_sums + at, o);
+                    tmem_store16(my_sums + c, o);
                   }
-                }
-#pragma unroll 1
-                for (int at = 0; at < 16 * c; at += 16) {
-                  uint32_t w[16];
-                  tmem_load16(my_scores + at, w);
-                  tmem_loaded<16>(w);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) w[i] = Half16<T>::pack(Half16<T>::value((uint16_t)w[i]) * keep, Half16<T>::value((uint16_t)(w[i] >> 16)) * keep);
-                  tmem_store16(my_scores + at, w);
                 }
               }
               const float base_log2 = top == -INFINITY ? 0.f : top;
-              uint32_t w[16];
+              float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
+              auto exponentials = [&](uint32_t* s, int c) {
+                hide(s, c);
+                uint32_t w[16];
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
-                const float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
-                t0 += e0;
-                t1 += e1;
-                t2 += e2;
-                t3 += e3;
-                w[i / 2] = Half16<T>::pack(e0, e1);
-                w[i / 2 + 1] = Half16<T>::pack(e2, e3);
-              }
-              tmem_store16(my_scores + 16 * c, w);                   // over scores that have been read
-            };
-            uint32_t v0[32], v1[32];
-            tmem_load32(my_scores, v0);
+                for (int i = 0; i < 32; i += 4) {
+                  const float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
+                  const float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
+                  t0 += e0;
+                  t1 += e1;
+                  t2 += e2;
+                  t3 += e3;
+                  w[i / 2] = Half16<T>::pack(e0, e1);
+                  w[i / 2 + 1] = Half16<T>::pack(e2, e3);
+                }
+                tmem_store16(my_scores + 16 * c, w);                 // over scores that have been read
+              };
 #pragma unroll 1
-            for (int c = 0; c < chunks; c += 2) {
-              tmem_loaded32(v0);
-              tmem_load32(my_scores + 32 * (c + 1), v1);
-              weigh(v0, c);
-              tmem_loaded32(v1);
-              if (c + 2 < chunks) tmem_load32(my_scores + 32 * (c + 2), v0);
-              weigh(v1, c + 1);
-            }
-            total += (t0 + t1) + (t2 + t3);
+              for (int c = 0; c < chunks; c += 2) {
+                tmem_loaded32(v0);
+                tmem_load32(my_scores + 32 * (c + 1), v1);
+                exponentials(v0, c);
+                tmem_loaded32(v1);
+                if (c + 2 < chunks) tmem_load32(my_scores + 32 * (c + 2), v0);
+                exponentials(v1, c + 1);
+              }
+              total += (t0 + t1) + (t2 + t3);
+            };
+            if (cached < chunks * 32 || hidden) weigh(std::true_type());
+            else weigh(std::false_type());
             tc_wait_st();
           }
           any = true;
