@@ -397,19 +397,25 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          // (four contributors on their way at a time: with one the loads' latency made this 20,000 cycles for six of them)
 #pragma unroll 1
-          for (int t = first; t <= last; ++t) {
-            const float4* from = slot_of(t, t == first ? 1 : 0) + c * 8 * 32;
-            float4 w[8];
+          for (int t = first; t <= last; t += 4) {
+            float4 w[4][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __ldcg(from + i * 32);
+            for (int e = 0; e < 4; ++e) {
+              const float4* from = slot_of(min(t + e, last), t + e == first ? 1 : 0) + c * 8 * 32;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[4 * i] += w[i].x;
-              v[4 * i + 1] += w[i].y;
-              v[4 * i + 2] += w[i].z;
-              v[4 * i + 3] += w[i].w;
+              for (int i = 0; i < 8; ++i) w[e][i] = t + e <= last ? __ldcg(from + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                v[4 * i] += w[e][i].x;
+                v[4 * i + 1] += w[e][i].y;
+                v[4 * i + 2] += w[e][i].z;
+                v[4 * i + 3] += w[e][i].w;
+              }
           }
           put(v, row0, column0 + c * 32);
         }
@@ -430,28 +436,45 @@ mul_fp8_rows_kernel(const __grid_constant__ RowsParams p, const __grid_constant_
 
 struct RowsPlan {
   int group, row_tiles, tiles, teams, whole, extra, sharers;
+  double cost;
 };
-RowsPlan plan_rows(int M, int N, int K, int sms) {
+// One CTA or two per team, and whether the tiles that are left after the whole ones are cut along K: what takes the least time, in blocks of a single
+// CTA (540 cycles; a pair of CTAs takes 1.6 times that for four times the work).  An exchange of sums, from their store to the last result, took
+// as long as 26 blocks where a CTA has 128 x 128 of them, and as 56 with 128 x 256.  us with teams of one / two (shared or not as this rule
+// has it): 131 x 11008 x 4096 24 / 31, 256 x 4096 x 4096 13.6 / 26, 400 x 8192 x 8192 46 / 34, 512 x 4096 x 11008 37 / 42, 777 x 4096 x 11008
+// 55 / 54, 1024 x 4096 x 4096 24 / 20, 2048 x 8192 x 8192 150 / 127 (rows x K x columns).
+RowsPlan plan_teams(int group, int M, int N, int K, int sms) {
   RowsPlan plan;
-  plan.group = M <= 128 ? 1 : 2;
-  const int edge = 128 * plan.group, kb = (K + kBlock - 1) / kBlock;
+  plan.group = group;
+  const int edge = 128 * group, kb = (K + kBlock - 1) / kBlock;
+  const double block = group == 1 ? 1.0 : 1.6, exchange = group == 1 ? 26 : 56;
   plan.row_tiles = (M + edge - 1) / edge;
   plan.tiles = plan.row_tiles * ((N + edge - 1) / edge);
-  plan.teams = (sms > 0 && sms < kMaxTeams ? sms : kMaxTeams) / plan.group;
+  plan.teams = (sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas) / group;
   if (plan.teams < 1) plan.teams = 1;
   plan.whole = plan.tiles / plan.teams;
   const int left = plan.tiles - plan.whole * plan.teams;
   plan.extra = left;
   plan.sharers = 0;
-  // cut along K: at least four blocks each, and only where that saves more blocks than the exchange takes time
-  const long long blocks = (long long)left * kb;
-  const int sharers = (int)(blocks / 4 < plan.teams ? (blocks + 3) / 4 : plan.teams);
-  if (left > 0 && kb - (int)((blocks + sharers - 1) / sharers) >= 10) {
-    plan.extra = 0;
-    plan.sharers = sharers;
+  plan.cost = (plan.whole + (left > 0)) * (double)kb * block;
+  if (left > 0) {
+    const long long blocks = (long long)left * kb;
+    const int sharers = (int)(blocks / 4 < plan.teams ? (blocks + 3) / 4 : plan.teams);      // at least four blocks each
+    const double shared = ((double)plan.whole * kb + (double)((blocks + sharers - 1) / sharers)) * block + exchange;
+    if (shared < plan.cost) {
+      plan.cost = shared;
+      plan.extra = 0;
+      plan.sharers = sharers;
+    }
   }
   if (plan.whole == 0) plan.teams = plan.sharers ? plan.sharers : left;
   return plan;
+}
+RowsPlan plan_rows(int M, int N, int K, int sms) {
+  const RowsPlan one = plan_teams(1, M, N, K, sms);
+  if (M <= 128) return one;
+  const RowsPlan two = plan_teams(2, M, N, K, sms);
+  return two.cost < one.cost ? two : one;
 }
 size_t rows_bytes(const RowsPlan& plan) {
   return plan.sharers ? kRowsScratch + (size_t)plan.teams * plan.group * 2 * (plan.group * 64) * 256 * sizeof(float) : kRowsScratch;

@@ -52,6 +52,20 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return m;
 }
 
+// The sum over the CTA, in one order.
+__device__ __forceinline__ float sum_of_block(float sum, float* part) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if (warps == 1) return sum;
+  if (lane == 0) part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = lane < warps ? part[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
 struct RowParams {
   const void *x, *weight, *residual;
   void *residual_out, *y;
@@ -60,10 +74,104 @@ struct RowParams {
   float eps;
 };
 
-// One CTA a row, eight neighbouring values a thread at a time; every pass reads the row again.
-template <class T, bool kNorm, bool kFp8>
-__global__ void rows_kernel(const RowParams p) {
+// Stores vector v of a row: in 16 bits, or in E4M3 with the scale of the 128 values that sixteen neighbouring lanes hold.  All lanes of a warp call it.
+template <class T, bool kFp8>
+__device__ __forceinline__ void finish_vector(const RowParams& p, size_t row, int v, int vecs, int groups, const float (&f)[8]) {
+  if (kFp8) {
+    float top = kSmallest;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (v < vecs) {
+      const float up = kE4m3Max / top;
+      uint2 q;
+      auto two = [&](int i) { return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[i] * up, f[i + 1] * up), __NV_SATFINITE, __NV_E4M3); };
+      q.x = two(0) | two(2) << 16;
+      q.y = two(4) | two(6) << 16;
+      static_cast<uint2*>(p.y)[row * vecs + v] = q;
+      if (v % 16 == 0) p.scales[row * groups + v / 16] = top / kE4m3Max;
+    }
+  } else if (v < vecs) {
+    static_cast<uint4*>(p.y)[row * vecs + v] = pack8<T>(f);
+  }
+}
+
+// One CTA a row; a thread holds kVecs groups of eight neighbouring values of it (a vector), blockDim.x vectors apart.  Every value is read once: what the
+// second half of the work needs stays in registers, and the weights are on their way while the squares are summed.  Sixteen lanes hold the
+// 128 values that share a scale.  Bound by memory: 16384 x 8192 with residual, fp16 to E4M3, NORM_FIGURE.  Where rows are few, what counts
+// is latency: more threads with a vector each (launch_rows).
+template <class T, bool kNorm, bool kFp8, int kVecs>
+__global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024) rows_kernel(const RowParams p) {
   __shared__ float part[32];
+  const size_t row = blockIdx.x;
+  const int vecs = p.N / 8, groups = (p.N + kGroup - 1) / kGroup;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint4* x = static_cast<const uint4*>(p.x) + row * vecs;
+  uint4 in[kVecs], add[kVecs], weight[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (v < vecs) in[i] = x[v];
+  }
+  const bool residual = kNorm && p.residual;
+  if (residual) {
+    const uint4* r = static_cast<const uint4*>(p.residual) + row * vecs;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < vecs) add[i] = r[v];
+    }
+  }
+  if (kNorm) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int v = threadIdx.x + i * blockDim.x;
+      if (v < vecs) weight[i] = static_cast<const uint4*>(p.weight)[v];
+    }
+  }
+  float f[kVecs][8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[i][e] = 0.f;
+    if (v < vecs) {
+      unpack8<T>(in[i], f[i]);
+      if (residual) {
+        float more[8];
+        unpack8<T>(add[i], more);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] += more[e];
+        static_cast<uint4*>(p.residual_out)[row * vecs + v] = pack8<T>(f[i]);
+      }
+    }
+    if (kNorm) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += f[i][e] * f[i][e];
+    }
+  }
+  float factor = 1.f;
+  if (kNorm) factor = rsqrtf(sum_of_block(sum, part) / p.N + p.eps);
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    if (kNorm && v < vecs) {
+      float w[8];
+      unpack8<T>(weight[i], w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * factor * w[e];
+    }
+    finish_vector<T, kFp8>(p, row, v, vecs, groups, f[i]);
+  }
+}
+
+// Rows of any length: every pass reads the row again (from L2, mostly).
+template <class T, bool kNorm, bool kFp8>
+__global__ void __launch_bounds__(1024) long_rows_kernel(const RowParams p) {
+  __shared__ float part[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const size_t row = blockIdx.x;
   const int vecs = p.N / 8, groups = (p.N + kGroup - 1) / kGroup;
@@ -87,18 +195,12 @@ __global__ void rows_kernel(const RowParams p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += f[i] * f[i];
     }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) sum += part[w];
-    factor = rsqrtf(sum / p.N + p.eps);
+    factor = rsqrtf(sum_of_block(sum, part) / p.N + p.eps);
   }
   for (int v0 = 0; v0 < vecs; v0 += blockDim.x) {
     const int v = v0 + threadIdx.x;
-    const bool live = v < vecs;
     float f[8] = {};
-    if (live) {
+    if (v < vecs) {
       load(v, f);
       if (kNorm) {
         if (p.residual_out) static_cast<uint4*>(p.residual_out)[row * vecs + v] = pack8<T>(f);
@@ -108,33 +210,23 @@ __global__ void rows_kernel(const RowParams p) {
         for (int i = 0; i < 8; ++i) f[i] = f[i] * factor * w[i];
       }
     }
-    if (kFp8) {
-      float top = kSmallest;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(f[i]));
-#pragma unroll
-      for (int o = 8; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));     // the 16 lanes of a group
-      if (live) {
-        const float up = kE4m3Max / top;
-        uint2 q;
-        auto two = [&](int i) { return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[i] * up, f[i + 1] * up), __NV_SATFINITE, __NV_E4M3); };
-        q.x = two(0) | two(2) << 16;
-        q.y = two(4) | two(6) << 16;
-        static_cast<uint2*>(p.y)[row * vecs + v] = q;
-        if (v % 16 == 0) p.scales[row * groups + v / 16] = top / kE4m3Max;
-      }
-    } else if (live) {
-      static_cast<uint4*>(p.y)[row * vecs + v] = pack8<T>(f);
-    }
+    finish_vector<T, kFp8>(p, row, v, vecs, groups, f);
   }
 }
 
+template <class T, bool kNorm, bool kFp8>
+cudaError_t launch_kind(const RowParams& p, cudaStream_t stream) {
+  const int vecs = p.N / 8;
+  // Few rows (a multiprocessor gets one or two): as many threads as there are vectors, up to 1024.  Many: four vectors a thread, so that more rows are in flight.
+  const int kind = p.M > 512 && vecs >= 128 ? 4 : vecs <= 1024 ? 1 : 2;
+  const int threads = ((vecs + kind - 1) / kind + 31) / 32 * 32;
+  if (vecs > 2048) return launch_overlapped(long_rows_kernel<T, kNorm, kFp8>, dim3(p.M), dim3(1024), 0, stream, p);
+  return launch_overlapped(kind == 1 ? rows_kernel<T, kNorm, kFp8, 1> : kind == 2 ? rows_kernel<T, kNorm, kFp8, 2> : rows_kernel<T, kNorm, kFp8, 4>, dim3(p.M), dim3(threads), 0,
+                           stream, p);
+}
 template <class T>
 cudaError_t launch_rows(const RowParams& p, bool norm, cudaStream_t stream) {
-  void (*kernel)(RowParams) = !norm ? rows_kernel<T, false, true> : p.scales ? rows_kernel<T, true, true> : rows_kernel<T, true, false>;
-  const int vecs = p.N / 8;
-  const int threads = vecs >= 512 ? 512 : (vecs + 31) / 32 * 32;
-  return launch_overlapped(kernel, dim3(p.M), dim3(threads), 0, stream, p);
+  return !norm ? launch_kind<T, false, true>(p, stream) : p.scales ? launch_kind<T, true, true>(p, stream) : launch_kind<T, true, false>(p, stream);
 }
 
 int rows_impl(const RowParams& p, bool norm, int type, int dev, void* stream, const char* what) {
