@@ -41,8 +41,16 @@ class _GeneralPathOnly:
         warnings.warn(f"fp6_marlin_b200: calls take the slower general path, because {self.reason}; build with "
                       "`python fp6_marlin_b200/build.py`", RuntimeWarning, stacklevel=4)
 
+    def bind_operators(self, *addresses):
+        pass
+
+    def set_operator_scratch(self, *buffer):
+        pass
+
     def mul(self, *args):
         return -1                             # not handled
+
+    rms_norm = quantize_fp8 = mul_fp8 = tree_attention = mul
 
 
 def _native_call_path():

@@ -14,13 +14,17 @@ import ctypes
 import torch
 
 from . import _lib
-from .api import _buffers_lock, _device_buffers, _ptr, _status, _stream_handle
+from .api import _buffers_lock, _call, _device_buffers, _ptr, _sm_count, _status, _stream_handle
 from ._lib import lib
 
 GROUP = 128                                       # neighbours that share a scale
 E4M3_MAX = 448.0
 SMALLEST = 1e-30                                  # largest magnitude that a group of zeros is given
 _TYPES = {torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
+
+_call.bind_operators(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+    "fp6m_rms_norm", "fp6m_quantize_fp8", "fp6m_mul_fp8", "fp6m_mul_fp8_scratch_bytes", "fp6m_tree_attention", "fp6m_tree_attention_scratch_bytes")))
+_OWNERS = {"mul_fp8": 1, "tree_attention": 2}     # of a scratch, as the native call path numbers them
 
 _scratch: dict[tuple, list[torch.Tensor]] = {}    # (operator, device, stream) -> buffers, the last is in use
 
@@ -38,11 +42,11 @@ def _operator_buffers(name: str, device: torch.device, nbytes: int, stream: int)
                 nbytes = max(nbytes, 2 * buffers[-1].numel())
             with torch.cuda.device(device):
                 buffers.append(torch.zeros(nbytes, dtype=torch.uint8, device=device))
+            _call.set_operator_scratch(_OWNERS[name], device.index, stream, _ptr(buffers[-1]), nbytes)
         return buffers[-1], _status[device.index]
 
 
 def _sms(device: torch.device) -> int:
-    from .api import _sm_count
     if device.index not in _sm_count:
         _sm_count[device.index] = torch.cuda.get_device_properties(device.index).multi_processor_count
     return _sm_count[device.index]
@@ -90,6 +94,12 @@ def rms_norm(x, weight, y, eps=1e-6, *, scales=None, residual=None, residual_out
     (M, ceil(N/128)) float32, ``y`` is float8_e4m3fn and ``y * scales`` (a scale for each 128 neighbours of a row: their
     largest magnitude / 448) stands for the result: what :func:`mul_fp8` takes.  N must be a multiple of 8.
     """
+    # plain CUDA tensors that pass every check: one call into native code; anything else takes the general path below
+    rc = _call.rms_norm(x, weight, y, eps, scales, residual, residual_out)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise("rms_norm", rc)
     m, n = _rows("rms_norm", x, y, scales)
     if weight.dtype != x.dtype or weight.shape != (n,):
         raise RuntimeError(f"rms_norm: weight must hold {n} values of x's type")
@@ -115,6 +125,11 @@ def quantize_fp8(x, q, scales):
     neighbours / 448 and ``q`` (float8_e4m3fn) the values divided by it.  N must be a multiple of 8."""
     if scales is None:
         raise RuntimeError("quantize_fp8: scales are needed")
+    rc = _call.quantize_fp8(x, q, scales)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise("quantize_fp8", rc)
     m, n = _rows("quantize_fp8", x, q, scales)
     device = x.device
     _check("quantize_fp8", device, x=x, q=q, scales=scales)
@@ -145,6 +160,11 @@ def mul_fp8(A, B, C, sa, sb):
 
     ``sa`` (M, ceil(K/128)) float32 holds a scale for each 128 neighbours of a row of A, ``sb`` (ceil(N/128), ceil(K/128)) one for
     each 128 x 128 block of B.  Sums are fp32 and rounded once.  K must be a multiple of 16 and N of 8."""
+    rc = _call.mul_fp8(A, B, C, sa, sb)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise("mul_fp8", rc)
     if not A.is_cuda:
         raise RuntimeError("fp6_marlin_b200.mul_fp8 needs CUDA tensors: there is no CPU implementation")
     if A.dtype != torch.float8_e4m3fn or B.dtype != torch.float8_e4m3fn or A.dim() != 2 or B.dim() != 2:
@@ -217,6 +237,11 @@ def tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, *,
     committed token, in the table or in a page, is not read.
     """
     what = "tree_attention"
+    rc = _call.tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise(what, rc)
     if not q.is_cuda:
         raise RuntimeError("fp6_marlin_b200.tree_attention needs CUDA tensors: there is no CPU implementation")
     if q.dtype not in _TYPES or q.dim() != 4:

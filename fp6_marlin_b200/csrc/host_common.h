@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace fp6m {
 
 // Records the error for fp6m_last_cuda_error() and returns FP6M_ERR_CUDA (c_api.cu).
@@ -21,6 +23,20 @@ struct DeviceGuard {
   }
   ~DeviceGuard() { if (switched) cudaSetDevice(prev); }
 };
+
+// Lets a kernel use that much dynamic shared memory, once per device and kernel (the attribute costs a driver call).
+template <auto kKernel>
+cudaError_t allow_shared_memory(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kKernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit);
+  return e;
+}
 
 // A launch that may start while the kernel in front of it finishes (programmatic dependent launch): the kernel touches memory
 // only after griddepcontrol.wait.

@@ -367,7 +367,7 @@ size_t fp8_scratch_bytes(int M, int N, int K, int sms) {
 
 template <class T, class C>
 cudaError_t launch_with(const Fp8Params& p, int ctas, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(mul_fp8_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  cudaError_t e = allow_shared_memory<mul_fp8_kernel<T, C>>(C::kSmemBytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(mul_fp8_kernel<T, C>, dim3(ctas), dim3(C::kThreads), C::kSmemBytes, stream, p, amap, bmap);
 }

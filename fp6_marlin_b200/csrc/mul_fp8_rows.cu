@@ -484,7 +484,7 @@ template <class T, int kGroup>
 cudaError_t launch_rows(const RowsParams& p, int teams, const CUtensorMap& amap, const CUtensorMap& bmap, cudaStream_t stream) {
   using C = RowsCfg<kGroup>;
   static_assert(C::kSlotFloat4 * 4 == kGroup * 64 * 256, "slot");
-  cudaError_t e = cudaFuncSetAttribute(mul_fp8_rows_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  cudaError_t e = allow_shared_memory<mul_fp8_rows_kernel<T, C>>(C::kSmemBytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(teams * kGroup);

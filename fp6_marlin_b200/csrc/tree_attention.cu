@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 template <class T, int D, int kRowTile>
 cudaError_t launch_tile(const TreeParams& p, int ctas, cudaStream_t stream) {
   constexpr int bytes = 3 * 128 / D * 2 * kKeys * D * 2 + 16 * D * 4 + 4 * 32 * 4 + 4 * 8 + 16 + 2 * kThreads * 8;
-  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, D, kRowTile>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t e = allow_shared_memory<tree_attention_kernel<T, D, kRowTile>>(bytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(tree_attention_kernel<T, D, kRowTile>, dim3(ctas), dim3(kThreads), bytes, stream, p);
 }

@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
 
 template <class T, class C>
 cudaError_t launch_tc5(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(tree_attention_tc5_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  cudaError_t e = allow_shared_memory<tree_attention_tc5_kernel<T, C>>(C::kSmemBytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(tree_attention_tc5_kernel<T, C>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p, kmap, vmap);
 }
