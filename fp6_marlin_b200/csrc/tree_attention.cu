@@ -21,7 +21,7 @@ using namespace fp6m;
 
 constexpr int kThreads = 128;
 constexpr int kMaxCtas = 512;
-constexpr int kLeastUnits = 3;           // of a CTA: fewer key tiles cost less than joining what more CTAs leave
+constexpr int kLeastUnits = 3, kSlack = 8;       // see make_plan
 constexpr int kCounterBytes = kMaxCtas * 4;
 
 template <class T> struct Mma;
@@ -57,30 +57,23 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
   extern __shared__ __align__(128) uint8_t smem[];
   float* pool = reinterpret_cast<float*>(smem + kStages * 2 * kTileBytes);        // [kRowTile][kPool]
   float* stats = pool + kRowTile * kPool;                                          // [warp][2][16]: maxima, totals
-  long long* plan = reinterpret_cast<long long*>(stats + 4 * 32);                  // total units; unit of the first item, its sequence
-  int* flags = reinterpret_cast<int*>(plan + 4);                                   // [0] a page did not exist, [1] last to arrive
+  Plan* plan = reinterpret_cast<Plan*>(stats + 4 * 32);
+  int* flags = reinterpret_cast<int*>(plan + 1);                                   // [0] a page did not exist, [1] last to arrive
   const T** places = reinterpret_cast<const T**>(flags + 4);                       // [2][128]: where the keys, then the values, of a tile are
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row_warp = warp / kKeyWarps, key_warp = warp % kKeyWarps;
   const fp6m_tree_attention_args& a = p.a;
   if (tid == 0) flags[0] = 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  // ---- the plan: units of all sequences, and where this CTA's range starts
   const int cta = blockIdx.x;
-  auto ctas_of = [&](long long units) { return (long long)gridDim.x < units / kLeastUnits ? (int)gridDim.x : max((int)(units / kLeastUnits), 1); };
-  if (warp == 0)
-    make_plan(p, plan, [&](long long units) {
-      const int n = ctas_of(units);
-      return cta < n ? range_start(units, n, cta) : units;
-    });
+  if (warp == 0) make_plan(p, plan, kLeastUnits, kSlack);
   __syncthreads();
-  const long long units = plan[0];
-  const int ctas = ctas_of(units);
+  const long long units = plan->units;
+  const int ctas = plan->ctas;
   if (cta >= ctas) return;
-  const long long u0 = range_start(units, ctas, cta);
-  Segments seg(p, plan, u0, range_start(units, ctas, cta + 1) - u0);
+  Segments seg(p, *plan);
 
   // ---- copies of a tile: a row of keys and one of values per token, zeros behind the last.  A thread works out where one row is (the
   // same by all threads that copy a piece of it cost half of the kernel's instructions); the others take it from shared memory.
@@ -456,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 
 template <class T, int D, int kRowTile>
 cudaError_t launch_tile(const TreeParams& p, int ctas, cudaStream_t stream) {
-  constexpr int bytes = 3 * 128 / D * 2 * kKeys * D * 2 + 16 * D * 4 + 4 * 32 * 4 + 4 * 8 + 16 + 2 * kThreads * 8;
+  constexpr int bytes = 3 * 128 / D * 2 * kKeys * D * 2 + 16 * D * 4 + 4 * 32 * 4 + sizeof(Plan) + 16 + 2 * kThreads * 8;
   cudaError_t e = allow_shared_memory<tree_attention_kernel<T, D, kRowTile>>(bytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(tree_attention_kernel<T, D, kRowTile>, dim3(ctas), dim3(kThreads), bytes, stream, p);

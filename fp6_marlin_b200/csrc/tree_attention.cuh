@@ -53,33 +53,68 @@ __device__ __forceinline__ int cta_of(long long units, int ctas, long long unit)
   return c;
 }
 
-// Of one warp: the total of the units, and the sequence in which `first_of(total)` lies with the unit that it starts at; lane 0's answer
-// goes to plan[0 .. 2].
-template <class F>
-__device__ __forceinline__ void make_plan(const TreeParams& p, long long* plan, F&& first_of) {
-  const int lane = threadIdx.x & 31;
+// How the units are shared out, and where this CTA starts: worked out by one warp, in shared memory.
+struct Plan {
+  long long units, start, count;         // in all; this CTA's first and how many
+  long long at;                          // its first unit, from the start of the sequence on
+  int ctas, b, length, apart;            // CTAs that work; the sequence of the first unit, and its length; apart: an item per CTA
+};
+// `least`: units of a CTA, fewer cost less than joining what more CTAs leave; `slack`: what that joining takes, in key tiles: where there
+// are CTAs enough for an item each, and the longest item is not that much longer than an equal share, every CTA gets one item.
+__device__ __forceinline__ void make_plan(const TreeParams& p, Plan* plan, int least, int slack) {
+  const int lane = threadIdx.x & 31, cta = blockIdx.x, grid = gridDim.x;
   const long long items = (long long)p.a.kv_heads * p.parts;
   long long units = 0;
-  for (int b = lane; b < p.a.batch; b += 32) units += (tiles_of(p, length_of(p, b)) + p.overhead) * items;
-  for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-  const long long first = first_of(units);
+  int longest = 0;
+  for (int b = lane; b < p.a.batch; b += 32) {
+    const int size = tiles_of(p, length_of(p, b)) + p.overhead;
+    units += size * items;
+    longest = max(longest, size);
+  }
+  for (int o = 16; o; o >>= 1) {
+    units += __shfl_xor_sync(0xffffffffu, units, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  const int ctas = (long long)grid < units / least ? grid : max((int)(units / least), 1);
+  const bool apart = items * p.a.batch <= grid && longest - units / ctas <= slack;
+  if (apart) {
+    if (lane == 0) {
+      plan->ctas = (int)items * p.a.batch;
+      plan->apart = 1;
+      plan->b = min(cta / (int)items, p.a.batch - 1);
+      plan->length = length_of(p, plan->b);
+      plan->units = units;
+      plan->count = tiles_of(p, plan->length) + p.overhead;
+      plan->at = (cta % (int)items) * plan->count;
+      plan->start = 0;
+    }
+    return;
+  }
+  const long long first = cta < ctas ? range_start(units, ctas, cta) : units;
   long long before = 0;
   for (int b0 = 0; b0 < p.a.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const long long mine = b < p.a.batch ? (tiles_of(p, length_of(p, b)) + p.overhead) * items : 0;
+    const int b = b0 + lane, length = b < p.a.batch ? length_of(p, b) : 0;
+    const long long mine = b < p.a.batch ? (tiles_of(p, length) + p.overhead) * items : 0;
     long long upto = mine;
     for (int o = 1; o < 32; o <<= 1) {
       const long long other = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += other;
     }
     if (first >= before + upto - mine && first < before + upto) {
-      plan[1] = first - (before + upto - mine);
-      plan[2] = b;
+      plan->at = first - (before + upto - mine);
+      plan->b = b;
+      plan->length = length;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
     if (before > first) break;
   }
-  if (lane == 0) plan[0] = units;
+  if (lane == 0) {
+    plan->units = units;
+    plan->ctas = ctas;
+    plan->apart = 0;
+    plan->start = first;
+    plan->count = cta < ctas ? range_start(units, ctas, cta + 1) - first : 0;
+  }
 }
 
 // A CTA's range as a sequence of segments: the key tiles t0 .. t1 - 1 of an item.
@@ -88,15 +123,15 @@ struct Segments {
   long long unit;                        // where its item starts
   int at;                                // unit inside the item of what follows
   long long left;                        // units that follow
-  __device__ __forceinline__ Segments(const TreeParams& p, const long long* plan, long long start, long long count) {
-    b = (int)plan[2];
-    length = length_of(p, b);
+  __device__ __forceinline__ Segments(const TreeParams& p, const Plan& plan) {
+    b = plan.b;
+    length = plan.length;
     tiles = tiles_of(p, length);
     const int size = tiles + p.overhead;
-    item = (int)(plan[1] / size);
-    at = (int)(plan[1] - (long long)item * size);
-    unit = start - at;
-    left = count;
+    item = (int)(plan.at / size);
+    at = (int)(plan.at - (long long)item * size);
+    unit = plan.start - at;
+    left = plan.count;
   }
   __device__ __forceinline__ bool next(const TreeParams& p) {
     while (left > 0) {

@@ -26,6 +26,7 @@ namespace {
 constexpr int kRowTile = 128;
 constexpr int kMostTreeCtas = 192;       // one per multiprocessor
 constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs (three idle), twice four that compute weights
+constexpr int kSlack = 32;               // see make_plan
 constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass
 
 template <int D_, bool PAIR_>
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 16, product = weights + 16;
   volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, [2, 3] last to arrive
   volatile uint32_t* odd_ring = misc + 4;                            // [segment]: infinities or NaN among its drafted values
-  __shared__ long long plan[4];
+  __shared__ Plan plan;
   const int tid = threadIdx.x, warp = uniform_warp_index(), lane = tid & 31;
   const fp6m_tree_attention_args& a = p.a;
 
@@ -143,29 +144,24 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(const_cast<uint32_t*>(misc))) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  launch_dependents();
   grid_dependency_wait();
   const int cta = blockIdx.x;
-  auto ctas_of = [&](long long units) { return (long long)gridDim.x < units / 3 ? (int)gridDim.x : max((int)(units / 3), 1); };
-  if (warp == 0)
-    make_plan(p, plan, [&](long long units) {
-      const int n = ctas_of(units);
-      return cta < n ? range_start(units, n, cta) : units;
-    });
+  if (warp == 0) make_plan(p, &plan, 3, kSlack);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, misc[0], 0);
-  const long long units = plan[0];
-  const int ctas = ctas_of(units);
+  const long long units = plan.units;
+  const int ctas = plan.ctas;
   const bool works = cta < ctas;
-  const long long u0 = works ? range_start(units, ctas, cta) : 0;
   bool dead = false;
   // Up to 64 rows there is room for the queries of two items; a row tile is 128 rows all the same, what the others hold is nobody's.
   const int q_rows = !kPair && p.rows <= 64 ? 64 : kRowTile, q_sets = !kPair && p.rows <= 64 ? 2 : 1;
   const uint32_t q_bytes = q_rows * D * 2;                           // of a row tile; halves of a row of 128 values lie q_rows * 128 bytes apart
 
   if (works) {
-    Segments seg(p, plan, u0, range_start(units, ctas, cta + 1) - u0);
+    Segments seg(p, plan);
     // score tiles [group][2] of 64 columns, then a tile of sums per group
     const uint32_t tmem_o = tmem + 256;
     if (warp < 4) {
