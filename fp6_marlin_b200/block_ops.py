@@ -214,7 +214,7 @@ def _strides(what, name, t, dtype, shape, device, written=False):
         raise RuntimeError(f"{what}: {name} must be of shape {shape} and q's type")
     if t.device != device:
         raise RuntimeError(f"{what}: {name} must be on q's device")
-    s = t.stride()
+    s = [shape[3] if size == 1 else step for size, step in zip(shape[:3], t.stride())] + [t.stride(3)]      # (that of a single place says nothing)
     if t.numel() and (s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or t.data_ptr() % 16):
         raise RuntimeError(f"{what}: the values of a head of {name} must lie next to one another, on 16-byte boundaries")
     if written and any(size > 1 and step == 0 for size, step in zip(shape, s)):

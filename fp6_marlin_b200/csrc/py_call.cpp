@@ -224,7 +224,7 @@ bool heads_of(const at::Tensor* t, int64_t a, int64_t b, int64_t c, int64_t d, a
       t->stride(3) != 1 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16)
     return false;
   for (int i = 0; i < 3; ++i) {
-    strides[i] = t->stride(i);
+    strides[i] = t->size(i) == 1 ? d : t->stride(i);          // (that of a single place says nothing)
     if (strides[i] % 8 || (written && strides[i] == 0 && t->size(i) > 1)) return false;
   }
   return true;

@@ -75,7 +75,7 @@ def _check(out, x, scale=None):
 
 
 CASES = [
-    # b, t, heads, kv heads, d, lengths, page
+    # b, t, heads, kv heads, d, lengths, page (up to 32 rows of a head of keys, up to 128, more; whole runs of a page and single tokens)
     (1, 1, 1, 1, 128, [0], 16), (1, 1, 32, 32, 128, [1], 16), (1, 1, 32, 32, 128, [300], 16), (1, 1, 8, 1, 64, [63], 16), (1, 1, 8, 1, 64, [64], 16),
     (2, 1, 8, 8, 64, [65, 0], 1), (3, 5, 32, 8, 128, [0, 1000, 17], 16), (1, 64, 64, 8, 128, [500], 48), (2, 64, 8, 8, 64, [129, 2048], 64), (1, 16, 1, 1, 128, [4097], 24),
     (4, 7, 10, 2, 128, [5, 6, 7, 8], 3), (2, 33, 9, 3, 64, [100, 31], 7), (1, 3, 64, 1, 128, [1025], 256), (5, 2, 4, 4, 128, [900, 3, 64, 128, 127], 128),
@@ -155,6 +155,16 @@ def test_one_mask_for_all_and_strided_tensors():
     out = torch.zeros((3, 8, 4, 128), dtype=torch.float16, device="cuda").transpose(1, 2)
     fm.tree_attention(*(y[n] for n in ("q", "k", "v", "k_cache", "v_cache", "page_table", "lengths", "tree")), out)
     assert torch.equal(out, one)
+
+
+def test_strides_of_single_places():
+    """One sequence, one token, one head of keys, one page: whatever their strides are."""
+    x = _inputs(1, 1, 4, 1, 64, [9], 16, spare=0)
+    expect = _run(x)
+    for n, at in (("k", (0, 1, 2)), ("v", (0, 1, 2)), ("k_cache", (0, 2)), ("v_cache", (0, 2)), ("q", (0, 1))):
+        steps = [1 if i in at else s for i, s in enumerate(x[n].stride())]
+        x[n] = x[n].contiguous().as_strided(x[n].shape, steps)
+    assert torch.equal(_run(x), expect)
 
 
 def test_lengths_and_pages_out_of_range():
