@@ -40,7 +40,7 @@ struct TreeCfg {
   static constexpr int kStageBytes = 2 * kTileBytes, kHalfBytes = 2 * kKeys * 128;     // [half of a row][128 keys][64 values]
   static constexpr int kExchange = kRowTile * 32 * 4;        // 32 columns of a group's sums
   static constexpr int kNumBars = 2 * kKeyStages + 2 * kValueStages + 2 + 2 + 2 + 2;
-  static constexpr int kQ = 0, kK = (kPair ? 2 : 1) * kQBytes, kV = kK + kKeyStages * kStageBytes, kX = kV + kValueStages * kStageBytes;
+  static constexpr int kK = 0, kQ = kKeyStages * kStageBytes, kV = kQ + (kPair ? 2 : 1) * kQBytes, kX = kV + kValueStages * kStageBytes;
   static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
   static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
   static constexpr int kBars = kPlaces + 4 * kKeys * 8;
@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   const int ctas = plan.ctas;
   const bool works = cta < ctas;
   bool dead = false;
-  // Up to 64 rows there is room for the queries of two items; a row tile is 128 rows all the same, what the others hold is nobody's.
+  // Up to 64 rows there is room for the queries of two items; a row tile is 128 rows all the same, what the others hold is nobody's.  The first group
+  // has the rows in the first 64 lanes then and the second in the last, so that their warps share no quarter of the multiprocessor.
   const int q_rows = !kPair && p.rows <= 64 ? 64 : kRowTile, q_sets = !kPair && p.rows <= 64 ? 2 : 1;
   const uint32_t q_bytes = q_rows * D * 2;                           // of a row tile; halves of a row of 128 values lie q_rows * 128 bytes apart
 
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         const int set = q_sets == 2 ? segment & 1 : 0;
         if (!kPair || w == 0) front.wait(full_k, fresh, p.status, dead);
         fresh = false;
-        const uint64_t k_desc = rows_desc(base + C::kK + front.stage * C::kStageBytes), q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * q_bytes);
+        const uint64_t k_desc = rows_desc(base + C::kK + front.stage * C::kStageBytes), q_desc = rows_desc(base + C::kQ + (kPair ? w : set) * q_bytes - (q_sets == 2 && w == 1 ? 64 * 128 : 0));
         const uint32_t idesc = front.left > 1 ? idesc_s2 : idesc_s;
         const bool whole_job = !kPair || w + 1 == front.groups;
         if (elect_one()) {
@@ -407,7 +408,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       }
     } else if (warp >= 8) {
       // ================================================================== weights: thread = row
-      const int group = (warp - 8) >> 2, quarter = warp & 3, row_in = quarter * 32 + lane;
+      const int group = (warp - 8) >> 2, quarter = warp & 3, first_lane = q_sets == 2 && group == 1 ? 64 : 0;
+      const int row_in = quarter * 32 + lane - first_lane;           // negative: nobody's
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
       const uint32_t my_scores = tmem + lanes + group * 128, my_sums = tmem_o + lanes + group * 128;
       const float sl = fabsf(p.scale_log2);                          // its sign is in the scores
@@ -418,8 +420,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         ++segment;
         const int g = seg.item / p.parts, row_tile = kPair ? seg.item % p.parts * 2 + group : seg.item % p.parts;
         const int row = row_tile * kRowTile + row_in;
-        const bool row_lives = row < p.rows;
-        const bool warp_lives = row_tile * kRowTile + quarter * 32 < p.rows;
+        const bool warp_lives = quarter * 32 >= first_lane && row_tile * kRowTile + quarter * 32 - first_lane < p.rows;
+        const bool row_lives = row_in >= 0 && row < p.rows;
         const int t = row_lives ? row / p.group : 0, head = g * p.group + (row_lives ? row - t * p.group : 0);
         const unsigned long long mask = row_lives ? mask_of(p, seg.b, t) : 0;
         float top = -INFINITY, total = 0.f;                          // the maximum that the weights are relative to
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         float mine = 1.f, theirs = 0.f;
         if (!kPair) {
           // the second group hands its maxima, totals and sums to the first
-          if (group == 1) {
+          if (group == 1 && row_in >= 0) {
             stats[row_in] = top;
             stats[kRowTile + row_in] = total;
           }
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
           if (!kPair) {
-            if (group == 1) {
+            if (group == 1 && row_in >= 0) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) exchange[i * kRowTile + row_in] = make_float4(as_float(o[4 * i]), as_float(o[4 * i + 1]), as_float(o[4 * i + 2]), as_float(o[4 * i + 3]));
             }
