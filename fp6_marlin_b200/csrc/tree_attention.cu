@@ -107,16 +107,30 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
       copy16(to + kTileBytes, v ? v + chunk * 8 : static_cast<const T*>(a.q), v ? 16 : 0);
     }
   };
-  put_place(look_up(), 0);
+  int page = look_up();
+  // (the page of the next tile is looked up before the place of this one is worked out: the first two look-ups take one latency)
+  auto look_up_next = [&] {
+    const Segments before = ahead;
+    const int tile_before = ahead_tile;
+    const bool lived = ahead_lives;
+    advance();
+    const int next = look_up();
+    ahead = before;
+    ahead_tile = tile_before;
+    ahead_lives = lived;
+    return next;
+  };
+  int next_page = look_up_next();
+  put_place(page, 0);
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
     __syncthreads();
     const bool live = ahead_lives;
     advance();
-    const int page = look_up();
+    if (s > 0) next_page = look_up();
     if (live) copy(s, s & 1);
     copies_commit();
-    put_place(page, (s + 1) & 1);
+    put_place(next_page, (s + 1) & 1);
   }
 
   const int quad = lane >> 2, col = (lane & 3) * 2;                  // this thread's rows quad and quad + 8, columns col and col + 1 of a fragment
@@ -338,6 +352,25 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
           top[h] = m;
           total[h] = sum;
         }
+        if (kKeyWarps == 4 && p.rows <= 4) {
+          // there is room for the rows of all warps at once
+          if (key_warp > 0 && quad < p.rows) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(pool + ((key_warp - 1) * 4 + quad) * D + i * 8 + col) = make_float2(o[i][0], o[i][1]);
+          }
+          __syncthreads();
+          if (key_warp == 0 && quad < p.rows) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+              for (int w = 2; w >= 0; --w) {
+                const float2 more = *reinterpret_cast<const float2*>(pool + (w * 4 + quad) * D + i * 8 + col);
+                o[i][0] += more.x;
+                o[i][1] += more.y;
+              }
+          }
+          __syncthreads();
+        } else {
 #pragma unroll
         for (int part = 0; part < kRowWarps; ++part) {
 #pragma unroll
@@ -359,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             }
             __syncthreads();
           }
+        }
         }
       }
       const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
