@@ -22,7 +22,8 @@ constexpr int kStripBytes = kBlock * kBlock;
 constexpr int kMaxFp8Ctas = 192;         // one CTA per multiprocessor
 // The scratch: launch epoch and counters, then the tagged words of the kernel for few rows, then the sums of the other.  Each keeps to
 // its own part: sums must not be taken for tags.
-constexpr int kMostColumnsRows = 64;     // rows of A of the kernel for few rows
+// Rows of A of the kernel for few rows: LINE64
+constexpr int kMostColumnsRows = 64;
 constexpr size_t kFp8Header = (kEpochWords + kMaxFp8Ctas) * sizeof(unsigned int);
 constexpr size_t kRowsScratch = kFp8Header + (size_t)kMaxFp8Ctas * kMostColumnsRows * kBlock * sizeof(unsigned long long);
 

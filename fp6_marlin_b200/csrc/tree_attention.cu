@@ -11,6 +11,12 @@
 // cut is made on the device, from the lengths, and the launch does not depend on them.  One pass over the keys keeps a
 // running maximum and sum per row in fp32.  Rows whose keys are shared by several CTAs are joined by the one that finishes
 // last (an arrival counter; nobody waits), in the order of the ranges, so results do not depend on who that is.
+//
+// This file: up to 32 rows per head of keys, where mma.sync keeps up with memory (rows are padded to 16 or 32, a tile of tcgen05 would have 128) and what counts is
+// the time from a key's arrival to its use.  Two CTAs per multiprocessor, three tiles of keys and values on their way in each.  8 x 5 tokens, 32 heads, up to
+// 4096 cached: 55 us, 4.9 TB/s, 0.75 of what a copy reaches; bound by the instructions between two tiles (about 1660 cycles a tile and CTA) and
+// the tails of CTAs.  One token over 300: 10.4 us where the bytes take 0.8: the plan (2000 cycles), first look-ups and queries (2900), first data
+// (1200), two or three tiles, the end (1700).
 #include "device_utils.cuh"
 #include "host_common.h"
 #include "tree_attention.cuh"
@@ -21,8 +27,17 @@ using namespace fp6m;
 
 constexpr int kThreads = 128;
 constexpr int kMaxCtas = 512;
-constexpr int kLeastUnits = 3, kSlack = 8;       // see make_plan
-constexpr int kCounterBytes = kMaxCtas * 4;
+// see make_plan.  us with a slack of 4 / 8 / 16: one token over 300, 32 heads 12.9 / 12.2 / 12.2; four over 500 13.4 / 13.3 / 15.6.
+// With at least 3 / 6 units per CTA: one token over 1000, 32 heads over 8, 12.9 / 17.0; sixteen over up to 500 13.4 / 15.4; one over 8000 17.9 / 19.1.
+constexpr int kLeastUnits = 3, kSlack = 8;
+constexpr int kCounterBytes = kMaxCtas * 2 * 3 * 4;
+// contributors of a group: see Joining
+__device__ __forceinline__ int join_step(int count) {
+  if (count <= 24) return count;
+  int step = 8;
+  while (step * step < count) step += 8;
+  return step;
+}
 
 template <class T> struct Mma;
 template <> struct Mma<half> {
@@ -435,45 +450,103 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
         }
         const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
         const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          const unsigned int before = atomicAdd(p.arrived + first_cta, 1u);
-          const bool is_last = before == (unsigned)(last_cta - first_cta);
-          if (is_last) p.arrived[first_cta] = 0;                     // for the next launch
-          flags[1] = is_last;
-        }
-        __syncthreads();
-        if (flags[1]) {
+        const Joining join(first_cta, last_cta, cta, join_step(last_cta - first_cta + 1));
+        // whether this CTA is the last of those that a counter waits for; what the others wrote is visible then
+        auto last_at = [&](unsigned int* counter, int others) {
           __threadfence();
-          // a warp per row, sixteen or eight bytes a lane
-          constexpr int V = D / 32;
-          for (int r = warp; r < p.rows; r += 4) {
-            float m = -INFINITY, sum = 0.f, acc[V] = {};
-            for (int c = first_cta; c <= last_cta; ++c) {
-              const float* from = p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot;
-              const float cm = __ldcg(from + kRowTile * D + r), ct = __ldcg(from + kRowTile * (D + 1) + r);
-              float v[V];
-#pragma unroll
-              for (int i = 0; i < V; i += 2) {
-                const float2 two = __ldcg(reinterpret_cast<const float2*>(from + r * D + lane * V + i));
-                v[i] = two.x;
-                v[i + 1] = two.y;
-              }
-              const float now = fmaxf(m, cm), base = now == -INFINITY ? 0.f : now;
-              const float old = exp2_approx(m - base), add = exp2_approx(cm - base);
-              sum = sum * old + ct * add;
-#pragma unroll
-              for (int i = 0; i < V; ++i) acc[i] = acc[i] * old + v[i] * add;
-              m = now;
-            }
-            const int t = r / p.group;
-            const bool none = mask_of(p, seg.b, t) == 0 || sum == 0.f;
-            const float f = 1.f / sum;
-            T* out = out_row(r) + lane * V;
-#pragma unroll
-            for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[i] * f, acc[i + 1] * f);
+          __syncthreads();
+          if (tid == 0) {
+            const bool is_last = atomicAdd(counter, 1u) == (unsigned)others;
+            if (is_last) *counter = 0;                               // for the next launch
+            flags[1] = is_last;
           }
+          __syncthreads();
+          const bool is_last = flags[1] != 0;
+          __threadfence();
+          return is_last;
+        };
+        auto slot_of = [&](int c) { return p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot; };
+        // Joins `count` partials, `step` CTAs apart: into the output, or into the first one's slot.  A warp has two rows at a time, a lane four or two columns of
+        // each; a lane fetches the maximum and total of one contributor, and eight contributors' sums are on their way together (one after the other took
+        // a latency each; 24 rows of 19 contributors: 43 us in all then, 35 now).
+        auto add_up = [&](int c0, int count, int step, bool ends) {
+          constexpr int V = D / 32, kTogether = 8;
+          for (int r0 = warp; r0 < p.rows; r0 += 8) {
+            float m[2] = {-INFINITY, -INFINITY}, sum[2] = {}, acc[2][V] = {};
+            const int rows[2] = {r0, r0 + 4 < p.rows ? r0 + 4 : r0};
+            for (int k0 = 0; k0 < count; k0 += 32) {
+              const int here = min(count - k0, 32);
+              float by[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float* from = slot_of(c0 + (k0 + min(lane, here - 1)) * step) + kRowTile * D + rows[h];
+                const float cm = lane < here ? __ldcg(from) : -INFINITY, ct = lane < here ? __ldcg(from + kRowTile) : 0.f;
+                float most = cm;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float now = fmaxf(m[h], most), base = now == -INFINITY ? 0.f : now, old = exp2_approx(m[h] - base);
+                by[h] = exp2_approx(cm - base);
+                float part = ct * by[h];
+#pragma unroll
+                for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+                sum[h] = sum[h] * old + part;
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[h][i] *= old;
+                m[h] = now;
+              }
+              for (int j0 = 0; j0 < here; j0 += kTogether) {
+                float2 v[kTogether][2][V / 2];
+#pragma unroll
+                for (int e = 0; e < kTogether; ++e)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i)
+                      v[e][h][i] = j0 + e < here ? __ldcg(reinterpret_cast<const float2*>(slot_of(c0 + (k0 + j0 + e) * step) + rows[h] * D + lane * V) + i) : make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < kTogether; ++e)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const float f = __shfl_sync(0xffffffffu, by[h], (j0 + e) & 31);
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i) {
+                      acc[h][2 * i] = fmaf(v[e][h][i].x, f, acc[h][2 * i]);
+                      acc[h][2 * i + 1] = fmaf(v[e][h][i].y, f, acc[h][2 * i + 1]);
+                    }
+                  }
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = r0 + 4 * h;
+              if (r >= p.rows) break;
+              if (ends) {
+                const int t = r / p.group;
+                const bool none = mask_of(p, seg.b, t) == 0 || sum[h] == 0.f;      // padding, and rows that see nothing, are zero
+                const float f = 1.f / sum[h];
+                T* out = out_row(r) + lane * V;
+#pragma unroll
+                for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[h][i] * f, acc[h][i + 1] * f);
+              } else {
+                float* to = slot_of(c0);
+#pragma unroll
+                for (int i = 0; i < V; i += 2) __stcg(reinterpret_cast<float2*>(to + r * D + lane * V + i), make_float2(acc[h][i], acc[h][i + 1]));
+                if (lane == 0) {
+                  __stcg(to + kRowTile * D + r, m[h]);
+                  __stcg(to + kRowTile * (D + 1) + r, sum[h]);
+                }
+              }
+            }
+          }
+        };
+        // (one loop, so that its code is there once: what runs for the first time takes longer to fetch than to run)
+        const bool grouped = join.step < join.count;
+        bool ends = !grouped;
+#pragma unroll 1
+        while (last_at(ends && grouped ? join.item_counter(p, 0) : join.group_counter(p, 0), (ends && grouped ? join.groups() : join.size) - 1)) {
+          add_up(ends ? first_cta : join.group, ends && grouped ? join.groups() : join.size, ends && grouped ? join.step : 1, ends);
+          if (ends) break;
+          ends = true;
         }
       }
   }

@@ -21,12 +21,13 @@ struct TreeParams {
   int page_shift;
   int run;                               // tokens of a page that one TMA copy brings (0: none does)
   float scale_log2;                      // scale * log2(e): the softmax is computed in powers of two
-  unsigned int* arrived;                 // contributors that have left their partial for the rows that start in a CTA
+  unsigned int* arrived;                 // [CTA][row tile of two][3] contributors that have left their partial, see Joining
   float* partials;
   int* status;
 };
 
-// tree_attention_tc5.cu: more rows than kFewRows
+// tree_attention_tc5.cu: more rows than kFewRows.  us for 20 to 32 rows, few / many: 8 x 4 tokens, 32 heads over 4, 2048 cached 27.8 / 26.4;
+// 2 x 3, 64 over 8, 8192: 34.9 / 36.7; 64 x 4, 64 over 8, up to 4096: 114.2 / 114.7; 16 x 5, 32 over 8, up to 4000: 41.4 / 44.4.
 constexpr int kFewRows = 32;
 size_t tree_tc5_partial_bytes(int sms);
 cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream);
@@ -156,6 +157,24 @@ struct Segments {
     }
     return false;
   }
+};
+
+// How the partials of an item's contributors (the CTAs first .. last) become one: by the contributor that is the last to leave its own, all of them in
+// their order - or, where they are many, in groups of `step` first: the last of a group leaves the sum in the slot of its first, and the
+// last of those adds up the groups.  Every group has a counter, at its first CTA: [0] the item starts there, [1] it started before
+// (a CTA has one such item at most); [2] counts the groups, where the item starts.  Nobody waits, and the order of the sums is the ranges'.
+struct Joining {
+  int first, count, step, group, size;   // the item's contributors; this CTA's group's first, and how many it has
+  __device__ __forceinline__ Joining(int first_cta, int last_cta, int cta, int step_) {
+    first = first_cta;
+    count = last_cta - first_cta + 1;
+    step = step_;
+    group = first + (cta - first) / step * step;
+    size = min(step, last_cta + 1 - group);
+  }
+  __device__ __forceinline__ int groups() const { return (count + step - 1) / step; }
+  __device__ __forceinline__ unsigned int* group_counter(const TreeParams& p, int which) const { return p.arrived + (group * 2 + which) * 3 + (group == first ? 0 : 1); }
+  __device__ __forceinline__ unsigned int* item_counter(const TreeParams& p, int which) const { return p.arrived + (first * 2 + which) * 3 + 2; }
 };
 
 // The first value of key (or value) j of a sequence, null where there is none: behind the last one, or in a page that does not exist.

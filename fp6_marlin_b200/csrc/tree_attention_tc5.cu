@@ -10,6 +10,13 @@
 //
 // O is rescaled only where a row's maximum grows by more than a factor of 2^8: until then the weights are taken relative to the older
 // maximum, which changes neither the result nor, in fp32 sums and 16-bit floating-point weights, its precision.
+//
+// 2 x 64 tokens, 64 heads over 8, up to 32768 cached: 172 us, 800 TFLOP/s, 0.48 of what a library product reaches.  A job takes a pair of row tiles about 4700 cycles, the
+// tensor cores 2048 of them: a group's weights take 2400 (the maxima 290, then 128 exponentials at 1660 to 2000: 660 of other instructions and 1024 of the unit for
+// special functions, which a single warp per quarter does not overlap), then it waits for its product and its next scores, because tensor memory holds one
+// tile of scores per group beside the sums.  Measured and not kept: a fourth, an eighth or a sixteenth of the exponentials by a polynomial (+3, +1, 0 %),
+// sums and exponents in pairs (0), exponentials of one chunk between the sums of the last (+5 %, with or without registers moved to these warps).  The copies take 4 %.
+// 64 x 7 tokens, 64 heads over 8, up to 6144: 163 us, 5.0 TB/s, 0.77 of what a copy reaches.
 #include <type_traits>
 
 #include "../../include/fp6m.h"
@@ -26,7 +33,8 @@ namespace {
 constexpr int kRowTile = 128;
 constexpr int kMostTreeCtas = 192;       // one per multiprocessor
 constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs (three idle), twice four that compute weights
-constexpr int kSlack = 32;               // see make_plan
+constexpr int kSlack = 32;               // see make_plan; us with 8 / 32: four sequences of eight tokens over 1000, 32 heads over 8, 23.3 / 18.6
+constexpr int kLeastUnits = 3;           // us with 3 / 8 / 16: four sequences of eight tokens, up to 3000 cached, 25.7 / 35.4 / 29.8; one over 8000, 30.0 / 35.5 / 28.6
 constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass
 
 template <int D_, bool PAIR_>
@@ -48,6 +56,14 @@ struct TreeCfg {
   static constexpr int kSlotFloats = kRowTile * (D + 2) + 4; // a partial: sums [4 columns][row], maxima, totals, whether odd values were met
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
+// Contributors of a group, see Joining.  Eight tokens over 8000, 32 heads over 4 (37 contributors): 66 us with all of them one after the other, 30 in two steps;
+// four sequences of eight, up to 3000: 38 and 26.
+__device__ __forceinline__ int join_step(int count) {
+  if (count <= 8) return count;
+  int step = 4;
+  while (step * step < count) ++step;
+  return step;
+}
 constexpr int kOddRing = 32;             // segments: more than the copies can be ahead of the sums
 
 // What was written to shared memory by copies and stores is seen by the MMAs that follow.  It stands where the MMAs are issued, behind the
@@ -147,7 +163,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   launch_dependents();
   grid_dependency_wait();
   const int cta = blockIdx.x;
-  if (warp == 0) make_plan(p, &plan, 3, kSlack);
+  if (warp == 0) make_plan(p, &plan, kLeastUnits, kSlack);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -421,9 +437,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         const int g = seg.item / p.parts, row_tile = kPair ? seg.item % p.parts * 2 + group : seg.item % p.parts;
         const int row = row_tile * kRowTile + row_in;
         const bool warp_lives = quarter * 32 >= first_lane && row_tile * kRowTile + quarter * 32 - first_lane < p.rows;
-        const bool row_lives = row_in >= 0 && row < p.rows;
+        bool row_lives = row_in >= 0 && row < p.rows;
         const int t = row_lives ? row / p.group : 0, head = g * p.group + (row_lives ? row - t * p.group : 0);
-        const unsigned long long mask = row_lives ? mask_of(p, seg.b, t) : 0;
+        unsigned long long mask = row_lives ? mask_of(p, seg.b, t) : 0;
         float top = -INFINITY, total = 0.f;                          // the maximum that the weights are relative to
         bool any = false;                                            // the sums hold something
         const bool group_lives = !kPair || row_tile < p.row_tiles;
@@ -646,62 +662,119 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         if (row_in == 0) reinterpret_cast<int*>(slot)[kRowTile * (D + 2)] = odd;
         const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
         const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
-        __threadfence();
-        named_bar_sync(4 + which, 128);
-        if (row_in == 0) {
-          unsigned int* counter = p.arrived + first_cta * 2 + which;
-          const bool is_last = atomicAdd(counter, 1u) == (unsigned)(last_cta - first_cta);
-          if (is_last) *counter = 0;                                 // for the next launch
-          misc[2 + which] = is_last;
-        }
-        named_bar_sync(4 + which, 128);
-        if (!misc[2 + which]) continue;
-        __threadfence();
-        // (two contributors at a time: what this takes is the latency of its loads)
-        float m = -INFINITY, sum = 0.f;
-        odd = false;
-#pragma unroll 2
-        for (int c = first_cta; c <= last_cta; ++c) {
-          const float* from = slot_of(c, c == first_cta);
-          const float cm = __ldcg(from + kRowTile * D + row_in), ct = __ldcg(from + kRowTile * (D + 1) + row_in);
-          odd = odd || __ldcg(reinterpret_cast<const int*>(from) + kRowTile * (D + 2)) != 0;
-          const float now = fmaxf(m, cm), base_log2 = now == -INFINITY ? 0.f : now;
-          sum = sum * exp2_approx(m - base_log2) + ct * exp2_approx(cm - base_log2);
-          m = now;
-        }
-        const float base_log2 = m == -INFINITY ? 0.f : m;
-        if (warp_lives) {
+        const Joining join(first_cta, last_cta, cta, join_step(last_cta - first_cta + 1));
+        // whether this CTA is the last of those that a counter waits for; what the others wrote is visible then
+        auto last_at = [&](unsigned int* counter, int others) {
+          __threadfence();
+          named_bar_sync(4 + which, 128);
+          if (row_in == 0) {
+            const bool is_last = atomicAdd(counter, 1u) == (unsigned)others;
+            if (is_last) *counter = 0;                               // for the next launch
+            misc[2 + which] = is_last;
+          }
+          named_bar_sync(4 + which, 128);
+          const bool is_last = misc[2 + which] != 0;
+          __threadfence();
+          return is_last;
+        };
+        // Up to 64 rows, two threads share a row when partials are joined.
+        const bool shared = q_sets == 2;
+        const int join_row = shared ? row_in & 63 : row_in, c_begin = shared ? row_in / 64 * (D / 2) : 0, c_end = shared ? c_begin + D / 2 : D;
+        // Joins `count` partials, `step` CTAs apart: into the output, or into the first one's slot.
+        auto add_up = [&](int c0, int count, int step, bool ends) {
+          const int last = c0 + (count - 1) * step;
+          auto from = [&](int k) {
+            const int c = min(c0 + k * step, last);
+            return slot_of(c, c == first_cta);
+          };
+          float m = -INFINITY, sum = 0.f;
+          bool odd = false;
+          for (int k = 0; k < count; k += 4) {
+            float cm[4], ct[4], most = m;
+            int any_odd = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float* at = from(k + e);
+              cm[e] = __ldcg(at + kRowTile * D + join_row);
+              ct[e] = __ldcg(at + kRowTile * (D + 1) + join_row);
+              any_odd |= __ldcg(reinterpret_cast<const int*>(at) + kRowTile * (D + 2));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k + e < count) most = fmaxf(most, cm[e]);
+            const float base_log2 = most == -INFINITY ? 0.f : most;
+            sum *= exp2_approx(m - base_log2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k + e < count) sum += ct[e] * exp2_approx(cm[e] - base_log2);
+            m = most;
+            odd = odd || any_odd != 0;
+          }
+          const float base_log2 = m == -INFINITY ? 0.f : m;
+          float* to = slot_of(c0, c0 == first_cta);
+          if (row_tile * kRowTile + join_row < p.rows) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            float v[32];
+            for (int c = c_begin; c < c_end; c += 32) {
+              float v[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
+              // (two contributors at a time: what this takes is the latency of its loads)
 #pragma unroll 1
-            for (int c = first_cta; c <= last_cta; c += 2) {
-              float by[2];
-              float4 x[2][8];
+              for (int k = 0; k < count; k += 2) {
+                float by[2];
+                float4 x[2][8];
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float* from = slot_of(min(c + e, last_cta), c + e == first_cta);
-                const float4* at = reinterpret_cast<const float4*>(from) + c0 / 4 * kRowTile + row_in;
-                by[e] = __ldcg(from + kRowTile * D + row_in);
+                for (int e = 0; e < 2; ++e) {
+                  const float4* at = reinterpret_cast<const float4*>(from(k + e)) + c / 4 * kRowTile + join_row;
+                  by[e] = __ldcg(from(k + e) + kRowTile * D + join_row);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[e][i] = __ldcg(at + i * kRowTile);
-              }
+                  for (int i = 0; i < 8; ++i) x[e][i] = __ldcg(at + i * kRowTile);
+                }
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float f = c + e <= last_cta ? exp2_approx(by[e] - base_log2) : 0.f;
+                for (int e = 0; e < 2; ++e) {
+                  if (k + e >= count) continue;
+                  const float f = exp2_approx(by[e] - base_log2);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  v[4 * i] = fmaf(x[e][i].x, f, v[4 * i]);
-                  v[4 * i + 1] = fmaf(x[e][i].y, f, v[4 * i + 1]);
-                  v[4 * i + 2] = fmaf(x[e][i].z, f, v[4 * i + 2]);
-                  v[4 * i + 3] = fmaf(x[e][i].w, f, v[4 * i + 3]);
+                  for (int i = 0; i < 8; ++i) {
+                    v[4 * i] = fmaf(x[e][i].x, f, v[4 * i]);
+                    v[4 * i + 1] = fmaf(x[e][i].y, f, v[4 * i + 1]);
+                    v[4 * i + 2] = fmaf(x[e][i].z, f, v[4 * i + 2]);
+                    v[4 * i + 3] = fmaf(x[e][i].w, f, v[4 * i + 3]);
+                  }
                 }
               }
+              if (ends) {
+                put(v, c, 1.f / sum, mask == 0 || sum == 0.f, odd);
+              } else {
+                float4* at = reinterpret_cast<float4*>(to) + c / 4 * kRowTile + join_row;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) __stcg(at + i * kRowTile, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+              }
             }
-            put(v, c0, 1.f / sum, mask == 0 || sum == 0.f, odd);
           }
+          if (ends) return;
+          named_bar_sync(4 + which, 128);                            // all have read the first one's maxima
+          if (c_begin == 0) {
+            __stcg(to + kRowTile * D + join_row, m);
+            __stcg(to + kRowTile * (D + 1) + join_row, sum);
+            if (row_in == 0) __stcg(reinterpret_cast<int*>(to) + kRowTile * (D + 2), odd ? 1 : 0);
+          }
+        };
+        if (shared) {
+          // the row that this thread joins, in place of its own
+          row_lives = join_row < p.rows;
+          const int join_t = row_lives ? join_row / p.group : 0;
+          mask = row_lives ? mask_of(p, seg.b, join_t) : 0;
+          out = static_cast<T*>(a.out) + seg.b * a.out_stride[0] + join_t * a.out_stride[1] + (g * p.group + (row_lives ? join_row - join_t * p.group : 0)) * a.out_stride[2];
+        }
+        // (one loop, so that its code is there once: what runs for the first time takes longer to fetch than to run)
+        const bool grouped = join.step < join.count;
+        bool ends = !grouped;
+#pragma unroll 1
+        while (last_at(ends && grouped ? join.item_counter(p, which) : join.group_counter(p, which), (ends && grouped ? join.groups() : join.size) - 1)) {
+          add_up(ends ? first_cta : join.group, ends && grouped ? join.groups() : join.size, ends && grouped ? join.step : 1, ends);
+          if (ends) break;
+          ends = true;
         }
       }
     }

@@ -94,6 +94,21 @@ def test_attention(b, t, h, g, d, lengths, page, dtype):
     assert torch.equal(out, _run(x)) and fm.device_status() == 0
 
 
+@pytest.mark.parametrize("t,h,g,d", [(1, 4, 1, 128), (8, 32, 4, 128), (7, 8, 1, 64), (16, 8, 1, 128), (40, 8, 2, 64)])
+def test_rows_joined_from_many_ranges(t, h, g, d):
+    """One long sequence and few heads of keys: every multiprocessor leaves a part of the same rows; few and many rows after one another."""
+    x, other = _inputs(1, t, h, g, d, [12345], 16, torch.bfloat16), _inputs(1, 3, 2, 1, d, [4321], 16, torch.bfloat16)
+    first, first_other = _run(x), _run(other)
+    _check(first, x)
+    _check(first_other, other)
+    for _ in range(5):
+        assert torch.equal(_run(x), first) and torch.equal(_run(other), first_other)
+    x["v"][0, 0, 0, 3] = float("inf")                                # it reaches the rows that see it through the joined parts as well
+    heads = h // g
+    out, sees = _run(x)[0].float(), (x["tree"].reshape(-1) & 1).bool()
+    assert (out[:, :heads, 3].isposinf() == sees[:, None]).all() and out[~sees].isfinite().all() and fm.device_status() == 0
+
+
 @pytest.mark.parametrize("lengths", [[0, 0], [200, 0], [65, 1300]])
 def test_padding_and_rows_that_see_nothing(lengths):
     x = _inputs(2, 6, 8, 2, 128, lengths, 16, fill=float("inf"))
