@@ -22,7 +22,8 @@ constexpr int kStripBytes = kBlock * kBlock;
 constexpr int kMaxFp8Ctas = 192;         // one CTA per multiprocessor
 // The scratch: launch epoch and counters, then the tagged words of the kernel for few rows, then the sums of the other.  Each keeps to
 // its own part: sums must not be taken for tags.
-// Rows of A of the kernel for few rows: LINE64
+// Most rows of A of the kernel for few rows.  us, few / many (rows x K x columns): 33 x 4096 x 4096 12.1 / 11.7, 64 x 4096 x 4096 13.0 / 11.9, 48 x 11008 x 4096
+// 17.5 / 20.6, 64 x 8192 x 57344 87 / 97.
 constexpr int kMostColumnsRows = 64;
 constexpr size_t kFp8Header = (kEpochWords + kMaxFp8Ctas) * sizeof(unsigned int);
 constexpr size_t kRowsScratch = kFp8Header + (size_t)kMaxFp8Ctas * kMostColumnsRows * kBlock * sizeof(unsigned long long);
