@@ -93,34 +93,11 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uin
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
                : "memory");
 }
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-      "%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-               : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
                "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
                : "memory");
 }
-// waits for the loads; the registers pass through, so that nothing that uses them can be moved in front of the wait
-template <int kCount>
-__device__ __forceinline__ void tmem_loaded(uint32_t* r) {
-  tc_wait_ld();
-#pragma unroll
-  for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(r[i]));
-}
-__device__ __forceinline__ void tmem_loaded32(uint32_t* r) { tmem_loaded<32>(r); }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
 
 template <class T, class C>
@@ -491,14 +468,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
                   m3 = fmaxf(m3, fmaxf(as_float(s[i + 6]), as_float(s[i + 7])));
                 }
               };
-              tmem_load32(my_scores, v0);
+              tmem_load<32>(my_scores, v0);
 #pragma unroll 1
               for (int c = 0; c < chunks; c += 2) {
-                tmem_loaded32(v0);
-                tmem_load32(my_scores + 32 * (c + 1), v1);
+                tmem_loaded<32>(v0);
+                tmem_load<32>(my_scores + 32 * (c + 1), v1);
                 largest(v0, c);
-                tmem_loaded32(v1);
-                tmem_load32(my_scores + 32 * (c + 2 < chunks ? c + 2 : 0), v0);        // (the last one: the first again)
+                tmem_loaded<32>(v1);
+                tmem_load<32>(my_scores + 32 * (c + 2 < chunks ? c + 2 : 0), v0);        // (the last one: the first again)
                 largest(v1, c + 1);
               }
               const float m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * sl;
@@ -512,7 +489,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
 #pragma unroll 1
                   for (int c = 0; c < D; c += 16) {
                     uint32_t o[16];
-                    tmem_load16(my_sums + c, o);
+                    tmem_load<16>(my_sums + c, o);
                     tmem_loaded<16>(o);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(as_float(o[i]) * keep);
@@ -540,11 +517,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               };
 #pragma unroll 1
               for (int c = 0; c < chunks; c += 2) {
-                tmem_loaded32(v0);
-                tmem_load32(my_scores + 32 * (c + 1), v1);
+                tmem_loaded<32>(v0);
+                tmem_load<32>(my_scores + 32 * (c + 1), v1);
                 exponentials(v0, c);
-                tmem_loaded32(v1);
-                if (c + 2 < chunks) tmem_load32(my_scores + 32 * (c + 2), v0);
+                tmem_loaded<32>(v1);
+                if (c + 2 < chunks) tmem_load<32>(my_scores + 32 * (c + 2), v0);
                 exponentials(v1, c + 1);
               }
               total += (t0 + t1) + (t2 + t3);
@@ -619,8 +596,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t o[32];
           if (any && warp_lives) {
-            tmem_load32(my_sums + c0, o);
-            tmem_loaded32(o);
+            tmem_load<32>(my_sums + c0, o);
+            tmem_loaded<32>(o);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
