@@ -11,12 +11,12 @@
 // O is rescaled only where a row's maximum grows by more than a factor of 2^8: until then the weights are taken relative to the older
 // maximum, which changes neither the result nor, in fp32 sums and 16-bit floating-point weights, its precision.
 //
-// 2 x 64 tokens, 64 heads over 8, up to 32768 cached: 172 us, 800 TFLOP/s, 0.48 of what a library product reaches.  A job takes a pair of row tiles about 4700 cycles, the
+// 2 x 64 tokens, 64 heads over 8, up to 32768 cached: 168 us, 820 TFLOP/s, 0.49 of what a library product reaches.  A job takes a pair of row tiles about 4700 cycles, the
 // tensor cores 2048 of them: a group's weights take 2400 (the maxima 290, then 128 exponentials at 1660 to 2000: 660 of other instructions and 1024 of the unit for
 // special functions, which a single warp per quarter does not overlap), then it waits for its product and its next scores, because tensor memory holds one
 // tile of scores per group beside the sums.  Measured and not kept: a fourth, an eighth or a sixteenth of the exponentials by a polynomial (+3, +1, 0 %),
 // sums and exponents in pairs (0), exponentials of one chunk between the sums of the last (+5 %, with or without registers moved to these warps).  The copies take 4 %.
-// 64 x 7 tokens, 64 heads over 8, up to 6144: 163 us, 5.0 TB/s, 0.77 of what a copy reaches.
+// 64 x 7 tokens, 64 heads over 8, up to 6144: 156 us, 5.3 TB/s, 0.80 of what a copy reaches.
 #include <type_traits>
 
 #include "../../include/fp6m.h"
@@ -33,8 +33,10 @@ namespace {
 constexpr int kRowTile = 128;
 constexpr int kMostTreeCtas = 192;       // one per multiprocessor
 constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs (three idle), twice four that compute weights
-constexpr int kSlack = 32;               // see make_plan; us with 8 / 32: four sequences of eight tokens over 1000, 32 heads over 8, 23.3 / 18.6
-constexpr int kLeastUnits = 3;           // us with 3 / 8 / 16: four sequences of eight tokens, up to 3000 cached, 25.7 / 35.4 / 29.8; one over 8000, 30.0 / 35.5 / 28.6
+// See make_plan (a pair's unit takes about twice as long).  us with a slack of 8 / 32: 8 x 16 tokens, 32 heads over 8, up to 2000 cached, 32.3 / 25.9; one of eight over 1000, 32
+// over 4, 19.0 / 15.9; pairs, 16 / 32: one of 64 over 2000, 64 over 8, 38.9 / 47.0.  At least 3 / 6 / 9 units: that one 40.3 / 38.9 / 39.9; one of
+// eight over 8000, 32 over 4, 28.7 / 27.9 / 29.4; four of eight over up to 3000 24.4 / 26.0 / 25.6.
+constexpr int kSlack = 32, kPairSlack = 16, kLeastUnits = 6;
 constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass
 
 template <int D_, bool PAIR_>
@@ -57,9 +59,9 @@ struct TreeCfg {
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 // Contributors of a group, see Joining.  Eight tokens over 8000, 32 heads over 4 (37 contributors): 66 us with all of them one after the other, 30 in two steps;
-// four sequences of eight, up to 3000: 38 and 26.
+// four sequences of eight, up to 3000 (nine): 38 and 26, but with the planning of now 25.2 in one step of up to 12 and 27.0 in two.
 __device__ __forceinline__ int join_step(int count) {
-  if (count <= 8) return count;
+  if (count <= 12) return count;
   int step = 4;
   while (step * step < count) ++step;
   return step;
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   launch_dependents();
   grid_dependency_wait();
   const int cta = blockIdx.x;
-  if (warp == 0) make_plan(p, &plan, kLeastUnits, kSlack);
+  if (warp == 0) make_plan(p, &plan, kLeastUnits, kPair ? kPairSlack : kSlack);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -195,15 +197,22 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
           constexpr int kTiles = kPair ? 2 : 1;
           const int first_row = ahead.item % p.parts * kTiles * kRowTile;
+          // (token and head are counted on: with a division for each row 256 of them took 20,000 cycles)
+          const int r0 = first_row + row0, t0_q = r0 / p.group, step_t = kRowsPerPass / p.group, step_h = kRowsPerPass - step_t * p.group;
+          const long long step = step_t * a.q_stride[1] + step_h * a.q_stride[2], wrap = a.q_stride[1] - p.group * a.q_stride[2];
+          int h = r0 - t0_q * p.group;
+          const T* src = static_cast<const T*>(a.q) + ahead.b * a.q_stride[0] + t0_q * a.q_stride[1] + (g * p.group + h) * a.q_stride[2] + chunk * 8;
+          const uint32_t q_to = base + C::kQ + (kPair ? 0 : set) * q_bytes + (chunk >> 3) * (q_rows * 128);
+#pragma unroll 4
           for (int i = row0; i < kTiles * q_rows; i += kRowsPerPass) {
-            const int r = first_row + i;
-            const T* src = nullptr;
-            if (r < p.rows) {
-              const int t = r / p.group, head = g * p.group + (r - t * p.group);
-              src = static_cast<const T*>(a.q) + ahead.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
+            const bool there = first_row + i < p.rows;
+            copy16(q_to + (kPair ? i / kRowTile : 0) * q_bytes + (i & (q_rows - 1)) * 128 + (((chunk & 7) ^ (i & 7)) * 16), there ? src : static_cast<const T*>(a.q), there ? 16 : 0);
+            src += step;
+            h += step_h;
+            if (h >= p.group) {
+              h -= p.group;
+              src += wrap;
             }
-            const uint32_t to = base + C::kQ + (kPair ? i / kRowTile : set) * q_bytes + (chunk >> 3) * (q_rows * 128) + (i % q_rows) * 128 + (((chunk & 7) ^ (i & 7)) * 16);
-            copy16(to, src ? src + chunk * 8 : static_cast<const T*>(a.q), src ? 16 : 0);
           }
         }
         int pages = 0, pages_next = 0, slot = 0;
