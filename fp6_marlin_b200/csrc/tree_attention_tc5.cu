@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           if (warp_lives) {
             const int chunks = tile + 1 < seg.t1 ? 4 : 2;            // of 32 keys
             const int cached = seg.length - tile * kKeys;            // from the job's first key on
-            const bool hidden = misc[1] != 0;
+            // One answer for the warp: the copies run ahead and set the flag at any time, and the two bodies below hold warp-wide instructions.
+            const bool hidden = __any_sync(0xffffffffu, misc[1] != 0);
             // The largest score, then the weights: scores are read twice, because 128 of them would not stay in registers.  `hides`: some of the job's keys are
             // not seen by every row.  (A branch for every 32 scores, for what is hidden or grows, cost 150 cycles each: the two cases are apart.)
             auto weigh = [&](auto hides) {
