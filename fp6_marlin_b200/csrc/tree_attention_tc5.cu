@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         const int odd_tile = (tile - t0) & 1;
         const uint32_t dst = ring + stage * C::kStageBytes + odd_tile * (kKeys * 128), bar = full + 8 * stage;
         const bool runs = p.run > 0 && (tile + 1) * kKeys <= length;
+        bool missing = false;                                      // this thread has found a page that does not exist
         const bool drafted = values && (tile + 1) * kKeys > length;
         if (runs) {
           const int at = tile & (block_tiles - 1);
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           for (int i = 0; i < tile_runs; ++i) {
             int page = __shfl_sync(0xffffffffu, pages, at * tile_runs + i);
             if ((unsigned)page >= (unsigned)a.pages) {
-              misc[1] = 1;
+              missing = true;
               page = a.pages;                                        // behind the last page the copy reads zeros
             }
             if (kWarpRuns == 1 || (i & 1) == second) {
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         } else {
           const int j = tile * kKeys + me;
           const T* place = place_of<T>(p, ahead, g, j, page_of(p, ahead, j), values);
-          if (!place && j < length) misc[1] = 1;
+          missing = !place && j < length;
           places[parity * kKeys + me] = place;
           named_bar_sync(bar_id, 64);
           if (!odd_tile) mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
@@ -265,7 +266,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           }
           parity ^= 1;
         }
-        if (!drafted) copies_arrive(bar);
+        // The arrival of asynchronous copies does not order a thread's stores, a plain one does.
+        missing = __any_sync(0xffffffffu, missing);
+        if (missing) misc[1] = 1;
+        if (!drafted && missing) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          mbar_arrive(bar);
+        } else if (!drafted) {
+          copies_arrive(bar);
+        }
         if (drafted) {
           // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
           // that see them at the end.
