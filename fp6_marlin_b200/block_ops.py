@@ -229,8 +229,8 @@ def tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, *,
     of G; they may be views of one projection's output.  k_cache and v_cache (pages, page size, G, D): the cache, any
     page size.  page_table (B, P) int32: the pages of each sequence in order; lengths (B,) int32: its committed tokens.
     tree (B, T) or (T,) int64: bit j of entry i says whether drafted token i sees drafted token j (see :func:`tree_masks`); every
-    token sees all committed ones, except that an entry of 0 marks padding, which sees nothing and gives zeros.  With T = 1
-    and tree = 1 this is ordinary decoding.  out: like q, overwritten.  ``scale`` defaults to ``D ** -0.5``.
+    token sees all committed ones, except that an entry of 0 marks padding, which sees nothing and gives zeros.  Bits from T
+    on mean nothing.  With T = 1 and tree = 1 this is ordinary decoding.  out: like q, overwritten.  ``scale`` defaults to ``D ** -0.5``.
 
     Lengths and page numbers stay on the device: lengths are cut to what the page table can hold, and a page number that
     does not exist hides its tokens and is reported by :func:`device_status` (4).  What lies behind a sequence's last

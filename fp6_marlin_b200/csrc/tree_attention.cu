@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int t = j0 + i * 8 + col + (e & 1) - seg.length;      // drafted token, negative: cached
-          if (t >= 0 && (t >= 64 || !(mask[e >> 1] >> t & 1))) s[i][e] = -INFINITY;
+          if (t >= 0 && (t >= a.tokens || !(mask[e >> 1] >> t & 1))) s[i][e] = -INFINITY;
         }
     }
     if (hidden) {
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t bits = e & 1 ? two >> 16 : two & 0xffffu;
-              const bool sees = t >= 0 && t < 64 && (mask[e >> 1] >> t & 1);
+              const bool sees = t >= 0 && t < a.tokens && (mask[e >> 1] >> t & 1);
               if (sees && (bits & Half16<T>::kExponent) == Half16<T>::kExponent) o[i][e] += w[e >> 1] * Half16<T>::value((uint16_t)bits);
             }
           }

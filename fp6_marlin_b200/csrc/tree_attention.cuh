@@ -34,10 +34,8 @@ cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream);
 
 #ifdef __CUDACC__
 
-// The drafted tokens that token t of sequence b sees.
-__device__ __forceinline__ unsigned long long mask_of(const TreeParams& p, int b, int t) {
-  return p.a.tree[b * p.a.tree_stride + t] & (~0ull >> (64 - p.a.tokens));
-}
+// The mask of token t of sequence b: the drafted tokens that it sees (bits behind the last of them mean nothing), 0 for padding.
+__device__ __forceinline__ unsigned long long mask_of(const TreeParams& p, int b, int t) { return p.a.tree[b * p.a.tree_stride + t]; }
 __device__ __forceinline__ int length_of(const TreeParams& p, int b) {
   const int n = p.a.lengths[b], most = p.a.max_pages * p.a.page_size;
   return n < 0 ? 0 : n > most ? most : n;

@@ -454,11 +454,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               // The row sees all cached keys, then those of its mask; the score of another is the lowest there is.
               uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
               if constexpr (kHides) {
+                const unsigned long long drafted = mask & (~0ull >> (64 - a.tokens));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   const int here = cached - h * kKeys;
                   unsigned long long word = ~0ull;
-                  if (here < kKeys) word = here > 0 ? mask << here | ((1ull << here) - 1) : here > -64 ? mask >> -here : 0ull;
+                  if (here < kKeys) word = here > 0 ? drafted << here | ((1ull << here) - 1) : here > -64 ? drafted >> -here : 0ull;
                   if (hidden) {
                     for (int i = 0; i < min(here, kKeys); ++i)
                       if ((unsigned)page_of(p, seg, (tile + h) * kKeys + i) >= (unsigned)a.pages) word &= ~(1ull << i);

@@ -267,3 +267,16 @@ def test_nothing_to_do_and_refusals():
     big = _inputs(1, 64, 2, 2, 64, [5], 16)
     with pytest.raises(RuntimeError):
         fm.tree_attention(*(torch.cat([big[n]] * 2, 1) if n in "qkv" else big[n] for n in names[:-1]), torch.cat([big["tree"]] * 2, 1), torch.cat([big["q"]] * 2, 1).contiguous())
+
+
+@pytest.mark.parametrize("t,h,g,d", [(1, 4, 1, 128), (3, 8, 2, 64), (5, 8, 1, 128), (40, 16, 2, 128), (63, 2, 1, 64)])
+def test_bits_behind_the_last_token(t, h, g, d):
+    """They stand for no token; an entry that has only such bits is not 0, so not padding: it sees the committed tokens."""
+    x = _inputs(3, t, h, g, d, [200, 64, 7], 16)
+    expect = _run(x)
+    x["tree"] |= -1 << t
+    assert torch.equal(_run(x), expect)
+    x["tree"][:, t // 2] = 1 << t if t < 63 else -(1 << 63)
+    x["tree"][2, 0] = -(1 << 63)
+    x["tree"][1, t - 1] = 0
+    _check(_run(x), x)
