@@ -75,6 +75,7 @@ SIGNATURES = {
     "fp6m_mul_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _i, _vp, _vp]),
     "fp6m_tree_attention_scratch_bytes": (_sz, [_i]),
     "fp6m_tree_attention": (_i, [ctypes.POINTER(TreeAttentionArgs), _vp, _sz, _i, _vp, _vp]),
+    "fp6m_zeroed_memory": (_i, [_sz, _i, ctypes.POINTER(_vp)]),
     "fp6m_set_launch_overlap": (ctypes.c_int, [ctypes.c_int]),
     "fp6m_set_ordered_sums": (ctypes.c_int, [ctypes.c_int]),
     "fp6m_last_cuda_error": (ctypes.c_char_p, []),

@@ -341,6 +341,31 @@ def _stream_handle(idx: int, device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _DeviceMemory:
+    """Device memory that is kept for the life of the process, as torch.as_tensor takes it."""
+
+    def __init__(self, address: int, nbytes: int):
+        self.__cuda_array_interface__ = {"shape": (nbytes,), "typestr": "|u1", "data": (address, False), "version": 3}
+
+
+def _zeroed_outside_a_capture(nbytes: int, device: torch.device) -> torch.Tensor:
+    address = ctypes.c_void_p()
+    rc = lib.fp6m_zeroed_memory(nbytes, device.index, ctypes.byref(address))
+    if rc:
+        raise RuntimeError(f"no memory for the scratch that a call inside a graph capture needs ({_lib.last_cuda_error()}); make one such call on the "
+                           "stream before the capture")
+    return torch.as_tensor(_DeviceMemory(address.value, nbytes), device=device)
+
+
+def _zeros(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Bytes that are zero before anything that follows on the current stream of `device` - which torch.zeros would not see to while that stream
+    is captured: its memory would belong to the graph, hold anything until the first replay, and be zeroed again by each."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            return _zeroed_outside_a_capture(nbytes, device)
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
 def _device_buffers(device: torch.device, shape=None, stream=None):
     """(device index, split-K scratch, status word) for a GEMM on the CURRENT stream of `device`
     (`stream`: its handle, if the caller has it already).
@@ -359,7 +384,7 @@ def _device_buffers(device: torch.device, shape=None, stream=None):
     # device, would register them in an order of their own and drop one that the native call path goes on using.
     with _buffers_lock:
         if idx not in _status:
-            _status[idx] = torch.zeros(1, dtype=torch.int32, device=device)
+            _status[idx] = _zeros(4, torch.device("cuda", idx)).view(torch.int32)
             _sm_count[idx] = torch.cuda.get_device_properties(idx).multi_processor_count
             _call.set_device(idx, _ptr(_status[idx]), _sm_count[idx])
         need_key = (idx, shape)
@@ -378,8 +403,7 @@ def _device_buffers(device: torch.device, shape=None, stream=None):
             if buffers:
                 nbytes = max(nbytes, 2 * buffers[-1].numel())
             # zero once: the kernels keep the epoch and the tagged slots in it between calls
-            with torch.cuda.device(device):
-                buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            buf = _zeros(nbytes, torch.device("cuda", idx))
             buffers.append(buf)
             _call.set_scratch(idx, key[1], _ptr(buf), nbytes)
         return idx, buffers[-1], _status[idx]

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .api import _buffers_lock, _call, _device_buffers, _ptr, _sm_count, _status, _stream_handle
+from .api import _buffers_lock, _call, _device_buffers, _ptr, _sm_count, _status, _stream_handle, _zeros
 from ._lib import lib
 
 GROUP = 128                                       # neighbours that share a scale
@@ -40,8 +40,7 @@ def _operator_buffers(name: str, device: torch.device, nbytes: int, stream: int)
         if not buffers or buffers[-1].numel() < nbytes:
             if buffers:
                 nbytes = max(nbytes, 2 * buffers[-1].numel())
-            with torch.cuda.device(device):
-                buffers.append(torch.zeros(nbytes, dtype=torch.uint8, device=device))
+            buffers.append(_zeros(nbytes, device))
             _call.set_operator_scratch(_OWNERS[name], device.index, stream, _ptr(buffers[-1]), nbytes)
         return buffers[-1], _status[device.index]
 

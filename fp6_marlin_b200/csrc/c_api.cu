@@ -311,6 +311,28 @@ int fp6m_dump_operands(const void* B, const void* s, void* W_out, int N, int K, 
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "dump_operands launch");
 }
 
+int fp6m_zeroed_memory(size_t bytes, int dev, void** out) {
+  if (!out || bytes == 0) return FP6M_ERR_BAD_ARG;
+  *out = nullptr;
+  DeviceGuard guard(dev);
+  // A thread whose captures are of another mode may not allocate while they last.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
+  void* memory = nullptr;
+  cudaStream_t own = nullptr;            // one that nobody captures and that waits for no other
+  e = cudaMalloc(&memory, bytes);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(memory, 0, bytes, own);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+  if (own) cudaStreamDestroy(own);
+  if (e != cudaSuccess && memory) cudaFree(memory);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return cuda_fail(e, "zeroed memory");
+  *out = memory;
+  return FP6M_OK;
+}
+
 int fp6m_set_launch_overlap(int enable) {
   const int before = tc5_get_overlap() ? 1 : 0;
   if (enable >= 0) tc5_set_overlap(enable != 0);

@@ -279,6 +279,11 @@ typedef struct fp6m_tree_attention_args {
 size_t fp6m_tree_attention_scratch_bytes(int sms);
 int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
 
+/* `bytes` bytes of device memory, all zero when the call returns: for scratch and status words.  Also while a stream is captured, by this thread or
+ * another: neither the allocation nor the zeroing becomes part of a graph (memory zeroed inside a graph is not zero before its first
+ * replay, and is zeroed again by each).  To be freed with cudaFree.  The reference's caller brings zeroed memory (fp6_marlin_cuda.cpp:47-92). */
+int fp6m_zeroed_memory(size_t bytes, int dev, void** out);
+
 /* Process-wide option, off by default; returns the previous setting (a negative argument only queries).
  * GEMMs of up to 128 rows are always launched with programmatic stream serialisation: such a GEMM sets itself up (and brings the first
  * lines of B into L2) while the kernel before it in the stream finishes, and reads and writes memory only after that
