@@ -66,6 +66,9 @@ __device__ __forceinline__ float sum_of_block(float sum, float* part) {
   return sum;
 }
 
+// (N - 1 and not N + 127: rows may be as long as an int can say)
+__device__ __forceinline__ int groups_of(int N) { return (N - 1) / kGroup + 1; }
+
 struct RowParams {
   const void *x, *weight, *residual;
   void *residual_out, *y;
@@ -107,7 +110,7 @@ template <class T, bool kNorm, bool kFp8, int kVecs>
 __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024) rows_kernel(const RowParams p) {
   __shared__ float part[32];
   const size_t row = blockIdx.x;
-  const int vecs = p.N / 8, groups = (p.N + kGroup - 1) / kGroup;
+  const int vecs = p.N / 8, groups = groups_of(p.N);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint4* x = static_cast<const uint4*>(p.x) + row * vecs;
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(1024) long_rows_kernel(const RowParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const size_t row = blockIdx.x;
-  const int vecs = p.N / 8, groups = (p.N + kGroup - 1) / kGroup;
+  const int vecs = p.N / 8, groups = groups_of(p.N);
   const uint4* x = static_cast<const uint4*>(p.x) + row * vecs;
   const uint4* r = p.residual ? static_cast<const uint4*>(p.residual) + row * vecs : nullptr;
   auto load = [&](int v, float (&f)[8]) {

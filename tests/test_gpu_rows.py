@@ -129,3 +129,19 @@ def test_no_rows_and_refusals():
                 lambda: fm.quantize_fp8(x, q, s.half()), lambda: fm.rms_norm(x.flatten()[4:4 + 512].view(2, 256), w, y[:2])):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_rows_as_long_as_an_int_can_say():
+    """Two rows of 2^31 - 8 values: the scales and values of the second lie where they belong."""
+    n = (1 << 31) - 8
+    x = torch.full((2, n), 1.0, dtype=torch.bfloat16, device="cuda")
+    top = torch.full((2, -(-n // 128)), 1.0, device="cuda")
+    spots = [1, 100, 128, n // 2 - 50, n - 200, n - 120, n - 1]      # the last group has 120 values
+    for i, at in enumerate(spots):
+        x[1, at] = -2.0 - i
+        top[1, at // 128] = 2.0 + i                                  # (a later spot is larger)
+    q, s = torch.empty((2, n), dtype=torch.float8_e4m3fn, device="cuda"), torch.full_like(top, 7.0)
+    fm.quantize_fp8(x, q, s)
+    assert ((s.double() * 448 - top).abs() <= ARITHMETIC * top).all()
+    for first in (0, 128, n // 2 // 128 * 128, n - 248, n - 120):
+        _check_fp8(q[:, first:first + 120], s[:, first // 128][:, None], x[:, first:first + 120].double())
