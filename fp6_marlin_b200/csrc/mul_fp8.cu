@@ -13,6 +13,8 @@
 // The blocks are cut into as many ranges as there are multiprocessors, so a strip's sums mostly come from two or three CTAs: words of
 // {value, tag} that the CTA in which the strip starts polls for; a tag needs no flag, no fence and no clearing.  A thread keeps at most 32 sums: with 64 of
 // them (rows 65 to 192 in this form) they were spilled and 128 rows of 11008 x 4096 took 39 us, against 21 in the other kernel.
+#include <limits.h>
+
 #include "../../include/fp6m.h"
 #include "host_common.h"
 #include "mul_fp8.cuh"
@@ -359,6 +361,8 @@ mul_fp8_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUte
   if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
 }
 
+// The kernels' places are of 32 bits, also those of the last tile's end.
+bool fp8_sizes_fit(int M, int N, int K) { return M <= INT_MAX - 255 && N <= INT_MAX - 255 && K <= INT_MAX - 255; }
 int columns_ctas(int N, int K, int sms) {
   const long long blocks = (long long)((N + kBlock - 1) / kBlock) * ((K + kBlock - 1) / kBlock);
   const int ctas = sms > 0 && sms < kMaxFp8Ctas ? sms : kMaxFp8Ctas;
@@ -414,7 +418,7 @@ cudaError_t launch_fp8_columns(const Fp8Args& a, int sms, cudaStream_t stream) {
 extern "C" {
 
 size_t fp6m_mul_fp8_scratch_bytes(int M, int N, int K, int sms) {
-  if (M <= 0 || N <= 0 || K <= 0) return 256;
+  if (M <= 0 || N <= 0 || K <= 0 || !fp6m::fp8_sizes_fit(M, N, K)) return 256;
   return (fp6m::fp8_scratch_bytes(M, N, K, sms) + 255) & ~(size_t)255;
 }
 
@@ -422,7 +426,7 @@ int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const vo
                  int dev, void* stream, int* status_dev) {
   using namespace fp6m;
   if (M < 0 || N < 0 || K < 0 || (type != FP6M_TYPE_F16 && type != FP6M_TYPE_BF16)) return FP6M_ERR_BAD_ARG;
-  if (K % 16 || N % 8) return FP6M_ERR_PROB_SHAPE;
+  if (K % 16 || N % 8 || !fp8_sizes_fit(M, N, K)) return FP6M_ERR_PROB_SHAPE;
   if (M == 0 || N == 0) return FP6M_OK;
   if (!C || !aligned16(C)) return FP6M_ERR_BAD_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

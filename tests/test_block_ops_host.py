@@ -76,3 +76,10 @@ def _changed(args, change):
     for name, value in change.items():
         setattr(copy, name, value)
     return copy
+
+
+def test_products_whose_places_do_not_fit_an_int():
+    lib, one = _lib.lib, 16
+    for m, n, k in ((1, 8, (1 << 31) - 128), (100, 8, (1 << 31) - 16), (1, (1 << 31) - 128, 16), ((1 << 31) - 200, 8, 16)):
+        assert lib.fp6m_mul_fp8(one, one, one, one, one, m, n, k, 0, one, 1 << 40, 0, None, 0) == _lib.ERR_PROB_SHAPE
+        assert lib.fp6m_mul_fp8_scratch_bytes(m, n, k, 148) == 256
