@@ -596,7 +596,8 @@ int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, siz
   if (a.tokens > 64 || (a.head_dim != 64 && a.head_dim != 128)) return FP6M_ERR_PROB_SHAPE;
   if (a.batch == 0 || a.tokens == 0 || a.heads == 0) return FP6M_OK;
   if (a.kv_heads <= 0 || a.heads % a.kv_heads) return FP6M_ERR_PROB_SHAPE;
-  if (a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fffff00ll) return FP6M_ERR_PROB_SHAPE;
+  // (pages are looked up in blocks of up to 2048 tokens, two of them ahead, so tokens stay that far from 2^31)
+  if (a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fff0000ll) return FP6M_ERR_PROB_SHAPE;
   if ((long long)a.tokens * a.heads > 0xffffffll) return FP6M_ERR_PROB_SHAPE;
   if (!rows_aligned(a.q, a.q_stride) || !rows_aligned(a.k, a.k_stride) || !rows_aligned(a.v, a.v_stride) || !rows_aligned(a.out, a.out_stride)) return FP6M_ERR_BAD_ARG;
   if (!a.lengths || !a.tree || a.tree_stride < 0 || !scratch || !aligned16(scratch)) return FP6M_ERR_BAD_ARG;

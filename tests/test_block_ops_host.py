@@ -83,3 +83,10 @@ def test_products_whose_places_do_not_fit_an_int():
     for m, n, k in ((1, 8, (1 << 31) - 128), (100, 8, (1 << 31) - 16), (1, (1 << 31) - 128, 16), ((1 << 31) - 200, 8, 16)):
         assert lib.fp6m_mul_fp8(one, one, one, one, one, m, n, k, 0, one, 1 << 40, 0, None, 0) == _lib.ERR_PROB_SHAPE
         assert lib.fp6m_mul_fp8_scratch_bytes(m, n, k, 148) == 256
+
+
+def test_tables_whose_tokens_do_not_fit_an_int():
+    """2^31 - 2048 of them and more: the look-up of pages goes up to 4160 tokens past a sequence's end."""
+    args = _lib.TreeAttentionArgs(*([16] * 9), batch=1, tokens=64, heads=2, kv_heads=1, head_dim=64, pages=1)
+    for page_size, max_pages in ((64, (1 << 25) - 32), (1, (1 << 31) - 256), (1 << 30, 2)):
+        assert _lib.lib.fp6m_tree_attention(_changed(args, dict(page_size=page_size, max_pages=max_pages)), 16, 1 << 40, 0, None, 0) == _lib.ERR_PROB_SHAPE
