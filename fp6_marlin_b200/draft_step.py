@@ -73,9 +73,10 @@ class DraftBlock:
         """Writes the keys and values of accepted drafted tokens (``accepted``: a list of token numbers per sequence) behind the
         committed ones and returns the new lengths."""
         page_size = self.k_cache.shape[1]
-        sequence = torch.tensor([i for i, tokens in enumerate(accepted) for _ in tokens], device=keys.device)
-        token = torch.tensor([t for tokens in accepted for t in tokens], device=keys.device)
-        rank = torch.tensor([j for tokens in accepted for j in range(len(tokens))], device=keys.device)
+        index = lambda values: torch.tensor(values, dtype=torch.long, device=keys.device)          # noqa: E731  (also of none)
+        sequence = index([i for i, tokens in enumerate(accepted) for _ in tokens])
+        token = index([t for tokens in accepted for t in tokens])
+        rank = index([j for tokens in accepted for j in range(len(tokens))])
         at = lengths.long()[sequence] + rank
         page, slot = page_table.long()[sequence, at // page_size], at % page_size
         self.k_cache[page, slot], self.v_cache[page, slot] = keys[sequence, token], values[sequence, token]
