@@ -71,14 +71,20 @@ class DraftBlock:
 
     def accept(self, keys, values, accepted, page_table, lengths):
         """Writes the keys and values of accepted drafted tokens (``accepted``: a list of token numbers per sequence) behind the
-        committed ones and returns the new lengths."""
+        committed ones and returns the new lengths.  Raises ``ValueError``, and writes nothing, where there is no such token or no place for it
+        (this check synchronises; on the GPU an index out of range would end the process's use of it)."""
         page_size = self.k_cache.shape[1]
+        if not len(accepted) == keys.shape[0] == lengths.shape[0] == page_table.shape[0] or any(not 0 <= t < keys.shape[1] for tokens in accepted for t in tokens):
+            raise ValueError("accept: a list of numbers of drafted tokens for each sequence is needed")
         index = lambda values: torch.tensor(values, dtype=torch.long, device=keys.device)          # noqa: E731  (also of none)
         sequence = index([i for i, tokens in enumerate(accepted) for _ in tokens])
         token = index([t for tokens in accepted for t in tokens])
         rank = index([j for tokens in accepted for j in range(len(tokens))])
         at = lengths.long()[sequence] + rank
-        page, slot = page_table.long()[sequence, at // page_size], at % page_size
+        place, slot = (at // page_size).clamp(0, max(page_table.shape[1] - 1, 0)), at % page_size
+        page = page_table.long()[sequence, place] if page_table.shape[1] else torch.full_like(at, -1)
+        if bool(((place != at // page_size) | (page < 0) | (page >= self.k_cache.shape[0])).any()):
+            raise ValueError("accept: the page table has no place for an accepted token")
         self.k_cache[page, slot], self.v_cache[page, slot] = keys[sequence, token], values[sequence, token]
         return lengths + torch.tensor([len(tokens) for tokens in accepted], dtype=torch.int32, device=keys.device)
 

@@ -31,3 +31,25 @@ def test_accepted_tokens_follow_the_committed_ones(accepted):
             at = int(lengths[i]) + j
             k[TABLE[i, at // 4], at % 4], v[TABLE[i, at // 4], at % 4] = keys[i, t], values[i, t]
     assert torch.equal(block.k_cache, k) and torch.equal(block.v_cache, v)
+
+
+@pytest.mark.parametrize("what", ["past the table", "no table", "a page that does not exist", "a negative page", "a negative length", "no such token", "too few lists"])
+def test_what_has_no_place_is_refused_and_nothing_is_written(what):
+    block, (keys, values), lengths, table, accepted = _block(), _drafted(), torch.tensor([3, 7, 0], dtype=torch.int32), TABLE.clone(), [[0, 1], [2], [0]]
+    if what == "past the table":
+        lengths[1] = 8
+    elif what == "no table":
+        table = table[:, :0]
+    elif what == "a page that does not exist":
+        table[0, 1] = 8
+    elif what == "a negative page":
+        table[0, 1] = -1
+    elif what == "a negative length":
+        lengths[2] = -1
+    elif what == "no such token":
+        accepted[2] = [5]
+    else:
+        accepted.pop()
+    with pytest.raises(ValueError):
+        block.accept(keys, values, accepted, table, lengths)
+    assert not block.k_cache.any() and not block.v_cache.any()
