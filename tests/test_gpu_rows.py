@@ -145,3 +145,32 @@ def test_rows_as_long_as_an_int_can_say():
     assert ((s.double() * 448 - top).abs() <= ARITHMETIC * top).all()
     for first in (0, 128, n // 2 // 128 * 128, n - 248, n - 120):
         _check_fp8(q[:, first:first + 120], s[:, first // 128][:, None], x[:, first:first + 120].double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_are_divided_by_the_scale_that_is_stored(dtype):
+    """Bit for bit, also where the quotient lies on the boundary between two E4M3 values: few distinct values, so that many do."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x = (torch.randint(-255, 256, (301, 2056), generator=gen, device="cuda") * torch.exp2(torch.randint(-6, 3, (301, 1), generator=gen, device="cuda"))).to(dtype)
+    q, s = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((301, 17), device="cuda")
+    fm.quantize_fp8(x, q, s)
+    top = torch.nn.functional.pad(x.float().abs(), (0, 120)).view(301, 17, 128).amax(2).clamp(min=1e-30).cpu()
+    assert torch.equal(s.cpu(), top / torch.full_like(top, 448.0))
+    expect = (x.float().cpu() / s.cpu().repeat_interleave(128, 1)[:, :2056]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    assert torch.equal(q.cpu().view(torch.uint8), expect.view(torch.uint8))
+
+
+def test_division_by_infinite_and_by_small_scales():
+    x = torch.zeros((6, 128), dtype=torch.bfloat16, device="cuda")
+    x[:, ::3] = 1.0
+    x[0, 5], x[1, 7] = float("inf"), float("-inf")                   # finite values by infinity are 0
+    x[2] *= 1e-30
+    x[3], x[3, 9] = 1e-39, 1e-31                                     # below the least scale
+    x[4], x[4, 1] = torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).min
+    x[5] *= torch.linspace(1e-38, 1e-30, 128, device="cuda")
+    q, s = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((6, 1), device="cuda")
+    fm.quantize_fp8(x, q, s)
+    top = x.float().abs().amax(1, keepdim=True).clamp(min=1e-30).cpu()
+    assert torch.equal(s.cpu(), top / torch.full_like(top, 448.0))
+    expect = (x.float().cpu() / s.cpu()).clamp(-448, 448).to(torch.float8_e4m3fn).float()
+    assert torch.equal(q.cpu().float().nan_to_num(nan=1000.0), expect.nan_to_num(nan=1000.0)) and int(q.float().isnan().sum()) == 2
