@@ -41,7 +41,6 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
-#include <cstring>
 
 #include "device_utils.cuh"
 #include "fp6m_layout.h"
@@ -656,7 +655,6 @@ namespace {
 struct MapKey {
   const void* A;
   int M, K, box_rows, dims;
-  long long more[5] = {};                 // of a paged cache: heads, tokens and strides
 };
 struct MapCache {
   static constexpr int kEntries = 96;      // a GEMM of many launches onto eight outputs has 64 output maps
@@ -665,8 +663,7 @@ struct MapCache {
   int next = 0;
   bool find(const MapKey& k, CUtensorMap* out) const {
     for (int i = 0; i < kEntries; ++i)
-      if (key[i].A == k.A && key[i].M == k.M && key[i].K == k.K && key[i].box_rows == k.box_rows && key[i].dims == k.dims &&
-          (k.dims != 6 || std::memcmp(key[i].more, k.more, sizeof(k.more)) == 0)) {
+      if (key[i].A == k.A && key[i].M == k.M && key[i].K == k.K && key[i].box_rows == k.box_rows && key[i].dims == k.dims) {
         *out = map[i];
         return true;
       }
@@ -721,30 +718,24 @@ cudaError_t encode_activation_segment_map(const half* A, int M, int K, int box_r
   return e;
 }
 
+// The two below are encoded anew by every call (about 50 ns): a model's weights and caches are more than the maps that are kept, and would push out
+// those of the activations, which come again and again.
 // A matrix of bytes (E4M3), `rows` x K, K contiguous; one box = 128 bytes x `box_rows` rows with the 128-byte swizzle; what lies
 // outside reads as zero.
 cudaError_t encode_bytes_map(const void* base, int rows, int K, int box_rows, CUtensorMap* map) {
-  const MapKey mk = {base, rows, K, box_rows, 5};
-  if (g_map_cache.find(mk, map)) return cudaSuccess;
   const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)K};
   const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
-  const cudaError_t e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
-  if (e == cudaSuccess) g_map_cache.put(mk, *map);
-  return e;
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 // A paged cache of 16-bit values as a tensor of head_dim x heads x page_size x pages with any strides (elements: page, slot, head); one box
 // = 64 values of `run` neighbouring tokens, in 128-byte rows with the 128-byte swizzle; what lies outside reads as zero.
 cudaError_t encode_cache_map(const void* base, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, CUtensorMap* map) {
-  const MapKey mk = {base, pages, head_dim, run, 6, {heads, page_size, strides[0], strides[1], strides[2]}};
-  if (g_map_cache.find(mk, map)) return cudaSuccess;
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)page_size, (cuuint64_t)pages};
   const cuuint64_t pitches[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
   const cuuint32_t box[4] = {64, 1, (cuuint32_t)run, 1};
-  const cudaError_t e = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, pitches, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
-  if (e == cudaSuccess) g_map_cache.put(mk, *map);
-  return e;
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, pitches, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
 static int tile_height(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) / 16 * 16; }
