@@ -265,7 +265,7 @@ def tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, *,
         raise RuntimeError(f"{what}: tree must be int64 of shape ({t},) or ({b}, {t})")
     if page_table.device != device or lengths.device != device or tree.device != device:
         raise RuntimeError(f"{what}: page_table, lengths and tree must be on q's device")
-    if (page_table.numel() and page_table.stride(1) != 1) or not lengths.is_contiguous() or (tree.numel() and tree.stride(-1) != 1):
+    if any(x.numel() and x.shape[-1] > 1 and x.stride(-1) != 1 for x in (page_table, lengths, tree)):
         raise RuntimeError(f"{what}: the rows of page_table and tree, and lengths, must be contiguous")
     if b == 0 or t == 0 or h == 0:
         return

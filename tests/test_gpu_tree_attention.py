@@ -280,3 +280,18 @@ def test_bits_behind_the_last_token(t, h, g, d):
     x["tree"][2, 0] = -(1 << 63)
     x["tree"][1, t - 1] = 0
     _check(_run(x), x)
+
+
+def test_tables_and_masks_of_single_places():
+    """One page a sequence, one drafted token, one sequence: the step to a next one that there is not may be anything."""
+    x = _inputs(3, 1, 4, 1, 64, [9, 16, 0], 16)
+    expect = _run(x)
+    x["page_table"], x["tree"] = x["page_table"].t().contiguous().t(), x["tree"].t().contiguous().t()
+    for n in ("page_table", "tree"):
+        x[n] = x[n].as_strided((3, 1), (1, 3))
+    assert torch.equal(_run(x), expect)
+    one = _inputs(1, 1, 4, 1, 64, [9], 16)
+    expect = _run(one)
+    one["lengths"], one["tree"] = one["lengths"].as_strided((1,), (5,)), one["tree"][0].as_strided((1,), (7,))
+    one["page_table"] = one["page_table"].as_strided((1, 1), (4, 6))
+    assert torch.equal(_run(one), expect)
