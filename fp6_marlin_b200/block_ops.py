@@ -64,6 +64,8 @@ def _check(what: str, device: torch.device, **tensors):
 def _raise(what: str, rc: int):
     if rc == _lib.ERR_PROB_SHAPE:
         raise RuntimeError(f"{what}: the shape is not supported")
+    if rc == _lib.ERR_BAD_ARG:                     # (what else it stands for is checked before)
+        raise RuntimeError(f"{what}: the tensors must start on 16-byte boundaries")
     if rc == _lib.ERR_CUDA:
         raise RuntimeError(f"{what}: CUDA error: {_lib.last_cuda_error()}")
     raise RuntimeError(f"{what} failed with code {rc}")

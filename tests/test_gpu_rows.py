@@ -174,3 +174,13 @@ def test_division_by_infinite_and_by_small_scales():
     assert torch.equal(s.cpu(), top / torch.full_like(top, 448.0))
     expect = (x.float().cpu() / s.cpu()).clamp(-448, 448).to(torch.float8_e4m3fn).float()
     assert torch.equal(q.cpu().float().nan_to_num(nan=1000.0), expect.nan_to_num(nan=1000.0)) and int(q.float().isnan().sum()) == 2
+
+
+def test_misaligned_tensors_are_named():
+    x, w = _rows(2, 256, torch.float16), torch.ones(264, dtype=torch.float16, device="cuda")
+    q, s = torch.empty(520, dtype=torch.uint8, device="cuda")[8:].view(torch.float8_e4m3fn).view(2, 256), torch.empty((2, 2), device="cuda")
+    b, c = torch.empty((8, 256), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((2, 8), dtype=torch.float16, device="cuda")
+    for call in (lambda: fm.rms_norm(x, w[4:260], torch.empty_like(x)), lambda: fm.rms_norm(x, w[:256], q, scales=s), lambda: fm.quantize_fp8(x, q, s),
+                 lambda: fm.mul_fp8(q, b, c, s, s[:1])):
+        with pytest.raises(RuntimeError, match="16-byte boundaries"):
+            call()
