@@ -52,3 +52,16 @@ def test_pages_that_do_not_exist(t, h, g, d, page):
     _check(out, _without(dict(x, page_table=good), gone))
     x["page_table"].copy_(good)
     assert torch.equal(_run(x), expect) and fm.device_status() == 0
+
+
+@pytest.mark.parametrize("t,h,g,d", [(12, 16, 4, 128), (40, 16, 2, 64)])
+def test_heads_that_share_memory(t, h, g, d):
+    """One head of keys and values for all, and one page for all places of the table."""
+    x = _inputs(2, t, h, g, d, [150, 700], 16)
+    for n in ("k_cache", "v_cache", "k", "v"):
+        x[n] = x[n][:, :, :1].expand_as(x[n])
+    _check(_run(x), x)
+    for n in ("k_cache", "v_cache"):
+        x[n] = x[n][3:4].expand_as(x[n])
+    _check(_run(x), x)
+    assert fm.device_status() == 0
