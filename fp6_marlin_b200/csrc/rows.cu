@@ -20,7 +20,8 @@ namespace {
 using namespace fp6m;
 
 constexpr int kGroup = 128;              // neighbours that share a scale
-constexpr float kE4m3Max = 448.f, kSmallest = 1e-30f;
+constexpr float kPart = 1.f / 448.f;      // of the largest magnitude: the scale.  One product, as torch on a GPU divides by a number: the same scales, bit for bit
+constexpr float kSmallest = 1e-30f;
 
 template <class T> struct Pair;
 template <> struct Pair<half> {
@@ -115,9 +116,7 @@ __device__ __forceinline__ void finish_vector(const RowParams& p, size_t row, in
 #pragma unroll
     for (int o = 8; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (v < vecs) {
-      // (a division by a constant, likewise; infinity stays that)
-      constexpr float kPart = 1.f / kE4m3Max;
-      const float near = top * kPart, scale = isinf(top) ? top : fmaf(fmaf(-near, kE4m3Max, top), kPart, near);
+      const float scale = top * kPart;
       const Divisor by(scale);
       uint2 q;
       auto two = [&](int i) { return (uint32_t)__nv_cvt_float2_to_fp8x2(by.divide(f[i], f[i + 1]), __NV_SATFINITE, __NV_E4M3); };

@@ -236,7 +236,8 @@ enum { FP6M_TYPE_F16 = 0, FP6M_TYPE_BF16 = 1 };
  * y = h * rsqrt(mean(h^2) + eps) * weight.  The norm goes on with the sum before that rounding.
  *   scales == null: y is M x N in x's type
  *   else            y is M x N in E4M3 and scales M x ceil(N / 128) fp32: max(largest |y| of the 128 neighbours, 1e-30) / 448,
- *                   y[m, n] * scales[m, n / 128] stands for the value; this is what fp6m_mul_fp8 takes
+ *                   (one product with 1 / 448 in fp32); y[m, n] is the value divided by its scale and rounded, and y[m, n] * scales[m, n / 128]
+ *                   stands for the value; this is what fp6m_mul_fp8 takes
  * residual and residual_out are given together or not at all.  N a multiple of 8, pointers 16-byte aligned (scales: 4).
  * No counterpart in the reference; nor have the next ones. */
 int fp6m_rms_norm(const void* x, const void* weight, const void* residual, void* residual_out, void* y, void* scales, int M, int N, float eps,

@@ -155,7 +155,7 @@ def test_values_are_divided_by_the_scale_that_is_stored(dtype):
     q, s = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((301, 17), device="cuda")
     fm.quantize_fp8(x, q, s)
     top = torch.nn.functional.pad(x.float().abs(), (0, 120)).view(301, 17, 128).amax(2).clamp(min=1e-30).cpu()
-    assert torch.equal(s.cpu(), top / torch.full_like(top, 448.0))
+    assert torch.equal(s.cpu(), top * torch.tensor(1.0 / 448.0))     # (one product in fp32)
     expect = (x.float().cpu() / s.cpu().repeat_interleave(128, 1)[:, :2056]).clamp(-448, 448).to(torch.float8_e4m3fn)
     assert torch.equal(q.cpu().view(torch.uint8), expect.view(torch.uint8))
 
@@ -171,7 +171,7 @@ def test_division_by_infinite_and_by_small_scales():
     q, s = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((6, 1), device="cuda")
     fm.quantize_fp8(x, q, s)
     top = x.float().abs().amax(1, keepdim=True).clamp(min=1e-30).cpu()
-    assert torch.equal(s.cpu(), top / torch.full_like(top, 448.0))
+    assert torch.equal(s.cpu(), top * torch.tensor(1.0 / 448.0))     # (one product in fp32)
     expect = (x.float().cpu() / s.cpu()).clamp(-448, 448).to(torch.float8_e4m3fn).float()
     assert torch.equal(q.cpu().float().nan_to_num(nan=1000.0), expect.nan_to_num(nan=1000.0)) and int(q.float().isnan().sum()) == 2
 
@@ -184,3 +184,15 @@ def test_misaligned_tensors_are_named():
                  lambda: fm.mul_fp8(q, b, c, s, s[:1])):
         with pytest.raises(RuntimeError, match="16-byte boundaries"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(37, 8192), (301, 2056), (5, 30000)])
+def test_quantised_rows_are_those_of_torch_operations(m, n, dtype):
+    """On the GPU, where torch divides by a number as a product with its reciprocal and by a tensor with one rounding."""
+    x = _rows(m, n, dtype, 9, 3.0)
+    q, s = torch.empty((m, n), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((m, -(-n // 128)), device="cuda")
+    fm.quantize_fp8(x, q, s)
+    scales = torch.nn.functional.pad(x.float(), (0, -n % 128)).view(m, -1, 128).abs().amax(2).clamp(min=1e-30) / 448
+    expect = (x.float() / scales.repeat_interleave(128, 1)[:, :n]).to(torch.float8_e4m3fn)
+    assert torch.equal(s, scales) and torch.equal(q.view(torch.uint8), expect.view(torch.uint8))
