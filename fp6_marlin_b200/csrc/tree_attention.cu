@@ -152,240 +152,240 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
   int stage = 0, turn = (kStages - 1) & 1;                           // turn: of the places
 #pragma unroll 1
   while (seg.next(p)) {
-  const int g = seg.item;
-  // ---- new rows: queries and masks
-  uint32_t q[D / 16][4];
-  float o[D / 8][4], top[2], total[2];
-  unsigned long long mask[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = row_warp * 16 + quad + 8 * h;
-    mask[h] = 0;
-    const T* src = nullptr;
-    if (r < p.rows) {
-      const int t = r / p.group, head = g * p.group + (r - t * p.group);
-      mask[h] = mask_of(p, seg.b, t);
-      src = static_cast<const T*>(a.q) + seg.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
-    }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      q[i][h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + col) : 0u;
-      q[i][2 + h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + 8 + col) : 0u;
-    }
-    top[h] = -INFINITY;
-    total[h] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-#pragma unroll 1
-  for (int tile = seg.t0; tile < seg.t1; ++tile) {
-    copies_wait<kStages - 2>();
-    __syncthreads();
-    const bool live = ahead_lives;
-    advance();
-    const int page = look_up();
-    if (live) copy((stage + kStages - 1) % kStages, turn);
-    copies_commit();
-    turn ^= 1;
-
-    // ---- scores of this warp's keys
-    const uint32_t keys = smem_base + stage * 2 * kTileBytes + key_warp * kMine * kRowBytes, values = keys + kTileBytes;
-    float s[kMine / 8][4];
-#pragma unroll
-    for (int i = 0; i < kMine / 8; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
-      const int row = i * 8 + (lane & 7);
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        uint32_t k[4];
-        ldsm(k, keys + row * kRowBytes + (((d * 4 + (lane >> 3)) ^ (row & 7)) * 16));
-        Mma<T>::run(s[i], q[2 * d], k[0], k[1]);
-        Mma<T>::run(s[i], q[2 * d + 1], k[2], k[3]);
-      }
-    }
-    const int j0 = tile * kKeys + key_warp * kMine;               // this warp's first key
-    const bool drafted = tile * kKeys + kKeys > seg.length;        // the tile holds drafted tokens, or the end
-    const bool hidden = flags[0] != 0;                               // a page of this CTA's tiles did not exist
-#pragma unroll
-    for (int i = 0; i < kMine / 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
-    if (drafted) {
-#pragma unroll
-      for (int i = 0; i < kMine / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = j0 + i * 8 + col + (e & 1) - seg.length;      // drafted token, negative: cached
-          if (t >= 0 && (t >= a.tokens || !(mask[e >> 1] >> t & 1))) s[i][e] = -INFINITY;
-        }
-    }
-    if (hidden) {
-#pragma unroll 1
-      for (int i = 0; i < kMine; ++i) {
-        const int j = j0 + i;
-        if (j >= seg.length || (unsigned)page_of(p, seg, j) < (unsigned)a.pages) continue;
-#pragma unroll
-        for (int k = 0; k < kMine / 8; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (k * 8 + col + (e & 1) == i) s[k][e] = -INFINITY;
-      }
-    }
-
-    // ---- running maximum and sum; weights in the values' type for the second product
-    float keep[2];
+    const int g = seg.item;
+    // ---- new rows: queries and masks
+    uint32_t q[D / 16][4];
+    float o[D / 8][4], top[2], total[2];
+    unsigned long long mask[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float m = top[h];
+      const int r = row_warp * 16 + quad + 8 * h;
+      mask[h] = 0;
+      const T* src = nullptr;
+      if (r < p.rows) {
+        const int t = r / p.group, head = g * p.group + (r - t * p.group);
+        mask[h] = mask_of(p, seg.b, t);
+        src = static_cast<const T*>(a.q) + seg.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
+      }
 #pragma unroll
-      for (int i = 0; i < kMine / 8; ++i) m = fmaxf(m, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const float base = m == -INFINITY ? 0.f : m;                   // nothing seen so far
-      keep[h] = exp2_approx(top[h] - base);
-      top[h] = m;
-      total[h] *= keep[h];
-#pragma unroll
-      for (int i = 0; i < kMine / 8; ++i)
-#pragma unroll
-        for (int e = 2 * h; e < 2 * h + 2; ++e) {
-          s[i][e] = exp2_approx(s[i][e] - base);
-          total[h] += s[i][e];
-        }
+      for (int i = 0; i < D / 16; ++i) {
+        q[i][h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + col) : 0u;
+        q[i][2 + h] = src ? *reinterpret_cast<const uint32_t*>(src + 16 * i + 8 + col) : 0u;
+      }
+      top[h] = -INFINITY;
+      total[h] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] *= keep[e >> 1];
-
-    // ---- infinities and NaN among the drafted values: a weight of zero must not meet them
-    if (drafted) {
-      const int from = max(seg.length - tile * kKeys, 0), upto = min(seg.length + a.tokens - tile * kKeys, kKeys);
-      const uint32_t tile_values = smem_base + stage * 2 * kTileBytes + kTileBytes;
-      bool odd = false;
-      for (int i = tid; i < (upto - from) * kChunks; i += kThreads) {
-        const int row = from + i / kChunks;
-        uint4 w;
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(tile_values + row * kRowBytes + i % kChunks * 16) : "memory");
-        odd = odd || is_odd<T>(w.x) || is_odd<T>(w.y) || is_odd<T>(w.z) || is_odd<T>(w.w);
-      }
-      if (__syncthreads_or(odd)) {
-        // each is multiplied by the weights of the rows that see it only, and is zero in the product below
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 #pragma unroll 1
-        for (int j = 0; j < kMine; ++j) {
-          float w[2];
+    for (int tile = seg.t0; tile < seg.t1; ++tile) {
+      copies_wait<kStages - 2>();
+      __syncthreads();
+      const bool live = ahead_lives;
+      advance();
+      const int page = look_up();
+      if (live) copy((stage + kStages - 1) % kStages, turn);
+      copies_commit();
+      turn ^= 1;
+
+      // ---- scores of this warp's keys
+      const uint32_t keys = smem_base + stage * 2 * kTileBytes + key_warp * kMine * kRowBytes, values = keys + kTileBytes;
+      float s[kMine / 8][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mine = 0.f;
+      for (int i = 0; i < kMine / 8; ++i) {
 #pragma unroll
-            for (int k = 0; k < kMine / 8; ++k)
+        for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        const int row = i * 8 + (lane & 7);
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (k * 8 + e == (j & ~7) + (j & 1)) mine = s[k][2 * h + e];
-            w[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + (j & 7) / 2);
-          }
-          const int t = j0 + j - seg.length;
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            uint32_t two;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(values + j * kRowBytes + ((i ^ (j & 7)) * 16) + col * 2) : "memory");
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t bits = e & 1 ? two >> 16 : two & 0xffffu;
-              const bool sees = t >= 0 && t < a.tokens && (mask[e >> 1] >> t & 1);
-              if (sees && (bits & Half16<T>::kExponent) == Half16<T>::kExponent) o[i][e] += w[e >> 1] * Half16<T>::value((uint16_t)bits);
-            }
-          }
+        for (int d = 0; d < D / 32; ++d) {
+          uint32_t k[4];
+          ldsm(k, keys + row * kRowBytes + (((d * 4 + (lane >> 3)) ^ (row & 7)) * 16));
+          Mma<T>::run(s[i], q[2 * d], k[0], k[1]);
+          Mma<T>::run(s[i], q[2 * d + 1], k[2], k[3]);
         }
-        __syncthreads();
-        for (int i = tid; i < (upto - from) * D / 2; i += kThreads) {
-          const uint32_t addr = tile_values + (from + i / (D / 2)) * kRowBytes + i % (D / 2) * 4;
-          uint32_t two;
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(addr) : "memory");
-          constexpr uint32_t E = Half16<T>::kExponent;
-          if ((two & E) == E) two &= 0xffff0000u;
-          if ((two >> 16 & E) == E) two &= 0xffffu;
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(two) : "memory");
+      }
+      const int j0 = tile * kKeys + key_warp * kMine;               // this warp's first key
+      const bool drafted = tile * kKeys + kKeys > seg.length;        // the tile holds drafted tokens, or the end
+      const bool hidden = flags[0] != 0;                               // a page of this CTA's tiles did not exist
+#pragma unroll
+      for (int i = 0; i < kMine / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] *= p.scale_log2;
+      if (drafted) {
+#pragma unroll
+        for (int i = 0; i < kMine / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = j0 + i * 8 + col + (e & 1) - seg.length;      // drafted token, negative: cached
+            if (t >= 0 && (t >= a.tokens || !(mask[e >> 1] >> t & 1))) s[i][e] = -INFINITY;
+          }
+      }
+      if (hidden) {
+#pragma unroll 1
+        for (int i = 0; i < kMine; ++i) {
+          const int j = j0 + i;
+          if (j >= seg.length || (unsigned)page_of(p, seg, j) < (unsigned)a.pages) continue;
+#pragma unroll
+          for (int k = 0; k < kMine / 8; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (k * 8 + col + (e & 1) == i) s[k][e] = -INFINITY;
         }
-        __syncthreads();
       }
-    }
 
-    // ---- weights times values
-#pragma unroll
-    for (int k = 0; k < kMine / 16; ++k) {
-      const uint32_t w[4] = {Half16<T>::pack(s[2 * k][0], s[2 * k][1]), Half16<T>::pack(s[2 * k][2], s[2 * k][3]),
-                             Half16<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), Half16<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
-      const int row = k * 16 + (lane & 15);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        uint32_t v[4];
-        ldsm_t(v, values + row * kRowBytes + (((2 * i + (lane >> 4)) ^ (row & 7)) * 16));
-        Mma<T>::run(o[2 * i], w, v[0], v[1]);
-        Mma<T>::run(o[2 * i + 1], w, v[2], v[3]);
-      }
-    }
-    stage = (stage + 1) % kStages;
-
-    put_place(page, turn);
-  }
-
-      // ---- the end of this CTA's keys for these rows
+      // ---- running maximum and sum; weights in the values' type for the second product
+      float keep[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        total[h] += __shfl_xor_sync(0xffffffffu, total[h], 1);
-        total[h] += __shfl_xor_sync(0xffffffffu, total[h], 2);
-      }
-      if constexpr (kKeyWarps > 1) {
-        // the warps that shared the keys pool their sums, the last one first
-        if ((lane & 3) == 0) {
+        float m = top[h];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            stats[warp * 32 + quad + 8 * h] = top[h];
-            stats[warp * 32 + 16 + quad + 8 * h] = total[h];
+        for (int i = 0; i < kMine / 8; ++i) m = fmaxf(m, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float base = m == -INFINITY ? 0.f : m;                   // nothing seen so far
+        keep[h] = exp2_approx(top[h] - base);
+        top[h] = m;
+        total[h] *= keep[h];
+#pragma unroll
+        for (int i = 0; i < kMine / 8; ++i)
+#pragma unroll
+          for (int e = 2 * h; e < 2 * h + 2; ++e) {
+            s[i][e] = exp2_approx(s[i][e] - base);
+            total[h] += s[i][e];
           }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= keep[e >> 1];
+
+      // ---- infinities and NaN among the drafted values: a weight of zero must not meet them
+      if (drafted) {
+        const int from = max(seg.length - tile * kKeys, 0), upto = min(seg.length + a.tokens - tile * kKeys, kKeys);
+        const uint32_t tile_values = smem_base + stage * 2 * kTileBytes + kTileBytes;
+        bool odd = false;
+        for (int i = tid; i < (upto - from) * kChunks; i += kThreads) {
+          const int row = from + i / kChunks;
+          uint4 w;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(tile_values + row * kRowBytes + i % kChunks * 16) : "memory");
+          odd = odd || is_odd<T>(w.x) || is_odd<T>(w.y) || is_odd<T>(w.z) || is_odd<T>(w.w);
         }
-        __syncthreads();
+        if (__syncthreads_or(odd)) {
+          // each is multiplied by the weights of the rows that see it only, and is zero in the product below
+#pragma unroll 1
+          for (int j = 0; j < kMine; ++j) {
+            float w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float mine = 0.f;
+#pragma unroll
+              for (int k = 0; k < kMine / 8; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (k * 8 + e == (j & ~7) + (j & 1)) mine = s[k][2 * h + e];
+              w[h] = __shfl_sync(0xffffffffu, mine, (lane & ~3) + (j & 7) / 2);
+            }
+            const int t = j0 + j - seg.length;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              uint32_t two;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(values + j * kRowBytes + ((i ^ (j & 7)) * 16) + col * 2) : "memory");
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t bits = e & 1 ? two >> 16 : two & 0xffffu;
+                const bool sees = t >= 0 && t < a.tokens && (mask[e >> 1] >> t & 1);
+                if (sees && (bits & Half16<T>::kExponent) == Half16<T>::kExponent) o[i][e] += w[e >> 1] * Half16<T>::value((uint16_t)bits);
+              }
+            }
+          }
+          __syncthreads();
+          for (int i = tid; i < (upto - from) * D / 2; i += kThreads) {
+            const uint32_t addr = tile_values + (from + i / (D / 2)) * kRowBytes + i % (D / 2) * 4;
+            uint32_t two;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(addr) : "memory");
+            constexpr uint32_t E = Half16<T>::kExponent;
+            if ((two & E) == E) two &= 0xffff0000u;
+            if ((two >> 16 & E) == E) two &= 0xffffu;
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(two) : "memory");
+          }
+          __syncthreads();
+        }
+      }
+
+      // ---- weights times values
+#pragma unroll
+      for (int k = 0; k < kMine / 16; ++k) {
+        const uint32_t w[4] = {Half16<T>::pack(s[2 * k][0], s[2 * k][1]), Half16<T>::pack(s[2 * k][2], s[2 * k][3]),
+                               Half16<T>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), Half16<T>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
+        const int row = k * 16 + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t v[4];
+          ldsm_t(v, values + row * kRowBytes + (((2 * i + (lane >> 4)) ^ (row & 7)) * 16));
+          Mma<T>::run(o[2 * i], w, v[0], v[1]);
+          Mma<T>::run(o[2 * i + 1], w, v[2], v[3]);
+        }
+      }
+      stage = (stage + 1) % kStages;
+
+      put_place(page, turn);
+    }
+
+    // ---- the end of this CTA's keys for these rows
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      total[h] += __shfl_xor_sync(0xffffffffu, total[h], 1);
+      total[h] += __shfl_xor_sync(0xffffffffu, total[h], 2);
+    }
+    if constexpr (kKeyWarps > 1) {
+      // the warps that shared the keys pool their sums, the last one first
+      if ((lane & 3) == 0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float* of = stats + row_warp * kKeyWarps * 32 + quad + 8 * h;
-          float m = -INFINITY, sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < kKeyWarps; ++w) m = fmaxf(m, of[w * 32]);
-          const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-          for (int w = 0; w < kKeyWarps; ++w) sum += of[w * 32 + 16] * exp2_approx(of[w * 32] - base);
-          const float mine = exp2_approx(top[h] - base);
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][2 * h] *= mine;
-            o[i][2 * h + 1] *= mine;
-          }
-          top[h] = m;
-          total[h] = sum;
+          stats[warp * 32 + quad + 8 * h] = top[h];
+          stats[warp * 32 + 16 + quad + 8 * h] = total[h];
         }
-        if (kKeyWarps == 4 && p.rows <= 4) {
-          // there is room for the rows of all warps at once
-          if (key_warp > 0 && quad < p.rows) {
+      }
+      __syncthreads();
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(pool + ((key_warp - 1) * 4 + quad) * D + i * 8 + col) = make_float2(o[i][0], o[i][1]);
-          }
-          __syncthreads();
-          if (key_warp == 0 && quad < p.rows) {
+      for (int h = 0; h < 2; ++h) {
+        const float* of = stats + row_warp * kKeyWarps * 32 + quad + 8 * h;
+        float m = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i)
+        for (int w = 0; w < kKeyWarps; ++w) m = fmaxf(m, of[w * 32]);
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-              for (int w = 2; w >= 0; --w) {
-                const float2 more = *reinterpret_cast<const float2*>(pool + (w * 4 + quad) * D + i * 8 + col);
-                o[i][0] += more.x;
-                o[i][1] += more.y;
-              }
-          }
-          __syncthreads();
-        } else {
+        for (int w = 0; w < kKeyWarps; ++w) sum += of[w * 32 + 16] * exp2_approx(of[w * 32] - base);
+        const float mine = exp2_approx(top[h] - base);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][2 * h] *= mine;
+          o[i][2 * h + 1] *= mine;
+        }
+        top[h] = m;
+        total[h] = sum;
+      }
+      if (kKeyWarps == 4 && p.rows <= 4) {
+        // there is room for the rows of all warps at once
+        if (key_warp > 0 && quad < p.rows) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(pool + ((key_warp - 1) * 4 + quad) * D + i * 8 + col) = make_float2(o[i][0], o[i][1]);
+        }
+        __syncthreads();
+        if (key_warp == 0 && quad < p.rows) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int w = 2; w >= 0; --w) {
+              const float2 more = *reinterpret_cast<const float2*>(pool + (w * 4 + quad) * D + i * 8 + col);
+              o[i][0] += more.x;
+              o[i][1] += more.y;
+            }
+        }
+        __syncthreads();
+      } else {
 #pragma unroll
         for (int part = 0; part < kRowWarps; ++part) {
 #pragma unroll
@@ -408,147 +408,147 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             __syncthreads();
           }
         }
+      }
+    }
+    const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
+    auto out_row = [&](int r) {
+      const int t = r / p.group, head = g * p.group + (r - t * p.group);
+      return static_cast<T*>(a.out) + seg.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+    };
+    if (whole) {
+      if (key_warp == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = row_warp * 16 + quad + 8 * h;
+          if (r < p.rows) {
+            // padding, and rows that see nothing, are zero
+            const bool none = mask[h] == 0 || total[h] == 0.f;
+            const float f = 1.f / total[h];
+            T* out = out_row(r) + col;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<uint32_t*>(out + 8 * i) = none ? 0u : Half16<T>::pack(o[i][2 * h] * f, o[i][2 * h + 1] * f);
+          }
         }
       }
-      const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
-      auto out_row = [&](int r) {
-        const int t = r / p.group, head = g * p.group + (r - t * p.group);
-        return static_cast<T*>(a.out) + seg.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
+    } else {
+      // a partial: the slot of a range's first rows, or that of its last ones
+      float* slot = p.partials + (size_t)(2 * cta + (seg.t0 == 0 ? 1 : 0)) * kSlot;
+      if (key_warp == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = row_warp * 16 + quad + 8 * h;
+          if (r < p.rows) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(slot + r * D + i * 8 + col) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+            if ((lane & 3) == 0) {
+              slot[kRowTile * D + r] = top[h];
+              slot[kRowTile * (D + 1) + r] = total[h];
+            }
+          }
+        }
+      }
+      const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
+      const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
+      const Joining join(first_cta, last_cta, cta, join_step(last_cta - first_cta + 1));
+      // whether this CTA is the last of those that a counter waits for; what the others wrote is visible then
+      auto last_at = [&](unsigned int* counter, int others) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const bool is_last = atomicAdd(counter, 1u) == (unsigned)others;
+          if (is_last) *counter = 0;                               // for the next launch
+          flags[1] = is_last;
+        }
+        __syncthreads();
+        const bool is_last = flags[1] != 0;
+        __threadfence();
+        return is_last;
       };
-      if (whole) {
-        if (key_warp == 0) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = row_warp * 16 + quad + 8 * h;
-            if (r < p.rows) {
-              // padding, and rows that see nothing, are zero
-              const bool none = mask[h] == 0 || total[h] == 0.f;
-              const float f = 1.f / total[h];
-              T* out = out_row(r) + col;
-#pragma unroll
-              for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<uint32_t*>(out + 8 * i) = none ? 0u : Half16<T>::pack(o[i][2 * h] * f, o[i][2 * h + 1] * f);
-            }
-          }
-        }
-      } else {
-        // a partial: the slot of a range's first rows, or that of its last ones
-        float* slot = p.partials + (size_t)(2 * cta + (seg.t0 == 0 ? 1 : 0)) * kSlot;
-        if (key_warp == 0) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = row_warp * 16 + quad + 8 * h;
-            if (r < p.rows) {
-#pragma unroll
-              for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(slot + r * D + i * 8 + col) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-              if ((lane & 3) == 0) {
-                slot[kRowTile * D + r] = top[h];
-                slot[kRowTile * (D + 1) + r] = total[h];
-              }
-            }
-          }
-        }
-        const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
-        const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
-        const Joining join(first_cta, last_cta, cta, join_step(last_cta - first_cta + 1));
-        // whether this CTA is the last of those that a counter waits for; what the others wrote is visible then
-        auto last_at = [&](unsigned int* counter, int others) {
-          __threadfence();
-          __syncthreads();
-          if (tid == 0) {
-            const bool is_last = atomicAdd(counter, 1u) == (unsigned)others;
-            if (is_last) *counter = 0;                               // for the next launch
-            flags[1] = is_last;
-          }
-          __syncthreads();
-          const bool is_last = flags[1] != 0;
-          __threadfence();
-          return is_last;
-        };
-        auto slot_of = [&](int c) { return p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot; };
-        // Joins `count` partials, `step` CTAs apart: into the output, or into the first one's slot.  A warp has two rows at a time, a lane four or two columns of
-        // each; a lane fetches the maximum and total of one contributor, and eight contributors' sums are on their way together (one after the other took
-        // a latency each; 24 rows of 19 contributors: 43 us in all then, 35 now).
-        auto add_up = [&](int c0, int count, int step, bool ends) {
-          constexpr int V = D / 32, kTogether = 8;
-          for (int r0 = warp; r0 < p.rows; r0 += 8) {
-            float m[2] = {-INFINITY, -INFINITY}, sum[2] = {}, acc[2][V] = {};
-            const int rows[2] = {r0, r0 + 4 < p.rows ? r0 + 4 : r0};
-            for (int k0 = 0; k0 < count; k0 += 32) {
-              const int here = min(count - k0, 32);
-              float by[2];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float* from = slot_of(c0 + (k0 + min(lane, here - 1)) * step) + kRowTile * D + rows[h];
-                const float cm = lane < here ? __ldcg(from) : -INFINITY, ct = lane < here ? __ldcg(from + kRowTile) : 0.f;
-                float most = cm;
-#pragma unroll
-                for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float now = fmaxf(m[h], most), base = now == -INFINITY ? 0.f : now, old = exp2_approx(m[h] - base);
-                by[h] = exp2_approx(cm - base);
-                float part = ct * by[h];
-#pragma unroll
-                for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-                sum[h] = sum[h] * old + part;
-#pragma unroll
-                for (int i = 0; i < V; ++i) acc[h][i] *= old;
-                m[h] = now;
-              }
-              for (int j0 = 0; j0 < here; j0 += kTogether) {
-                float2 v[kTogether][2][V / 2];
-#pragma unroll
-                for (int e = 0; e < kTogether; ++e)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < V / 2; ++i)
-                      v[e][h][i] = j0 + e < here ? __ldcg(reinterpret_cast<const float2*>(slot_of(c0 + (k0 + j0 + e) * step) + rows[h] * D + lane * V) + i) : make_float2(0.f, 0.f);
-#pragma unroll
-                for (int e = 0; e < kTogether; ++e)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const float f = __shfl_sync(0xffffffffu, by[h], (j0 + e) & 31);
-#pragma unroll
-                    for (int i = 0; i < V / 2; ++i) {
-                      acc[h][2 * i] = fmaf(v[e][h][i].x, f, acc[h][2 * i]);
-                      acc[h][2 * i + 1] = fmaf(v[e][h][i].y, f, acc[h][2 * i + 1]);
-                    }
-                  }
-              }
-            }
+      auto slot_of = [&](int c) { return p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot; };
+      // Joins `count` partials, `step` CTAs apart: into the output, or into the first one's slot.  A warp has two rows at a time, a lane four or two columns of
+      // each; a lane fetches the maximum and total of one contributor, and eight contributors' sums are on their way together (one after the other took
+      // a latency each; 24 rows of 19 contributors: 43 us in all then, 35 now).
+      auto add_up = [&](int c0, int count, int step, bool ends) {
+        constexpr int V = D / 32, kTogether = 8;
+        for (int r0 = warp; r0 < p.rows; r0 += 8) {
+          float m[2] = {-INFINITY, -INFINITY}, sum[2] = {}, acc[2][V] = {};
+          const int rows[2] = {r0, r0 + 4 < p.rows ? r0 + 4 : r0};
+          for (int k0 = 0; k0 < count; k0 += 32) {
+            const int here = min(count - k0, 32);
+            float by[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int r = r0 + 4 * h;
-              if (r >= p.rows) break;
-              if (ends) {
-                const int t = r / p.group;
-                const bool none = mask_of(p, seg.b, t) == 0 || sum[h] == 0.f;      // padding, and rows that see nothing, are zero
-                const float f = 1.f / sum[h];
-                T* out = out_row(r) + lane * V;
+              const float* from = slot_of(c0 + (k0 + min(lane, here - 1)) * step) + kRowTile * D + rows[h];
+              const float cm = lane < here ? __ldcg(from) : -INFINITY, ct = lane < here ? __ldcg(from + kRowTile) : 0.f;
+              float most = cm;
 #pragma unroll
-                for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[h][i] * f, acc[h][i + 1] * f);
-              } else {
-                float* to = slot_of(c0);
+              for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+              const float now = fmaxf(m[h], most), base = now == -INFINITY ? 0.f : now, old = exp2_approx(m[h] - base);
+              by[h] = exp2_approx(cm - base);
+              float part = ct * by[h];
 #pragma unroll
-                for (int i = 0; i < V; i += 2) __stcg(reinterpret_cast<float2*>(to + r * D + lane * V + i), make_float2(acc[h][i], acc[h][i + 1]));
-                if (lane == 0) {
-                  __stcg(to + kRowTile * D + r, m[h]);
-                  __stcg(to + kRowTile * (D + 1) + r, sum[h]);
+              for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+              sum[h] = sum[h] * old + part;
+#pragma unroll
+              for (int i = 0; i < V; ++i) acc[h][i] *= old;
+              m[h] = now;
+            }
+            for (int j0 = 0; j0 < here; j0 += kTogether) {
+              float2 v[kTogether][2][V / 2];
+#pragma unroll
+              for (int e = 0; e < kTogether; ++e)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int i = 0; i < V / 2; ++i)
+                    v[e][h][i] = j0 + e < here ? __ldcg(reinterpret_cast<const float2*>(slot_of(c0 + (k0 + j0 + e) * step) + rows[h] * D + lane * V) + i) : make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < kTogether; ++e)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const float f = __shfl_sync(0xffffffffu, by[h], (j0 + e) & 31);
+#pragma unroll
+                  for (int i = 0; i < V / 2; ++i) {
+                    acc[h][2 * i] = fmaf(v[e][h][i].x, f, acc[h][2 * i]);
+                    acc[h][2 * i + 1] = fmaf(v[e][h][i].y, f, acc[h][2 * i + 1]);
+                  }
                 }
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = r0 + 4 * h;
+            if (r >= p.rows) break;
+            if (ends) {
+              const int t = r / p.group;
+              const bool none = mask_of(p, seg.b, t) == 0 || sum[h] == 0.f;      // padding, and rows that see nothing, are zero
+              const float f = 1.f / sum[h];
+              T* out = out_row(r) + lane * V;
+#pragma unroll
+              for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[h][i] * f, acc[h][i + 1] * f);
+            } else {
+              float* to = slot_of(c0);
+#pragma unroll
+              for (int i = 0; i < V; i += 2) __stcg(reinterpret_cast<float2*>(to + r * D + lane * V + i), make_float2(acc[h][i], acc[h][i + 1]));
+              if (lane == 0) {
+                __stcg(to + kRowTile * D + r, m[h]);
+                __stcg(to + kRowTile * (D + 1) + r, sum[h]);
               }
             }
           }
-        };
-        // (one loop, so that its code is there once: what runs for the first time takes longer to fetch than to run)
-        const bool grouped = join.step < join.count;
-        bool ends = !grouped;
-#pragma unroll 1
-        while (last_at(ends && grouped ? join.item_counter(p, 0) : join.group_counter(p, 0), (ends && grouped ? join.groups() : join.size) - 1)) {
-          add_up(ends ? first_cta : join.group, ends && grouped ? join.groups() : join.size, ends && grouped ? join.step : 1, ends);
-          if (ends) break;
-          ends = true;
         }
+      };
+      // (one loop, so that its code is there once: what runs for the first time takes longer to fetch than to run)
+      const bool grouped = join.step < join.count;
+      bool ends = !grouped;
+#pragma unroll 1
+      while (last_at(ends && grouped ? join.item_counter(p, 0) : join.group_counter(p, 0), (ends && grouped ? join.groups() : join.size) - 1)) {
+        add_up(ends ? first_cta : join.group, ends && grouped ? join.groups() : join.size, ends && grouped ? join.step : 1, ends);
+        if (ends) break;
+        ends = true;
       }
+    }
   }
   copies_wait<0>();
   if (tid == 0 && flags[0] && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
@@ -584,7 +584,7 @@ bool rows_aligned(const void* p, const long long (&strides)[kStrides]) {
 
 extern "C" {
 
-size_t fp6m_tree_attention_scratch_bytes(int sms) { 
+size_t fp6m_tree_attention_scratch_bytes(int sms) {
   const size_t few = (size_t)tree_ctas(sms) * 2 * kFewRows * (128 + 2) * sizeof(float), many = tree_tc5_partial_bytes(sms);
   return kCounterBytes + (few > many ? few : many);
 }
