@@ -92,8 +92,8 @@ def rms_norm(x, weight, y, eps=1e-6, *, scales=None, residual=None, residual_out
 
     ``residual`` (optional, like x) is added in fp32; the sum, rounded once, goes to ``residual_out`` (default: ``residual``
     itself, in place), and the norm goes on with the sum before that rounding.  Without ``scales`` ``y`` has x's type; with ``scales``
-    (M, ceil(N/128)) float32, ``y`` is float8_e4m3fn and ``y * scales`` (a scale for each 128 neighbours of a row: their
-    largest magnitude / 448) stands for the result: what :func:`mul_fp8` takes.  N must be a multiple of 8.
+    (M, ceil(N/128)) float32, ``y`` is float8_e4m3fn, the result divided by its scale (one for each 128 neighbours of a row: their
+    largest magnitude / 448), and ``y * scales`` stands for the result: what :func:`mul_fp8` takes.  N must be a multiple of 8.
     """
     # plain CUDA tensors that pass every check: one call into native code; anything else takes the general path below
     rc = _call.rms_norm(x, weight, y, eps, scales, residual, residual_out)
@@ -233,7 +233,8 @@ def tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, *,
     token sees all committed ones, except that an entry of 0 marks padding, which sees nothing and gives zeros.  Bits from T
     on mean nothing.  With T = 1 and tree = 1 this is ordinary decoding.  out: like q, overwritten.  ``scale`` defaults to ``D ** -0.5``.
 
-    Lengths and page numbers stay on the device: lengths are cut to what the page table can hold, and a page number that
+    Scores, maxima and sums are fp32; the weights of the softmax are rounded once, to q's type, before they meet the values, the result
+    once more.  Lengths and page numbers stay on the device: lengths are cut to what the page table can hold, and a page number that
     does not exist hides its tokens and is reported by :func:`device_status` (4).  What lies behind a sequence's last
     committed token, in the table or in a page, is not read.
     """

@@ -8,8 +8,9 @@
 // change with every block of 128 values of K, so a block is one accumulator tile of its own (four MMAs, the first one overwrites):
 // warps read it back, multiply it by sa * sb and add it to their sums in registers while the tensor cores work on the next blocks.
 //
-// Bound by the bytes of B.  8192 x 57344 (K x N), 16 rows: 86 us, 5.5 TB/s, 0.84 of what a copy reaches; the rest is the first data of a CTA (about 4 us
-// with the set-up) and the last ones' end.  4096 x 4096, one row: 7.3 us where the bytes take 2.6: set-up, first data, the exchange of sums.
+// Bound by the bytes of B.  8192 x 57344 (K x N), 16 rows, public calls one behind the other: 87.7 us, 5.4 TB/s, 0.82 of what a copy reaches; the rest is the first
+// data of a CTA (about 4 us with the set-up) and the last ones' end.  4096 x 4096, one row: 7.6 us where the bytes take 2.6: set-up, first data, the exchange of sums.
+// (Here and in the other kernel, figures of both sides of a choice are of replays of a graph.)
 // The blocks are cut into as many ranges as there are multiprocessors, so a strip's sums mostly come from two or three CTAs: words of
 // {value, tag} that the CTA in which the strip starts polls for; a tag needs no flag, no fence and no clearing.  A thread keeps at most 32 sums: with 64 of
 // them (rows 65 to 192 in this form) they were spilled and 128 rows of 11008 x 4096 took 39 us, against 21 in the other kernel.

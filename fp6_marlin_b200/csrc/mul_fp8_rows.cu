@@ -10,9 +10,9 @@
 // into equal ranges if that shortens the end by more than the exchange of their sums takes: all leave theirs in the scratch, and the
 // CTA that does so last adds them in the order of the ranges (an arrival counter; nobody waits).
 //
-// 4096 rows, 8192 x 28672 (K x N): 935 us, 2060 TFLOP/s, 1.23 times what a library product in bf16 reaches.  A block takes a pair 875 cycles, of which the tensor cores
+// 4096 rows, 8192 x 28672 (K x N), public calls one behind the other: 942 us, 2040 TFLOP/s, 1.22 times what a library product in bf16 reaches.  A block takes a pair 875 cycles, of which the tensor cores
 // work 512: between them lies the sums' way (256 read-backs, 256 multiply-adds and the barriers per thread and block), which two accumulator tiles - all that tensor
-// memory holds of 256 columns - do not hide in full, and the clock falls to about 1.6 GHz under the power limit.  131 rows, 11008 x 4096: 24 us where the bytes
+// memory holds of 256 columns - do not hide in full, and the clock falls to about 1.6 GHz under the power limit.  131 rows, 11008 x 4096: 25.4 us where the bytes
 // take 7: two row tiles of 32 KB a block each (37 blocks of 540 cycles), set-up and first data (7500 cycles), exchange (10000).
 #include "../../include/fp6m.h"
 #include "host_common.h"

@@ -72,8 +72,8 @@ __device__ __forceinline__ int groups_of(int N) { return (N - 1) / kGroup + 1; }
 
 // x / d, rounded once, from a reciprocal that is rounded once: the product's remainder is exact in a fused multiply-add, and what it adds makes up for the
 // reciprocal's error (P. Markstein, IBM Journal of Research and Development 34, 1990).  Two values at a time: three instructions, and one reciprocal for all
-// of a divisor's.  16384 x 8192 with the norm / 4099 x 11008 without, us through the public call: divisions
-// 178 / 36.2, this 155 / 26.8 (a multiplication by a reciprocal, which is off where a quotient lies between two E4M3 values: 152 / 26.4).
+// of a divisor's.  Against a multiplication by the reciprocal, which is off where a quotient lies between two E4M3 values, calls of 16384 x 8192 with the norm /
+// 4099 x 11008 without take 1 / 2 % longer, with divisions 17 / 37 %.
 struct Divisor {
   unsigned long long d, inverse;         // twice the same
   __device__ __forceinline__ explicit Divisor(float by) {
@@ -132,10 +132,10 @@ __device__ __forceinline__ void finish_vector(const RowParams& p, size_t row, in
 
 // One CTA a row; a thread holds kVecs groups of eight neighbouring values of it (a vector), blockDim.x vectors apart.  Every value is read once: what the
 // second half of the work needs stays in registers, and the weights are on their way while the squares are summed.  Sixteen lanes hold the
-// 128 values that share a scale.  Bound by memory: 16384 x 8192 with residual, fp16 to E4M3, takes 139 to 144 us,
-// 6.55 TB/s or more, which is what a plain copy reaches here (rows read twice, from L2 the second time: 190 us).  4099 x 11008 without the norm, fp16 to E4M3:
-// 27 us, 5.0 TB/s; its 4099 rows of eleven warps leave a last round of CTAs a quarter full.  Where rows are few, what counts is latency
-// (1 x 4096: 1.6 us): more threads with a vector each (launch_kind).
+// 128 values that share a scale.  Bound by memory: 16384 x 8192 with residual, fp16 to E4M3, takes 145 us in replays of a graph,
+// 6.5 TB/s, which is what a plain copy reaches here, and 162 us, 5.8 TB/s, in public calls one behind the other (rows read twice, from L2 the second time: 190 us in a
+// graph).  4099 x 11008 without the norm, fp16 to E4M3: 27.8 us, 4.9 TB/s, in calls; its 4099 rows of eleven warps leave a last round of CTAs a
+// quarter full.  Where rows are few, what counts is latency (1 x 4096: 1.6 us in a graph, 3.0 in calls): more threads with a vector each (launch_kind).
 template <class T, bool kNorm, bool kFp8, int kVecs>
 __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024) rows_kernel(const RowParams p) {
   __shared__ float part[32];
@@ -253,7 +253,7 @@ template <class T, bool kNorm, bool kFp8>
 cudaError_t launch_kind(const RowParams& p, cudaStream_t stream) {
   const int vecs = p.N / 8;
   // Few rows (a multiprocessor gets one or two): as many threads as there are vectors, up to 1024.  Many: four vectors a thread, so that more rows are in flight
-  // (16384 x 8192, norm, residual and E4M3: 144 us; two vectors a thread 163).
+  // (16384 x 8192, norm, residual and E4M3, in a graph: 144 us; two vectors a thread 163).
   const int kind = p.M > 512 && vecs >= 128 ? 4 : vecs <= 1024 ? 1 : 2;
   const int threads = ((vecs + kind - 1) / kind + 31) / 32 * 32;
   if (vecs > 2048) return launch_overlapped(long_rows_kernel<T, kNorm, kFp8>, dim3(p.M), dim3(1024), 0, stream, p);

@@ -14,9 +14,12 @@
 //
 // This file: up to 32 rows per head of keys, where mma.sync keeps up with memory (rows are padded to 16 or 32, a tile of tcgen05 would have 128) and what counts is
 // the time from a key's arrival to its use.  Two CTAs per multiprocessor, three tiles of keys and values on their way in each.  8 x 5 tokens, 32 heads, up to
-// 4096 cached: 55 us, 4.9 TB/s, 0.75 of what a copy reaches; bound by the instructions between two tiles (about 1660 cycles a tile and CTA) and
-// the tails of CTAs.  One token over 300: 10.4 us where the bytes take 0.8: the plan (2000 cycles), first look-ups and queries (2900), first data
-// (1200), two or three tiles, the end (1700).
+// 4096 cached, public calls one behind the other: 56 us, 4.8 TB/s, 0.73 of what a copy reaches; bound by the instructions between two tiles (about 1660 cycles a tile and CTA) and
+// the tails of CTAs.  One token over 300: 10.6 us where the bytes take 0.8: the plan (2000 cycles), first look-ups and queries (2900), first data
+// (1200), two or three tiles, the end (1700).  Figures of both sides of a choice are of replays of a graph.
+//
+// The weights are rounded once, to the values' type, for the second product (tensor cores take 16 bits; the sum that they are divided by has them unrounded): 2^-8 of
+// a weight at most in bf16, 2^-11 in fp16, where weights below 2^-14 of the largest become multiples of 2^-24.
 #include "device_utils.cuh"
 #include "host_common.h"
 #include "tree_attention.cuh"

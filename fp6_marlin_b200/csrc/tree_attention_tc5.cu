@@ -11,12 +11,13 @@
 // O is rescaled only where a row's maximum grows by more than a factor of 2^8: until then the weights are taken relative to the older
 // maximum, which changes neither the result nor, in fp32 sums and 16-bit floating-point weights, its precision.
 //
-// 2 x 64 tokens, 64 heads over 8, up to 32768 cached: 168 us, 820 TFLOP/s, 0.49 of what a library product reaches.  A job takes a pair of row tiles about 4700 cycles, the
+// 2 x 64 tokens, 64 heads over 8, up to 32768 cached, public calls one behind the other: 190 us, 724 TFLOP/s, 0.43 of what a library product reaches (replays of a graph: 160
+// to 176).  A job takes a pair of row tiles about 4700 cycles, the
 // tensor cores 2048 of them: a group's weights take 2400 (the maxima 290, then 128 exponentials at 1660 to 2000: 660 of other instructions and 1024 of the unit for
 // special functions, which a single warp per quarter does not overlap), then it waits for its product and its next scores, because tensor memory holds one
 // tile of scores per group beside the sums.  Measured and not kept: a fourth, an eighth or a sixteenth of the exponentials by a polynomial (+3, +1, 0 %),
 // sums and exponents in pairs (0), exponentials of one chunk between the sums of the last (+5 %, with or without registers moved to these warps).  The copies take 4 %.
-// 64 x 7 tokens, 64 heads over 8, up to 6144: 156 us, 5.3 TB/s, 0.80 of what a copy reaches.
+// 64 x 7 tokens, 64 heads over 8, up to 6144: 182 us, 4.5 TB/s, 0.69 of what a copy reaches (in a graph: 158 to 170).  Figures of both sides of a choice are of replays of a graph.
 #include <type_traits>
 
 #include "../../include/fp6m.h"

@@ -9,7 +9,7 @@ down projections in INT4 / FP6.  A step takes the drafted tokens of every sequen
     -> rms_norm with the residual's addition -> E4M3 -> mul_fp8 (gate, up) -> silu * up -> mul_fused (down projection + residual)
 
 What the drafted tokens are not needed for any more once some are accepted - their keys and values - then goes into the cache
-(:meth:`DraftBlock.accept`).  The program prints the time of a step and how far it is from the same step in elementary torch operations.
+(:meth:`DraftBlock.accept`).  The program prints the time of a step and the relative error of its result against the same step in elementary torch operations.
 """
 from __future__ import annotations
 

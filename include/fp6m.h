@@ -262,7 +262,8 @@ int fp6m_mul_fp8(const void* A, const void* B, void* C, const void* sa, const vo
  * and gives zeros.  With one token and the mask 1 this is ordinary decoding.  Heads of queries share the heads of keys in groups of heads / kv_heads neighbours.
  * Strides are in elements, multiples of 8; the head_dim (64 or 128) values of a head lie next to one another; pointers 16-byte
  * aligned.  Lengths are read on the device, cut to 0 .. max_pages * page_size (2^31 - 65536 at most); a page number outside 0 .. pages - 1 hides its
- * tokens and sets the status word to FP6M_ERR_BAD_ARG.  Entries of page_table behind a sequence's last page, and slots
+ * tokens and sets the status word to FP6M_ERR_BAD_ARG.  Scores, maxima and sums are fp32; the softmax's weights are rounded to `type` before
+ * they meet the values.  Entries of page_table behind a sequence's last page, and slots
  * of a page behind its last token, are not read. */
 typedef struct fp6m_tree_attention_args {
   const void *q, *k, *v;              /* batch x tokens x (heads | kv_heads) x head_dim */
