@@ -247,8 +247,8 @@ int fp6m_quantize_fp8(const void* x, void* q, void* scales, int M, int N, int ty
 
 /* C[M, N] = A[M, K] B[N, K]^T, A and B in E4M3 (row-major), C in `type` (overwritten), with fp32 scales for blocks of 128:
  * sa (M x ceil(K / 128)) for 128 neighbours of a row of A, sb (ceil(N / 128) x ceil(K / 128)) for 128 x 128 values of B.  Sums in
- * fp32, one rounding.  K a multiple of 16, N of 8, none above 2^31 - 256 (FP6M_ERR_PROB_SHAPE
- * otherwise); A, B, C and scratch 16-byte aligned.
+ * fp32, one rounding.  K a multiple of 16, N of 8, none above 2^31 - 256, fewer than 2^30 blocks of
+ * 128 x 128 x 128 in all (FP6M_ERR_PROB_SHAPE otherwise); A, B, C and scratch 16-byte aligned.
  *   scratch     >= fp6m_mul_fp8_scratch_bytes(...) bytes of device memory, zeroed before the first use and then left to this
  *               function; calls that can overlap on the GPU need one each
  *   status_dev  optional device int: set to FP6M_ERR_TIMEOUT if a bounded wait ran out */
