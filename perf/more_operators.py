@@ -308,7 +308,7 @@ def _verify(state):
         p = torch.where(inside, rest.gather(1, token)[:, 0], 0)
         if draft is None:
             accept = uniforms[:, i].double() < p
-            less = rest.scatter(1, token, 0)
+            less = rest.scatter(1, token, torch.where(inside, 0, rest.gather(1, token)[:, 0])[:, None])
         else:
             row = _clean(draft[at, node])
             accept = uniforms[:, i].double() * torch.where(inside, row.gather(1, token)[:, 0], 0) < p
