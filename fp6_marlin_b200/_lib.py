@@ -17,7 +17,7 @@ OK, ERR_PROB_SHAPE, ERR_KERN_SHAPE, ERR_VALUE_RANGE, ERR_BAD_ARG = 0, 1, 2, 3, 4
 ERR_WORKSPACE, ERR_SCRATCH, ERR_CUDA, ERR_TIMEOUT, ERR_NO_MEMORY = 5, 6, 7, 8, 9
 LAYOUT_REFERENCE, LAYOUT_B200 = 0, 1
 EPILOGUE_NONE, EPILOGUE_SILU_MUL, EPILOGUE_RESIDUAL = 0, 1, 2
-TYPE_F16, TYPE_BF16 = 0, 1
+TYPE_F16, TYPE_BF16, TYPE_F32 = 0, 1, 2
 
 
 class TreeAttentionArgs(ctypes.Structure):
@@ -28,6 +28,29 @@ class TreeAttentionArgs(ctypes.Structure):
                 + [(name, ctypes.c_longlong) for name in ("page_table_stride", "tree_stride")]
                 + [(name, ctypes.c_int) for name in ("batch", "tokens", "heads", "kv_heads", "head_dim", "pages", "page_size", "max_pages", "type")]
                 + [("scale", ctypes.c_float)])
+
+
+class CacheScales(ctypes.Structure):
+    """fp6m_cache_scales of include/fp6m.h."""
+
+    _fields_ = [("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p), ("k_scales_stride", ctypes.c_longlong * 3), ("v_scales_stride", ctypes.c_longlong * 3)]
+
+
+class CacheFp8Args(ctypes.Structure):
+    """fp6m_cache_fp8_args of include/fp6m.h."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("k", "v", "k_cache", "v_cache", "page_table", "lengths", "list", "counts", "starts")]
+                + [(name, ctypes.c_longlong * 3) for name in ("k_stride", "v_stride", "k_cache_stride", "v_cache_stride")]
+                + [(name, ctypes.c_longlong) for name in ("page_table_stride", "list_stride")]
+                + [(name, ctypes.c_int) for name in ("batch", "tokens", "entries", "kv_heads", "head_dim", "pages", "page_size", "max_pages", "type")])
+
+
+class VerifyDraftsArgs(ctypes.Structure):
+    """fp6m_verify_drafts_args of include/fp6m.h."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("target", "draft", "drafted", "tree", "uniforms", "accepted", "counts", "next_tokens")]
+                + [("target_stride", ctypes.c_longlong * 2), ("draft_stride", ctypes.c_longlong * 2), ("tree_stride", ctypes.c_longlong)]
+                + [(name, ctypes.c_int) for name in ("batch", "tokens", "vocab", "type")])
 
 
 # every symbol include/fp6m.h declares, with its ctypes signature
@@ -75,6 +98,11 @@ SIGNATURES = {
     "fp6m_mul_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz, _i, _vp, _vp]),
     "fp6m_tree_attention_scratch_bytes": (_sz, [_i]),
     "fp6m_tree_attention": (_i, [ctypes.POINTER(TreeAttentionArgs), _vp, _sz, _i, _vp, _vp]),
+    "fp6m_write_cache_fp8": (_i, [ctypes.POINTER(CacheFp8Args), ctypes.POINTER(CacheScales), _i, _vp, _vp]),
+    "fp6m_read_cache_fp8": (_i, [ctypes.POINTER(CacheFp8Args), ctypes.POINTER(CacheScales), _i, _vp, _vp]),
+    "fp6m_tree_attention_fp8_scratch_bytes": (_sz, [_i]),
+    "fp6m_tree_attention_fp8": (_i, [ctypes.POINTER(TreeAttentionArgs), ctypes.POINTER(CacheScales), _vp, _sz, _i, _vp, _vp]),
+    "fp6m_verify_drafts": (_i, [ctypes.POINTER(VerifyDraftsArgs), _i, _vp]),
     "fp6m_zeroed_memory": (_i, [_sz, _i, ctypes.POINTER(_vp)]),
     "fp6m_set_launch_overlap": (ctypes.c_int, [ctypes.c_int]),
     "fp6m_set_ordered_sums": (ctypes.c_int, [ctypes.c_int]),

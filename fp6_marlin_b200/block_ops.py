@@ -24,7 +24,7 @@ _TYPES = {torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 
 _call.bind_operators(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
     "fp6m_rms_norm", "fp6m_quantize_fp8", "fp6m_mul_fp8", "fp6m_mul_fp8_scratch_bytes", "fp6m_tree_attention", "fp6m_tree_attention_scratch_bytes")))
-_OWNERS = {"mul_fp8": 1, "tree_attention": 2}     # of a scratch, as the native call path numbers them
+_OWNERS = {"mul_fp8": 1, "tree_attention": 2, "tree_attention_fp8": 3}     # of a scratch, as the native call path numbers them
 
 _scratch: dict[tuple, list[torch.Tensor]] = {}    # (operator, device, stream) -> buffers, the last is in use
 
@@ -212,15 +212,53 @@ def tree_masks(parents):
 
 def _strides(what, name, t, dtype, shape, device, written=False):
     if t.dtype != dtype or t.dim() != 4 or tuple(t.shape) != shape:
-        raise RuntimeError(f"{what}: {name} must be of shape {shape} and q's type")
+        raise RuntimeError(f"{what}: {name} must be of shape {shape} and {'type float8_e4m3fn' if dtype == torch.float8_e4m3fn else 'of the same type as the others of 16 bits'}")
     if t.device != device:
-        raise RuntimeError(f"{what}: {name} must be on q's device")
+        raise RuntimeError(f"{what}: {name} must be on the same CUDA device as the other tensors")
     s = [shape[3] if size == 1 else step for size, step in zip(shape[:3], t.stride())] + [t.stride(3)]      # (that of a single place says nothing)
-    if t.numel() and (s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or t.data_ptr() % 16):
+    of = 16 // dtype.itemsize
+    if t.numel() and (s[3] != 1 or s[0] % of or s[1] % of or s[2] % of or t.data_ptr() % 16):
         raise RuntimeError(f"{what}: the values of a head of {name} must lie next to one another, on 16-byte boundaries")
     if written and any(size > 1 and step == 0 for size, step in zip(shape, s)):
         raise RuntimeError(f"{what}: places of {name} share memory")
     return (ctypes.c_longlong * 3)(*s[:3])
+
+
+def _tree_args(what, q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale, cache_type):
+    """The checks of attention over a paged cache, and its arguments for the C ABI (None: there is nothing to do)."""
+    if not q.is_cuda:
+        raise RuntimeError(f"fp6_marlin_b200.{what} needs CUDA tensors: there is no CPU implementation")
+    if q.dtype not in _TYPES or q.dim() != 4:
+        raise RuntimeError(f"{what}: q must be (B, T, H, D) of float16 or bfloat16")
+    b, t, h, d = q.shape
+    g = k.shape[2] if k.dim() == 4 else 0
+    if t > 64 or d not in (64, 128) or g == 0 or h % g:
+        raise RuntimeError(f"{what}: at most 64 tokens, heads of 64 or 128 values, and a multiple of the heads of keys as heads of queries")
+    if k_cache.dim() != 4 or page_table.dim() != 2:
+        raise RuntimeError(f"{what}: the cache must be (pages, page size, {g}, {d}) and the page table (B, P)")
+    pages, page_size = k_cache.shape[:2]
+    device = q.device
+    args = _lib.TreeAttentionArgs(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(page_table), _ptr(lengths), _ptr(tree),
+        _strides(what, "q", q, q.dtype, (b, t, h, d), device), _strides(what, "k", k, q.dtype, (b, t, g, d), device),
+        _strides(what, "v", v, q.dtype, (b, t, g, d), device), _strides(what, "out", out, q.dtype, (b, t, h, d), device, True),
+        _strides(what, "k_cache", k_cache, cache_type, (pages, page_size, g, d), device),
+        _strides(what, "v_cache", v_cache, cache_type, (pages, page_size, g, d), device))
+    if page_table.dtype != torch.int32 or page_table.shape[0] != b or lengths.dtype != torch.int32 or lengths.shape != (b,):
+        raise RuntimeError(f"{what}: page_table must be int32 (B, P) and lengths int32 (B,)")
+    if tree.dtype != torch.int64 or tree.shape not in ((t,), (b, t)):
+        raise RuntimeError(f"{what}: tree must be int64 of shape ({t},) or ({b}, {t})")
+    if page_table.device != device or lengths.device != device or tree.device != device:
+        raise RuntimeError(f"{what}: page_table, lengths and tree must be on q's device")
+    if any(x.numel() and x.shape[-1] > 1 and x.stride(-1) != 1 for x in (page_table, lengths, tree)):
+        raise RuntimeError(f"{what}: the rows of page_table and tree, and lengths, must be contiguous")
+    if b == 0 or t == 0 or h == 0:
+        return None
+    args.page_table_stride, args.tree_stride = page_table.stride(0), tree.stride(0) if tree.dim() == 2 else 0
+    args.batch, args.tokens, args.heads, args.kv_heads, args.head_dim = b, t, h, g, d
+    args.pages, args.page_size, args.max_pages, args.type = pages, max(page_size, 1), page_table.shape[1] if pages and page_size else 0, _TYPES[q.dtype]
+    args.scale = d ** -0.5 if scale is None else scale
+    return args
 
 
 def tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, *, scale=None):
@@ -244,38 +282,10 @@ def tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, *,
         return
     if rc > 0:
         _raise(what, rc)
-    if not q.is_cuda:
-        raise RuntimeError("fp6_marlin_b200.tree_attention needs CUDA tensors: there is no CPU implementation")
-    if q.dtype not in _TYPES or q.dim() != 4:
-        raise RuntimeError(f"{what}: q must be (B, T, H, D) of float16 or bfloat16")
-    b, t, h, d = q.shape
-    g = k.shape[2] if k.dim() == 4 else 0
-    if t > 64 or d not in (64, 128) or g == 0 or h % g:
-        raise RuntimeError(f"{what}: at most 64 tokens, heads of 64 or 128 values, and a multiple of the heads of keys as heads of queries")
-    if k_cache.dim() != 4 or page_table.dim() != 2:
-        raise RuntimeError(f"{what}: the cache must be (pages, page size, {g}, {d}) and the page table (B, P)")
-    pages, page_size = k_cache.shape[:2]
-    device = q.device
-    args = _lib.TreeAttentionArgs(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(page_table), _ptr(lengths), _ptr(tree),
-        _strides(what, "q", q, q.dtype, (b, t, h, d), device), _strides(what, "k", k, q.dtype, (b, t, g, d), device),
-        _strides(what, "v", v, q.dtype, (b, t, g, d), device), _strides(what, "out", out, q.dtype, (b, t, h, d), device, True),
-        _strides(what, "k_cache", k_cache, q.dtype, (pages, page_size, g, d), device),
-        _strides(what, "v_cache", v_cache, q.dtype, (pages, page_size, g, d), device))
-    if page_table.dtype != torch.int32 or page_table.shape[0] != b or lengths.dtype != torch.int32 or lengths.shape != (b,):
-        raise RuntimeError(f"{what}: page_table must be int32 (B, P) and lengths int32 (B,)")
-    if tree.dtype != torch.int64 or tree.shape not in ((t,), (b, t)):
-        raise RuntimeError(f"{what}: tree must be int64 of shape ({t},) or ({b}, {t})")
-    if page_table.device != device or lengths.device != device or tree.device != device:
-        raise RuntimeError(f"{what}: page_table, lengths and tree must be on q's device")
-    if any(x.numel() and x.shape[-1] > 1 and x.stride(-1) != 1 for x in (page_table, lengths, tree)):
-        raise RuntimeError(f"{what}: the rows of page_table and tree, and lengths, must be contiguous")
-    if b == 0 or t == 0 or h == 0:
+    args = _tree_args(what, q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale, q.dtype)
+    if args is None:
         return
-    args.page_table_stride, args.tree_stride = page_table.stride(0), tree.stride(0) if tree.dim() == 2 else 0
-    args.batch, args.tokens, args.heads, args.kv_heads, args.head_dim = b, t, h, g, d
-    args.pages, args.page_size, args.max_pages, args.type = pages, max(page_size, 1), page_table.shape[1] if pages and page_size else 0, _TYPES[q.dtype]
-    args.scale = d ** -0.5 if scale is None else scale
+    device = q.device
     stream = _stream_handle(device.index, device)
     scratch, status = _operator_buffers(what, device, lib.fp6m_tree_attention_scratch_bytes(_sms(device)), stream)
     rc = lib.fp6m_tree_attention(ctypes.byref(args), _ptr(scratch), scratch.numel(), device.index, stream, _ptr(status))

@@ -22,7 +22,7 @@ CALL_SOURCES = [os.path.join(CSRC, "py_call.cpp"), os.path.join(os.path.dirname(
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 
 CUDA_SOURCES = ["c_api.cu", "gemm_few.cu", "gemm_team.cu", "gemm_tc5.cu", "gemm_wide.cu", "dump_operands.cu", "prep_gpu.cu", "gather_columns.cu", "peer.cu",
-                "rows.cu", "mul_fp8.cu", "mul_fp8_rows.cu", "tree_attention.cu", "tree_attention_tc5.cu"]
+                "rows.cu", "mul_fp8.cu", "mul_fp8_rows.cu", "tree_attention.cu", "tree_attention_tc5.cu", "tree_attention_fp8.cu", "cache_fp8.cu", "verify_drafts.cu"]
 HOST_SOURCES = ["host_pack.cpp"]
 
 NVCC_FLAGS = [

@@ -51,8 +51,8 @@ struct StreamKey {
 struct StreamKeyHash {
   size_t operator()(const StreamKey& k) const { return std::hash<void*>()(k.stream) * 31 + (size_t)k.dev; }
 };
-// of the GEMMs, of mul_fp8, of tree_attention
-enum { kOfGemms = 0, kOfMulFp8 = 1, kOfTreeAttention = 2, kOwners = 3 };
+// of the GEMMs, of mul_fp8, of tree_attention, of tree_attention_fp8
+enum { kOfGemms = 0, kOfMulFp8 = 1, kOfTreeAttention = 2, kOfTreeAttentionFp8 = 3, kOwners = 4 };
 std::unordered_map<StreamKey, Scratch, StreamKeyHash>& scratches(int owner = kOfGemms) {
   static auto* m = new std::unordered_map<StreamKey, Scratch, StreamKeyHash>[kOwners];
   return m[owner];
@@ -374,7 +374,7 @@ PyObject* py_set_scratch(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// set_operator_scratch(owner, dev, stream, address, bytes): likewise, of mul_fp8 (1) or tree_attention (2)
+// set_operator_scratch(owner, dev, stream, address, bytes): likewise, of mul_fp8 (1), tree_attention (2) or tree_attention_fp8 (3)
 PyObject* py_set_operator_scratch(PyObject*, PyObject* args) {
   int owner, dev;
   unsigned long long stream, ptr, bytes;

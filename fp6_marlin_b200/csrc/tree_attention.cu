@@ -34,34 +34,7 @@ constexpr int kMaxCtas = 512;
 // With at least 3 / 6 units per CTA: one token over 1000, 32 heads over 8, 12.9 / 17.0; sixteen over up to 500 13.4 / 15.4; one over 8000 17.9 / 19.1.
 constexpr int kLeastUnits = 3, kSlack = 8;
 constexpr int kCounterBytes = kMaxCtas * 2 * 3 * 4;
-// contributors of a group: see Joining
-__device__ __forceinline__ int join_step(int count) {
-  if (count <= 24) return count;
-  int step = 8;
-  while (step * step < count) step += 8;
-  return step;
-}
 
-template <class T> struct Mma;
-template <> struct Mma<half> {
-  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Mma<__nv_bfloat16> {
-  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-
-__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 // kRowTile rows, a warp for every 16 of them; the warps that this leaves share the keys of a tile and pool their sums.
 template <class T, int D, int kRowTile>
 __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __grid_constant__ TreeParams p) {
@@ -71,7 +44,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
   constexpr int kStages = 3 * 128 / D;
   constexpr int kChunks = D / 8, kRowsPerPass = kThreads / kChunks, kPasses = kKeys / kRowsPerPass;
   constexpr int kPool = D / kRowWarps;                               // columns of the sums that are pooled at a time
-  constexpr int kSlot = kRowTile * (D + 2);                          // floats of a partial
+  constexpr int kSlot = slot_floats<D, kRowTile, false>();
   extern __shared__ __align__(128) uint8_t smem[];
   float* pool = reinterpret_cast<float*>(smem + kStages * 2 * kTileBytes);        // [kRowTile][kPool]
   float* stats = pool + kRowTile * kPool;                                          // [warp][2][16]: maxima, totals
@@ -414,10 +387,6 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
       }
     }
     const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
-    auto out_row = [&](int r) {
-      const int t = r / p.group, head = g * p.group + (r - t * p.group);
-      return static_cast<T*>(a.out) + seg.b * a.out_stride[0] + t * a.out_stride[1] + head * a.out_stride[2];
-    };
     if (whole) {
       if (key_warp == 0) {
 #pragma unroll
@@ -427,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
             // padding, and rows that see nothing, are zero
             const bool none = mask[h] == 0 || total[h] == 0.f;
             const float f = 1.f / total[h];
-            T* out = out_row(r) + col;
+            T* out = out_row<T>(p, seg.b, g, r) + col;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
               *reinterpret_cast<uint32_t*>(out + 8 * i) = none ? 0u : Half16<T>::pack(o[i][2 * h] * f, o[i][2 * h + 1] * f);
@@ -453,104 +422,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_attention_kernel(const __gri
       }
       const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
       const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
-      const Joining join(first_cta, last_cta, cta, join_step(last_cta - first_cta + 1));
-      // whether this CTA is the last of those that a counter waits for; what the others wrote is visible then
-      auto last_at = [&](unsigned int* counter, int others) {
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          const bool is_last = atomicAdd(counter, 1u) == (unsigned)others;
-          if (is_last) *counter = 0;                               // for the next launch
-          flags[1] = is_last;
-        }
-        __syncthreads();
-        const bool is_last = flags[1] != 0;
-        __threadfence();
-        return is_last;
-      };
-      auto slot_of = [&](int c) { return p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot; };
-      // Joins `count` partials, `step` CTAs apart: into the output, or into the first one's slot.  A warp has two rows at a time, a lane four or two columns of
-      // each; a lane fetches the maximum and total of one contributor, and eight contributors' sums are on their way together (one after the other took
-      // a latency each; 24 rows of 19 contributors: 43 us in all then, 35 now).
-      auto add_up = [&](int c0, int count, int step, bool ends) {
-        constexpr int V = D / 32, kTogether = 8;
-        for (int r0 = warp; r0 < p.rows; r0 += 8) {
-          float m[2] = {-INFINITY, -INFINITY}, sum[2] = {}, acc[2][V] = {};
-          const int rows[2] = {r0, r0 + 4 < p.rows ? r0 + 4 : r0};
-          for (int k0 = 0; k0 < count; k0 += 32) {
-            const int here = min(count - k0, 32);
-            float by[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float* from = slot_of(c0 + (k0 + min(lane, here - 1)) * step) + kRowTile * D + rows[h];
-              const float cm = lane < here ? __ldcg(from) : -INFINITY, ct = lane < here ? __ldcg(from + kRowTile) : 0.f;
-              float most = cm;
-#pragma unroll
-              for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-              const float now = fmaxf(m[h], most), base = now == -INFINITY ? 0.f : now, old = exp2_approx(m[h] - base);
-              by[h] = exp2_approx(cm - base);
-              float part = ct * by[h];
-#pragma unroll
-              for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-              sum[h] = sum[h] * old + part;
-#pragma unroll
-              for (int i = 0; i < V; ++i) acc[h][i] *= old;
-              m[h] = now;
-            }
-            for (int j0 = 0; j0 < here; j0 += kTogether) {
-              float2 v[kTogether][2][V / 2];
-#pragma unroll
-              for (int e = 0; e < kTogether; ++e)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                  for (int i = 0; i < V / 2; ++i)
-                    v[e][h][i] = j0 + e < here ? __ldcg(reinterpret_cast<const float2*>(slot_of(c0 + (k0 + j0 + e) * step) + rows[h] * D + lane * V) + i) : make_float2(0.f, 0.f);
-#pragma unroll
-              for (int e = 0; e < kTogether; ++e)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const float f = __shfl_sync(0xffffffffu, by[h], (j0 + e) & 31);
-#pragma unroll
-                  for (int i = 0; i < V / 2; ++i) {
-                    acc[h][2 * i] = fmaf(v[e][h][i].x, f, acc[h][2 * i]);
-                    acc[h][2 * i + 1] = fmaf(v[e][h][i].y, f, acc[h][2 * i + 1]);
-                  }
-                }
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = r0 + 4 * h;
-            if (r >= p.rows) break;
-            if (ends) {
-              const int t = r / p.group;
-              const bool none = mask_of(p, seg.b, t) == 0 || sum[h] == 0.f;      // padding, and rows that see nothing, are zero
-              const float f = 1.f / sum[h];
-              T* out = out_row(r) + lane * V;
-#pragma unroll
-              for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[h][i] * f, acc[h][i + 1] * f);
-            } else {
-              float* to = slot_of(c0);
-#pragma unroll
-              for (int i = 0; i < V; i += 2) __stcg(reinterpret_cast<float2*>(to + r * D + lane * V + i), make_float2(acc[h][i], acc[h][i + 1]));
-              if (lane == 0) {
-                __stcg(to + kRowTile * D + r, m[h]);
-                __stcg(to + kRowTile * (D + 1) + r, sum[h]);
-              }
-            }
-          }
-        }
-      };
-      // (one loop, so that its code is there once: what runs for the first time takes longer to fetch than to run)
-      const bool grouped = join.step < join.count;
-      bool ends = !grouped;
-#pragma unroll 1
-      while (last_at(ends && grouped ? join.item_counter(p, 0) : join.group_counter(p, 0), (ends && grouped ? join.groups() : join.size) - 1)) {
-        add_up(ends ? first_cta : join.group, ends && grouped ? join.groups() : join.size, ends && grouped ? join.step : 1, ends);
-        if (ends) break;
-        ends = true;
-      }
+      const Joining join(first_cta, last_cta, cta, few_rows_join_step(last_cta - first_cta + 1));
+      join_rows<T, D, kRowTile, false>(p, seg.b, g, 0, p.rows, join, cta, flags + 1);
     }
   }
   copies_wait<0>();
@@ -575,14 +448,6 @@ int tree_ctas(int sms) {
   return want < kMaxCtas ? want : kMaxCtas;
 }
 
-// addresses and strides (in elements) of a tensor that is read or written sixteen bytes at a time
-template <int kStrides>
-bool rows_aligned(const void* p, const long long (&strides)[kStrides]) {
-  bool ok = p && aligned16(p);
-  for (long long s : strides) ok = ok && s >= 0 && s % 8 == 0;
-  return ok;
-}
-
 }  // namespace
 
 extern "C" {
@@ -594,39 +459,16 @@ size_t fp6m_tree_attention_scratch_bytes(int sms) {
 
 int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev) {
   if (!args) return FP6M_ERR_BAD_ARG;
-  const fp6m_tree_attention_args& a = *args;
-  if (a.batch < 0 || a.tokens < 0 || a.heads < 0 || (a.type != FP6M_TYPE_F16 && a.type != FP6M_TYPE_BF16)) return FP6M_ERR_BAD_ARG;
-  if (a.tokens > 64 || (a.head_dim != 64 && a.head_dim != 128)) return FP6M_ERR_PROB_SHAPE;
-  if (a.batch == 0 || a.tokens == 0 || a.heads == 0) return FP6M_OK;
-  if (a.kv_heads <= 0 || a.heads % a.kv_heads) return FP6M_ERR_PROB_SHAPE;
-  // (pages are looked up in blocks of up to 2048 tokens, two of them ahead, so tokens stay that far from 2^31)
-  if (a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fff0000ll) return FP6M_ERR_PROB_SHAPE;
-  if ((long long)a.tokens * a.heads > 0xffffffll) return FP6M_ERR_PROB_SHAPE;
-  if (!rows_aligned(a.q, a.q_stride) || !rows_aligned(a.k, a.k_stride) || !rows_aligned(a.v, a.v_stride) || !rows_aligned(a.out, a.out_stride)) return FP6M_ERR_BAD_ARG;
-  if (!a.lengths || !a.tree || a.tree_stride < 0 || !scratch || !aligned16(scratch)) return FP6M_ERR_BAD_ARG;
-  if (a.max_pages > 0 && (!rows_aligned(a.k_cache, a.k_cache_stride) || !rows_aligned(a.v_cache, a.v_cache_stride) || !a.page_table || a.page_table_stride < 0)) return FP6M_ERR_BAD_ARG;
+  const int rc = check_tree_args(*args, 8, scratch);
+  if (rc != FP6M_OK || args->batch == 0 || args->tokens == 0 || args->heads == 0) return rc;
   DeviceGuard guard(dev);
   const int sms = sm_count(dev);
   if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
   if (scratch_bytes < fp6m_tree_attention_scratch_bytes(sms)) return FP6M_ERR_SCRATCH;
-  TreeParams p;
-  p.a = a;
-  p.group = a.heads / a.kv_heads;
-  p.rows = a.tokens * p.group;
-  p.row_tiles = p.parts = 1;
-  p.overhead = 4;
-  int log2 = 0;
-  while ((1ll << log2) < a.page_size) ++log2;
-  p.page_shift = 31 + log2;
-  p.page_magic = ((1ull << p.page_shift) + a.page_size - 1) / a.page_size;
-  p.scale_log2 = a.scale * 1.4426950408889634f;
-  if (p.scale_log2 == 0.f) p.scale_log2 = 1e-37f;      // a masked score of minus infinity stays that
-  p.arrived = static_cast<unsigned int*>(scratch);
-  p.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + kCounterBytes);
-  p.status = status_dev;
+  const TreeParams p = tree_params(*args, scratch, kCounterBytes, status_dev);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = p.rows > kFewRows ? launch_tree_tc5(p, sms, st)
-                        : a.type == FP6M_TYPE_F16 ? launch_tree<half>(p, tree_ctas(sms), st) : launch_tree<__nv_bfloat16>(p, tree_ctas(sms), st);
+                        : args->type == FP6M_TYPE_F16 ? launch_tree<half>(p, tree_ctas(sms), st) : launch_tree<__nv_bfloat16>(p, tree_ctas(sms), st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "tree_attention launch");
 }
 

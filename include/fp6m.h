@@ -228,8 +228,8 @@ int fp6m_gather_columns(const void* c, void* y, const void* src, const void* bia
 /* GPU side: what stands between the products of a decoder block                              */
 /* ------------------------------------------------------------------------------------------ */
 
-/* 16-bit types of the operators below. */
-enum { FP6M_TYPE_F16 = 0, FP6M_TYPE_BF16 = 1 };
+/* Types of the operators below (the last of probabilities only). */
+enum { FP6M_TYPE_F16 = 0, FP6M_TYPE_BF16 = 1, FP6M_TYPE_F32 = 2 };
 
 /* Root-mean-square norm of the M rows of x (M x N, row-major, 16 bits), with the residual's addition and, if `scales` is
  * given, E4M3 output:  h = x + residual (fp32; written to residual_out, rounded once, which may be x or residual itself),
@@ -281,6 +281,66 @@ typedef struct fp6m_tree_attention_args {
 /* Scratch as in fp6m_mul_fp8; enough for any shape on a device with `sms` multiprocessors. */
 size_t fp6m_tree_attention_scratch_bytes(int sms);
 int fp6m_tree_attention(const fp6m_tree_attention_args* args, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
+
+/* A paged cache in 8 bits: keys and values in E4M3, a byte for each token and head with the exponent of its power of two, plus 127; K * 2^(byte - 127)
+ * stands for the key (bytes 1..254).  Strides are in elements: of the caches multiples of 16, the head_dim values of a head next to one another; of
+ * the bytes any. */
+typedef struct fp6m_cache_scales {
+  void *k_scales, *v_scales;          /* pages x page_size x kv_heads bytes */
+  long long k_scales_stride[3], v_scales_stride[3];                    /* page, slot, head */
+} fp6m_cache_scales;
+/* Tokens into and out of such a cache.
+ * fp6m_write_cache_fp8: the first counts[b] (counts null: all `entries`) entries of sequence b's list become the tokens lengths[b], lengths[b] + 1, ... of
+ * its pages.  An entry is a number 0 .. tokens - 1 of k and v, or negative: nothing is written for it; list null: entry i is token i.  Each
+ * head gets the least exponent in -15..8 (fp16) or -40..120 (bf16) with which its largest finite magnitude stays within 448, its values are divided by
+ * that power, rounded to E4M3, and end at 240 where the exponent is the highest (so that what is read back is finite in their type);
+ * infinities and NaN become NaN.  An entry without a place - behind the page table, in a page that does not exist, a token that does not - is not
+ * written and sets the status word to FP6M_ERR_BAD_ARG.
+ * fp6m_read_cache_fp8: row i of sequence b of k and v (`entries` rows) becomes token starts[b] + i (starts null: token i), times its power and rounded to
+ * `type`; rows of tokens before the first or from lengths[b] on are left as they were, as are those in a page that does not exist, which sets the status word.
+ * Lengths are cut to 0 .. max_pages * page_size (2^31 - 65536 at most). */
+typedef struct fp6m_cache_fp8_args {
+  void *k, *v;                        /* batch x (tokens | entries) x kv_heads x head_dim, 16 bits */
+  void *k_cache, *v_cache;            /* pages x page_size x kv_heads x head_dim */
+  const int *page_table;              /* batch x max_pages */
+  const int *lengths;                 /* batch */
+  const int *list, *counts;           /* write: batch x entries, batch, or null */
+  const int *starts;                  /* read: batch, or null */
+  long long k_stride[3], v_stride[3]; /* batch, token, head */
+  long long k_cache_stride[3], v_cache_stride[3];                      /* page, slot, head */
+  long long page_table_stride, list_stride;
+  int batch, tokens, entries, kv_heads, head_dim, pages, page_size, max_pages, type;
+} fp6m_cache_fp8_args;
+int fp6m_write_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, int dev, void* stream, int* status_dev);
+int fp6m_read_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, int dev, void* stream, int* status_dev);
+/* fp6m_tree_attention over such a cache: k_cache and v_cache of `args` are E4M3 (strides as above); the drafted tokens' q, k, v and out are of its type.  The
+ * softmax's weights, each times its value's power of two, are rounded to fp16 (up to 32 rows of a head of keys) or `type` before they meet the values. */
+size_t fp6m_tree_attention_fp8_scratch_bytes(int sms);
+int fp6m_tree_attention_fp8(const fp6m_tree_attention_args* args, const fp6m_cache_scales* scales, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
+
+/* Which drafted tokens of each sequence are accepted, and the token after them, so that the tokens are distributed as the target's probabilities say.
+ * The drafted tokens form a tree: `tree` as in fp6m_tree_attention, a token's parent is the last earlier token that it sees.  Token 0 is the one that the
+ * step before has chosen; it is accepted as it is (with a mask of zero the sequence is padding: nothing is accepted, the next token is -1).
+ * target[b, i] and draft[b, i] are the probabilities of the token after token i, the target's and those that i's children were drawn from.  From a
+ * token n that is accepted on, with r = target[b, n]: its children c are looked at in order, and c is accepted, and takes n's place, if
+ *   uniforms[b, c] * draft[b, n][id] < r[id],  id = drafted[b, c];    otherwise r <- max(r - draft[b, n], 0) divided by its sum.
+ * Where none is accepted, the next token is the lowest x with r[0] + ... + r[x] > uniforms[b, 0] * (sum of r).  Without draft the children were chosen and not
+ * drawn: 1 takes the place of draft[b, n][id], and r[id] <- 0 that of the subtraction.  If nothing of r remains, further children are not accepted and the next token is
+ * drawn from target[b, n] itself (-1 if that holds nothing).  Probabilities that are negative, infinite or NaN count as 0, sums are taken in 64 bits; an id
+ * outside 0 .. vocab - 1 has the probability 0 in both.
+ *   accepted    batch x tokens ints: the accepted tokens' numbers in order, then -1;  counts: how many;  next_tokens: 64-bit ints */
+typedef struct fp6m_verify_drafts_args {
+  const void *target, *draft;         /* batch x tokens x vocab; draft may be null */
+  const long long* drafted;           /* batch x tokens */
+  const unsigned long long* tree;     /* batch x tokens */
+  const float* uniforms;              /* batch x tokens, 0 <= u < 1 */
+  int *accepted, *counts;
+  long long* next_tokens;
+  long long target_stride[2], draft_stride[2];                         /* batch, token */
+  long long tree_stride;              /* from one sequence to the next (0: all alike) */
+  int batch, tokens, vocab, type;     /* tokens at most 64; type of the probabilities, FP6M_TYPE_F32 too */
+} fp6m_verify_drafts_args;
+int fp6m_verify_drafts(const fp6m_verify_drafts_args* args, int dev, void* stream);
 
 /* `bytes` bytes of device memory, all zero when the call returns: for scratch and status words.  Also while a stream is captured, by this thread or
  * another: neither the allocation nor the zeroing becomes part of a graph (memory zeroed inside a graph is not zero before its first
