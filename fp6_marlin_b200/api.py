@@ -50,7 +50,7 @@ class _GeneralPathOnly:
     def mul(self, *args):
         return -1                             # not handled
 
-    rms_norm = quantize_fp8 = mul_fp8 = tree_attention = mul
+    rms_norm = quantize_fp8 = mul_fp8 = tree_attention = write_cache_fp8 = read_cache_fp8 = tree_attention_fp8 = verify_drafts = mul
 
 
 def _native_call_path():

@@ -23,7 +23,8 @@ SMALLEST = 1e-30                                  # largest magnitude that a gro
 _TYPES = {torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 
 _call.bind_operators(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-    "fp6m_rms_norm", "fp6m_quantize_fp8", "fp6m_mul_fp8", "fp6m_mul_fp8_scratch_bytes", "fp6m_tree_attention", "fp6m_tree_attention_scratch_bytes")))
+    "fp6m_rms_norm", "fp6m_quantize_fp8", "fp6m_mul_fp8", "fp6m_mul_fp8_scratch_bytes", "fp6m_tree_attention", "fp6m_tree_attention_scratch_bytes",
+    "fp6m_write_cache_fp8", "fp6m_read_cache_fp8", "fp6m_tree_attention_fp8", "fp6m_tree_attention_fp8_scratch_bytes", "fp6m_verify_drafts")))
 _OWNERS = {"mul_fp8": 1, "tree_attention": 2, "tree_attention_fp8": 3}     # of a scratch, as the native call path numbers them
 
 _scratch: dict[tuple, list[torch.Tensor]] = {}    # (operator, device, stream) -> buffers, the last is in use

@@ -729,17 +729,26 @@ cudaError_t encode_bytes_map(const void* base, int rows, int K, int box_rows, CU
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 
-// A paged cache of 16-bit values as a tensor of head_dim x heads x page_size x pages with any strides but 0 (elements: page, slot, head); one box
-// = 64 values of `run` neighbouring tokens, in 128-byte rows with the 128-byte swizzle; what lies outside reads as zero.
-cudaError_t encode_cache_map(const void* base, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, CUtensorMap* map) {
+// A paged cache of values of `value_bytes` bytes (1 or 2) as a tensor of head_dim x heads x page_size x pages with any strides but 0 (elements: page, slot, head); one
+// box = 128 bytes of `run` neighbouring tokens (64, where a head has no more), in rows with a swizzle of as many bytes; what lies outside reads as zero.
+static cudaError_t encode_cache(const void* base, int value_bytes, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, bool swizzled, CUtensorMap* map) {
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)page_size, (cuuint64_t)pages};
-  cuuint64_t pitches[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
+  cuuint64_t pitches[3] = {(cuuint64_t)(strides[2] * value_bytes), (cuuint64_t)(strides[1] * value_bytes), (cuuint64_t)(strides[0] * value_bytes)};
   for (int i = 0; i < 3; ++i) {
-    if (dims[i + 1] == 1) pitches[i] = (cuuint64_t)head_dim * 2;          // (says nothing)
+    if (dims[i + 1] == 1) pitches[i] = (cuuint64_t)(head_dim * value_bytes);      // (says nothing)
     if (pitches[i] == 0) return cudaErrorInvalidValue;                  // heads, tokens or pages that share memory are not a tensor map's
   }
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)run, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, pitches, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+  const bool narrow = head_dim * value_bytes < 128;
+  const cuuint32_t box[4] = {(cuuint32_t)((narrow ? 64 : 128) / value_bytes), 1, (cuuint32_t)run, 1};
+  return encode(map, value_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, pitches, box,
+                !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+}
+cudaError_t encode_cache_map(const void* base, int value_bytes, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, CUtensorMap* map) {
+  return encode_cache(base, value_bytes, head_dim, heads, page_size, pages, strides, run, true, map);
+}
+// The same for values of a byte, rows as they are.
+cudaError_t encode_plain_cache_map(const void* base, int head_dim, int heads, int page_size, int pages, const long long (&strides)[3], int run, CUtensorMap* map) {
+  return encode_cache(base, 1, head_dim, heads, page_size, pages, strides, run, false, map);
 }
 
 static int tile_height(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 15) / 16 * 16; }

@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <type_traits>
 #include <unordered_map>
 
 #include "../../include/fp6m.h"
@@ -35,6 +36,11 @@ decltype(&fp6m_mul_fp8) g_mul_fp8 = nullptr;
 decltype(&fp6m_mul_fp8_scratch_bytes) g_mul_fp8_scratch_bytes = nullptr;
 decltype(&fp6m_tree_attention) g_tree_attention = nullptr;
 decltype(&fp6m_tree_attention_scratch_bytes) g_tree_attention_scratch_bytes = nullptr;
+decltype(&fp6m_write_cache_fp8) g_write_cache_fp8 = nullptr;
+decltype(&fp6m_read_cache_fp8) g_read_cache_fp8 = nullptr;
+decltype(&fp6m_tree_attention_fp8) g_tree_attention_fp8 = nullptr;
+decltype(&fp6m_tree_attention_fp8_scratch_bytes) g_tree_attention_fp8_scratch_bytes = nullptr;
+decltype(&fp6m_verify_drafts) g_verify_drafts = nullptr;
 
 constexpr long kNotHandled = -1;
 
@@ -223,65 +229,198 @@ bool heads_of(const at::Tensor* t, int64_t a, int64_t b, int64_t c, int64_t d, a
   if (!t || t->dim() != 4 || t->size(0) != a || t->size(1) != b || t->size(2) != c || t->size(3) != d || t->scalar_type() != type || t->device().index() != dev ||
       t->stride(3) != 1 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16)
     return false;
+  const int of = 16 / (int)t->element_size();
   for (int i = 0; i < 3; ++i) {
     strides[i] = t->size(i) == 1 ? d : t->stride(i);          // (that of a single place says nothing)
-    if (strides[i] % 8 || (written && strides[i] == 0 && t->size(i) > 1)) return false;
+    if (strides[i] % of || (written && strides[i] == 0 && t->size(i) > 1)) return false;
   }
   return true;
 }
+// The bytes of a cache's powers of two.
+bool scales_of(const at::Tensor* t, int64_t a, int64_t b, int64_t c, int dev, bool written, long long (&strides)[3]) {
+  if (!t || t->dim() != 3 || t->size(0) != a || t->size(1) != b || t->size(2) != c || t->scalar_type() != at::kByte || t->device().index() != dev) return false;
+  for (int i = 0; i < 3; ++i) {
+    strides[i] = t->size(i) == 1 ? 1 : t->stride(i);
+    if (written && strides[i] == 0 && t->size(i) > 1) return false;
+  }
+  return true;
+}
+// Ints of `dims` dimensions whose rows are contiguous.
+bool ints_of(const at::Tensor* t, int64_t rows, int dev, int dims = 1) {
+  return t && t->dim() == dims && t->size(0) == rows && t->scalar_type() == at::kInt && t->device().index() == dev && (t->size(dims - 1) <= 1 || t->stride(dims - 1) == 1);
+}
+bool pages_of(const at::Tensor& cache, const at::Tensor& table) {
+  return cache.dim() == 4 && table.dim() == 2 && cache.size(0) > 0 && cache.size(1) > 0 && table.size(1) > 0 && cache.size(0) <= INT32_MAX && cache.size(1) <= INT32_MAX && table.size(1) <= INT32_MAX;
+}
 
-// tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale)
-PyObject* tree_attention_impl(PyObject* const* args) {
-  const at::Tensor* t[9];
-  for (int i = 0; i < 9; ++i)
-    if (!(t[i] = plain_strided(args[i]))) return PyLong_FromLong(kNotHandled);
+// q, k, v, k_cache, v_cache, page_table, lengths, tree, out and the scale -> the arguments of the C ABI; false: not handled
+bool tree_args_of(const at::Tensor* const (&t)[9], PyObject* scale, bool fp8, fp6m_tree_attention_args* a) {
   const at::Tensor &q = *t[0], &k = *t[1], &k_cache = *t[3], &table = *t[5], &lengths = *t[6], &tree = *t[7];
-  fp6m_tree_attention_args a;
-  if (q.dim() != 4 || k.dim() != 4 || k_cache.dim() != 4 || table.dim() != 2 || lengths.dim() != 1 || !type_of(q, &a.type)) return PyLong_FromLong(kNotHandled);
+  if (q.dim() != 4 || k.dim() != 4 || !pages_of(k_cache, table) || lengths.dim() != 1 || !type_of(q, &a->type)) return false;
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3), G = k.size(2), pages = k_cache.size(0), page_size = k_cache.size(1), most = table.size(1);
   const int dev = q.device().index();
-  const at::ScalarType type = q.scalar_type();
-  if (B <= 0 || T <= 0 || H <= 0 || T > 64 || (D != 64 && D != 128) || G <= 0 || H % G || pages <= 0 || page_size <= 0 || most <= 0 || dev < 0 || dev >= 64 ||
-      !g_devices[dev].status || B > INT32_MAX || H > INT32_MAX || pages > INT32_MAX || page_size > INT32_MAX || most > INT32_MAX)
-    return PyLong_FromLong(kNotHandled);
-  if (!heads_of(t[0], B, T, H, D, type, dev, false, a.q_stride) || !heads_of(t[1], B, T, G, D, type, dev, false, a.k_stride) ||
-      !heads_of(t[2], B, T, G, D, type, dev, false, a.v_stride) || !heads_of(t[3], pages, page_size, G, D, type, dev, false, a.k_cache_stride) ||
-      !heads_of(t[4], pages, page_size, G, D, type, dev, false, a.v_cache_stride) || !heads_of(t[8], B, T, H, D, type, dev, true, a.out_stride))
-    return PyLong_FromLong(kNotHandled);
+  const at::ScalarType type = q.scalar_type(), cache_type = fp8 ? at::kFloat8_e4m3fn : type;
+  if (B <= 0 || T <= 0 || H <= 0 || T > 64 || (D != 64 && D != 128) || G <= 0 || H % G || dev < 0 || dev >= 64 || !g_devices[dev].status || B > INT32_MAX || H > INT32_MAX) return false;
+  if (!heads_of(t[0], B, T, H, D, type, dev, false, a->q_stride) || !heads_of(t[1], B, T, G, D, type, dev, false, a->k_stride) ||
+      !heads_of(t[2], B, T, G, D, type, dev, false, a->v_stride) || !heads_of(t[3], pages, page_size, G, D, cache_type, dev, false, a->k_cache_stride) ||
+      !heads_of(t[4], pages, page_size, G, D, cache_type, dev, false, a->v_cache_stride) || !heads_of(t[8], B, T, H, D, type, dev, true, a->out_stride))
+    return false;
   const bool own_masks = tree.dim() == 2;
   if (table.scalar_type() != at::kInt || table.size(0) != B || table.stride(1) != 1 || table.device().index() != dev || lengths.scalar_type() != at::kInt || lengths.size(0) != B ||
       !lengths.is_contiguous() || lengths.device().index() != dev || tree.scalar_type() != at::kLong || tree.device().index() != dev || (!own_masks && tree.dim() != 1) ||
       tree.size(own_masks ? 1 : 0) != T || (own_masks && tree.size(0) != B) || tree.stride(own_masks ? 1 : 0) != 1)
-    return PyLong_FromLong(kNotHandled);
-  a.scale = D == 64 ? 0.125f : 0.08838834764831845f;
-  if (args[9] != Py_None && !as_float(args[9], &a.scale)) return PyLong_FromLong(kNotHandled);
-  a.q = q.data_ptr();
-  a.k = k.data_ptr();
-  a.v = t[2]->data_ptr();
-  a.out = t[8]->data_ptr();
-  a.k_cache = k_cache.data_ptr();
-  a.v_cache = t[4]->data_ptr();
-  a.page_table = static_cast<const int*>(table.data_ptr());
-  a.lengths = static_cast<const int*>(lengths.data_ptr());
-  a.tree = static_cast<const unsigned long long*>(tree.data_ptr());
-  a.page_table_stride = table.stride(0);
-  a.tree_stride = own_masks ? tree.stride(0) : 0;
-  a.batch = (int)B;
-  a.tokens = (int)T;
-  a.heads = (int)H;
-  a.kv_heads = (int)G;
-  a.head_dim = (int)D;
-  a.pages = (int)pages;
-  a.page_size = (int)page_size;
-  a.max_pages = (int)most;
+    return false;
+  a->scale = D == 64 ? 0.125f : 0.08838834764831845f;
+  if (scale != Py_None && !as_float(scale, &a->scale)) return false;
+  a->q = q.data_ptr();
+  a->k = k.data_ptr();
+  a->v = t[2]->data_ptr();
+  a->out = t[8]->data_ptr();
+  a->k_cache = k_cache.data_ptr();
+  a->v_cache = t[4]->data_ptr();
+  a->page_table = static_cast<const int*>(table.data_ptr());
+  a->lengths = static_cast<const int*>(lengths.data_ptr());
+  a->tree = static_cast<const unsigned long long*>(tree.data_ptr());
+  a->page_table_stride = table.stride(0);
+  a->tree_stride = own_masks ? tree.stride(0) : 0;
+  a->batch = (int)B;
+  a->tokens = (int)T;
+  a->heads = (int)H;
+  a->kv_heads = (int)G;
+  a->head_dim = (int)D;
+  a->pages = (int)pages;
+  a->page_size = (int)page_size;
+  a->max_pages = (int)most;
+  return true;
+}
+
+// tree_attention(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale); tree_attention_fp8 has (k_scales, v_scales) behind them
+PyObject* tree_attention_impl(PyObject* const* args, bool fp8) {
+  const at::Tensor* t[9];
+  for (int i = 0; i < 9; ++i)
+    if (!(t[i] = plain_strided(args[i]))) return PyLong_FromLong(kNotHandled);
+  fp6m_tree_attention_args a;
+  if (!tree_args_of(t, args[9], fp8, &a)) return PyLong_FromLong(kNotHandled);
+  const int dev = t[0]->device().index();
+  fp6m_cache_scales s;
+  if (fp8) {
+    const at::Tensor *ks = plain_strided(args[10]), *vs = plain_strided(args[11]);
+    if (!scales_of(ks, a.pages, a.page_size, a.kv_heads, dev, false, s.k_scales_stride) || !scales_of(vs, a.pages, a.page_size, a.kv_heads, dev, false, s.v_scales_stride)) return PyLong_FromLong(kNotHandled);
+    s.k_scales = ks->data_ptr();
+    s.v_scales = vs->data_ptr();
+  }
   void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-  const auto it = scratches(kOfTreeAttention).find({dev, stream});
-  if (it == scratches(kOfTreeAttention).end() || it->second.bytes < g_tree_attention_scratch_bytes(g_devices[dev].sms)) return PyLong_FromLong(kNotHandled);
+  const int owner = fp8 ? kOfTreeAttentionFp8 : kOfTreeAttention;
+  const auto it = scratches(owner).find({dev, stream});
+  if (it == scratches(owner).end() || it->second.bytes < (fp8 ? g_tree_attention_fp8_scratch_bytes : g_tree_attention_scratch_bytes)(g_devices[dev].sms)) return PyLong_FromLong(kNotHandled);
   const Scratch scratch = it->second;
   int* status = g_devices[dev].status;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = g_tree_attention(&a, scratch.ptr, scratch.bytes, dev, stream, status);
+  rc = fp8 ? g_tree_attention_fp8(&a, &s, scratch.ptr, scratch.bytes, dev, stream, status) : g_tree_attention(&a, scratch.ptr, scratch.bytes, dev, stream, status);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// write_cache_fp8(k, v, k_cache, v_cache, k_scales, v_scales, page_table, lengths, tokens, counts); read_cache_fp8 has (starts) in place of the last two
+PyObject* cache_impl(PyObject* const* args, bool write) {
+  const at::Tensor* t[8];
+  for (int i = 0; i < 8; ++i)
+    if (!(t[i] = plain_strided(args[i]))) return PyLong_FromLong(kNotHandled);
+  const at::Tensor &k = *t[0], &k_cache = *t[2], &table = *t[6];
+  fp6m_cache_fp8_args a = {};
+  fp6m_cache_scales s;
+  if (k.dim() != 4 || !pages_of(k_cache, table) || !type_of(k, &a.type)) return PyLong_FromLong(kNotHandled);
+  const int64_t B = k.size(0), T = k.size(1), G = k.size(2), D = k.size(3), pages = k_cache.size(0), page_size = k_cache.size(1);
+  const int dev = k.device().index();
+  const at::ScalarType type = k.scalar_type();
+  if (B <= 0 || T <= 0 || G <= 0 || (D != 64 && D != 128) || dev < 0 || dev >= 64 || !g_devices[dev].status || B > INT32_MAX || T > INT32_MAX || G > INT32_MAX) return PyLong_FromLong(kNotHandled);
+  if (!heads_of(t[0], B, T, G, D, type, dev, !write, a.k_stride) || !heads_of(t[1], B, T, G, D, type, dev, !write, a.v_stride) ||
+      !heads_of(t[2], pages, page_size, G, D, at::kFloat8_e4m3fn, dev, write, a.k_cache_stride) || !heads_of(t[3], pages, page_size, G, D, at::kFloat8_e4m3fn, dev, write, a.v_cache_stride) ||
+      !scales_of(t[4], pages, page_size, G, dev, write, s.k_scales_stride) || !scales_of(t[5], pages, page_size, G, dev, write, s.v_scales_stride) || !ints_of(t[6], B, dev, 2) || !ints_of(t[7], B, dev))
+    return PyLong_FromLong(kNotHandled);
+  a.entries = (int)T;
+  for (int i = 8; i < (write ? 10 : 9); ++i) {
+    if (args[i] == Py_None) continue;
+    const at::Tensor* list = plain_strided(args[i]);
+    const bool tokens = write && i == 8;
+    if (!ints_of(list, B, dev, tokens ? 2 : 1)) return PyLong_FromLong(kNotHandled);
+    const int* ptr = static_cast<const int*>(list->data_ptr());
+    if (tokens) {
+      if (list->size(1) <= 0 || list->size(1) > INT32_MAX) return PyLong_FromLong(kNotHandled);
+      a.list = ptr;
+      a.entries = (int)list->size(1);
+      a.list_stride = list->stride(0);
+    } else {
+      (write ? a.counts : a.starts) = ptr;
+    }
+  }
+  a.k = k.data_ptr();
+  a.v = t[1]->data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = t[3]->data_ptr();
+  s.k_scales = t[4]->data_ptr();
+  s.v_scales = t[5]->data_ptr();
+  a.page_table = static_cast<const int*>(table.data_ptr());
+  a.lengths = static_cast<const int*>(t[7]->data_ptr());
+  a.page_table_stride = table.stride(0);
+  a.batch = (int)B;
+  a.tokens = (int)T;
+  a.kv_heads = (int)G;
+  a.head_dim = (int)D;
+  a.pages = (int)pages;
+  a.page_size = (int)page_size;
+  a.max_pages = (int)table.size(1);
+  void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  int* status = g_devices[dev].status;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = (write ? g_write_cache_fp8 : g_read_cache_fp8)(&a, &s, dev, stream, status);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+// verify_drafts(target, draft, drafted, tree, uniforms, accepted, counts, next_tokens)
+PyObject* verify_drafts_impl(PyObject* const* args) {
+  const at::Tensor* target = plain_strided(args[0]);
+  const bool has_draft = args[1] != Py_None;
+  const at::Tensor* draft = has_draft ? plain_strided(args[1]) : target;
+  const at::Tensor *drafted = plain_cuda(args[2]), *tree = plain_strided(args[3]), *uniforms = plain_cuda(args[4]), *accepted = plain_cuda(args[5]), *counts = plain_cuda(args[6]), *next = plain_cuda(args[7]);
+  if (!target || !draft || !drafted || !tree || !uniforms || !accepted || !counts || !next || target->dim() != 3 || draft->dim() != 3) return PyLong_FromLong(kNotHandled);
+  fp6m_verify_drafts_args a;
+  if (target->scalar_type() == at::kFloat) a.type = FP6M_TYPE_F32;
+  else if (!type_of(*target, &a.type)) return PyLong_FromLong(kNotHandled);
+  const int64_t B = target->size(0), T = target->size(1), V = target->size(2);
+  const int dev = target->device().index();
+  if (B <= 0 || T <= 0 || T > 64 || V <= 0 || B > INT32_MAX || V > INT32_MAX || dev < 0) return PyLong_FromLong(kNotHandled);
+  for (const at::Tensor* t : {target, draft})
+    if (t->size(0) != B || t->size(1) != T || t->size(2) != V || (V > 1 && t->stride(2) != 1) || t->scalar_type() != target->scalar_type() || t->device().index() != dev) return PyLong_FromLong(kNotHandled);
+  const bool own_masks = tree->dim() == 2;
+  if (!is_matrix(drafted, B, T, at::kLong, dev) || !is_matrix(uniforms, B, T, at::kFloat, dev) || !is_matrix(accepted, B, T, at::kInt, dev) || counts->dim() != 1 || counts->size(0) != B ||
+      counts->scalar_type() != at::kInt || counts->device().index() != dev || next->dim() != 1 || next->size(0) != B || next->scalar_type() != at::kLong || next->device().index() != dev ||
+      tree->scalar_type() != at::kLong || tree->device().index() != dev || (!own_masks && tree->dim() != 1) || tree->size(own_masks ? 1 : 0) != T || (own_masks && tree->size(0) != B) ||
+      (T > 1 && tree->stride(own_masks ? 1 : 0) != 1))
+    return PyLong_FromLong(kNotHandled);
+  a.target = target->data_ptr();
+  a.draft = has_draft ? draft->data_ptr() : nullptr;
+  a.drafted = static_cast<const long long*>(drafted->data_ptr());
+  a.tree = static_cast<const unsigned long long*>(tree->data_ptr());
+  a.uniforms = static_cast<const float*>(uniforms->data_ptr());
+  a.accepted = static_cast<int*>(accepted->data_ptr());
+  a.counts = static_cast<int*>(counts->data_ptr());
+  a.next_tokens = static_cast<long long*>(next->data_ptr());
+  for (int i = 0; i < 2; ++i) {
+    a.target_stride[i] = target->stride(i);
+    a.draft_stride[i] = draft->stride(i);
+  }
+  a.tree_stride = own_masks ? tree->stride(0) : 0;
+  a.batch = (int)B;
+  a.tokens = (int)T;
+  a.vocab = (int)V;
+  void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_verify_drafts(&a, dev, stream);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);
 }
@@ -310,7 +449,19 @@ PyObject* py_mul_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded("mul_fp8", nargs, 5, [&] { return mul_fp8_impl(args); });
 }
 PyObject* py_tree_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  return guarded("tree_attention", nargs, 10, [&] { return tree_attention_impl(args); });
+  return guarded("tree_attention", nargs, 10, [&] { return tree_attention_impl(args, false); });
+}
+PyObject* py_tree_attention_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded("tree_attention_fp8", nargs, 12, [&] { return tree_attention_impl(args, true); });
+}
+PyObject* py_write_cache_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded("write_cache_fp8", nargs, 10, [&] { return cache_impl(args, true); });
+}
+PyObject* py_read_cache_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded("read_cache_fp8", nargs, 9, [&] { return cache_impl(args, false); });
+}
+PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded("verify_drafts", nargs, 8, [&] { return verify_drafts_impl(args); });
 }
 
 PyObject* py_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -336,16 +487,24 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// bind_operators(rms_norm, quantize_fp8, mul_fp8, its scratch_bytes, tree_attention, its scratch_bytes): likewise
+// bind_operators(rms_norm, quantize_fp8, mul_fp8, its scratch_bytes, tree_attention, its scratch_bytes, write_cache_fp8, read_cache_fp8, tree_attention_fp8, its
+// scratch_bytes, verify_drafts): likewise
 PyObject* py_bind_operators(PyObject*, PyObject* args) {
-  unsigned long long a, b, c, d, e, f;
-  if (!PyArg_ParseTuple(args, "KKKKKK", &a, &b, &c, &d, &e, &f)) return nullptr;
-  g_rms_norm = reinterpret_cast<decltype(g_rms_norm)>(a);
-  g_quantize_fp8 = reinterpret_cast<decltype(g_quantize_fp8)>(b);
-  g_mul_fp8 = reinterpret_cast<decltype(g_mul_fp8)>(c);
-  g_mul_fp8_scratch_bytes = reinterpret_cast<decltype(g_mul_fp8_scratch_bytes)>(d);
-  g_tree_attention = reinterpret_cast<decltype(g_tree_attention)>(e);
-  g_tree_attention_scratch_bytes = reinterpret_cast<decltype(g_tree_attention_scratch_bytes)>(f);
+  unsigned long long a[11];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10])) return nullptr;
+  int i = 0;
+  auto set = [&](auto& function) { function = reinterpret_cast<std::remove_reference_t<decltype(function)>>(a[i++]); };
+  set(g_rms_norm);
+  set(g_quantize_fp8);
+  set(g_mul_fp8);
+  set(g_mul_fp8_scratch_bytes);
+  set(g_tree_attention);
+  set(g_tree_attention_scratch_bytes);
+  set(g_write_cache_fp8);
+  set(g_read_cache_fp8);
+  set(g_tree_attention_fp8);
+  set(g_tree_attention_fp8_scratch_bytes);
+  set(g_verify_drafts);
   Py_RETURN_NONE;
 }
 
@@ -396,6 +555,10 @@ PyMethodDef kMethods[] = {
     {"quantize_fp8", (PyCFunction)(void (*)(void))py_quantize_fp8, METH_FASTCALL, "rows to E4M3, likewise"},
     {"mul_fp8", (PyCFunction)(void (*)(void))py_mul_fp8, METH_FASTCALL, "8-bit product, likewise"},
     {"tree_attention", (PyCFunction)(void (*)(void))py_tree_attention, METH_FASTCALL, "attention over a paged cache, likewise"},
+    {"tree_attention_fp8", (PyCFunction)(void (*)(void))py_tree_attention_fp8, METH_FASTCALL, "attention over a cache in 8 bits, likewise"},
+    {"write_cache_fp8", (PyCFunction)(void (*)(void))py_write_cache_fp8, METH_FASTCALL, "tokens into a cache in 8 bits, likewise"},
+    {"read_cache_fp8", (PyCFunction)(void (*)(void))py_read_cache_fp8, METH_FASTCALL, "tokens out of it, likewise"},
+    {"verify_drafts", (PyCFunction)(void (*)(void))py_verify_drafts, METH_FASTCALL, "verification of drafted tokens, likewise"},
     {"bind_operators", py_bind_operators, METH_VARARGS, "addresses of the C ABI's functions of the operators"},
     {"set_operator_scratch", py_set_operator_scratch, METH_VARARGS, "scratch of an operator on a device's stream"},
     {"mul", (PyCFunction)(void (*)(void))py_mul, METH_FASTCALL, "GEMM on plain CUDA tensors: C ABI status, or -1 when the call is not handled here"},

@@ -7,11 +7,14 @@
 #include <stdint.h>
 
 #include "../../include/fp6m.h"
+#include "device_utils.cuh"
 #include "host_common.h"
 
 namespace fp6m {
 
 constexpr int kKeys = 64;                // keys per tile
+constexpr int kMaxTreeCtas = 512;
+constexpr int kCounterBytes = kMaxTreeCtas * 2 * 3 * 4;
 
 struct TreeParams {
   fp6m_tree_attention_args a;
@@ -31,7 +34,7 @@ struct TreeParams {
 // 2 x 3, 64 over 8, 8192: 34.9 / 36.7; 64 x 4, 64 over 8, up to 4096: 114.2 / 114.7; 16 x 5, 32 over 8, up to 4000: 41.4 / 44.4.
 constexpr int kFewRows = 32;
 size_t tree_tc5_partial_bytes(int sms);
-cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream);
+cudaError_t launch_tree_tc5(TreeParams p, const fp6m_cache_scales* scales, int sms, cudaStream_t stream);      // scales: of a cache in 8 bits, or null
 
 // Addresses and strides of a tensor that is read or written sixteen bytes at a time, `of` elements.
 template <int kStrides>
@@ -252,6 +255,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t b
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass: weights are relative to an older one until then
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -278,7 +282,7 @@ __device__ __forceinline__ bool is_odd(uint32_t two) {
   return (two & E) == E || (two >> 16 & E) == E;
 }
 
-// ---- for the kernels of four warps whose rows are few (tree_attention.cu, tree_attention_fp8.cu) ----
+// ---- for the kernels whose rows are few (tree_attention.cu, tree_attention_fp8.cu)
 
 template <class T> struct Mma;
 template <> struct Mma<half> {
@@ -298,142 +302,6 @@ __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-
-// contributors of a group: see Joining
-__device__ __forceinline__ int few_rows_join_step(int count) {
-  if (count <= 24) return count;
-  int step = 8;
-  while (step * step < count) step += 8;
-  return step;
-}
-// Where row r of a head of keys goes.
-template <class T>
-__device__ __forceinline__ T* out_row(const TreeParams& p, int b, int g, int r) {
-  const int t = r / p.group, head = g * p.group + (r - t * p.group);
-  return static_cast<T*>(p.a.out) + b * p.a.out_stride[0] + t * p.a.out_stride[1] + head * p.a.out_stride[2];
-}
-// A partial: sums [row][column], maxima, totals, and (kOdd) whether infinities or NaN were met among the drafted values, which are added at the end.
-template <int D, int kRowTile, bool kOdd>
-constexpr int slot_floats() { return kRowTile * (D + 2) + (kOdd ? 4 : 0); }
-// The infinite and NaN values of the drafted tokens that row r sees, added to columns c .. c + N - 1 of its result.
-template <class T, int N>
-__device__ __forceinline__ void add_odd_values(const TreeParams& p, int b, int g, int r, int c, float (&v)[N]) {
-  const unsigned long long mask = mask_of(p, b, r / p.group);
-  for (int j = 0; j < p.a.tokens; ++j) {
-    if (!(mask >> j & 1)) continue;
-    const uint16_t* from = static_cast<const uint16_t*>(p.a.v) + b * p.a.v_stride[0] + j * p.a.v_stride[1] + g * p.a.v_stride[2] + c;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if ((from[i] & Half16<T>::kExponent) == Half16<T>::kExponent) v[i] += Half16<T>::value(from[i]);
-  }
-}
-// Called by all threads of a CTA that has left its partial of rows row0 .. row0 + rows - 1 of (b, g): the last contributor joins them (see Joining).
-template <class T, int D, int kRowTile, bool kOdd>
-__device__ __forceinline__ void join_rows(const TreeParams& p, int b, int g, int row0, int rows, const Joining& join, int cta, int* last_flag) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, first_cta = join.first;
-  constexpr int kSlot = slot_floats<D, kRowTile, kOdd>();
-  // whether this CTA is the last of those that a counter waits for; what the others wrote is visible then
-  auto last_at = [&](unsigned int* counter, int others) {
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      const bool is_last = atomicAdd(counter, 1u) == (unsigned)others;
-      if (is_last) *counter = 0;                               // for the next launch
-      *last_flag = is_last;
-    }
-    __syncthreads();
-    const bool is_last = *last_flag != 0;
-    __threadfence();
-    return is_last;
-  };
-  auto slot_of = [&](int c) { return p.partials + (size_t)(2 * c + (c == first_cta ? 1 : 0)) * kSlot; };
-  // Joins `count` partials, `step` CTAs apart: into the output, or into the first one's slot.  A warp has two rows at a time, a lane four or two columns of
-  // each; a lane fetches the maximum and total of one contributor, and eight contributors' sums are on their way together (one after the other took
-  // a latency each; 24 rows of 19 contributors: 43 us in all then, 35 now).
-  auto add_up = [&](int c0, int count, int step, bool ends) {
-    constexpr int V = D / 32, kTogether = 8;
-    // (the drafted tokens are the last contributor's)
-    const bool odd = kOdd && ends && __ldcg(reinterpret_cast<const int*>(slot_of(first_cta + join.count - 1)) + kRowTile * (D + 2)) != 0;
-    for (int r0 = warp; r0 < rows; r0 += 8) {
-      float m[2] = {-INFINITY, -INFINITY}, sum[2] = {}, acc[2][V] = {};
-      const int of[2] = {r0, r0 + 4 < rows ? r0 + 4 : r0};
-      for (int k0 = 0; k0 < count; k0 += 32) {
-        const int here = min(count - k0, 32);
-        float by[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float* from = slot_of(c0 + (k0 + min(lane, here - 1)) * step) + kRowTile * D + of[h];
-          const float cm = lane < here ? __ldcg(from) : -INFINITY, ct = lane < here ? __ldcg(from + kRowTile) : 0.f;
-          float most = cm;
-#pragma unroll
-          for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const float now = fmaxf(m[h], most), base = now == -INFINITY ? 0.f : now, old = exp2_approx(m[h] - base);
-          by[h] = exp2_approx(cm - base);
-          float part = ct * by[h];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-          sum[h] = sum[h] * old + part;
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[h][i] *= old;
-          m[h] = now;
-        }
-        for (int j0 = 0; j0 < here; j0 += kTogether) {
-          float2 v[kTogether][2][V / 2];
-#pragma unroll
-          for (int e = 0; e < kTogether; ++e)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < V / 2; ++i)
-                v[e][h][i] = j0 + e < here ? __ldcg(reinterpret_cast<const float2*>(slot_of(c0 + (k0 + j0 + e) * step) + of[h] * D + lane * V) + i) : make_float2(0.f, 0.f);
-#pragma unroll
-          for (int e = 0; e < kTogether; ++e)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float f = __shfl_sync(0xffffffffu, by[h], (j0 + e) & 31);
-#pragma unroll
-              for (int i = 0; i < V / 2; ++i) {
-                acc[h][2 * i] = fmaf(v[e][h][i].x, f, acc[h][2 * i]);
-                acc[h][2 * i + 1] = fmaf(v[e][h][i].y, f, acc[h][2 * i + 1]);
-              }
-            }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = r0 + 4 * h;
-        if (r >= rows) break;
-        if (ends) {
-          const bool none = mask_of(p, b, (row0 + r) / p.group) == 0 || sum[h] == 0.f;      // padding, and rows that see nothing, are zero
-          const float f = 1.f / sum[h];
-          T* out = out_row<T>(p, b, g, row0 + r) + lane * V;
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[h][i] *= f;
-          if (kOdd && odd) add_odd_values<T>(p, b, g, row0 + r, lane * V, acc[h]);
-#pragma unroll
-          for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(out + i) = none ? 0u : Half16<T>::pack(acc[h][i], acc[h][i + 1]);
-        } else {
-          float* to = slot_of(c0);
-#pragma unroll
-          for (int i = 0; i < V; i += 2) __stcg(reinterpret_cast<float2*>(to + r * D + lane * V + i), make_float2(acc[h][i], acc[h][i + 1]));
-          if (lane == 0) {
-            __stcg(to + kRowTile * D + r, m[h]);
-            __stcg(to + kRowTile * (D + 1) + r, sum[h]);
-          }
-        }
-      }
-    }
-  };
-  // (one loop, so that its code is there once: what runs for the first time takes longer to fetch than to run)
-  const bool grouped = join.step < join.count;
-  bool ends = !grouped;
-#pragma unroll 1
-  while (last_at(ends && grouped ? join.item_counter(p, 0) : join.group_counter(p, 0), (ends && grouped ? join.groups() : join.size) - 1)) {
-    add_up(ends ? first_cta : join.group, ends && grouped ? join.groups() : join.size, ends && grouped ? join.step : 1, ends);
-    if (ends) break;
-    ends = true;
-  }
 }
 
 #endif  // __CUDACC__

@@ -13,8 +13,18 @@
 // Drafted keys and values are 16 bits.  They make a tile of their own behind the cached ones, which is brought into the form of the others when it is worked
 // on: fp16 with a power of two per token (bf16 as the queries, fp16 as it is).
 //
-// Work is cut into equal ranges of (sequence, head of keys, row tile, key tile) units as in tree_attention.cu; tiles have 128 cached tokens, as many bytes as 64 there.
+// Work is cut into equal ranges of (sequence, head of keys, row tile, key tile) units as in tree_attention.cu.
+//
+// Products are transposed, so that a step of mma.sync covers 16 tokens and 8 rows and what is converted to fp16 - sixteen tokens' keys or values, a
+// warp's share of a tile - serves all rows:   S^T (tokens x rows) = K Q^T,   O^T (values x rows) += V^T W^T.   With a thread's four neighbouring E4M3 values as the pairs that
+// the two halves of a step's operand want, queries are permuted alike and nothing is shuffled; values are transposed by ldmatrix in pairs and come apart into even and odd ones.
+// One warp copies (runs of a page by TMA, else sixteen bytes a thread) and works out the tokens' constants, four compute; nothing but a stage's two barriers is between them.
+#include <cuda.h>
+
+#include <type_traits>
+
 #include "device_utils.cuh"
+#include "gemm_params.h"
 #include "host_common.h"
 #include "tree_attention.cuh"
 
@@ -22,18 +32,20 @@ namespace {
 
 using namespace fp6m;
 
-constexpr int kThreads = 128;
-constexpr int kTile = 128, kDrafted = 64;          // cached tokens of a tile; places for drafted ones in theirs
-constexpr int kStages = 3;
-constexpr int kMaxCtas = 512;
+constexpr int kWorkers = 128, kThreads = kWorkers + 64;
+constexpr int kTile = 64, kDrafted = 32;           // cached tokens of a tile; places for drafted ones in theirs
+constexpr int kRowTile = kFewRows;
 constexpr int kLeastUnits = 3, kSlack = 8;
-constexpr int kCounterBytes = kMaxCtas * 2 * 3 * 4;
-constexpr int kPoolFloats = 3 * 16 * 32;           // what the warps that share keys pool at a time
 
-struct Fp8Params {
-  TreeParams tree;
+struct Fp8Params : TreeParams {
+  int grain;                             // tokens of a page that start at a multiple of their number in a tile
   fp6m_cache_scales scales;
 };
+
+// A partial: sums [row][value], maxima, totals.  A CTA has three: of an item that it does not start, of one that it starts, of a group (see join_step).
+template <int D>
+constexpr int slot_floats() { return kRowTile * (D + 2); }
+constexpr int kSlots = 3;
 
 // Tiles of cached tokens, then one of the drafted tokens.
 struct TilesApart {
@@ -41,553 +53,858 @@ struct TilesApart {
 };
 using Ranges = SegmentsOf<TilesApart>;
 
+// NT: groups of eight rows.
+template <int D, int NT>
+struct Cfg {
+  static constexpr int kCtas = 2;                                    // per multiprocessor
+  static constexpr int kTogether = NT <= 2 ? 2 : 1;                  // tiles that a warp works on side by side
+  static constexpr int kTileBytes = kTile * D, kStageBytes = 2 * kTileBytes;     // keys or values of a tile
+  static constexpr int kStages = 5 * 128 / D;
+  static constexpr int kPoolRow = D + 8;                             // floats, so that rows start in different banks
+  static constexpr int kPowers = kStages * kStageBytes;              // uint32_t [stage][keys, values][kTile]: words with a token's exponent
+  static constexpr int kWhere = kPowers + kStages * kTile * 8;       // uint32_t [stage][kTile]: where in these words
+  static constexpr int kPool = kWhere + kStages * kTile * 4;         // float [warp][8][kPoolRow]
+  static constexpr int kStats = kPool + 4 * 8 * kPoolRow * 4;        // float2 [warp][8 NT]: maximum, total
+  static constexpr int kMasks = kStats + 4 * 8 * NT * 8;             // [8 NT]
+  static constexpr int kBars = kMasks + 8 * NT * 8;
+  static constexpr int kPlan = kBars + 2 * kStages * 8;
+  static constexpr int kQueries = (kPlan + (int)sizeof(Plan) + 15) / 16 * 16;      // uint2 [D / 16][NT][32], float [8 NT]; NT = 4 only
+  static constexpr int kBytes = kQueries + (NT == 4 ? D / 16 * NT * 32 * 8 + 8 * NT * 4 : 0) + 1024;
+  static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory");
+};
+
 // two E4M3 values in fp16 (exact)
 __device__ __forceinline__ uint32_t halves_of(uint32_t two) {
   uint32_t h;
   asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(two));
   return h;
 }
+__device__ __forceinline__ uint32_t upper_halves_of(uint32_t two) {
+  uint32_t h;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, hi;\n}\n" : "=r"(h) : "r"(two));
+  return h;
+}
+// an 8 x 8 matrix of 16-bit values, two neighbours of a row a thread: transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t m) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(m));
+  return t;
+}
 // 2^n, -127 <= n <= 128
 __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(n > -127 ? (uint32_t)(n + 127) << 23 : 0x00400000u); }
 // the exponent that brings values of up to `top` below 2^15: fp16 holds them and what is up to 2^29 times smaller
 __device__ __forceinline__ int exponent_for_half(float top) { return top == 0.f ? 0 : max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100); }
 __device__ __forceinline__ float finite_magnitude(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+template <class T>
+__device__ __forceinline__ float largest_of(uint32_t two) { return fmaxf(finite_magnitude(Half16<T>::value((uint16_t)two)), finite_magnitude(Half16<T>::value((uint16_t)(two >> 16)))); }
+template <class T>
+__device__ __forceinline__ uint32_t scaled_halves(uint32_t two, float by) { return Half16<half>::pack(Half16<T>::value((uint16_t)two) * by, Half16<T>::value((uint16_t)(two >> 16)) * by); }
+
+// Where row r of a head of keys goes.
+template <class T>
+__device__ __forceinline__ T* out_row(const TreeParams& p, int b, int g, int r) {
+  const int t = r / p.group, head = g * p.group + (r - t * p.group);
+  return static_cast<T*>(p.a.out) + b * p.a.out_stride[0] + t * p.a.out_stride[1] + head * p.a.out_stride[2];
+}
+// Stores N values of a row's result; padding, and rows that see nothing, are zero.  `odd`: infinities and NaN of drafted values are added for those that see them.
+template <class T, int N>
+__device__ __forceinline__ void put_result(const TreeParams& p, int b, int g, int r, int c, float (&v)[N], float sum, bool odd) {
+  const unsigned long long mask = mask_of(p, b, r / p.group);
+  const bool none = mask == 0 || sum == 0.f;
+  const float f = 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] *= f;
+  if (odd) {
+    for (int j = 0; j < p.a.tokens; ++j) {
+      if (!(mask >> j & 1)) continue;
+      const uint16_t* from = static_cast<const uint16_t*>(p.a.v) + b * p.a.v_stride[0] + j * p.a.v_stride[1] + g * p.a.v_stride[2] + c;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((from[i] & Half16<T>::kExponent) == Half16<T>::kExponent) v[i] += Half16<T>::value(from[i]);
+    }
+  }
+  T* out = out_row<T>(p, b, g, r) + c;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) *reinterpret_cast<uint2*>(out + i) = none ? make_uint2(0u, 0u) : make_uint2(Half16<T>::pack(v[i], v[i + 1]), Half16<T>::pack(v[i + 2], v[i + 3]));
+}
+// Words of a partial: what is not there yet is zero, so a word is stored as its complement (and the NaN that would be zero then as another).
+__device__ __forceinline__ uint32_t word_of(float x) { return __float_as_uint(x) == 0xffffffffu ? ~0x7fffffffu : ~__float_as_uint(x); }
+__device__ __forceinline__ float float_of(uint32_t word) { return __uint_as_float(~word); }
+__device__ __forceinline__ uint32_t load_word(const float* at) {
+  uint32_t v;
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 load_words(const float* at) {
+  uint4 v;
+  asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_word(float* at, uint32_t v) { asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void store_words(float* at, const uint4& v) {
+  asm volatile("st.relaxed.gpu.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// Values c .. c + N - 1 of a row, and by one thread its maximum and total, into a partial.
+template <int D, int N>
+__device__ __forceinline__ void put_partial(float* slot, int r, int c, const float (&v)[N], float most, float sum) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) store_words(slot + r * D + c + i, make_uint4(word_of(v[i]), word_of(v[i + 1]), word_of(v[i + 2]), word_of(v[i + 3])));
+  if (c == 0) {
+    store_word(slot + kRowTile * D + r, word_of(most));
+    store_word(slot + kRowTile * (D + 1) + r, word_of(sum));
+  }
+}
+// How an item's partials become one.  Contributors are the CTAs first .. last; their last one adds all up - or, where they are many, the last of every
+// `step` adds up a group, and the last of all what the groups have made.  It does so when its own range is done, and waits (with a limit) for CTAs of lower numbers only, which
+// were dispatched before it and wait for still lower ones.  A word that has been read is made zero again for the next launch.  No fence and no counter: a fence behind copies
+// in flight takes 2.5 us, and a counter that all contributors add to, with one before and one behind it, took 5 us a partial.
+//
+// Partials whose words are on their way together, and contributors of a group.  Cycles from the end of a range to the end of a join, with 2 / 4 / 6 / 12 together (code that runs once is
+// fetched as it runs, and unrolled code is long): two to three contributors 4280 / 4230 / 4480 / 6630, 25 in one step 23600 / 17500 / 16900 / 18500.
+constexpr int kTogether = 4;
+__device__ __forceinline__ int join_step(int count) {
+  if (count <= kTogether) return count;
+  int step = kTogether;
+  while (step * step < count) ++step;
+  return step;
+}
 
 template <int D>
-__device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 7 : row >> 1 & 3; }      // of 16-byte pieces of rows of D bytes
+__device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 7 : row >> 1 & 3; }      // of 16-byte pieces of rows of D bytes, as TMA's
+__device__ __forceinline__ void lds64(uint32_t (&v)[2], uint32_t addr) { asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory"); }
+__device__ __forceinline__ void lds128(uint32_t* v, uint32_t addr) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory"); }
+// a barrier of the warps that compute; whether any of them says so
+__device__ __forceinline__ bool any_worker(bool mine) {
+  int any;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.or.pred q, 1, %2, p;\nselp.s32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"((int)mine), "n"(kWorkers) : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void workers_sync() { named_bar_sync(1, kWorkers); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+// p.run tokens of a head: value 0, head, slot, page (the first coordinate is 0, so the copy starts on a 16-byte boundary)
+__device__ __forceinline__ void tma_load_run(uint32_t dst, const CUtensorMap* map, int head, int slot, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(0), "r"(head), "r"(slot), "r"(page), "r"(bar) : "memory");
+}
 
-// kRowTile rows, a warp for every 16 of them; the warps that this leaves share the keys of a tile and pool their sums.
-template <class T, int D, int kRowTile>
-__global__ void __launch_bounds__(kThreads, 2) tree_attention_fp8_kernel(const __grid_constant__ Fp8Params params) {
-  constexpr int kRowWarps = kRowTile / 16, kKeyWarps = 4 / kRowWarps;
-  constexpr int kMine = kTile / kKeyWarps, kMyDrafted = kDrafted / kKeyWarps;     // tokens of a tile that a warp works on
-  constexpr int kTileBytes = kTile * D, kStageBytes = 2 * kTileBytes;             // keys or values of a tile
-  constexpr int kChunks = D / 16, kRowsPerPass = kThreads / kChunks;              // 16-byte pieces of a cached row
-  constexpr int kWide = D / 8;                                                    // and of a drafted one
-  constexpr int kSlot = slot_floats<D, kRowTile, true>();
-  constexpr bool kHalf = sizeof(T) == 2 && Half16<T>::kMmaFormat == 0;            // 16-bit operands are fp16 as they come
-  const TreeParams& p = params.tree;
+// ldmatrix of what makes two operands
+__device__ __forceinline__ void ldsm_two(uint32_t (&a)[2], uint32_t (&b)[2], uint32_t addr) {
+  uint32_t r[4];
+  ldsm(r, addr);
+  a[0] = r[0]; a[1] = r[1]; b[0] = r[2]; b[1] = r[3];
+}
+__device__ __forceinline__ void ldsm_t_two(uint32_t (&a)[2], uint32_t (&b)[2], uint32_t addr) {
+  uint32_t r[4];
+  ldsm_t(r, addr);
+  a[0] = r[0]; a[1] = r[1]; b[0] = r[2]; b[1] = r[3];
+}
+// four bytes
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+// (not volatile: to be moved between the steps of other chains)
+__device__ __forceinline__ void mma_halves(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Where the exponents of a token's key and value are in their words (bits), and whether it is seen.
+constexpr uint32_t kUnseen = 1u << 31;
+__device__ __forceinline__ uint32_t where_of(const void* key_power, const void* value_power) {
+  return (uint32_t)(reinterpret_cast<uintptr_t>(key_power) & 3) * 8 | (uint32_t)(reinterpret_cast<uintptr_t>(value_power) & 3) * (8 << 8);
+}
+
+// Of a thread's two tokens: 2^x scale log2(e); y and 2^-y.
+struct Constants {
+  float key_by[2], value_power[2], value_by[2];
+};
+
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp8_kernel(const __grid_constant__ Fp8Params params, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<D, NT>;
+  constexpr int S = C::kStages, kParts = D / 16;                     // 16-byte pieces of a cached row, half of a drafted one's
+  constexpr int kSlot = slot_floats<D>();
+  constexpr bool kHalf = Half16<T>::kMmaFormat == 0;                 // 16-bit operands are fp16 as they come
+  const Fp8Params& p = params;
   const fp6m_tree_attention_args& a = p.a;
   const fp6m_cache_scales& sc = params.scales;
-  extern __shared__ __align__(128) uint8_t smem[];
-  // constants of a tile's tokens: 2^x scale log2(e); y and 2^-y
-  float* key_by = reinterpret_cast<float*>(smem + kStages * kStageBytes);                            // [stage][kTile]
-  float2* value_by = reinterpret_cast<float2*>(key_by + kStages * kTile);
-  float* pool = reinterpret_cast<float*>(value_by + kStages * kTile);
-  float* stats = pool + kPoolFloats;                                                // [warp][2][16]: maxima, totals
-  const uint8_t** places = reinterpret_cast<const uint8_t**>(stats + 4 * 32);      // [2][keys, values][kTile]: where the tokens of a tile are
-  Plan* plan = reinterpret_cast<Plan*>(places + 4 * kTile);
-  int* flags = reinterpret_cast<int*>(plan + 1);                                   // [0] a page did not exist, [1] last to arrive
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t base = smem_u32(smem), full = base + C::kBars, empty = full + 8 * S;
+  uint32_t* powers = reinterpret_cast<uint32_t*>(smem + C::kPowers);
+  uint32_t* where = reinterpret_cast<uint32_t*>(smem + C::kWhere);
+  float* pool = reinterpret_cast<float*>(smem + C::kPool);
+  float2* stats = reinterpret_cast<float2*>(smem + C::kStats);
+  unsigned long long* masks = reinterpret_cast<unsigned long long*>(smem + C::kMasks);
+  Plan* plan = reinterpret_cast<Plan*>(smem + C::kPlan);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row_warp = warp / kKeyWarps, key_warp = warp % kKeyWarps;
-  if (tid == 0) flags[0] = 0;
+  const int tid = threadIdx.x, warp = uniform_warp_index(), lane = tid & 31, cta = blockIdx.x;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full + 8 * s, 128);                                  // the copying lanes, for what they have stored and for their copies
+      mbar_init(empty + 8 * s, 4);                                   // the warps that compute
+    }
+    mbar_fence_init();
+  }
+  if (tid == 32 * 4 && p.run > 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int cta = blockIdx.x;
   if (warp == 0) make_plan<TilesApart>(p, plan, kLeastUnits, kSlack);
   __syncthreads();
   const long long units = plan->units;
   const int ctas = plan->ctas;
   if (cta >= ctas) return;
   Ranges seg(p, *plan);
+  bool dead = false;
 
-  // ---- copies of a tile, a row of keys and one of values per token.  A thread works out where one token's rows are; the others take it from shared memory.
-  const uint32_t smem_base = smem_u32(smem);
-  Ranges ahead = seg;                                                // of the places, which are worked out a tile ahead of the copies
-  int ahead_tile = 0;
-  bool ahead_lives = ahead.next(p);
-  if (ahead_lives) ahead_tile = ahead.t0;
-  auto advance = [&] {
-    if (!ahead_lives || ++ahead_tile < ahead.t1) return;
-    ahead_lives = ahead.next(p);
-    ahead_tile = ahead.t0;
-  };
-  auto ahead_drafted = [&] { return ahead_tile + 1 == ahead.tiles; };
-  // the page of this thread's token, -1 where there is none
-  auto look_up = [&] {
-    const int j = ahead_tile * kTile + tid;
-    return ahead_lives && !ahead_drafted() && j < ahead.length ? a.page_table[ahead.b * a.page_table_stride + (int)((unsigned long long)j * p.page_magic >> p.page_shift)] : -1;
-  };
-  int key_scale = -1, value_scale = -1;                              // exponents + 127 of this thread's token of the tile that is copied next, -1: it is not seen
-  auto put_place = [&](int page, int parity) {
-    if (!ahead_lives) return;
-    const int g = ahead.item / p.parts;
-    const uint8_t *k = nullptr, *v = nullptr;
-    key_scale = value_scale = -1;
-    if (ahead_drafted()) {
-      if (tid < a.tokens) {
-        k = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.k) + ahead.b * a.k_stride[0] + tid * a.k_stride[1] + g * a.k_stride[2]);
-        v = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.v) + ahead.b * a.v_stride[0] + tid * a.v_stride[1] + g * a.v_stride[2]);
-      }
-    } else {
-      const int j = ahead_tile * kTile + tid;
-      if (j < ahead.length) {
-        if ((unsigned)page < (unsigned)a.pages) {
-          const int slot = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
-          k = static_cast<const uint8_t*>(a.k_cache) + page * a.k_cache_stride[0] + slot * a.k_cache_stride[1] + g * a.k_cache_stride[2];
-          v = static_cast<const uint8_t*>(a.v_cache) + page * a.v_cache_stride[0] + slot * a.v_cache_stride[1] + g * a.v_cache_stride[2];
-          key_scale = static_cast<const uint8_t*>(sc.k_scales)[page * sc.k_scales_stride[0] + slot * sc.k_scales_stride[1] + g * sc.k_scales_stride[2]];
-          value_scale = static_cast<const uint8_t*>(sc.v_scales)[page * sc.v_scales_stride[0] + slot * sc.v_scales_stride[1] + g * sc.v_scales_stride[2]];
-        } else {
-          flags[0] = 1;
-        }
-      }
-    }
-    places[parity * 2 * kTile + tid] = k;
-    places[parity * 2 * kTile + kTile + tid] = v;
-  };
-  auto copy = [&](int stage, int parity, bool drafted) {
-    const uint32_t dst = smem_base + stage * kStageBytes;
-    const uint8_t** from = places + parity * 2 * kTile;
-    if (drafted) {
-      const int chunk = tid % kWide;
-      for (int row = tid / kWide; row < a.tokens; row += kThreads / kWide) {
-        const uint32_t to = dst + row * 2 * D + ((chunk ^ (row & 7)) * 16);
-        copy16(to, from[row] + chunk * 16, 16);
-        copy16(to + kTileBytes, from[kTile + row] + chunk * 16, 16);
-      }
-      return;
-    }
-    const int chunk = tid % kChunks;
-#pragma unroll
-    for (int i = 0; i < kTile / kRowsPerPass; ++i) {
-      const int row = tid / kChunks + i * kRowsPerPass;
-      const uint8_t *k = from[row], *v = from[kTile + row];
-      const uint32_t to = dst + row * D + ((chunk ^ swizzle<D>(row)) * 16);
-      copy16(to, k ? k + chunk * 16 : static_cast<const uint8_t*>(a.q), k ? 16 : 0);
-      copy16(to + kTileBytes, v ? v + chunk * 16 : static_cast<const uint8_t*>(a.q), v ? 16 : 0);
-    }
-  };
-  // a token that is not seen: any score becomes minus infinity, a weight of zero
-  auto put_constants = [&](int stage, int k, int v) {
-    key_by[stage * kTile + tid] = k < 0 ? 0.f : power_of_two(k - 127) * p.scale_log2;
-    value_by[stage * kTile + tid] = v < 0 ? make_float2(-INFINITY, 0.f) : make_float2((float)(v - 127), power_of_two(127 - v));
-  };
-  put_place(look_up(), 0);
+  if (warp >= 4) {
+    // ==================================================================== copies: a warp the keys and values, one the powers of two
+    const bool copies = warp == 4;
+    // A granule is p.grain tokens of a page that start at a multiple of their number: those that a TMA copy brings, or fewer.  A warp keeps the pages of 64 granules, two
+    // a lane, and those of the next 64 are on their way.  A token's powers of two, a byte each, come as the words that hold them.
+    const int grain_log2 = __ffs(p.grain) - 1;
+    const int step_slots = kTile % a.page_size;
+    bool missing = false;
+    int stage = 0;
+    uint32_t phase = 1;                                              // of `empty`; the first round of stages is free
 #pragma unroll 1
-  for (int s = 0; s < kStages - 1; ++s) {
-    __syncthreads();
-    const bool live = ahead_lives, drafted = live && ahead_drafted();
-    if (live) copy(s, s & 1, drafted);
-    copies_commit();
-    if (live && !drafted) put_constants(s, key_scale, value_scale);
-    advance();
-    put_place(look_up(), (s + 1) & 1);
+    while (__shfl_sync(0xffffffffu, (int)seg.next(p), 0)) {
+      // What decides about the copies is made uniform to the compiler (read from lane 0): TMA copies with operands that differ between lanes take longer to issue.
+      const int t0 = __shfl_sync(0xffffffffu, seg.t0, 0), t1 = __shfl_sync(0xffffffffu, seg.t1, 0), length = __shfl_sync(0xffffffffu, seg.length, 0);
+      const int g = __shfl_sync(0xffffffffu, seg.item, 0), tiles = __shfl_sync(0xffffffffu, seg.tiles, 0);
+      const int* table = a.page_table + seg.b * a.page_table_stride;
+      const uint8_t *k_powers = static_cast<const uint8_t*>(sc.k_scales) + g * sc.k_scales_stride[2], *v_powers = static_cast<const uint8_t*>(sc.v_scales) + g * sc.v_scales_stride[2];
+      int pages[2], next_pages[2], slot[2];
+      auto look_up = [&](int block, int (&into)[2]) {                // the pages of granules 64 block ..
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const long long j = ((long long)block * 64 + 32 * i + lane) << grain_log2;
+          into[i] = j < length ? table[(int)((unsigned long long)j * p.page_magic >> p.page_shift)] : -1;
+        }
+      };
+      look_up(t0 >> grain_log2, pages);
+      look_up((t0 >> grain_log2) + 1, next_pages);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = t0 * kTile + 32 * i + lane;
+        slot[i] = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
+      }
+#pragma unroll 1
+      for (int tile = t0; tile < t1; ++tile) {
+        const int at_block = tile & (p.grain - 1);                   // tiles of a block: as many as tokens of a granule
+        if (at_block == 0 && tile != t0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) pages[i] = next_pages[i];
+          look_up((tile >> grain_log2) + 1, next_pages);
+        }
+        const bool drafted = tile + 1 == tiles, by_tma = p.run > 0 && (tile + 1) * kTile <= length;
+        const uint32_t keys = base + stage * C::kStageBytes, values = keys + C::kTileBytes, bar = full + 8 * stage;
+        auto page_at = [&](int granule) {                            // of the tile
+          const int in = (at_block << (6 - grain_log2)) + granule, lo = __shfl_sync(0xffffffffu, pages[0], in & 31), hi = __shfl_sync(0xffffffffu, pages[1], in & 31);
+          return in < 32 ? lo : hi;
+        };
+        mbar_wait_bounded<20>(empty + 8 * stage, phase, p.status, dead);
+        if (copies && by_tma) {
+          if (elect_one()) mbar_expect_tx(bar, C::kStageBytes);
+          __syncwarp();
+          const int first_slot = __shfl_sync(0xffffffffu, slot[0], 0);
+          auto bring = [&](auto runs) {
+            constexpr int R = decltype(runs)::value;
+            int page[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const int of = page_at(r);
+              page[r] = (unsigned)of < (unsigned)a.pages ? of : a.pages;       // behind the last page the copy reads zeros
+            }
+            if (elect_one()) {
+              int at = first_slot;
+#pragma unroll
+              for (int r = 0; r < R; ++r) {
+                tma_load_run(keys + r * (kTile / R) * D, &kmap, g, at, page[r], bar);
+                tma_load_run(values + r * (kTile / R) * D, &vmap, g, at, page[r], bar);
+                at += kTile / R;
+                if (at == a.page_size) at = 0;
+              }
+            }
+            __syncwarp();
+          };
+          if (p.run == 64) bring(std::integral_constant<int, 1>());
+          else if (p.run == 32) bring(std::integral_constant<int, 2>());
+          else if (p.run == 16) bring(std::integral_constant<int, 4>());
+          else bring(std::integral_constant<int, 8>());
+        } else if (copies && drafted) {
+          constexpr int kWide = D / 8;
+          const int part = lane % kWide;
+          for (int row = lane / kWide; row < a.tokens; row += 32 / kWide) {
+            const uint32_t to = row * 2 * D + ((part ^ (row & 7)) * 16);
+            copy16(keys + to, static_cast<const T*>(a.k) + seg.b * a.k_stride[0] + row * a.k_stride[1] + g * a.k_stride[2] + part * 8, 16);
+            copy16(values + to, static_cast<const T*>(a.v) + seg.b * a.v_stride[0] + row * a.v_stride[1] + g * a.v_stride[2] + part * 8, 16);
+          }
+        } else if (!drafted) {
+          int page[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            page[i] = page_at((32 * i + lane) >> grain_log2);
+            const bool there = tile * kTile + 32 * i + lane < length;
+            missing = missing || (there && (unsigned)page[i] >= (unsigned)a.pages);
+            if (!there || (unsigned)page[i] >= (unsigned)a.pages) page[i] = -1;
+          }
+          if (!copies) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t at_word = kUnseen;                              // any score becomes minus infinity, a weight of zero
+              if (page[i] >= 0) {
+                auto in = [&](const long long (&stride)[3]) { return (unsigned long long)(unsigned)page[i] * (unsigned)stride[0] + (unsigned long long)(unsigned)slot[i] * (unsigned)stride[1]; };
+                const uint8_t *k = k_powers + in(sc.k_scales_stride), *v = v_powers + in(sc.v_scales_stride);
+                const uint32_t to = base + C::kPowers + (stage * 2 * kTile + 32 * i + lane) * 4;
+                copy4(to, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(k) & ~(uintptr_t)3));
+                copy4(to + kTile * 4, reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(v) & ~(uintptr_t)3));
+                at_word = where_of(k, v);
+              }
+              where[stage * kTile + 32 * i + lane] = at_word;
+            }
+          } else {
+            const uint8_t *k[2], *v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              k[i] = page[i] >= 0 ? static_cast<const uint8_t*>(a.k_cache) + page[i] * a.k_cache_stride[0] + slot[i] * a.k_cache_stride[1] + g * a.k_cache_stride[2] : nullptr;
+              v[i] = page[i] >= 0 ? static_cast<const uint8_t*>(a.v_cache) + page[i] * a.v_cache_stride[0] + slot[i] * a.v_cache_stride[1] + g * a.v_cache_stride[2] : nullptr;
+            }
+            const int part = lane % kParts;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll 4
+              for (int r0 = 0; r0 < 32; r0 += 32 / kParts) {
+                const int in = r0 + lane / kParts, row = 32 * i + in;
+                const uint8_t* from_k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k[i]), in));
+                const uint8_t* from_v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v[i]), in));
+                const uint32_t to = row * D + ((part ^ swizzle<D>(row)) * 16);
+                copy16(keys + to, from_k ? from_k + part * 16 : static_cast<const uint8_t*>(a.q), from_k ? 16 : 0);
+                copy16(values + to, from_v ? from_v + part * 16 : static_cast<const uint8_t*>(a.q), from_v ? 16 : 0);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          slot[i] += step_slots;
+          if (slot[i] >= a.page_size) slot[i] -= a.page_size;
+        }
+        // (the arrival of asynchronous copies does not order a thread's stores, a plain one does)
+        copies_arrive(bar);
+        mbar_arrive(bar);
+        if (++stage == S) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (missing && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
+    return;
   }
 
-  const int quad = lane >> 2, col = lane & 3;                        // this thread's rows quad and quad + 8; tokens 2 col and 2 col + 1 of 8, values 4 col .. 4 col + 3 of 16
-  int stage = 0, turn = (kStages - 1) & 1;                           // turn: of the places
+  // ====================================================================== scores, weights, sums: a warp has sixteen tokens of a tile and all rows
+  const int quad = lane >> 2, col = lane & 3;                        // tokens quad and quad + 8; of eight rows 2 col and 2 col + 1; values 2 quad and 2 quad + 1 of sixteen
+  const int first = warp * 16;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool joins = false, join_odd = false;                              // the item of this CTA's first segment, if it started before
+  int join_b = 0, join_g = 0, join_first = 0, join_last = 0;
 #pragma unroll 1
   while (seg.next(p)) {
-    const int g = seg.item / p.parts, row0 = seg.item % p.parts * kRowTile, rows = min(p.rows - row0, kRowTile);
-    // ---- new rows: queries and masks
-    uint32_t q[D / 16][4];
-    float o[D / 16][2][4], top[2], total[2], row_by[2];              // sums: [16 values][even and odd ones][row, two values]
-    unsigned long long mask[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = row_warp * 16 + quad + 8 * h;
-      mask[h] = 0;
+    const int g = seg.item, rows = p.rows;
+    // ---- queries: fp16, and for bf16 the power of two of each row
+    uint32_t q[NT == 4 ? 1 : kParts][NT == 4 ? 1 : NT][2];
+    float row_by[NT][2];
+    uint2* shared_q = reinterpret_cast<uint2*>(smem + C::kQueries);
+    float* shared_row_by = reinterpret_cast<float*>(smem + C::kQueries + kParts * NT * 32 * 8);
+    auto load_queries = [&](int n, auto&& put) {                     // of rows 8 n .. 8 n + 7: this thread's values of row 8 n + quad
+      const int r = 8 * n + quad;
       const T* src = nullptr;
       if (r < rows) {
-        const int t = (row0 + r) / p.group, head = g * p.group + (row0 + r - t * p.group);
-        mask[h] = mask_of(p, seg.b, t);
+        const int t = r / p.group, head = g * p.group + (r - t * p.group);
         src = static_cast<const T*>(a.q) + seg.b * a.q_stride[0] + t * a.q_stride[1] + head * a.q_stride[2];
       }
+      uint2 four[kParts];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint2 four = src ? *reinterpret_cast<const uint2*>(src + 16 * i + 4 * col) : make_uint2(0u, 0u);
-        q[i][h] = four.x;
-        q[i][2 + h] = four.y;
-      }
-      row_by[h] = 1.f;
+      for (int i = 0; i < kParts; ++i) four[i] = src ? *reinterpret_cast<const uint2*>(src + 16 * i + 4 * col) : make_uint2(0u, 0u);
+      int x = 0;
       if constexpr (!kHalf) {
         float most = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2)
-            most = fmaxf(most, fmaxf(finite_magnitude(Half16<T>::value((uint16_t)q[i][e + h])), finite_magnitude(Half16<T>::value((uint16_t)(q[i][e + h] >> 16)))));
+        for (int i = 0; i < kParts; ++i) most = fmaxf(most, fmaxf(largest_of<T>(four[i].x), largest_of<T>(four[i].y)));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int x = exponent_for_half(most);
+        x = exponent_for_half(most);
         const float down = power_of_two(-x);
-        row_by[h] = power_of_two(x);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2)
-            q[i][e + h] = Half16<half>::pack(Half16<T>::value((uint16_t)q[i][e + h]) * down, Half16<T>::value((uint16_t)(q[i][e + h] >> 16)) * down);
+        for (int i = 0; i < kParts; ++i) four[i] = make_uint2(scaled_halves<T>(four[i].x, down), scaled_halves<T>(four[i].y, down));
       }
-      top[h] = -INFINITY;
-      total[h] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) put(i, four[i]);
+      return power_of_two(x);
+    };
+    if constexpr (NT == 4) {
+      const float by = load_queries(warp, [&](int i, uint2 four) { shared_q[(i * NT + warp) * 32 + lane] = four; });
+      if (col == 0) shared_row_by[8 * warp + quad] = by;
+      workers_sync();
+      if constexpr (!kHalf) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) row_by[n][e] = shared_row_by[8 * n + 2 * col + e];
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float by = load_queries(n, [&](int i, uint2 four) {
+          q[i][n][0] = four.x;
+          q[i][n][1] = four.y;
+        });
+        if constexpr (!kHalf) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) row_by[n][e] = __shfl_sync(0xffffffffu, by, (2 * col + e) * 4);
+        }
+      }
     }
+    float o[kParts][NT][4], top[NT][2], total[NT][2];                // sums: even value of two rows, odd value of two rows
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][0][e] = o[i][1][e] = 0.f;
+      for (int i = 0; i < kParts; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+      top[n][0] = top[n][1] = -INFINITY;
+      total[n][0] = total[n][1] = 0.f;
+    }
     bool odd = false;                                                // infinities or NaN among the drafted values
-#pragma unroll 1
-    for (int tile = seg.t0; tile < seg.t1; ++tile) {
-      copies_wait<kStages - 2>();
-      __syncthreads();
-      const int refilled = (stage + kStages - 1) % kStages;
-      const bool live = ahead_lives, copies_drafted = live && ahead_drafted();
-      if (live) copy(refilled, turn, copies_drafted);
-      copies_commit();
-      const int copied_key_scale = key_scale, copied_value_scale = value_scale;
-      advance();
-      const int page = look_up();
-      turn ^= 1;
-
-      const uint32_t tile_keys = smem_base + stage * kStageBytes, tile_values = tile_keys + kTileBytes;
-      const bool drafted = tile + 1 == seg.tiles;
-      float s[kMine / 8][4];
-      int first = key_warp * kMine, mine = kMine;                    // this warp's tokens of the tile
-      if (drafted) {
-        // ---- drafted tokens: fp16 with a power of two each; of the values the even ones of 16 before the odd ones, which is how E4M3 values come apart below.
-        // Infinities and NaN of values must not meet a weight of zero: they are zero here, and added to the rows that see them at the end.
-        first = key_warp * kMyDrafted;
-        mine = min(max((a.tokens - first + 15) & ~15, 0), kMyDrafted);
-        const int padded = (a.tokens + 15) & ~15;
-        bool mine_odd = false;
-#pragma unroll 1
-        for (int i0 = 0; i0 < 2 * padded * kChunks; i0 += kThreads) {
-          const int i = i0 + tid, row = i / kChunks % padded, part = i % kChunks;
-          const bool is_value = i / kChunks >= padded, there = i < 2 * padded * kChunks && row < a.tokens;
-          const uint32_t at = (is_value ? tile_values : tile_keys) + row * 2 * D;
-          const uint32_t lo = at + (((2 * part) ^ (row & 7)) * 16), hi = at + (((2 * part + 1) ^ (row & 7)) * 16);
-          uint32_t w[8] = {};
-          if (there) {
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(lo) : "memory");
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "r"(hi) : "memory");
-          }
-          if (is_value) {
+    // M tiles' scores of sixteen tokens each -> weights for the second product (fp16), with the running maximum and sum
+    auto weigh = [&](auto tiles, float (&s)[decltype(tiles)::value][NT][4], const Constants (&of)[decltype(tiles)::value], bool drafted, uint32_t (&w)[decltype(tiles)::value][NT][2]) {
+      constexpr int M = decltype(tiles)::value;
+      bool grows = false;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              constexpr uint32_t E = Half16<T>::kExponent;
-              if ((w[e] & E) == E) { w[e] &= 0xffff0000u; mine_odd = true; }
-              if ((w[e] >> 16 & E) == E) { w[e] &= 0xffffu; mine_odd = true; }
-            }
-          }
-          int x = 0;
-          if constexpr (!kHalf) {
-            float most = 0.f;
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fmaxf(finite_magnitude(Half16<T>::value((uint16_t)w[e])), finite_magnitude(Half16<T>::value((uint16_t)(w[e] >> 16)))));
-#pragma unroll
-            for (int d = 1; d < kChunks; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            x = exponent_for_half(most);
-            const float down = power_of_two(-x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = Half16<half>::pack(Half16<T>::value((uint16_t)w[e]) * down, Half16<T>::value((uint16_t)(w[e] >> 16)) * down);
-          }
-          if (i < 2 * padded * kChunks) {
-            if (is_value) {
-              const uint32_t even[4] = {prmt(w[0], w[1], 0x5410), prmt(w[2], w[3], 0x5410), prmt(w[4], w[5], 0x5410), prmt(w[6], w[7], 0x5410)};
-              const uint32_t uneven[4] = {prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x7632), prmt(w[4], w[5], 0x7632), prmt(w[6], w[7], 0x7632)};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) { w[e] = even[e]; w[4 + e] = uneven[e]; }
-              if (part == 0) value_by[stage * kTile + row] = make_float2((float)x, power_of_two(-x));
-            } else if (part == 0) {
-              key_by[stage * kTile + row] = power_of_two(x) * p.scale_log2;
-            }
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(lo), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(hi), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-          }
-        }
-        odd = __syncthreads_or(mine_odd);
-      }
-      const int tokens8 = mine / 8;                                  // (a warp without drafted tokens has nothing to do)
-
-      // ---- scores of this warp's tokens
-      const float* keys_by = key_by + stage * kTile + first;
-      const float2* values_by = value_by + stage * kTile + first;
-#pragma unroll
-      for (int i = 0; i < kMine / 8; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][e] = drafted ? -INFINITY : 0.f;
-      }
-      if (!drafted) {
-#pragma unroll
-        for (int i = 0; i < kMine / 8; ++i) {
-          const int row = first + i * 8 + (lane & 7);
-#pragma unroll
-          for (int d = 0; d < D / 64; ++d) {
-            uint32_t k[4];
-            ldsm(k, tile_keys + row * D + (((d * 4 + (lane >> 3)) ^ swizzle<D>(row)) * 16));
-#pragma unroll
-            for (int c = 0; c < 4; ++c) Mma<half>::run(s[i], q[4 * d + c], halves_of(k[c]), halves_of(k[c] >> 16));
-          }
-          const float2 by = *reinterpret_cast<const float2*>(keys_by + i * 8 + 2 * col);
-          const float4 add = *reinterpret_cast<const float4*>(values_by + i * 8 + 2 * col);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = fmaf(kHalf ? s[i][e] : s[i][e] * row_by[e >> 1], e & 1 ? by.y : by.x, e & 1 ? add.z : add.x);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kMyDrafted / 8; ++i) {
-          if (i >= tokens8) break;
-          const int row = first + i * 8 + quad;
-          float x[4] = {};
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            uint32_t b0, b1;
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(tile_keys + row * 2 * D + (((2 * d + (col >> 1)) ^ (row & 7)) * 16) + (col & 1) * 8) : "memory");
-            Mma<half>::run(x, q[d], b0, b1);
-          }
-          const float2 by = *reinterpret_cast<const float2*>(keys_by + i * 8 + 2 * col);
-          const float4 add = *reinterpret_cast<const float4*>(values_by + i * 8 + 2 * col);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int t = first + i * 8 + 2 * col + (e & 1);
-            const bool sees = t < a.tokens && (mask[e >> 1] >> t & 1);
-            s[i][e] = sees ? fmaf(kHalf ? x[e] : x[e] * row_by[e >> 1], e & 1 ? by.y : by.x, e & 1 ? add.z : add.x) : -INFINITY;
-          }
-        }
-      }
-
-      // ---- running maximum and sum; weights in fp16 for the second product
-      float keep[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float m = top[h];
-#pragma unroll
-        for (int i = 0; i < kMine / 8; ++i) m = fmaxf(m, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float base = m == -INFINITY ? 0.f : m;                   // nothing seen so far
-        keep[h] = exp2_approx(top[h] - base);
-        top[h] = m;
-        total[h] *= keep[h];
-#pragma unroll
-        for (int i = 0; i < kMine / 8; ++i) {
-          if (drafted && i >= tokens8) break;
-          const float4 add = *reinterpret_cast<const float4*>(values_by + i * 8 + 2 * col);
-#pragma unroll
-          for (int e = 2 * h; e < 2 * h + 2; ++e) {
-            s[i][e] = exp2_approx(s[i][e] - base);
-            total[h] = fmaf(s[i][e], e & 1 ? add.w : add.y, total[h]);
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[i][0][e] *= keep[e >> 1];
-          o[i][1][e] *= keep[e >> 1];
-        }
-
-      // ---- weights times values
-#pragma unroll
-      for (int k = 0; k < kMine / 16; ++k) {
-        if (drafted && 2 * k >= tokens8) break;
-        const uint32_t w[4] = {Half16<half>::pack(s[2 * k][0], s[2 * k][1]), Half16<half>::pack(s[2 * k][2], s[2 * k][3]),
-                               Half16<half>::pack(s[2 * k + 1][0], s[2 * k + 1][1]), Half16<half>::pack(s[2 * k + 1][2], s[2 * k + 1][3])};
-        const int row = first + k * 16 + (lane & 15);
-        if (!drafted) {
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t v[4];
-            ldsm_t(v, tile_values + row * D + (((2 * i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              // two tokens' values 2n and 2n + 1 -> the two tokens' values 2n, then those 2n + 1
-              const uint32_t x = prmt(v[2 * c], 0, 0x3120), y = prmt(v[2 * c + 1], 0, 0x3120);
-              Mma<half>::run(o[2 * i + c][0], w, halves_of(x), halves_of(y));
-              Mma<half>::run(o[2 * i + c][1], w, halves_of(x >> 16), halves_of(y >> 16));
+            s[m][n][e] = fmaf(kHalf ? s[m][n][e] : s[m][n][e] * row_by[n][e & 1], of[m].key_by[e >> 1], of[m].value_power[e >> 1]);
+            if (drafted) {
+              const int t = first + quad + (e & 2) * 4;
+              if (t >= a.tokens || !(masks[8 * n + 2 * col + (e & 1)] >> t & 1)) s[m][n][e] = -INFINITY;
             }
+            grows = grows || s[m][n][e] > top[n][e & 1] + kGrowth;
           }
-        } else {
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            uint32_t v[4];
-            ldsm_t(v, tile_values + row * 2 * D + (((2 * i + (lane >> 4)) ^ (row & 7)) * 16));
-            Mma<half>::run(o[i][0], w, v[0], v[1]);
-            Mma<half>::run(o[i][1], w, v[2], v[3]);
+        for (int n = 0; n < NT; ++n) {
+          float keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float now = top[n][e];
+#pragma unroll
+            for (int m = 0; m < M; ++m) now = fmaxf(now, fmaxf(s[m][n][e], s[m][n][2 + e]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
+            keep[e] = exp2_approx(top[n][e] - (now == -INFINITY ? 0.f : now));
+            top[n][e] = now;
+            total[n][e] *= keep[e];
           }
+#pragma unroll
+          for (int i = 0; i < kParts; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][n][e] *= keep[e & 1];
         }
       }
-      stage = (stage + 1) % kStages;
-
-      if (live && !copies_drafted) put_constants(refilled, copied_key_scale, copied_value_scale);
-      put_place(page, turn);
-    }
-
-    // ---- the end of this CTA's keys for these rows
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      total[h] += __shfl_xor_sync(0xffffffffu, total[h], 1);
-      total[h] += __shfl_xor_sync(0xffffffffu, total[h], 2);
-    }
-    // the warps that shared the keys pool their sums, the first one adds them up
-    if ((lane & 3) == 0) {
+      for (int n = 0; n < NT; ++n) {
+        const float below[2] = {top[n][0] == -INFINITY ? 0.f : top[n][0], top[n][1] == -INFINITY ? 0.f : top[n][1]};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        stats[warp * 32 + quad + 8 * h] = top[h];
-        stats[warp * 32 + 16 + quad + 8 * h] = total[h];
-      }
-    }
-    __syncthreads();
+        for (int m = 0; m < M; ++m) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float* of = stats + row_warp * kKeyWarps * 32 + quad + 8 * h;
-      float m = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kKeyWarps; ++w) m = fmaxf(m, of[w * 32]);
-      const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int w = 0; w < kKeyWarps; ++w) sum += of[w * 32 + 16] * exp2_approx(of[w * 32] - base);
-      const float by = exp2_approx(top[h] - base);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int e = 2 * h; e < 2 * h + 2; ++e) {
-          o[i][0][e] *= by;
-          o[i][1][e] *= by;
+          for (int e = 0; e < 4; ++e) {
+            s[m][n][e] = exp2_approx(s[m][n][e] - below[e & 1]);
+            total[n][e & 1] = fmaf(s[m][n][e], of[m].value_by[e >> 1], total[n][e & 1]);
+          }
+          w[m][n][0] = transposed(Half16<half>::pack(s[m][n][0], s[m][n][1]));
+          w[m][n][1] = transposed(Half16<half>::pack(s[m][n][2], s[m][n][3]));
         }
-      top[h] = m;
-      total[h] = sum;
-    }
-    // four neighbouring values of a row
-    auto four_of = [&](int i, int h) { return make_float4(o[i][0][2 * h], o[i][1][2 * h], o[i][0][2 * h + 1], o[i][1][2 * h + 1]); };
-    auto add_four = [&](int i, int h, const float4& x) {
-      o[i][0][2 * h] += x.x;
-      o[i][1][2 * h] += x.y;
-      o[i][0][2 * h + 1] += x.z;
-      o[i][1][2 * h + 1] += x.w;
+      }
     };
-    if (kKeyWarps == 4 && rows <= 4) {
-      // there is room for the rows of all warps at once
-      float4* place = reinterpret_cast<float4*>(pool) + quad * (D / 4) + col;                       // [warp - 1][row][4 values]
-      if (key_warp > 0 && quad < rows) {
+    auto multiply_keys = [&](int i, const uint32_t (&k)[4], float (&into)[NT][4]) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) place[(key_warp - 1) * D + i * 4] = four_of(i, 0);
-      }
-      __syncthreads();
-      if (key_warp == 0 && quad < rows) {
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int w = 0; w < 3; ++w) add_four(i, 0, place[w * D + i * 4]);
-      }
-      __syncthreads();
-    } else {
-      float4* place = reinterpret_cast<float4*>(pool) + (row_warp * (kKeyWarps - 1) * 16 + quad) * 8 + col;      // [row warp][warp - 1][16 rows][8 times 4 values]
-#pragma unroll
-      for (int part = 0; part < D / 32; ++part) {
-        if (key_warp > 0) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) place[((key_warp - 1) * 16 + 8 * h) * 8 + i * 4] = four_of(part * 2 + i, h);
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (NT == 4) {
+          const uint2 b = shared_q[(i * NT + n) * 32 + lane];
+          mma_halves(into[n], k, b.x, b.y);
+        } else {
+          mma_halves(into[n], k, q[i][n][0], q[i][n][1]);
         }
-        __syncthreads();
-        if (key_warp == 0) {
+      }
+    };
+    // M tiles of cached tokens, from the stage on that is next; side by side, so that one chain of latencies serves all
+    auto cached_tiles = [&](auto tiles) {
+      constexpr int M = decltype(tiles)::value;
+      int at[M];
+      at[0] = stage;
+      if constexpr (M == 2) at[1] = stage + 1 == S ? 0 : stage + 1;
+      const int row = first + (lane & 15);
+      float s[M][NT][4] = {};
+      Constants of[M];
+      uint32_t w[M][NT][2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+      for (int m = 0; m < M; ++m) {
+        const uint32_t keys = base + at[m] * C::kStageBytes;
+        uint32_t k[kParts][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < kParts; i += 2) ldsm_two(k[i], k[i + 1], keys + row * D + (((i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
 #pragma unroll
-              for (int w = 0; w < kKeyWarps - 1; ++w) add_four(part * 2 + i, h, place[(w * 16 + 8 * h) * 8 + i * 4]);
+        for (int e = 0; e < 2; ++e) {
+          const int j = first + quad + 8 * e;
+          const uint32_t place = where[at[m] * kTile + j], kw = powers[at[m] * 2 * kTile + j], vw = powers[(at[m] * 2 + 1) * kTile + j];
+          const int x = (int)(kw >> (place & 31) & 255) - 127, y = (int)(vw >> (place >> 8 & 31) & 255) - 127;
+          of[m].key_by[e] = place == kUnseen ? 0.f : power_of_two(x) * p.scale_log2;
+          of[m].value_power[e] = place == kUnseen ? -INFINITY : (float)y;
+          of[m].value_by[e] = place == kUnseen ? 0.f : power_of_two(-y);
         }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          const uint32_t operand[4] = {halves_of(k[i][0]), halves_of(k[i][1]), upper_halves_of(k[i][0]), upper_halves_of(k[i][1])};
+          multiply_keys(i, operand, s[m]);
+        }
+      }
+      weigh(tiles, s, of, false, w);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const uint32_t values = base + at[m] * C::kStageBytes + C::kTileBytes;
+        uint32_t v[kParts][2];
+#pragma unroll
+        for (int i = 0; i < kParts; i += 2) ldsm_t_two(v[i], v[i + 1], values + row * D + (((i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          // two tokens' values 2 n and 2 n + 1 -> the two tokens' values 2 n, then those 2 n + 1
+          const uint32_t x = prmt(v[i][0], 0, 0x3120), y = prmt(v[i][1], 0, 0x3120);
+          const uint32_t operand[4] = {halves_of(x), upper_halves_of(x), halves_of(y), upper_halves_of(y)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_halves(o[i][n], operand, w[m][n][0], w[m][n][1]);
+        }
+      }
+    };
+    // The drafted tokens: fp16 with a power of two each; of the values the even ones of 16 before the odd ones, which is how E4M3 values come apart above.
+    // Infinities and NaN of values must not meet a weight of zero: they are zero here, and added to the rows that see them at the end.
+    auto drafted_tile = [&] {
+      const uint32_t keys = base + stage * C::kStageBytes, values = keys + C::kTileBytes;
+      const int padded = (a.tokens + 15) & ~15;
+      bool mine_odd = false;
+      if (tid < 8 * NT) masks[tid] = tid < rows ? mask_of(p, seg.b, tid / p.group) : 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 2 * padded * kParts; i0 += kWorkers) {
+        const int i = i0 + tid, row = i / kParts % padded, part = i % kParts;
+        const bool is_value = i / kParts >= padded, lives = i < 2 * padded * kParts, there = lives && row < a.tokens;
+        const uint32_t at = (is_value ? values : keys) + row * 2 * D;
+        const uint32_t lo = at + (((2 * part) ^ (row & 7)) * 16), hi = at + (((2 * part + 1) ^ (row & 7)) * 16);
+        uint32_t w[8] = {};
+        if (there) {
+          lds128(w, lo);
+          lds128(w + 4, hi);
+        }
+        if (is_value) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            constexpr uint32_t E = Half16<T>::kExponent;
+            if ((w[e] & E) == E) { w[e] &= 0xffff0000u; mine_odd = true; }
+            if ((w[e] >> 16 & E) == E) { w[e] &= 0xffffu; mine_odd = true; }
+          }
+        }
+        int x = 0;
+        if constexpr (!kHalf) {
+          float most = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most = fmaxf(most, largest_of<T>(w[e]));
+#pragma unroll
+          for (int d = 1; d < kParts; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+          x = exponent_for_half(most);
+          const float down = power_of_two(-x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = scaled_halves<T>(w[e], down);
+        }
+        if (lives) {
+          if (is_value) {
+            const uint32_t even[4] = {prmt(w[0], w[1], 0x5410), prmt(w[2], w[3], 0x5410), prmt(w[4], w[5], 0x5410), prmt(w[6], w[7], 0x5410)};
+            const uint32_t uneven[4] = {prmt(w[0], w[1], 0x7632), prmt(w[2], w[3], 0x7632), prmt(w[4], w[5], 0x7632), prmt(w[6], w[7], 0x7632)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { w[e] = even[e]; w[4 + e] = uneven[e]; }
+          }
+          if (part == 0) powers[(stage * 2 + is_value) * kTile + row] = (uint32_t)x;
+          sts128(lo, w);
+          sts128(hi, w + 4);
+        }
+      }
+      odd = any_worker(mine_odd);
+      if (first >= padded) return;
+      float s[1][NT][4] = {};
+      Constants of[1];
+      uint32_t w[1][NT][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int x = (int)powers[stage * 2 * kTile + first + quad + 8 * e], y = (int)powers[(stage * 2 + 1) * kTile + first + quad + 8 * e];
+        of[0].key_by[e] = power_of_two(x) * p.scale_log2;
+        of[0].value_power[e] = (float)y;
+        of[0].value_by[e] = power_of_two(-y);
+      }
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        uint32_t k0[2], k1[2];                                       // (rows that are eight apart are swizzled alike)
+        const uint32_t at = keys + (first + quad) * 2 * D + (((2 * i + (col >> 1)) ^ (quad & 7)) * 16) + (col & 1) * 8;
+        lds64(k0, at);
+        lds64(k1, at + 8 * 2 * D);
+        const uint32_t operand[4] = {k0[0], k1[0], k0[1], k1[1]};
+        multiply_keys(i, operand, s[0]);
+      }
+      weigh(std::integral_constant<int, 1>(), s, of, true, w);
+      const int row = first + (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        uint32_t wide[4];
+        ldsm_t(wide, values + row * 2 * D + (((2 * i + (lane >> 3 & 1)) ^ (row & 7)) * 16));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_halves(o[i][n], wide, w[0][n][0], w[0][n][1]);
+      }
+    };
+    // waits for the stage that is next, and gives it back
+    auto take = [&](int at) { mbar_wait_bounded<20>(full + 8 * at, at < stage ? phase ^ 1 : phase, p.status, dead); };
+    auto give_back = [&](bool other_copies) {
+      if (other_copies) fence_async_proxy();                         // (what TMA did not bring is overwritten by it perhaps)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + 8 * stage);
+      if (++stage == S) { stage = 0; phase ^= 1; }
+    };
+#pragma unroll 1
+    for (int tile = seg.t0; tile < seg.t1;) {
+      const bool other_copies = p.run == 0 || (tile + C::kTogether) * kTile > seg.length;
+      take(stage);
+      if (C::kTogether == 2 && tile + 1 < min(seg.t1, seg.tiles - 1)) {
+        take(stage + 1 == S ? 0 : stage + 1);
+        cached_tiles(std::integral_constant<int, C::kTogether>());
+        give_back(other_copies);
+        give_back(other_copies);
+        tile += 2;
+      } else {
+        if (tile + 1 == seg.tiles) drafted_tile();
+        else cached_tiles(std::integral_constant<int, 1>());
+        give_back(other_copies);
+        ++tile;
       }
     }
+
+    // ---- the end of this CTA's keys for these rows: the warps pool their sums
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) total[n][e] += __shfl_xor_sync(0xffffffffu, total[n][e], d);
+        if (quad == 0) stats[warp * 8 * NT + 8 * n + 2 * col + e] = make_float2(top[n][e], total[n][e]);
+      }
     const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
-    if (whole) {
-      if (key_warp == 0) {
+    float* slot = p.partials + (size_t)(kSlots * cta + (seg.t0 == 0 ? 1 : 0)) * kSlot;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = row_warp * 16 + quad + 8 * h;
-          if (r < rows) {
-            // padding, and rows that see nothing, are zero
-            const bool none = mask[h] == 0 || total[h] == 0.f;
-            const float f = 1.f / total[h];
-            T* out = out_row<T>(p, seg.b, g, row0 + r) + 4 * col;
+    for (int n = 0; n < NT; ++n) {
+      if (8 * n >= rows) break;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              const float4 x = four_of(i, h);
-              float v[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
-              if (odd) add_odd_values<T>(p, seg.b, g, row0 + r, 16 * i + 4 * col, v);
-              *reinterpret_cast<uint2*>(out + 16 * i) = none ? make_uint2(0u, 0u) : make_uint2(Half16<T>::pack(v[0], v[1]), Half16<T>::pack(v[2], v[3]));
-            }
+      for (int e = 0; e < 2; ++e)
+        if (8 * n + 2 * col + e < rows) {
+          float* to = pool + (warp * 8 + 2 * col + e) * C::kPoolRow + 2 * quad;
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) *reinterpret_cast<float2*>(to + 16 * i) = make_float2(o[i][n][e], o[i][n][2 + e]);
+        }
+      workers_sync();
+      constexpr int V = D / 16;                                      // values of a thread
+      const int in = tid >> 4, r = 8 * n + in, c = (tid & 15) * V;
+      if (r < rows) {
+        float2 of[4];
+        float most = -INFINITY, sum = 0.f, v[V] = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          of[w] = stats[w * 8 * NT + r];
+          most = fmaxf(most, of[w].x);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = exp2_approx(of[w].x - (most == -INFINITY ? 0.f : most));
+          sum = fmaf(of[w].y, f, sum);
+          const float4* from = reinterpret_cast<const float4*>(pool + (w * 8 + in) * C::kPoolRow + c);
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) {
+            const float4 x = from[i];
+            v[4 * i] = fmaf(x.x, f, v[4 * i]);
+            v[4 * i + 1] = fmaf(x.y, f, v[4 * i + 1]);
+            v[4 * i + 2] = fmaf(x.z, f, v[4 * i + 2]);
+            v[4 * i + 3] = fmaf(x.w, f, v[4 * i + 3]);
           }
         }
-      }
-    } else {
-      // a partial: the slot of a range's first rows, or that of its last ones
-      float* slot = p.partials + (size_t)(2 * cta + (seg.t0 == 0 ? 1 : 0)) * kSlot;
-      if (key_warp == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = row_warp * 16 + quad + 8 * h;
-          if (r < rows) {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float4*>(slot + r * D + i * 16 + col * 4) = four_of(i, h);
-            if ((lane & 3) == 0) {
-              slot[kRowTile * D + r] = top[h];
-              slot[kRowTile * (D + 1) + r] = total[h];
-            }
-          }
+        if (whole) {
+          put_result<T>(p, seg.b, g, r, c, v, sum, odd);
+        } else {
+          put_partial<D>(slot, r, c, v, most, sum);
         }
       }
-      if (tid == 0) reinterpret_cast<int*>(slot)[kRowTile * (D + 2)] = odd;
-      const int first_cta = seg.t0 == 0 ? cta : cta_of(units, ctas, seg.unit + p.overhead);
-      const int last_cta = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
-      const Joining join(first_cta, last_cta, cta, few_rows_join_step(last_cta - first_cta + 1));
-      join_rows<T, D, kRowTile, true>(p, seg.b, g, row0, rows, join, cta, flags + 1);
+      workers_sync();
     }
+    if (seg.t0 == 0) continue;
+    joins = true;
+    join_odd = odd;
+    join_b = seg.b;
+    join_g = g;
+    join_first = cta_of(units, ctas, seg.unit + p.overhead);
+    join_last = cta_of(units, ctas, seg.unit + p.overhead + seg.tiles - 1);
   }
-  copies_wait<0>();
-  __syncthreads();
-  if (tid == 0 && flags[0] && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
+
+  if (!joins) return;
+  const int count = join_last - join_first + 1, step = join_step(count), group = (cta - join_first) / step;
+  const bool ends = cta == join_last;
+  if (!ends && (cta - join_first) % step != step - 1) return;
+  // the sums of the groups before (if this is the last CTA), then the partials of this group
+  const int before = ends ? group : 0, members = cta - join_first - group * step + 1;
+  auto source = [&](int k) {
+    if (k < before) return p.partials + (size_t)(kSlots * (join_first + k * step + step - 1) + 2) * kSlot;
+    const int c = join_first + group * step + k - before;
+    return p.partials + (size_t)(kSlots * c + (c == join_first ? 1 : 0)) * kSlot;
+  };
+  constexpr int V = D / 16;                                          // values of a thread
+#pragma unroll 1
+  for (int r0 = 0; r0 < p.rows; r0 += 8) {
+    const int r = r0 + (tid >> 4), c = (tid & 15) * V;
+    float most = -INFINITY, sum = 0.f, v[V] = {};
+#pragma unroll 1
+    for (int k0 = 0; k0 < before + members; k0 += kTogether) {
+      uint4 x[kTogether][V / 4];
+      uint32_t m[kTogether], t[kTogether];
+      bool there = r >= p.rows;
+      for (uint32_t polls = 0; !__all_sync(0xffffffffu, there); ++polls) {
+        if (!there) {
+          there = true;
+#pragma unroll
+          for (int e = 0; e < kTogether; ++e) {
+            const float* from = source(min(k0 + e, before + members - 1));
+            m[e] = load_word(from + kRowTile * D + r);
+            t[e] = load_word(from + kRowTile * (D + 1) + r);
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) x[e][i] = load_words(from + r * D + c + 4 * i);
+          }
+#pragma unroll
+          for (int e = 0; e < kTogether; ++e) {
+            there = there && m[e] && t[e];
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) there = there && x[e][i].x && x[e][i].y && x[e][i].z && x[e][i].w;
+          }
+        }
+        if (dead || polls > 1u << 19) {                              // (a round takes more than a microsecond)
+          if (!dead && p.status) atomicExch(p.status, FP6M_ERR_TIMEOUT);
+          dead = true;
+          break;
+        }
+      }
+      if (r >= p.rows) continue;
+      float now = most;
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e) now = fmaxf(now, float_of(m[e]));
+      const float below = now == -INFINITY ? 0.f : now, keep = exp2_approx(most - below);
+      most = now;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= keep;
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e) {
+        const float f = k0 + e < before + members ? exp2_approx(float_of(m[e]) - below) : 0.f;
+        sum = fmaf(float_of(t[e]), f, sum);
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+          v[4 * i] = fmaf(float_of(x[e][i].x), f, v[4 * i]);
+          v[4 * i + 1] = fmaf(float_of(x[e][i].y), f, v[4 * i + 1]);
+          v[4 * i + 2] = fmaf(float_of(x[e][i].z), f, v[4 * i + 2]);
+          v[4 * i + 3] = fmaf(float_of(x[e][i].w), f, v[4 * i + 3]);
+        }
+        if (k0 + e < before + members) {
+          float* from = source(k0 + e);
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) store_words(from + r * D + c + 4 * i, make_uint4(0, 0, 0, 0));
+          // (the sixteen threads of a row are in one warp, and have all read these)
+          if (c == 0) {
+            store_word(from + kRowTile * D + r, 0);
+            store_word(from + kRowTile * (D + 1) + r, 0);
+          }
+        }
+      }
+    }
+    if (r >= p.rows) continue;
+    if (ends) put_result<T>(p, join_b, join_g, r, c, v, sum, join_odd);
+    else put_partial<D>(p.partials + (size_t)(kSlots * cta + 2) * kSlot, r, c, v, most, sum);
+  }
 }
 
-template <class T, int D, int kRowTile>
-cudaError_t launch_tile(const Fp8Params& p, int ctas, cudaStream_t stream) {
-  constexpr int bytes = kStages * (2 * kTile * D + kTile * 12) + kPoolFloats * 4 + 4 * 32 * 4 + 4 * kTile * 8 + sizeof(Plan) + 16;
-  cudaError_t e = allow_shared_memory<tree_attention_fp8_kernel<T, D, kRowTile>>(bytes);
+int fp8_ctas(int sms, int per_sm) {
+  const int want = sms > 0 ? per_sm * sms : kMaxTreeCtas;
+  return want < kMaxTreeCtas ? want : kMaxTreeCtas;
+}
+
+template <class T, int D, int NT>
+cudaError_t launch_groups(const Fp8Params& p, int sms, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
+  using C = Cfg<D, NT>;
+  cudaError_t e = allow_shared_memory<tree_attention_fp8_kernel<T, D, NT>>(C::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(tree_attention_fp8_kernel<T, D, kRowTile>, dim3(ctas), dim3(kThreads), bytes, stream, p);
+  return launch_overlapped(tree_attention_fp8_kernel<T, D, NT>, dim3(fp8_ctas(sms, C::kCtas)), dim3(kThreads), C::kBytes, stream, p, kmap, vmap);
 }
-template <class T>
-cudaError_t launch_fp8(Fp8Params p, int ctas, cudaStream_t stream) {
-  const bool few = p.tree.rows <= 16;
-  p.tree.row_tiles = p.tree.parts = few ? 1 : (p.tree.rows + 31) / 32;
-  if (p.tree.a.head_dim == 64) return few ? launch_tile<T, 64, 16>(p, ctas, stream) : launch_tile<T, 64, 32>(p, ctas, stream);
-  return few ? launch_tile<T, 128, 16>(p, ctas, stream) : launch_tile<T, 128, 32>(p, ctas, stream);
+template <class T, int D>
+cudaError_t launch_head(const Fp8Params& p, int sms, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
+  return p.rows <= 8 ? launch_groups<T, D, 1>(p, sms, kmap, vmap, stream) : p.rows <= 16 ? launch_groups<T, D, 2>(p, sms, kmap, vmap, stream) : launch_groups<T, D, 4>(p, sms, kmap, vmap, stream);
+}
+cudaError_t launch_fp8(Fp8Params p, int sms, cudaStream_t stream) {
+  const fp6m_tree_attention_args& a = p.a;
+  p.grain = kTile;
+  while (a.page_size % p.grain) p.grain /= 2;
+  // swizzled rows come in eights
+  p.run = p.grain >= 8 ? p.grain : 0;
+  CUtensorMap kmap = {}, vmap = {};
+  if (p.run == 0 || a.max_pages == 0 || encode_cache_map(a.k_cache, 1, a.head_dim, a.kv_heads, a.page_size, a.pages, a.k_cache_stride, p.run, &kmap) != cudaSuccess ||
+      encode_cache_map(a.v_cache, 1, a.head_dim, a.kv_heads, a.page_size, a.pages, a.v_cache_stride, p.run, &vmap) != cudaSuccess)
+    p.run = 0;
+  if (a.type == FP6M_TYPE_F16) return a.head_dim == 64 ? launch_head<half, 64>(p, sms, kmap, vmap, stream) : launch_head<half, 128>(p, sms, kmap, vmap, stream);
+  return a.head_dim == 64 ? launch_head<__nv_bfloat16, 64>(p, sms, kmap, vmap, stream) : launch_head<__nv_bfloat16, 128>(p, sms, kmap, vmap, stream);
 }
 
-int fp8_ctas(int sms) {
-  const int want = sms > 0 ? 2 * sms : kMaxCtas;
-  return want < kMaxCtas ? want : kMaxCtas;
-}
+size_t few_rows_bytes(int sms) { return (size_t)fp8_ctas(sms, Cfg<128, 1>::kCtas) * kSlots * slot_floats<128>() * sizeof(float); }
 
 }  // namespace
 
 extern "C" {
 
-size_t fp6m_tree_attention_fp8_scratch_bytes(int sms) { return kCounterBytes + (size_t)fp8_ctas(sms) * 2 * slot_floats<128, 32, true>() * sizeof(float); }
+// (the two kernels keep apart what they leave there)
+size_t fp6m_tree_attention_fp8_scratch_bytes(int sms) { return few_rows_bytes(sms) + kCounterBytes + tree_tc5_partial_bytes(sms); }
 
 int fp6m_tree_attention_fp8(const fp6m_tree_attention_args* args, const fp6m_cache_scales* scales, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev) {
   if (!args || !scales) return FP6M_ERR_BAD_ARG;
-  Fp8Params p;
-  p.scales = *scales;
   const int rc = check_tree_args(*args, 16, scratch);
   if (rc != FP6M_OK || args->batch == 0 || args->tokens == 0 || args->heads == 0) return rc;
   if (args->max_pages > 0 && (!scales->k_scales || !scales->v_scales)) return FP6M_ERR_BAD_ARG;
   for (int i = 0; i < 3; ++i)
     if (scales->k_scales_stride[i] < 0 || scales->v_scales_stride[i] < 0) return FP6M_ERR_BAD_ARG;
+  for (int i = 0; i < 2; ++i)
+    if (scales->k_scales_stride[i] > 0xffffffffll || scales->v_scales_stride[i] > 0xffffffffll) return FP6M_ERR_PROB_SHAPE;
   DeviceGuard guard(dev);
   const int sms = sm_count(dev);
   if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
   if (scratch_bytes < fp6m_tree_attention_fp8_scratch_bytes(sms)) return FP6M_ERR_SCRATCH;
-  p.tree = tree_params(*args, scratch, kCounterBytes, status_dev);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = args->type == FP6M_TYPE_F16 ? launch_fp8<half>(p, fp8_ctas(sms), st) : launch_fp8<__nv_bfloat16>(p, fp8_ctas(sms), st);
+  cudaError_t e;
+  if (args->tokens * (args->heads / args->kv_heads) > kFewRows) {
+    e = launch_tree_tc5(tree_params(*args, static_cast<unsigned char*>(scratch) + few_rows_bytes(sms), kCounterBytes, status_dev), scales, sms, st);
+  } else {
+    Fp8Params p;
+    static_cast<TreeParams&>(p) = tree_params(*args, scratch, 0, status_dev);
+    p.scales = *scales;
+    e = launch_fp8(p, sms, st);
+  }
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "tree_attention_fp8 launch");
 }
 

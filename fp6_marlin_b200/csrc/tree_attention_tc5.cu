@@ -38,11 +38,11 @@ constexpr int kTreeThreads = 512;        // four warps that copy, one that issue
 // over 4, 19.0 / 15.9; pairs, 16 / 32: one of 64 over 2000, 64 over 8, 38.9 / 47.0.  At least 3 / 6 / 9 units: that one 40.3 / 38.9 / 39.9; one of
 // eight over 8000, 32 over 4, 28.7 / 27.9 / 29.4; four of eight over up to 3000 24.4 / 26.0 / 25.6.
 constexpr int kSlack = 32, kPairSlack = 16, kLeastUnits = 6;
-constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass
 
-template <int D_, bool PAIR_>
+template <int D_, bool PAIR_, bool FP8_ = false>
 struct TreeCfg {
   static constexpr int D = D_;
+  static constexpr bool kFp8 = FP8_;                         // the cache is E4M3 with a power of two for each token and head
   static constexpr bool kPair = PAIR_;                       // two row tiles of an item share its keys, a group each; else the groups share one row tile
   static constexpr int kTileBytes = kKeys * D * 2;           // keys or values of a tile
   static constexpr int kQBytes = kRowTile * D * 2;
@@ -50,11 +50,12 @@ struct TreeCfg {
   static constexpr int kKeyStages = 2 * 128 / D, kValueStages = (kPair ? 2 : 3) * 128 / D;
   static constexpr int kStageBytes = 2 * kTileBytes, kHalfBytes = 2 * kKeys * 128;     // [half of a row][128 keys][64 values]
   static constexpr int kExchange = kRowTile * 32 * 4;        // 32 columns of a group's sums
-  static constexpr int kNumBars = 2 * kKeyStages + 2 * kValueStages + 2 + 2 + 2 + 2;
+  static constexpr int kNumBars = 2 * kKeyStages + 2 * kValueStages + 2 + 2 + 2 + 2 + (kFp8 ? kKeyStages + kValueStages : 0);
   static constexpr int kK = 0, kQ = kKeyStages * kStageBytes, kV = kQ + (kPair ? 2 : 1) * kQBytes, kX = kV + kValueStages * kStageBytes;
   static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
   static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
-  static constexpr int kBars = kPlaces + 4 * kKeys * 8;
+  static constexpr int kPowers = kPlaces + 4 * kKeys * 8;    // [keys, values][64] powers of two of a tile's tokens (kFp8)
+  static constexpr int kBars = kPowers + (kFp8 ? 2 * kKeys * 4 : 0);
   static constexpr int kSmemBytes = kBars + kNumBars * 8 + (4 + 32) * 4 + 1024;
   static constexpr int kSlotFloats = kRowTile * (D + 2) + 4; // a partial: sums [4 columns][row], maxima, totals, whether odd values were met
   static_assert(kSmemBytes <= 232448, "shared memory");
@@ -102,16 +103,33 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) 
                : "memory");
 }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// Two E4M3 values (the lower or the upper ones of four) times a power of two, in 16 bits: exact where the type holds the result.
+template <class T>
+__device__ __forceinline__ uint32_t widened(uint32_t four, bool upper, float by) {
+  uint32_t h;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(upper ? four >> 16 : four));
+  const float2 two = __half22float2(*reinterpret_cast<half2*>(&h));
+  return Half16<T>::pack(two.x * by, two.y * by);
+}
 
-template <class T, class C>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+struct NoScales {};
+
+// Scales: fp6m_cache_scales where the cache is in 8 bits.
+template <class T, class C, class Scales>
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ Scales scales, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   constexpr int D = C::D, SK = C::kKeyStages, SV = C::kValueStages;
   constexpr bool kPair = C::kPair;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t base = smem_u32(smem);
   const uint32_t full_k = base + C::kBars, empty_k = full_k + 8 * SK, full_v = empty_k + 8 * SK, empty_v = full_v + 8 * SV;
-  const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 16, product = weights + 16;
+  const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 16, product = weights + 16, raw_k = product + 16, raw_v = raw_k + 8 * SK;
   volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, [2, 3] last to arrive
   volatile uint32_t* odd_ring = misc + 4;                            // [segment]: infinities or NaN among its drafted values
   __shared__ Plan plan;
@@ -133,6 +151,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       mbar_init(weights + 8 * i, 4);         // [group] its warps have written the weights of a job
       mbar_init(product + 8 * i, 1);         // [group] tcgen05.commit: a segment's last weights are multiplied
     }
+    if constexpr (C::kFp8)
+      for (int i = 0; i < SK + SV; ++i) mbar_init(raw_k + 8 * i, 2);    // the warps that issue a job's copies; its bytes have landed
     mbar_fence_init();
     misc[1] = 0;
   }
@@ -185,6 +205,197 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       };
       int stage = 0, parity = 0, segment = 0;
       uint32_t phase = 1;                                            // of `empty`; the first round of stages is free
+      // the queries of an item come with its first keys
+      auto load_queries = [&] {
+        const int set = segment % q_sets, turn = segment / q_sets;
+        if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
+        constexpr int kTiles = kPair ? 2 : 1;
+        const int first_row = ahead.item % p.parts * kTiles * kRowTile;
+        // (token and head are counted on: with a division for each row 256 of them took 20,000 cycles)
+        const int r0 = first_row + row0, t0_q = r0 / p.group, step_t = kRowsPerPass / p.group, step_h = kRowsPerPass - step_t * p.group;
+        const long long step = step_t * a.q_stride[1] + step_h * a.q_stride[2], wrap = a.q_stride[1] - p.group * a.q_stride[2];
+        int h = r0 - t0_q * p.group;
+        const T* src = static_cast<const T*>(a.q) + ahead.b * a.q_stride[0] + t0_q * a.q_stride[1] + (ahead.item / p.parts * p.group + h) * a.q_stride[2] + chunk * 8;
+        const uint32_t q_to = base + C::kQ + (kPair ? 0 : set) * q_bytes + (chunk >> 3) * (q_rows * 128);
+#pragma unroll 4
+        for (int i = row0; i < kTiles * q_rows; i += kRowsPerPass) {
+          const bool there = first_row + i < p.rows;
+          copy16(q_to + (kPair ? i / kRowTile : 0) * q_bytes + (i & (q_rows - 1)) * 128 + (((chunk & 7) ^ (i & 7)) * 16), there ? src : static_cast<const T*>(a.q), there ? 16 : 0);
+          src += step;
+          h += step_h;
+          if (h >= p.group) {
+            h -= p.group;
+            src += wrap;
+          }
+        }
+      };
+      if constexpr (C::kFp8) {
+        // Cached tiles come as they are, E4M3, into the place of the 16-bit tile that they become; a job later, when they have landed, each thread takes sixteen values of eight tokens,
+        // and when all have, puts them back in 16 bits, times the token's power of two.  So the loads of one job are on their way while the job before is widened.
+        const uint32_t raw = values ? raw_v : raw_k;
+        const void* power_base = values ? scales.v_scales : scales.k_scales;
+        const long long* power_stride = values ? scales.v_scales_stride : scales.k_scales_stride;
+        const long long* cache_stride = values ? a.v_cache_stride : a.k_cache_stride;
+        const uint8_t* cache = static_cast<const uint8_t*>(values ? a.v_cache : a.k_cache);
+        float* powers = reinterpret_cast<float*>(smem + C::kPowers) + (values ? kKeys : 0);
+        constexpr int kNarrow = D / 16, kNarrowRows = 64 / kNarrow;    // 16-byte pieces of a row, rows of a pass
+        const int narrow = me % kNarrow, narrow0 = me / kNarrow;
+        struct Job { int tile, tiles, length, b, g, segment, stage; uint32_t phase; bool other; int power[2]; };      // other: not all of it by TMA
+        // widens a job's tiles
+        auto finish = [&](const Job& job) {
+          mbar_wait_bounded<20>(raw + 8 * job.stage, job.phase, p.status, dead);
+          if (job.other) asm volatile("cp.async.wait_all;" ::: "memory");
+          for (int odd_tile = 0; odd_tile < 2; ++odd_tile) {
+            const uint32_t at = ring + job.stage * C::kStageBytes + odd_tile * (kKeys * 128), bar = full + 8 * job.stage;
+            if (odd_tile < job.tiles) {
+              const int cached = min(job.length - (job.tile + odd_tile) * kKeys, kKeys);
+              // (a power of 16-bit floating point at least: what the type holds)
+              powers[me] = __uint_as_float((uint32_t)max(job.power[odd_tile], 1) << 23);
+              named_bar_sync(bar_id, 64);
+              uint32_t v[kKeys / kNarrowRows][4];
+              float by[kKeys / kNarrowRows];
+#pragma unroll
+              for (int i = 0; i < kKeys / kNarrowRows; ++i) {
+                const int row = narrow0 + i * kNarrowRows;
+                by[i] = powers[row];
+                const uint4 w = lds128(at + row * D + narrow * 16);
+                v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w;
+              }
+              named_bar_sync(bar_id, 64);
+#pragma unroll
+              for (int i = 0; i < kKeys / kNarrowRows; ++i) {
+                const int row = narrow0 + i * kNarrowRows;
+                if (row < cached) {
+                  uint32_t w[8];
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) w[e] = widened<T>(v[i][e / 2], e & 1, by[i]);
+                  const uint32_t to = at + (2 * narrow >> 3) * C::kHalfBytes + row * 128;
+                  sts128(to + (((2 * narrow & 7) ^ (row & 7)) * 16), w);
+                  sts128(to + (((2 * narrow & 7) + 1 ^ (row & 7)) * 16), w + 4);
+                }
+              }
+              if (values && cached < kKeys) {
+                // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
+                // that see them at the end.
+                named_bar_sync(bar_id, 64);
+                bool odd = false;
+                if (me >= cached) {
+                  for (int c = 0; c < D / 8; ++c) {
+                    const uint32_t place = at + (c >> 3) * C::kHalfBytes + me * 128 + (((c & 7) ^ (me & 7)) * 16);
+                    const uint4 w = lds128(place);
+                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                    constexpr uint32_t E = Half16<T>::kExponent;
+                    for (int e = 0; e < 4; ++e) {
+                      if (!is_odd<T>(x[e])) continue;
+                      odd = true;
+                      if ((x[e] & E) == E) x[e] &= 0xffff0000u;
+                      if ((x[e] >> 16 & E) == E) x[e] &= 0xffffu;
+                      sts_u32(place + 4 * e, x[e]);
+                    }
+                  }
+                }
+                if (odd) odd_ring[job.segment % kOddRing] = 1;
+              }
+              // what was stored is seen by the MMAs, and by the copies that come into this place later
+              fence_async_proxy();
+            }
+            mbar_arrive(bar);
+          }
+        };
+        Job before = {};
+        bool pending = false;
+        while (__shfl_sync(0xffffffffu, (int)ahead.next(p), 0)) {
+          const int t0 = __shfl_sync(0xffffffffu, ahead.t0, 0), t1 = __shfl_sync(0xffffffffu, ahead.t1, 0), length = __shfl_sync(0xffffffffu, ahead.length, 0);
+          const int g = __shfl_sync(0xffffffffu, ahead.item / p.parts, 0);
+          const uint8_t* head_powers = static_cast<const uint8_t*>(power_base) + g * power_stride[2];
+          if (values) {
+            if (me == 0) odd_ring[segment % kOddRing] = 0;
+          } else {
+            // (the queries wait for the last scores of the item before, and those for the job that is pending)
+            if (pending && q_sets == 1) {
+              finish(before);
+              pending = false;
+            }
+            load_queries();
+          }
+          int pages = 0, pages_next = 0;
+          if (p.run > 0) {
+            pages = pages_of(t0 >> block_shift);
+            pages_next = pages_of((t0 >> block_shift) + 1);
+          }
+#pragma unroll 1
+          for (int tile = t0; tile < t1; tile += 2) {
+            Job job = {tile, min(t1 - tile, 2), length, ahead.b, g, segment, stage, (phase & 1) ^ 1, (!values && tile == t0), {127, 127}};
+            mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
+            bool missing = false;
+            uint32_t bytes = 0;                                        // that this warp brings by TMA
+#pragma unroll
+            for (int odd_tile = 0; odd_tile < 2; ++odd_tile) {
+              if (odd_tile >= job.tiles) continue;
+              const int at_tile = tile + odd_tile, in_block = at_tile & (block_tiles - 1);
+              const uint32_t dst = ring + stage * C::kStageBytes + odd_tile * (kKeys * 128);
+              if (p.run > 0 && in_block == 0 && at_tile != t0) {
+                pages = pages_next;
+                pages_next = pages_of((at_tile >> block_shift) + 1);
+              }
+              const int j = at_tile * kKeys + me;
+              const int page = p.run > 0 ? __shfl_sync(0xffffffffu, pages, in_block * tile_runs + me / p.run) : j < length ? page_of(p, ahead, j) : -1;
+              const int slot = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
+              const bool known = j < length && (unsigned)page < (unsigned)a.pages;
+              if (known) job.power[odd_tile] = head_powers[page * power_stride[0] + slot * power_stride[1]];
+              missing = missing || (j < length && !known);
+              if (p.run > 0 && (at_tile + 1) * kKeys <= length) {
+                if (second == odd_tile) {
+                  bytes = kKeys * D;
+                  if (elect_one()) mbar_arrive_tx(raw + 8 * stage, bytes);
+                  __syncwarp();
+                  int first_slot = at_tile * kKeys - (int)((unsigned long long)(at_tile * kKeys) * p.page_magic >> p.page_shift) * a.page_size;
+#pragma unroll 1
+                  for (int i = 0; i < tile_runs; ++i) {
+                    int of = __shfl_sync(0xffffffffu, pages, in_block * tile_runs + i);
+                    if ((unsigned)of >= (unsigned)a.pages) of = a.pages;        // behind the last page the copy reads zeros
+                    if (elect_one()) tma_load_run(dst + i * p.run * D, map, 0, g, first_slot, of, raw + 8 * stage);
+                    __syncwarp();
+                    first_slot += p.run;
+                    if (first_slot == a.page_size) first_slot = 0;
+                  }
+                }
+              } else {
+                job.other = true;
+                const uint8_t* place = known ? cache + page * cache_stride[0] + slot * cache_stride[1] + g * cache_stride[2] : nullptr;
+                const uint8_t** narrow_places = reinterpret_cast<const uint8_t**>(places);
+                named_bar_sync(bar_id, 64);                            // (the places of the tile before have been read)
+                narrow_places[me] = place;
+                named_bar_sync(bar_id, 64);
+                const int cached = min(length - at_tile * kKeys, kKeys);
+#pragma unroll 4
+                for (int i = 0; i < kKeys / kNarrowRows; ++i) {
+                  const int row = narrow0 + i * kNarrowRows;
+                  const uint8_t* src = narrow_places[row];
+                  if (row < cached) copy16(dst + row * D + narrow * 16, src ? src + narrow * 16 : static_cast<const uint8_t*>(a.q), src ? 16 : 0);
+                }
+                // drafted tokens as they are; zeros behind them
+                const long long* drafted_stride = values ? a.v_stride : a.k_stride;
+                for (int row = row0; row < kKeys; row += kRowsPerPass) {
+                  const int t = at_tile * kKeys + row - length;
+                  if (t < 0) continue;
+                  const T* src = static_cast<const T*>(values ? a.v : a.k) + ahead.b * drafted_stride[0] + min(t, a.tokens - 1) * drafted_stride[1] + g * drafted_stride[2];
+                  copy16(dst + (chunk >> 3) * C::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src + chunk * 8, t < a.tokens ? 16 : 0);
+                }
+              }
+            }
+            if (bytes == 0 && elect_one()) mbar_arrive(raw + 8 * stage);
+            __syncwarp();
+            if (__any_sync(0xffffffffu, missing)) misc[1] = 1;
+            if (pending) finish(before);
+            before = job;
+            pending = true;
+            if (++stage == stages) { stage = 0; phase ^= 1; }
+          }
+          ++segment;
+        }
+        if (pending) finish(before);
+      } else {
       while (__shfl_sync(0xffffffffu, (int)ahead.next(p), 0)) {
         // What follows from the lengths is made uniform to the compiler (read from lane 0): copies whose operands it takes to differ between
         // lanes cost 150 cycles each to issue.
@@ -193,28 +404,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         if (values) {
           if (me == 0) odd_ring[segment % kOddRing] = 0;
         } else {
-          // the queries of an item come with its first keys
-          const int set = segment % q_sets, turn = segment / q_sets;
-          if (turn > 0) mbar_wait_bounded<50>(q_free + 8 * set, (turn - 1) & 1, p.status, dead);
-          constexpr int kTiles = kPair ? 2 : 1;
-          const int first_row = ahead.item % p.parts * kTiles * kRowTile;
-          // (token and head are counted on: with a division for each row 256 of them took 20,000 cycles)
-          const int r0 = first_row + row0, t0_q = r0 / p.group, step_t = kRowsPerPass / p.group, step_h = kRowsPerPass - step_t * p.group;
-          const long long step = step_t * a.q_stride[1] + step_h * a.q_stride[2], wrap = a.q_stride[1] - p.group * a.q_stride[2];
-          int h = r0 - t0_q * p.group;
-          const T* src = static_cast<const T*>(a.q) + ahead.b * a.q_stride[0] + t0_q * a.q_stride[1] + (g * p.group + h) * a.q_stride[2] + chunk * 8;
-          const uint32_t q_to = base + C::kQ + (kPair ? 0 : set) * q_bytes + (chunk >> 3) * (q_rows * 128);
-#pragma unroll 4
-          for (int i = row0; i < kTiles * q_rows; i += kRowsPerPass) {
-            const bool there = first_row + i < p.rows;
-            copy16(q_to + (kPair ? i / kRowTile : 0) * q_bytes + (i & (q_rows - 1)) * 128 + (((chunk & 7) ^ (i & 7)) * 16), there ? src : static_cast<const T*>(a.q), there ? 16 : 0);
-            src += step;
-            h += step_h;
-            if (h >= p.group) {
-              h -= p.group;
-              src += wrap;
-            }
-          }
+          load_queries();
         }
         int pages = 0, pages_next = 0, slot = 0;
         if (p.run > 0) {
@@ -307,6 +497,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         }
         ++segment;
       }
+      }
     } else if (warp == 4) {
       // ================================================================== MMA issuer
       constexpr uint32_t kFormats = (1u << 4) | (Half16<T>::kMmaFormat << 7) | (Half16<T>::kMmaFormat << 10) | ((uint32_t)(kRowTile >> 4) << 24);
@@ -322,7 +513,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         __device__ __forceinline__ bool next(const TreeParams& p) {
           const bool lives = seg.next(p);
           left = __shfl_sync(0xffffffffu, lives ? seg.t1 - seg.t0 : 0, 0);
-          plain = p.run > 0 ? __shfl_sync(0xffffffffu, min(seg.t1, seg.length / kKeys) - seg.t0, 0) : 0;
+          plain = C::kFp8 ? left : p.run > 0 ? __shfl_sync(0xffffffffu, min(seg.t1, seg.length / kKeys) - seg.t0, 0) : 0;      // (widened tiles are fenced by who stores them)
           // of a pair of row tiles, the second may have no rows
           groups = __shfl_sync(0xffffffffu, kPair && seg.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1, 0);
           return left > 0;
@@ -784,17 +975,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <class T, class C>
-cudaError_t launch_tc5(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
-  cudaError_t e = allow_shared_memory<tree_attention_tc5_kernel<T, C>>(C::kSmemBytes);
+template <class T, class C, class Scales>
+cudaError_t launch_tc5(const TreeParams& p, const Scales& scales, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
+  cudaError_t e = allow_shared_memory<tree_attention_tc5_kernel<T, C, Scales>>(C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(tree_attention_tc5_kernel<T, C>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p, kmap, vmap);
+  return launch_overlapped(tree_attention_tc5_kernel<T, C, Scales>, dim3(ctas), dim3(kTreeThreads), C::kSmemBytes, stream, p, scales, kmap, vmap);
 }
-template <class T>
-cudaError_t launch_typed(const TreeParams& p, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
+template <class T, class Scales>
+cudaError_t launch_typed(const TreeParams& p, const Scales& scales, int ctas, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
+  constexpr bool kFp8 = !std::is_same<Scales, NoScales>::value;
   const bool pair = p.row_tiles > 1;
-  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64, true>>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<64, false>>(p, ctas, kmap, vmap, stream);
-  return pair ? launch_tc5<T, TreeCfg<128, true>>(p, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<128, false>>(p, ctas, kmap, vmap, stream);
+  if (p.a.head_dim == 64) return pair ? launch_tc5<T, TreeCfg<64, true, kFp8>>(p, scales, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<64, false, kFp8>>(p, scales, ctas, kmap, vmap, stream);
+  return pair ? launch_tc5<T, TreeCfg<128, true, kFp8>>(p, scales, ctas, kmap, vmap, stream) : launch_tc5<T, TreeCfg<128, false, kFp8>>(p, scales, ctas, kmap, vmap, stream);
 }
 
 }  // namespace
@@ -802,7 +994,7 @@ cudaError_t launch_typed(const TreeParams& p, int ctas, const CUtensorMap& kmap,
 // (a CTA leaves at most two partials for each of two row tiles)
 size_t tree_tc5_partial_bytes(int sms) { return (size_t)(sms > 0 && sms < kMostTreeCtas ? sms : kMostTreeCtas) * 4 * TreeCfg<128, true>::kSlotFloats * sizeof(float); }
 
-cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream) {
+cudaError_t launch_tree_tc5(TreeParams p, const fp6m_cache_scales* scales, int sms, cudaStream_t stream) {
   p.row_tiles = (p.rows + kRowTile - 1) / kRowTile;
   p.parts = (p.row_tiles + 1) / 2;
   p.overhead = 4;
@@ -812,10 +1004,14 @@ cudaError_t launch_tree_tc5(TreeParams p, int sms, cudaStream_t stream) {
   p.run = kKeys;
   while (a.page_size % p.run) p.run /= 2;
   CUtensorMap kmap = {}, vmap = {};
-  if (p.run < 8 || a.max_pages == 0 || encode_cache_map(a.k_cache, a.head_dim, a.kv_heads, a.page_size, a.pages, a.k_cache_stride, p.run, &kmap) != cudaSuccess ||
-      encode_cache_map(a.v_cache, a.head_dim, a.kv_heads, a.page_size, a.pages, a.v_cache_stride, p.run, &vmap) != cudaSuccess)
-    p.run = 0;
-  return a.type == FP6M_TYPE_F16 ? launch_typed<half>(p, ctas, kmap, vmap, stream) : launch_typed<__nv_bfloat16>(p, ctas, kmap, vmap, stream);
+  auto encode = [&](const void* cache, const long long (&strides)[3], CUtensorMap* map) {
+    return scales ? encode_plain_cache_map(cache, a.head_dim, a.kv_heads, a.page_size, a.pages, strides, p.run, map)
+                  : encode_cache_map(cache, 2, a.head_dim, a.kv_heads, a.page_size, a.pages, strides, p.run, map);
+  };
+  if (p.run < 8 || a.max_pages == 0 || encode(a.k_cache, a.k_cache_stride, &kmap) != cudaSuccess || encode(a.v_cache, a.v_cache_stride, &vmap) != cudaSuccess) p.run = 0;
+  const bool is_half = a.type == FP6M_TYPE_F16;
+  if (scales) return is_half ? launch_typed<half>(p, *scales, ctas, kmap, vmap, stream) : launch_typed<__nv_bfloat16>(p, *scales, ctas, kmap, vmap, stream);
+  return is_half ? launch_typed<half>(p, NoScales(), ctas, kmap, vmap, stream) : launch_typed<__nv_bfloat16>(p, NoScales(), ctas, kmap, vmap, stream);
 }
 
 }  // namespace fp6m

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .api import _device_buffers, _ptr, _status, _stream_handle
+from .api import _call, _device_buffers, _ptr, _status, _stream_handle
 from .block_ops import _TYPES, _buffers_lock, _operator_buffers, _raise, _sms, _strides, _tree_args
 from ._lib import lib
 
@@ -99,6 +99,12 @@ def write_cache_fp8(k, v, k_cache, v_cache, k_scales, v_scales, page_table, leng
     not written and reported by :func:`device_status` (4).  No two entries of a call may go to the same place of a page.
     """
     what = "write_cache_fp8"
+    # plain CUDA tensors that pass every check: one call into native code; anything else takes the general path below
+    rc = _call.write_cache_fp8(k, v, k_cache, v_cache, k_scales, v_scales, page_table, lengths, tokens, counts)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise(what, rc)
     b, t = k.shape[:2] if k.dim() == 4 else (0, 0)
     entries = t
     if tokens is not None:
@@ -115,7 +121,13 @@ def read_cache_fp8(k_cache, v_cache, k_scales, v_scales, page_table, lengths, k,
     value times its head's power of two.  Rows of tokens that the sequence does not have - before 0, from ``lengths[b]`` on - are left as they were, and so
     are those in a page that does not exist, which :func:`device_status` reports (4).  The other arguments as in :func:`write_cache_fp8`.
     """
-    _move("read_cache_fp8", lib.fp6m_read_cache_fp8, k, v, k_cache, v_cache, k_scales, v_scales, page_table, lengths, "rows",
+    what = "read_cache_fp8"
+    rc = _call.read_cache_fp8(k, v, k_cache, v_cache, k_scales, v_scales, page_table, lengths, starts)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise(what, rc)
+    _move(what, lib.fp6m_read_cache_fp8, k, v, k_cache, v_cache, k_scales, v_scales, page_table, lengths, "rows",
           k.shape[1] if k.dim() == 4 else 0, starts=(starts, (k.shape[0],) if k.dim() else ()))
 
 
@@ -127,6 +139,11 @@ def tree_attention_fp8(q, k, v, k_cache, v_cache, k_scales, v_scales, page_table
     fp32.  The weights of the softmax, each times its value's power of two, are rounded once, to fp16, before they meet the values, the result once more.
     """
     what = "tree_attention_fp8"
+    rc = _call.tree_attention_fp8(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale, k_scales, v_scales)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise(what, rc)
     args = _tree_args(what, q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale, torch.float8_e4m3fn)
     device = q.device
     scales = _scales(what, k_scales, v_scales, (*k_cache.shape[:2], k.shape[2]), device)
@@ -159,6 +176,11 @@ def verify_drafts(target, drafted, tree, uniforms, accepted, counts, next_tokens
     Overwritten: accepted (B, T) int32, the accepted tokens' numbers in order, then -1; counts (B,) int32, how many; next_tokens (B,) int64.
     """
     what = "verify_drafts"
+    rc = _call.verify_drafts(target, draft, drafted, tree, uniforms, accepted, counts, next_tokens)
+    if rc == _lib.OK:
+        return
+    if rc > 0:
+        _raise(what, rc)
     if not target.is_cuda:
         raise RuntimeError(f"fp6_marlin_b200.{what} needs CUDA tensors: there is no CPU implementation")
     if target.dtype not in _PROBABILITIES or target.dim() != 3:

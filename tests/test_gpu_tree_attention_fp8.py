@@ -2,7 +2,8 @@
 
 Bounds, with u = 2^-11 (fp16) or 2^-8 (bf16): the result is rounded once (u of itself); the weights, times their values' powers of two, are rounded once to fp16 (w = 2^-11,
 at most w = u where a head of keys has more than 32 rows) before they meet the E4M3 values: w of sum p |v|, and as much again where their sum is taken of the
-unrounded ones.  Weights are relative to the largest of a row, max p_j 2^y_j, and multiples of 2^-24 at least: 2^-25 * max_j (p_j 2^y_j) * sum_j |v_j| 2^-y_j.  Scores are fp32
+unrounded ones.  Weights are relative to the largest of a row, max p_j 2^y_j, and multiples of 2^-24 at least: 2^-25 * max_j (p_j 2^y_j) * sum_j |v_j| 2^-y_j; where a head of keys has
+more than 32 rows the values come times their powers and the weights are p_j alone: in fp16 each is off by up to 2^-25 * max_j p_j, which is 2^-25 * max_j p_j * sum_j |v_j|.  Scores are fp32
 sums of D products, each addition off by at most 2^-23: D * 2^-23 * scale * sum |q k| in the exponent; the exponent, a score in powers of two and y, is rounded twice, and so is the
 maximum that is taken from it: 4 * 2^-24 * (their largest magnitude); all of that twice (weight and total), plus 2^-20 for the exponentials and the running sums.
 """
@@ -38,6 +39,8 @@ def inputs(b, t, h, g, d, lengths, page, dtype=torch.float16, seed=0, spare=2, f
         x[n + "_cache"] = (100 * torch.randn((pages, page, g, d), generator=gen, device="cuda")).clamp(-448, 448).to(torch.float8_e4m3fn)
         power = (-7 + spread * torch.randn((pages, g, page), generator=gen, device="cuda")).round().clamp(-15, 8)
         x[n + "_scales"] = (power + 127).to(torch.uint8).transpose(1, 2)
+        # (as written from fp16: 448 * 2^8 is none of its values)
+        x[n + "_cache"] = x[n + "_cache"].float().clamp(-240, 240).where(x[n + "_scales"][..., None] == 127 + 8, x[n + "_cache"].float()).to(torch.float8_e4m3fn)
     if fill is not None:          # what must not be read: slots behind the last token, pages of nobody
         used = torch.zeros((pages, page), dtype=torch.bool, device="cuda")
         for i, n in enumerate(lengths.tolist()):
@@ -88,7 +91,8 @@ def exact(x, scale=None):
             size = torch.einsum("hn,nhd->hd", p, vs.abs())
             slack = (torch.einsum("hd,nhd->hn", q[i, j].abs(), ks.abs()) * abs(scale)).amax(1, keepdim=True) * d * 2.0 ** -23
             largest = (s.abs() / math.log(2) + torch.log2(ps.T).abs()).amax(1, keepdim=True)
-            least = 2.0 ** -25 * (p * ps.T).amax(1, keepdim=True) * (vs.abs() / ps[..., None]).sum(0)
+            many = t * group > 32
+            least = 2.0 ** -25 * (p if many else p * ps.T).amax(1, keepdim=True) * (vs.abs() / (1 if many else ps[..., None])).sum(0)
             bound[i, j] = u * out[i, j].abs() + (2 * w + 2 * slack + 8 * 2.0 ** -24 * largest + 2.0 ** -20) * size + least + 2.0 ** -25
     return out, bound
 
