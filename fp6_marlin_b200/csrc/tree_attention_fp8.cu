@@ -53,11 +53,12 @@ struct TilesApart {
 };
 using Ranges = SegmentsOf<TilesApart>;
 
-// NT: groups of eight rows.
-template <int D, int NT>
+// NT: groups of eight rows that a warp works on; RW: warps that share the rows of an item (the others share the tokens of a tile).
+template <int D, int NT, int RW>
 struct Cfg {
+  static constexpr int kGroups = NT * RW;
   static constexpr int kCtas = 2;                                    // per multiprocessor
-  static constexpr int kTogether = NT <= 2 ? 2 : 1;                  // tiles that a warp works on side by side
+  static constexpr int kKeyWarps = 4 / RW, kTogether = 2 / RW;       // a warp works on 32 tokens at a time, sixteen of two tiles or 32 of one
   static constexpr int kTileBytes = kTile * D, kStageBytes = 2 * kTileBytes;     // keys or values of a tile
   static constexpr int kStages = 5 * 128 / D;
   static constexpr int kPoolRow = D + 8;                             // floats, so that rows start in different banks
@@ -65,11 +66,14 @@ struct Cfg {
   static constexpr int kWhere = kPowers + kStages * kTile * 8;       // uint32_t [stage][kTile]: where in these words
   static constexpr int kPool = kWhere + kStages * kTile * 4;         // float [warp][8][kPoolRow]
   static constexpr int kStats = kPool + 4 * 8 * kPoolRow * 4;        // float2 [warp][8 NT]: maximum, total
-  static constexpr int kMasks = kStats + 4 * 8 * NT * 8;             // [8 NT]
-  static constexpr int kBars = kMasks + 8 * NT * 8;
+  static constexpr int kMasks = kStats + 4 * 8 * NT * 8;             // [8 kGroups]
+  static constexpr int kBars = kMasks + 8 * kGroups * 8;
   static constexpr int kPlan = kBars + 2 * kStages * 8;
-  static constexpr int kQueries = (kPlan + (int)sizeof(Plan) + 15) / 16 * 16;      // uint2 [D / 16][NT][32], float [8 NT]; NT = 4 only
-  static constexpr int kBytes = kQueries + (NT == 4 ? D / 16 * NT * 32 * 8 + 8 * NT * 4 : 0) + 1024;
+  // Queries: in registers where there is one group, else uint2 [D / 16][kGroups][32] and float [8 kGroups].  (What does not fit the 168 registers of a thread goes through the little that
+  // shared memory leaves of L1: with 100 to 800 bytes of it, steps of 16 and 32 rows took 3900 and 6900 cycles.)
+  static constexpr bool kSharedQueries = NT > 1;
+  static constexpr int kQueries = (kPlan + (int)sizeof(Plan) + 15) / 16 * 16;
+  static constexpr int kBytes = kQueries + (kSharedQueries ? D / 16 * kGroups * 32 * 8 + 8 * kGroups * 4 : 0) + 1024;
   static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory");
 };
 
@@ -108,8 +112,7 @@ __device__ __forceinline__ T* out_row(const TreeParams& p, int b, int g, int r) 
 }
 // Stores N values of a row's result; padding, and rows that see nothing, are zero.  `odd`: infinities and NaN of drafted values are added for those that see them.
 template <class T, int N>
-__device__ __forceinline__ void put_result(const TreeParams& p, int b, int g, int r, int c, float (&v)[N], float sum, bool odd) {
-  const unsigned long long mask = mask_of(p, b, r / p.group);
+__device__ __forceinline__ void put_result(const TreeParams& p, int b, int g, int r, unsigned long long mask, int c, float (&v)[N], float sum, bool odd) {
   const bool none = mask == 0 || sum == 0.f;
   const float f = 1.f / sum;
 #pragma unroll
@@ -219,9 +222,9 @@ struct Constants {
   float key_by[2], value_power[2], value_by[2];
 };
 
-template <class T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp8_kernel(const __grid_constant__ Fp8Params params, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-  using C = Cfg<D, NT>;
+template <class T, int D, int NT, int RW>
+__global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attention_fp8_kernel(const __grid_constant__ Fp8Params params, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<D, NT, RW>;
   constexpr int S = C::kStages, kParts = D / 16;                     // 16-byte pieces of a cached row, half of a drafted one's
   constexpr int kSlot = slot_floats<D>();
   constexpr bool kHalf = Half16<T>::kMmaFormat == 0;                 // 16-bit operands are fp16 as they come
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
 
   // ====================================================================== scores, weights, sums: a warp has sixteen tokens of a tile and all rows
   const int quad = lane >> 2, col = lane & 3;                        // tokens quad and quad + 8; of eight rows 2 col and 2 col + 1; values 2 quad and 2 quad + 1 of sixteen
-  const int first = warp * 16;
+  const int row_warp = warp / C::kKeyWarps, key_warp = warp % C::kKeyWarps, group0 = row_warp * NT;      // this warp's share of the rows and of the tokens, its first group of rows
   int stage = 0;
   uint32_t phase = 0;
   bool joins = false, join_odd = false;                              // the item of this CTA's first segment, if it started before
@@ -414,10 +417,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
   while (seg.next(p)) {
     const int g = seg.item, rows = p.rows;
     // ---- queries: fp16, and for bf16 the power of two of each row
-    uint32_t q[NT == 4 ? 1 : kParts][NT == 4 ? 1 : NT][2];
+    uint32_t q[C::kSharedQueries ? 1 : kParts][2];
     float row_by[NT][2];
     uint2* shared_q = reinterpret_cast<uint2*>(smem + C::kQueries);
-    float* shared_row_by = reinterpret_cast<float*>(smem + C::kQueries + kParts * NT * 32 * 8);
+    float* shared_row_by = reinterpret_cast<float*>(smem + C::kQueries + kParts * C::kGroups * 32 * 8);
     auto load_queries = [&](int n, auto&& put) {                     // of rows 8 n .. 8 n + 7: this thread's values of row 8 n + quad
       const int r = 8 * n + quad;
       const T* src = nullptr;
@@ -444,27 +447,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
       for (int i = 0; i < kParts; ++i) put(i, four[i]);
       return power_of_two(x);
     };
-    if constexpr (NT == 4) {
-      const float by = load_queries(warp, [&](int i, uint2 four) { shared_q[(i * NT + warp) * 32 + lane] = four; });
-      if (col == 0) shared_row_by[8 * warp + quad] = by;
+    if constexpr (C::kSharedQueries) {
+      if (warp < C::kGroups) {
+        const float by = load_queries(warp, [&](int i, uint2 four) { shared_q[(i * C::kGroups + warp) * 32 + lane] = four; });
+        if (col == 0) shared_row_by[8 * warp + quad] = by;
+      }
       workers_sync();
       if constexpr (!kHalf) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) row_by[n][e] = shared_row_by[8 * n + 2 * col + e];
+          for (int e = 0; e < 2; ++e) row_by[n][e] = shared_row_by[8 * (group0 + n) + 2 * col + e];
       }
     } else {
+      const float by = load_queries(0, [&](int i, uint2 four) {
+        q[i][0] = four.x;
+        q[i][1] = four.y;
+      });
+      if constexpr (!kHalf) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float by = load_queries(n, [&](int i, uint2 four) {
-          q[i][n][0] = four.x;
-          q[i][n][1] = four.y;
-        });
-        if constexpr (!kHalf) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) row_by[n][e] = __shfl_sync(0xffffffffu, by, (2 * col + e) * 4);
-        }
+        for (int e = 0; e < 2; ++e) row_by[0][e] = __shfl_sync(0xffffffffu, by, (2 * col + e) * 4);
       }
     }
     float o[kParts][NT][4], top[NT][2], total[NT][2];                // sums: even value of two rows, odd value of two rows
@@ -490,8 +492,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
           for (int e = 0; e < 4; ++e) {
             s[m][n][e] = fmaf(kHalf ? s[m][n][e] : s[m][n][e] * row_by[n][e & 1], of[m].key_by[e >> 1], of[m].value_power[e >> 1]);
             if (drafted) {
-              const int t = first + quad + (e & 2) * 4;
-              if (t >= a.tokens || !(masks[8 * n + 2 * col + (e & 1)] >> t & 1)) s[m][n][e] = -INFINITY;
+              const int t = key_warp * 16 + quad + (e & 2) * 4;
+              if (t >= a.tokens || !(masks[8 * (group0 + n) + 2 * col + (e & 1)] >> t & 1)) s[m][n][e] = -INFINITY;
             }
             grows = grows || s[m][n][e] > top[n][e & 1] + kGrowth;
           }
@@ -531,63 +533,84 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
         }
       }
     };
-    auto multiply_keys = [&](int i, const uint32_t (&k)[4], float (&into)[NT][4]) {
+    auto queries_of = [&](int i, uint32_t (&b)[NT][2]) {              // of sixteen values, all groups
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        if constexpr (NT == 4) {
-          const uint2 b = shared_q[(i * NT + n) * 32 + lane];
-          mma_halves(into[n], k, b.x, b.y);
+        if constexpr (C::kSharedQueries) {
+          const uint2 two = shared_q[(i * C::kGroups + group0 + n) * 32 + lane];
+          b[n][0] = two.x;
+          b[n][1] = two.y;
         } else {
-          mma_halves(into[n], k, q[i][n][0], q[i][n][1]);
+          b[n][0] = q[i][0];
+          b[n][1] = q[i][1];
         }
       }
     };
-    // M tiles of cached tokens, from the stage on that is next; side by side, so that one chain of latencies serves all
-    auto cached_tiles = [&](auto tiles) {
-      constexpr int M = decltype(tiles)::value;
-      int at[M];
+    // Sixteen cached tokens of each of M tiles, or M times sixteen of one, from the stage on that is next; side by side, so that one chain of latencies serves all.
+    auto cached_tiles = [&](auto parts) {
+      constexpr int M = decltype(parts)::value;
+      int at[M], first[M];
       at[0] = stage;
-      if constexpr (M == 2) at[1] = stage + 1 == S ? 0 : stage + 1;
-      const int row = first + (lane & 15);
+      first[0] = key_warp * (RW == 1 ? 16 : 32);
+      if constexpr (M == 2) {
+        at[1] = RW == 2 ? stage : stage + 1 == S ? 0 : stage + 1;
+        first[1] = first[0] + (RW == 1 ? 0 : 16);
+      }
       float s[M][NT][4] = {};
       Constants of[M];
       uint32_t w[M][NT][2];
+      const int in = lane & 15;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
-        const uint32_t keys = base + at[m] * C::kStageBytes;
-        uint32_t k[kParts][2];
-#pragma unroll
-        for (int i = 0; i < kParts; i += 2) ldsm_two(k[i], k[i + 1], keys + row * D + (((i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int j = first + quad + 8 * e;
+          const int j = first[m] + quad + 8 * e;
           const uint32_t place = where[at[m] * kTile + j], kw = powers[at[m] * 2 * kTile + j], vw = powers[(at[m] * 2 + 1) * kTile + j];
           const int x = (int)(kw >> (place & 31) & 255) - 127, y = (int)(vw >> (place >> 8 & 31) & 255) - 127;
           of[m].key_by[e] = place == kUnseen ? 0.f : power_of_two(x) * p.scale_log2;
           of[m].value_power[e] = place == kUnseen ? -INFINITY : (float)y;
           of[m].value_by[e] = place == kUnseen ? 0.f : power_of_two(-y);
         }
+      }
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-          const uint32_t operand[4] = {halves_of(k[i][0]), halves_of(k[i][1]), upper_halves_of(k[i][0]), upper_halves_of(k[i][1])};
-          multiply_keys(i, operand, s[m]);
+      for (int i = 0; i < kParts; i += 2) {
+        uint32_t k[M][2][2];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int row = first[m] + in;
+          ldsm_two(k[m][0], k[m][1], base + at[m] * C::kStageBytes + row * D + (((i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t b[NT][2];
+          queries_of(i + c, b);
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            const uint32_t operand[4] = {halves_of(k[m][c][0]), halves_of(k[m][c][1]), upper_halves_of(k[m][c][0]), upper_halves_of(k[m][c][1])};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_halves(s[m][n], operand, b[n][0], b[n][1]);
+          }
         }
       }
-      weigh(tiles, s, of, false, w);
+      weigh(parts, s, of, false, w);
 #pragma unroll
-      for (int m = 0; m < M; ++m) {
-        const uint32_t values = base + at[m] * C::kStageBytes + C::kTileBytes;
-        uint32_t v[kParts][2];
+      for (int i = 0; i < kParts; i += 2) {
+        uint32_t v[M][2][2];
 #pragma unroll
-        for (int i = 0; i < kParts; i += 2) ldsm_t_two(v[i], v[i + 1], values + row * D + (((i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
-#pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-          // two tokens' values 2 n and 2 n + 1 -> the two tokens' values 2 n, then those 2 n + 1
-          const uint32_t x = prmt(v[i][0], 0, 0x3120), y = prmt(v[i][1], 0, 0x3120);
-          const uint32_t operand[4] = {halves_of(x), upper_halves_of(x), halves_of(y), upper_halves_of(y)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_halves(o[i][n], operand, w[m][n][0], w[m][n][1]);
+        for (int m = 0; m < M; ++m) {
+          const int row = first[m] + in;
+          ldsm_t_two(v[m][0], v[m][1], base + at[m] * C::kStageBytes + C::kTileBytes + row * D + (((i + (lane >> 4)) ^ swizzle<D>(row)) * 16));
         }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            // two tokens' values 2 n and 2 n + 1 -> the two tokens' values 2 n, then those 2 n + 1
+            const uint32_t x = prmt(v[m][c][0], 0, 0x3120), y = prmt(v[m][c][1], 0, 0x3120);
+            const uint32_t operand[4] = {halves_of(x), upper_halves_of(x), halves_of(y), upper_halves_of(y)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_halves(o[i + c][n], operand, w[m][n][0], w[m][n][1]);
+          }
       }
     };
     // The drafted tokens: fp16 with a power of two each; of the values the even ones of 16 before the odd ones, which is how E4M3 values come apart above.
@@ -596,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
       const uint32_t keys = base + stage * C::kStageBytes, values = keys + C::kTileBytes;
       const int padded = (a.tokens + 15) & ~15;
       bool mine_odd = false;
-      if (tid < 8 * NT) masks[tid] = tid < rows ? mask_of(p, seg.b, tid / p.group) : 0;
+      if (tid < 8 * C::kGroups) masks[tid] = tid < rows ? mask_of(p, seg.b, tid / p.group) : 0;
 #pragma unroll 1
       for (int i0 = 0; i0 < 2 * padded * kParts; i0 += kWorkers) {
         const int i = i0 + tid, row = i / kParts % padded, part = i % kParts;
@@ -641,6 +664,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
         }
       }
       odd = any_worker(mine_odd);
+      const int first = key_warp * 16;
       if (first >= padded) return;
       float s[1][NT][4] = {};
       Constants of[1];
@@ -659,7 +683,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
         lds64(k0, at);
         lds64(k1, at + 8 * 2 * D);
         const uint32_t operand[4] = {k0[0], k1[0], k0[1], k1[1]};
-        multiply_keys(i, operand, s[0]);
+        uint32_t b[NT][2];
+        queries_of(i, b);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_halves(s[0][n], operand, b[n][0], b[n][1]);
       }
       weigh(std::integral_constant<int, 1>(), s, of, true, w);
       const int row = first + (lane & 7) + (lane >> 4) * 8;
@@ -685,13 +712,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
       take(stage);
       if (C::kTogether == 2 && tile + 1 < min(seg.t1, seg.tiles - 1)) {
         take(stage + 1 == S ? 0 : stage + 1);
-        cached_tiles(std::integral_constant<int, C::kTogether>());
+        cached_tiles(std::integral_constant<int, 2>());
         give_back(other_copies);
         give_back(other_copies);
         tile += 2;
       } else {
         if (tile + 1 == seg.tiles) drafted_tile();
-        else cached_tiles(std::integral_constant<int, 1>());
+        else cached_tiles(std::integral_constant<int, RW>());
         give_back(other_copies);
         ++tile;
       }
@@ -713,27 +740,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
       if (8 * n >= rows) break;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (8 * n + 2 * col + e < rows) {
+        if (8 * (group0 + n) + 2 * col + e < rows) {
           float* to = pool + (warp * 8 + 2 * col + e) * C::kPoolRow + 2 * quad;
 #pragma unroll
           for (int i = 0; i < kParts; ++i) *reinterpret_cast<float2*>(to + 16 * i) = make_float2(o[i][n][e], o[i][n][2 + e]);
         }
       workers_sync();
       constexpr int V = D / 16;                                      // values of a thread
-      const int in = tid >> 4, r = 8 * n + in, c = (tid & 15) * V;
-      if (r < rows) {
-        float2 of[4];
+      const int in = tid >> 4, c = (tid & 15) * V;
+#pragma unroll
+      for (int rw = 0; rw < RW; ++rw) {
+        const int r = 8 * (rw * NT + n) + in;
+        if (r >= rows) break;
+        float2 of[C::kKeyWarps];
         float most = -INFINITY, sum = 0.f, v[V] = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          of[w] = stats[w * 8 * NT + r];
-          most = fmaxf(most, of[w].x);
+        for (int k = 0; k < C::kKeyWarps; ++k) {
+          of[k] = stats[(rw * C::kKeyWarps + k) * 8 * NT + 8 * n + in];
+          most = fmaxf(most, of[k].x);
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float f = exp2_approx(of[w].x - (most == -INFINITY ? 0.f : most));
-          sum = fmaf(of[w].y, f, sum);
-          const float4* from = reinterpret_cast<const float4*>(pool + (w * 8 + in) * C::kPoolRow + c);
+        for (int k = 0; k < C::kKeyWarps; ++k) {
+          const float f = exp2_approx(of[k].x - (most == -INFINITY ? 0.f : most));
+          sum = fmaf(of[k].y, f, sum);
+          const float4* from = reinterpret_cast<const float4*>(pool + ((rw * C::kKeyWarps + k) * 8 + in) * C::kPoolRow + c);
 #pragma unroll
           for (int i = 0; i < V / 4; ++i) {
             const float4 x = from[i];
@@ -743,11 +773,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
             v[4 * i + 3] = fmaf(x.w, f, v[4 * i + 3]);
           }
         }
-        if (whole) {
-          put_result<T>(p, seg.b, g, r, c, v, sum, odd);
-        } else {
-          put_partial<D>(slot, r, c, v, most, sum);
-        }
+        if (whole) put_result<T>(p, seg.b, g, r, masks[r], c, v, sum, odd);
+        else put_partial<D>(slot, r, c, v, most, sum);
       }
       workers_sync();
     }
@@ -771,75 +798,94 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT>::kCtas) tree_attention_fp
     const int c = join_first + group * step + k - before;
     return p.partials + (size_t)(kSlots * c + (c == join_first ? 1 : 0)) * kSlot;
   };
-  constexpr int V = D / 16;                                          // values of a thread
+  // a thread has a few values of a row, or of two that are eight apart
+  constexpr int V = D / 16, R = C::kGroups > 1 ? 2 : 1, K = kTogether / R;
+  const int c = (tid & 15) * V;
 #pragma unroll 1
-  for (int r0 = 0; r0 < p.rows; r0 += 8) {
-    const int r = r0 + (tid >> 4), c = (tid & 15) * V;
-    float most = -INFINITY, sum = 0.f, v[V] = {};
-#pragma unroll 1
-    for (int k0 = 0; k0 < before + members; k0 += kTogether) {
-      uint4 x[kTogether][V / 4];
-      uint32_t m[kTogether], t[kTogether];
-      bool there = r >= p.rows;
-      for (uint32_t polls = 0; !__all_sync(0xffffffffu, there); ++polls) {
-        if (!there) {
-          there = true;
+  for (int r0 = tid >> 4; r0 < p.rows; r0 += 8 * R) {
+    float most[R], sum[R] = {}, v[R][V] = {};
+    bool lives[R];
+    unsigned long long mask[R] = {};
 #pragma unroll
-          for (int e = 0; e < kTogether; ++e) {
+    for (int i = 0; i < R; ++i) {
+      most[i] = -INFINITY;
+      lives[i] = r0 + 8 * i < p.rows;
+      if (ends && lives[i]) mask[i] = mask_of(p, join_b, (r0 + 8 * i) / p.group);
+    }
+#pragma unroll 1
+    for (int k0 = 0; k0 < before + members; k0 += K) {
+      uint4 x[R][K][V / 4];
+      uint32_t m[R][K], t[R][K];
+      bool there = false;
+      for (uint32_t polls = 0; !there; ++polls) {
+        there = true;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int e = 0; e < K; ++e) {
+            const int r = lives[i] ? r0 + 8 * i : r0;
             const float* from = source(min(k0 + e, before + members - 1));
-            m[e] = load_word(from + kRowTile * D + r);
-            t[e] = load_word(from + kRowTile * (D + 1) + r);
+            m[i][e] = load_word(from + kRowTile * D + r);
+            t[i][e] = load_word(from + kRowTile * (D + 1) + r);
 #pragma unroll
-            for (int i = 0; i < V / 4; ++i) x[e][i] = load_words(from + r * D + c + 4 * i);
+            for (int j = 0; j < V / 4; ++j) x[i][e][j] = load_words(from + r * D + c + 4 * j);
           }
 #pragma unroll
-          for (int e = 0; e < kTogether; ++e) {
-            there = there && m[e] && t[e];
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int i = 0; i < V / 4; ++i) there = there && x[e][i].x && x[e][i].y && x[e][i].z && x[e][i].w;
+          for (int e = 0; e < K; ++e) {
+            there = there && m[i][e] && t[i][e];
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) there = there && x[i][e][j].x && x[i][e][j].y && x[i][e][j].z && x[i][e][j].w;
           }
-        }
         if (dead || polls > 1u << 19) {                              // (a round takes more than a microsecond)
           if (!dead && p.status) atomicExch(p.status, FP6M_ERR_TIMEOUT);
-          dead = true;
-          break;
+          dead = there = true;
         }
       }
-      if (r >= p.rows) continue;
-      float now = most;
+      // the sixteen threads of a row are neighbours in a warp, and have all read it now
+      __syncwarp(0xffffu << (lane & 16));
 #pragma unroll
-      for (int e = 0; e < kTogether; ++e) now = fmaxf(now, float_of(m[e]));
-      const float below = now == -INFINITY ? 0.f : now, keep = exp2_approx(most - below);
-      most = now;
-      sum *= keep;
+      for (int i = 0; i < R; ++i) {
+        float now = most[i];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] *= keep;
+        for (int e = 0; e < K; ++e) now = fmaxf(now, float_of(m[i][e]));
+        const float below = now == -INFINITY ? 0.f : now, keep = exp2_approx(most[i] - below);
+        most[i] = now;
+        sum[i] *= keep;
 #pragma unroll
-      for (int e = 0; e < kTogether; ++e) {
-        const float f = k0 + e < before + members ? exp2_approx(float_of(m[e]) - below) : 0.f;
-        sum = fmaf(float_of(t[e]), f, sum);
+        for (int j = 0; j < V; ++j) v[i][j] *= keep;
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-          v[4 * i] = fmaf(float_of(x[e][i].x), f, v[4 * i]);
-          v[4 * i + 1] = fmaf(float_of(x[e][i].y), f, v[4 * i + 1]);
-          v[4 * i + 2] = fmaf(float_of(x[e][i].z), f, v[4 * i + 2]);
-          v[4 * i + 3] = fmaf(float_of(x[e][i].w), f, v[4 * i + 3]);
-        }
-        if (k0 + e < before + members) {
-          float* from = source(k0 + e);
+        for (int e = 0; e < K; ++e) {
+          const bool counts = k0 + e < before + members;
+          const float f = counts ? exp2_approx(float_of(m[i][e]) - below) : 0.f;
+          sum[i] = fmaf(float_of(t[i][e]), f, sum[i]);
 #pragma unroll
-          for (int i = 0; i < V / 4; ++i) store_words(from + r * D + c + 4 * i, make_uint4(0, 0, 0, 0));
-          // (the sixteen threads of a row are in one warp, and have all read these)
-          if (c == 0) {
-            store_word(from + kRowTile * D + r, 0);
-            store_word(from + kRowTile * (D + 1) + r, 0);
+          for (int j = 0; j < V / 4; ++j) {
+            v[i][4 * j] = fmaf(float_of(x[i][e][j].x), f, v[i][4 * j]);
+            v[i][4 * j + 1] = fmaf(float_of(x[i][e][j].y), f, v[i][4 * j + 1]);
+            v[i][4 * j + 2] = fmaf(float_of(x[i][e][j].z), f, v[i][4 * j + 2]);
+            v[i][4 * j + 3] = fmaf(float_of(x[i][e][j].w), f, v[i][4 * j + 3]);
+          }
+          if (counts && lives[i]) {
+            float* from = source(k0 + e);
+            const int r = r0 + 8 * i;
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) store_words(from + r * D + c + 4 * j, make_uint4(0, 0, 0, 0));
+            if (c == 0) {
+              store_word(from + kRowTile * D + r, 0);
+              store_word(from + kRowTile * (D + 1) + r, 0);
+            }
           }
         }
       }
     }
-    if (r >= p.rows) continue;
-    if (ends) put_result<T>(p, join_b, join_g, r, c, v, sum, join_odd);
-    else put_partial<D>(p.partials + (size_t)(kSlots * cta + 2) * kSlot, r, c, v, most, sum);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (!lives[i]) continue;
+      if (ends) put_result<T>(p, join_b, join_g, r0 + 8 * i, mask[i], c, v[i], sum[i], join_odd);
+      else put_partial<D>(p.partials + (size_t)(kSlots * cta + 2) * kSlot, r0 + 8 * i, c, v[i], most[i], sum[i]);
+    }
   }
 }
 
@@ -848,16 +894,16 @@ int fp8_ctas(int sms, int per_sm) {
   return want < kMaxTreeCtas ? want : kMaxTreeCtas;
 }
 
-template <class T, int D, int NT>
+template <class T, int D, int NT, int RW>
 cudaError_t launch_groups(const Fp8Params& p, int sms, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
-  using C = Cfg<D, NT>;
-  cudaError_t e = allow_shared_memory<tree_attention_fp8_kernel<T, D, NT>>(C::kBytes);
+  using C = Cfg<D, NT, RW>;
+  cudaError_t e = allow_shared_memory<tree_attention_fp8_kernel<T, D, NT, RW>>(C::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(tree_attention_fp8_kernel<T, D, NT>, dim3(fp8_ctas(sms, C::kCtas)), dim3(kThreads), C::kBytes, stream, p, kmap, vmap);
+  return launch_overlapped(tree_attention_fp8_kernel<T, D, NT, RW>, dim3(fp8_ctas(sms, C::kCtas)), dim3(kThreads), C::kBytes, stream, p, kmap, vmap);
 }
 template <class T, int D>
 cudaError_t launch_head(const Fp8Params& p, int sms, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t stream) {
-  return p.rows <= 8 ? launch_groups<T, D, 1>(p, sms, kmap, vmap, stream) : p.rows <= 16 ? launch_groups<T, D, 2>(p, sms, kmap, vmap, stream) : launch_groups<T, D, 4>(p, sms, kmap, vmap, stream);
+  return p.rows <= 8 ? launch_groups<T, D, 1, 1>(p, sms, kmap, vmap, stream) : p.rows <= 16 ? launch_groups<T, D, 2, 1>(p, sms, kmap, vmap, stream) : launch_groups<T, D, 2, 2>(p, sms, kmap, vmap, stream);
 }
 cudaError_t launch_fp8(Fp8Params p, int sms, cudaStream_t stream) {
   const fp6m_tree_attention_args& a = p.a;
@@ -873,7 +919,7 @@ cudaError_t launch_fp8(Fp8Params p, int sms, cudaStream_t stream) {
   return a.head_dim == 64 ? launch_head<__nv_bfloat16, 64>(p, sms, kmap, vmap, stream) : launch_head<__nv_bfloat16, 128>(p, sms, kmap, vmap, stream);
 }
 
-size_t few_rows_bytes(int sms) { return (size_t)fp8_ctas(sms, Cfg<128, 1>::kCtas) * kSlots * slot_floats<128>() * sizeof(float); }
+size_t few_rows_bytes(int sms) { return (size_t)fp8_ctas(sms, Cfg<128, 1, 1>::kCtas) * kSlots * slot_floats<128>() * sizeof(float); }
 
 }  // namespace
 
