@@ -6,16 +6,19 @@
 // However often r is reduced, it stays r = max(alpha p - beta q, 0): max(max(a, 0) / Z - q, 0) = max(a / Z - q, 0) for q >= 0, so a reduction by q changes beta to
 // beta + 1 and the division by its sum Z both to alpha / Z and beta / Z.  Two numbers are all that is kept, and the rows of p and q are read only where a sum is
 // needed: for a second child of a token whose first was not accepted, and for the next token.  Without draft r is alpha p, with zeros at the children that were
-// not accepted.
+// not accepted, and one sum, of p without any of the children, serves all of a token's children: what they have is added to it.
 //
 // Sums are taken in 64 bits: neighbouring sums of a row of 10^5 probabilities lie 10^-5 apart, and sums in 32 bits, off by 10^-7, would choose another token once in a hundred times.
 //
-// A cluster of CTAs a sequence: every warp sums a stretch of the row, the sums are exchanged through distributed shared memory, and every CTA goes the same way
-// through the tree.  What decides about a token - its probabilities in its parent's rows and its random number - is fetched for all tokens at once, before.
+// A cluster of CTAs a sequence: every warp sums a stretch of the row, chunk by chunk, the sums are exchanged through distributed shared memory, every CTA goes the same way
+// through the tree, and in the end one warp looks through the one chunk that the drawn number falls into.  What decides about a token - its probabilities in its parent's rows and
+// its random number - is fetched for all tokens at once, before.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <limits.h>
+
+#include <type_traits>
 
 #include "../../include/fp6m.h"
 #include "device_utils.cuh"
@@ -25,8 +28,8 @@ namespace {
 
 using namespace fp6m;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kMostTokens = 64, kMostCluster = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kCtas = 3;      // per multiprocessor
+constexpr int kMostTokens = 64, kMostCluster = 8, kChunks = 32;       // chunks of a stretch at most
 
 template <class P> struct Probability;
 template <> struct Probability<float> {
@@ -74,7 +77,7 @@ __device__ __forceinline__ double remote_double(uint32_t addr, int rank) {
 // r = max(alpha p - beta q, 0), or alpha p with holes
 template <class P>
 struct Rest {
-  const P *p, *q;                        // q null: no draft
+  const P *p, *q;                        // q null: nothing is subtracted
   double alpha, beta;
   const int* holes;                      // ids whose probability is gone (no draft)
   int hole_count;
@@ -89,64 +92,119 @@ struct Rest {
   }
 };
 
-// Calls take(first id, values[N]) for the warp's lanes with N neighbouring values of r each, from..upto in steps of 32 N.  `from` is a multiple of 32 N from `start`, which is
-// minus the number of values by which the rows lie behind a 16-byte boundary; a step that is not wholly inside the row comes by single values.
+// Calls take(first id, values[N]) for the warp's lanes with N neighbouring values of r each, from..upto in groups of kTogether steps of 32 N.  `from` is a multiple of a group from
+// `start`, which is minus the number of values by which the rows lie behind a 16-byte boundary.  Groups that are wholly inside the row come by vectors, and there only negative values
+// and NaN are looked for: `odd` says that infinities of q were met (those of p show in the sum).  Other groups come by single values.
+constexpr int kTogether = 4;             // steps whose loads are on their way together
 template <class P, class Take>
-__device__ __forceinline__ void for_values(const Rest<P>& r, int vocab, int start, bool vectors, bool any_holes, int from, int upto, Take&& take) {
-  constexpr int N = 16 / sizeof(P), kStep = 32 * N, kTogether = 4;
+__device__ __forceinline__ void for_values(const Rest<P>& r, int vocab, int start, bool vectors, bool any_holes, int from, int upto, bool& odd, Take&& take) {
+  constexpr int N = 16 / sizeof(P), kStep = 32 * N;
   const int lane = threadIdx.x & 31;
-  for (int base = from; base < upto; base += kStep * kTogether) {
+  const double alpha = r.alpha, minus_beta = -r.beta;
+  auto vector_group = [&](int first, auto subtracts) {
+    constexpr bool kSubtracts = decltype(subtracts)::value;
     uint4 pv[kTogether], qv[kTogether];
-    bool whole[kTogether];
 #pragma unroll
     for (int k = 0; k < kTogether; ++k) {
-      const int first = start + base + k * kStep;
-      whole[k] = vectors && base + k * kStep < upto && first >= 0 && first + kStep <= vocab;
-      const uint4 none = make_uint4(0, 0, 0, 0);
-      pv[k] = whole[k] ? __ldg(reinterpret_cast<const uint4*>(r.p + first) + lane) : none;
-      qv[k] = whole[k] && r.q ? __ldg(reinterpret_cast<const uint4*>(r.q + first) + lane) : none;
+      pv[k] = __ldg(reinterpret_cast<const uint4*>(r.p + first + k * kStep) + lane);
+      if (kSubtracts) qv[k] = __ldg(reinterpret_cast<const uint4*>(r.q + first + k * kStep) + lane);
     }
 #pragma unroll
     for (int k = 0; k < kTogether; ++k) {
-      if (base + k * kStep >= upto) return;
-      const int x = start + base + k * kStep + lane * N;
       float pf[N], qf[N];
+      double v[N];
       Probability<P>::unpack(pv[k], pf);
-      Probability<P>::unpack(qv[k], qf);
-      if (!whole[k]) {
+      if (kSubtracts) Probability<P>::unpack(qv[k], qf);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] = alpha * (double)fmaxf(pf[i], 0.f);
+        if (kSubtracts) {
+          const float q = fmaxf(qf[i], 0.f);
+          odd = odd || q == INFINITY;
+          const double x = fma(minus_beta, (double)q, v[i]);
+          v[i] = __double2hiint(x) < 0 ? 0.0 : x;
+        }
+      }
+      const int x = first + k * kStep + lane * N;
+      if (any_holes) {
+        for (int h = 0; h < r.hole_count; ++h) {
+          const int at = r.holes[h] - x;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (at == i) v[i] = 0.0;
+        }
+      }
+      if (!take(x, v)) return false;
+    }
+    return true;
+  };
+#pragma unroll 1
+  for (int base = from; base < upto; base += kStep * kTogether) {
+    const int first = start + base;
+    if (vectors && first >= 0 && first + kStep * kTogether <= vocab) {
+      if (!(r.q ? vector_group(first, std::true_type()) : vector_group(first, std::false_type()))) return;
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < kTogether; ++k) {
+        const int x = first + k * kStep + lane * N;
+        double v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const bool there = x + i >= 0 && x + i < vocab;
-          pf[i] = there ? Probability<P>::value(r.p + x + i) : 0.f;
-          qf[i] = there && r.q ? Probability<P>::value(r.q + x + i) : 0.f;
+          v[i] = there ? r.of(Probability<P>::value(r.p + x + i), r.q ? Probability<P>::value(r.q + x + i) : 0.f) : 0.0;
+          if (any_holes && r.hole(x + i)) v[i] = 0.0;
         }
+        if (!take(x, v)) return;
       }
-      double v[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = r.of(pf[i], qf[i]);
-      if (any_holes) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (r.hole(x + i)) v[i] = 0.0;
-      }
-      if (!take(x, v)) return;
     }
   }
 }
 
+// the sum over the lanes, in all of them
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The first of n numbers with which their sum exceeds the goal, and the sum before it; where none does, the last that is not zero, and minus infinity.  Called by a warp.
+__device__ __forceinline__ int find_first(const double* numbers, int n, double goal, double before, double& sum_before) {
+  const int lane = threadIdx.x & 31;
+  int last = -1;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const double x = i0 + lane < n ? numbers[i0 + lane] : 0.0;
+    double sum = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double other = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += other;
+    }
+    sum += before;
+    const unsigned over = __ballot_sync(0xffffffffu, sum > goal && x > 0.0), some = __ballot_sync(0xffffffffu, x > 0.0);
+    if (over) {
+      sum_before = __shfl_sync(0xffffffffu, sum - x, __ffs(over) - 1);
+      return i0 + __ffs(over) - 1;
+    }
+    if (some) last = i0 + 31 - __clz(some);
+    before = __shfl_sync(0xffffffffu, sum, 31);
+  }
+  sum_before = -INFINITY;
+  return last;
+}
+
 template <class P>
-__global__ void __launch_bounds__(kThreads) verify_drafts_kernel(const __grid_constant__ fp6m_verify_drafts_args a) {
+__global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __grid_constant__ fp6m_verify_drafts_args a) {
   constexpr int N = 16 / sizeof(P), kStep = 32 * N;
   __shared__ double sums[2][kWarps];                                // of the warps' stretches, in turn
+  __shared__ double fine[kWarps][kChunks];                          // of a stretch's chunks
+  __shared__ double every[kMostCluster * kWarps];
   __shared__ float p_of[kMostTokens], q_of[kMostTokens], u_of[kMostTokens];
   __shared__ int parent[kMostTokens], id_of[kMostTokens], holes[kMostTokens];
   __shared__ unsigned long long masks[kMostTokens];
-  __shared__ double every[kMostCluster * kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int rank, ranks;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-  const int b = blockIdx.x / ranks;
+  const int b = blockIdx.x / ranks, workers = ranks * kWarps;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -168,42 +226,61 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(const __grid_co
   __syncthreads();
   const bool alive = masks[0] != 0;                                  // (the same in all CTAs of the cluster)
 
-  Rest<P> r = {target, draft, 1.0, 0.0, holes, 0};
-  int node = 0, count = alive ? 1 : 0, start = 0, stretch = 0, pass = 0;
+  Rest<P> r = {target, nullptr, 1.0, 0.0, holes, 0};
+  int node = 0, count = alive ? 1 : 0, start = 0, stretch = 0, chunk = 0, pass = 0;
   bool vectors = false;
   double whole = 0.0;
-  // The sum of r, and in `every` those of the stretches of all warps of the cluster, in their order.
+  auto has_holes = [&](long long from, long long upto) {
+    bool any = false;
+    for (int i = 0; i < r.hole_count; ++i) any = any || (holes[i] >= start + from && holes[i] < start + upto);
+    return any;
+  };
+  // The sum of r; in `every` those of the stretches of all warps of the cluster, in `fine` those of this warp's chunks, in their order.
   auto add_up = [&] {
     const uintptr_t off = reinterpret_cast<uintptr_t>(r.p) & 15;
     vectors = off % sizeof(P) == 0 && (!r.q || (reinterpret_cast<uintptr_t>(r.q) & 15) == off);
     start = vectors ? -(int)(off / sizeof(P)) : 0;
-    const int steps = (a.vocab - start + kStep - 1) / kStep, workers = ranks * kWarps;
-    stretch = (steps + workers - 1) / workers * kStep;
-    const int me = rank * kWarps + warp;
-    const long long from = (long long)me * stretch;
-    const int end = a.vocab - start;
-    double sum = 0.0;
-    if (from < end) {
-      const int upto = (int)min(from + stretch, (long long)end);
-      bool any_holes = false;
-      for (int i = 0; i < r.hole_count; ++i) any_holes = any_holes || (holes[i] >= start + from && holes[i] < start + upto);
-      for_values(r, a.vocab, start, vectors, any_holes, (int)from, upto, [&](int, double (&v)[N]) {
+    const int end = a.vocab - start, steps = (end + kStep - 1) / kStep;
+    const int groups = ((steps + workers - 1) / workers + kTogether - 1) / kTogether;      // of a stretch
+    stretch = groups * kTogether * kStep;
+    chunk = (groups + kChunks - 1) / kChunks * kTogether * kStep;
+    bool again = false;
+#pragma unroll 1
+    while (true) {
+      const long long from = (long long)(rank * kWarps + warp) * stretch;
+      double sum = 0.0;
+      bool odd = false;
+      if (from < end) {
+        const int upto = (int)min(from + stretch, (long long)end);
+        const bool any_holes = has_holes(from, upto);
+#pragma unroll 1
+        for (int c = 0; from + (long long)c * chunk < upto; ++c) {
+          double part = 0.0;
+          for_values(r, a.vocab, start, vectors, any_holes, (int)from + c * chunk, min((int)min(from + (long long)(c + 1) * chunk, (long long)end), upto), odd, [&](int, double (&v)[N]) {
+            double two[2] = {};
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum += v[i];
-        return true;
-      });
+            for (int i = 0; i < N; ++i) two[i & 1] += v[i];
+            part += two[0] + two[1];
+            return true;
+          });
+          part = warp_sum(part);
+          if (lane == 0) fine[warp][c] = part;
+          sum += part;
+        }
+      }
+      if (__any_sync(0xffffffffu, odd)) sum = __longlong_as_double(0x7ff8000000000000ll);
+      if (lane == 0) sums[pass & 1][warp] = sum;
+      cluster_sync();
+      for (int i = tid; i < workers; i += kThreads) every[i] = remote_double(smem_u32(&sums[pass & 1][i % kWarps]), i / kWarps);
+      ++pass;
+      __syncthreads();
+      whole = 0.0;
+      for (int i = lane; i < workers; i += 32) whole += every[i];
+      whole = warp_sum(whole);
+      if (again || (__double2hiint(whole) & 0x7ff00000) != 0x7ff00000) break;
+      again = true;                                                  // there are infinities: value by value
+      vectors = false;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sums[pass & 1][warp] = sum;
-    cluster_sync();
-    for (int i = tid; i < workers; i += kThreads) every[i] = remote_double(smem_u32(&sums[pass & 1][i % kWarps]), i / kWarps);
-    ++pass;
-    __syncthreads();
-    whole = 0.0;
-    for (int i = lane; i < workers; i += 32) whole += every[i];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, o);
   };
   auto go_to = [&](int n) {
     node = n;
@@ -214,126 +291,131 @@ __global__ void __launch_bounds__(kThreads) verify_drafts_kernel(const __grid_co
     r.hole_count = 0;
   };
 
-  // ---- the way through the tree
-  bool reduced = false, gone = false;                                // r has been reduced since its sum was taken; nothing of it remains
+  // ---- the way through the tree.  (The sums are taken in one place, so that the code is there once.)
+  bool reduced = false, gone = false;      // r has been reduced and not been divided by its sum since; nothing of it remains
+  bool summed = false, last_sum = false;   // `whole` is the sum of r, without draft that of the row without the children; it is that of the row itself
   go_to(0);
-  for (int i = 1; alive && i < a.tokens; ++i) {
-    if (parent[i] != node) continue;
-    if (reduced) {
-      // a further child: r is divided by its sum
-      add_up();
-      gone = !(whole > 0.0);
-      if (!gone) {
-        r.alpha /= whole;
-        r.beta /= whole;
+  int i = 1;
+#pragma unroll 1
+  while (alive) {
+    bool asks = false;                     // a further child asks for the sum
+    for (; i < a.tokens && !last_sum; ++i) {
+      if (parent[i] != node) continue;
+      if (reduced) {
+        if (!summed) {
+          asks = true;
+          break;
+        }
+        double left = whole;
+        if (!draft) {
+          // the children that are still to come, each id once
+          for (int k = i; k < a.tokens; ++k) {
+            if (parent[k] != node || id_of[k] < 0) continue;
+            bool before = false;
+            for (int j = node + 1; j < k; ++j) before = before || (parent[j] == node && id_of[j] == id_of[k]);
+            if (!before) left += (double)p_of[k];
+          }
+        }
+        gone = !(left > 0.0);
+        if (!gone) {
+          r.alpha = draft ? r.alpha / left : 1.0 / left;
+          r.beta /= left;
+        }
+        reduced = false;
+        if (draft) summed = false;
       }
-      reduced = false;
-    }
-    bool is_hole = false;
-    for (int k = 0; k < r.hole_count; ++k) is_hole = is_hole || (holes[k] == id_of[i] && id_of[i] >= 0);
-    const double mine = gone || is_hole ? 0.0 : fmax(fma(-r.beta, (double)q_of[i], r.alpha * (double)p_of[i]), 0.0);
-    const double left = draft ? mine : gone || is_hole ? 0.0 : r.alpha * (double)p_of[i];
-    if ((double)u_of[i] * (double)q_of[i] < left) {
-      if (rank == 0 && tid == 0) a.accepted[(long long)b * a.tokens + count] = i;
-      ++count;
-      go_to(i);
-      gone = false;
-    } else {
-      if (draft) {
-        r.q = draft + node * a.draft_stride[1];
-        r.beta += 1.0;
-      } else if (id_of[i] >= 0 && !is_hole) {
-        __syncthreads();
-        if (tid == 0) holes[r.hole_count] = id_of[i];
-        __syncthreads();
-        ++r.hole_count;
+      bool nothing = gone;
+      if (!draft)                          // an id that was not accepted before has nothing left
+        for (int k = node + 1; k < i; ++k) nothing = nothing || (parent[k] == node && id_of[k] == id_of[i]);
+      const double x = draft ? fma(-r.beta, (double)q_of[i], r.alpha * (double)p_of[i]) : r.alpha * (double)p_of[i];
+      if (!nothing && (double)u_of[i] * (double)q_of[i] < fmax(x, 0.0)) {
+        if (rank == 0 && tid == 0) a.accepted[(long long)b * a.tokens + count] = i;
+        ++count;
+        go_to(i);
+        gone = summed = reduced = false;
+      } else {
+        if (draft) {
+          r.q = draft + node * a.draft_stride[1];
+          r.beta += 1.0;
+        }
+        reduced = !gone;
       }
-      reduced = !gone;
     }
-  }
-
-  // ---- the next token
-  long long next = -1;
-  if (alive) {
-    if (!gone) add_up();
-    if (gone || !(whole > 0.0)) {
-      go_to(node);
-      add_up();
+    // ---- the next token is drawn from r, without draft from the row without the children (none has been accepted); from the row itself if that is nothing
+    if (!asks) {
+      if (summed && (whole > 0.0 || last_sum)) {
+        if (!draft) r.alpha = 1.0;         // as the sums were taken
+        break;
+      }
+      if (summed || (draft && gone)) {
+        go_to(node);
+        last_sum = true;
+      }
     }
+    if (!draft && !last_sum) {
+      __syncthreads();
+      int n = 0;
+      for (int k = node + 1; k < a.tokens; ++k)
+        if (parent[k] == node && id_of[k] >= 0) {
+          if (tid == 0) holes[n] = id_of[k];
+          ++n;
+        }
+      __syncthreads();
+      r.hole_count = n;
+    }
+    const double alpha = r.alpha;
+    if (!draft) r.alpha = 1.0;
+    add_up();
+    if (!draft && asks) r.alpha = alpha;
+    summed = true;
   }
   const bool any = alive && whole > 0.0;
-  int owner = -1;
-  double before = 0.0;
-  const double goal = (double)u_of[0] * whole;
   if (any) {
-    // the first stretch with which the sum exceeds the goal; where rounding leaves none, the last that holds something
-    const int workers = ranks * kWarps;
-    double upto = 0.0;
-    for (int i0 = 0; i0 < workers && owner < 0; i0 += 32) {
-      const double x = i0 + lane < workers ? every[i0 + lane] : 0.0;
-      double sum = x;
+    const double goal = (double)u_of[0] * whole;
+    double before;
+    const int owner = find_first(every, workers, goal, 0.0, before);
+    if (owner == rank * kWarps + warp) {
+      // this warp's stretch; in it the chunk, in that the token
+      __syncwarp();
+      const long long from = (long long)owner * stretch;
+      const int end = a.vocab - start, upto = (int)min(from + stretch, (long long)end), chunks = (int)((upto - from + chunk - 1) / chunk);
+      const int c = find_first(fine[warp], chunks, goal, before, before);
+      const int first = (int)from + c * chunk, behind = (int)min((long long)first + chunk, (long long)upto);
+      double sum = before;
+      int found = -1, last = -1;
+      bool odd = false;
+      for_values(r, a.vocab, start, vectors, has_holes(first, behind), first, behind, odd, [&](int x, double (&v)[N]) {
+        double mine = 0.0;
+        int mine_last = -1;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += other;
-      }
-      sum += upto;
-      const unsigned over = __ballot_sync(0xffffffffu, sum > goal && x > 0.0);
-      if (over) {
-        owner = i0 + __ffs(over) - 1;
-        before = __shfl_sync(0xffffffffu, sum - x, __ffs(over) - 1);
-      }
-      upto = __shfl_sync(0xffffffffu, sum, 31);
+        for (int i = 0; i < N; ++i) {
+          mine += v[i];
+          if (v[i] > 0.0) mine_last = x + i;
+        }
+        double incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double other = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += other;
+        }
+        int here = -1;
+        double at = sum + (incl - mine);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          at += v[i];
+          if (here < 0 && v[i] > 0.0 && at > goal) here = x + i;
+        }
+        const unsigned over = __ballot_sync(0xffffffffu, here >= 0), some = __ballot_sync(0xffffffffu, mine_last >= 0);
+        if (some) last = __shfl_sync(0xffffffffu, mine_last, 31 - __clz(some));
+        if (over) {
+          found = __shfl_sync(0xffffffffu, here, __ffs(over) - 1);
+          return false;
+        }
+        sum += __shfl_sync(0xffffffffu, incl, 31);
+        return true;
+      });
+      if (lane == 0) a.next_tokens[b] = found >= 0 ? found : last;
     }
-    if (owner < 0) {
-      for (int i0 = 0; i0 < workers; i0 += 32) {
-        const unsigned some = __ballot_sync(0xffffffffu, i0 + lane < workers && every[i0 + lane] > 0.0);
-        if (some) owner = i0 + 31 - __clz(some);
-      }
-      before = -INFINITY;                                            // no sum exceeds the goal
-    }
-  }
-  if (any && owner == rank * kWarps + warp) {
-    const long long from = (long long)owner * stretch;
-    const int end = a.vocab - start, upto = (int)min(from + stretch, (long long)end);
-    bool any_holes = false;
-    for (int i = 0; i < r.hole_count; ++i) any_holes = any_holes || (holes[i] >= start + from && holes[i] < start + upto);
-    double sum = before;
-    int found = -1, last = -1;
-    for_values(r, a.vocab, start, vectors, any_holes, (int)from, upto, [&](int x, double (&v)[N]) {
-      double mine = 0.0;
-      int mine_last = -1;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        mine += v[i];
-        if (v[i] > 0.0) mine_last = x + i;
-      }
-      double incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += other;
-      }
-      const double below = sum + (incl - mine);
-      int here = -1;
-      double at = below;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        at += v[i];
-        if (here < 0 && v[i] > 0.0 && at > goal) here = x + i;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, here >= 0);
-      const unsigned some = __ballot_sync(0xffffffffu, mine_last >= 0);
-      if (some) last = __shfl_sync(0xffffffffu, mine_last, 31 - __clz(some));
-      if (over) {
-        found = __shfl_sync(0xffffffffu, here, __ffs(over) - 1);
-        return false;
-      }
-      sum += __shfl_sync(0xffffffffu, incl, 31);
-      return true;
-    });
-    next = found >= 0 ? found : last;
-    if (lane == 0) a.next_tokens[b] = next;
   }
   if (rank == 0) {
     if (tid == 0) {
@@ -378,7 +460,11 @@ extern "C" int fp6m_verify_drafts(const fp6m_verify_drafts_args* args, int dev, 
   for (int i = 0; i < 2; ++i)
     if (a.target_stride[i] < 0 || (a.draft && a.draft_stride[i] < 0)) return FP6M_ERR_BAD_ARG;
   DeviceGuard guard(dev);
-  const int ranks = kMostCluster;
+  const int sms = sm_count(dev);
+  if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
+  // as many CTAs a sequence as run at once, and as have a group of steps for every warp
+  const long long group = kTogether * 32 * (16 / (int)size), fit = (long long)kCtas * sms / a.batch, useful = (a.vocab + group * kWarps - 1) / (group * kWarps);
+  const int ranks = (int)(fit < useful ? (fit < 1 ? 1 : fit < kMostCluster ? fit : kMostCluster) : useful < kMostCluster ? useful : kMostCluster);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = a.type == FP6M_TYPE_F32 ? launch<float>(a, ranks, st) : a.type == FP6M_TYPE_F16 ? launch<half>(a, ranks, st) : launch<__nv_bfloat16>(a, ranks, st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "verify_drafts launch");
