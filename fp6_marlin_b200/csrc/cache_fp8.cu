@@ -26,10 +26,48 @@ using namespace fp6m;
 
 constexpr int kThreads = 256;
 
-template <class T> struct Exponents;
-template <> struct Exponents<half> { static constexpr int kLowest = -15, kHighest = 8; };
-template <> struct Exponents<__nv_bfloat16> { static constexpr int kLowest = -40, kHighest = 120; };
-constexpr float kMost = 448.f, kMostAtHighest = 240.f;
+constexpr float kMostAtHighest = 240.f;
+
+// What depends on the type: the exponents, and sixteen values at a time to and from E4M3.
+template <class T> struct Values;
+template <> struct Values<half> {
+  using Two = half2;
+  static constexpr int kLowest = -15, kHighest = 8;
+  // The products are exact, or so small that they become E4M3's zero.
+  static __device__ __forceinline__ void narrow(const uint32_t (&w)[8], int exponent, uint32_t (&q)[4]) {
+    const half2 by = __half2half2(__ushort_as_half((uint16_t)((15 - exponent) << 10)));
+    uint32_t pair[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      half2 x = __hmul2(*reinterpret_cast<const half2*>(&w[e]), by);
+      if (exponent == kHighest) x = __hmax2(__hmin2(x, __half2half2(__float2half_rn(kMostAtHighest))), __half2half2(__float2half_rn(-kMostAtHighest)));
+      pair[e] = __nv_cvt_halfraw2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = pair[2 * e] | pair[2 * e + 1] << 16;
+  }
+};
+template <> struct Values<__nv_bfloat16> {
+  using Two = __nv_bfloat162;
+  static constexpr int kLowest = -40, kHighest = 120;
+  static __device__ __forceinline__ void narrow(const uint32_t (&w)[8], int exponent, uint32_t (&q)[4]) {
+    const uint32_t one = (uint32_t)(127 - exponent) << 7, both = one | one << 16;
+    uint32_t pair[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const __nv_bfloat162 scaled = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), *reinterpret_cast<const __nv_bfloat162*>(&both));      // (exact)
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(&scaled);
+      float x = __uint_as_float(v << 16), y = __uint_as_float(v & 0xffff0000u);
+      if (exponent == kHighest) x = fminf(fmaxf(x, -kMostAtHighest), kMostAtHighest), y = fminf(fmaxf(y, -kMostAtHighest), kMostAtHighest);
+      pair[e] = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = pair[2 * e] | pair[2 * e + 1] << 16;
+  }
+};
+// The larger magnitudes of two pairs, NaN where there is one.
+__device__ __forceinline__ half2 larger(half2 a, half2 b) { return __hmax2_nan(a, __habs2(b)); }
+__device__ __forceinline__ __nv_bfloat162 larger(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, __habs2(b)); }
 
 struct CacheParams {
   fp6m_cache_fp8_args a;
@@ -37,122 +75,156 @@ struct CacheParams {
   unsigned long long page_magic;         // division by the page size, see tree_attention.cuh
   int page_shift;
   int at_once;                           // entries of a CTA
+  unsigned int entry_magic;              // division by an entry's units: n * magic >> 32, exact for n * units < 2^32
   int* status;
 };
 
-// Where token j of a page table's row lies: page and slot, or false.
-__device__ __forceinline__ bool find(const CacheParams& p, int b, int j, int* page, int* slot) {
-  const int place = (int)((unsigned long long)j * p.page_magic >> p.page_shift);
-  *page = p.a.page_table[b * p.a.page_table_stride + place];
-  *slot = j - place * p.a.page_size;
-  return (unsigned)*page < (unsigned)p.a.pages;
-}
-__device__ __forceinline__ void unpack16(const uint4& lo, const uint4& hi, uint32_t (&w)[8]) {
-  w[0] = lo.x; w[1] = lo.y; w[2] = lo.z; w[3] = lo.w;
-  w[4] = hi.x; w[5] = hi.y; w[6] = hi.z; w[7] = hi.w;
-}
-
-// A thread has sixteen neighbouring values of a head: 32 bytes on one side, 16 on the other; four or eight threads a head, the heads of a token's keys, then those of its
-// values, side by side.  Bound by memory where tokens are many, by four look-ups one after the other (length, list, page table, values) where they are few.
+// A CTA has some entries of a sequence, their keys or their values.  A unit is sixteen neighbouring values of a head: 32 bytes on one side, 16 on the other; four or eight units a
+// head, the heads of a token side by side.  A thread has up to kUnits units whose look-ups, then loads, are on their way together.  Bound by memory where tokens are many
+//, by look-ups one after the other (length, list, page table, values) where they are few.
+constexpr int kUnits = 2;
 template <class T, int D, bool kWrite>
 __global__ void __launch_bounds__(kThreads) cache_fp8_kernel(const __grid_constant__ CacheParams p) {
   constexpr int kPart = D / 16;
   const fp6m_cache_fp8_args& a = p.a;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int heads = 2 * a.kv_heads, per_entry = heads * kPart;
-  const long long entries = (long long)a.batch * a.entries, first = (long long)blockIdx.x * p.at_once;
-  const int here = (int)min((long long)p.at_once, entries - first), work = here * per_entry;
-  const long long most = (long long)a.max_pages * a.page_size;
+  const int b = blockIdx.y + (blockIdx.z >> 1) * gridDim.y;
+  if (b >= a.batch) return;
+  const bool values = blockIdx.z & 1;
+  const long long* wide_stride = values ? a.v_stride : a.k_stride;
+  const long long* narrow_stride = values ? a.v_cache_stride : a.k_cache_stride;
+  const long long* power_stride = values ? p.s.v_scales_stride : p.s.k_scales_stride;
+  T* const wide_rows = static_cast<T*>(values ? a.v : a.k) + b * wide_stride[0];
+  uint8_t* const narrow_rows = static_cast<uint8_t*>(values ? a.v_cache : a.k_cache);
+  uint8_t* const powers = static_cast<uint8_t*>(values ? p.s.v_scales : p.s.k_scales);
+  // (strides of tokens, pages and slots fit 32 bits)
+  const unsigned wide_step = (unsigned)wide_stride[1], page_step = (unsigned)narrow_stride[0], slot_step = (unsigned)narrow_stride[1], power_page = (unsigned)power_stride[0], power_slot = (unsigned)power_stride[1];
+  const long long wide_head = wide_stride[2], narrow_head = narrow_stride[2], power_head = power_stride[2];
+  const int per_entry = a.kv_heads * kPart, first = blockIdx.x * p.at_once, work = min(p.at_once, a.entries - first) * per_entry;
+  const int most = a.max_pages * a.page_size, length = min(max(a.lengths[b], 0), most), count = kWrite && a.counts ? a.counts[b] : a.entries;
+  const unsigned start = kWrite ? length : a.starts ? a.starts[b] : 0;      // (modulo 2^32: tokens before the first come behind all)
+  const int* table = a.page_table + b * a.page_table_stride;
+  const int part = threadIdx.x % kPart;
   bool bad = false;
-  for (int i0 = 0; i0 < work; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    bool lives = i < work;
-    const int entry_here = lives ? i / per_entry : 0, in_entry = i - entry_here * per_entry;
-    const int part = i % kPart, head = in_entry / kPart % a.kv_heads;
-    const bool values = in_entry / kPart >= a.kv_heads;
-    const int b = (int)((first + entry_here) / a.entries), entry = (int)((first + entry_here) - (long long)b * a.entries);
-    long long at = 0;
-    int token = entry;
-    if (lives) {
-      const int length = (int)min((long long)max(a.lengths[b], 0), most);
+#pragma unroll 1
+  for (int i0 = 0; i0 < work; i0 += kUnits * kThreads) {
+    bool lives[kUnits];
+    int token[kUnits], page[kUnits], slot[kUnits], head[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int i = i0 + u * kThreads + threadIdx.x;
+      const int in_cta = p.at_once == 1 ? 0 : (int)__umulhi((unsigned)i, p.entry_magic), entry = first + in_cta;
+      head[u] = (i - in_cta * per_entry) / kPart;
+      lives[u] = i < work;
+      token[u] = entry;
+      const unsigned at = start + entry;
       if (kWrite) {
-        if (a.counts && entry >= a.counts[b]) lives = false;
-        if (lives && a.list) token = a.list[b * a.list_stride + entry];
-        lives = lives && token >= 0;
-        at = (long long)length + entry;
-        if (lives && (at >= most || token >= a.tokens)) {
+        lives[u] = lives[u] && entry < count;
+        if (lives[u] && a.list) token[u] = a.list[b * a.list_stride + entry];
+        lives[u] = lives[u] && token[u] >= 0;
+        if (lives[u] && (at >= (unsigned)most || token[u] >= a.tokens)) {
           bad = true;
-          lives = false;
+          lives[u] = false;
         }
       } else {
-        at = (long long)(a.starts ? a.starts[b] : 0) + entry;
-        lives = at >= 0 && at < length;
+        lives[u] = lives[u] && at < (unsigned)length;
+      }
+      const int place = (int)((unsigned long long)at * (unsigned)p.page_magic >> p.page_shift);      // (the magic number is below 2^32)
+      slot[u] = (int)at - place * a.page_size;
+      page[u] = lives[u] ? table[place] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      if (lives[u] && (unsigned)page[u] >= (unsigned)a.pages) {
+        bad = true;
+        lives[u] = false;
       }
     }
-    int page = 0, slot = 0;
-    if (lives && !find(p, b, (int)at, &page, &slot)) {
-      bad = true;
-      lives = false;
-    }
-    const long long* wide_stride = values ? a.v_stride : a.k_stride;
-    const long long* narrow_stride = values ? a.v_cache_stride : a.k_cache_stride;
-    const long long* byte_stride = values ? p.s.v_scales_stride : p.s.k_scales_stride;
-    T* wide = static_cast<T*>(values ? a.v : a.k) + b * wide_stride[0] + token * wide_stride[1] + head * wide_stride[2] + part * 16;
-    uint8_t* narrow = static_cast<uint8_t*>(values ? a.v_cache : a.k_cache) + page * narrow_stride[0] + slot * narrow_stride[1] + head * narrow_stride[2] + part * 16;
-    uint8_t* byte = static_cast<uint8_t*>(values ? p.s.v_scales : p.s.k_scales) + page * byte_stride[0] + slot * byte_stride[1] + head * byte_stride[2];
+    auto wide = [&](int u) { return reinterpret_cast<uint4*>(wide_rows + (unsigned long long)(unsigned)token[u] * wide_step + head[u] * wide_head + part * 16); };
+    auto narrow = [&](int u) {
+      return reinterpret_cast<uint4*>(narrow_rows + (unsigned long long)(unsigned)page[u] * page_step + (unsigned long long)(unsigned)slot[u] * slot_step + head[u] * narrow_head + part * 16);
+    };
+    auto power = [&](int u) { return powers + (unsigned long long)(unsigned)page[u] * power_page + (unsigned long long)(unsigned)slot[u] * power_slot + head[u] * power_head; };
     if constexpr (kWrite) {
-      uint32_t w[8] = {};
-      if (lives) unpack16(reinterpret_cast<const uint4*>(wide)[0], reinterpret_cast<const uint4*>(wide)[1], w);
-      float x[16], top = 0.f;
+      uint4 in[kUnits][2];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        x[e] = Half16<T>::value((uint16_t)(w[e / 2] >> 16 * (e & 1)));
-        top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+      for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) in[u][h] = lives[u] ? wide(u)[h] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        constexpr uint32_t E = Half16<T>::kExponent;
+        uint32_t w[8] = {in[u][0].x, in[u][0].y, in[u][0].z, in[u][0].w, in[u][1].x, in[u][1].y, in[u][1].z, in[u][1].w};
+        using Two = typename Values<T>::Two;
+        uint32_t two = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const Two now = larger(*reinterpret_cast<const Two*>(&two), *reinterpret_cast<const Two*>(&w[e]));
+          two = *reinterpret_cast<const uint32_t*>(&now);
+        }
+        two &= 0x7fff7fffu;
+        uint32_t top = max(two & 0xffffu, two >> 16), odd = 0;       // (bits of magnitudes are ordered as they are); a bit for each value that is infinite or NaN
+        if (top >= E) {
+          // these become NaN, and the exponent is that of the others
+          top = 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t one = w[e / 2] >> 16 * (e & 1) & 0x7fffu;
+            if (one >= E) odd |= 1u << e;
+            else top = max(top, one);
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < kPart; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // = 1.m * 2^n; 448 = 1.75 * 2^8
+        const uint32_t bits = __float_as_uint(Half16<T>::value((uint16_t)top));
+        const int least = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
+        const int exponent = min(max(least, Values<T>::kLowest), Values<T>::kHighest);
+        uint32_t q[4];
+        Values<T>::narrow(w, exponent, q);
+        if (odd) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (odd >> e & 1) q[e / 4] |= 0x7fu << 8 * (e & 3);
+        }
+        if (lives[u]) {
+          *narrow(u) = make_uint4(q[0], q[1], q[2], q[3]);
+          if (part == 0) *power(u) = (uint8_t)(exponent + 127);
+        }
+      }
+    } else {
+      uint4 in[kUnits];
+      uint32_t by[kUnits];
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        in[u] = lives[u] ? *narrow(u) : make_uint4(0, 0, 0, 0);
+        by[u] = lives[u] ? *power(u) : 0;
       }
 #pragma unroll
-      for (int o = 1; o < kPart; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // top = 1.m * 2^n; 448 = 1.75 * 2^8
-      const uint32_t bits = __float_as_uint(top);
-      const int least = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
-      const int power = min(max(least, Exponents<T>::kLowest), Exponents<T>::kHighest);
-      const float down = __uint_as_float((uint32_t)(127 - power) << 23), limit = power == Exponents<T>::kHighest ? kMostAtHighest : kMost;
-      uint32_t q[4];
+      for (int u = 0; u < kUnits; ++u) {
+        if (!lives[u]) continue;
+        const float f = __uint_as_float(by[u] ? by[u] << 23 : 0x00400000u);
+        const uint32_t q[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
+        uint32_t w[8];
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        float two[2];
-#pragma unroll
-        for (int f = 0; f < 2; ++f) two[f] = fabsf(x[e + f]) < INFINITY ? fminf(fmaxf(x[e + f] * down, -limit), limit) : __uint_as_float(0x7fc00000u);
-        const uint32_t pair = __nv_cvt_float2_to_fp8x2(make_float2(two[0], two[1]), __NV_SATFINITE, __NV_E4M3);
-        q[e / 4] = e & 2 ? q[e / 4] | pair << 16 : pair;
+        for (int e = 0; e < 8; ++e) {
+          const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q[e / 2] >> 16 * (e & 1)), __NV_E4M3);
+          const float2 v = __half22float2(*reinterpret_cast<const half2*>(&two));
+          w[e] = Half16<T>::pack(v.x * f, v.y * f);
+        }
+        uint4* to = wide(u);
+        to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        to[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
-      if (lives) {
-        *reinterpret_cast<uint4*>(narrow) = make_uint4(q[0], q[1], q[2], q[3]);
-        if (part == 0) *byte = (uint8_t)(power + 127);
-      }
-    } else if (lives) {
-      const uint4 q = *reinterpret_cast<const uint4*>(narrow);
-      const uint32_t by_bits = *byte;
-      const float by = __uint_as_float(by_bits ? by_bits << 23 : 0x00400000u);
-      const uint32_t in[4] = {q.x, q.y, q.z, q.w};
-      uint32_t w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(in[e / 2] >> 16 * (e & 1)), __NV_E4M3);
-        const float2 f = __half22float2(*reinterpret_cast<const half2*>(&two));
-        w[e] = Half16<T>::pack(f.x * by, f.y * by);
-      }
-      reinterpret_cast<uint4*>(wide)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      reinterpret_cast<uint4*>(wide)[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
   if (bad && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
 }
 
 template <class T, int D>
-cudaError_t launch(const CacheParams& p, bool write, unsigned ctas, cudaStream_t stream) {
-  return write ? launch_overlapped(cache_fp8_kernel<T, D, true>, dim3(ctas), dim3(kThreads), 0, stream, p)
-               : launch_overlapped(cache_fp8_kernel<T, D, false>, dim3(ctas), dim3(kThreads), 0, stream, p);
+cudaError_t launch(const CacheParams& p, bool write, dim3 ctas, cudaStream_t stream) {
+  return write ? launch_overlapped(cache_fp8_kernel<T, D, true>, ctas, dim3(kThreads), 0, stream, p) : launch_overlapped(cache_fp8_kernel<T, D, false>, ctas, dim3(kThreads), 0, stream, p);
 }
 
 int run(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, bool write, int dev, void* stream, int* status_dev) {
@@ -161,7 +233,7 @@ int run(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, bool w
   if (a.batch < 0 || a.tokens < 0 || a.entries < 0 || (a.type != FP6M_TYPE_F16 && a.type != FP6M_TYPE_BF16)) return FP6M_ERR_BAD_ARG;
   if (a.head_dim != 64 && a.head_dim != 128) return FP6M_ERR_PROB_SHAPE;
   if (a.batch == 0 || a.entries == 0 || a.kv_heads == 0) return FP6M_OK;
-  if (a.kv_heads < 0 || a.kv_heads > 1 << 24 || a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fff0000ll) return FP6M_ERR_PROB_SHAPE;
+  if (a.kv_heads < 0 || a.kv_heads > 1 << 16 || a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fff0000ll) return FP6M_ERR_PROB_SHAPE;
   if (!a.lengths || a.list_stride < 0 || !rows_aligned(a.k, a.k_stride, 8) || !rows_aligned(a.v, a.v_stride, 8)) return FP6M_ERR_BAD_ARG;
   if (a.max_pages > 0) {
     if (!rows_aligned(a.k_cache, a.k_cache_stride, 16) || !rows_aligned(a.v_cache, a.v_cache_stride, 16) || !a.page_table || a.page_table_stride < 0) return FP6M_ERR_BAD_ARG;
@@ -169,20 +241,30 @@ int run(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, bool w
     for (int i = 0; i < 3; ++i)
       if (scales->k_scales_stride[i] < 0 || scales->v_scales_stride[i] < 0) return FP6M_ERR_BAD_ARG;
   }
+  constexpr long long kStep = 0xffffffffll;          // of tokens, pages and slots
+  if (a.k_stride[1] > kStep || a.v_stride[1] > kStep) return FP6M_ERR_PROB_SHAPE;
+  for (int i = 0; i < 2; ++i)
+    if (a.k_cache_stride[i] > kStep || a.v_cache_stride[i] > kStep || scales->k_scales_stride[i] > kStep || scales->v_scales_stride[i] > kStep) return FP6M_ERR_PROB_SHAPE;
   DeviceGuard guard(dev);
   CacheParams p;
   p.a = a;
   p.s = *scales;
   p.status = status_dev;
   division_by(a.page_size, &p.page_magic, &p.page_shift);
-  const int per_entry = 2 * a.kv_heads * (a.head_dim / 16);
-  p.at_once = per_entry >= kThreads ? 1 : kThreads / per_entry;
-  const long long ctas = ((long long)a.batch * a.entries + p.at_once - 1) / p.at_once;
-  if (ctas > INT_MAX) return FP6M_ERR_PROB_SHAPE;
+  const int sms = sm_count(dev);
+  if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
+  // a unit a thread where that leaves multiprocessors without work, else kUnits
+  const int per_entry = a.kv_heads * (a.head_dim / 16);
+  const bool many = 2ll * a.batch * a.entries * per_entry > (long long)sms * 8 * kThreads;
+  p.at_once = (many ? kUnits : 1) * kThreads / per_entry;
+  if (p.at_once < 1) p.at_once = 1;
+  p.entry_magic = (unsigned int)((1ull << 32) / per_entry + 1);
+  const dim3 ctas((unsigned)((a.entries + (long long)p.at_once - 1) / p.at_once), (unsigned)(a.batch < 65535 ? a.batch : 65535), (unsigned)(2 * ((a.batch + 65534ll) / 65535)));      // keys and values
+  if (ctas.z > 65535) return FP6M_ERR_PROB_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool is_half = a.type == FP6M_TYPE_F16;
-  const cudaError_t e = a.head_dim == 64 ? (is_half ? launch<half, 64>(p, write, (unsigned)ctas, st) : launch<__nv_bfloat16, 64>(p, write, (unsigned)ctas, st))
-                                         : (is_half ? launch<half, 128>(p, write, (unsigned)ctas, st) : launch<__nv_bfloat16, 128>(p, write, (unsigned)ctas, st));
+  const cudaError_t e = a.head_dim == 64 ? (is_half ? launch<half, 64>(p, write, ctas, st) : launch<__nv_bfloat16, 64>(p, write, ctas, st))
+                                         : (is_half ? launch<half, 128>(p, write, ctas, st) : launch<__nv_bfloat16, 128>(p, write, ctas, st));
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "cache_fp8 launch");
 }
 
