@@ -204,8 +204,6 @@ __device__ __forceinline__ void ldsm_t_two(uint32_t (&a)[2], uint32_t (&b)[2], u
   ldsm_t(r, addr);
   a[0] = r[0]; a[1] = r[1]; b[0] = r[2]; b[1] = r[3];
 }
-// four bytes
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 // (not volatile: to be moved between the steps of other chains)
 __device__ __forceinline__ void mma_halves(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

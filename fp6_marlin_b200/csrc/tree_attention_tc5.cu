@@ -54,8 +54,8 @@ struct TreeCfg {
   static constexpr int kK = 0, kQ = kKeyStages * kStageBytes, kV = kQ + (kPair ? 2 : 1) * kQBytes, kX = kV + kValueStages * kStageBytes;
   static constexpr int kStats = kX + kExchange;              // [128] maxima, [128] totals of the second group
   static constexpr int kPlaces = kStats + 2 * kRowTile * 4;  // [keys, values][2][64] addresses
-  static constexpr int kPowers = kPlaces + 4 * kKeys * 8;    // [keys, values][64] powers of two of a tile's tokens (kFp8)
-  static constexpr int kBars = kPowers + (kFp8 ? 2 * kKeys * 4 : 0);
+  static constexpr int kPowers = kPlaces + 4 * kKeys * 8;    // [stages of keys, then of values][128] powers of two of a job's tokens (kFp8)
+  static constexpr int kBars = kPowers + (kFp8 ? (kKeyStages + kValueStages) * 2 * kKeys * 4 : 0);
   static constexpr int kSmemBytes = kBars + kNumBars * 8 + (4 + 32) * 4 + 1024;
   static constexpr int kSlotFloats = kRowTile * (D + 2) + 4; // a partial: sums [4 columns][row], maxima, totals, whether odd values were met
   static_assert(kSmemBytes <= 232448, "shared memory");
@@ -103,20 +103,34 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) 
                : "memory");
 }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
-__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-// Two E4M3 values (the lower or the upper ones of four) times a power of two, in 16 bits: exact where the type holds the result.
-template <class T>
-__device__ __forceinline__ uint32_t widened(uint32_t four, bool upper, float by) {
-  uint32_t h;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(upper ? four >> 16 : four));
-  const float2 two = __half22float2(*reinterpret_cast<half2*>(&h));
-  return Half16<T>::pack(two.x * by, two.y * by);
+// Four E4M3 values times a power of two, in 16 bits: exact where the type holds the result.  In fp16 one product a pair (the powers that it holds are those that it was written
+// with).  of: the factor, from the exponent + 127.
+__device__ __forceinline__ void halves_of(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(four));
 }
+template <class T> struct Widen;
+template <> struct Widen<half> {
+  static __device__ __forceinline__ uint32_t of(int power) { return 0x10001u * __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)min(max(power, 127 - 24), 127 + 15) << 23))); }
+  static __device__ __forceinline__ void run(uint32_t four, uint32_t by, uint32_t& lo, uint32_t& hi) {
+    halves_of(four, lo, hi);
+    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(by));
+    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(by));
+  }
+};
+template <> struct Widen<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t of(int power) { return 0x10001u * ((uint32_t)min(max(power, 1), 254) << 7); }
+  static __device__ __forceinline__ void run(uint32_t four, uint32_t by, uint32_t& lo, uint32_t& hi) {
+    halves_of(four, lo, hi);
+    const float2 p = __half22float2(*reinterpret_cast<half2*>(&lo)), q = __half22float2(*reinterpret_cast<half2*>(&hi));
+    lo = Half16<__nv_bfloat16>::pack(p.x, p.y);
+    hi = Half16<__nv_bfloat16>::pack(q.x, q.y);
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(by));
+    asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(hi) : "r"(by));
+  }
+};
 
 struct NoScales {};
 
@@ -152,7 +166,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
       mbar_init(product + 8 * i, 1);         // [group] tcgen05.commit: a segment's last weights are multiplied
     }
     if constexpr (C::kFp8)
-      for (int i = 0; i < SK + SV; ++i) mbar_init(raw_k + 8 * i, 2);    // the warps that issue a job's copies; its bytes have landed
+      for (int i = 0; i < SK + SV; ++i) mbar_init(raw_k + 8 * i, 32);   // a warp that brings a job's tiles in 8 bits, and their powers of two
     mbar_fence_init();
     misc[1] = 0;
   }
@@ -230,171 +244,111 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         }
       };
       if constexpr (C::kFp8) {
-        // Cached tiles come as they are, E4M3, into the place of the 16-bit tile that they become; a job later, when they have landed, each thread takes sixteen values of eight tokens,
-        // and when all have, puts them back in 16 bits, times the token's power of two.  So the loads of one job are on their way while the job before is widened.
+        // Cached tiles come as they are, E4M3, into the place of the 16-bit tile that they become (warps 5 and 6 bring them, see there); each thread takes sixteen values of a few tokens
+        // and puts them back in 16 bits, times the token's power of two.  Heads of 128 values: a row lies where the first half of its 16-bit values goes, and both are one warp's; else
+        // all threads have read a tile before any writes.  Tiles that TMA does not bring - the last ones of a sequence - are fetched here.
         const uint32_t raw = values ? raw_v : raw_k;
-        const void* power_base = values ? scales.v_scales : scales.k_scales;
-        const long long* power_stride = values ? scales.v_scales_stride : scales.k_scales_stride;
         const long long* cache_stride = values ? a.v_cache_stride : a.k_cache_stride;
         const uint8_t* cache = static_cast<const uint8_t*>(values ? a.v_cache : a.k_cache);
-        float* powers = reinterpret_cast<float*>(smem + C::kPowers) + (values ? kKeys : 0);
-        constexpr int kNarrow = D / 16, kNarrowRows = 64 / kNarrow;    // 16-byte pieces of a row, rows of a pass
+        const uint32_t* powers = reinterpret_cast<const uint32_t*>(smem + C::kPowers) + (values ? SK * 2 * kKeys : 0);
+        constexpr int kNarrow = D / 16, kNarrowRows = 64 / kNarrow, kNarrowPasses = kKeys / kNarrowRows;    // 16-byte pieces of a row, rows of a pass
         const int narrow = me % kNarrow, narrow0 = me / kNarrow;
-        struct Job { int tile, tiles, length, b, g, segment, stage; uint32_t phase; bool other; int power[2]; };      // other: not all of it by TMA
-        // widens a job's tiles
-        auto finish = [&](const Job& job) {
-          mbar_wait_bounded<20>(raw + 8 * job.stage, job.phase, p.status, dead);
-          if (job.other) asm volatile("cp.async.wait_all;" ::: "memory");
-          for (int odd_tile = 0; odd_tile < 2; ++odd_tile) {
-            const uint32_t at = ring + job.stage * C::kStageBytes + odd_tile * (kKeys * 128), bar = full + 8 * job.stage;
-            if (odd_tile < job.tiles) {
-              const int cached = min(job.length - (job.tile + odd_tile) * kKeys, kKeys);
-              // (a power of 16-bit floating point at least: what the type holds)
-              powers[me] = __uint_as_float((uint32_t)max(job.power[odd_tile], 1) << 23);
-              named_bar_sync(bar_id, 64);
-              uint32_t v[kKeys / kNarrowRows][4];
-              float by[kKeys / kNarrowRows];
-#pragma unroll
-              for (int i = 0; i < kKeys / kNarrowRows; ++i) {
-                const int row = narrow0 + i * kNarrowRows;
-                by[i] = powers[row];
-                const uint4 w = lds128(at + row * D + narrow * 16);
-                v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w;
-              }
-              named_bar_sync(bar_id, 64);
-#pragma unroll
-              for (int i = 0; i < kKeys / kNarrowRows; ++i) {
-                const int row = narrow0 + i * kNarrowRows;
-                if (row < cached) {
-                  uint32_t w[8];
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) w[e] = widened<T>(v[i][e / 2], e & 1, by[i]);
-                  const uint32_t to = at + (2 * narrow >> 3) * C::kHalfBytes + row * 128;
-                  sts128(to + (((2 * narrow & 7) ^ (row & 7)) * 16), w);
-                  sts128(to + (((2 * narrow & 7) + 1 ^ (row & 7)) * 16), w + 4);
-                }
-              }
-              if (values && cached < kKeys) {
-                // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
-                // that see them at the end.
-                named_bar_sync(bar_id, 64);
-                bool odd = false;
-                if (me >= cached) {
-                  for (int c = 0; c < D / 8; ++c) {
-                    const uint32_t place = at + (c >> 3) * C::kHalfBytes + me * 128 + (((c & 7) ^ (me & 7)) * 16);
-                    const uint4 w = lds128(place);
-                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
-                    constexpr uint32_t E = Half16<T>::kExponent;
-                    for (int e = 0; e < 4; ++e) {
-                      if (!is_odd<T>(x[e])) continue;
-                      odd = true;
-                      if ((x[e] & E) == E) x[e] &= 0xffff0000u;
-                      if ((x[e] >> 16 & E) == E) x[e] &= 0xffffu;
-                      sts_u32(place + 4 * e, x[e]);
-                    }
-                  }
-                }
-                if (odd) odd_ring[job.segment % kOddRing] = 1;
-              }
-              // what was stored is seen by the MMAs, and by the copies that come into this place later
-              fence_async_proxy();
-            }
-            mbar_arrive(bar);
-          }
-        };
-        Job before = {};
-        bool pending = false;
+        phase = 0;                                                     // (here: of `raw`)
         while (__shfl_sync(0xffffffffu, (int)ahead.next(p), 0)) {
           const int t0 = __shfl_sync(0xffffffffu, ahead.t0, 0), t1 = __shfl_sync(0xffffffffu, ahead.t1, 0), length = __shfl_sync(0xffffffffu, ahead.length, 0);
           const int g = __shfl_sync(0xffffffffu, ahead.item / p.parts, 0);
-          const uint8_t* head_powers = static_cast<const uint8_t*>(power_base) + g * power_stride[2];
           if (values) {
             if (me == 0) odd_ring[segment % kOddRing] = 0;
           } else {
-            // (the queries wait for the last scores of the item before, and those for the job that is pending)
-            if (pending && q_sets == 1) {
-              finish(before);
-              pending = false;
-            }
             load_queries();
-          }
-          int pages = 0, pages_next = 0;
-          if (p.run > 0) {
-            pages = pages_of(t0 >> block_shift);
-            pages_next = pages_of((t0 >> block_shift) + 1);
           }
 #pragma unroll 1
           for (int tile = t0; tile < t1; tile += 2) {
-            Job job = {tile, min(t1 - tile, 2), length, ahead.b, g, segment, stage, (phase & 1) ^ 1, (!values && tile == t0), {127, 127}};
-            mbar_wait_bounded<50>(empty + 8 * stage, phase, p.status, dead);
-            bool missing = false;
-            uint32_t bytes = 0;                                        // that this warp brings by TMA
-#pragma unroll
-            for (int odd_tile = 0; odd_tile < 2; ++odd_tile) {
-              if (odd_tile >= job.tiles) continue;
-              const int at_tile = tile + odd_tile, in_block = at_tile & (block_tiles - 1);
-              const uint32_t dst = ring + stage * C::kStageBytes + odd_tile * (kKeys * 128);
-              if (p.run > 0 && in_block == 0 && at_tile != t0) {
-                pages = pages_next;
-                pages_next = pages_of((at_tile >> block_shift) + 1);
-              }
-              const int j = at_tile * kKeys + me;
-              const int page = p.run > 0 ? __shfl_sync(0xffffffffu, pages, in_block * tile_runs + me / p.run) : j < length ? page_of(p, ahead, j) : -1;
-              const int slot = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
-              const bool known = j < length && (unsigned)page < (unsigned)a.pages;
-              if (known) job.power[odd_tile] = head_powers[page * power_stride[0] + slot * power_stride[1]];
-              missing = missing || (j < length && !known);
-              if (p.run > 0 && (at_tile + 1) * kKeys <= length) {
-                if (second == odd_tile) {
-                  bytes = kKeys * D;
-                  if (elect_one()) mbar_arrive_tx(raw + 8 * stage, bytes);
-                  __syncwarp();
-                  int first_slot = at_tile * kKeys - (int)((unsigned long long)(at_tile * kKeys) * p.page_magic >> p.page_shift) * a.page_size;
+            mbar_wait_bounded<20>(raw + 8 * stage, phase, p.status, dead);
+            const uint32_t bar = full + 8 * stage;
 #pragma unroll 1
-                  for (int i = 0; i < tile_runs; ++i) {
-                    int of = __shfl_sync(0xffffffffu, pages, in_block * tile_runs + i);
-                    if ((unsigned)of >= (unsigned)a.pages) of = a.pages;        // behind the last page the copy reads zeros
-                    if (elect_one()) tma_load_run(dst + i * p.run * D, map, 0, g, first_slot, of, raw + 8 * stage);
-                    __syncwarp();
-                    first_slot += p.run;
-                    if (first_slot == a.page_size) first_slot = 0;
+            for (int odd_tile = 0; odd_tile < 2; ++odd_tile) {
+              const uint32_t at = ring + stage * C::kStageBytes + odd_tile * (kKeys * 128);
+              const int at_tile = tile + odd_tile;
+              if (at_tile < t1) {
+                const int cached = min(length - at_tile * kKeys, kKeys);
+                const bool by_tma = p.run > 0 && cached == kKeys, apart = D == 128 && by_tma;
+                if (!by_tma) {
+                  // a thread works out where its token is
+                  const uint8_t** narrow_places = reinterpret_cast<const uint8_t**>(places);
+                  const int j = at_tile * kKeys + me, page = j < length ? page_of(p, ahead, j) : -1;
+                  const int slot = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
+                  narrow_places[me] = (unsigned)page < (unsigned)a.pages ? cache + page * cache_stride[0] + slot * cache_stride[1] + g * cache_stride[2] : nullptr;
+                  named_bar_sync(bar_id, 64);
+#pragma unroll 4
+                  for (int i = 0; i < kNarrowPasses; ++i) {
+                    const int row = narrow0 + i * kNarrowRows;
+                    const uint8_t* src = narrow_places[row];
+                    if (row < cached) copy16(at + row * D + narrow * 16, src ? src + narrow * 16 : static_cast<const uint8_t*>(a.q), src ? 16 : 0);
+                  }
+                  // drafted tokens as they are; zeros behind them
+                  const long long* drafted_stride = values ? a.v_stride : a.k_stride;
+                  for (int row = row0; row < kKeys; row += kRowsPerPass) {
+                    const int t = at_tile * kKeys + row - length;
+                    if (t < 0) continue;
+                    const T* src = static_cast<const T*>(values ? a.v : a.k) + ahead.b * drafted_stride[0] + min(t, a.tokens - 1) * drafted_stride[1] + g * drafted_stride[2];
+                    copy16(at + (chunk >> 3) * C::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src + chunk * 8, t < a.tokens ? 16 : 0);
                   }
                 }
-              } else {
-                job.other = true;
-                const uint8_t* place = known ? cache + page * cache_stride[0] + slot * cache_stride[1] + g * cache_stride[2] : nullptr;
-                const uint8_t** narrow_places = reinterpret_cast<const uint8_t**>(places);
-                named_bar_sync(bar_id, 64);                            // (the places of the tile before have been read)
-                narrow_places[me] = place;
-                named_bar_sync(bar_id, 64);
-                const int cached = min(length - at_tile * kKeys, kKeys);
-#pragma unroll 4
-                for (int i = 0; i < kKeys / kNarrowRows; ++i) {
+                if (!by_tma || (!values && tile == t0)) asm volatile("cp.async.wait_all;" ::: "memory");      // (the queries, too)
+                if (!apart) named_bar_sync(bar_id, 64);
+                uint32_t v[kNarrowPasses][4];
+#pragma unroll
+                for (int i = 0; i < kNarrowPasses; ++i) {
+                  const uint4 w = lds128(at + (narrow0 + i * kNarrowRows) * D + narrow * 16);
+                  v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w;
+                }
+                if (apart) __syncwarp();
+                else named_bar_sync(bar_id, 64);
+#pragma unroll
+                for (int i = 0; i < kNarrowPasses; ++i) {
                   const int row = narrow0 + i * kNarrowRows;
-                  const uint8_t* src = narrow_places[row];
-                  if (row < cached) copy16(dst + row * D + narrow * 16, src ? src + narrow * 16 : static_cast<const uint8_t*>(a.q), src ? 16 : 0);
+                  const uint32_t by = powers[(stage * 2 + odd_tile) * kKeys + row];
+                  uint32_t w[8];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) Widen<T>::run(v[i][e], by, w[2 * e], w[2 * e + 1]);
+                  const uint32_t to = at + (2 * narrow >> 3) * C::kHalfBytes + row * 128;
+                  if (row < cached) {
+                    sts128(to + (((2 * narrow & 7) ^ (row & 7)) * 16), w);
+                    sts128(to + (((2 * narrow & 7) + 1 ^ (row & 7)) * 16), w + 4);
+                  }
                 }
-                // drafted tokens as they are; zeros behind them
-                const long long* drafted_stride = values ? a.v_stride : a.k_stride;
-                for (int row = row0; row < kKeys; row += kRowsPerPass) {
-                  const int t = at_tile * kKeys + row - length;
-                  if (t < 0) continue;
-                  const T* src = static_cast<const T*>(values ? a.v : a.k) + ahead.b * drafted_stride[0] + min(t, a.tokens - 1) * drafted_stride[1] + g * drafted_stride[2];
-                  copy16(dst + (chunk >> 3) * C::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) * 16), src + chunk * 8, t < a.tokens ? 16 : 0);
+                if (values && cached < kKeys) {
+                  // Infinities and NaN among the drafted values: a weight of zero must not meet them.  They are zero in the product, and added to the rows
+                  // that see them at the end.
+                  named_bar_sync(bar_id, 64);
+                  bool odd = false;
+                  if (me >= cached) {
+                    for (int c = 0; c < D / 8; ++c) {
+                      const uint32_t place = at + (c >> 3) * C::kHalfBytes + me * 128 + (((c & 7) ^ (me & 7)) * 16);
+                      const uint4 w = lds128(place);
+                      uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                      constexpr uint32_t E = Half16<T>::kExponent;
+                      for (int e = 0; e < 4; ++e) {
+                        if (!is_odd<T>(x[e])) continue;
+                        odd = true;
+                        if ((x[e] & E) == E) x[e] &= 0xffff0000u;
+                        if ((x[e] >> 16 & E) == E) x[e] &= 0xffffu;
+                        sts_u32(place + 4 * e, x[e]);
+                      }
+                    }
+                  }
+                  if (odd) odd_ring[segment % kOddRing] = 1;
                 }
+                // what was stored is seen by the MMAs, and by the copies that come into this place later
+                fence_async_proxy();
               }
+              mbar_arrive(bar);
             }
-            if (bytes == 0 && elect_one()) mbar_arrive(raw + 8 * stage);
-            __syncwarp();
-            if (__any_sync(0xffffffffu, missing)) misc[1] = 1;
-            if (pending) finish(before);
-            before = job;
-            pending = true;
             if (++stage == stages) { stage = 0; phase ^= 1; }
           }
           ++segment;
         }
-        if (pending) finish(before);
       } else {
       while (__shfl_sync(0xffffffffu, (int)ahead.next(p), 0)) {
         // What follows from the lengths is made uniform to the compiler (read from lane 0): copies whose operands it takes to differ between
@@ -608,6 +562,115 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         const bool segment_ends = back.left <= 2;
         back_lives = back.advance(p, SV);
         if (segment_ends) started = 0;
+      }
+    } else if (C::kFp8 && (warp == 5 || warp == 6)) {
+      // ================================================================== tiles in 8 bits: a warp the keys, one the values
+      if constexpr (C::kFp8) {
+        const bool values = warp == 6;
+        const uint32_t ring = base + (values ? C::kV : C::kK), empty = values ? empty_v : empty_k, raw = values ? raw_v : raw_k;
+        const int stages = values ? SV : SK;
+        const CUtensorMap* map = values ? &vmap : &kmap;
+        const void* power_base = values ? scales.v_scales : scales.k_scales;
+        const long long* power_stride = values ? scales.v_scales_stride : scales.k_scales_stride;
+        const unsigned power_page = (unsigned)power_stride[0], power_slot = (unsigned)power_stride[1];
+        uint32_t* powers = reinterpret_cast<uint32_t*>(smem + C::kPowers) + (values ? SK * 2 * kKeys : 0);
+        // the pages of 32 runs, a lane each, and those of the next 32 are on their way; without runs each token's is looked up
+        const int tile_runs = p.run > 0 ? kKeys / p.run : 1, block_tiles = 32 / tile_runs, block_shift = 31 - __clz(block_tiles), run_log2 = __ffs(max(p.run, 1)) - 1, step_slots = kKeys % a.page_size;
+        auto pages_of = [&](int block) {
+          const int j = (block * 32 + lane) * p.run;
+          return j < seg.length ? page_of(p, seg, j) : -1;
+        };
+        int stage = 0;
+        uint32_t phase = 1;                                            // of `empty`; the first round of stages is free
+        while (__shfl_sync(0xffffffffu, (int)seg.next(p), 0)) {
+          const int t0 = __shfl_sync(0xffffffffu, seg.t0, 0), t1 = __shfl_sync(0xffffffffu, seg.t1, 0), length = __shfl_sync(0xffffffffu, seg.length, 0);
+          const int g = __shfl_sync(0xffffffffu, seg.item / p.parts, 0);
+          const uint8_t* head_powers = static_cast<const uint8_t*>(power_base) + g * power_stride[2];
+          int block = t0 >> block_shift, pages = 0, pages_next = 0, slot[2], power[2][2];
+          if (p.run > 0) {
+            pages = pages_of(block);
+            pages_next = pages_of(block + 1);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int j = t0 * kKeys + 32 * i + lane;
+            slot[i] = j - (int)((unsigned long long)j * p.page_magic >> p.page_shift) * a.page_size;
+          }
+          int first_slot = __shfl_sync(0xffffffffu, slot[0], 0);
+          bool missing = false;
+          // the exponents of a job's tokens; looked up while the job before is waited for
+          auto look_up = [&](int tile) {
+#pragma unroll
+            for (int odd_tile = 0; odd_tile < 2; ++odd_tile) {
+              const int at_tile = tile + odd_tile, of_block = at_tile >> block_shift == block ? pages : pages_next;
+              power[odd_tile][0] = power[odd_tile][1] = 127;
+              if (at_tile >= t1) continue;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int in = 32 * i + lane, j = at_tile * kKeys + in;
+                const int page = p.run > 0 ? __shfl_sync(0xffffffffu, of_block, (at_tile & (block_tiles - 1)) * tile_runs + (in >> run_log2)) : j < length ? page_of(p, seg, j) : -1;
+                if (j < length) {
+                  const bool known = (unsigned)page < (unsigned)a.pages;
+                  if (known) power[odd_tile][i] = head_powers[(unsigned long long)(unsigned)page * power_page + (unsigned long long)(unsigned)slot[i] * power_slot];
+                  missing = missing || !known;
+                }
+                slot[i] += step_slots;
+                if (slot[i] >= a.page_size) slot[i] -= a.page_size;
+              }
+            }
+          };
+          look_up(t0);
+#pragma unroll 1
+          for (int tile = t0; tile < t1; tile += 2) {
+            mbar_wait_bounded<20>(empty + 8 * stage, phase, p.status, dead);
+            const uint32_t bar = raw + 8 * stage;
+#pragma unroll 1
+            for (int at_tile = tile; at_tile < min(tile + 2, t1); ++at_tile) {
+              if (p.run > 0 && at_tile >> block_shift != block) {
+                ++block;
+                pages = pages_next;
+                pages_next = pages_of(block + 1);
+              }
+              if (p.run > 0 && (at_tile + 1) * kKeys <= length) {
+                const uint32_t dst = ring + stage * C::kStageBytes + (at_tile - tile) * (kKeys * 128);
+                const int in_block = at_tile & (block_tiles - 1);
+                if (elect_one()) mbar_expect_tx(bar, kKeys * D);
+                __syncwarp();
+                auto bring = [&](auto runs) {
+                  constexpr int R = decltype(runs)::value;
+                  int of[R];
+#pragma unroll
+                  for (int r = 0; r < R; ++r) {
+                    of[r] = __shfl_sync(0xffffffffu, pages, in_block * R + r);
+                    if ((unsigned)of[r] >= (unsigned)a.pages) of[r] = a.pages;        // behind the last page the copy reads zeros
+                  }
+                  if (elect_one()) {
+                    int from = first_slot;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                      tma_load_run(dst + r * (kKeys / R) * D, map, 0, g, from, of[r], bar);
+                      from += kKeys / R;
+                      if (from == a.page_size) from = 0;
+                    }
+                  }
+                  __syncwarp();
+                };
+                if (tile_runs == 1) bring(std::integral_constant<int, 1>());
+                else if (tile_runs == 2) bring(std::integral_constant<int, 2>());
+                else if (tile_runs == 4) bring(std::integral_constant<int, 4>());
+                else bring(std::integral_constant<int, 8>());
+              }
+              first_slot += step_slots;
+              if (first_slot >= a.page_size) first_slot -= a.page_size;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) powers[stage * 2 * kKeys + 32 * i + lane] = Widen<T>::of(power[i >> 1][i & 1]);
+            if (missing) misc[1] = 1;
+            mbar_arrive(bar);
+            if (++stage == stages) { stage = 0; phase ^= 1; }
+            look_up(tile + 2);
+          }
+        }
       }
     } else if (warp >= 8) {
       // ================================================================== weights: thread = row
