@@ -1,6 +1,6 @@
 """One decoder block over trees of drafted tokens: the operators of this package as they follow one another.
 
-    python -m fp6_marlin_b200.draft_step [--sequences 8] [--tokens 16] [--cached 2048]
+    python -m fp6_marlin_b200.draft_step [--sequences 8] [--tokens 16] [--cached 2048] [--fp8-cache]
 
 A block of a 7B model with random weights.  The queries / keys / values and gate / up projections are kept in 8 bits, the output and
 down projections in INT4 / FP6.  A step takes the drafted tokens of every sequence through the block:
@@ -9,7 +9,12 @@ down projections in INT4 / FP6.  A step takes the drafted tokens of every sequen
     -> rms_norm with the residual's addition -> E4M3 -> mul_fp8 (gate, up) -> silu * up -> mul_fused (down projection + residual)
 
 What the drafted tokens are not needed for any more once some are accepted - their keys and values - then goes into the cache
-(:meth:`DraftBlock.accept`).  The program prints the time of a step and the relative error of its result against the same step in elementary torch operations.
+(:meth:`DraftBlock.accept`).  With a cache in 8 bits (``fp8_cache``, and ``vocab`` for a projection onto a vocabulary) the step is closed on the device:
+
+    ... -> tree_attention_fp8 -> ... -> rms_norm -> mul_fp8 (vocabulary) -> softmax -> verify_drafts -> write_cache_fp8 of the accepted tokens
+
+(:meth:`DraftBlock.choose`, :meth:`DraftBlock.commit`), with no synchronisation, so that all of it can be captured in a CUDA graph.  The program prints the time of a step and
+the relative error of its result against the same step in elementary torch operations.
 """
 from __future__ import annotations
 
@@ -19,13 +24,14 @@ import torch
 
 from .api import mul, mul_fused
 from .block_ops import GROUP, make_fp8_weight, mul_fp8, rms_norm, tree_attention, tree_masks
+from .decode_ops import make_cache_fp8, tree_attention_fp8, verify_drafts, write_cache_fp8
 from .quant import make_w46_weight
 
 
 class DraftBlock:
     """Weights, cache and work buffers of one decoder block for up to ``sequences * tokens`` rows at a time."""
 
-    def __init__(self, hidden=4096, inter=11008, heads=32, kv_heads=32, sequences=8, tokens=16, pages=1024, page_size=16, quant_cols=256, seed=0, device="cuda"):
+    def __init__(self, hidden=4096, inter=11008, heads=32, kv_heads=32, sequences=8, tokens=16, pages=1024, page_size=16, quant_cols=256, seed=0, device="cuda", fp8_cache=False, vocab=0):
         gen = torch.Generator(device=device).manual_seed(seed)
         randn = lambda *shape: torch.randn(shape, generator=gen, device=device)          # noqa: E731
         self.heads, self.kv_heads, self.dim = heads, kv_heads, hidden // heads
@@ -36,7 +42,18 @@ class DraftBlock:
         self.out = make_w46_weight((randn(hidden, hidden) * 0.02).half(), quant_cols, GROUP, quant_device=device)
         self.down = make_w46_weight((randn(inter, hidden) * 0.02).half(), quant_cols, GROUP, quant_device=device)
         self.k_cache, self.v_cache = (randn(pages, page_size, kv_heads, self.dim).half() for _ in range(2))
+        self.fp8 = None
+        if fp8_cache:
+            # the same values in 8 bits: every page is written as the first tokens of a sequence of its own
+            self.fp8 = make_cache_fp8(pages, page_size, kv_heads, self.dim, device)
+            write_cache_fp8(self.k_cache, self.v_cache, *self.fp8, torch.arange(pages, dtype=torch.int32, device=device)[:, None], torch.zeros(pages, dtype=torch.int32, device=device))
+            self.k_cache = self.v_cache = None
         rows, half = sequences * tokens, dict(dtype=torch.float16, device=device)
+        if vocab:
+            self.norm3, self.head = (1 + 0.1 * randn(hidden)).half(), make_fp8_weight(randn(vocab, hidden) * 0.05)
+            self.logits = torch.empty((rows, vocab), **half)
+            self.accepted, self.counts = (torch.empty(shape, dtype=torch.int32, device=device) for shape in ((sequences, tokens), (sequences,)))
+            self.next_tokens = torch.empty(sequences, dtype=torch.int64, device=device)
         self.rows8, self.scales = torch.empty((rows, hidden), dtype=torch.float8_e4m3fn, device=device), torch.empty((rows, -(-hidden // GROUP)), device=device)
         self.qkv_out = torch.empty((rows, self.qkv[0].shape[0]), **half)
         self.gate_up_out, self.act = torch.empty((rows, 2 * inter), **half), torch.empty((rows, inter), **half)
@@ -60,7 +77,11 @@ class DraftBlock:
         depth = ((tree[..., None] >> bits) & 1).sum(-1) - 1                       # ancestors of a drafted token
         positions = (lengths[:, None] + depth).float()
         q, k = self._rotate(q, positions), self._rotate(k, positions)
-        tree_attention(q, k, v, self.k_cache, self.v_cache, page_table, lengths, tree, self.attended.view(b, t, h, d))
+        attended = self.attended.view(b, t, h, d)
+        if self.fp8 is None:
+            tree_attention(q, k, v, self.k_cache, self.v_cache, page_table, lengths, tree, attended)
+        else:
+            tree_attention_fp8(q, k, v, *self.fp8, page_table, lengths, tree, attended)
         mul(self.attended, self.out.B, self.projected, self.out.s, self.workspace, self.quant_cols, group_size=GROUP, layout="b200")
         rms_norm(self.projected, self.norm2, self.rows8, scales=self.scales, residual=x, residual_out=self.stream)
         mul_fp8(self.rows8, self.gate_up[0], self.gate_up_out, self.scales, self.gate_up[1])
@@ -69,10 +90,33 @@ class DraftBlock:
         mul_fused(self.act, self.down.B, self.result, self.down.s, self.workspace, self.quant_cols, epilogue="residual", residual=self.stream, group_size=GROUP)
         return self.result, k, v
 
+    def choose(self, result, drafted, tree, uniforms, draft=None):
+        """From the rows of a step to the accepted drafted tokens: ``(accepted, counts, next_tokens)`` as :func:`verify_drafts` gives them.  The target's probabilities are the softmax
+        of a projection onto the vocabulary in 8 bits; drafted (sequences, tokens): the ids; uniforms: random numbers; draft: the probabilities that the ids were drawn from."""
+        rms_norm(result, self.norm3, self.rows8, scales=self.scales)
+        mul_fp8(self.rows8, self.head[0], self.logits, self.scales, self.head[1])
+        target = torch.softmax(self.logits.float(), 1).view(self.sequences, self.tokens, -1)
+        verify_drafts(target, drafted, tree, uniforms, self.accepted, self.counts, self.next_tokens, draft=draft)
+        return self.accepted, self.counts, self.next_tokens
+
+    def commit(self, keys, values, accepted, counts, page_table, lengths):
+        """Writes the keys and values of the accepted drafted tokens into the 8-bit cache, behind the committed ones, and counts them into ``lengths``, all on the device.  The page table must have
+        places for them (what has none is not written and reported by ``device_status``)."""
+        write_cache_fp8(keys, values, *self.fp8, page_table, lengths, tokens=accepted, counts=counts)
+        lengths += counts
+
+    def cached_values(self):
+        """The cache's keys and values in fp32."""
+        if self.fp8 is None:
+            return self.k_cache.float(), self.v_cache.float()
+        return tuple(c.float() * torch.exp2(e.float() - 127)[..., None] for c, e in zip(self.fp8[:2], self.fp8[2:]))
+
     def accept(self, keys, values, accepted, page_table, lengths):
         """Writes the keys and values of accepted drafted tokens (``accepted``: a list of token numbers per sequence) behind the
         committed ones and returns the new lengths.  Raises ``ValueError``, and writes nothing, where there is no such token or no place for it
         (this check synchronises; on the GPU an index out of range would end the process's use of it)."""
+        if self.k_cache is None:
+            raise ValueError("accept: a cache in 8 bits is written by commit")
         page_size = self.k_cache.shape[1]
         if not len(accepted) == keys.shape[0] == lengths.shape[0] == page_table.shape[0] or any(not 0 <= t < keys.shape[1] for tokens in accepted for t in tokens):
             raise ValueError("accept: a list of numbers of drafted tokens for each sequence is needed")
@@ -108,8 +152,9 @@ def plain_step(block: DraftBlock, x, page_table, lengths, tree):
     positions = (lengths[:, None] + sees.sum(-1) - 1).float()
     q, k = block._rotate(q, positions).float(), block._rotate(k, positions).float()
     attended = torch.empty((b, t, h, d), device=x.device)
+    k_cache, v_cache = block.cached_values()
     for i, n in enumerate(lengths.tolist()):
-        keys, values = (torch.cat([c[page_table[i].long()].flatten(0, 1)[:n].float(), new[i]]).repeat_interleave(h // g, 1) for c, new in ((block.k_cache, k), (block.v_cache, v)))
+        keys, values = (torch.cat([c[page_table[i].long()].flatten(0, 1)[:n], new[i]]).repeat_interleave(h // g, 1) for c, new in ((k_cache, k), (v_cache, v)))
         scores = torch.einsum("thd,nhd->thn", q[i], keys) * d ** -0.5
         scores[..., n:].masked_fill_(~sees[i][:, None], -torch.inf)
         attended[i] = torch.einsum("thn,nhd->thd", scores.softmax(-1), values)
@@ -120,10 +165,11 @@ def plain_step(block: DraftBlock, x, page_table, lengths, tree):
 
 def make_inputs(block: DraftBlock, cached: int, seed=0):
     """Rows, page table, ragged lengths and random trees for a step."""
-    gen, device = torch.Generator().manual_seed(seed), block.k_cache.device
-    b, t, page_size = block.sequences, block.tokens, block.k_cache.shape[1]
+    cache = block.k_cache if block.fp8 is None else block.fp8[0]
+    gen, device = torch.Generator().manual_seed(seed), cache.device
+    b, t, page_size = block.sequences, block.tokens, cache.shape[1]
     per = -(-(cached + t) // page_size)
-    page_table = torch.randperm(block.k_cache.shape[0], generator=gen)[: b * per].view(b, per).int().to(device)
+    page_table = torch.randperm(cache.shape[0], generator=gen)[: b * per].view(b, per).int().to(device)
     lengths = torch.tensor([cached * (i + 1) // b for i in range(b)], dtype=torch.int32, device=device)
     parents = (torch.rand((b, t), generator=gen) * torch.arange(t)).long() - 1
     return torch.randn((b * t, block.norm1.numel()), generator=gen).half().to(device), page_table, lengths, tree_masks(parents).to(device)
@@ -134,25 +180,40 @@ def main():
     parser.add_argument("--sequences", type=int, default=8)
     parser.add_argument("--tokens", type=int, default=16)
     parser.add_argument("--cached", type=int, default=2048)
+    parser.add_argument("--fp8-cache", action="store_true", help="a cache in 8 bits, and the choice among the drafted tokens")
     options = parser.parse_args()
     per = -(-(options.cached + options.tokens) // 16)
-    block = DraftBlock(sequences=options.sequences, tokens=options.tokens, pages=options.sequences * per)
+    block = DraftBlock(sequences=options.sequences, tokens=options.tokens, pages=options.sequences * per, fp8_cache=options.fp8_cache, vocab=32000 if options.fp8_cache else 0)
     x, page_table, lengths, tree = make_inputs(block, options.cached)
     result, keys, values = block.step(x, page_table, lengths, tree)
     expect = plain_step(block, x, page_table, lengths, tree)
     print(f"{options.sequences} sequences x {options.tokens} drafted tokens over up to {options.cached} cached ones: relative error "
           f"{float((result.float() - expect).norm() / expect.norm()):.2e}")
+    if options.fp8_cache:
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        drafted = torch.randint(32000, tree.shape, generator=gen, device="cuda")
+        uniforms = torch.rand(tree.shape, generator=gen, device="cuda")
+
+    def whole_step():
+        result, keys, values = block.step(x, page_table, lengths, tree)
+        return (*block.choose(result, drafted, tree, uniforms), keys, values) if options.fp8_cache else (keys, values)
+
     start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     for _ in range(3):
-        block.step(x, page_table, lengths, tree)
+        whole_step()
     start.record()
     for _ in range(20):
-        block.step(x, page_table, lengths, tree)
+        *chosen, keys, values = whole_step()
     end.record()
     torch.cuda.synchronize()
     print(f"a step: {start.elapsed_time(end) * 50:.0f} us")
-    lengths = block.accept(keys, values, [[0]] * options.sequences, page_table, lengths)
-    print("lengths with one accepted token each:", lengths.tolist())
+    if options.fp8_cache:
+        accepted, counts, next_tokens = chosen
+        block.commit(keys, values, accepted, counts, page_table, lengths)
+        print("accepted tokens:", counts.tolist(), "next:", next_tokens.tolist(), "lengths:", lengths.tolist())
+    else:
+        lengths = block.accept(keys, values, [[0]] * options.sequences, page_table, lengths)
+        print("lengths with one accepted token each:", lengths.tolist())
 
 
 if __name__ == "__main__":
