@@ -35,7 +35,10 @@ using namespace fp6m;
 constexpr int kWorkers = 128, kThreads = kWorkers + 64;
 constexpr int kTile = 64, kDrafted = 32;           // cached tokens of a tile; places for drafted ones in theirs
 constexpr int kRowTile = kFewRows;
-constexpr int kLeastUnits = 3, kSlack = 8;
+// See make_plan.  us in graph replays with a slack of 4 / 8 / 16 / 32: one token over 300, 32 heads 10.1 / 8.5 / 8.5 / 8.6; sixteen over up to 500, 32 over 8 11.7 / 11.6 / 10.7 / 10.8; one
+// over 1000, 32 over 8 10.1 / 9.9 / 10.1 / 14.4.  With at least 2 / 3 / 5 units per CTA: the last one 9.6 / 9.9 / 10.8, twice eight tokens over 2000 22.4 / 22.7 / 24.3, one over 8000 15.5 /
+// 15.5 / 14.9.  With rows taken to cost 2 / 4 / 7 tiles: 8 x 5 tokens, 32 heads, up to 4096 42.8 / 34.1 / 34.3.
+constexpr int kLeastUnits = 3, kSlack = 16;
 
 struct Fp8Params : TreeParams {
   int grain;                             // tokens of a page that start at a multiple of their number in a tile
@@ -210,6 +213,7 @@ __device__ __forceinline__ void mma_halves(float (&d)[4], const uint32_t (&a)[4]
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Where the exponents of a token's key and value are in their words (bits), and whether it is seen.
+// (A word lies in the same four bytes of memory as its byte, so it can be read where that can.)
 constexpr uint32_t kUnseen = 1u << 31;
 __device__ __forceinline__ uint32_t where_of(const void* key_power, const void* value_power) {
   return (uint32_t)(reinterpret_cast<uintptr_t>(key_power) & 3) * 8 | (uint32_t)(reinterpret_cast<uintptr_t>(value_power) & 3) * (8 << 8);
