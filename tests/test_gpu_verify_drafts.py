@@ -97,6 +97,12 @@ def test_verify(b, t, vocab, chain, with_draft, dtype):
 
 
 @pytest.mark.parametrize("with_draft", [True, False])
+@pytest.mark.parametrize("b", [18, 19])
+def test_long_rows_of_as_many_sequences_as_get_wide_clusters_and_of_one_more(b, with_draft):
+    check(inputs(b, 3, 70001, with_draft=with_draft))
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
 def test_many_children_that_are_not_accepted(with_draft):
     """All hang on token 0: r is reduced up to 63 times, some ids come twice, some not from the vocabulary."""
     x = inputs(6, 64, 300, with_draft=with_draft, sharp=1.0)
