@@ -15,7 +15,7 @@
 // its random number - is fetched for all tokens at once, before.
 //
 // Bound by latencies that follow one another: launch and the tokens' numbers (about 4 us), then for each sum a round of loads, an exchange and a decision (about 2 us), and the search (1.5 us).  One
-// sequence, vocabulary 32000, no draft: 7.0 us; five trees of sixteen tokens, 50257: 21.6; 64 chains of seven, 131072, 32 bits: 20.4, where its one sum a sequence reads 3.3 TB/s over the whole call.
+// sequence, vocabulary 32000, no draft: 7.2 us; five trees of sixteen tokens, 50257: 21.3; 64 chains of seven, 131072, 32 bits: 20.4, where its one sum a sequence reads 3.3 TB/s over the whole call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -204,13 +204,17 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
   __shared__ double every[kMostCluster * kWarps];
   __shared__ float p_of[kMostTokens], q_of[kMostTokens], u_of[kMostTokens];
   __shared__ int parent[kMostTokens], id_of[kMostTokens], holes[kMostTokens];
-  __shared__ unsigned long long masks[kMostTokens];
+  __shared__ unsigned long long children[kMostTokens], firsts;      // of a token; those whose id is in the vocabulary and that of no sister before them
+  __shared__ bool lives;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int rank, ranks;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int b = blockIdx.x / ranks, workers = ranks * kWarps;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid < kMostTokens) children[tid] = 0;
+  if (tid == 0) firsts = 0;
+  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const P* target = static_cast<const P*>(a.target) + b * a.target_stride[0];
@@ -221,7 +225,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
     const int above = mask ? 63 - __clzll(earlier) : -2;             // the last earlier token that it sees, -1: none; -2: padding
     const long long id = a.drafted[(long long)b * a.tokens + tid];
     const bool inside = id >= 0 && id < a.vocab && above >= 0;
-    masks[tid] = mask;
+    if (tid == 0) lives = mask != 0;
+    if (above >= 0) atomicOr(&children[above], 1ull << tid);         // (the result does not depend on the order)
     parent[tid] = above;
     id_of[tid] = inside ? (int)id : -1;
     p_of[tid] = inside ? clean(Probability<P>::value(target + above * a.target_stride[1] + id)) : 0.f;
@@ -229,7 +234,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
     u_of[tid] = a.uniforms[(long long)b * a.tokens + tid];
   }
   __syncthreads();
-  const bool alive = masks[0] != 0;                                  // (the same in all CTAs of the cluster)
+  if (!draft && a.tokens > 1) {
+    if (tid < a.tokens && id_of[tid] >= 0) {
+      bool first = true;
+      for (int k = parent[tid] + 1; k < tid; ++k) first = first && (parent[k] != parent[tid] || id_of[k] != id_of[tid]);
+      if (first) atomicOr(&firsts, 1ull << tid);
+    }
+    __syncthreads();
+  }
+  const bool alive = lives;                                          // (the same in all CTAs of the cluster)
 
   Rest<P> r = {target, nullptr, 1.0, 0.0, holes, 0};
   int node = 0, count = alive ? 1 : 0, start = 0, stretch = 0, chunk = 0, pass = 0;
@@ -300,26 +313,21 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
   bool reduced = false, gone = false;      // r has been reduced and not been divided by its sum since; nothing of it remains
   bool summed = false, last_sum = false;   // `whole` is the sum of r, without draft that of the row without the children; it is that of the row itself
   go_to(0);
-  int i = 1;
+  unsigned long long rest = children[0];   // of the node, those that have not had their turn
 #pragma unroll 1
   while (alive) {
     bool asks = false;                     // a further child asks for the sum
-    for (; i < a.tokens && !last_sum; ++i) {
-      if (parent[i] != node) continue;
+    while (rest && !last_sum) {
+      const int i = __ffsll(rest) - 1;
       if (reduced) {
         if (!summed) {
           asks = true;
           break;
         }
         double left = whole;
-        if (!draft) {
-          // the children that are still to come, each id once
-          for (int k = i; k < a.tokens; ++k) {
-            if (parent[k] != node || id_of[k] < 0) continue;
-            bool before = false;
-            for (int j = node + 1; j < k; ++j) before = before || (parent[j] == node && id_of[j] == id_of[k]);
-            if (!before) left += (double)p_of[k];
-          }
+        if (!draft) {                      // the children that are still to come
+          const unsigned long long of = rest & firsts;
+          left += warp_sum((of >> lane & 1 ? (double)p_of[lane] : 0.0) + (of >> (lane + 32) & 1 ? (double)p_of[lane + 32] : 0.0));
         }
         gone = !(left > 0.0);
         if (!gone) {
@@ -329,16 +337,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
         reduced = false;
         if (draft) summed = false;
       }
-      bool nothing = gone;
-      if (!draft)                          // an id that was not accepted before has nothing left
-        for (int k = node + 1; k < i; ++k) nothing = nothing || (parent[k] == node && id_of[k] == id_of[i]);
+      const bool nothing = gone || (!draft && !(firsts >> i & 1));   // an id that was not accepted before has nothing left
       const double x = draft ? fma(-r.beta, (double)q_of[i], r.alpha * (double)p_of[i]) : r.alpha * (double)p_of[i];
       if (!nothing && (double)u_of[i] * (double)q_of[i] < fmax(x, 0.0)) {
         if (rank == 0 && tid == 0) a.accepted[(long long)b * a.tokens + count] = i;
         ++count;
         go_to(i);
+        rest = children[i];
         gone = summed = reduced = false;
       } else {
+        rest &= rest - 1;
         if (draft) {
           r.q = draft + node * a.draft_stride[1];
           r.beta += 1.0;
@@ -358,15 +366,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
       }
     }
     if (!draft && !last_sum) {
-      __syncthreads();
-      int n = 0;
-      for (int k = node + 1; k < a.tokens; ++k)
-        if (parent[k] == node && id_of[k] >= 0) {
-          if (tid == 0) holes[n] = id_of[k];
-          ++n;
-        }
-      __syncthreads();
-      r.hole_count = n;
+      const unsigned long long of = children[node] & firsts;
+      if (of) {
+        __syncthreads();
+        if (tid < kMostTokens && of >> tid & 1) holes[__popcll(of & ((1ull << tid) - 1))] = id_of[tid];
+        __syncthreads();
+      }
+      r.hole_count = __popcll(of);
     }
     const double alpha = r.alpha;
     if (!draft) r.alpha = 1.0;
