@@ -80,8 +80,10 @@ struct CacheParams {
 };
 
 // A CTA has some entries of a sequence, their keys or their values.  A unit is sixteen neighbouring values of a head: 32 bytes on one side, 16 on the other; four or eight units a
-// head, the heads of a token side by side.  A thread has up to kUnits units whose look-ups, then loads, are on their way together.  Bound by memory where tokens are many
-//, by look-ups one after the other (length, list, page table, values) where they are few.
+// head, the heads of a token side by side.  A thread has up to kUnits units whose look-ups, then loads, are on their way together.
+// Writing 4 x 4096 tokens of 8 heads of 128 from bf16: 23.4 us, 4.3 TB/s; reading 16 times up to 6144 of them: 60.8 us, 5.0 TB/s: of what a copy reaches 0.66 and 0.76, the rest is one round of CTAs
+// that all look up before they load.  16 x 7 tokens: 3.2 us, latencies one after the other (length, list, page table, values).  With units of eight values 45 and 107 us (instructions: a
+// head's address and power come twice as often), with keys and values in one CTA and strides in 64 bits 37 and 97.
 constexpr int kUnits = 2;
 template <class T, int D, bool kWrite>
 __global__ void __launch_bounds__(kThreads) cache_fp8_kernel(const __grid_constant__ CacheParams p) {

@@ -18,6 +18,11 @@
 // tile of scores per group beside the sums.  Measured and not kept: a fourth, an eighth or a sixteenth of the exponentials by a polynomial (+3, +1, 0 %),
 // sums and exponents in pairs (0), exponentials of one chunk between the sums of the last (+5 %, with or without registers moved to these warps).  The copies take 4 %.
 // 64 x 7 tokens, 64 heads over 8, up to 6144: 182 us, 4.5 TB/s, 0.69 of what a copy reaches (in a graph: 158 to 170).  Figures of both sides of a choice are of replays of a graph.
+//
+// A cache in 8 bits (kFp8; cache_fp8.cu): two more warps bring tiles as they are, with their tokens' powers of two, and the copying warps widen them in place to 16 bits, so all behind
+// them is the same.  Exact, so results are those of the widened cache.  2 x 64 tokens as above: 192 us in replays of a graph (16 bits there: 160 to 176): issue slots 49 %, a group's weights and the widening
+// of the next tiles on the same schedulers.  64 x 5 / 16 tokens, 64 heads over 8, up to 6144: 235 / 250 us in bf16, 209 / 228 in fp16 (a conversion less for each pair).  Measured and not kept: 4-byte
+// copies of the exponents that the widening warps decode (215 for the first, 318 for 64 x 5), all of a thread's powers read before its first store (213 / 283).
 #include <type_traits>
 
 #include "../../include/fp6m.h"

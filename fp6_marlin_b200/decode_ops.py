@@ -97,6 +97,7 @@ def write_cache_fp8(k, v, k_cache, v_cache, k_scales, v_scales, page_table, leng
     -40..120 for bf16; at the highest, magnitudes end at 240 times it, so that what is read back is finite); its values are divided by it and
     rounded to E4M3, infinities and NaN become NaN.  What has no place - behind the page table, in a page that does not exist, a token number from T on - is
     not written and reported by :func:`device_status` (4).  No two entries of a call may go to the same place of a page.
+    At most 65536 heads; steps from token to token, page to page and slot to slot stay below 2^32 elements, the others are free.
     """
     what = "write_cache_fp8"
     # plain CUDA tensors that pass every check: one call into native code; anything else takes the general path below
@@ -136,7 +137,11 @@ def tree_attention_fp8(q, k, v, k_cache, v_cache, k_scales, v_scales, page_table
 
     q, k, v, out, page_table, lengths, tree and ``scale`` are as there, with the drafted tokens' queries, keys and values in fp16 or bf16; k_cache,
     v_cache, k_scales and v_scales hold the committed tokens, whose keys and values are the E4M3 values times their powers of two.  Scores, maxima and sums are
-    fp32.  The weights of the softmax, each times its value's power of two, are rounded once, to fp16, before they meet the values, the result once more.
+    fp32.  The weights of the softmax, each times its value's power of two, are rounded once before they meet the values, and the result once more.
+
+    Up to 32 rows (tokens times heads) per head of keys the weights are rounded to fp16 and any E4M3 value and exponent byte from 0 to 254 will do.
+    With more rows keys and values are widened to the type of q, and the weights rounded to it: the cache must have been written from that type, by :func:`write_cache_fp8` or
+    with its exponents and largest values.  Steps from page to page and slot to slot of k_scales and v_scales stay below 2^32.
     """
     what = "tree_attention_fp8"
     rc = _call.tree_attention_fp8(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale, k_scales, v_scales)

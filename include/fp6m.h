@@ -298,7 +298,7 @@ typedef struct fp6m_cache_scales {
  * written and sets the status word to FP6M_ERR_BAD_ARG.
  * fp6m_read_cache_fp8: row i of sequence b of k and v (`entries` rows) becomes token starts[b] + i (starts null: token i), times its power and rounded to
  * `type`; rows of tokens before the first or from lengths[b] on are left as they were, as are those in a page that does not exist, which sets the status word.
- * Lengths are cut to 0 .. max_pages * page_size (2^31 - 65536 at most). */
+ * Lengths are cut to 0 .. max_pages * page_size (2^31 - 65536 at most).  At most 65536 heads; strides of tokens, pages and slots below 2^32. */
 typedef struct fp6m_cache_fp8_args {
   void *k, *v;                        /* batch x (tokens | entries) x kv_heads x head_dim, 16 bits */
   void *k_cache, *v_cache;            /* pages x page_size x kv_heads x head_dim */
@@ -314,7 +314,9 @@ typedef struct fp6m_cache_fp8_args {
 int fp6m_write_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, int dev, void* stream, int* status_dev);
 int fp6m_read_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, int dev, void* stream, int* status_dev);
 /* fp6m_tree_attention over such a cache: k_cache and v_cache of `args` are E4M3 (strides as above); the drafted tokens' q, k, v and out are of its type.  The
- * softmax's weights, each times its value's power of two, are rounded to fp16 (up to 32 rows of a head of keys) or `type` before they meet the values. */
+ * softmax's weights, each times its value's power of two, are rounded to fp16 (up to 32 rows of a head of keys) or `type` before they meet the values; with more
+ * rows keys and values are widened to `type`, from which the cache must have been written.  Page and slot strides of the scales stay below 2^32.  Scratch as in
+ * fp6m_tree_attention; zero it again after a call that set the status word to FP6M_ERR_TIMEOUT. */
 size_t fp6m_tree_attention_fp8_scratch_bytes(int sms);
 int fp6m_tree_attention_fp8(const fp6m_tree_attention_args* args, const fp6m_cache_scales* scales, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
 

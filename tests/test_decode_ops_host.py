@@ -49,6 +49,9 @@ def test_cache_entries_refuse_before_they_touch_the_gpu(function):
     assert call(_lib.CacheScales(0, ONE)) == call(_lib.CacheScales(ONE, ONE, three(0, 0, -1))) == call(None) == getattr(_lib.lib, function)(None, scales, 0, None, None) == _lib.ERR_BAD_ARG
     for page_size, max_pages in ((64, (1 << 25) - 32), (1, (1 << 31) - 256), (1 << 30, 2)):
         assert call(page_size=page_size, max_pages=max_pages) == _lib.ERR_PROB_SHAPE
+    far = 1 << 32
+    assert call(k_stride=three(0, far, 0)) == call(v_stride=three(0, far, 0)) == call(k_cache_stride=three(far, 0, 0)) == call(v_cache_stride=three(0, far, 0)) == _lib.ERR_PROB_SHAPE
+    assert call(_lib.CacheScales(ONE, ONE, three(far, 0, 0))) == call(_lib.CacheScales(ONE, ONE, three(), three(0, far, 0))) == _lib.ERR_PROB_SHAPE
     assert call(batch=0) == call(entries=0) == call(kv_heads=0) == _lib.OK
 
 
@@ -60,6 +63,8 @@ def test_attention_refuses_before_it_touches_the_gpu():
     assert call(batch=-1) == call(type=2) == call(q=0) == call(out=24) == call(page_table=0) == call(lengths=0) == call(tree=0) == _lib.ERR_BAD_ARG
     assert call(k_cache_stride=three(0, 8, 0)) == call(v_cache_stride=three(24, 0, 0)) == call(q_stride=three(0, 0, 4)) == _lib.ERR_BAD_ARG      # 16 values of 8 bits, 8 of 16
     assert call(_lib.CacheScales(ONE, 0)) == call(_lib.CacheScales(ONE, ONE, three(), three(-1, 0, 0))) == call(None) == _lib.ERR_BAD_ARG
+    far = 1 << 32
+    assert call(_lib.CacheScales(ONE, ONE, three(far, 0, 0))) == call(_lib.CacheScales(ONE, ONE, three(), three(0, far, 0))) == _lib.ERR_PROB_SHAPE
     assert call(batch=0) == call(tokens=0) == call(heads=0) == _lib.OK
     for page_size, max_pages in ((64, (1 << 25) - 32), (1, (1 << 31) - 256), (1 << 30, 2)):
         assert call(page_size=page_size, max_pages=max_pages, tokens=64) == _lib.ERR_PROB_SHAPE
