@@ -16,6 +16,8 @@
 #include <cuda_runtime.h>
 #include <limits.h>
 
+#include <algorithm>
+
 #include "../../include/fp6m.h"
 #include "host_common.h"
 #include "tree_attention.cuh"
@@ -80,11 +82,14 @@ struct CacheParams {
 };
 
 // A CTA has some entries of a sequence, their keys or their values.  A unit is sixteen neighbouring values of a head: 32 bytes on one side, 16 on the other; four or eight units a
-// head, the heads of a token side by side.  A thread has up to kUnits units whose look-ups, then loads, are on their way together.
-// Writing 4 x 4096 tokens of 8 heads of 128 from bf16: 23.4 us, 4.3 TB/s; reading 16 times up to 6144 of them: 60.8 us, 5.0 TB/s: of what a copy reaches 0.66 and 0.76, the rest is one round of CTAs
-// that all look up before they load.  16 x 7 tokens: 3.2 us, latencies one after the other (length, list, page table, values).  With units of eight values 45 and 107 us (instructions: a
-// head's address and power come twice as often), with keys and values in one CTA and strides in 64 bits 37 and 97.
-constexpr int kUnits = 2;
+// head, the heads of a token side by side.  A thread has a unit a round; where the next one lies is looked up while this one's values are on their way.
+// Writing 4 x 4096 tokens of 8 heads of 128 from bf16: 22.1 us, 4.6 TB/s; reading 16 times up to 6144 of them: 54.0 us, 5.6 TB/s: of what a copy reaches 0.70 and 0.86, the rest is the start of a
+// CTA (its length, then its page, then its values), for short calls all there is: 16 x 7 tokens of 32 heads 2.4 us.  Not kept: 2, 3 and 4 units of a thread in flight together (23.3, 25.2, 27.3 and 60.8, 59.6,
+// 64.4 us: registers that warps lack); accesses of 32 bytes (23.2, 62.1 of 23.3, 60.8); units of eight values (45 and 107: a head's address and power twice as often).
+struct Place {
+  bool lives;
+  int token, page, slot, head;
+};
 template <class T, int D, bool kWrite>
 __global__ void __launch_bounds__(kThreads) cache_fp8_kernel(const __grid_constant__ CacheParams p) {
   constexpr int kPart = D / 16;
@@ -109,116 +114,101 @@ __global__ void __launch_bounds__(kThreads) cache_fp8_kernel(const __grid_consta
   const int* table = a.page_table + b * a.page_table_stride;
   const int part = threadIdx.x % kPart;
   bool bad = false;
-#pragma unroll 1
-  for (int i0 = 0; i0 < work; i0 += kUnits * kThreads) {
-    bool lives[kUnits];
-    int token[kUnits], page[kUnits], slot[kUnits], head[kUnits];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int i = i0 + u * kThreads + threadIdx.x;
-      const int in_cta = p.at_once == 1 ? 0 : (int)__umulhi((unsigned)i, p.entry_magic), entry = first + in_cta;
-      head[u] = (i - in_cta * per_entry) / kPart;
-      lives[u] = i < work;
-      token[u] = entry;
-      const unsigned at = start + entry;
-      if (kWrite) {
-        lives[u] = lives[u] && entry < count;
-        if (lives[u] && a.list) token[u] = a.list[b * a.list_stride + entry];
-        lives[u] = lives[u] && token[u] >= 0;
-        if (lives[u] && (at >= (unsigned)most || token[u] >= a.tokens)) {
-          bad = true;
-          lives[u] = false;
-        }
-      } else {
-        lives[u] = lives[u] && at < (unsigned)length;
-      }
-      const int place = (int)((unsigned long long)at * (unsigned)p.page_magic >> p.page_shift);      // (the magic number is below 2^32)
-      slot[u] = (int)at - place * a.page_size;
-      page[u] = lives[u] ? table[place] : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      if (lives[u] && (unsigned)page[u] >= (unsigned)a.pages) {
+  // where unit i of this CTA comes from or goes to
+  auto look_up = [&](int i) {
+    Place at;
+    const int in_cta = p.at_once == 1 ? 0 : (int)__umulhi((unsigned)i, p.entry_magic), entry = first + in_cta;
+    at.head = (i - in_cta * per_entry) / kPart;
+    at.lives = i < work;
+    at.token = entry;
+    const unsigned j = start + entry;
+    if (kWrite) {
+      at.lives = at.lives && entry < count;
+      if (at.lives && a.list) at.token = a.list[b * a.list_stride + entry];
+      at.lives = at.lives && at.token >= 0;
+      if (at.lives && (j >= (unsigned)most || at.token >= a.tokens)) {
         bad = true;
-        lives[u] = false;
-      }
-    }
-    auto wide = [&](int u) { return reinterpret_cast<uint4*>(wide_rows + (unsigned long long)(unsigned)token[u] * wide_step + head[u] * wide_head + part * 16); };
-    auto narrow = [&](int u) {
-      return reinterpret_cast<uint4*>(narrow_rows + (unsigned long long)(unsigned)page[u] * page_step + (unsigned long long)(unsigned)slot[u] * slot_step + head[u] * narrow_head + part * 16);
-    };
-    auto power = [&](int u) { return powers + (unsigned long long)(unsigned)page[u] * power_page + (unsigned long long)(unsigned)slot[u] * power_slot + head[u] * power_head; };
-    if constexpr (kWrite) {
-      uint4 in[kUnits][2];
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) in[u][h] = lives[u] ? wide(u)[h] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        constexpr uint32_t E = Half16<T>::kExponent;
-        uint32_t w[8] = {in[u][0].x, in[u][0].y, in[u][0].z, in[u][0].w, in[u][1].x, in[u][1].y, in[u][1].z, in[u][1].w};
-        using Two = typename Values<T>::Two;
-        uint32_t two = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const Two now = larger(*reinterpret_cast<const Two*>(&two), *reinterpret_cast<const Two*>(&w[e]));
-          two = *reinterpret_cast<const uint32_t*>(&now);
-        }
-        two &= 0x7fff7fffu;
-        uint32_t top = max(two & 0xffffu, two >> 16), odd = 0;       // (bits of magnitudes are ordered as they are); a bit for each value that is infinite or NaN
-        if (top >= E) {
-          // these become NaN, and the exponent is that of the others
-          top = 0;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t one = w[e / 2] >> 16 * (e & 1) & 0x7fffu;
-            if (one >= E) odd |= 1u << e;
-            else top = max(top, one);
-          }
-        }
-#pragma unroll
-        for (int o = 1; o < kPart; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // = 1.m * 2^n; 448 = 1.75 * 2^8
-        const uint32_t bits = __float_as_uint(Half16<T>::value((uint16_t)top));
-        const int least = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
-        const int exponent = min(max(least, Values<T>::kLowest), Values<T>::kHighest);
-        uint32_t q[4];
-        Values<T>::narrow(w, exponent, q);
-        if (odd) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (odd >> e & 1) q[e / 4] |= 0x7fu << 8 * (e & 3);
-        }
-        if (lives[u]) {
-          *narrow(u) = make_uint4(q[0], q[1], q[2], q[3]);
-          if (part == 0) *power(u) = (uint8_t)(exponent + 127);
-        }
+        at.lives = false;
       }
     } else {
-      uint4 in[kUnits];
-      uint32_t by[kUnits];
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        in[u] = lives[u] ? *narrow(u) : make_uint4(0, 0, 0, 0);
-        by[u] = lives[u] ? *power(u) : 0;
+      at.lives = at.lives && j < (unsigned)length;
+    }
+    const int place = (int)((unsigned long long)j * (unsigned)p.page_magic >> p.page_shift);      // (the magic number is below 2^32)
+    at.slot = (int)j - place * a.page_size;
+    at.page = at.lives ? table[place] : 0;
+    return at;
+  };
+  Place next = look_up(threadIdx.x);
+#pragma unroll 1
+  for (int i0 = 0; i0 < work; i0 += kThreads) {
+    Place at = next;
+    if (i0 + kThreads < work) next = look_up(i0 + kThreads + threadIdx.x);
+    if (at.lives && (unsigned)at.page >= (unsigned)a.pages) {
+      bad = true;
+      at.lives = false;
+    }
+    uint4* const wide = reinterpret_cast<uint4*>(wide_rows + (unsigned long long)(unsigned)at.token * wide_step + at.head * wide_head + part * 16);
+    uint4* const narrow = reinterpret_cast<uint4*>(narrow_rows + (unsigned long long)(unsigned)at.page * page_step + (unsigned long long)(unsigned)at.slot * slot_step + at.head * narrow_head + part * 16);
+    uint8_t* const power = powers + (unsigned long long)(unsigned)at.page * power_page + (unsigned long long)(unsigned)at.slot * power_slot + at.head * power_head;
+    if constexpr (kWrite) {
+      uint4 in[2] = {};
+      if (at.lives) {
+        in[0] = wide[0];
+        in[1] = wide[1];
       }
+      constexpr uint32_t E = Half16<T>::kExponent;
+      uint32_t w[8] = {in[0].x, in[0].y, in[0].z, in[0].w, in[1].x, in[1].y, in[1].z, in[1].w};
+      using Two = typename Values<T>::Two;
+      uint32_t two = 0;
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        if (!lives[u]) continue;
-        const float f = __uint_as_float(by[u] ? by[u] << 23 : 0x00400000u);
-        const uint32_t q[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
-        uint32_t w[8];
+      for (int e = 0; e < 8; ++e) {
+        const Two now = larger(*reinterpret_cast<const Two*>(&two), *reinterpret_cast<const Two*>(&w[e]));
+        two = *reinterpret_cast<const uint32_t*>(&now);
+      }
+      two &= 0x7fff7fffu;
+      uint32_t top = max(two & 0xffffu, two >> 16), odd = 0;         // (bits of magnitudes are ordered as they are); a bit for each value that is infinite or NaN
+      if (top >= E) {
+        // these become NaN, and the exponent is that of the others
+        top = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q[e / 2] >> 16 * (e & 1)), __NV_E4M3);
-          const float2 v = __half22float2(*reinterpret_cast<const half2*>(&two));
-          w[e] = Half16<T>::pack(v.x * f, v.y * f);
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t one = w[e / 2] >> 16 * (e & 1) & 0x7fffu;
+          if (one >= E) odd |= 1u << e;
+          else top = max(top, one);
         }
-        uint4* to = wide(u);
-        to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        to[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
+#pragma unroll
+      for (int o = 1; o < kPart; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // = 1.m * 2^n; 448 = 1.75 * 2^8
+      const uint32_t bits = __float_as_uint(Half16<T>::value((uint16_t)top));
+      const int least = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
+      const int exponent = min(max(least, Values<T>::kLowest), Values<T>::kHighest);
+      uint32_t q[4];
+      Values<T>::narrow(w, exponent, q);
+      if (odd) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (odd >> e & 1) q[e / 4] |= 0x7fu << 8 * (e & 3);
+      }
+      if (at.lives) {
+        *narrow = make_uint4(q[0], q[1], q[2], q[3]);
+        if (part == 0) *power = (uint8_t)(exponent + 127);
+      }
+    } else {
+      if (!at.lives) continue;
+      const uint4 in = *narrow;
+      const uint32_t by = *power;
+      const float f = __uint_as_float(by ? by << 23 : 0x00400000u);
+      const uint32_t q[4] = {in.x, in.y, in.z, in.w};
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q[e / 2] >> 16 * (e & 1)), __NV_E4M3);
+        const float2 v = __half22float2(*reinterpret_cast<const half2*>(&two));
+        w[e] = Half16<T>::pack(v.x * f, v.y * f);
+      }
+      wide[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      wide[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
   if (bad && p.status) atomicExch(p.status, FP6M_ERR_BAD_ARG);
@@ -255,10 +245,11 @@ int run(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, bool w
   division_by(a.page_size, &p.page_magic, &p.page_shift);
   const int sms = sm_count(dev);
   if (sms <= 0) return cuda_fail(cudaGetLastError(), "cudaDeviceGetAttribute");
-  // a unit a thread where that leaves multiprocessors without work, else kUnits
+  // A CTA goes round once for every two times that the multiprocessors are full of such, six times at most.  us with 1 / 2 / 4 / 6 / 8 rounds: reading 16 x 6144 tokens of 8 heads of 128 (41 times full)
+  // 77.2 / 61.4 / 55.0 / 54.0 / 54.3; 4 x 4096 of 64 (3.5) 11.9 / 11.8 / 12.0 / 15.1 / 15.6; writing 4 x 4096 of 128 (6.9) 23.9 / 22.1 / 22.1 / 23.8 / 25.2; 8 x 512 (1.7) 7.3 / 7.6 / 9.2 / 10.5 / 11.5.
   const int per_entry = a.kv_heads * (a.head_dim / 16);
-  const bool many = 2ll * a.batch * a.entries * per_entry > (long long)sms * 8 * kThreads;
-  p.at_once = (many ? kUnits : 1) * kThreads / per_entry;
+  const long long full = 2ll * a.batch * a.entries * per_entry / ((long long)sms * 8 * kThreads);
+  p.at_once = (int)std::max(1ll, std::min(full / 2, 6ll)) * kThreads / per_entry;
   if (p.at_once < 1) p.at_once = 1;
   p.entry_magic = (unsigned int)((1ull << 32) / per_entry + 1);
   const dim3 ctas((unsigned)((a.entries + (long long)p.at_once - 1) / p.at_once), (unsigned)(a.batch < 65535 ? a.batch : 65535), (unsigned)(2 * ((a.batch + 65534ll) / 65535)));      // keys and values

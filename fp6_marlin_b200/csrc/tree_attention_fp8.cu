@@ -23,9 +23,11 @@
 // mma.sync and not tcgen05: E4M3 times E4M3 is not wanted (queries and weights keep 11 bits), so keys and values pass through registers in any case, and at up to 32 rows the tensor pipe is
 // busy a sixth of the time.  Above 32 rows a tcgen05 tile is full enough: 64 sequences, 64 heads over 8, up to 6144: 4 tokens (32 rows) take 152 us here, 5 tokens 235 there.
 //
-// Replays of a graph, heads of 128: 64 x 1 token, 64 heads over 8, up to 8192: 104.5 us, 5.2 TB/s, 0.79 of what a copy reaches: memory, and conversions (alu pipe 44 %, issue slots 42 %).
-// 3 x 1, 32 heads over 4, 65537: 44 us, 0.71: the same, and the joins of 296 ranges.  8 x 5, 32 over 32, up to 4096: 33.8 us, 0.62: queries, first data and ends of four items a CTA.
-// 1 x 1, 32 over 32, 300: 8.6 us: plan, look-ups, queries, first data, tiles and a join, one after the other.
+// Bound by the copies: the same kernel with no arithmetic at all takes as long (issue slots are busy 42 % of the time, the pipe of the conversions 44 %).  Replays of a graph, heads of 128:
+//   64 x 1 token, 64 heads over 8, up to 8192    104.5 us, 5.2 TB/s, 0.79 of what a copy reaches; without joins 101; with a cache that lies head by head 98 to 101
+//   3 x 1, 32 over 4, 65537                      44 us, 0.71; without joins 39
+//   8 x 5, 32 over 32, up to 4096                33.8 us, 0.62; without joins 31
+//   1 x 1, 32 over 32, 300                       8.6 us, without arithmetic 7.3: plan, look-ups, queries, first data, tiles and a join, one after the other
 #include <cuda.h>
 
 #include <type_traits>
