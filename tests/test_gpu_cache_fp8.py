@@ -92,11 +92,11 @@ def test_write_and_read(b, t, g, d, page, listed, dtype):
             for n, x in enumerate((k, v)):
                 code, power = encoded(x[i, token])
                 expect[n][page_of, slot], expect[2 + n][page_of, slot] = code, power
-    fits = all(int(lengths[i]) + len(row) <= per_tokens for i, row in enumerate(order))
+    fits = not any(token >= 0 and int(lengths[i]) + j >= per_tokens for i, row in enumerate(order) for j, token in enumerate(row))
     on = lambda x: None if x is None else x.cuda()                  # noqa: E731
     args = [table.cuda(), lengths.cuda()]
     fm.write_cache_fp8(k.cuda(), v.cuda(), *made, *args, tokens=on(tokens), counts=on(counts))
-    assert fm.device_status() == 0 if fits else 4
+    assert fm.device_status() == (0 if fits else 4)
     for got, want in zip(made, expect):
         assert same_bytes(got.view(torch.uint8), want) if got.dtype == torch.float8_e4m3fn else torch.equal(got.cpu(), want)
 
@@ -117,6 +117,26 @@ def test_write_and_read(b, t, g, d, page, listed, dtype):
                         want[i, row] = value * torch.pow(2.0, expect[2 + n][page_of, slot].double() - 127)[:, None]
             assert torch.equal(out.cpu().double().nan_to_num(nan=1e300), want.to(dtype).double().nan_to_num(nan=1e300))
     assert fm.device_status() == 0
+
+
+@pytest.mark.parametrize("b,t,g,d,page", [(4, 2600, 8, 128, 40), (3, 9500, 8, 128, 16), (2, 21001, 5, 64, 7), (1, 4001, 100, 64, 64)])
+def test_many_tokens_at_once_are_the_same_as_few_at_a_time(b, t, g, d, page):
+    """Calls so large that a CTA has several rounds of tokens, against calls of 100 tokens; each sequence has one token fewer than the one before it."""
+    per = -(-t // page)
+    k, v = (x.cuda() for x in (data(b, t, g, d, torch.bfloat16, 1), data(b, t, g, d, torch.bfloat16, 2)))
+    table = torch.randperm(b * per, generator=torch.Generator().manual_seed(t)).view(b, per).int().cuda()
+    lengths, counts = torch.zeros(b, dtype=torch.int32, device="cuda"), t - torch.arange(b, dtype=torch.int32, device="cuda")
+    at_once, one_by_one = cache(b * per, page, g, d), cache(b * per, page, g, d)
+    fm.write_cache_fp8(k, v, *at_once, table, lengths, counts=counts)
+    for i in range(0, t, 100):
+        fm.write_cache_fp8(k[:, i:i + 100], v[:, i:i + 100], *one_by_one, table, lengths + i, counts=counts - i)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(at_once, one_by_one))
+    outs, pieces = ([torch.full((b, t + 3, g, d), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)] for _ in range(2))
+    fm.read_cache_fp8(*at_once, table, counts, *outs)
+    for i in range(0, t + 3, 100):
+        fm.read_cache_fp8(*at_once, table, counts, *(x[:, i:i + 100] for x in pieces), starts=torch.full_like(lengths, i))
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(outs, pieces)) and fm.device_status() == 0
+    assert all((x[i, t - i:] == 7).all() for x in outs for i in range(b))
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
