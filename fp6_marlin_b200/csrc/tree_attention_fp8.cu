@@ -176,6 +176,7 @@ __device__ __forceinline__ void put_partial(float* slot, int r, int c, const flo
 //
 // Partials whose words are on their way together, and contributors of a group.  Cycles from the end of a range to the end of a join, with 2 / 4 / 6 / 12 together (code that runs once is
 // fetched as it runs, and unrolled code is long): two to three contributors 4280 / 4230 / 4480 / 6630, 25 in one step 23600 / 17500 / 16900 / 18500.
+// Not kept, for 3 x 1 token over 65537 (25 contributors, 44 us): the next words on their way while some are added up 44; all partials copied into shared memory, and again until they are there, 52.
 constexpr int kTogether = 4;
 __device__ __forceinline__ int join_step(int count) {
   if (count <= kTogether) return count;
