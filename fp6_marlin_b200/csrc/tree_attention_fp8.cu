@@ -25,8 +25,8 @@
 //
 // Bound by the copies: the same kernel with no arithmetic at all takes as long (issue slots are busy 42 % of the time, the pipe of the conversions 44 %).  Replays of a graph, heads of 128:
 //   64 x 1 token, 64 heads over 8, up to 8192    104.5 us, 5.2 TB/s, 0.79 of what a copy reaches; without joins 101; with a cache that lies head by head 98 to 101
-//   3 x 1, 32 over 4, 65537                      44 us, 0.71; without joins 39
-//   8 x 5, 32 over 32, up to 4096                33.8 us, 0.62; without joins 31
+//   3 x 1, 32 over 4, 65537                      43 us, 0.72; without joins 38
+//   8 x 5, 32 over 32, up to 4096                33.4 us, 0.62; without joins 31
 //   1 x 1, 32 over 32, 300                       8.6 us, without arithmetic 7.3: plan, look-ups, queries, first data, tiles and a join, one after the other
 #include <cuda.h>
 
@@ -142,9 +142,9 @@ __device__ __forceinline__ void put_result(const TreeParams& p, int b, int g, in
 #pragma unroll
   for (int i = 0; i < N; i += 4) *reinterpret_cast<uint2*>(out + i) = none ? make_uint2(0u, 0u) : make_uint2(Half16<T>::pack(v[i], v[i + 1]), Half16<T>::pack(v[i + 2], v[i + 3]));
 }
-// Words of a partial: what is not there yet is zero, so a word is stored as its complement (and the NaN that would be zero then as another).
-__device__ __forceinline__ uint32_t word_of(float x) { return __float_as_uint(x) == 0xffffffffu ? ~0x7fffffffu : ~__float_as_uint(x); }
-__device__ __forceinline__ float float_of(uint32_t word) { return __uint_as_float(~word); }
+// Words of a partial: what is not there yet is zero, so a zero is stored as minus zero.
+__device__ __forceinline__ uint32_t word_of(float x) { return __float_as_uint(x) == 0 ? 0x80000000u : __float_as_uint(x); }
+__device__ __forceinline__ uint32_t least_of(const uint4& v) { return min(min(v.x, v.y), min(v.z, v.w)); }
 __device__ __forceinline__ uint32_t load_word(const float* at) {
   uint32_t v;
   asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
@@ -176,7 +176,9 @@ __device__ __forceinline__ void put_partial(float* slot, int r, int c, const flo
 //
 // Partials whose words are on their way together, and contributors of a group.  Cycles from the end of a range to the end of a join, with 2 / 4 / 6 / 12 together (code that runs once is
 // fetched as it runs, and unrolled code is long): two to three contributors 4280 / 4230 / 4480 / 6630, 25 in one step 23600 / 17500 / 16900 / 18500.
-// Not kept, for 3 x 1 token over 65537 (25 contributors, 44 us): the next words on their way while some are added up 44; all partials copied into shared memory, and again until they are there, 52.
+// What bounds a join is instructions: a round of two partials of sixteen rows took 2200 cycles when all words were there at the first poll, as long with twice as many words on their way.  With fewer of them
+// (no decoding, the least word in place of a chain of tests, one address a partial; this code) 4 tokens, 64 heads over 8, over 8192 / 32768: 33.4 / 45.0 -> 29.7 / 42.0 us, 3 x 1 over 65537: 43.9 -> 42.4.
+// Not kept: the next words on their way while some are added up (0 to 3 %); all partials copied into shared memory, and again until they are there (43.5 -> 52).
 constexpr int kTogether = 4;
 __device__ __forceinline__ int join_step(int count) {
   if (count <= kTogether) return count;
@@ -805,52 +807,51 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
   if (!ends && (cta - join_first) % step != step - 1) return;
   // the sums of the groups before (if this is the last CTA), then the partials of this group
   const int before = ends ? group : 0, members = cta - join_first - group * step + 1;
-  auto source = [&](int k) {
-    if (k < before) return p.partials + (size_t)(kSlots * (join_first + k * step + step - 1) + 2) * kSlot;
+  auto source = [&](int k) {                                         // (offsets fit an int)
     const int c = join_first + group * step + k - before;
-    return p.partials + (size_t)(kSlots * c + (c == join_first ? 1 : 0)) * kSlot;
+    return p.partials + (k < before ? (kSlots * (join_first + k * step + step - 1) + 2) * kSlot : (kSlots * c + (c == join_first ? 1 : 0)) * kSlot);
   };
-  // a thread has a few values of a row, or of two that are eight apart
+  // Few instructions a word: one warp per scheduler goes through this, with nothing beside it.  A thread has four values, and 64 behind them four more (D = 128), of a row, or of two that are
+  // eight apart.
   constexpr int V = D / 16, R = C::kGroups > 1 ? 2 : 1, K = kTogether / R;
-  const int c = (tid & 15) * V;
+  const int c = (tid & 15) * 4, total_sources = before + members;
 #pragma unroll 1
   for (int r0 = tid >> 4; r0 < p.rows; r0 += 8 * R) {
     float most[R], sum[R] = {}, v[R][V] = {};
-    bool lives[R];
-    unsigned long long mask[R] = {};
+    const bool second = R == 2 && r0 + 8 < p.rows;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      most[i] = -INFINITY;
-      lives[i] = r0 + 8 * i < p.rows;
-      if (ends && lives[i]) mask[i] = mask_of(p, join_b, (r0 + 8 * i) / p.group);
-    }
+    for (int i = 0; i < R; ++i) most[i] = -INFINITY;
+    const int at_values = r0 * D + c, at_stats = kRowTile * D + r0, next_values = second ? 8 * D : 0, next_stats = second ? 8 : 0;
 #pragma unroll 1
-    for (int k0 = 0; k0 < before + members; k0 += K) {
+    for (int k0 = 0; k0 < total_sources; k0 += K) {
+      float* from[K];
       uint4 x[R][K][V / 4];
       uint32_t m[R][K], t[R][K];
+#pragma unroll
+      for (int e = 0; e < K; ++e) from[e] = source(min(k0 + e, total_sources - 1));
       bool there = false;
       for (uint32_t polls = 0; !there; ++polls) {
-        there = true;
+        uint32_t least = ~0u;
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
           for (int e = 0; e < K; ++e) {
-            const int r = lives[i] ? r0 + 8 * i : r0;
-            const float* from = source(min(k0 + e, before + members - 1));
-            m[i][e] = load_word(from + kRowTile * D + r);
-            t[i][e] = load_word(from + kRowTile * (D + 1) + r);
+            const float *stats_at = from[e] + at_stats + (i ? next_stats : 0), *values_at = from[e] + at_values + (i ? next_values : 0);
+            m[i][e] = load_word(stats_at);
+            t[i][e] = load_word(stats_at + kRowTile);
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) x[i][e][j] = load_words(from + r * D + c + 4 * j);
+            for (int j = 0; j < V / 4; ++j) x[i][e][j] = load_words(values_at + 64 * j);
           }
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
           for (int e = 0; e < K; ++e) {
-            there = there && m[i][e] && t[i][e];
+            least = min(least, min(m[i][e], t[i][e]));
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) there = there && x[i][e][j].x && x[i][e][j].y && x[i][e][j].z && x[i][e][j].w;
+            for (int j = 0; j < V / 4; ++j) least = min(least, least_of(x[i][e][j]));
           }
-        if (dead || polls > 1u << 19) {                              // (a round takes more than a microsecond)
+        there = least != 0;
+        if (dead || polls > 1u << 19) {                              // (a round takes about a microsecond)
           if (!dead && p.status) atomicExch(p.status, FP6M_ERR_TIMEOUT);
           dead = there = true;
         }
@@ -861,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
       for (int i = 0; i < R; ++i) {
         float now = most[i];
 #pragma unroll
-        for (int e = 0; e < K; ++e) now = fmaxf(now, float_of(m[i][e]));
+        for (int e = 0; e < K; ++e) now = fmaxf(now, __uint_as_float(m[i][e]));
         const float below = now == -INFINITY ? 0.f : now, keep = exp2_approx(most[i] - below);
         most[i] = now;
         sum[i] *= keep;
@@ -869,24 +870,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
         for (int j = 0; j < V; ++j) v[i][j] *= keep;
 #pragma unroll
         for (int e = 0; e < K; ++e) {
-          const bool counts = k0 + e < before + members;
-          const float f = counts ? exp2_approx(float_of(m[i][e]) - below) : 0.f;
-          sum[i] = fmaf(float_of(t[i][e]), f, sum[i]);
+          const bool counts = k0 + e < total_sources;
+          const float f = counts ? exp2_approx(__uint_as_float(m[i][e]) - below) : 0.f;
+          sum[i] = fmaf(__uint_as_float(t[i][e]), f, sum[i]);
 #pragma unroll
           for (int j = 0; j < V / 4; ++j) {
-            v[i][4 * j] = fmaf(float_of(x[i][e][j].x), f, v[i][4 * j]);
-            v[i][4 * j + 1] = fmaf(float_of(x[i][e][j].y), f, v[i][4 * j + 1]);
-            v[i][4 * j + 2] = fmaf(float_of(x[i][e][j].z), f, v[i][4 * j + 2]);
-            v[i][4 * j + 3] = fmaf(float_of(x[i][e][j].w), f, v[i][4 * j + 3]);
+            v[i][4 * j] = fmaf(__uint_as_float(x[i][e][j].x), f, v[i][4 * j]);
+            v[i][4 * j + 1] = fmaf(__uint_as_float(x[i][e][j].y), f, v[i][4 * j + 1]);
+            v[i][4 * j + 2] = fmaf(__uint_as_float(x[i][e][j].z), f, v[i][4 * j + 2]);
+            v[i][4 * j + 3] = fmaf(__uint_as_float(x[i][e][j].w), f, v[i][4 * j + 3]);
           }
-          if (counts && lives[i]) {
-            float* from = source(k0 + e);
-            const int r = r0 + 8 * i;
+          if (counts && (i == 0 || second)) {
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) store_words(from + r * D + c + 4 * j, make_uint4(0, 0, 0, 0));
+            for (int j = 0; j < V / 4; ++j) store_words(from[e] + at_values + 8 * D * i + 64 * j, make_uint4(0, 0, 0, 0));
             if (c == 0) {
-              store_word(from + kRowTile * D + r, 0);
-              store_word(from + kRowTile * (D + 1) + r, 0);
+              store_word(from[e] + at_stats + 8 * i, 0);
+              store_word(from[e] + at_stats + kRowTile + 8 * i, 0);
             }
           }
         }
@@ -894,9 +893,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      if (!lives[i]) continue;
-      if (ends) put_result<T>(p, join_b, join_g, r0 + 8 * i, mask[i], c, v[i], sum[i], join_odd);
-      else put_partial<D>(p.partials + (size_t)(kSlots * cta + 2) * kSlot, r0 + 8 * i, c, v[i], most[i], sum[i]);
+      if (i && !second) continue;
+      const int r = r0 + 8 * i;
+      const unsigned long long mask = ends ? mask_of(p, join_b, r / p.group) : 0;
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) {
+        float four[4] = {v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]};
+        if (ends) put_result<T>(p, join_b, join_g, r, mask, c + 64 * j, four, sum[i], join_odd);
+        else put_partial<D>(p.partials + (size_t)(kSlots * cta + 2) * kSlot, r, c + 64 * j, four, most[i], sum[i]);
+      }
     }
   }
 }
