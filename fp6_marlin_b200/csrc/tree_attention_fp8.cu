@@ -45,9 +45,9 @@ constexpr int kWorkers = 128, kThreads = kWorkers + 64;
 constexpr int kTile = 64, kDrafted = 32;           // cached tokens of a tile; places for drafted ones in theirs
 constexpr int kRowTile = kFewRows;
 // See make_plan.  us in graph replays with a slack of 4 / 8 / 16 / 32: one token over 300, 32 heads 10.1 / 8.5 / 8.5 / 8.6; sixteen over up to 500, 32 over 8 11.7 / 11.6 / 10.7 / 10.8; one
-// over 1000, 32 over 8 10.1 / 9.9 / 10.1 / 14.4.  With at least 2 / 3 / 5 units per CTA: the last one 9.6 / 9.9 / 10.8, twice eight tokens over 2000 22.4 / 22.7 / 24.3, one over 8000 15.5 /
-// 15.5 / 14.9.  With rows taken to cost 2 / 4 / 7 tiles: 8 x 5 tokens, 32 heads, up to 4096 42.8 / 34.1 / 34.3.
-constexpr int kLeastUnits = 3, kSlack = 16;
+// over 1000, 32 over 8 10.1 / 9.9 / 10.1 / 14.4.  With at least 3 / 4 / 6 units per CTA: the last one 9.6 / 10.1 / 14.6, twice eight tokens over 2000 21.9 / 21.2 /
+// 23.4; over 8192, 64 heads over 8, four tokens 29.7 / 27.0 / 27.9, two 22.0 / 20.5 / 20.7, one 15.5 / 14.7 / 15.0.  With rows taken to cost 2 / 4 / 7 tiles: 8 x 5 tokens, 32 heads, up to 4096 42.8 / 34.1 / 34.3.
+constexpr int kLeastUnits = 4, kSlack = 16;
 
 struct Fp8Params : TreeParams {
   int grain;                             // tokens of a page that start at a multiple of their number in a tile
