@@ -332,6 +332,7 @@ _prepared: dict[int, tuple] = {}
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _scratch_need: dict[tuple, int] = {}
+_zero_between_calls: dict[int, list[torch.Tensor]] = {}      # device -> scratches that device_status makes zero after an error
 
 
 def _stream_handle(idx: int, device: torch.device) -> int:
@@ -427,8 +428,11 @@ def set_ordered_sums(enable: bool) -> bool:
 
 
 def device_status(device=None) -> int:
-    """Reads (and clears) the device status word: 0, or FP6M_ERR_TIMEOUT (8) if a bounded wait
-    inside a kernel ran out since the last call.  Synchronises the device."""
+    """Reads (and clears) the device status word: 0, or the last error that a kernel reported since the last call: FP6M_ERR_TIMEOUT (8) if a bounded wait
+    ran out, FP6M_ERR_BAD_ARG (4) for a page, a token or the like that does not exist.  Waits for what the current stream was given; what other streams still run shows later.
+
+    After an error it also waits for the whole device and makes those scratches zero whose words must be that between calls (:func:`tree_attention_fp8`: a
+    part of a sum that came after its reader had given up would be taken for one of the next call): nothing may be launched meanwhile."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
     if idx not in _status:
@@ -436,7 +440,13 @@ def device_status(device=None) -> int:
     status = _status[idx]
     value = int(status.item())
     if value:
+        # (any error: it may have taken the place of a wait's)
+        torch.cuda.synchronize(idx)
+        with _buffers_lock:
+            for buffer in _zero_between_calls.get(idx, ()):
+                buffer.zero_()
         status.zero_()
+        torch.cuda.synchronize(idx)
     return value
 
 

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .api import _buffers_lock, _call, _device_buffers, _ptr, _sm_count, _status, _stream_handle, _zeros
+from .api import _buffers_lock, _call, _device_buffers, _ptr, _sm_count, _status, _stream_handle, _zero_between_calls, _zeros
 from ._lib import lib
 
 GROUP = 128                                       # neighbours that share a scale
@@ -42,6 +42,8 @@ def _operator_buffers(name: str, device: torch.device, nbytes: int, stream: int)
             if buffers:
                 nbytes = max(nbytes, 2 * buffers[-1].numel())
             buffers.append(_zeros(nbytes, device))
+            if name == "tree_attention_fp8":          # (the others' are tagged with the launch, or counted)
+                _zero_between_calls.setdefault(device.index, []).append(buffers[-1])
             _call.set_operator_scratch(_OWNERS[name], device.index, stream, _ptr(buffers[-1]), nbytes)
         return buffers[-1], _status[device.index]
 
