@@ -3,10 +3,11 @@
 //   a child c of the last accepted token n is accepted where u_c q(c) < r(c), else r <- max(r - q, 0) / sum;   r = p = target[n] at first, q = draft[n]
 //   none accepted: the next token is the lowest x with sum_{y <= x} r(y) > u_0 sum r
 //
-// However often r is reduced, it stays r = max(alpha p - beta q, 0): max(max(a, 0) / Z - q, 0) = max(a / Z - q, 0) for q >= 0, so a reduction by q changes beta to
-// beta + 1 and the division by its sum Z both to alpha / Z and beta / Z.  Two numbers are all that is kept, and the rows of p and q are read only where a sum is
-// needed: for a second child of a token whose first was not accepted, and for the next token.  Without draft r is alpha p, with zeros at the children that were
-// not accepted, and one sum, of p without any of the children, serves all of a token's children: what they have is added to it.
+// However often r is reduced, it stays r = max(p - q - less q, 0) / S: with less = 0 after the first reduction by q, and with S the sum of the numerators, a division by the sum makes S of 1,
+// and max(max(a, 0) / S - q, 0) = max(a - S q, 0) / S for q >= 0, so a further reduction adds S to `less`.  Two numbers are all that is kept, and the rows of p and q are read only
+// where a sum is needed: for a second child of a token whose first was not accepted, and for the next token.  (p - q first: 64 bits hold the difference of neighbours, so nothing is left where p = q, and
+// no error of p is left where p - q is small; in alpha p - beta q both were.)  Without draft r is p / S, with zeros at the children that were not
+// accepted, and one sum, of p without any of the children, serves all of a token's children: what they have is added to it.
 //
 // Sums are taken in 64 bits: neighbouring sums of a row of 10^5 probabilities lie 10^-5 apart, and sums in 32 bits, off by 10^-7, would choose another token once in a hundred times.
 //
@@ -15,7 +16,7 @@
 // its random number - is fetched for all tokens at once, before.
 //
 // Bound by latencies that follow one another: launch and the tokens' numbers (about 4 us), then for each sum a round of loads, an exchange and a decision (about 2 us), and the search (1.5 us).  One
-// sequence, vocabulary 32000, no draft: 7.2 us; five trees of sixteen tokens, 50257: 21.3; 64 chains of seven, 131072, 32 bits: 20.4, where its one sum a sequence reads 3.3 TB/s over the whole call.
+// sequence, vocabulary 32000, no draft: 7.0 us; five trees of sixteen tokens, 50257: 20.4; 64 chains of seven, 131072, 32 bits: 20.3, where its one sum a sequence reads 3.3 TB/s over the whole call.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -79,16 +80,16 @@ __device__ __forceinline__ double remote_double(uint32_t addr, int rank) {
   return v;
 }
 
-// r = max(alpha p - beta q, 0), or alpha p with holes
+// The numerator of r: max(p - q - less q, 0), or p with holes
 template <class P>
 struct Rest {
   const P *p, *q;                        // q null: nothing is subtracted
-  double alpha, beta;
+  double less;
   const int* holes;                      // ids whose probability is gone (no draft)
   int hole_count;
   __device__ __forceinline__ double of(float p_value, float q_value) const {
-    const double x = alpha * (double)clean(p_value);
-    return q ? fmax(fma(-beta, (double)clean(q_value), x), 0.0) : x;
+    const double p_clean = clean(p_value), q_clean = clean(q_value);
+    return q ? fmax(fma(-less, q_clean, p_clean - q_clean), 0.0) : p_clean;
   }
   __device__ __forceinline__ bool hole(int x) const {
     for (int i = 0; i < hole_count; ++i)
@@ -105,7 +106,7 @@ template <class P, class Take>
 __device__ __forceinline__ void for_values(const Rest<P>& r, int vocab, int start, bool vectors, bool any_holes, int from, int upto, bool& odd, Take&& take) {
   constexpr int N = 16 / sizeof(P), kStep = 32 * N;
   const int lane = threadIdx.x & 31;
-  const double alpha = r.alpha, minus_beta = -r.beta;
+  const double minus_less = -r.less;
   auto vector_group = [&](int first, auto subtracts) {
     constexpr bool kSubtracts = decltype(subtracts)::value;
     uint4 pv[kTogether], qv[kTogether];
@@ -122,12 +123,14 @@ __device__ __forceinline__ void for_values(const Rest<P>& r, int vocab, int star
       if (kSubtracts) Probability<P>::unpack(qv[k], qf);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        v[i] = alpha * (double)fmaxf(pf[i], 0.f);
+        const float p = fmaxf(pf[i], 0.f);
         if (kSubtracts) {
           const float q = fmaxf(qf[i], 0.f);
           odd = odd || q == INFINITY;
-          const double x = fma(minus_beta, (double)q, v[i]);
+          const double x = fma(minus_less, (double)q, (double)p - (double)q);
           v[i] = __double2hiint(x) < 0 ? 0.0 : x;
+        } else {
+          v[i] = (double)p;
         }
       }
       const int x = first + k * kStep + lane * N;
@@ -244,7 +247,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
   }
   const bool alive = lives;                                          // (the same in all CTAs of the cluster)
 
-  Rest<P> r = {target, nullptr, 1.0, 0.0, holes, 0};
+  Rest<P> r = {target, nullptr, 0.0, holes, 0};
+  double over = 1.0;                     // S
   int node = 0, count = alive ? 1 : 0, start = 0, stretch = 0, chunk = 0, pass = 0;
   bool vectors = false;
   double whole = 0.0;
@@ -304,9 +308,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
     node = n;
     r.p = target + n * a.target_stride[1];
     r.q = nullptr;                                                   // nothing to subtract yet
-    r.alpha = 1.0;
-    r.beta = 0.0;
+    r.less = 0.0;
     r.hole_count = 0;
+    over = 1.0;
   };
 
   // ---- the way through the tree.  (The sums are taken in one place, so that the code is there once.)
@@ -330,16 +334,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
           left += warp_sum((of >> lane & 1 ? (double)p_of[lane] : 0.0) + (of >> (lane + 32) & 1 ? (double)p_of[lane + 32] : 0.0));
         }
         gone = !(left > 0.0);
-        if (!gone) {
-          r.alpha = draft ? r.alpha / left : 1.0 / left;
-          r.beta /= left;
-        }
+        if (!gone) over = left;
         reduced = false;
         if (draft) summed = false;
       }
       const bool nothing = gone || (!draft && !(firsts >> i & 1));   // an id that was not accepted before has nothing left
-      const double x = draft ? fma(-r.beta, (double)q_of[i], r.alpha * (double)p_of[i]) : r.alpha * (double)p_of[i];
-      if (!nothing && (double)u_of[i] * (double)q_of[i] < fmax(x, 0.0)) {
+      if (!nothing && (double)u_of[i] * (double)q_of[i] * over < r.of(p_of[i], q_of[i])) {
         if (rank == 0 && tid == 0) a.accepted[(long long)b * a.tokens + count] = i;
         ++count;
         go_to(i);
@@ -348,18 +348,15 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
       } else {
         rest &= rest - 1;
         if (draft) {
+          if (r.q) r.less += over;
           r.q = draft + node * a.draft_stride[1];
-          r.beta += 1.0;
         }
         reduced = !gone;
       }
     }
     // ---- the next token is drawn from r, without draft from the row without the children (none has been accepted); from the row itself if that is nothing
     if (!asks) {
-      if (summed && (whole > 0.0 || last_sum)) {
-        if (!draft) r.alpha = 1.0;         // as the sums were taken
-        break;
-      }
+      if (summed && (whole > 0.0 || last_sum)) break;
       if (summed || (draft && gone)) {
         go_to(node);
         last_sum = true;
@@ -374,10 +371,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
       }
       r.hole_count = __popcll(of);
     }
-    const double alpha = r.alpha;
-    if (!draft) r.alpha = 1.0;
     add_up();
-    if (!draft && asks) r.alpha = alpha;
     summed = true;
   }
   const bool any = alive && whole > 0.0;
