@@ -7,11 +7,13 @@
 //
 // so that the scales cost one fused multiply-add per score and none per key or value: the values' power is an addend of the exponent, and the maximum that
 // keeps the exponentials in range is that of the weights as they meet the values.  These are rounded once, to fp16 (2^-11 of a weight; below 2^-14 of the largest they
-// become multiples of 2^-24), for both types of queries; the sum that they are divided by has them unrounded.  Queries in bf16 come as fp16 times a power of
+// become multiples of 2^-24), for both types of queries; the sum that they are divided by has them unrounded, 2^-y_j w_ij = 2^(a_ij - M_i - y_j) as an exponential of its own:
+// a w_ij that is zero beside values 2^150 times larger may be all of the sum.  Its terms come times 2^40, so that fp32 holds them for powers of values from 2^-54 (the largest
+// term is below 2^(8 + 54 + 40)) to 2^120 (the largest is not below 2^(40 - 120), and what is below 2^-126 counts nothing).  Queries in bf16 come as fp16 times a power of
 // two for each row, with the largest value between 2^14 and 2^15: exact but for values 2^-28 times smaller than that.
 //
 // Drafted keys and values are 16 bits.  They make a tile of their own behind the cached ones, which is brought into the form of the others when it is worked
-// on: fp16 with a power of two per token (bf16 as the queries, fp16 as it is).
+// on: fp16 with a power of two per token (bf16 as the queries, values with 2^-54 at least; fp16 as it is).
 //
 // Work is cut into equal ranges of (sequence, head of keys, row tile, key tile) units as in tree_attention.cu.
 //
@@ -21,7 +23,7 @@
 // One warp copies (runs of a page by TMA, else sixteen bytes a thread), one brings the tokens' powers of two, four compute; nothing but a stage's two barriers is between them.
 //
 // mma.sync and not tcgen05: E4M3 times E4M3 is not wanted (queries and weights keep 11 bits), so keys and values pass through registers in any case, and at up to 32 rows the tensor pipe is
-// busy a sixth of the time.  Above 32 rows a tcgen05 tile is full enough: 64 sequences, 64 heads over 8, up to 6144: 4 tokens (32 rows) take 152 us here, 5 tokens 235 there.
+// busy a sixth of the time.  Above 32 rows a tcgen05 tile is full enough: 64 sequences, 64 heads over 8, up to 6144: 4 tokens (32 rows) take 154 us here, 5 tokens 235 to 239 there.
 //
 // Bound by the copies: the same kernel with no arithmetic at all takes as long (issue slots are busy 42 % of the time, the pipe of the conversions 44 %).  Replays of a graph, heads of 128:
 //   64 x 1 token, 64 heads over 8, up to 8192    104.5 us, 5.2 TB/s, 0.79 of what a copy reaches; without joins 101; with a cache that lies head by head 98 to 101
@@ -44,6 +46,7 @@ using namespace fp6m;
 constexpr int kWorkers = 128, kThreads = kWorkers + 64;
 constexpr int kTile = 64, kDrafted = 32;           // cached tokens of a tile; places for drafted ones in theirs
 constexpr int kRowTile = kFewRows;
+constexpr int kLeastPower = -54, kTotalPower = 40; // of values; of what a row's total is kept times
 // See make_plan.  us in graph replays with a slack of 4 / 8 / 16 / 32: one token over 300, 32 heads 10.1 / 8.5 / 8.5 / 8.6; sixteen over up to 500, 32 over 8 11.7 / 11.6 / 10.7 / 10.8; one
 // over 1000, 32 over 8 10.1 / 9.9 / 10.1 / 14.4.  With at least 3 / 4 / 6 units per CTA: the last one 9.6 / 10.1 / 14.6, twice eight tokens over 2000 21.9 / 21.2 /
 // 23.4; over 8192, 64 heads over 8, four tokens 29.7 / 27.0 / 27.9, two 22.0 / 20.5 / 20.7, one 15.5 / 14.7 / 15.0.  With rows taken to cost 2 / 4 / 7 tiles: 8 x 5 tokens, 32 heads, up to 4096 42.8 / 34.1 / 34.3.
@@ -126,7 +129,7 @@ __device__ __forceinline__ T* out_row(const TreeParams& p, int b, int g, int r) 
 template <class T, int N>
 __device__ __forceinline__ void put_result(const TreeParams& p, int b, int g, int r, unsigned long long mask, int c, float (&v)[N], float sum, bool odd) {
   const bool none = mask == 0 || sum == 0.f;
-  const float f = 1.f / sum;
+  const float f = 1.f / (sum * power_of_two(-kTotalPower));
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] *= f;
   if (odd) {
@@ -231,9 +234,9 @@ __device__ __forceinline__ uint32_t where_of(const void* key_power, const void* 
   return (uint32_t)(reinterpret_cast<uintptr_t>(key_power) & 3) * 8 | (uint32_t)(reinterpret_cast<uintptr_t>(value_power) & 3) * (8 << 8);
 }
 
-// Of a thread's two tokens: 2^x scale log2(e); y and 2^-y.
+// Of a thread's two tokens: 2^x scale log2(e); y; from the exponent of a weight to that of what it adds to the total.
 struct Constants {
-  float key_by[2], value_power[2], value_by[2];
+  float key_by[2], value_power[2], to_total[2];
 };
 
 template <class T, int D, int NT, int RW>
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[m][n][e] = fmaf(kHalf ? s[m][n][e] : s[m][n][e] * row_by[n][e & 1], of[m].key_by[e >> 1], of[m].value_power[e >> 1]);
+            s[m][n][e] = fmaf(s[m][n][e], kHalf ? of[m].key_by[e >> 1] : of[m].key_by[e >> 1] * row_by[n][e & 1], of[m].value_power[e >> 1]);
             if (drafted) {
               const int t = key_warp * 16 + quad + (e & 2) * 4;
               if (t >= a.tokens || !(masks[8 * (group0 + n) + 2 * col + (e & 1)] >> t & 1)) s[m][n][e] = -INFINITY;
@@ -539,8 +542,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
         for (int m = 0; m < M; ++m) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[m][n][e] = exp2_approx(s[m][n][e] - below[e & 1]);
-            total[n][e & 1] = fmaf(s[m][n][e], of[m].value_by[e >> 1], total[n][e & 1]);
+            const float x = s[m][n][e] - below[e & 1];
+            s[m][n][e] = exp2_approx(x);
+            total[n][e & 1] += exp2_approx(x + of[m].to_total[e >> 1]);
           }
           w[m][n][0] = transposed(Half16<half>::pack(s[m][n][0], s[m][n][1]));
           w[m][n][1] = transposed(Half16<half>::pack(s[m][n][2], s[m][n][3]));
@@ -583,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
           const int x = (int)(kw >> (place & 31) & 255) - 127, y = (int)(vw >> (place >> 8 & 31) & 255) - 127;
           of[m].key_by[e] = place == kUnseen ? 0.f : power_of_two(x) * p.scale_log2;
           of[m].value_power[e] = place == kUnseen ? -INFINITY : (float)y;
-          of[m].value_by[e] = place == kUnseen ? 0.f : power_of_two(-y);
+          of[m].to_total[e] = (float)(kTotalPower - y);
         }
       }
 #pragma unroll
@@ -661,6 +665,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
 #pragma unroll
           for (int d = 1; d < kParts; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
           x = exponent_for_half(most);
+          if (is_value) x = max(x, kLeastPower);
           const float down = power_of_two(-x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = scaled_halves<T>(w[e], down);
@@ -688,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
         const int x = (int)powers[stage * 2 * kTile + first + quad + 8 * e], y = (int)powers[(stage * 2 + 1) * kTile + first + quad + 8 * e];
         of[0].key_by[e] = power_of_two(x) * p.scale_log2;
         of[0].value_power[e] = (float)y;
-        of[0].value_by[e] = power_of_two(-y);
+        of[0].to_total[e] = (float)(kTotalPower - y);
       }
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
