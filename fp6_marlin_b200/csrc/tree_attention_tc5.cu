@@ -697,6 +697,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
         unsigned long long mask = row_lives ? mask_of(p, seg.b, t) : 0;
         float top = -INFINITY, total = 0.f;                          // the maximum that the weights are relative to
         bool any = false;                                            // the sums hold something
+        bool rounds = false;                                         // scores are rounded before the maximum is taken from them
         const bool group_lives = !kPair || row_tile < p.row_tiles;
         for (int tile = seg.t0; tile < seg.t1; tile += 2, ++n) {
           if (!group_lives || (!kPair && (n & 1) != group)) continue;
@@ -709,6 +710,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
             const bool hidden = __any_sync(0xffffffffu, misc[1] != 0);
             // The largest score, then the weights: scores are read twice, because 128 of them would not stay in registers.  `hides`: some of the job's keys are
             // not seen by every row.  (A branch for every 32 scores, for what is hidden or grows, cost 150 cycles each: the two cases are apart.)
+            // A fused multiply-add leaves the rounding of the maximum, 2^-24 of it, in the exponent, and at 2^28 weights leave fp16's range: from 2^22 on (a quarter) scores are
+            // rounded as it was, so that the largest has a weight of 1.  That is done with what is hidden: false, and there are no weights, where a job turns out to need it.
+            // (A second copy of the exponentials in each case took 10 % longer for 64 x 5 tokens: it does not fit beside the rest of the code.)
             auto weigh = [&](auto hides) {
               constexpr bool kHides = decltype(hides)::value;
               // The row sees all cached keys, then those of its mask; the score of another is the lowest there is.
@@ -764,6 +768,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
                 const float keep = exp2_approx(top - (now == -INFINITY ? 0.f : now));
                 top = now;
                 total *= keep;
+                rounds = __any_sync(0xffffffffu, fabsf(top) >= 4194304.f);
                 if (any) {
                   // (the product before these scores is done: the tensor cores work in the order of issue)
 #pragma unroll 1
@@ -777,15 +782,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
                   }
                 }
               }
+              if (!kHides && rounds) {
+                tmem_loaded<32>(v0);
+                return false;
+              }
+              const float before = kHides && rounds ? sl : 1.f, within = kHides && rounds ? 1.f : sl;      // scores are multiplied by, rounded, and by
               const float base_log2 = top == -INFINITY ? 0.f : top;
               float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
               auto exponentials = [&](uint32_t* s, int c) {
                 hide(s, c);
+                auto weight = [&](uint32_t score) { return exp2_approx(fmaf(kHides ? as_float(score) * before : as_float(score), within, -base_log2)); };
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                  const float e0 = exp2_approx(fmaf(as_float(s[i]), sl, -base_log2)), e1 = exp2_approx(fmaf(as_float(s[i + 1]), sl, -base_log2));
-                  const float e2 = exp2_approx(fmaf(as_float(s[i + 2]), sl, -base_log2)), e3 = exp2_approx(fmaf(as_float(s[i + 3]), sl, -base_log2));
+                  const float e0 = weight(s[i]), e1 = weight(s[i + 1]), e2 = weight(s[i + 2]), e3 = weight(s[i + 3]);
                   t0 += e0;
                   t1 += e1;
                   t2 += e2;
@@ -805,9 +815,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
                 exponentials(v1, c + 1);
               }
               total += (t0 + t1) + (t2 + t3);
+              return true;
             };
-            if (cached < chunks * 32 || hidden) weigh(std::true_type());
-            else weigh(std::false_type());
+            if (cached < chunks * 32 || hidden || rounds || !weigh(std::false_type())) weigh(std::true_type());
             tc_wait_st();
           }
           any = true;
