@@ -101,9 +101,16 @@ class DraftBlock:
 
     def commit(self, keys, values, accepted, counts, page_table, lengths):
         """Writes the keys and values of the accepted drafted tokens into the 8-bit cache, behind the committed ones, and counts them into ``lengths``, all on the device.  The page table must have
-        places for them (what has none is not written and reported by ``device_status``)."""
+        places for them: what has none is not written and reported by ``device_status`` (4), and ``lengths`` go up to the first such token only."""
         write_cache_fp8(keys, values, *self.fp8, page_table, lengths, tokens=accepted, counts=counts)
-        lengths += counts
+        places, (pages, page_size) = page_table.shape[1], self.fp8[0].shape[:2]
+        if not places:
+            return
+        entry = torch.arange(accepted.shape[1], device=keys.device)
+        place = (lengths.long()[:, None] + entry) // page_size
+        page = page_table.gather(1, place.clamp(0, places - 1))
+        written = (entry < counts[:, None]) & (accepted >= 0) & (accepted < keys.shape[1]) & (place < places) & (page >= 0) & (page < pages)
+        lengths += written.int().cumprod(1).sum(1)
 
     def cached_values(self):
         """The cache's keys and values in fp32."""
