@@ -35,7 +35,7 @@ class DraftBlock:
         gen = torch.Generator(device=device).manual_seed(seed)
         randn = lambda *shape: torch.randn(shape, generator=gen, device=device)          # noqa: E731
         self.heads, self.kv_heads, self.dim = heads, kv_heads, hidden // heads
-        self.sequences, self.tokens, self.quant_cols = sequences, tokens, quant_cols
+        self.sequences, self.tokens, self.quant_cols, self.vocab = sequences, tokens, quant_cols, vocab
         self.norm1, self.norm2 = ((1 + 0.1 * randn(hidden)).half() for _ in range(2))
         self.qkv = make_fp8_weight(randn((heads + 2 * kv_heads) * self.dim, hidden) * 0.02)
         self.gate_up = make_fp8_weight(randn(2 * inter, hidden) * 0.02)
@@ -93,6 +93,8 @@ class DraftBlock:
     def choose(self, result, drafted, tree, uniforms, draft=None):
         """From the rows of a step to the accepted drafted tokens: ``(accepted, counts, next_tokens)`` as :func:`verify_drafts` gives them.  The target's probabilities are the softmax
         of a projection onto the vocabulary in 8 bits; drafted (sequences, tokens): the ids; uniforms: random numbers; draft: the probabilities that the ids were drawn from."""
+        if not self.vocab:
+            raise ValueError("choose: a block with vocab= is needed")
         rms_norm(result, self.norm3, self.rows8, scales=self.scales)
         mul_fp8(self.rows8, self.head[0], self.logits, self.scales, self.head[1])
         target = torch.softmax(self.logits.float(), 1).view(self.sequences, self.tokens, -1)
@@ -102,6 +104,8 @@ class DraftBlock:
     def commit(self, keys, values, accepted, counts, page_table, lengths):
         """Writes the keys and values of the accepted drafted tokens into the 8-bit cache, behind the committed ones, and counts them into ``lengths``, all on the device.  The page table must have
         places for them: what has none is not written and reported by ``device_status`` (4), and ``lengths`` go up to the first such token only."""
+        if self.fp8 is None:
+            raise ValueError("commit: a 16-bit cache is written by accept")
         write_cache_fp8(keys, values, *self.fp8, page_table, lengths, tokens=accepted, counts=counts)
         places, (pages, page_size) = page_table.shape[1], self.fp8[0].shape[:2]
         if not places:
