@@ -226,7 +226,8 @@ int run(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, bool w
   if (a.head_dim != 64 && a.head_dim != 128) return FP6M_ERR_PROB_SHAPE;
   if (a.batch == 0 || a.entries == 0 || a.kv_heads == 0) return FP6M_OK;
   if (a.kv_heads < 0 || a.kv_heads > 1 << 16 || a.max_pages < 0 || a.pages < 0 || a.page_size <= 0 || (long long)a.max_pages * a.page_size > 0x7fff0000ll) return FP6M_ERR_PROB_SHAPE;
-  if (!a.lengths || a.list_stride < 0 || !rows_aligned(a.k, a.k_stride, 8) || !rows_aligned(a.v, a.v_stride, 8)) return FP6M_ERR_BAD_ARG;
+  if (!a.lengths || a.list_stride < 0) return FP6M_ERR_BAD_ARG;
+  if (!(write && a.tokens == 0) && (!rows_aligned(a.k, a.k_stride, 8) || !rows_aligned(a.v, a.v_stride, 8))) return FP6M_ERR_BAD_ARG;      // (of no tokens nothing is read)
   if (a.max_pages > 0) {
     if (!rows_aligned(a.k_cache, a.k_cache_stride, 16) || !rows_aligned(a.v_cache, a.v_cache_stride, 16) || !a.page_table || a.page_table_stride < 0) return FP6M_ERR_BAD_ARG;
     if (!scales->k_scales || !scales->v_scales) return FP6M_ERR_BAD_ARG;

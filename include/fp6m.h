@@ -300,7 +300,7 @@ typedef struct fp6m_cache_scales {
  * `type`; rows of tokens before the first or from lengths[b] on are left as they were, as are those in a page that does not exist, which sets the status word.
  * Lengths are cut to 0 .. max_pages * page_size (2^31 - 65536 at most).  At most 65536 heads; strides of tokens, pages and slots below 2^32. */
 typedef struct fp6m_cache_fp8_args {
-  void *k, *v;                        /* batch x (tokens | entries) x kv_heads x head_dim, 16 bits */
+  void *k, *v;                        /* batch x (tokens | entries) x kv_heads x head_dim, 16 bits (write, 0 tokens: may be null) */
   void *k_cache, *v_cache;            /* pages x page_size x kv_heads x head_dim */
   const int *page_table;              /* batch x max_pages */
   const int *lengths;                 /* batch */
