@@ -20,8 +20,8 @@
 // 64 x 7 tokens, 64 heads over 8, up to 6144: 182 us, 4.5 TB/s, 0.69 of what a copy reaches (in a graph: 158 to 170).  Figures of both sides of a choice are of replays of a graph.
 //
 // A cache in 8 bits (kFp8; cache_fp8.cu): two more warps bring tiles as they are, with their tokens' powers of two, and the copying warps widen them in place to 16 bits, so all behind
-// them is the same.  Exact, so results are those of the widened cache.  2 x 64 tokens as above: 192 us in replays of a graph (16 bits there: 160 to 176): issue slots 49 %, a group's weights and the widening
-// of the next tiles on the same schedulers.  64 x 5 / 16 tokens, 64 heads over 8, up to 6144: 235 / 250 us in bf16, 209 / 228 in fp16 (a conversion less for each pair).  Measured and not kept: 4-byte
+// them is the same.  Exact, so results are those of the widened cache.  2 x 64 tokens as above: 190 us in replays of a graph (16 bits there: 156 to 176): issue slots 49 %, a group's weights and the widening
+// of the next tiles on the same schedulers.  64 x 5 / 16 tokens, 64 heads over 8, up to 6144: 241 / 256 us in bf16, 195 / 222 in fp16 (a conversion less for each pair).  Measured and not kept: 4-byte
 // copies of the exponents that the widening warps decode (215 for the first, 318 for 64 x 5), all of a thread's powers read before its first store (213 / 283).
 #include <type_traits>
 
@@ -112,13 +112,14 @@ __device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 // Four E4M3 values times a power of two, in 16 bits: exact where the type holds the result.  In fp16 one product a pair (the powers that it holds are those that it was written
-// with).  of: the factor, from the exponent + 127.
+// with).  of: the factor, from the exponent + 127; fp16 has those from kLeast to kMost.
 __device__ __forceinline__ void halves_of(uint32_t four, uint32_t& lo, uint32_t& hi) {
   asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 template <class T> struct Widen;
 template <> struct Widen<half> {
-  static __device__ __forceinline__ uint32_t of(int power) { return 0x10001u * __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)min(max(power, 127 - 24), 127 + 15) << 23))); }
+  static constexpr int kLeast = 127 - 24, kMost = 127 + 15;
+  static __device__ __forceinline__ uint32_t of(int power) { return 0x10001u * __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)min(max(power, kLeast), kMost) << 23))); }
   static __device__ __forceinline__ void run(uint32_t four, uint32_t by, uint32_t& lo, uint32_t& hi) {
     halves_of(four, lo, hi);
     asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(by));
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
   const uint32_t base = smem_u32(smem);
   const uint32_t full_k = base + C::kBars, empty_k = full_k + 8 * SK, full_v = empty_k + 8 * SK, empty_v = full_v + 8 * SV;
   const uint32_t q_free = empty_v + 8 * SV, scores = q_free + 16, weights = scores + 16, product = weights + 16, raw_k = product + 16, raw_v = raw_k + 8 * SK;
-  volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, [2, 3] last to arrive
+  volatile uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kBars + C::kNumBars * 8);      // [0] TMEM base, [1] a page did not exist, or a power of two is none in fp16, [2, 3] last to arrive
   volatile uint32_t* odd_ring = misc + 4;                            // [segment]: infinities or NaN among its drafted values
   __shared__ Plan plan;
   const int tid = threadIdx.x, warp = uniform_warp_index(), lane = tid & 31;
@@ -669,7 +670,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
               if (first_slot >= a.page_size) first_slot -= a.page_size;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) powers[stage * 2 * kKeys + 32 * i + lane] = Widen<T>::of(power[i >> 1][i & 1]);
+            for (int i = 0; i < 4; ++i) {
+              const int of = power[i >> 1][i & 1];
+              powers[stage * 2 * kKeys + 32 * i + lane] = Widen<T>::of(of);
+              // (reported alike; not where it is looked up, which would wait for it: 39 -> 57 us for 8 x 16 tokens over up to 2000)
+              if constexpr (Half16<T>::kMmaFormat == 0) missing = missing || of < Widen<T>::kLeast || of > Widen<T>::kMost;
+            }
             if (missing) misc[1] = 1;
             mbar_arrive(bar);
             if (++stage == stages) { stage = 0; phase ^= 1; }

@@ -142,7 +142,8 @@ def tree_attention_fp8(q, k, v, k_cache, v_cache, k_scales, v_scales, page_table
     Up to 32 rows (tokens times heads) per head of keys the weights are rounded to fp16, and any E4M3 values will do, with exponent bytes of keys from 0 to 254 and of values from 73 to 247
     (-54 to 120, which holds all that write_cache_fp8 stores).
     With more rows keys and values are widened to the type of q, and the weights rounded to it: the cache must have been written from that type, by :func:`write_cache_fp8` or
-    with its exponents and largest values.  Steps from page to page and slot to slot of k_scales and v_scales stay below 2^32.
+    with its exponents and largest values; powers of two that fp16 does
+    not hold (exponents below -24 or above 15) are reported by :func:`device_status` (4) where q is that, and results are wrong.  Steps from page to page and slot to slot of k_scales and v_scales stay below 2^32.
     """
     what = "tree_attention_fp8"
     rc = _call.tree_attention_fp8(q, k, v, k_cache, v_cache, page_table, lengths, tree, out, scale, k_scales, v_scales)

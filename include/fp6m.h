@@ -315,8 +315,9 @@ int fp6m_write_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scale
 int fp6m_read_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scales* scales, int dev, void* stream, int* status_dev);
 /* fp6m_tree_attention over such a cache: k_cache and v_cache of `args` are E4M3 (strides as above); the drafted tokens' q, k, v and out are of its type.  The
  * softmax's weights, each times its value's power of two, are rounded to fp16 (up to 32 rows of a head of keys) or `type` before they meet the values; with more
- * rows keys and values are widened to `type`, from which the cache must have been written; up to 32 rows bytes of keys may be 0..254 and of values 73..247.  Page and slot strides of the scales stay below 2^32.  Scratch as in
- * fp6m_tree_attention; zero it again after a call that set the status word to FP6M_ERR_TIMEOUT. */
+ * rows keys and values are widened to `type`, from which the cache must have been written (with fp16, an
+ * exponent outside -24..15 sets the status word to FP6M_ERR_BAD_ARG); up to 32 rows bytes of keys may be 0..254 and of values 73..247.  Page and slot strides of the scales
+ * stay below 2^32.  Scratch as in fp6m_tree_attention; zero it again after a call that set the status word to FP6M_ERR_TIMEOUT. */
 size_t fp6m_tree_attention_fp8_scratch_bytes(int sms);
 int fp6m_tree_attention_fp8(const fp6m_tree_attention_args* args, const fp6m_cache_scales* scales, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
 
