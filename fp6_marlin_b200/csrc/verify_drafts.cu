@@ -433,20 +433,29 @@ __global__ void __launch_bounds__(kThreads, kCtas) verify_drafts_kernel(const __
   cluster_sync();                                                    // (the others may still read this CTA's sums)
 }
 
+// The most CTAs that a cluster of this kernel may have on a device: more than eight have to be allowed, and a part of a GPU may have room for fewer.  Asked once for each device.
 template <class P>
-cudaError_t launch(const fp6m_verify_drafts_args& a, int ranks, cudaStream_t stream) {
-  if (ranks > kPortable) {               // (to be allowed once for each device)
-    static std::atomic<unsigned long long> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-      e = cudaFuncSetAttribute(reinterpret_cast<const void*>(verify_drafts_kernel<P>), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-      done.fetch_or(bit);
-    }
-  }
+cudaError_t largest_cluster(int dev, int* most) {
+  static std::atomic<int> known[64];
+  if (dev < 64 && (*most = known[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(verify_drafts_kernel<P>), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kMostCluster);
+  cfg.blockDim = dim3(kThreads);
+  e = cudaOccupancyMaxPotentialClusterSize(most, verify_drafts_kernel<P>, &cfg);
+  if (e != cudaSuccess) return e;
+  if (*most < 1) *most = 1;
+  if (dev < 64) known[dev].store(*most, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+template <class P>
+cudaError_t launch(const fp6m_verify_drafts_args& a, int dev, int ranks, cudaStream_t stream) {
+  int most = 0;
+  const cudaError_t e = largest_cluster<P>(dev, &most);
+  if (e != cudaSuccess) return e;
+  ranks = std::min(ranks, most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.batch * ranks));
   cfg.blockDim = dim3(kThreads);
@@ -485,6 +494,6 @@ extern "C" int fp6m_verify_drafts(const fp6m_verify_drafts_args* args, int dev, 
   const long long most = (long long)a.batch * kMostCluster <= 2ll * sms ? kMostCluster : kPortable;
   const int ranks = (int)std::max(1ll, std::min({fit, useful, most}));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a.type == FP6M_TYPE_F32 ? launch<float>(a, ranks, st) : a.type == FP6M_TYPE_F16 ? launch<half>(a, ranks, st) : launch<__nv_bfloat16>(a, ranks, st);
+  const cudaError_t e = a.type == FP6M_TYPE_F32 ? launch<float>(a, dev, ranks, st) : a.type == FP6M_TYPE_F16 ? launch<half>(a, dev, ranks, st) : launch<__nv_bfloat16>(a, dev, ranks, st);
   return e == cudaSuccess ? FP6M_OK : cuda_fail(e, "verify_drafts launch");
 }
