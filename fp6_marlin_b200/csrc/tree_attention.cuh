@@ -1,6 +1,7 @@
 // Shared by the kernels of attention over a paged cache (tree_attention.cu, tree_attention_tc5.cu, tree_attention_fp8.cu).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -32,6 +33,7 @@ struct TreeParams {
 
 // tree_attention_tc5.cu: more rows than kFewRows.  us for 20 to 32 rows, few / many: 8 x 4 tokens, 32 heads over 4, 2048 cached 27.8 / 26.4;
 // 2 x 3, 64 over 8, 8192: 34.9 / 36.7; 64 x 4, 64 over 8, up to 4096: 114.2 / 114.7; 16 x 5, 32 over 8, up to 4000: 41.4 / 44.4.
+// With a cache in 8 bits: 21.3 / 35.5; 24.7 / 34.3; up to 6144 148 / 195 (bf16 154 / 241); 36.6 / 54.3; one sequence of 32768, 4 tokens, 41.9 / 50.8.
 constexpr int kFewRows = 32;
 size_t tree_tc5_partial_bytes(int sms);
 cudaError_t launch_tree_tc5(TreeParams p, const fp6m_cache_scales* scales, int sms, cudaStream_t stream);      // scales: of a cache in 8 bits, or null
@@ -257,6 +259,31 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src) { asm volat
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+// arrives once this thread's copies so far have landed
+__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// p.run tokens of a head, a box's values from x on: value x, head, slot, page.  x is 0 or 64 values of 16 bits (128 bytes), so the copy starts on a 16-byte boundary.
+__device__ __forceinline__ void tma_load_run(uint32_t dst, const CUtensorMap* map, int x, int head, int slot, int page, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// the lower and the upper two of four E4M3 values in fp16 (exact)
+__device__ __forceinline__ uint32_t halves_of(uint32_t four) {
+  uint32_t h;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(four));
+  return h;
+}
+__device__ __forceinline__ uint32_t upper_halves_of(uint32_t four) {
+  uint32_t h;
+  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, hi;\n}\n" : "=r"(h) : "r"(four));
+  return h;
+}
 constexpr float kGrowth = 8.f;           // log2 of the growth of a maximum that is let pass: weights are relative to an older one until then
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -285,20 +312,6 @@ __device__ __forceinline__ bool is_odd(uint32_t two) {
 }
 
 // ---- for the kernels whose rows are few (tree_attention.cu, tree_attention_fp8.cu)
-
-template <class T> struct Mma;
-template <> struct Mma<half> {
-  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Mma<__nv_bfloat16> {
-  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }

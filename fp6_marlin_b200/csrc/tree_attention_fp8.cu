@@ -23,10 +23,13 @@
 // One warp copies (runs of a page by TMA, else sixteen bytes a thread), one brings the tokens' powers of two, four compute; nothing but a stage's two barriers is between them.
 //
 // mma.sync and not tcgen05: E4M3 times E4M3 is not wanted (queries and weights keep 11 bits), so keys and values pass through registers in any case, and at up to 32 rows the tensor pipe is
-// busy a sixth of the time.  Above 32 rows a tcgen05 tile is full enough: 64 sequences, 64 heads over 8, up to 6144: 4 tokens (32 rows) take 154 us here, 5 tokens 235 to 239 there.
+// busy a sixth (one row) to a third (32) of the time.  32 rows take less here than there: see kFewRows.
 //
-// Bound by the copies: the same kernel with no arithmetic at all takes as long (issue slots are busy 42 % of the time, the pipe of the conversions 44 %).  Replays of a graph, heads of 128:
-//   64 x 1 token, 64 heads over 8, up to 8192    104.5 us, 5.2 TB/s, 0.79 of what a copy reaches; without joins 101; with a cache that lies head by head 98 to 101
+// Up to 8 rows bound by the copies: the same kernel with no arithmetic at all takes as long (issue slots are busy 42 % of the time, the pipe of the conversions 44 %).  More rows: by the
+// chains of the four computing warps, whose tiles follow one another through products, maxima, exponentials and products; no unit is busy half of the time (32 rows: issue slots 45 %, conversions 41 %,
+// tensor pipe 31 %, special functions 17 %, memory 32 %).  Replays of a graph, heads of 128:
+//   64 x 1 token, 64 heads over 8, up to 8192    101 to 104 us, 5.2 TB/s, 0.79 of what a copy reaches; without joins 101; with a cache that lies head by head 98 to 101
+//   64 x 2 / 3 / 4 (16, 24, 32 rows), 6144       106 / 152 / 154 us in bf16, 99 / 146 / 148 in fp16; 1 row of a head of queries (8 of keys) 82 / 79
 //   3 x 1, 32 over 4, 65537                      43 us, 0.72; without joins 38
 //   8 x 5, 32 over 32, up to 4096                33.4 us, 0.62; without joins 31
 //   1 x 1, 32 over 32, 300                       8.6 us, without arithmetic 7.3: plan, look-ups, queries, first data, tiles and a join, one after the other
@@ -92,17 +95,6 @@ struct Cfg {
   static_assert(kCtas * (kBytes + 1024) <= 233472, "shared memory");
 };
 
-// two E4M3 values in fp16 (exact)
-__device__ __forceinline__ uint32_t halves_of(uint32_t two) {
-  uint32_t h;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(two));
-  return h;
-}
-__device__ __forceinline__ uint32_t upper_halves_of(uint32_t two) {
-  uint32_t h;
-  asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\ncvt.rn.f16x2.e4m3x2 %0, hi;\n}\n" : "=r"(h) : "r"(two));
-  return h;
-}
 // an 8 x 8 matrix of 16-bit values, two neighbours of a row a thread: transposed
 __device__ __forceinline__ uint32_t transposed(uint32_t m) {
   uint32_t t;
@@ -182,10 +174,10 @@ __device__ __forceinline__ void put_partial(float* slot, int r, int c, const flo
 // What bounds a join is instructions: a round of two partials of sixteen rows took 2200 cycles when all words were there at the first poll, as long with twice as many words on their way.  With fewer of them
 // (no decoding, the least word in place of a chain of tests, one address a partial; this code) 4 tokens, 64 heads over 8, over 8192 / 32768: 33.4 / 45.0 -> 29.7 / 42.0 us, 3 x 1 over 65537: 43.9 -> 42.4.
 // Not kept: the next words on their way while some are added up (0 to 3 %); all partials copied into shared memory, and again until they are there (43.5 -> 52).
-constexpr int kTogether = 4;
+constexpr int kPartialsTogether = 4;
 __device__ __forceinline__ int join_step(int count) {
-  if (count <= kTogether) return count;
-  int step = kTogether;
+  if (count <= kPartialsTogether) return count;
+  int step = kPartialsTogether;
   while (step * step < count) ++step;
   return step;
 }
@@ -194,7 +186,6 @@ template <int D>
 __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 7 : row >> 1 & 3; }      // of 16-byte pieces of rows of D bytes, as TMA's
 __device__ __forceinline__ void lds64(uint32_t (&v)[2], uint32_t addr) { asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory"); }
 __device__ __forceinline__ void lds128(uint32_t* v, uint32_t addr) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory"); }
-__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory"); }
 // a barrier of the warps that compute; whether any of them says so
 __device__ __forceinline__ bool any_worker(bool mine) {
   int any;
@@ -202,14 +193,6 @@ __device__ __forceinline__ bool any_worker(bool mine) {
   return any != 0;
 }
 __device__ __forceinline__ void workers_sync() { named_bar_sync(1, kWorkers); }
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
-// p.run tokens of a head: value 0, head, slot, page (the first coordinate is 0, so the copy starts on a 16-byte boundary)
-__device__ __forceinline__ void tma_load_run(uint32_t dst, const CUtensorMap* map, int head, int slot, int page, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-               ::"r"(dst), "l"(map), "r"(0), "r"(head), "r"(slot), "r"(page), "r"(bar) : "memory");
-}
 
 // ldmatrix of what makes two operands
 __device__ __forceinline__ void ldsm_two(uint32_t (&a)[2], uint32_t (&b)[2], uint32_t addr) {
@@ -343,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
               int at = first_slot;
 #pragma unroll
               for (int r = 0; r < R; ++r) {
-                tma_load_run(keys + r * (kTile / R) * D, &kmap, g, at, page[r], bar);
-                tma_load_run(values + r * (kTile / R) * D, &vmap, g, at, page[r], bar);
+                tma_load_run(keys + r * (kTile / R) * D, &kmap, 0, g, at, page[r], bar);
+                tma_load_run(values + r * (kTile / R) * D, &vmap, 0, g, at, page[r], bar);
                 at += kTile / R;
                 if (at == a.page_size) at = 0;
               }
@@ -818,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
   };
   // Few instructions a word: one warp per scheduler goes through this, with nothing beside it.  A thread has four values, and 64 behind them four more (D = 128), of a row, or of two that are
   // eight apart.
-  constexpr int V = D / 16, R = C::kGroups > 1 ? 2 : 1, K = kTogether / R;
+  constexpr int V = D / 16, R = C::kGroups > 1 ? 2 : 1, K = kPartialsTogether / R;
   const int c = (tid & 15) * 4, total_sources = before + members;
 #pragma unroll 1
   for (int r0 = tid >> 4; r0 < p.rows; r0 += 8 * R) {

@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kRowTile = 128;
 constexpr int kMostTreeCtas = 192;       // one per multiprocessor
-constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs (three idle), twice four that compute weights
+constexpr int kTreeThreads = 512;        // four warps that copy, one that issues MMAs, three idle (with a cache in 8 bits two of them bring tiles), twice four that compute weights
 // See make_plan (a pair's unit takes about twice as long).  us with a slack of 8 / 32: 8 x 16 tokens, 32 heads over 8, up to 2000 cached, 32.3 / 25.9; one of eight over 1000, 32
 // over 4, 19.0 / 15.9; pairs, 16 / 32: one of 64 over 2000, 64 over 8, 38.9 / 47.0.  At least 3 / 6 / 9 units: that one 40.3 / 38.9 / 39.9; one of
 // eight over 8000, 32 over 4, 28.7 / 27.9 / 29.4; four of eight over up to 3000 24.4 / 26.0 / 25.6.
@@ -75,20 +75,6 @@ __device__ __forceinline__ int join_step(int count) {
 }
 constexpr int kOddRing = 32;             // segments: more than the copies can be ahead of the sums
 
-// What was written to shared memory by copies and stores is seen by the MMAs that follow.  It stands where the MMAs are issued, behind the
-// barrier that counts the copies: in a thread that copies it would wait for all of that thread's copies in flight (measured: a tile
-// per latency of memory, 7000 cycles, in place of four tiles on their way).
-__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// arrives once this thread's copies so far have landed
-__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
-// 64 values of p.run tokens: value x, head, slot, page.  x is 0 or 64 (bytes: a multiple of 128), so the copy starts on a 16-byte boundary.
-__device__ __forceinline__ void tma_load_run(uint32_t dst, const CUtensorMap* map, int x, int head, int slot, int page, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 // operand with 128-byte swizzle whose 128-byte rows hold 64 values of K (keys and queries), or of N (`pitch`: from one 64 columns to the next)
 __device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return wide_act_desc(addr); }
 __device__ __forceinline__ uint64_t columns_desc(uint32_t addr, uint32_t pitch) {
@@ -108,20 +94,15 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) 
                : "memory");
 }
 __device__ __forceinline__ float as_float(uint32_t v) { return __uint_as_float(v); }
-__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t* v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-}
 // Four E4M3 values times a power of two, in 16 bits: exact where the type holds the result.  In fp16 one product a pair (the powers that it holds are those that it was written
 // with).  of: the factor, from the exponent + 127; fp16 has those from kLeast to kMost.
-__device__ __forceinline__ void halves_of(uint32_t four, uint32_t& lo, uint32_t& hi) {
-  asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(four));
-}
 template <class T> struct Widen;
 template <> struct Widen<half> {
   static constexpr int kLeast = 127 - 24, kMost = 127 + 15;
   static __device__ __forceinline__ uint32_t of(int power) { return 0x10001u * __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)min(max(power, kLeast), kMost) << 23))); }
   static __device__ __forceinline__ void run(uint32_t four, uint32_t by, uint32_t& lo, uint32_t& hi) {
-    halves_of(four, lo, hi);
+    lo = halves_of(four);
+    hi = upper_halves_of(four);
     asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(by));
     asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(by));
   }
@@ -129,7 +110,8 @@ template <> struct Widen<half> {
 template <> struct Widen<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t of(int power) { return 0x10001u * ((uint32_t)min(max(power, 1), 254) << 7); }
   static __device__ __forceinline__ void run(uint32_t four, uint32_t by, uint32_t& lo, uint32_t& hi) {
-    halves_of(four, lo, hi);
+    lo = halves_of(four);
+    hi = upper_halves_of(four);
     const float2 p = __half22float2(*reinterpret_cast<half2*>(&lo)), q = __half22float2(*reinterpret_cast<half2*>(&hi));
     lo = Half16<__nv_bfloat16>::pack(p.x, p.y);
     hi = Half16<__nv_bfloat16>::pack(q.x, q.y);
@@ -478,7 +460,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_attention_tc5_kernel(con
           groups = __shfl_sync(0xffffffffu, kPair && seg.item % p.parts * 2 + 1 < p.row_tiles ? 2 : 1, 0);
           return left > 0;
         }
-        // waits for the next stage; other copies than TMA's (the queries come with a segment's first) need a proxy fence
+        // waits for the next stage; other copies than TMA's (the queries come with a segment's first) need a proxy fence, so that the MMAs that follow see them.  It stands here, behind the
+        // barrier that counts the copies: in a thread that copies it would wait for all of that thread's copies in flight (measured: a tile per latency of memory, 7000
+        // cycles, in place of four tiles on their way).
         __device__ __forceinline__ void wait(uint32_t full, bool other_copies, int* status, bool& dead) {
           mbar_wait_bounded<20>(full + 8 * stage, phase, status, dead);
           if (other_copies || plain < min(left, 2)) fence_async_proxy();
