@@ -165,7 +165,8 @@ def tree_attention_fp8(q, k, v, k_cache, v_cache, k_scales, v_scales, page_table
 
 def verify_drafts(target, drafted, tree, uniforms, accepted, counts, next_tokens, *, draft=None):
     """Decides for each of B sequences which of T (at most 64) drafted tokens are accepted, and which token follows them, so that
-    the tokens are distributed as the target's probabilities say.
+    the tokens are distributed as the target's probabilities say: with ``draft``, where the children of a token were drawn from it independently of one another, so that an id may
+    come twice (for children drawn without repetition the rule is biased); without ``draft``, however they were chosen, as long as it was without looking at ``uniforms``.
 
     target (B, T, V), fp32, fp16 or bf16: row i holds the target's probabilities of the token after drafted token i.  drafted (B, T) int64: the tokens' ids.
     tree (B, T) or (T,) int64: the masks that :func:`tree_attention` takes; a token's parent is the last earlier one that it sees.

@@ -321,7 +321,8 @@ int fp6m_read_cache_fp8(const fp6m_cache_fp8_args* args, const fp6m_cache_scales
 size_t fp6m_tree_attention_fp8_scratch_bytes(int sms);
 int fp6m_tree_attention_fp8(const fp6m_tree_attention_args* args, const fp6m_cache_scales* scales, void* scratch, size_t scratch_bytes, int dev, void* stream, int* status_dev);
 
-/* Which drafted tokens of each sequence are accepted, and the token after them, so that the tokens are distributed as the target's probabilities say.
+/* Which drafted tokens of each sequence are accepted, and the token after them, so that the tokens are distributed as the target's probabilities say: with draft,
+ * where the children of a token were drawn from it independently of one another (the same id may come twice; drawn without repetition, they bias the result); without draft, however they were chosen.
  * The drafted tokens form a tree: `tree` as in fp6m_tree_attention, a token's parent is the last earlier token that it sees.  Token 0 is the one that the
  * step before has chosen; it is accepted as it is (with a mask of zero the sequence is padding: nothing is accepted, the next token is -1).
  * target[b, i] and draft[b, i] are the probabilities of the token after token i, the target's and those that i's children were drawn from.  From a
