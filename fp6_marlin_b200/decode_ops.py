@@ -139,7 +139,8 @@ def tree_attention_fp8(q, k, v, k_cache, v_cache, k_scales, v_scales, page_table
     v_cache, k_scales and v_scales hold the committed tokens, whose keys and values are the E4M3 values times their powers of two.  Scores, maxima and sums are
     fp32.  The weights of the softmax, each times its value's power of two, are rounded once before they meet the values, and the result once more.
 
-    Up to 32 rows (tokens times heads) per head of keys the weights are rounded to fp16, and any E4M3 values will do, with exponent bytes of keys from 0 to 254 and of values from 73 to 247
+    Up to 32 rows (tokens times heads) per head of keys this takes less time than :func:`tree_attention` over a 16-bit cache, with more rows it takes more (by a fifth to a half) and
+    what an 8-bit cache saves is memory.  Up to 32 rows the weights are rounded to fp16, and any E4M3 values will do, with exponent bytes of keys from 0 to 254 and of values from 73 to 247
     (-54 to 120, which holds all that write_cache_fp8 stores).
     With more rows keys and values are widened to the type of q, and the weights rounded to it: the cache must have been written from that type, by :func:`write_cache_fp8` or
     with its exponents and largest values; powers of two that fp16 does
