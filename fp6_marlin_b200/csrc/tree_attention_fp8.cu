@@ -111,6 +111,12 @@ __device__ __forceinline__ float largest_of(uint32_t two) { return fmaxf(finite_
 template <class T>
 __device__ __forceinline__ uint32_t scaled_halves(uint32_t two, float by) { return Half16<half>::pack(Half16<T>::value((uint16_t)two) * by, Half16<T>::value((uint16_t)(two >> 16)) * by); }
 
+// A total that is kept relative to one maximum, relative to another: times 2^by, in two halves, because 2^by alone may be zero where the total is not (maxima hold the values' powers, totals do not).
+__device__ __forceinline__ float moved(float total, float by) {
+  const float half_of = exp2_approx(0.5f * by);
+  return total * half_of * half_of;
+}
+
 // Where row r of a head of keys goes.
 template <class T>
 __device__ __forceinline__ T* out_row(const TreeParams& p, int b, int g, int r) {
@@ -508,9 +514,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
             for (int m = 0; m < M; ++m) now = fmaxf(now, fmaxf(s[m][n][e], s[m][n][2 + e]));
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, d));
-            keep[e] = exp2_approx(top[n][e] - (now == -INFINITY ? 0.f : now));
+            const float by = top[n][e] - (now == -INFINITY ? 0.f : now);
+            keep[e] = exp2_approx(by);
             top[n][e] = now;
-            total[n][e] *= keep[e];
+            total[n][e] = moved(total[n][e], by);
           }
 #pragma unroll
           for (int i = 0; i < kParts; ++i)
@@ -763,8 +770,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
         }
 #pragma unroll
         for (int k = 0; k < C::kKeyWarps; ++k) {
-          const float f = exp2_approx(of[k].x - (most == -INFINITY ? 0.f : most));
-          sum = fmaf(of[k].y, f, sum);
+          const float by = of[k].x - (most == -INFINITY ? 0.f : most), f = exp2_approx(by);
+          sum += moved(of[k].y, by);
           const float4* from = reinterpret_cast<const float4*>(pool + ((rw * C::kKeyWarps + k) * 8 + in) * C::kPoolRow + c);
 #pragma unroll
           for (int i = 0; i < V / 4; ++i) {
@@ -852,15 +859,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, NT, RW>::kCtas) tree_attentio
 #pragma unroll
         for (int e = 0; e < K; ++e) now = fmaxf(now, __uint_as_float(m[i][e]));
         const float below = now == -INFINITY ? 0.f : now, keep = exp2_approx(most[i] - below);
+        sum[i] = moved(sum[i], most[i] - below);
         most[i] = now;
-        sum[i] *= keep;
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] *= keep;
 #pragma unroll
         for (int e = 0; e < K; ++e) {
           const bool counts = k0 + e < total_sources;
-          const float f = counts ? exp2_approx(__uint_as_float(m[i][e]) - below) : 0.f;
-          sum[i] = fmaf(__uint_as_float(t[i][e]), f, sum[i]);
+          const float by = counts ? __uint_as_float(m[i][e]) - below : -INFINITY, f = exp2_approx(by);
+          sum[i] += moved(__uint_as_float(t[i][e]), by);
 #pragma unroll
           for (int j = 0; j < V / 4; ++j) {
             v[i][4 * j] = fmaf(__uint_as_float(x[i][e][j].x), f, v[i][4 * j]);

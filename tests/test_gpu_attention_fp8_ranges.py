@@ -24,6 +24,24 @@ def test_values_of_zero_beside_very_large_ones(t, h, g, d, lengths):
 
 
 @pytest.mark.parametrize("t,h,g,d", SHAPES)
+@pytest.mark.parametrize("run_length", [16, 64, 192, 2500])
+@pytest.mark.parametrize("zeros_first", [True, False])
+def test_runs_of_zeros_and_of_very_large_values(t, h, g, d, run_length, zeros_first):
+    """As above, by turns of tokens: a maximum that grows by 2^140 within a warp's tokens, between warps and between multiprocessors leaves the tokens before it in the sum."""
+    lengths, page = [5000, 700], 16
+    x = inputs(2, t, h, g, d, lengths, page, torch.bfloat16)
+    x["v_scales"] += 107
+    x["q"] = x["q"] / 16                                           # (so that many tokens count)
+    for i, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        at = at[(at // run_length % 2 == 0) == zeros_first]
+        rows, slots = x["page_table"][i].long()[at // page], at % page
+        _bytes(x["v_cache"])[rows, slots], x["v_scales"][rows, slots] = 0, 127 - 40
+    x["v"][:] = 0
+    check(run(x), x)
+
+
+@pytest.mark.parametrize("t,h,g,d", SHAPES)
 def test_small_and_large_values_as_write_cache_fp8_writes_them(t, h, g, d):
     """From 2^-60, below what the lowest exponent holds, to 2^110, through the cache itself."""
     x = inputs(2, t, h, g, d, [900, 70], 16, torch.bfloat16)
