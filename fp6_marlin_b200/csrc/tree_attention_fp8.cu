@@ -8,7 +8,7 @@
 // so that the scales cost one fused multiply-add per score and none per key or value: the values' power is an addend of the exponent, and the maximum that
 // keeps the exponentials in range is that of the weights as they meet the values.  These are rounded once, to fp16 (2^-11 of a weight; below 2^-14 of the largest they
 // become multiples of 2^-24), for both types of queries; the sum that they are divided by has them unrounded, 2^-y_j w_ij = 2^(a_ij - M_i - y_j) as an exponential of its own:
-// a w_ij that is zero beside values 2^150 times larger may be all of the sum.  Its terms come times 2^40, so that fp32 holds them for powers of values from 2^-54 (the largest
+// a w_ij that is zero beside those of values 2^150 times larger may be most of the sum.  Its terms come times 2^40, so that fp32 holds them for powers of values from 2^-54 (the largest
 // term is below 2^(8 + 54 + 40)) to 2^120 (the largest is not below 2^(40 - 120), and what is below 2^-126 counts nothing).  Queries in bf16 come as fp16 times a power of
 // two for each row, with the largest value between 2^14 and 2^15: exact but for values 2^-28 times smaller than that.
 //
@@ -29,7 +29,7 @@
 // chains of the four computing warps, whose tiles follow one another through products, maxima, exponentials and products; no unit is busy half of the time (32 rows: issue slots 45 %, conversions 41 %,
 // tensor pipe 31 %, special functions 17 %, memory 32 %).  Replays of a graph, heads of 128:
 //   64 x 1 token, 64 heads over 8, up to 8192    101 to 104 us, 5.2 TB/s, 0.79 of what a copy reaches; without joins 101; with a cache that lies head by head 98 to 101
-//   64 x 2 / 3 / 4 (16, 24, 32 rows), 6144       106 / 152 / 154 us in bf16, 99 / 146 / 148 in fp16; 1 row of a head of queries (8 of keys) 82 / 79
+//   64 x 1 / 2 / 3 / 4 (8 to 32 rows), 6144      82 / 106 / 152 / 155 us in bf16, 79 / 100 / 146 / 149 in fp16
 //   3 x 1, 32 over 4, 65537                      43 us, 0.72; without joins 38
 //   8 x 5, 32 over 32, up to 4096                33.4 us, 0.62; without joins 31
 //   1 x 1, 32 over 32, 300                       8.6 us, without arithmetic 7.3: plan, look-ups, queries, first data, tiles and a join, one after the other
